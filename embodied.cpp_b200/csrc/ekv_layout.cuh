@@ -77,11 +77,14 @@ __host__ __device__ inline uint32_t tile_elem_off(int row, int d, int D, int W) 
 }
 
 // Byte offset of int8 element (row, d) in the qs plane of a Q8_0 tile: rows of D bytes whose
-// 16-byte units are XOR-swizzled by the row (unit ^ (row & m), m = min(D/16, 8) - 1), so that
-// 8 consecutive rows of one 16-byte column fall in 8 different shared-memory bank groups.
+// 16-byte units are XOR-swizzled by the row (unit ^ (row & m), m + 1 = the largest power of two that
+// divides D/16, at most 8), so that 8 consecutive rows of one 16-byte column fall in 8 different
+// shared-memory bank groups where D is a multiple of 128. A larger m would carry the last units of a row
+// into the next one where D/16 is not a power of two (D = 96: units 2 and 3 of odd rows).
 __host__ __device__ inline uint32_t q8_qs_off(int row, int d, int D) {
     const int units = D / 16;
-    const int m = (units < 8 ? units : 8) - 1;
+    const int p2 = units & -units;
+    const int m = (p2 < 8 ? p2 : 8) - 1;
     return (uint32_t)(row * D + (((d >> 4) ^ (row & m)) << 4) + (d & 15));
 }
 
