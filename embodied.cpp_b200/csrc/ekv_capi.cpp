@@ -630,4 +630,148 @@ int ekv_append_suffix_attention(ekv_pool *p, const ekv_attn_params *prm, const v
     return ekv::launch_attention_tc(a, s, ekv::TcKernel::Auto);
 }
 
+int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_batch, const int32_t *seq_ids,
+                    const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int32_t max_rows,
+                    const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
+                    const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream) {
+    if (!p || !rope || !n_rows || !src_row || !positions) return EKV_ERR_INVALID_ARG;
+    if ((q == nullptr) != (q_out == nullptr) || (k == nullptr) != (v == nullptr) || (!q && !k)) return EKV_ERR_INVALID_ARG;
+    if (k && (!seq_ids || !dst_pos)) return EKV_ERR_INVALID_ARG;
+    const ekv_pool_config &c = p->cfg;
+    if (layer < 0 || layer >= c.n_layers || n_batch < 0 || n_batch > 65535 || max_rows < 0) return EKV_ERR_INVALID_ARG;
+    if (q && q_heads <= 0) return EKV_ERR_INVALID_ARG;
+    if (ekv::rope_dims(rope) > c.head_dim) return EKV_ERR_INVALID_ARG;
+    const int64_t q_row = q ? (int64_t)q_heads * c.head_dim : 0, kv_row = (int64_t)c.kv_heads * c.head_dim;
+    if (q_stride == 0) q_stride = q_row;
+    if (kv_stride == 0) kv_stride = kv_row;
+    if ((q && (q_stride < q_row || q_stride % 8)) || (k && (kv_stride < kv_row || kv_stride % 8))) return EKV_ERR_INVALID_ARG;
+    if (q && q == q_out && q_stride != q_row) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) return EKV_ERR_INVALID_ARG;
+    if (n_batch == 0 || max_rows == 0) return EKV_OK;
+    if (ekv::rope_device(rope) != c.device) return EKV_ERR_INVALID_ARG;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    return ekv::launch_rope_append(p->view, rope, layer, n_batch, seq_ids, dst_pos, n_rows, src_row, max_rows, positions,
+                                   q_heads, q, q_stride, q_out, k, v, kv_stride, p->sms, (cudaStream_t)stream);
+}
+
+// Checks what attention and key weights share, and the longest live sequence (which only sizes grids).
+static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const void *q, ekv::TreeArgs &a, int &max_len) {
+    if (!p || !prm || !q || !prm->seq_ids) return EKV_ERR_INVALID_ARG;
+    const ekv_pool_config &c = p->cfg;
+    if (prm->layer < 0 || prm->layer >= c.n_layers || prm->n_batch <= 0 || prm->n_draft <= 0 || prm->q_heads <= 0 ||
+        prm->q_heads % c.kv_heads)
+        return EKV_ERR_INVALID_ARG;
+    if (prm->n_draft > EKV_MAX_DRAFT) return EKV_ERR_RANGE;
+    if (!(prm->scale > 0.0f) || !std::isfinite(prm->scale) || !(prm->softcap >= 0.0f) || !std::isfinite(prm->softcap))
+        return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)q | ((uintptr_t)prm->ancestors << 1)) & 15) return EKV_ERR_INVALID_ARG;
+    if (c.head_dim != 48 && c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return EKV_ERR_UNSUPPORTED;
+    const float log2e = 1.4426950408889634f;
+    a = ekv::TreeArgs{};
+    a.pool = p->view;
+    a.layer = prm->layer;
+    a.n_batch = prm->n_batch;
+    a.n_draft = prm->n_draft;
+    a.q_heads = prm->q_heads;
+    a.group = prm->q_heads / c.kv_heads;
+    a.scale_log2 = prm->scale * log2e;
+    a.cap_log2 = prm->softcap * log2e;
+    a.cap_in = prm->softcap > 0.0f ? 2.0f * log2e * prm->scale / prm->softcap : 0.0f;
+    a.seq_ids = prm->seq_ids;
+    a.prefix_len = prm->prefix_len;
+    a.n_nodes = prm->n_nodes;
+    a.ancestors = prm->ancestors;
+    a.q = (const uint16_t *)q;
+    max_len = 0;
+    for (const ekv_pool::Seq &s : p->seqs)
+        if (s.live) max_len = std::max(max_len, s.n_tokens);
+    return EKV_OK;
+}
+
+size_t ekv_tree_attention_workspace_size(const ekv_pool *p, const ekv_tree_params *prm) {
+    if (!p || !prm || prm->n_batch <= 0 || prm->n_draft <= 0 || prm->n_draft > EKV_MAX_DRAFT || prm->q_heads <= 0 ||
+        prm->q_heads % p->cfg.kv_heads)
+        return 0;
+    return ekv::tree_workspace(p->view, prm->n_batch, prm->n_draft, prm->q_heads, p->sms);
+}
+
+int ekv_tree_attention(ekv_pool *p, const ekv_tree_params *prm, const void *q, const void *k_draft, const void *v_draft,
+                       void *out, float *lse, void *workspace, size_t workspace_bytes, ekv_stream_t stream) {
+    ekv::TreeArgs a;
+    int max_len = 0;
+    if (const int rc = fill_tree_args(p, prm, q, a, max_len)) return rc;
+    if (!k_draft || !v_draft || !out) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)k_draft | (uintptr_t)v_draft | (uintptr_t)out | (uintptr_t)workspace) & 15) return EKV_ERR_INVALID_ARG;
+    if ((uintptr_t)lse & 3) return EKV_ERR_INVALID_ARG;
+    if (prm->out_dtype != EKV_DTYPE_BF16 && prm->out_dtype != EKV_DTYPE_F32) return EKV_ERR_UNSUPPORTED;
+    a.k_draft = (const uint16_t *)k_draft;
+    a.v_draft = (const uint16_t *)v_draft;
+    a.out = out;
+    a.lse = lse;
+    a.out_dtype = prm->out_dtype;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    return ekv::launch_tree_attention(a, max_len, workspace, workspace_bytes, p->sms, (cudaStream_t)stream);
+}
+
+int ekv_key_weights(ekv_pool *p, const ekv_tree_params *prm, const void *q, const float *lse, float *weights,
+                    int64_t weight_stride, float decay, ekv_stream_t stream) {
+    ekv::TreeArgs a;
+    int max_len = 0;
+    if (const int rc = fill_tree_args(p, prm, q, a, max_len)) return rc;
+    if (!lse || !weights || weight_stride < 0 || !std::isfinite(decay)) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)lse | (uintptr_t)weights) & 3) return EKV_ERR_INVALID_ARG;
+    a.lse = const_cast<float *>(lse);
+    a.weights = weights;
+    a.weight_stride = weight_stride;
+    a.decay = decay;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    return ekv::launch_key_weights(a, max_len, p->sms, (cudaStream_t)stream);
+}
+
+int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t stream) {
+    if (!p || !prm || !prm->seq_ids || !prm->weights || !prm->kept) return EKV_ERR_INVALID_ARG;
+    const ekv_pool_config &c = p->cfg;
+    if (prm->layer0 < 0 || prm->n_layers <= 0 || prm->n_layers > c.n_layers - prm->layer0 || prm->n_batch <= 0)
+        return EKV_ERR_INVALID_ARG;
+    if (prm->keep <= 0 || prm->first < 0 || prm->recent < 0 || (int64_t)prm->first + prm->recent > prm->keep)
+        return EKV_ERR_INVALID_ARG;
+    if (prm->weight_stride < 0 || ((prm->weights_out || prm->positions_out) && prm->out_stride < prm->keep))
+        return EKV_ERR_INVALID_ARG;
+    // in place only where slot i is the same entry on both sides
+    if (((const float *)prm->weights_out == prm->weights || (prm->positions && prm->positions_out == prm->positions)) &&
+        prm->out_stride != prm->weight_stride)
+        return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)prm->weights | (uintptr_t)prm->kept | (uintptr_t)prm->positions | (uintptr_t)prm->weights_out |
+         (uintptr_t)prm->positions_out) & 3)
+        return EKV_ERR_INVALID_ARG;
+    int max_len = 0;
+    for (const ekv_pool::Seq &s : p->seqs)
+        if (s.live) max_len = std::max(max_len, s.n_tokens);
+    if (max_len > EKV_MAX_EVICT_TOKENS) return EKV_ERR_RANGE;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    ekv::EvictArgs a{};
+    a.pool = p->view;
+    a.layer0 = prm->layer0;
+    a.n_layers = prm->n_layers;
+    a.n_batch = prm->n_batch;
+    a.keep = prm->keep;
+    a.first = prm->first;
+    a.recent = prm->recent;
+    a.seq_ids = prm->seq_ids;
+    a.seen = prm->seen;
+    a.weights = prm->weights;
+    a.positions = prm->positions;
+    a.weight_stride = prm->weight_stride;
+    a.out_stride = prm->out_stride;
+    a.kept = prm->kept;
+    a.weights_out = prm->weights_out;
+    a.positions_out = prm->positions_out;
+    a.max_len = (int32_t)std::min<int64_t>((int64_t)c.max_blocks_per_seq * c.block_tokens, EKV_MAX_EVICT_TOKENS);
+    return ekv::launch_evict(a, (cudaStream_t)stream);
+}
+
 }  // extern "C"

@@ -1,0 +1,309 @@
+// ekv_decode.cuh -- shared parts of the decoding kernels over the paged pool (draft-tree attention and
+// key weights): work partition over ragged requests, the copy-engine feeder of 64-key tiles, and the
+// warp-level matrix instructions with their shared-memory operand loads.
+//
+// These kernels have few query rows per cached key (one row per drafted token and query head of a KV
+// head's group), so the bytes of the cache bound them, not the tensor pipe: 16 rows take
+// 32 * head_dim multiply-adds per key of 4 * head_dim bytes. mma.sync with operands in registers keeps
+// the whole row state (maximum, sum, output) in one warp and needs no tensor-memory round trip per tile.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "ekv_device.cuh"
+#include "ekv_internal.h"
+#include "ekv_sm100.cuh"
+
+namespace ekv {
+namespace decode {
+
+constexpr int kTile = 64;                       // keys per tile
+constexpr long long kWait = kDefaultWaitBudget; // clock cycles a bounded wait gives up after
+
+// ---- storage of a tile in shared memory ----
+template <int D, bool Q8>
+struct TileCfg {
+    static constexpr int W = (D * 2) % 128 == 0 ? 128 : (D * 2) % 64 == 0 ? 64 : 32;  // swizzle chunk (bf16)
+    static constexpr int G32 = D / 32;                                                // Q8_0 scale groups
+    static constexpr int KV_BYTES = Q8 ? kTile * D + kTile * G32 * 2 : kTile * D * 2; // K or V of a tile
+    static constexpr int SCALES = kTile * D;  // offset of the scales (Q8_0)
+};
+
+// Byte offset of (row, d) of a bf16 tile, compile-time head_dim.
+template <int D>
+__device__ __forceinline__ uint32_t bf16_off(int row, int d) {
+    constexpr int W = TileCfg<D, false>::W;
+    return tile_elem_off(row, d, D, W);
+}
+
+// ---- matrix instructions ----
+// D[16x8] += A[16x16] * B[16x8], bf16 operands, f32 accumulators.
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_f16(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return f16_bits_to_f32(v);
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t *)&h;
+}
+
+// Four int8 of a word to two bf16 pairs, exactly: with x = low7 - 128 * sign, the bf16 with upper byte
+// 0x43 and lower byte low7 is 128 + low7, and the one with lower byte (x & 0x80) is 128 or 256; their
+// difference is x.
+__device__ __forceinline__ void int8x4_to_bf16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const uint32_t m = w & 0x7f7f7f7fu, s = w & 0x80808080u;
+    const uint32_t a0 = __byte_perm(m, 0x43434343u, 0x4140), a1 = __byte_perm(m, 0x43434343u, 0x4342);
+    const uint32_t b0 = __byte_perm(s, 0x43434343u, 0x4140), b1 = __byte_perm(s, 0x43434343u, 0x4342);
+    const __nv_bfloat162 r0 = __hsub2(*(const __nv_bfloat162 *)&a0, *(const __nv_bfloat162 *)&b0);
+    const __nv_bfloat162 r1 = __hsub2(*(const __nv_bfloat162 *)&a1, *(const __nv_bfloat162 *)&b1);
+    lo = *(const uint32_t *)&r0;
+    hi = *(const uint32_t *)&r1;
+}
+
+// Score of q.k in the log2 domain: scale * q.k * log2(e), or cap * tanh(scale * q.k / cap) * log2(e) with
+// tanh(y) = 1 - 2 / (exp(2y) + 1) (f32; absolute error about 2^-23 of the cap, where a half-precision
+// tanh would lose 2^-11 of it).
+struct ScoreFn {
+    float scale_log2;  // scale * log2(e)
+    float cap_log2;    // cap * log2(e), 0 = no cap
+    float cap_in;      // 2 * log2(e) * scale / cap
+    __device__ __forceinline__ float operator()(float s) const {
+        if (cap_log2 == 0.0f) return s * scale_log2;
+        const float e = sm100::ex2(s * cap_in);
+        return cap_log2 * (1.0f - __fdividef(2.0f, e + 1.0f));
+    }
+};
+
+// ---- requests and the work partition ----
+// One request of the call: cached keys [0, n_prefix) and n_nodes drafted tokens.
+struct Req {
+    int seq, n_prefix, n_nodes;
+};
+
+__device__ __forceinline__ Req load_req(const TreeArgs &a, int b, bool report) {
+    Req r;
+    r.seq = a.seq_ids[b];
+    r.n_prefix = 0;
+    r.n_nodes = a.n_draft;
+    if (a.n_nodes) r.n_nodes = min(max(a.n_nodes[b], 0), a.n_draft);
+    if (r.seq < 0 || r.seq >= a.pool.max_seqs) {
+        if (report) report_error(a.pool.status, DEV_ERR_BAD_SEQ, b, r.seq, 5);
+        r.seq = 0;
+        return r;
+    }
+    const int len = a.pool.seq_lens[r.seq];
+    const int np = a.prefix_len ? a.prefix_len[b] : len;
+    if (np < 0 || np > len) {
+        if (report) report_error(a.pool.status, DEV_ERR_BAD_POS, b, np, len);
+        return r;
+    }
+    r.n_prefix = np;
+    return r;
+}
+
+// A flat order of all tiles of the call -- request, then unit (KV head, row tile), then tile -- is cut
+// into G = min(gridDim.x, T) equal ranges, whatever the requests' lengths: CTA c < G takes
+// [c T / G, (c + 1) T / G), at least one tile.
+struct Range {
+    long long total, lo, hi;  // T and this CTA's range
+    int ctas;                 // G
+    int b;                    // request that holds tile lo
+    long long base;           // first tile of request b
+};
+
+struct RangeScratch {
+    long long warp_sum[32];
+    long long base;
+    int b;
+};
+
+__device__ __forceinline__ long long range_lo(long long total, int c, int g) { return total * c / g; }
+
+// All threads of the block (NT of them). tiles(b): tiles of one unit of request b.
+template <int NT, class Tiles>
+__device__ __forceinline__ Range find_range(int n_batch, int units_per_req, RangeScratch &sh, Tiles tiles) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NW = NT / 32;
+    // inclusive scan of one chunk of NT requests; returns this thread's inclusive sum and the chunk's total
+    auto scan = [&](long long v, long long &chunk) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) sh.warp_sum[warp] = v;
+        __syncthreads();
+        long long before = 0;
+        chunk = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const long long s = sh.warp_sum[w];
+            if (w < warp) before += s;
+            chunk += s;
+        }
+        __syncthreads();
+        return v + before;
+    };
+    Range r;
+    r.total = 0;
+    long long v0 = tid < n_batch ? (long long)tiles(tid) * units_per_req : 0, incl0 = 0, chunk = 0;
+    if (tid == 0) {
+        sh.b = n_batch;
+        sh.base = 0;
+    }
+    for (int b0 = 0; b0 < n_batch; b0 += NT) {
+        const long long v = b0 == 0 ? v0 : (b0 + tid < n_batch ? (long long)tiles(b0 + tid) * units_per_req : 0);
+        const long long incl = scan(v, chunk);
+        if (b0 == 0) incl0 = incl;
+        r.total += chunk;
+    }
+    r.ctas = (int)min((long long)gridDim.x, r.total);
+    r.lo = r.hi = r.total;
+    if ((int)blockIdx.x < r.ctas) {
+        r.lo = range_lo(r.total, blockIdx.x, r.ctas);
+        r.hi = range_lo(r.total, blockIdx.x + 1, r.ctas);
+    }
+    long long base = 0;
+    for (int b0 = 0; b0 < n_batch; b0 += NT) {
+        long long v = v0, incl = incl0;
+        if (n_batch > NT) {
+            v = b0 + tid < n_batch ? (long long)tiles(b0 + tid) * units_per_req : 0;
+            incl = scan(v, chunk);
+        }
+        if (v > 0 && base + incl - v <= r.lo && r.lo < base + incl) {
+            sh.b = b0 + tid;
+            sh.base = base + incl - v;
+        }
+        base += chunk;
+    }
+    __syncthreads();
+    r.b = sh.b;
+    r.base = sh.base;
+    return r;
+}
+
+// ---- copy-engine feeder ----
+// One lane's share of a 64-key tile of the paged prefix: lanes 0-15 copy K, 16-31 V, one run of rows
+// inside one block each (blocks hold a multiple of 8 rows, so a tile spans at most 9 of them).
+struct Piece {
+    const uint8_t *src;  // first row of the run (bf16: its row group; Q8_0: its int8 row), or null
+    int row, n;          // first row inside the tile, rows (multiple of 8)
+    int rib;             // first row inside the block
+};
+
+template <int D, bool Q8>
+__device__ __forceinline__ Piece find_piece(const TreeArgs &a, const Req &rq, int head, int key0, int lane) {
+    const PoolView &p = a.pool;
+    const int valid = min(kTile, rq.n_prefix - key0), n8 = (valid + 7) & ~7;
+    const int kv = lane >> 4, i = lane & 15;
+    Piece pc;
+    pc.src = nullptr;
+    pc.row = pc.n = pc.rib = 0;
+    const int bt = p.block_tokens;
+    const int blk0 = p.bt_shift >= 0 ? key0 >> p.bt_shift : key0 / bt;
+    const int e = blk0 + i;
+    const int r0 = max(key0, e * bt), r1 = min(key0 + n8, (e + 1) * bt);
+    if (r1 <= r0) return pc;
+    const int blk = lookup_block(p, rq.seq, e);
+    if (blk < 0) return pc;
+    pc.row = r0 - key0;
+    pc.n = r1 - r0;
+    pc.rib = r0 - e * bt;
+    pc.src = p.prefix + prefix_tile_index(p, a.layer, blk, kv, head) * p.tile_bytes;
+    return pc;
+}
+
+// Issue the lane's copies of a tile whose K lands at `dst_k` (completion on bar_k) and V at `dst_v`.
+// With WITH_V false only K is copied.
+template <int D, bool Q8, bool WITH_V>
+__device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, uint32_t dst_k, uint32_t dst_v,
+                                            uint32_t bar_k, uint32_t bar_v, int lane) {
+    using C = TileCfg<D, Q8>;
+    using namespace sm100;
+    const bool is_v = lane >= 16;
+    const bool on = pc.src != nullptr && (WITH_V || !is_v);
+    const uint32_t bytes = !on ? 0u : Q8 ? (uint32_t)(pc.n * (D + C::G32 * 2)) : (uint32_t)(pc.n * D * 2);
+    const uint32_t kb = __reduce_add_sync(0xffffffffu, is_v ? 0u : bytes);
+    const uint32_t vb = WITH_V ? __reduce_add_sync(0xffffffffu, is_v ? bytes : 0u) : 0u;
+    if (lane == 0) {
+        mbar_arrive_expect_tx(bar_k, kb);
+        if (WITH_V) mbar_arrive_expect_tx(bar_v, vb);
+    }
+    __syncwarp();
+    if (!on) return;
+    const uint32_t dst = is_v ? dst_v : dst_k, bar = is_v ? bar_v : bar_k;
+    if (Q8) {
+        bulk_g2s(dst + pc.row * D, pc.src + pc.rib * D, (uint32_t)(pc.n * D), bar);
+        bulk_g2s(dst + C::SCALES + pc.row * C::G32 * 2, pc.src + (int64_t)a.pool.block_tokens * D + pc.rib * C::G32 * 2,
+                 (uint32_t)(pc.n * C::G32 * 2), bar);
+    } else {
+        bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2), bar);
+    }
+}
+
+// ---- scores of one warp's 16 keys ----
+// Column order of the matrix products. bf16 caches: natural. Q8_0 caches: step 2 g + i of group g (32
+// columns) gives lane c of a quad the columns 32 g + 8 c + 4 i + {0, 1 | 2, 3}, so that a lane reads its
+// 8 bytes of a group in one load; query rows are loaded in the same order, and a product does not depend
+// on it.
+template <bool Q8>
+__device__ __forceinline__ int q_col(int step, int c, int half) {
+    return Q8 ? 32 * (step >> 1) + 8 * c + 4 * (step & 1) + 2 * half : 16 * step + 2 * c + 8 * half;
+}
+
+// B operands of one 16-key x 16-column step of a bf16 tile: b[0..1] keys 0-7, b[2..3] keys 8-15.
+template <int D>
+__device__ __forceinline__ void load_k_step(uint32_t tile, int key0, int step, int lane, uint32_t (&b)[4]) {
+    const int row = key0 + (lane & 7) + ((lane >> 4) << 3);
+    ldmatrix_x4(b, tile + bf16_off<D>(row, 16 * step + ((lane >> 3) & 1) * 8));
+}
+
+// B operands of one 16-key x 16-column step of V^T: b[0..1] columns 0-7 of the step, b[2..3] columns 8-15.
+template <int D>
+__device__ __forceinline__ void load_v_step(uint32_t tile, int key0, int step, int lane, uint32_t (&b)[4]) {
+    const int row = key0 + (lane & 15);
+    ldmatrix_x4_trans(b, tile + bf16_off<D>(row, 16 * step + (lane >> 4) * 8));
+}
+
+}  // namespace decode
+}  // namespace ekv

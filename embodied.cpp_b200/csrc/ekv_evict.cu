@@ -1,0 +1,303 @@
+// ekv_evict.cu -- eviction from the paged cache by accumulated attention weight.
+//
+// Every (layer, request, KV head) keeps `keep` of its rows: the first tokens, the most recent ones, and the
+// heaviest others (ties to the lower slot). Survivors below `keep` stay where they are; the i-th free slot
+// takes the i-th survivor at or above `keep`. So the bytes moved go with the rows that left, not with the
+// rows that stay: a cache that gave up 100 of 1100 rows moves at most 100. Sources and destinations are
+// disjoint, so rows move in any order.
+//   evict_select_kernel  one CTA per (layer, request, KV head): the keep-th largest key by radix selection on
+//                        its bits, one bit per slot for the choice, then a slot for each survivor
+//   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed
+#include <algorithm>
+
+#include "ekv_device.cuh"
+#include "ekv_internal.h"
+
+namespace ekv {
+namespace {
+
+constexpr int kSelThreads = 1024;
+constexpr int kBins = 2048;  // 11 bits of the key at a time: 11, 11, 10
+constexpr int kMoveWarps = 8;
+
+// Larger is kept first. Protected rows are above every weight, NaN is below.
+__device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
+    if (safe) return 0xffffffffu;
+    if (w != w) return 0u;
+    const uint32_t b = __float_as_uint(w + 0.0f);  // -0 counts as 0
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+struct SelShared {
+    uint32_t hist[kBins];
+    uint32_t warp_sum[2][32];
+    uint32_t digit, above;
+};
+
+// Block-wide exclusive scan of one value per thread; the total in `total`.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sum, uint32_t &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t w = warp_sum[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += u;
+        }
+        warp_sum[lane] = w;
+    }
+    __syncthreads();
+    total = warp_sum[31];
+    const uint32_t r = s - v + (warp ? warp_sum[warp - 1] : 0u);
+    __syncthreads();
+    return r;
+}
+
+__global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a) {
+    extern __shared__ uint32_t s_mem[];
+    __shared__ SelShared sh;
+    const int hk = a.pool.kv_heads;
+    const int lbh = blockIdx.x, b = (lbh / hk) % a.n_batch;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int seq = a.seq_ids[b];
+    int n = 0;
+    if (seq < 0 || seq >= a.pool.max_seqs) {
+        if (tid == 0) report_error(a.pool.status, DEV_ERR_BAD_SEQ, b, seq, 10);
+    } else {
+        n = a.pool.seq_lens[seq];
+        if (n > a.weight_stride || n > a.max_len) {
+            if (tid == 0) report_error(a.pool.status, DEV_ERR_BAD_POS, seq, n, 10);
+            n = 0;
+        }
+    }
+    const float *w = a.weights + (int64_t)lbh * a.weight_stride;
+    const int32_t *pos = a.positions ? a.positions + (int64_t)lbh * a.weight_stride : nullptr;
+    int32_t *kept = a.kept + (int64_t)lbh * a.keep;
+    float *w_out = a.weights_out ? a.weights_out + (int64_t)lbh * a.out_stride : nullptr;
+    int32_t *p_out = a.positions_out ? a.positions_out + (int64_t)lbh * a.out_stride : nullptr;
+    const int recent_from = (a.seen ? a.seen[b] : n) - a.recent;
+    auto key_of = [&](int i) {
+        const int age = pos ? pos[i] : i;
+        return evict_key(w[i], age < a.first || age >= recent_from);
+    };
+
+    if (n <= a.keep) {  // everything stays
+        for (int i = tid; i < a.keep; i += kSelThreads) {
+            const bool on = i < n;
+            kept[i] = on ? i : -1;
+            const float wi = on ? w[i] : 0.0f;
+            const int32_t pi = on ? (pos ? pos[i] : i) : -1;
+            if (w_out) w_out[i] = wi;
+            if (p_out) p_out[i] = pi;
+        }
+        return;
+    }
+
+    // ---- the keep-th largest key, from its upper bits down ----
+    uint32_t prefix = 0, mask = 0;
+    uint32_t need = (uint32_t)a.keep;  // how many of the keys that match `prefix` are kept
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1024u : 2048u;
+        for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSelThreads) {
+            const uint32_t k = key_of(i);
+            if ((k & mask) == prefix) atomicAdd(&sh.hist[(k >> shift) & (digits - 1)], 1u);
+        }
+        __syncthreads();
+        // digits from the top: thread t holds digits 2 (1023 - t) + 1 and 2 (1023 - t)
+        const int d = 2 * (kSelThreads - 1 - tid);
+        const uint32_t hi = sh.hist[d + 1], lo = sh.hist[d];
+        uint32_t total;
+        const uint32_t before = block_scan(hi + lo, sh.warp_sum[0], total);
+        if (before < need && need <= before + hi) {
+            sh.digit = d + 1;
+            sh.above = before;
+        } else if (before + hi < need && need <= before + hi + lo) {
+            sh.digit = d;
+            sh.above = before + hi;
+        }
+        __syncthreads();
+        prefix |= sh.digit << shift;
+        mask |= (digits - 1) << shift;
+        need -= sh.above;
+        __syncthreads();
+    }
+
+    // ---- one bit per slot: keys above the threshold, and the first `need` equal to it ----
+    const int words = (n + 31) / 32;
+    uint32_t *sel = s_mem, *cnt = s_mem + a.max_words;  // chosen slots; ties, then survivors at or above keep before a word
+    for (int wd = warp; wd < words; wd += kSelThreads / 32) {
+        const int i = 32 * wd + lane;
+        const uint32_t k = i < n ? key_of(i) : 0u;
+        const uint32_t gt = __ballot_sync(0xffffffffu, i < n && k > prefix);
+        const uint32_t eq = __ballot_sync(0xffffffffu, i < n && k == prefix);
+        if (lane == 0) {
+            sel[wd] = gt;
+            cnt[wd] = eq;
+        }
+    }
+    __syncthreads();
+    uint32_t ties = 0;
+    for (int w0 = 0; w0 < words; w0 += kSelThreads) {
+        const int wd = w0 + tid;
+        const uint32_t eq = wd < words ? cnt[wd] : 0u;
+        uint32_t total;
+        uint32_t rank = ties + block_scan(__popc(eq), sh.warp_sum[0], total);
+        if (eq && rank < need) {
+            uint32_t take = need - rank, e = eq, got = 0;
+            if (take >= (uint32_t)__popc(eq)) {
+                got = eq;
+            } else {
+                for (; take; --take) {
+                    got |= e & (0u - e);
+                    e &= e - 1;
+                }
+            }
+            sel[wd] |= got;
+        }
+        ties += total;
+    }
+    __syncthreads();
+    // ---- survivors at or above keep before each word ----
+    const int first_tail = a.keep >> 5;  // the word that holds slot keep
+    auto tail_bits = [&](int wd) {
+        return wd < first_tail ? 0u : wd == first_tail ? sel[wd] & ~((1u << (a.keep & 31)) - 1u) : sel[wd];
+    };
+    uint32_t tails = 0;
+    for (int w0 = first_tail; w0 < words; w0 += kSelThreads) {
+        const int wd = w0 + tid;
+        uint32_t total;
+        const uint32_t before = tails + block_scan(wd < words ? __popc(tail_bits(wd)) : 0u, sh.warp_sum[0], total);
+        if (wd < words) cnt[wd] = before;
+        tails += total;
+    }
+    __syncthreads();
+    // ---- free slots below keep, in order, take them ----
+    uint32_t holes = 0;
+    for (int i0 = 0; i0 < a.keep; i0 += kSelThreads) {
+        const int i = i0 + tid;
+        const bool hole = i < a.keep && !((sel[i >> 5] >> (i & 31)) & 1u);
+        uint32_t total;
+        const uint32_t rank = holes + block_scan(hole ? 1u : 0u, sh.warp_sum[0], total);
+        holes += total;
+        if (i >= a.keep) continue;
+        int from = i;
+        if (hole) {
+            int lo = first_tail, hi = words - 1;  // the last word with at most `rank` survivors before it
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (cnt[mid] <= rank) lo = mid;
+                else hi = mid - 1;
+            }
+            uint32_t bits = tail_bits(lo);
+            for (uint32_t k = rank - cnt[lo]; k; --k) bits &= bits - 1;
+            from = 32 * lo + __ffs(bits) - 1;
+        }
+        kept[i] = from;
+        const float wi = w[from];
+        const int32_t pi = pos ? pos[from] : from;
+        if (w_out) w_out[i] = wi;
+        if (p_out) p_out[i] = pi;
+    }
+}
+
+__global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a, int chunks) {
+    __shared__ const uint8_t *s_src[kMoveWarps][32];
+    __shared__ uint8_t *s_dst[kMoveWarps][32];
+    __shared__ int s_rows[kMoveWarps][32];  // row inside the source block << 16 | inside the destination block
+    const PoolView &p = a.pool;
+    const int lbh = blockIdx.x / chunks, chunk = blockIdx.x - lbh * chunks;
+    const int h = lbh % p.kv_heads, lb = lbh / p.kv_heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slot = (chunk * kMoveWarps + warp) * 32 + lane;
+    const int seq = a.seq_ids[b];
+    int from = slot;
+    if (slot < a.keep) from = a.kept[(int64_t)lbh * a.keep + slot];
+    bool move = slot < a.keep && from >= 0 && from != slot;
+    int bs = -1, bd = -1;
+    if (move) {
+        bs = lookup_block(p, seq, from / p.block_tokens);
+        bd = lookup_block(p, seq, slot / p.block_tokens);
+        move = bs >= 0 && bd >= 0;
+    }
+    const uint32_t moving = __ballot_sync(0xffffffffu, move);
+    if (!moving) return;
+    const int n = __popc(moving);
+    if (move) {
+        const int i = __popc(moving & ((1u << lane) - 1u));
+        s_src[warp][i] = p.prefix + prefix_tile_index(p, layer, bs, 0, h) * p.tile_bytes;
+        s_dst[warp][i] = p.prefix + prefix_tile_index(p, layer, bd, 0, h) * p.tile_bytes;
+        s_rows[warp][i] = from % p.block_tokens << 16 | slot % p.block_tokens;
+    }
+    __syncwarp();
+    const int D = p.head_dim;
+    const int64_t kv_bytes = (int64_t)p.kv_heads * p.tile_bytes;
+    const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
+    const int per = q8 ? D / 16 : D / 8, units = 2 * per;  // 16-byte units of a row, K then V
+    constexpr int UNROLL = 4;
+    for (int i0 = lane; i0 < n * units; i0 += 32 * UNROLL) {
+        uint4 v[UNROLL];
+        uint8_t *to[UNROLL];
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+            const int i = i0 + 32 * j;
+            to[j] = nullptr;
+            if (i >= n * units) continue;
+            const int m = i / units;
+            int u = i - m * units;
+            const int64_t kv = u >= per ? kv_bytes : 0;
+            if (u >= per) u -= per;
+            const int rs = s_rows[warp][m] >> 16, rd = s_rows[warp][m] & 0xffff;
+            const uint32_t os = q8 ? q8_qs_off(rs, 16 * u, D) : tile_elem_off(rs, 8 * u, D, p.swz_bytes);
+            const uint32_t od = q8 ? q8_qs_off(rd, 16 * u, D) : tile_elem_off(rd, 8 * u, D, p.swz_bytes);
+            v[j] = *(const uint4 *)(s_src[warp][m] + kv + os);
+            to[j] = s_dst[warp][m] + kv + od;
+        }
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j)
+            if (to[j]) *(uint4 *)to[j] = v[j];
+    }
+    if (!q8) return;
+    const int g = D / 32;
+    for (int i = lane; i < n * 2 * g; i += 32) {
+        const int m = i / (2 * g);
+        int u = i - m * 2 * g;
+        const int64_t base = (u >= g ? kv_bytes : 0) + (int64_t)p.block_tokens * D;
+        if (u >= g) u -= g;
+        const int rs = s_rows[warp][m] >> 16, rd = s_rows[warp][m] & 0xffff;
+        *(uint16_t *)(s_dst[warp][m] + base + (rd * g + u) * 2) = *(const uint16_t *)(s_src[warp][m] + base + (rs * g + u) * 2);
+    }
+}
+
+}  // namespace
+
+int launch_evict(EvictArgs a, cudaStream_t s) {
+    const int64_t n = (int64_t)a.n_layers * a.n_batch * a.pool.kv_heads;
+    const int chunks = (a.keep + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
+    if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
+    a.max_words = (a.max_len + 31) / 32 + 1;
+    const size_t smem = (size_t)a.max_words * 2 * sizeof(uint32_t);
+    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+        cudaGetLastError();
+        return EKV_ERR_CUDA;
+    }
+    evict_select_kernel<<<(unsigned)n, kSelThreads, smem, s>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
+    evict_move_kernel<<<(unsigned)(n * chunks), kMoveWarps * 32, 0, s>>>(a, chunks);
+    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
+    note_launches(2);
+    return EKV_OK;
+}
+
+}  // namespace ekv

@@ -65,6 +65,46 @@ struct AttnArgs {
     int32_t mask_bits_words, mask_bits_nb;
 };
 
+// A decoding call (draft-tree attention, key weights).
+struct TreeArgs {
+    PoolView pool;
+    int32_t layer, n_batch, n_draft, q_heads, group;
+    float scale_log2;  // scale * log2(e)
+    float cap_log2;    // softcap * log2(e), 0 = none
+    float cap_in;      // 2 * log2(e) * scale / softcap
+    int32_t out_dtype;
+    const int32_t *seq_ids, *prefix_len, *n_nodes;
+    const uint64_t *ancestors;  // [n_batch][n_draft], or null: a chain
+    const uint16_t *q, *k_draft, *v_draft;
+    void *out;
+    float *lse;        // attention: written, or null; key weights: read
+    // attention: partial results of units cut between CTAs
+    int32_t split;     // 0: CTA = unit
+    int32_t row_tiles; // row tiles of one (request, KV head)
+    int2 *parts;       // [units] first and last CTA of each unit
+    float2 *ws_ml;     // [2 * CTAs][rows] maximum (log2 domain) and sum
+    float *ws_o;       // [2 * CTAs][rows][D] unnormalised output
+    // key weights
+    float *weights;    // [n_batch][kv_heads][weight_stride]
+    int64_t weight_stride;
+    float decay;
+};
+
+// An eviction (ekv_evict_params, with the pool).
+struct EvictArgs {
+    PoolView pool;
+    int32_t layer0, n_layers, n_batch, keep, first, recent;
+    const int32_t *seq_ids, *seen;
+    const float *weights;
+    const int32_t *positions;
+    int64_t weight_stride, out_stride;
+    int32_t *kept;
+    float *weights_out;
+    int32_t *positions_out;
+    int32_t max_len;    // slots that the selection has room for
+    int32_t max_words;  // (set by the launcher)
+};
+
 constexpr long long kDefaultWaitBudget = 4000000000LL;  // clock cycles, about 2 s
 constexpr long long kDebugWaitBudget = 20000000LL;      // about 10 ms
 // Consumed by the next launch of the 64-key CTA-pair kernel (ekv_debug_expire_wait).
@@ -111,6 +151,21 @@ int launch_attention_heads(const AttnArgs &a, cudaStream_t s, int sms);
 int launch_project_qkv(const PoolView &p, int layer, int n_batch, const int32_t *seq_ids, int tokens, int q_heads,
                        int hidden, const void *x, const void *wq, const void *wk, const void *wv, const int32_t *positions,
                        float rope_base, void *q_out, void *k_out, void *v_out, cudaStream_t s);
+// Draft-tree attention (ekv_tree.cu). The workspace size depends on the call's shape alone; max_len, an
+// upper bound of the cached lengths, only sizes the grid.
+size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, int sms);
+int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s);
+// Key weights (ekv_weights.cu)
+int launch_key_weights(const TreeArgs &a, int max_len, int sms, cudaStream_t s);
+// Rotary positions and append (ekv_rope.cu)
+int rope_device(const ekv_rope *r);
+int rope_dims(const ekv_rope *r);
+int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n_batch, const int32_t *seq_ids,
+                       const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int max_rows,
+                       const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
+                       const void *v, int64_t kv_stride, int sms, cudaStream_t s);
+// Eviction by weight (ekv_evict.cu)
+int launch_evict(EvictArgs a, cudaStream_t s);
 // combine key-split partial outputs (head_dim of the pool) into a.out
 int launch_merge_splits(const AttnArgs &a, int n_qtiles, cudaStream_t s);
 #ifdef EKV_TRACE

@@ -1,0 +1,326 @@
+// ekv_rope.cu -- rotary positions on q and k, with the rotated k and the v written into the pool's pages.
+//
+// Pair i of a head turns by pos * f_i: (a, b) -> mag * (a cos - b sin, a sin + b cos). The angle is taken in
+// turns, pos * (f_i / 2 pi) in 64 bits, reduced to its fraction, and only then rounded to 32: at position
+// 100000 a 32-bit product would be off by 0.004 radians. One CTA computes the sines of its rows once and uses
+// them for every head; the rest is a stream of 16-byte loads and stores.
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "ekv_device.cuh"
+#include "ekv_internal.h"
+
+struct ekv_rope {
+    int32_t device, interleaved, rotary;
+    float magnitude;
+    double freq[128];      // radians per position of each pair
+    double *dev_turns;     // the same in turns, on the device
+};
+
+namespace ekv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRows = 8;  // rows per CTA
+
+struct RopeArgs {
+    PoolView pool;
+    int32_t layer, n_batch, max_rows, rows_per_cta, q_heads, interleaved, rotary;
+    float magnitude;
+    const double *turns;
+    const int32_t *seq_ids, *dst_pos, *n_rows, *src_row, *positions;
+    const uint16_t *q, *k, *v;
+    int64_t q_stride, kv_stride;  // elements per source row
+    uint16_t *q_out;
+};
+
+__device__ __forceinline__ uint32_t rot_pair(uint32_t lo_hi, float2 cs) {  // an interleaved pair in one word
+    const float x = bf16_bits_to_f32((uint16_t)lo_hi), y = bf16_bits_to_f32((uint16_t)(lo_hi >> 16));
+    const uint32_t a = f32_to_bf16_bits(x * cs.x - y * cs.y), b = f32_to_bf16_bits(x * cs.y + y * cs.x);
+    return a | b << 16;
+}
+
+// One head's unit u: 16 bytes, or the two 16-byte halves of eight split pairs. `put(d, value)` writes the 16
+// bytes of columns d .. d + 7.
+template <class Put>
+__device__ __forceinline__ void rot_unit(const RopeArgs &a, const uint16_t *src, int u, const float2 *cs, Put put) {
+    const int n = a.rotary;
+    if (a.interleaved) {
+        const int d = 8 * u;
+        uint4 x = *(const uint4 *)(src + d);
+        if (d < n) {
+            x.x = rot_pair(x.x, cs[d / 2]);
+            if (d + 2 < n) x.y = rot_pair(x.y, cs[d / 2 + 1]);
+            if (d + 4 < n) x.z = rot_pair(x.z, cs[d / 2 + 2]);
+            if (d + 6 < n) x.w = rot_pair(x.w, cs[d / 2 + 3]);
+        }
+        put(d, x);
+        return;
+    }
+    const int pairs = n / 16;  // units of eight split pairs; the columns past the rotated ones follow
+    if (u >= pairs) {
+        const int d = n + 8 * (u - pairs);
+        put(d, *(const uint4 *)(src + d));
+        return;
+    }
+    const int d = 8 * u, h = n / 2;
+    const uint4 x = *(const uint4 *)(src + d), y = *(const uint4 *)(src + d + h);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    uint32_t p[4], q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t e = rot_pair((xs[i] & 0xffffu) | ys[i] << 16, cs[d + 2 * i]);
+        const uint32_t o = rot_pair(xs[i] >> 16 | (ys[i] & 0xffff0000u), cs[d + 2 * i + 1]);
+        p[i] = (e & 0xffffu) | o << 16;
+        q[i] = e >> 16 | (o & 0xffff0000u);
+    }
+    put(d, make_uint4(p[0], p[1], p[2], p[3]));
+    put(d + h, make_uint4(q[0], q[1], q[2], q[3]));
+}
+
+// Element i of the odd forms (split pairs that are not whole 16-byte units): i < n / 2 a pair, then the rest.
+template <class Put>
+__device__ __forceinline__ void rot_item(const RopeArgs &a, const uint16_t *src, int i, const float2 *cs, Put put) {
+    const int h = a.rotary / 2;
+    if (i >= h) {
+        put(i + h, src[i + h]);
+        return;
+    }
+    const uint32_t r = rot_pair((uint32_t)src[i] | (uint32_t)src[i + h] << 16, cs[i]);
+    put(i, (uint16_t)r);
+    put(i + h, (uint16_t)(r >> 16));
+}
+
+// Rotated, bf16-rounded column d of a head (Q8_0 pools quantise whole 32-column groups).
+__device__ __forceinline__ float rot_at(const RopeArgs &a, const uint16_t *src, int d, const float2 *cs) {
+    if (d >= a.rotary) return bf16_bits_to_f32(src[d]);
+    const int h = a.rotary / 2;
+    const int i = a.interleaved ? d >> 1 : d < h ? d : d - h;
+    const bool second = a.interleaved ? d & 1 : d >= h;
+    const uint32_t w = a.interleaved ? (uint32_t)src[2 * i] | (uint32_t)src[2 * i + 1] << 16
+                                     : (uint32_t)src[i] | (uint32_t)src[i + h] << 16;
+    const uint32_t r = rot_pair(w, cs[i]);
+    return bf16_bits_to_f32(second ? (uint16_t)(r >> 16) : (uint16_t)r);
+}
+
+// Grid: (row chunk, request). WIDE: every head is whole 16-byte units.
+template <bool Q8, bool WIDE>
+__global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a) {
+    extern __shared__ float2 s_cs[];  // [rows][rotary / 2]
+    __shared__ int s_blk[kMaxRows], s_rib[kMaxRows];
+    const PoolView &p = a.pool;
+    const int b = blockIdx.y, r0 = blockIdx.x * a.rows_per_cta;
+    const int nr = min(a.rows_per_cta, min(a.max_rows, a.n_rows[b]) - r0);
+    if (nr <= 0) return;
+    const int half = a.rotary / 2, D = p.head_dim;
+    const int64_t row0 = (int64_t)a.src_row[b] + r0;
+    if (a.k && (int)threadIdx.x < nr) {
+        const int seq = a.seq_ids[b], pos = a.dst_pos[b] + r0 + (int)threadIdx.x;
+        int blk = -1;
+        if (seq < 0 || seq >= p.max_seqs) {
+            report_error(p.status, DEV_ERR_BAD_SEQ, seq, pos, 9);
+        } else if (pos < 0 || pos >= p.seq_lens[seq]) {
+            report_error(p.status, DEV_ERR_BAD_POS, seq, pos, p.seq_lens[seq]);
+        } else {
+            blk = lookup_block(p, seq, pos / p.block_tokens);
+        }
+        s_blk[threadIdx.x] = blk;
+        s_rib[threadIdx.x] = pos < 0 ? 0 : pos % p.block_tokens;
+    }
+    for (int i = threadIdx.x; i < nr * half; i += kThreads) {
+        const int r = i / half, j = i - r * half;
+        const double t = (double)a.positions[row0 + r] * a.turns[j];
+        float sn, cn;
+        sincospif(2.0f * (float)(t - rint(t)), &sn, &cn);
+        s_cs[i] = make_float2(cn * a.magnitude, sn * a.magnitude);
+    }
+    __syncthreads();
+    // items of a row: q heads, k heads, v heads
+    const int per = WIDE ? (a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8) : half + D - a.rotary;
+    const int nq = a.q ? a.q_heads * per : 0;
+    const int nk = !a.k ? 0 : p.kv_heads * (Q8 ? D / 32 : per), nv = !a.k ? 0 : p.kv_heads * (Q8 ? D / 32 : D / 8);
+    const int items = nq + nk + nv;
+    for (int i = threadIdx.x; i < nr * items; i += kThreads) {
+        const int r = i / items;
+        int u = i - r * items;
+        const float2 *cs = s_cs + r * half;
+        if (u < nq) {
+            const int h = u / per;
+            u -= h * per;
+            const uint16_t *src = a.q + (row0 + r) * a.q_stride + h * D;
+            uint16_t *dst = a.q_out + ((row0 + r) * a.q_heads + h) * D;
+            if (WIDE) rot_unit(a, src, u, cs, [&](int d, uint4 x) { *(uint4 *)(dst + d) = x; });
+            else rot_item(a, src, u, cs, [&](int d, uint16_t x) { dst[d] = x; });
+            continue;
+        }
+        const int blk = s_blk[r], rib = s_rib[r];
+        if (blk < 0) continue;
+        u -= nq;
+        const bool is_v = u >= nk;
+        if (is_v) u -= nk;
+        const int n_u = Q8 ? D / 32 : is_v ? D / 8 : per;
+        const int h = u / n_u;
+        u -= h * n_u;
+        const uint16_t *src = (is_v ? a.v : a.k) + (row0 + r) * a.kv_stride + h * D;
+        uint8_t *tile = p.prefix + prefix_tile_index(p, a.layer, blk, is_v ? 1 : 0, h) * p.tile_bytes;
+        if (!Q8) {
+            const auto put = [&](int d, uint4 x) { *(uint4 *)(tile + tile_elem_off(rib, d, D, p.swz_bytes)) = x; };
+            if (is_v) put(8 * u, *(const uint4 *)(src + 8 * u));
+            else if (WIDE) rot_unit(a, src, u, cs, put);
+            else rot_item(a, src, u, cs, [&](int d, uint16_t x) { *(uint16_t *)(tile + tile_elem_off(rib, d, D, p.swz_bytes)) = x; });
+            continue;
+        }
+        // the group's values as ekv_append would get them (bf16), quantised by its rule
+        float x[32], amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            x[j] = is_v ? bf16_bits_to_f32(src[32 * u + j]) : rot_at(a, src, 32 * u + j, cs);
+            amax = fmaxf(amax, fabsf(x[j]));
+        }
+        const float d = __fdiv_rn(amax, 127.0f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[j] |= ((uint32_t)(uint8_t)(int8_t)(int)roundf(__fmul_rn(x[4 * j + e], id))) << (8 * e);
+        }
+        *(uint4 *)(tile + q8_qs_off(rib, 32 * u, D)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *(uint4 *)(tile + q8_qs_off(rib, 32 * u + 16, D)) = make_uint4(w[4], w[5], w[6], w[7]);
+        *((uint16_t *)(tile + (int64_t)p.block_tokens * D) + rib * (D / 32) + u) = __half_as_ushort(__float2half_rn(d));
+    }
+}
+
+}  // namespace
+
+int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n_batch, const int32_t *seq_ids,
+                       const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int max_rows,
+                       const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
+                       const void *v, int64_t kv_stride, int sms, cudaStream_t s) {
+    RopeArgs a{};
+    a.pool = p;
+    a.layer = layer;
+    a.n_batch = n_batch;
+    a.max_rows = max_rows;
+    a.q_heads = q_heads;
+    a.interleaved = rope->interleaved;
+    a.rotary = rope->rotary;
+    a.magnitude = rope->magnitude;
+    a.turns = rope->dev_turns;
+    a.seq_ids = seq_ids;
+    a.dst_pos = dst_pos;
+    a.n_rows = n_rows;
+    a.src_row = src_row;
+    a.positions = positions;
+    a.q = (const uint16_t *)q;
+    a.k = (const uint16_t *)k;
+    a.v = (const uint16_t *)v;
+    a.q_stride = q_stride;
+    a.kv_stride = kv_stride;
+    a.q_out = (uint16_t *)q_out;
+    a.rows_per_cta = (int)std::min<int64_t>(kMaxRows, std::max<int64_t>(1, (int64_t)max_rows * n_batch / (8 * sms)));
+    const dim3 grid((unsigned)((max_rows + a.rows_per_cta - 1) / a.rows_per_cta), (unsigned)n_batch);
+    const size_t smem = (size_t)a.rows_per_cta * (a.rotary / 2) * sizeof(float2);
+    const bool wide = a.interleaved || a.rotary % 16 == 0;
+    if (p.dtype == EKV_DTYPE_Q8_0) {
+        if (wide) rope_append_kernel<true, true><<<grid, kThreads, smem, s>>>(a);
+        else rope_append_kernel<true, false><<<grid, kThreads, smem, s>>>(a);
+    } else {
+        if (wide) rope_append_kernel<false, true><<<grid, kThreads, smem, s>>>(a);
+        else rope_append_kernel<false, false><<<grid, kThreads, smem, s>>>(a);
+    }
+    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
+    note_launches(1);
+    return EKV_OK;
+}
+
+int rope_device(const ekv_rope *r) { return r->device; }
+int rope_dims(const ekv_rope *r) { return r->rotary; }
+
+}  // namespace ekv
+
+extern "C" int ekv_rope_create(const ekv_rope_config *c, ekv_rope **out) {
+    if (!c || !out) return EKV_ERR_INVALID_ARG;
+    *out = nullptr;
+    if (c->rotary_dims < 2 || c->rotary_dims % 2) return EKV_ERR_INVALID_ARG;
+    if (c->rotary_dims > 256) return EKV_ERR_UNSUPPORTED;
+    if (c->layout != EKV_ROPE_HALF && c->layout != EKV_ROPE_INTERLEAVED) return EKV_ERR_INVALID_ARG;
+    if (!(c->freq_base > 1.0f) || !std::isfinite(c->freq_base) || !(c->freq_scale > 0.0f) || !std::isfinite(c->freq_scale) ||
+        !std::isfinite(c->attn_factor) || !(c->ext_factor >= 0.0f && c->ext_factor <= 1.0f))
+        return EKV_ERR_INVALID_ARG;
+    const double n = c->rotary_dims, base = c->freq_base;
+    double low = 0, high = 0;
+    if (c->ext_factor != 0.0f) {
+        if (c->n_ctx_orig <= 0 || !(c->beta_fast > 0.0f) || !(c->beta_slow > 0.0f)) return EKV_ERR_INVALID_ARG;
+        // the pair that turns `beta` times over the trained length
+        const double two_pi = 6.283185307179586476925;
+        low = std::floor(n * std::log(c->n_ctx_orig / (c->beta_fast * two_pi)) / (2 * std::log(base)));
+        high = std::ceil(n * std::log(c->n_ctx_orig / (c->beta_slow * two_pi)) / (2 * std::log(base)));
+        low = std::max(0.0, low);
+        high = std::min(n - 1, high);
+    }
+    ekv_rope *r = new (std::nothrow) ekv_rope();
+    if (!r) return EKV_ERR_ALLOC;
+    r->device = c->device;
+    r->interleaved = c->layout == EKV_ROPE_INTERLEAVED;
+    r->rotary = c->rotary_dims;
+    r->magnitude = c->attn_factor;
+    if (c->ext_factor != 0.0f) r->magnitude *= (float)(1.0 + 0.1 * std::log(1.0 / (double)c->freq_scale));
+    r->dev_turns = nullptr;
+    double turns[128];
+    for (int i = 0; i < c->rotary_dims / 2; ++i) {
+        const double ff = c->freq_factors ? (double)c->freq_factors[i] : 1.0;
+        if (!(ff > 0.0) || !std::isfinite(ff)) {
+            delete r;
+            return EKV_ERR_INVALID_ARG;
+        }
+        const double f = std::pow(base, -2.0 * i / n) / ff;
+        double kept = 0.0;  // the share of the unscaled frequency
+        if (c->ext_factor != 0.0f)
+            kept = (1.0 - std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low)))) * c->ext_factor;
+        r->freq[i] = f * (kept + (1.0 - kept) * c->freq_scale);
+        turns[i] = r->freq[i] / 6.283185307179586476925;
+    }
+    if (c->device >= 0) {
+        int prev = 0;
+        if (cudaGetDevice(&prev) != cudaSuccess || (prev != c->device && cudaSetDevice(c->device) != cudaSuccess)) {
+            cudaGetLastError();
+            delete r;
+            return EKV_ERR_CUDA;
+        }
+        const size_t bytes = (size_t)(c->rotary_dims / 2) * sizeof(double);
+        int rc = cudaMalloc((void **)&r->dev_turns, bytes) == cudaSuccess ? EKV_OK : EKV_ERR_ALLOC;
+        if (!rc && cudaMemcpy(r->dev_turns, turns, bytes, cudaMemcpyHostToDevice) != cudaSuccess) rc = EKV_ERR_CUDA;
+        if (rc && r->dev_turns) cudaFree(r->dev_turns);
+        if (rc) cudaGetLastError();
+        if (prev != c->device) cudaSetDevice(prev);
+        if (rc) {
+            delete r;
+            return rc;
+        }
+    }
+    *out = r;
+    return EKV_OK;
+}
+
+extern "C" int ekv_rope_destroy(ekv_rope *r) {
+    if (!r) return EKV_ERR_INVALID_ARG;
+    if (r->dev_turns) {
+        int prev = 0;
+        const bool have = cudaGetDevice(&prev) == cudaSuccess;
+        if (have && prev != r->device) cudaSetDevice(r->device);
+        cudaFree(r->dev_turns);
+        if (have && prev != r->device) cudaSetDevice(prev);
+    }
+    delete r;
+    return EKV_OK;
+}
+
+extern "C" int ekv_rope_get(const ekv_rope *r, double *freq, int32_t cap, float *magnitude) {
+    if (!r || cap < 0 || (cap > 0 && !freq)) return EKV_ERR_INVALID_ARG;
+    for (int i = 0; i < std::min(cap, r->rotary / 2); ++i) freq[i] = r->freq[i];
+    if (magnitude) *magnitude = r->magnitude;
+    return EKV_OK;
+}

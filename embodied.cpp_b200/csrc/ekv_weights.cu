@@ -1,0 +1,273 @@
+// ekv_weights.cu -- the attention weight that each cached key got from a call's query rows:
+//   w[b][h][k] = decay * w[b][h][k] + sum over rows r of KV head h of exp(s_rk - lse_r)
+// with the scores s and the lse of ekv_tree_attention. Every key's sum is one CTA's, in a fixed order: no
+// atomics, the same result every time. K is read once, V not at all.
+#include <algorithm>
+
+#include "ekv_decode.cuh"
+
+namespace ekv {
+namespace {
+
+using namespace decode;
+using namespace sm100;
+
+constexpr int kWarps = 4;  // 16 keys of a 64-key tile each
+constexpr int kThreads = kWarps * 32 + 32;
+
+template <int D, bool Q8>
+struct WCfg {
+    using T = TileCfg<D, Q8>;
+    static constexpr int STAGE = (T::KV_BYTES + 1023) / 1024 * 1024;
+    static constexpr int NST_64K = 65536 / STAGE;
+    static constexpr int NST = NST_64K < 3 ? 3 : NST_64K > 8 ? 8 : NST_64K;
+    static constexpr int QROW = 2 * D + 16;                  // bytes of a query row in shared memory
+    static constexpr int QROWS = D > 128 ? 128 : 256;        // query rows held at a time
+    static constexpr int smem(int rows) { return NST * STAGE + rows * (QROW + 4) + 1024 + 1024; }
+};
+
+template <int NST>
+struct WShared {
+    uint64_t full[NST], empty[NST];
+    RangeScratch range;
+    int abort;
+};
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs a, int q_rows) {
+    using C = WCfg<D, Q8>;
+    using T = TileCfg<D, Q8>;
+    constexpr int NST = C::NST, KS = D / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    using Sh = WShared<NST>;
+    static_assert(sizeof(Sh) <= 1024, "barrier block");
+    Sh &sh = *(Sh *)(smem + NST * C::STAGE);
+    uint8_t *sq = smem + NST * C::STAGE + 1024;           // [q_rows] rows of C::QROW bytes
+    float *slse = (float *)(sq + q_rows * C::QROW);       // [q_rows] lse in the log2 domain
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hk = a.pool.kv_heads, rows_all = a.n_draft * a.group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(smem_addr(&sh.full[i]), 1);
+            mbar_init(smem_addr(&sh.empty[i]), kWarps);
+        }
+        sh.abort = 0;
+        mbar_init_fence();
+    }
+    auto request = [&](int b, bool report) {
+        Req r = load_req(a, b, report);
+        if (r.n_prefix > a.weight_stride) {  // no room for its weights
+            if (report) report_error(a.pool.status, DEV_ERR_BAD_POS, b, r.n_prefix, 6);
+            r.n_prefix = (int)a.weight_stride;
+        }
+        return r;
+    };
+    const Range rg = find_range<kThreads>(a.n_batch, hk, sh.range, [&](int b) {
+        return (request(b, false).n_prefix + kTile - 1) / kTile;
+    });
+
+    int it = 0;
+    bool ok = true;
+    int b = rg.b;
+    long long base = rg.base;
+    for (long long x = rg.lo; x < rg.hi && b < a.n_batch;) {
+        const Req rq = request(b, warp == 0);
+        const int n_tiles = (rq.n_prefix + kTile - 1) / kTile;
+        const long long span = (long long)n_tiles * hk;
+        if (x >= base + span) {
+            base += span;
+            ++b;
+            continue;
+        }
+        const int g = (int)((x - base) / n_tiles);
+        const int t0 = (int)((x - base) - (long long)g * n_tiles);
+        const int t1 = (int)min((long long)n_tiles, t0 + (rg.hi - x));
+
+        for (int c0 = 0; c0 < rows_all; c0 += q_rows) {
+            const int rows = min(q_rows, (rows_all - c0 + 15) / 16 * 16);
+            if (warp == kWarps) {
+                // ---- feeder ----
+                Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
+                for (int j = t0; j < t1; ++j, ++it) {
+                    const int st = it % NST;
+                    const Piece pc = next;
+                    if (j + 1 < t1) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
+                    if (it >= NST) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), ((it / NST) - 1) & 1, abort, kWait);
+                    if (!ok) {
+                        *abort = 1;
+                        continue;
+                    }
+                    issue_piece<D, Q8, false>(a, pc, smem_addr(smem + st * C::STAGE), 0, smem_addr(&sh.full[st]), 0, lane);
+                }
+                continue;
+            }
+            // ---- query rows c0 .. c0 + rows to shared memory, in the products' column order ----
+            asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");  // the last rows are done with
+            for (int i = threadIdx.x; i < rows * (D / 8); i += kWarps * 32) {
+                const int r = i / (D / 8), u = i - r * (D / 8);
+                const int row = c0 + r, t = row / a.group;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < rows_all && t < rq.n_nodes)
+                    v = __ldg((const uint4 *)(a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row -
+                                                     t * a.group) * D) + u);
+                uint8_t *dst = sq + r * C::QROW;
+                if (Q8) {
+                    // columns 32 g + 8 c + 4 i + 2 h + {0, 1} go to place 32 g + 16 i + 2 c + 8 h
+                    const int g32 = u >> 2, cc = u & 3;
+                    uint32_t *d32 = (uint32_t *)(dst + 64 * g32);
+                    d32[cc] = v.x;
+                    d32[cc + 4] = v.y;
+                    d32[cc + 8] = v.z;
+                    d32[cc + 12] = v.w;
+                } else {
+                    *(uint4 *)(dst + 16 * u) = v;
+                }
+            }
+            for (int r = threadIdx.x; r < rows; r += kWarps * 32) {
+                const int row = c0 + r, t = row / a.group;
+                float l = INFINITY;  // no such row, or one that saw nothing: weight 0
+                if (row < rows_all && t < rq.n_nodes) {
+                    l = a.lse[((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group] * 1.4426950408889634f;
+                    if (l == -INFINITY) l = INFINITY;
+                }
+                slse[r] = l;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+
+            const int rq0 = lane >> 2, c = lane & 3;
+            const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
+            const int key_l = 16 * warp + 8 * ((rq0 >> 1) & 1) + 2 * c + (rq0 & 1);  // the key this lane writes (rq0 < 4)
+            float *wrow = a.weights + ((long long)b * hk + g) * a.weight_stride;
+            for (int j = t0; j < t1; ++j, ++it) {
+                const int st = it % NST, par = (it / NST) & 1;
+                const uint32_t sk = smem_addr(smem + st * C::STAGE);
+                const int key = j * kTile + key_l;
+                const bool writes = rq0 < 4 && key < rq.n_prefix;
+                float old = 0.0f;
+                if (writes && (c0 > 0 || a.decay != 0.0f)) old = wrow[key] * (c0 > 0 ? 1.0f : a.decay);
+                ok = ok && mbar_wait(smem_addr(&sh.full[st]), par, abort, kWait);
+                if (!ok) {
+                    *abort = 1;
+                    continue;
+                }
+                const int key0 = 16 * warp;
+                uint32_t kf[KS][4];
+                if constexpr (!Q8) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) load_k_step<D>(sk, key0, ks, lane, kf[ks]);
+                } else {
+#pragma unroll
+                    for (int gr = 0; gr < KS / 2; ++gr)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const uint2 w = lds64(sk + q8_qs_off(key0 + 8 * n + rq0, 32 * gr + 8 * c, D));
+                            int8x4_to_bf16(w.x, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
+                            int8x4_to_bf16(w.y, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
+                        }
+                }
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys (n, e): 8 n + 2 c + e, rows of this lane
+                for (int r0 = 0; r0 < rows; r0 += 16) {
+                    float s[2][4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+                    const uint32_t qa = smem_addr(sq) + (r0 + (lane & 15)) * C::QROW + (lane >> 4) * 16;
+                    if constexpr (!Q8) {
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) {
+                            uint32_t qf[4];
+                            ldmatrix_x4(qf, qa + 32 * ks);
+                            mma_bf16(s[0], qf, kf[ks][0], kf[ks][1]);
+                            mma_bf16(s[1], qf, kf[ks][2], kf[ks][3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int gr = 0; gr < KS / 2; ++gr) {
+                            uint32_t q0[4], q1[4];
+                            ldmatrix_x4(q0, qa + 64 * gr);
+                            ldmatrix_x4(q1, qa + 64 * gr + 32);
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_bf16(p, q0, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
+                                mma_bf16(p, q1, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
+                                const int krow = key0 + 8 * n + 2 * c;
+                                const float s0 = lds_f16(sk + T::SCALES + (krow * T::G32 + gr) * 2);
+                                const float s1 = lds_f16(sk + T::SCALES + ((krow + 1) * T::G32 + gr) * 2);
+                                s[n][0] = fmaf(p[0], s0, s[n][0]);
+                                s[n][1] = fmaf(p[1], s1, s[n][1]);
+                                s[n][2] = fmaf(p[2], s0, s[n][2]);
+                                s[n][3] = fmaf(p[3], s1, s[n][3]);
+                            }
+                        }
+                    }
+                    const float l0 = slse[r0 + rq0], l1 = slse[r0 + rq0 + 8];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            acc[2 * n + e] += ex2(score(s[n][e]) - l0) + ex2(score(s[n][2 + e]) - l1);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.empty[st]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int m = 4; m < 32; m <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], m);
+                const float mine = rq0 & 2 ? (rq0 & 1 ? acc[3] : acc[2]) : (rq0 & 1 ? acc[1] : acc[0]);
+                if (writes) wrow[key] = old + mine;
+            }
+        }
+        x += t1 - t0;
+    }
+    if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 8);
+    if (warp == kWarps && !ok && lane == 0) {
+        for (int st = 0; st < NST; ++st) {  // leave no copy writing this CTA's shared memory
+            mbar_wait_drain(smem_addr(&sh.full[st]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full[st]), 1, kWait / 64);
+        }
+    }
+}
+
+template <int D, bool Q8>
+int launch(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
+    using C = WCfg<D, Q8>;
+    const int64_t rows = (int64_t)a.n_draft * a.group;
+    const int q_rows = (int)std::min<int64_t>((rows + 15) / 16 * 16, C::QROWS);
+    const int smem = C::smem(q_rows);
+    auto k = key_weights_kernel<D, Q8>;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(C::QROWS)) != cudaSuccess)
+        return EKV_ERR_CUDA;
+    const int64_t tiles = (int64_t)a.n_batch * a.pool.kv_heads * ((max_len + kTile - 1) / kTile);
+    const int ctas = std::max(1, std::min(3, 226 * 1024 / (smem + 1024)));
+    const int grid = (int)std::min<int64_t>((int64_t)sms * ctas, std::max<int64_t>(1, tiles));
+    k<<<grid, kThreads, smem, s>>>(a, q_rows);
+    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
+    note_launches(1);
+    return EKV_OK;
+}
+
+template <int D>
+int launch_dim(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
+    if (a.pool.dtype != EKV_DTYPE_Q8_0) return launch<D, false>(a, max_len, sms, s);
+    if constexpr (D % 32 == 0) return launch<D, true>(a, max_len, sms, s);
+    return EKV_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+int launch_key_weights(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
+    switch (a.pool.head_dim) {
+        case 48: return launch_dim<48>(a, max_len, sms, s);
+        case 64: return launch_dim<64>(a, max_len, sms, s);
+        case 128: return launch_dim<128>(a, max_len, sms, s);
+        case 256: return launch_dim<256>(a, max_len, sms, s);
+        default: return EKV_ERR_UNSUPPORTED;
+    }
+}
+
+}  // namespace ekv

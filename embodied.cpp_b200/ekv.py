@@ -81,6 +81,31 @@ class SchedBatch(C.Structure):
                 ("blocks_reused", C.c_int64), ("queued", C.c_int32)]
 
 
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+MAX_DRAFT = 64
+MAX_EVICT_TOKENS = 1 << 19
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("device", C.c_int32), ("layout", C.c_int32), ("rotary_dims", C.c_int32), ("n_ctx_orig", C.c_int32),
+                ("freq_base", C.c_float), ("freq_scale", C.c_float), ("ext_factor", C.c_float),
+                ("attn_factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("freq_factors", C.POINTER(C.c_float))]
+
+
+class TreeParams(C.Structure):
+    _fields_ = [("layer", C.c_int32), ("n_batch", C.c_int32), ("n_draft", C.c_int32), ("q_heads", C.c_int32),
+                ("scale", C.c_float), ("softcap", C.c_float), ("out_dtype", C.c_int32), ("reserved", C.c_int32),
+                ("seq_ids", C.c_void_p), ("prefix_len", C.c_void_p), ("n_nodes", C.c_void_p), ("ancestors", C.c_void_p)]
+
+
+class EvictParams(C.Structure):
+    _fields_ = [("layer0", C.c_int32), ("n_layers", C.c_int32), ("n_batch", C.c_int32), ("keep", C.c_int32),
+                ("first", C.c_int32), ("recent", C.c_int32), ("seq_ids", C.c_void_p), ("seen", C.c_void_p),
+                ("weights", C.c_void_p), ("positions", C.c_void_p), ("weight_stride", C.c_int64), ("kept", C.c_void_p),
+                ("weights_out", C.c_void_p), ("positions_out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
 class Tensor(C.Structure):
     """ekv_tensor: a ggml-ordered strided device tensor (ne[0] fastest, nb in bytes)."""
     _fields_ = [("data", C.c_void_p), ("type", C.c_int32), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
@@ -98,6 +123,8 @@ EXPORTED = [
     "ekv_mul_mat_soft_max_mul_mat_workspace_size", "ekv_mul_mat_soft_max_mul_mat_ws", "ekv_append_suffix_attention", "ekv_launch_count", "ekv_debug_expire_wait",
     "ekv_flow_step_f32", "ekv_guidance_f32", "ekv_sched_create", "ekv_sched_destroy", "ekv_sched_submit",
     "ekv_sched_begin_tick", "ekv_sched_end_tick", "ekv_sched_stats", "ekv_project_qkv_rope",
+    "ekv_rope_create", "ekv_rope_destroy", "ekv_rope_get", "ekv_rope_append", "ekv_tree_attention_workspace_size",
+    "ekv_tree_attention", "ekv_key_weights", "ekv_evict_by_weight",
 ]
 NOALLOC_SCRATCH_BYTES = 16 << 20  # EKV_NOALLOC_SCRATCH_BYTES
 
@@ -155,6 +182,15 @@ def _load():
                                                                                          C.c_size_t, vp], C.c_int),
         "ekv_project_qkv_rope": ([vp, i32, i32, vp, i32, i32, i32, vp, vp, vp, vp, vp, C.c_float, vp, vp, vp, vp],
                                  C.c_int),
+        "ekv_rope_create": ([C.POINTER(RopeConfig), C.POINTER(vp)], C.c_int),
+        "ekv_rope_destroy": ([vp], C.c_int),
+        "ekv_rope_get": ([vp, C.POINTER(C.c_double), i32, C.POINTER(C.c_float)], C.c_int),
+        "ekv_rope_append": ([vp, vp, i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, C.c_int64, vp, vp, vp, C.c_int64, vp],
+                            C.c_int),
+        "ekv_tree_attention_workspace_size": ([vp, C.POINTER(TreeParams)], C.c_size_t),
+        "ekv_tree_attention": ([vp, C.POINTER(TreeParams), vp, vp, vp, vp, vp, vp, C.c_size_t, vp], C.c_int),
+        "ekv_key_weights": ([vp, C.POINTER(TreeParams), vp, vp, vp, C.c_int64, C.c_float, vp], C.c_int),
+        "ekv_evict_by_weight": ([vp, C.POINTER(EvictParams), vp], C.c_int),
         "ekv_version": ([], C.c_char_p),
         "ekv_launch_count": ([], C.c_uint64),
         "ekv_strerror": ([C.c_int], C.c_char_p),
@@ -323,6 +359,103 @@ class Pool:
         check(lib.ekv_append_suffix_attention(self.h, C.byref(params), _ptr(k_suffix), _ptr(v_suffix), _ptr(q),
                                               _ptr(out), _ptr(workspace), ws_bytes, _stream(stream)),
               "ekv_append_suffix_attention")
+
+
+    # ---- token-by-token decoding ----
+    def rope_append(self, rope, layer, seq_ids, dst_pos, n_rows, src_row, max_rows, positions, *, q=None, q_out=None,
+                    k=None, v=None, stream=None):
+        """ekv_rope_append: turn q [rows, q_heads, head_dim] into q_out and k into the pages beside v ([rows, kv_heads,
+        head_dim]), all bf16 and by source row. q, k and v may be slices of one [rows, columns] projection output:
+        rows may be any distance apart, a row's heads are adjacent. Either pair may be left out."""
+        q_heads, q_stride = self._rows(q, self.cfg.head_dim, "q")
+        kv_heads, kv_stride = self._rows(k, self.cfg.head_dim, "k")
+        v_heads, v_stride = self._rows(v, self.cfg.head_dim, "v")
+        if (kv_heads, kv_stride) != (v_heads, v_stride) or (k is not None and kv_heads != self.cfg.kv_heads):
+            raise ValueError("k and v must have the pool's KV heads and the same distance from row to row")
+        if q is not None and (q_out is None or not q_out.is_contiguous() or q_out.shape != q.shape):
+            raise ValueError("q_out must be contiguous and of q's shape")
+        check(lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), _ptr(seq_ids), _ptr(dst_pos), _ptr(n_rows),
+                                  _ptr(src_row), max_rows, _ptr(positions), q_heads, _ptr(q), q_stride, _ptr(q_out),
+                                  _ptr(k), _ptr(v), kv_stride, _stream(stream)), "ekv_rope_append")
+
+    @staticmethod
+    def _rows(t, head_dim, name):
+        """Heads of a [rows, heads, head_dim] tensor and the elements from row to row; a row must be adjacent."""
+        if t is None:
+            return 0, 0
+        if t.dim() != 3 or t.shape[2] != head_dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != head_dim):
+            raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
+        return t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * head_dim
+
+    def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
+                    prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
+        p = TreeParams(layer, seq_ids.numel(), n_draft, q_heads, scale, softcap, out_dtype, 0, seq_ids.data_ptr(),
+                       None if prefix_len is None else prefix_len.data_ptr(),
+                       None if n_nodes is None else n_nodes.data_ptr(),
+                       None if ancestors is None else ancestors.data_ptr())
+        p._keep = (seq_ids, prefix_len, n_nodes, ancestors)
+        return p
+
+    def tree_attention_workspace_size(self, params: TreeParams) -> int:
+        return lib.ekv_tree_attention_workspace_size(self.h, C.byref(params))
+
+    def tree_attention(self, params: TreeParams, q, k_draft, v_draft, out, lse=None, workspace=None, stream=None):
+        """ekv_tree_attention: q [n_batch, n_draft, q_heads, head_dim], k_draft / v_draft [n_batch, n_draft, kv_heads,
+        head_dim] bf16 over the cached prefix; out like q (bf16 or f32), lse f32 [n_batch, n_draft, q_heads]."""
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        check(lib.ekv_tree_attention(self.h, C.byref(params), _ptr(q), _ptr(k_draft), _ptr(v_draft), _ptr(out), _ptr(lse),
+                                     _ptr(workspace), ws_bytes, _stream(stream)), "ekv_tree_attention")
+
+    def key_weights(self, params: TreeParams, q, lse, weights, decay=1.0, stream=None):
+        """ekv_key_weights: weights [n_batch, kv_heads, stride] f32 = decay * weights + what the rows give each key."""
+        check(lib.ekv_key_weights(self.h, C.byref(params), _ptr(q), _ptr(lse), _ptr(weights), weights.shape[-1], decay,
+                                  _stream(stream)), "ekv_key_weights")
+
+    def evict_by_weight(self, layer0, n_layers, seq_ids, weights, *, keep, first, recent, kept, weights_out=None,
+                        positions=None, positions_out=None, seen=None, stream=None):
+        """ekv_evict_by_weight: weights (and positions) [n_layers, n_batch, kv_heads, stride], kept int32 [n_layers,
+        n_batch, kv_heads, keep]; weights_out and positions_out have one stride of their own, or are the inputs."""
+        outs = [t for t in (weights_out, positions_out) if t is not None]
+        p = EvictParams(layer0, n_layers, seq_ids.numel(), keep, first, recent, seq_ids.data_ptr(),
+                        None if seen is None else seen.data_ptr(), weights.data_ptr(),
+                        None if positions is None else positions.data_ptr(), weights.shape[-1], kept.data_ptr(),
+                        None if weights_out is None else weights_out.data_ptr(),
+                        None if positions_out is None else positions_out.data_ptr(), outs[0].shape[-1] if outs else 0)
+        check(lib.ekv_evict_by_weight(self.h, C.byref(p), _stream(stream)), "ekv_evict_by_weight")
+
+
+class Rope:
+    """Rotary frequencies (ekv_rope_create): layout, rotated columns and long-context scaling, as ggml_rope_ext."""
+
+    def __init__(self, *, device=0, interleaved=False, rotary_dims, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0,
+                 attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0, freq_factors=None):
+        ff = None
+        if freq_factors is not None:
+            if len(freq_factors) != rotary_dims // 2:
+                raise ValueError("freq_factors: one for each pair")
+            ff = (C.c_float * len(freq_factors))(*freq_factors)
+        cfg = RopeConfig(device, ROPE_INTERLEAVED if interleaved else ROPE_HALF, rotary_dims, n_ctx_orig, freq_base,
+                         freq_scale, ext_factor, attn_factor, beta_fast, beta_slow, ff)
+        self.rotary_dims = rotary_dims
+        self.h = C.c_void_p()
+        check(lib.ekv_rope_create(C.byref(cfg), C.byref(self.h)), "ekv_rope_create")
+
+    def frequencies(self):
+        """Radians per position of each pair, and the factor of the rotation."""
+        f, m = (C.c_double * (self.rotary_dims // 2))(), C.c_float()
+        check(lib.ekv_rope_get(self.h, f, self.rotary_dims // 2, C.byref(m)), "ekv_rope_get")
+        return list(f), m.value
+
+    def close(self):
+        if self.h:
+            check(lib.ekv_rope_destroy(self.h), "ekv_rope_destroy")
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def project_qkv_rope(pool: "Pool", layer, seq_ids, x, wq, wk, wv, positions, rope_base, q_out, k_out=None, v_out=None,

@@ -299,6 +299,112 @@ int ekv_project_qkv_rope(ekv_pool *pool, int32_t layer, int32_t n_batch, const i
                          const int32_t *positions, float rope_base, void *q_out, void *k_out, void *v_out,
                          ekv_stream_t stream);
 
+/* ---- token-by-token decoding over the pool ----
+ * What an autoregressive head or a language backbone needs beside the denoise loop: rotary positions on the
+ * way into the pages, attention of one token or a tree of drafted tokens, the weight that every cached key
+ * got, and eviction by it. No counterpart in the reference, whose models decode through llama.cpp; the rotary
+ * parameters are those of ggml_rope_ext, which its graphs call (models/pi05.cpp:308-315). */
+#define EKV_ROPE_HALF 0        /* pairs (i, i + rotary_dims / 2): ggml's NEOX mode */
+#define EKV_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1): ggml's normal mode          */
+typedef struct ekv_rope_config {
+    int32_t device;        /* CUDA device ordinal; -1: frequencies only (ekv_rope_get)             */
+    int32_t layout;        /* EKV_ROPE_HALF or EKV_ROPE_INTERLEAVED                                  */
+    int32_t rotary_dims;   /* leading columns of a head that turn (even, 2 .. 256); the rest pass      */
+    int32_t n_ctx_orig;    /* trained length (ext_factor != 0)                                        */
+    float freq_base;       /* pair i turns by base^(-2 i / rotary_dims) radians per position           */
+    float freq_scale;      /* 1 / context scaling factor: slow pairs' frequencies are multiplied by it */
+    float ext_factor;      /* 0: every pair is scaled (linear scaling). Above: pairs that turn more than
+                              beta_fast times over n_ctx_orig keep their frequency (this share of it), those
+                              that turn less than beta_slow times are scaled, with a ramp between          */
+    float attn_factor;     /* the rotation is multiplied by it, and by 1 + 0.1 ln(1 / freq_scale) where
+                              ext_factor != 0                                                         */
+    float beta_fast, beta_slow;
+    const float *freq_factors; /* host [rotary_dims / 2] divisors of the frequencies, or NULL           */
+} ekv_rope_config;
+typedef struct ekv_rope ekv_rope;
+int ekv_rope_create(const ekv_rope_config *cfg, ekv_rope **out);
+/* No call that uses the handle may still be running on the device. */
+int ekv_rope_destroy(ekv_rope *rope);
+/* Radians per position of the first `cap` pairs, and the factor of the rotation (either may be NULL / 0). */
+int ekv_rope_get(const ekv_rope *rope, double *freq, int32_t cap, float *magnitude);
+/* Turn q and k by their positions and append k and v to the paged prefix, in one pass. Rows as in ekv_append:
+ * for request i, n_rows[i] rows (at most max_rows) from row src_row[i] of q / k / v go to positions dst_pos[i]
+ * onwards of sequence seq_ids[i]; row r turns by positions[r] (device int32, by source row). q, k and v are bf16
+ * rows of q_heads (kv_heads) x head_dim with q_stride (kv_stride) elements from row to row (multiples of 8; 0:
+ * rows are adjacent), so that they may be parts of one projection's output. q_out is [rows][q_heads][head_dim]
+ * by source row; it may be q itself where q's rows are adjacent. q and q_out may be NULL (append only), or k and
+ * v (then seq_ids and dst_pos may be NULL too). Turned values are rounded to bf16; the pages get what ekv_append
+ * of those rows would write, Q8_0 blocks included. Pointers 16-byte aligned; at most 65535 requests. */
+int ekv_rope_append(ekv_pool *pool, const ekv_rope *rope, int32_t layer, int32_t n_batch, const int32_t *seq_ids,
+                    const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int32_t max_rows,
+                    const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
+                    const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream);
+
+#define EKV_MAX_DRAFT 64
+typedef struct ekv_tree_params {
+    int32_t layer;
+    int32_t n_batch;
+    int32_t n_draft;        /* drafted tokens per request (1 .. EKV_MAX_DRAFT); 1 = plain decoding     */
+    int32_t q_heads;        /* a multiple of the pool's kv_heads                                      */
+    float scale;
+    float softcap;          /* > 0: scores are softcap * tanh(scale * q.k / softcap); 0: scale * q.k    */
+    int32_t out_dtype;      /* EKV_DTYPE_BF16 or EKV_DTYPE_F32                                        */
+    int32_t reserved;
+    /* device arrays; NULL selects the default                                                        */
+    const int32_t *seq_ids;     /* [n_batch], required                                                */
+    const int32_t *prefix_len;  /* [n_batch] cached keys used; default: the sequence length            */
+    const int32_t *n_nodes;     /* [n_batch] drafted tokens in use; default: n_draft                    */
+    const uint64_t *ancestors;  /* [n_batch][n_draft]: bit j of word t lets token t see drafted token j (its
+                                   own bit included); bits at or above n_nodes do not count. Default: a chain,
+                                   token t sees 0 .. t                                                */
+} ekv_tree_params;
+
+/* Bytes of workspace with which ekv_tree_attention cuts long caches into parts for all SMs. */
+size_t ekv_tree_attention_workspace_size(const ekv_pool *pool, const ekv_tree_params *p);
+/* Attention of drafted tokens over the cached prefix and over each other. q is bf16 [n_batch][n_draft][q_heads]
+ * [head_dim]; k_draft and v_draft, the drafted tokens' own rows, are bf16 [n_batch][n_draft][kv_heads][head_dim]
+ * and are not appended (append the accepted path with ekv_append or ekv_rope_append). out is [n_batch][n_draft]
+ * [q_heads][head_dim]; lse, f32 [n_batch][n_draft][q_heads] or NULL, gets the natural logarithm of the sum of
+ * exp(score) over the visible keys. Rows that see no key, and tokens at or above n_nodes, get 0 and -inf. What a
+ * row may not see does not reach it, whatever it holds. head_dim 48 (bf16 pools), 64, 128 or 256. Without a
+ * workspace (or with a smaller one) each KV head of a request is one CTA's work. Pointers 16-byte aligned. */
+int ekv_tree_attention(ekv_pool *pool, const ekv_tree_params *p, const void *q, const void *k_draft,
+                       const void *v_draft, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                       ekv_stream_t stream);
+/* The weight that the call's rows give to each cached key: for k below the prefix length
+ *   weights[b][h][k] = decay * weights[b][h][k] + sum over t < n_nodes, query heads of KV head h, of
+ *                      exp(score - lse[b][t][head])
+ * (weights f32 [n_batch][kv_heads][weight_stride]; later entries are left alone, and decay 0 does not read the
+ * old ones). q and lse as ekv_tree_attention got and gave them; out_dtype and ancestors do not count. Rows with
+ * lse -inf add nothing. The same inputs give the same bits. */
+int ekv_key_weights(ekv_pool *pool, const ekv_tree_params *p, const void *q, const float *lse, float *weights,
+                    int64_t weight_stride, float decay, ekv_stream_t stream);
+
+#define EKV_MAX_EVICT_TOKENS (1 << 19) /* longest sequence ekv_evict_by_weight takes */
+typedef struct ekv_evict_params {
+    int32_t layer0, n_layers;   /* the layers [layer0, layer0 + n_layers)                              */
+    int32_t n_batch;
+    int32_t keep;               /* rows each (layer, request, KV head) keeps                           */
+    int32_t first, recent;      /* positions below first, and the last `recent` of those seen, stay;
+                                   first + recent <= keep                                             */
+    const int32_t *seq_ids;     /* device [n_batch], distinct                                         */
+    const int32_t *seen;        /* device [n_batch] tokens seen so far; NULL: the sequence length        */
+    const float *weights;       /* device [n_layers][n_batch][kv_heads][weight_stride], by slot          */
+    const int32_t *positions;   /* the token position in each slot, same layout; NULL: the slot          */
+    int64_t weight_stride;      /* at least the longest sequence                                       */
+    int32_t *kept;              /* out [n_layers][n_batch][kv_heads][keep]: the slot each row came from   */
+    float *weights_out;         /* out [n_layers][n_batch][kv_heads][out_stride], or NULL; may be weights */
+    int32_t *positions_out;     /* out, same layout, or NULL; may be positions                          */
+    int64_t out_stride;         /* at least keep                                                      */
+} ekv_evict_params;
+/* Cut sequences longer than `keep` down to it, per layer and KV head: besides the first and the most recent
+ * tokens the rows of largest weight stay (ties: the lower slot; NaN goes first). Rows that stay below slot
+ * `keep` stay in place; the i-th free slot takes the i-th row that stays from above, K and V. kept, weights_out
+ * and positions_out describe slots 0 .. keep - 1 afterwards (-1, 0, -1 at or past a shorter sequence's end).
+ * Lengths do not change here: once every layer is done call ekv_seq_resize(pool, seq, keep), which frees the
+ * blocks. Order among slots is not kept, which attention over turned keys does not see. */
+int ekv_evict_by_weight(ekv_pool *pool, const ekv_evict_params *p, ekv_stream_t stream);
+
 /* ---- ggml op surface: GGML_OP_FLASH_ATTN_EXT on strided device tensors ----
  * Replaces ggml_flash_attn_ext (models/hy_vla.cpp:376-378, :439-441, :460, :492, :859 (GQA, mask);
  * models/lingbot_va.cpp:1263-1266) for a ggml backend that routes the op here: the tensors keep

@@ -1,0 +1,145 @@
+"""Argument checks of the token-by-token decoding entry points and the rotary frequencies; no kernel is launched (the pool
+is host-only, so a call that passes the checks ends with EKV_ERR_UNSUPPORTED)."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import decode_cases as dc
+import ekv
+
+P = 0x10000  # a pointer that is never followed
+L = ekv.lib
+
+
+def pool(**kw):
+    cfg = dict(device=-1, dtype=ekv.DTYPE_BF16, block_tokens=16, n_blocks=40, kv_heads=2, head_dim=64, n_layers=2, max_seqs=6,
+               max_blocks_per_seq=12)
+    cfg.update(kw)
+    return ekv.Pool(**cfg)
+
+
+def tree_params(**kw):
+    p = ekv.TreeParams(0, 3, 4, 8, 0.125, 0.0, ekv.DTYPE_BF16, 0, P, None, None, P)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def tree(p, prm, q=P, k=P, v=P, out=P, lse=P, ws=P):
+    return L.ekv_tree_attention(p.h, C.byref(prm), q, k, v, out, lse, ws, 1 << 20, None)
+
+
+def test_tree_attention_refusals():
+    p = pool()
+    assert tree(p, tree_params()) == ekv.ERR_UNSUPPORTED  # no device
+    for kw in (dict(layer=2), dict(layer=-1), dict(n_batch=0), dict(n_draft=0), dict(q_heads=0), dict(q_heads=7), dict(scale=0.0),
+               dict(scale=math.nan), dict(scale=math.inf), dict(softcap=-1.0), dict(softcap=math.nan), dict(seq_ids=None),
+               dict(ancestors=P + 4)):
+        assert tree(p, tree_params(**kw)) == ekv.ERR_INVALID_ARG, kw
+    assert tree(p, tree_params(n_draft=65)) == ekv.ERR_RANGE
+    assert tree(p, tree_params(out_dtype=ekv.DTYPE_F16)) == ekv.ERR_UNSUPPORTED
+    for kw in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=P + 8), dict(k=P + 2), dict(v=P + 2), dict(out=P + 8),
+               dict(ws=P + 8), dict(lse=P + 2)):
+        assert tree(p, tree_params(), **kw) == ekv.ERR_INVALID_ARG, kw
+    assert tree(pool(head_dim=80), tree_params()) == ekv.ERR_UNSUPPORTED
+    assert L.ekv_tree_attention(None, C.byref(tree_params()), P, P, P, P, None, None, 0, None) == ekv.ERR_INVALID_ARG
+    assert L.ekv_tree_attention(p.h, None, P, P, P, P, None, None, 0, None) == ekv.ERR_INVALID_ARG
+
+
+def test_tree_workspace_size():
+    p = pool()
+    assert L.ekv_tree_attention_workspace_size(p.h, C.byref(tree_params())) > 0
+    for kw in (dict(n_draft=65), dict(n_draft=0), dict(q_heads=7), dict(n_batch=0)):
+        assert L.ekv_tree_attention_workspace_size(p.h, C.byref(tree_params(**kw))) == 0
+    assert L.ekv_tree_attention_workspace_size(None, C.byref(tree_params())) == 0
+
+
+def test_key_weights_refusals():
+    p = pool()
+
+    def call(prm=None, q=P, lse=P, w=P, stride=100, decay=1.0):
+        return L.ekv_key_weights(p.h, C.byref(prm or tree_params()), q, lse, w, stride, decay, None)
+
+    assert call() == ekv.ERR_UNSUPPORTED
+    for kw in (dict(q=None), dict(lse=None), dict(w=None), dict(stride=-1), dict(decay=math.nan), dict(w=P + 2), dict(lse=P + 1),
+               dict(prm=tree_params(layer=5))):
+        assert call(**kw) == ekv.ERR_INVALID_ARG, kw
+    assert call(prm=tree_params(n_draft=65)) == ekv.ERR_RANGE
+
+
+def test_evict_refusals():
+    p = pool()
+
+    def call(**kw):
+        e = ekv.EvictParams(0, 2, 3, 32, 4, 8, P, None, P, None, 100, P, None, None, 0)
+        for k, v in kw.items():
+            setattr(e, k, v)
+        return L.ekv_evict_by_weight(p.h, C.byref(e), None)
+
+    assert call() == ekv.ERR_UNSUPPORTED
+    for kw in (dict(layer0=-1), dict(layer0=1), dict(n_layers=0), dict(n_layers=3), dict(n_batch=0), dict(keep=0), dict(first=-1),
+               dict(recent=-1), dict(first=16, recent=17), dict(first=2 ** 31 - 1, recent=2 ** 31 - 1), dict(weight_stride=-1),
+               dict(seq_ids=None), dict(weights=None), dict(kept=None), dict(weights_out=P, out_stride=32),
+               dict(positions=P, positions_out=P, out_stride=64), dict(weights_out=P + 4096, out_stride=31), dict(kept=P + 2)):
+        assert call(**kw) == ekv.ERR_INVALID_ARG, kw
+    assert call(weights_out=P, out_stride=100) == ekv.ERR_UNSUPPORTED
+    big = pool(n_blocks=3000, block_tokens=256, max_blocks_per_seq=3000)
+    s = big.seq_create()
+    big.seq_resize(s, ekv.MAX_EVICT_TOKENS + 1)
+    e = ekv.EvictParams(0, 1, 1, 32, 4, 8, P, None, P, None, 1 << 20, P, None, None, 0)
+    assert L.ekv_evict_by_weight(big.h, C.byref(e), None) == ekv.ERR_RANGE
+
+
+def test_rope_append_refusals():
+    p, rope = pool(), ekv.Rope(device=-1, rotary_dims=64)
+
+    def call(pl=None, r=None, layer=0, n=3, seq=P, dst=P, rows=P, src=P, most=5, pos=P, hq=4, q=P, qs=0, qo=P, k=P, v=P, kvs=0):
+        return L.ekv_rope_append((pl or p).h, r or rope.h, layer, n, seq, dst, rows, src, most, pos, hq, q, qs, qo, k, v, kvs, None)
+
+    assert call() == ekv.ERR_UNSUPPORTED
+    assert call(n=0) == ekv.OK and call(most=0) == ekv.OK
+    for kw in (dict(layer=2), dict(n=-1), dict(n=65536), dict(most=-1), dict(seq=None), dict(dst=None), dict(rows=None), dict(src=None),
+               dict(pos=None), dict(hq=0), dict(q=None), dict(qo=None), dict(k=None), dict(v=None), dict(q=None, qo=None, k=None, v=None),
+               dict(qs=255), dict(qs=260), dict(kvs=127), dict(kvs=132), dict(q=P + 8, qo=P), dict(k=P + 2), dict(qs=512, qo=P)):
+        assert call(**kw) == ekv.ERR_INVALID_ARG, kw
+    assert call(qs=512, qo=P + 4096) == ekv.ERR_UNSUPPORTED
+    assert call(pl=pool(head_dim=48)) == ekv.ERR_INVALID_ARG  # more rotated columns than a head has
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dims=0), dict(rotary_dims=7), dict(rotary_dims=64, freq_base=1.0), dict(rotary_dims=64, freq_scale=0.0),
+                                dict(rotary_dims=64, freq_scale=math.nan), dict(rotary_dims=64, ext_factor=1.0), dict(rotary_dims=64, ext_factor=-1.0),
+                                dict(rotary_dims=64, ext_factor=1.0, n_ctx_orig=4096, beta_slow=0.0), dict(rotary_dims=64, attn_factor=math.inf),
+                                dict(rotary_dims=4, freq_factors=[1.0, 0.0])])
+def test_rope_create_refusals(kw):
+    with pytest.raises(ekv.EkvError) as e:
+        ekv.Rope(device=-1, **kw)
+    assert e.value.code == ekv.ERR_INVALID_ARG
+    with pytest.raises(ekv.EkvError) as e:
+        ekv.Rope(device=-1, rotary_dims=258)
+    assert e.value.code == ekv.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("n", [2, 34, 64, 256])
+@pytest.mark.parametrize("kw", [dict(), dict(freq_scale=0.25), dict(freq_base=1e6, freq_scale=0.125, ext_factor=1.0, n_ctx_orig=4096),
+                                dict(freq_scale=0.5, ext_factor=0.25, n_ctx_orig=100, beta_fast=8.0, beta_slow=2.0)])
+def test_rope_frequencies(n, kw):
+    f, m = ekv.Rope(device=-1, rotary_dims=n, **kw).frequencies()
+    want = dc.rope_table(n, kw.get("freq_base", 10000.0), kw.get("freq_scale", 1.0), kw.get("ext_factor", 0.0), kw.get("beta_fast", 32.0),
+                         kw.get("beta_slow", 1.0), kw.get("n_ctx_orig", 0))
+    np.testing.assert_allclose(f, want, rtol=1e-13)
+    assert abs(m - (1 + 0.1 * math.log(1 / kw["freq_scale"]) if kw.get("ext_factor") else 1.0)) < 1e-6
+
+
+def test_python_checks_of_rope_rows():
+    torch = pytest.importorskip("torch")
+    p, rope = pool(), ekv.Rope(device=-1, rotary_dims=64)
+    x = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    n = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        p.rope_append(rope, 0, n, n, n, n, 3, n, q=x.transpose(0, 1), q_out=x)
+    with pytest.raises(ValueError):
+        p.rope_append(rope, 0, n, n, n, n, 3, n, q=x, q_out=x[:2])
+    with pytest.raises(ValueError):
+        p.rope_append(rope, 0, n, n, n, n, 3, n, k=x, v=x)  # 4 KV heads, the pool has 2
