@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "ekv_device.cuh"
@@ -20,6 +21,47 @@
 
 namespace ekv {
 namespace decode {
+
+// ---- launches ----
+// The decoding calls are short and follow one another, so their kernels start while the one before them in the
+// stream drains (programmatic launch): each waits for it with grid_wait() before it touches global memory.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+int launch_after(void (*k)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    if (cudaLaunchKernelEx(&c, k, P(args)...) != cudaSuccess) {
+        cudaGetLastError();
+        return EKV_ERR_CUDA;
+    }
+    note_launches(1);
+    return EKV_OK;
+}
+
+// Dynamic shared memory above 48 KB, asked for once per kernel and device (`done`: the devices asked on).
+template <class K>
+int allow_smem(K k, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return EKV_ERR_CUDA;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return EKV_OK;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return EKV_ERR_CUDA;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return EKV_OK;
+}
 
 constexpr int kTile = 64;                       // keys per tile
 constexpr long long kWait = kDefaultWaitBudget; // clock cycles a bounded wait gives up after
@@ -39,6 +81,15 @@ __device__ __forceinline__ uint32_t bf16_off(int row, int d) {
     constexpr int W = TileCfg<D, false>::W;
     return tile_elem_off(row, d, D, W);
 }
+
+// The same with run-time head_dim, for kernels of any: 8 W bytes of 2 D / W chunks are 16 D bytes per 8 rows, and
+// W = 2^w, so that no division is left.
+__device__ __forceinline__ uint32_t bf16_off_any(int row, int d, int D, int w) {
+    const int byte = 2 * d;
+    return (uint32_t)((row >> 3) * 16 * D + ((byte >> w) << (w + 3))) +
+           swz((uint32_t)(((row & 7) << w) + (byte & ((1 << w) - 1))), (1u << (w - 4)) - 1);
+}
+__device__ __forceinline__ int log2_of(int pow2) { return 31 - __clz(pow2); }
 
 // ---- matrix instructions ----
 // D[16x8] += A[16x16] * B[16x8], bf16 operands, f32 accumulators.
@@ -68,6 +119,41 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// The G f16 scales of one key's row, two to a word, and one of them.
+template <int G>
+__device__ __forceinline__ void load_scales(uint32_t addr, uint32_t (&s)[(G + 1) / 2]) {
+    static_assert(G % 2 == 0, "whole words");
+    if constexpr (G % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < G / 8; ++i) {
+            const uint4 v = lds128(addr + 16 * i);
+            s[4 * i] = v.x;
+            s[4 * i + 1] = v.y;
+            s[4 * i + 2] = v.z;
+            s[4 * i + 3] = v.w;
+        }
+    } else if constexpr (G % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < G / 4; ++i) {
+            const uint2 v = lds64(addr + 8 * i);
+            s[2 * i] = v.x;
+            s[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) s[i] = lds32(addr + 4 * i);
+    }
+}
+template <int N>
+__device__ __forceinline__ float scale_of(const uint32_t (&s)[N], int g) {
+    const __half2 h = *(const __half2 *)&s[g >> 1];
+    return g & 1 ? __high2float(h) : __low2float(h);
 }
 __device__ __forceinline__ float lds_f16(uint32_t addr) {
     uint16_t v;
@@ -281,6 +367,26 @@ __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, 
     }
 }
 
+// A query row in shared memory: padded by 16 bytes, so that eight rows' 16-byte units fall in eight different
+// bank groups; in the column order of the products (q_col).
+template <int D>
+__host__ __device__ constexpr int q_row_bytes() { return 2 * D + 16; }
+
+// 16 bytes (columns 8 u .. 8 u + 7) of a query row to their places.
+template <bool Q8>
+__device__ __forceinline__ void store_q_unit(uint8_t *row, int u, uint4 v) {
+    if (!Q8) {
+        *(uint4 *)(row + 16 * u) = v;
+        return;
+    }
+    // columns 32 g + 8 c + 4 i + 2 h + {0, 1} go to places 32 g + 16 i + 8 h + 2 c + {0, 1}
+    uint32_t *d = (uint32_t *)(row + 64 * (u >> 2)) + (u & 3);
+    d[0] = v.x;
+    d[4] = v.y;
+    d[8] = v.z;
+    d[12] = v.w;
+}
+
 // ---- scores of one warp's 16 keys ----
 // Column order of the matrix products. bf16 caches: natural. Q8_0 caches: step 2 g + i of group g (32
 // columns) gives lane c of a quad the columns 32 g + 8 c + 4 i + {0, 1 | 2, 3}, so that a lane reads its
@@ -298,11 +404,24 @@ __device__ __forceinline__ void load_k_step(uint32_t tile, int key0, int step, i
     ldmatrix_x4(b, tile + bf16_off<D>(row, 16 * step + ((lane >> 3) & 1) * 8));
 }
 
-// B operands of one 16-key x 16-column step of V^T: b[0..1] columns 0-7 of the step, b[2..3] columns 8-15.
+// A operand of the same step: keys are its rows.
 template <int D>
-__device__ __forceinline__ void load_v_step(uint32_t tile, int key0, int step, int lane, uint32_t (&b)[4]) {
-    const int row = key0 + (lane & 15);
-    ldmatrix_x4_trans(b, tile + bf16_off<D>(row, 16 * step + (lane >> 4) * 8));
+__device__ __forceinline__ void load_k_rows(uint32_t tile, int key0, int step, int lane, uint32_t (&a)[4]) {
+    ldmatrix_x4(a, tile + bf16_off<D>(key0 + (lane & 15), 16 * step + (lane >> 4) * 8));
+}
+
+// A operand V^T: 16 columns of V (step `step`) are its rows, 16 keys its columns.
+template <int D>
+__device__ __forceinline__ void load_v_cols(uint32_t tile, int key0, int step, int lane, uint32_t (&a)[4]) {
+    const int row = key0 + (lane & 7) + ((lane >> 4) << 3);
+    ldmatrix_x4_trans(a, tile + bf16_off<D>(row, 16 * step + ((lane >> 3) & 1) * 8));
+}
+
+// An 8 x 8 matrix of 16-bit elements, transposed across the warp.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 }  // namespace decode

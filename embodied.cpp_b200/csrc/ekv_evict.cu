@@ -10,7 +10,7 @@
 //   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed
 #include <algorithm>
 
-#include "ekv_device.cuh"
+#include "ekv_decode.cuh"
 #include "ekv_internal.h"
 
 namespace ekv {
@@ -28,45 +28,49 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+constexpr int kCopies = 4;   // histograms, by lane: weights share few exponents, so lanes meet in few bins
+constexpr int kInRegs = 16;  // keys a thread keeps (16384 slots); longer rows are read again by each pass
+
 struct SelShared {
-    uint32_t hist[kBins];
+    uint32_t hist[kCopies][kBins];
     uint32_t warp_sum[2][32];
-    uint32_t digit, above;
+    uint32_t digit, above, count;
 };
 
-// Block-wide exclusive scan of one value per thread; the total in `total`.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sum, uint32_t &total) {
+// Block-wide exclusive scan of one value per thread; the total in `total`. One barrier: consecutive scans
+// alternate between two buffers (`turn`).
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, SelShared &sh, int &turn, uint32_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t *sums = sh.warp_sum[turn];
+    turn ^= 1;
     uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += u;
     }
-    if (lane == 31) warp_sum[warp] = s;
+    if (lane == 31) sums[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t w = warp_sum[lane];
+    uint32_t w = sums[lane];
+    const uint32_t mine = __shfl_sync(0xffffffffu, w, warp);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += u;
-        }
-        warp_sum[lane] = w;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += u;
     }
-    __syncthreads();
-    total = warp_sum[31];
-    const uint32_t r = s - v + (warp ? warp_sum[warp - 1] : 0u);
-    __syncthreads();
-    return r;
+    total = __shfl_sync(0xffffffffu, w, 31);
+    return s - v + __shfl_sync(0xffffffffu, w, warp) - mine;
 }
 
 __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t s_mem[];
     __shared__ SelShared sh;
+    int turn = 0;
+    decode::grid_wait();
+    decode::grid_launch_next();
     const int hk = a.pool.kv_heads;
     const int lbh = blockIdx.x, b = (lbh / hk) % a.n_batch;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
     const int seq = a.seq_ids[b];
     int n = 0;
     if (seq < 0 || seq >= a.pool.max_seqs) {
@@ -102,58 +106,88 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     }
 
     // ---- the keep-th largest key, from its upper bits down ----
+    const bool in_regs = n <= kInRegs * kSelThreads;
+    uint32_t keys[kInRegs];
+    if (in_regs) {
+#pragma unroll
+        for (int j = 0; j < kInRegs; ++j) {
+            const int i = tid + j * kSelThreads;
+            keys[j] = i < n ? key_of(i) : 0u;
+        }
+    }
+    // f(slot, key) for this thread's slots tid, tid + 1024, ...
+    auto each = [&](auto f) {
+        if (in_regs) {
+#pragma unroll
+            for (int j = 0; j < kInRegs; ++j) {
+                if (j * kSelThreads >= n) break;
+                f(tid + j * kSelThreads, keys[j]);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = tid; i - tid < n; i += kSelThreads) f(i, i < n ? key_of(i) : 0u);
+        }
+    };
     uint32_t prefix = 0, mask = 0;
     uint32_t need = (uint32_t)a.keep;  // how many of the keys that match `prefix` are kept
+    bool all = false;                  // every key that matches is kept
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
+    for (int pass = 0; pass < 3 && !all; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digits = pass == 2 ? 1024u : 2048u;
-        for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
+        for (int i = tid; i < kCopies * kBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += kSelThreads) {
-            const uint32_t k = key_of(i);
-            if ((k & mask) == prefix) atomicAdd(&sh.hist[(k >> shift) & (digits - 1)], 1u);
-        }
+        each([&](int i, uint32_t k) {
+            if (i < n && (k & mask) == prefix) atomicAdd(&sh.hist[lane % kCopies][(k >> shift) & (digits - 1)], 1u);
+        });
         __syncthreads();
         // digits from the top: thread t holds digits 2 (1023 - t) + 1 and 2 (1023 - t)
         const int d = 2 * (kSelThreads - 1 - tid);
-        const uint32_t hi = sh.hist[d + 1], lo = sh.hist[d];
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            const uint2 h = *(const uint2 *)&sh.hist[c][d];
+            lo += h.x;
+            hi += h.y;
+        }
         uint32_t total;
-        const uint32_t before = block_scan(hi + lo, sh.warp_sum[0], total);
+        const uint32_t before = block_scan(hi + lo, sh, turn, total);
         if (before < need && need <= before + hi) {
             sh.digit = d + 1;
             sh.above = before;
+            sh.count = hi;
         } else if (before + hi < need && need <= before + hi + lo) {
             sh.digit = d;
             sh.above = before + hi;
+            sh.count = lo;
         }
         __syncthreads();
         prefix |= sh.digit << shift;
         mask |= (digits - 1) << shift;
         need -= sh.above;
-        __syncthreads();
+        all = sh.count == need;
     }
+    // kept: keys above `prefix` in the digits seen, and the first `need` equal to it there
 
-    // ---- one bit per slot: keys above the threshold, and the first `need` equal to it ----
+    // ---- one bit per slot ----
     const int words = (n + 31) / 32;
     uint32_t *sel = s_mem, *cnt = s_mem + a.max_words;  // chosen slots; ties, then survivors at or above keep before a word
-    for (int wd = warp; wd < words; wd += kSelThreads / 32) {
-        const int i = 32 * wd + lane;
-        const uint32_t k = i < n ? key_of(i) : 0u;
-        const uint32_t gt = __ballot_sync(0xffffffffu, i < n && k > prefix);
-        const uint32_t eq = __ballot_sync(0xffffffffu, i < n && k == prefix);
-        if (lane == 0) {
+    each([&](int i, uint32_t k) {
+        const uint32_t gt = __ballot_sync(0xffffffffu, i < n && (k & mask) > prefix);
+        const uint32_t eq = __ballot_sync(0xffffffffu, i < n && (k & mask) == prefix);
+        const int wd = i >> 5;
+        if (lane == 0 && wd < words) {
             sel[wd] = gt;
             cnt[wd] = eq;
         }
-    }
+    });
     __syncthreads();
     uint32_t ties = 0;
     for (int w0 = 0; w0 < words; w0 += kSelThreads) {
         const int wd = w0 + tid;
         const uint32_t eq = wd < words ? cnt[wd] : 0u;
         uint32_t total;
-        uint32_t rank = ties + block_scan(__popc(eq), sh.warp_sum[0], total);
+        uint32_t rank = ties + block_scan(__popc(eq), sh, turn, total);
         if (eq && rank < need) {
             uint32_t take = need - rank, e = eq, got = 0;
             if (take >= (uint32_t)__popc(eq)) {
@@ -178,7 +212,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     for (int w0 = first_tail; w0 < words; w0 += kSelThreads) {
         const int wd = w0 + tid;
         uint32_t total;
-        const uint32_t before = tails + block_scan(wd < words ? __popc(tail_bits(wd)) : 0u, sh.warp_sum[0], total);
+        const uint32_t before = tails + block_scan(wd < words ? __popc(tail_bits(wd)) : 0u, sh, turn, total);
         if (wd < words) cnt[wd] = before;
         tails += total;
     }
@@ -189,7 +223,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
         const int i = i0 + tid;
         const bool hole = i < a.keep && !((sel[i >> 5] >> (i & 31)) & 1u);
         uint32_t total;
-        const uint32_t rank = holes + block_scan(hole ? 1u : 0u, sh.warp_sum[0], total);
+        const uint32_t rank = holes + block_scan(hole ? 1u : 0u, sh, turn, total);
         holes += total;
         if (i >= a.keep) continue;
         int from = i;
@@ -217,6 +251,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
     __shared__ uint8_t *s_dst[kMoveWarps][32];
     __shared__ int s_rows[kMoveWarps][32];  // row inside the source block << 16 | inside the destination block
     const PoolView &p = a.pool;
+    decode::grid_wait();
     const int lbh = blockIdx.x / chunks, chunk = blockIdx.x - lbh * chunks;
     const int h = lbh % p.kv_heads, lb = lbh / p.kv_heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -245,28 +280,31 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
     const int64_t kv_bytes = (int64_t)p.kv_heads * p.tile_bytes;
     const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
     const int per = q8 ? D / 16 : D / 8, units = 2 * per;  // 16-byte units of a row, K then V
-    constexpr int UNROLL = 4;
-    for (int i0 = lane; i0 < n * units; i0 += 32 * UNROLL) {
-        uint4 v[UNROLL];
-        uint8_t *to[UNROLL];
+    // A lane keeps one unit of the row; where a row has at most 16 units, several rows are taken at a time.
+    const int wlog = decode::log2_of(p.swz_bytes);
+    const int at_once = units <= 16 ? 32 / units : 1, sub = units <= 16 ? lane / units : 0;
+    constexpr int UNROLL = 8;
+    for (int u0 = units <= 16 ? lane - sub * units : lane; u0 < units; u0 += 32) {
+        if (sub >= at_once) break;
+        const int u = u0 >= per ? u0 - per : u0;
+        const int64_t kv = u0 >= per ? kv_bytes : 0;
+        for (int m0 = sub; m0 < n; m0 += at_once * UNROLL) {
+            uint4 v[UNROLL];
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
-            const int i = i0 + 32 * j;
-            to[j] = nullptr;
-            if (i >= n * units) continue;
-            const int m = i / units;
-            int u = i - m * units;
-            const int64_t kv = u >= per ? kv_bytes : 0;
-            if (u >= per) u -= per;
-            const int rs = s_rows[warp][m] >> 16, rd = s_rows[warp][m] & 0xffff;
-            const uint32_t os = q8 ? q8_qs_off(rs, 16 * u, D) : tile_elem_off(rs, 8 * u, D, p.swz_bytes);
-            const uint32_t od = q8 ? q8_qs_off(rd, 16 * u, D) : tile_elem_off(rd, 8 * u, D, p.swz_bytes);
-            v[j] = *(const uint4 *)(s_src[warp][m] + kv + os);
-            to[j] = s_dst[warp][m] + kv + od;
+            for (int j = 0; j < UNROLL; ++j) {
+                const int m = m0 + j * at_once;
+                if (m >= n) continue;
+                const int rs = s_rows[warp][m] >> 16;
+                v[j] = *(const uint4 *)(s_src[warp][m] + kv + (q8 ? q8_qs_off(rs, 16 * u, D) : decode::bf16_off_any(rs, 8 * u, D, wlog)));
+            }
+#pragma unroll
+            for (int j = 0; j < UNROLL; ++j) {
+                const int m = m0 + j * at_once;
+                if (m >= n) continue;
+                const int rd = s_rows[warp][m] & 0xffff;
+                *(uint4 *)(s_dst[warp][m] + kv + (q8 ? q8_qs_off(rd, 16 * u, D) : decode::bf16_off_any(rd, 8 * u, D, wlog))) = v[j];
+            }
         }
-#pragma unroll
-        for (int j = 0; j < UNROLL; ++j)
-            if (to[j]) *(uint4 *)to[j] = v[j];
     }
     if (!q8) return;
     const int g = D / 32;
@@ -288,16 +326,11 @@ int launch_evict(EvictArgs a, cudaStream_t s) {
     if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
     a.max_words = (a.max_len + 31) / 32 + 1;
     const size_t smem = (size_t)a.max_words * 2 * sizeof(uint32_t);
-    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-        cudaGetLastError();
-        return EKV_ERR_CUDA;
-    }
-    evict_select_kernel<<<(unsigned)n, kSelThreads, smem, s>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    evict_move_kernel<<<(unsigned)(n * chunks), kMoveWarps * 32, 0, s>>>(a, chunks);
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    note_launches(2);
-    return EKV_OK;
+    static std::atomic<uint64_t> smem_done{0};
+    if (const int rc = decode::allow_smem(evict_select_kernel, (EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 * (int)sizeof(uint32_t), smem_done))
+        return rc;
+    if (const int rc = decode::launch_after(evict_select_kernel, (unsigned)n, kSelThreads, smem, s, a)) return rc;
+    return decode::launch_after(evict_move_kernel, (unsigned)(n * chunks), kMoveWarps * 32, 0, s, a, chunks);
 }
 
 }  // namespace ekv

@@ -8,7 +8,7 @@
 #include <cmath>
 #include <new>
 
-#include "ekv_device.cuh"
+#include "ekv_decode.cuh"
 #include "ekv_internal.h"
 
 struct ekv_rope {
@@ -23,10 +23,22 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRows = 8;  // rows per CTA
+constexpr int kLoads = 2;    // units (of 16 or 32 bytes) a thread loads before it stores
+
+// Division of small numbers by a fixed one: floor(i / d) = (i * ceil(2^32 / d)) >> 32 while i * d < 2^32.
+struct SmallDiv {
+    uint32_t m;
+    SmallDiv() = default;
+    explicit SmallDiv(uint32_t d) : m((uint32_t)(((1ull << 32) + d - 1) / d)), one(d == 1) {}
+    uint32_t one;
+    __device__ __forceinline__ int operator()(int i) const { return one ? i : (int)__umulhi((uint32_t)i, m); }
+};
 
 struct RopeArgs {
     PoolView pool;
     int32_t layer, n_batch, max_rows, rows_per_cta, q_heads, interleaved, rotary;
+    int32_t per;  // units (items of the odd forms) of a turned head
+    SmallDiv div_per, div_q, div_kv, div_v;
     float magnitude;
     const double *turns;
     const int32_t *seq_ids, *dst_pos, *n_rows, *src_row, *positions;
@@ -41,37 +53,48 @@ __device__ __forceinline__ uint32_t rot_pair(uint32_t lo_hi, float2 cs) {  // an
     return a | b << 16;
 }
 
-// One head's unit u: 16 bytes, or the two 16-byte halves of eight split pairs. `put(d, value)` writes the 16
-// bytes of columns d .. d + 7.
+// One head's unit u: 16 bytes, or the two 16-byte halves of eight split pairs (the columns past the rotated ones
+// follow them, 16 bytes each).
+struct Unit {
+    uint4 x, y;
+};
+__device__ __forceinline__ Unit load_unit(const RopeArgs &a, const uint16_t *src, int u) {
+    Unit r;
+    const int n = a.rotary, pairs = n / 16;
+    const bool pair = !a.interleaved && u < pairs;
+    const int d = a.interleaved || pair ? 8 * u : n + 8 * (u - pairs);
+    r.x = *(const uint4 *)(src + d);
+    r.y = pair ? *(const uint4 *)(src + d + n / 2) : make_uint4(0, 0, 0, 0);
+    return r;
+}
+// `put(d, value)` writes the 16 bytes of columns d .. d + 7.
 template <class Put>
-__device__ __forceinline__ void rot_unit(const RopeArgs &a, const uint16_t *src, int u, const float2 *cs, Put put) {
+__device__ __forceinline__ void turn_unit(const RopeArgs &a, Unit r, int u, const float2 *cs, Put put) {
     const int n = a.rotary;
     if (a.interleaved) {
         const int d = 8 * u;
-        uint4 x = *(const uint4 *)(src + d);
         if (d < n) {
-            x.x = rot_pair(x.x, cs[d / 2]);
-            if (d + 2 < n) x.y = rot_pair(x.y, cs[d / 2 + 1]);
-            if (d + 4 < n) x.z = rot_pair(x.z, cs[d / 2 + 2]);
-            if (d + 6 < n) x.w = rot_pair(x.w, cs[d / 2 + 3]);
+            r.x.x = rot_pair(r.x.x, cs[d / 2]);
+            if (d + 2 < n) r.x.y = rot_pair(r.x.y, cs[d / 2 + 1]);
+            if (d + 4 < n) r.x.z = rot_pair(r.x.z, cs[d / 2 + 2]);
+            if (d + 6 < n) r.x.w = rot_pair(r.x.w, cs[d / 2 + 3]);
         }
-        put(d, x);
+        put(d, r.x);
         return;
     }
-    const int pairs = n / 16;  // units of eight split pairs; the columns past the rotated ones follow
+    const int pairs = n / 16;
     if (u >= pairs) {
-        const int d = n + 8 * (u - pairs);
-        put(d, *(const uint4 *)(src + d));
+        put(n + 8 * (u - pairs), r.x);
         return;
     }
     const int d = 8 * u, h = n / 2;
-    const uint4 x = *(const uint4 *)(src + d), y = *(const uint4 *)(src + d + h);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    const uint32_t xs[4] = {r.x.x, r.x.y, r.x.z, r.x.w}, ys[4] = {r.y.x, r.y.y, r.y.z, r.y.w};
     uint32_t p[4], q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t e = rot_pair((xs[i] & 0xffffu) | ys[i] << 16, cs[d + 2 * i]);
-        const uint32_t o = rot_pair(xs[i] >> 16 | (ys[i] & 0xffff0000u), cs[d + 2 * i + 1]);
+        const float4 c = *(const float4 *)&cs[d + 2 * i];
+        const uint32_t e = rot_pair((xs[i] & 0xffffu) | ys[i] << 16, make_float2(c.x, c.y));
+        const uint32_t o = rot_pair(xs[i] >> 16 | (ys[i] & 0xffff0000u), make_float2(c.z, c.w));
         p[i] = (e & 0xffffu) | o << 16;
         q[i] = e >> 16 | (o & 0xffff0000u);
     }
@@ -107,13 +130,14 @@ __device__ __forceinline__ float rot_at(const RopeArgs &a, const uint16_t *src, 
 // Grid: (row chunk, request). WIDE: every head is whole 16-byte units.
 template <bool Q8, bool WIDE>
 __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a) {
-    extern __shared__ float2 s_cs[];  // [rows][rotary / 2]
+    extern __shared__ __align__(16) float2 s_cs[];  // [rows][rotary / 2]
     __shared__ int s_blk[kMaxRows], s_rib[kMaxRows];
     const PoolView &p = a.pool;
+    decode::grid_wait();
     const int b = blockIdx.y, r0 = blockIdx.x * a.rows_per_cta;
     const int nr = min(a.rows_per_cta, min(a.max_rows, a.n_rows[b]) - r0);
     if (nr <= 0) return;
-    const int half = a.rotary / 2, D = p.head_dim;
+    const int half = a.rotary / 2, D = p.head_dim, wlog = decode::log2_of(p.swz_bytes);
     const int64_t row0 = (int64_t)a.src_row[b] + r0;
     if (a.k && (int)threadIdx.x < nr) {
         const int seq = a.seq_ids[b], pos = a.dst_pos[b] + r0 + (int)threadIdx.x;
@@ -136,60 +160,116 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
         s_cs[i] = make_float2(cn * a.magnitude, sn * a.magnitude);
     }
     __syncthreads();
-    // items of a row: q heads, k heads, v heads
-    const int per = WIDE ? (a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8) : half + D - a.rotary;
-    const int nq = a.q ? a.q_heads * per : 0;
-    const int nk = !a.k ? 0 : p.kv_heads * (Q8 ? D / 32 : per), nv = !a.k ? 0 : p.kv_heads * (Q8 ? D / 32 : D / 8);
-    const int items = nq + nk + nv;
-    for (int i = threadIdx.x; i < nr * items; i += kThreads) {
-        const int r = i / items;
-        int u = i - r * items;
-        const float2 *cs = s_cs + r * half;
-        if (u < nq) {
-            const int h = u / per;
-            u -= h * per;
-            const uint16_t *src = a.q + (row0 + r) * a.q_stride + h * D;
-            uint16_t *dst = a.q_out + ((row0 + r) * a.q_heads + h) * D;
-            if (WIDE) rot_unit(a, src, u, cs, [&](int d, uint4 x) { *(uint4 *)(dst + d) = x; });
-            else rot_item(a, src, u, cs, [&](int d, uint16_t x) { dst[d] = x; });
-            continue;
+    // Items of the CTA's rows: (row, head, unit) of q, then of k, then of v, kLoads of them in flight per thread.
+    const int per = a.per, hk = p.kv_heads;
+    if (a.q) {
+        const int total = nr * a.q_heads * per;
+        for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kLoads) {
+            Unit x[kLoads];
+            int rr[kLoads], uu[kLoads];
+            int64_t at[kLoads];
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int i = i0 + j * kThreads;
+                rr[j] = -1;
+                if (i >= total) continue;
+                const int hr = a.div_per(i), r = a.div_q(hr), h = hr - r * a.q_heads;
+                rr[j] = r;
+                uu[j] = i - hr * per;
+                const uint16_t *src = a.q + (row0 + r) * a.q_stride + h * D;
+                at[j] = ((row0 + r) * a.q_heads + h) * D;
+                if (WIDE) x[j] = load_unit(a, src, uu[j]);
+                else rot_item(a, src, uu[j], s_cs + r * half, [&](int d, uint16_t v) { a.q_out[at[j] + d] = v; });
+            }
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j)
+                    if (rr[j] >= 0)
+                        turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, [&](int d, uint4 v) { *(uint4 *)(a.q_out + at[j] + d) = v; });
+            }
         }
-        const int blk = s_blk[r], rib = s_rib[r];
-        if (blk < 0) continue;
-        u -= nq;
-        const bool is_v = u >= nk;
-        if (is_v) u -= nk;
-        const int n_u = Q8 ? D / 32 : is_v ? D / 8 : per;
-        const int h = u / n_u;
-        u -= h * n_u;
-        const uint16_t *src = (is_v ? a.v : a.k) + (row0 + r) * a.kv_stride + h * D;
-        uint8_t *tile = p.prefix + prefix_tile_index(p, a.layer, blk, is_v ? 1 : 0, h) * p.tile_bytes;
-        if (!Q8) {
-            const auto put = [&](int d, uint4 x) { *(uint4 *)(tile + tile_elem_off(rib, d, D, p.swz_bytes)) = x; };
-            if (is_v) put(8 * u, *(const uint4 *)(src + 8 * u));
-            else if (WIDE) rot_unit(a, src, u, cs, put);
-            else rot_item(a, src, u, cs, [&](int d, uint16_t x) { *(uint16_t *)(tile + tile_elem_off(rib, d, D, p.swz_bytes)) = x; });
-            continue;
-        }
+    }
+    if (!a.k) return;
+    if (Q8) {
         // the group's values as ekv_append would get them (bf16), quantised by its rule
-        float x[32], amax = 0.0f;
+        const int groups = D / 32, total = nr * hk * groups;
+        for (int i = threadIdx.x; i < 2 * total; i += kThreads) {
+            const bool is_v = i >= total;
+            const int hr = (is_v ? i - total : i) / groups, u = (is_v ? i - total : i) - hr * groups;
+            const int r = a.div_kv(hr), h = hr - r * hk;
+            if (s_blk[r] < 0) continue;
+            const uint16_t *src = (is_v ? a.v : a.k) + (row0 + r) * a.kv_stride + h * D;
+            uint8_t *tile = p.prefix + prefix_tile_index(p, a.layer, s_blk[r], is_v ? 1 : 0, h) * p.tile_bytes;
+            float x[32], amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            x[j] = is_v ? bf16_bits_to_f32(src[32 * u + j]) : rot_at(a, src, 32 * u + j, cs);
-            amax = fmaxf(amax, fabsf(x[j]));
+            for (int j = 0; j < 32; ++j) {
+                x[j] = is_v ? bf16_bits_to_f32(src[32 * u + j]) : rot_at(a, src, 32 * u + j, s_cs + r * half);
+                amax = fmaxf(amax, fabsf(x[j]));
+            }
+            const float d = __fdiv_rn(amax, 127.0f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[j] |= ((uint32_t)(uint8_t)(int8_t)(int)roundf(__fmul_rn(x[4 * j + e], id))) << (8 * e);
+            }
+            const int rib = s_rib[r];
+            *(uint4 *)(tile + q8_qs_off(rib, 32 * u, D)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *(uint4 *)(tile + q8_qs_off(rib, 32 * u + 16, D)) = make_uint4(w[4], w[5], w[6], w[7]);
+            *((uint16_t *)(tile + (int64_t)p.block_tokens * D) + rib * groups + u) = __half_as_ushort(__float2half_rn(d));
         }
-        const float d = __fdiv_rn(amax, 127.0f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-        uint32_t w[8];
+        return;
+    }
+    const int total_k = nr * hk * per;
+    for (int i0 = threadIdx.x; i0 < total_k; i0 += kThreads * kLoads) {
+        Unit x[kLoads];
+        int rr[kLoads], uu[kLoads];
+        uint8_t *tile[kLoads];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            w[j] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[j] |= ((uint32_t)(uint8_t)(int8_t)(int)roundf(__fmul_rn(x[4 * j + e], id))) << (8 * e);
+        for (int j = 0; j < kLoads; ++j) {
+            const int i = i0 + j * kThreads;
+            rr[j] = -1;
+            if (i >= total_k) continue;
+            const int hr = a.div_per(i), r = a.div_kv(hr), h = hr - r * hk;
+            if (s_blk[r] < 0) continue;
+            rr[j] = r;
+            uu[j] = i - hr * per;
+            const uint16_t *src = a.k + (row0 + r) * a.kv_stride + h * D;
+            tile[j] = p.prefix + prefix_tile_index(p, a.layer, s_blk[r], 0, h) * p.tile_bytes;
+            if (WIDE) x[j] = load_unit(a, src, uu[j]);
+            else
+                rot_item(a, src, uu[j], s_cs + r * half, [&](int d, uint16_t v) {
+                    *(uint16_t *)(tile[j] + decode::bf16_off_any(s_rib[r], d, D, wlog)) = v;
+                });
         }
-        *(uint4 *)(tile + q8_qs_off(rib, 32 * u, D)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *(uint4 *)(tile + q8_qs_off(rib, 32 * u + 16, D)) = make_uint4(w[4], w[5], w[6], w[7]);
-        *((uint16_t *)(tile + (int64_t)p.block_tokens * D) + rib * (D / 32) + u) = __half_as_ushort(__float2half_rn(d));
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j)
+                if (rr[j] >= 0)
+                    turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, [&](int d, uint4 v) {
+                        *(uint4 *)(tile[j] + decode::bf16_off_any(s_rib[rr[j]], d, D, wlog)) = v;
+                    });
+        }
+    }
+    const int pv = D / 8, total_v = nr * hk * pv;
+    for (int i0 = threadIdx.x; i0 < total_v; i0 += kThreads * 2 * kLoads) {
+        uint4 x[2 * kLoads];
+        uint8_t *to[2 * kLoads];
+#pragma unroll
+        for (int j = 0; j < 2 * kLoads; ++j) {
+            const int i = i0 + j * kThreads;
+            to[j] = nullptr;
+            if (i >= total_v) continue;
+            const int hr = a.div_v(i), u = i - hr * pv, r = a.div_kv(hr), h = hr - r * hk;
+            if (s_blk[r] < 0) continue;
+            x[j] = *(const uint4 *)(a.v + (row0 + r) * a.kv_stride + h * D + 8 * u);
+            to[j] = p.prefix + prefix_tile_index(p, a.layer, s_blk[r], 1, h) * p.tile_bytes + decode::bf16_off_any(s_rib[r], 8 * u, D, wlog);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * kLoads; ++j)
+            if (to[j]) *(uint4 *)to[j] = x[j];
     }
 }
 
@@ -224,16 +304,21 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
     const dim3 grid((unsigned)((max_rows + a.rows_per_cta - 1) / a.rows_per_cta), (unsigned)n_batch);
     const size_t smem = (size_t)a.rows_per_cta * (a.rotary / 2) * sizeof(float2);
     const bool wide = a.interleaved || a.rotary % 16 == 0;
+    const int D = p.head_dim;
+    a.per = !wide ? a.rotary / 2 + D - a.rotary : a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8;
+    if ((int64_t)kMaxRows * std::max(q_heads, p.kv_heads) * D * std::max({a.per, q_heads, p.kv_heads, D / 8}) >= 1ll << 32)
+        return EKV_ERR_UNSUPPORTED;
+    a.div_per = SmallDiv((uint32_t)a.per);
+    a.div_q = SmallDiv((uint32_t)std::max(1, q_heads));
+    a.div_kv = SmallDiv((uint32_t)p.kv_heads);
+    a.div_v = SmallDiv((uint32_t)(D / 8));
     if (p.dtype == EKV_DTYPE_Q8_0) {
-        if (wide) rope_append_kernel<true, true><<<grid, kThreads, smem, s>>>(a);
-        else rope_append_kernel<true, false><<<grid, kThreads, smem, s>>>(a);
+        if (wide) return decode::launch_after(rope_append_kernel<true, true>, grid, kThreads, smem, s, a);
+        else return decode::launch_after(rope_append_kernel<true, false>, grid, kThreads, smem, s, a);
     } else {
-        if (wide) rope_append_kernel<false, true><<<grid, kThreads, smem, s>>>(a);
-        else rope_append_kernel<false, false><<<grid, kThreads, smem, s>>>(a);
+        if (wide) return decode::launch_after(rope_append_kernel<false, true>, grid, kThreads, smem, s, a);
+        else return decode::launch_after(rope_append_kernel<false, false>, grid, kThreads, smem, s, a);
     }
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    note_launches(1);
-    return EKV_OK;
 }
 
 int rope_device(const ekv_rope *r) { return r->device; }

@@ -4,8 +4,13 @@
 // drafted keys that t's ancestor word names:
 //   s_k = scale * q.k  (or cap * tanh(scale * q.k / cap)),  out = sum exp(s_k - m) v_k / sum exp(s_k - m),
 //   lse = m + ln sum exp(s_k - m).
-// One pass over the keys: a warp keeps the running maximum m, the sum and the output of its 16 rows in
-// registers (flash attention's recurrence, Dao et al. 2022; Milakov and Gimelshein 2018 for the softmax).
+// One pass over the keys: a warp keeps the reference maximum m, the sum and the output of its rows in
+// registers (the running softmax of Milakov and Gimelshein 2018, with the output as in flash attention,
+// Dao et al. 2022). m moves only when a score is more than 2^8 above it; every quotient is exact about that.
+//
+// Products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and value columns fill the 16 rows of
+// the matrix instruction and query rows its 8 columns, so that the usual 4 or 8 rows of a decoded token's KV
+// head waste nothing, and a row's output over D columns takes D / 4 registers of a thread for 8 rows.
 #include <algorithm>
 
 #include "ekv_decode.cuh"
@@ -18,16 +23,18 @@ using namespace sm100;
 
 constexpr int kXCols = 32;  // columns that the key groups' outputs are joined in at a time
 
-// CTAs per SM: two where a thread's share of the output (16 * MT rows by D columns over a warp) leaves the
-// registers for it.
-constexpr int rows_ctas(int d, int mt) { return d / 2 * mt > 64 ? 1 : 2; }
+// CTAs per SM: two where a thread's share of the output (8 * NR rows by D columns over a warp) leaves the
+// registers for it and two tiles in flight fit the shared memory of half an SM.
+constexpr int rows_ctas(int d, bool q8, int nr, int wr) {
+    return d * nr > 256 || wr * 8 * nr > 64 || (d > 128 && !q8) || (d > 128 && wr > 1) ? 1 : 2;
+}
 
-// WR row groups of 16 * MT rows times WK groups of 64 / WK keys: one warp each, and one feeder warp.
-template <int D, bool Q8, int MT, int WR, int WK>
+// WR row groups of 8 * NR rows times WK groups of 64 / WK keys: one warp each, and one feeder warp.
+template <int D, bool Q8, int NR, int WR, int WK>
 struct Cfg {
     using T = TileCfg<D, Q8>;
     static constexpr int NW = WR * WK, NC = NW * 32, THREADS = NC + 32;
-    static constexpr int ROWS = 16 * MT * WR;
+    static constexpr int ROWS = 8 * NR * WR;
     static constexpr int KPW = kTile / WK;          // keys of a tile per warp
     static constexpr int NB = KPW / 16;             // 16-key steps per warp and tile
     // drafted keys per tile: bf16 rows in the tile's own layout, or padded rows where the tile is Q8_0
@@ -38,9 +45,11 @@ struct Cfg {
     static constexpr int V_OFF = T::KV_BYTES, DRAFT_V_OFF = Q8 ? DT * DROW : T::KV_BYTES;
     static constexpr int X_BYTES = WK * ROWS * kXCols * 4;
     static constexpr int ML_BYTES = WK * ROWS * 8;
-    static constexpr int FIXED = X_BYTES + ML_BYTES + 1024 + 1024;
-    // two CTAs per SM where the rows' state leaves registers for it
-    static constexpr int CTAS = rows_ctas(D, MT);
+    // query rows in shared memory where the output's share of the registers leaves no room for them
+    static constexpr bool Q_SMEM = D * NR > 256;
+    static constexpr int Q_BYTES = Q_SMEM ? ROWS * q_row_bytes<D>() : 0;
+    static constexpr int FIXED = X_BYTES + ML_BYTES + Q_BYTES + 1024 + 1024;
+    static constexpr int CTAS = rows_ctas(D, Q8, NR, WR);
     static constexpr int BUDGET = CTAS == 2 ? 112 * 1024 : 220 * 1024;
     static constexpr int NST_FIT = (BUDGET - FIXED) / STAGE;
     static constexpr int NST = NST_FIT > 8 ? 8 : NST_FIT;
@@ -56,17 +65,18 @@ struct Shared {
     int abort;
 };
 
-// Column of output accumulator (n-tile nt, element i) of lane c in its quad.
+// Column of output accumulator (16-column step ds, element i) of lane row kq. Q8_0 kernels take the columns of a
+// 32-column group in the order that one word of a key's row gives them to a lane.
 template <bool Q8>
-__device__ __forceinline__ int o_col(int nt, int c, int i) {
-    return Q8 ? 32 * (nt >> 2) + 8 * c + 4 * (i & 1) + (nt & 3) : 8 * nt + 2 * c + (i & 1);
+__device__ __forceinline__ int o_col(int ds, int kq, int i) {
+    return Q8 ? 32 * (ds >> 1) + 4 * kq + 2 * (ds & 1) + (i >> 1) : 16 * ds + kq + 8 * (i >> 1);
 }
 
-template <int D, bool Q8, int MT, int WR, int WK>
-__global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT, WR, WK>::CTAS)
+template <int D, bool Q8, int NR, int WR, int WK>
+__global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR, WR, WK>::CTAS)
     tree_rows_kernel(const TreeArgs a) {
-    using C = Cfg<D, Q8, MT, WR, WK>;
-    constexpr int NST = C::NST, KS = D / 16, NT = D / 8;
+    using C = Cfg<D, Q8, NR, WR, WK>;
+    constexpr int NST = C::NST, KS = D / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float *xb = (float *)(smem + NST * C::STAGE);                   // [WK][ROWS][kXCols]
@@ -74,6 +84,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
     using Sh = Shared<NST>;
     static_assert(sizeof(Sh) <= 1024, "barrier block");
     Sh &sh = *(Sh *)(smem + NST * C::STAGE + C::X_BYTES + C::ML_BYTES);
+    uint8_t *sq = smem + NST * C::STAGE + C::X_BYTES + C::ML_BYTES + 1024;  // [ROWS] query rows (Q_SMEM)
     volatile int *abort = &sh.abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -95,6 +106,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
         return max(1, (r.n_prefix + kTile - 1) / kTile + (r.n_nodes + C::DT - 1) / C::DT);
     };
     Range rg;
+    grid_wait();
+    grid_launch_next();  // the merge's blocks may take their places; they wait for this grid's end
     if (a.split) {
         rg = find_range<C::THREADS>(a.n_batch, units_per_req, sh.range,
                                     [&](int b) { return unit_tiles(load_req(a, b, false)); });
@@ -109,7 +122,13 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
         rg.ctas = 0;
     }
 
-    int it = 0;  // tile counter of the CTA: stage it % NST, use it / NST
+    int st = 0, turn = 0;  // stage of the next tile, and how often the ring went round
+    auto advance = [&]() {
+        if (++st == NST) {
+            st = 0;
+            ++turn;
+        }
+    };
     bool ok = true;
     int b = rg.b;
     long long base = rg.base;
@@ -129,16 +148,20 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
         const int rows = min(C::ROWS, rows_all - row0);
         const int p_tiles = (rq.n_prefix + kTile - 1) / kTile;
         const long long kv_row = ((long long)b * a.n_draft * hk + g) * D;  // drafted token 0 of this head
+        // query row r of the unit, or null where it does not take part
+        auto q_row = [&](int r) -> const uint16_t * {
+            const int t = r / a.group;
+            if (r >= rows_all || t >= rq.n_nodes) return nullptr;
+            return a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (r - t * a.group)) * D;
+        };
 
         if (warp == C::NW) {
             // ---- feeder ----
             Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
-            for (int j = t0; j < t1; ++j, ++it) {
-                const int st = it % NST;
+            for (int j = t0; j < t1; ++j, advance()) {
                 const Piece pc = next;
                 if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
-                if (it >= NST)
-                    ok = ok && mbar_wait(smem_addr(&sh.empty[st]), ((it / NST) - 1) & 1, abort, kWait);
+                if (turn > 0) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort, kWait);
                 if (!ok) {
                     *abort = 1;
                     continue;
@@ -194,47 +217,68 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
         } else {
             // ---- rows ----
             const int wr = warp / WK, wk = warp % WK;
-            const int rq0 = lane >> 2, c = lane & 3;
-            // query fragments: rows row0 + (wr * MT + m) * 16 + rq0 (+ 8)
-            uint32_t qf[MT][KS][4];
-            int t_of[MT][2];
+            const int kq = lane >> 2, c = lane & 3;  // key (or value column) and query row pair of the lane's elements
+            const int wrow = wr * 8 * NR;
+            // query operands: row wrow + 8 n + kq
+            uint32_t qf[C::Q_SMEM ? 1 : NR][C::Q_SMEM ? 1 : KS][2];
+            int t_of[NR][2];  // drafted token of rows wrow + 8 n + 2 c (+ 1), -1 where the row does not take part
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < NR; ++n) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = row0 + (wr * MT + m) * 16 + rq0 + 8 * h;
-                    const int t = r / a.group;
-                    const bool on = r < rows_all && t < rq.n_nodes;
-                    t_of[m][h] = on ? t : -1;
-                    const uint16_t *src =
-                        a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (r - t * a.group)) * D;
+                for (int e = 0; e < 2; ++e) {
+                    const int r = row0 + wrow + 8 * n + 2 * c + e, t = r / a.group;
+                    t_of[n][e] = r < rows_all && t < rq.n_nodes ? t : -1;
+                }
+                if constexpr (!C::Q_SMEM) {
+                    const uint16_t *src = q_row(row0 + wrow + 8 * n + kq);
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                         for (int half = 0; half < 2; ++half)
-                            qf[m][ks][h + 2 * half] = on ? __ldg((const uint32_t *)(src + q_col<Q8>(ks, c, half))) : 0u;
+                            qf[n][ks][half] = src ? __ldg((const uint32_t *)(src + q_col<Q8>(ks, c, half))) : 0u;
                 }
-            float o[MT][NT][4];
-            float mx[MT][2], sum[MT][2];
+            }
+            if constexpr (C::Q_SMEM) {  // the last rows were done with at the barriers of their end
+                for (int i = threadIdx.x; i < C::ROWS * (D / 8); i += C::NC) {
+                    const int rr = i / (D / 8), uu = i - rr * (D / 8);
+                    const uint16_t *src = q_row(row0 + rr);
+                    store_q_unit<Q8>(sq + rr * q_row_bytes<D>(), uu, src ? __ldg((const uint4 *)src + uu) : make_uint4(0, 0, 0, 0));
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
+            }
+            // operands of steps 2 i and 2 i + 1 (D is a multiple of 32 where they come from shared memory)
+            auto load_q2 = [&](int n, int i, uint32_t (&f)[4]) {
+                if constexpr (C::Q_SMEM) {
+                    ldmatrix_x4(f, smem_addr(sq) + (wrow + 8 * n + (lane & 7)) * q_row_bytes<D>() + 64 * i + (lane >> 3) * 16);
+                } else {
+                    f[0] = qf[n][2 * i][0];
+                    f[1] = qf[n][2 * i][1];
+                    if (2 * i + 1 < KS) {
+                        f[2] = qf[n][2 * i + 1][0];
+                        f[3] = qf[n][2 * i + 1][1];
+                    }
+                }
+            };
+            float o[NR][KS][4];  // O^T: columns o_col(ds, kq, i), row 2 c + (i & 1)
+            float mx[NR][2], sum[NR][2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                mx[m][0] = mx[m][1] = -INFINITY;
-                sum[m][0] = sum[m][1] = 0.0f;
+            for (int n = 0; n < NR; ++n) {
+                mx[n][0] = mx[n][1] = -INFINITY;
+                sum[n][0] = sum[n][1] = 0.0f;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int ds = 0; ds < KS; ++ds)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[m][nt][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) o[n][ds][i] = 0.0f;
             }
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
 
-            for (int j = t0; j < t1; ++j, ++it) {
-                const int st = it % NST, par = (it / NST) & 1;
+            for (int j = t0; j < t1; ++j, advance()) {
+                const int par = turn & 1;
                 uint8_t *tile = smem + st * C::STAGE;
                 const uint32_t sk = smem_addr(tile);
                 const bool draft = j >= p_tiles;
                 const int d0 = (j - p_tiles) * C::DT;
                 const int valid = draft ? min(C::DT, rq.n_nodes - d0) : min(kTile, rq.n_prefix - j * kTile);
-                const bool full = !draft && valid == kTile;
                 const uint32_t sv = sk + (draft ? C::DRAFT_V_OFF : C::V_OFF);
                 ok = ok && mbar_wait(smem_addr(&sh.full_k[st]), par, abort, kWait);
                 if (!ok) {
@@ -246,123 +290,131 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
                 for (int kb = 0; kb < C::NB; ++kb) {
                     const int key0 = wk * C::KPW + kb * 16;  // 16 keys of the tile
                     if (key0 >= valid) break;
-                    // ---- S = Q K^T ----
-                    float s[MT][2][4];
+                    // ---- S^T = K Q^T: keys kq, kq + 8; rows 2 c, 2 c + 1 ----
+                    float s[NR][4];
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                    for (int n = 0; n < NR; ++n)
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.0f;
+                        for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
                     if constexpr (!Q8) {
 #pragma unroll
-                        for (int ks = 0; ks < KS; ++ks) {
-                            uint32_t kf[4];
-                            load_k_step<D>(sk, key0, ks, lane, kf);
+                        for (int i = 0; i < (KS + 1) / 2; ++i) {
+                            uint32_t k0[4], k1[4];
+                            load_k_rows<D>(sk, key0, 2 * i, lane, k0);
+                            if (2 * i + 1 < KS) load_k_rows<D>(sk, key0, 2 * i + 1, lane, k1);
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) {
-                                mma_bf16(s[m][0], qf[m][ks], kf[0], kf[1]);
-                                mma_bf16(s[m][1], qf[m][ks], kf[2], kf[3]);
+                            for (int n = 0; n < NR; ++n) {
+                                uint32_t f[4];
+                                load_q2(n, i, f);
+                                mma_bf16(s[n], k0, f[0], f[1]);
+                                if (2 * i + 1 < KS) mma_bf16(s[n], k1, f[2], f[3]);
                             }
                         }
                     } else if (draft) {
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                        for (int i = 0; i < KS / 2; ++i) {
+                            // 8 columns of two keys in one load: steps 2 i and 2 i + 1
+                            const uint32_t at = sk + (key0 + kq) * C::DROW + 2 * (32 * i + 8 * c);
+                            const uint4 w0 = lds128(at), w1 = lds128(at + 8 * C::DROW);
+                            const uint32_t k0[4] = {w0.x, w1.x, w0.y, w1.y}, k1[4] = {w0.z, w1.z, w0.w, w1.w};
 #pragma unroll
-                            for (int ks = 0; ks < KS; ++ks) {
-                                const uint2 w = lds64(sk + (key0 + 8 * n + rq0) * C::DROW + 2 * q_col<true>(ks, c, 0));
-#pragma unroll
-                                for (int m = 0; m < MT; ++m) mma_bf16(s[m][n], qf[m][ks], w.x, w.y);
+                            for (int n = 0; n < NR; ++n) {
+                                uint32_t f[4];
+                                load_q2(n, i, f);
+                                mma_bf16(s[n], k0, f[0], f[1]);
+                                mma_bf16(s[n], k1, f[2], f[3]);
                             }
+                        }
                     } else {
-                        // integer products of a 32-column group are exact; its two scales join in f32
+                        // integer products of a 32-column group are exact; the keys' scales join in f32
                         using T = TileCfg<D, true>;
+                        uint32_t sc0[(T::G32 + 1) / 2], sc1[(T::G32 + 1) / 2];
+                        load_scales<T::G32>(sk + T::SCALES + (key0 + kq) * T::G32 * 2, sc0);
+                        load_scales<T::G32>(sk + T::SCALES + (key0 + kq + 8) * T::G32 * 2, sc1);
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            const int row = key0 + 8 * n + rq0, krow = key0 + 8 * n + 2 * c;
+                        for (int gr = 0; gr < T::G32; ++gr) {
+                            const uint2 w0 = lds64(sk + q8_qs_off(key0 + kq, 32 * gr + 8 * c, D));
+                            const uint2 w1 = lds64(sk + q8_qs_off(key0 + kq + 8, 32 * gr + 8 * c, D));
+                            uint32_t k0[4], k1[4];
+                            int8x4_to_bf16(w0.x, k0[0], k0[2]);
+                            int8x4_to_bf16(w1.x, k0[1], k0[3]);
+                            int8x4_to_bf16(w0.y, k1[0], k1[2]);
+                            int8x4_to_bf16(w1.y, k1[1], k1[3]);
+                            const float f0 = scale_of(sc0, gr), f1 = scale_of(sc1, gr);
 #pragma unroll
-                            for (int gr = 0; gr < T::G32; ++gr) {
-                                const uint2 w = lds64(sk + q8_qs_off(row, 32 * gr + 8 * c, D));
-                                uint32_t k0, k1, k2, k3;
-                                int8x4_to_bf16(w.x, k0, k1);
-                                int8x4_to_bf16(w.y, k2, k3);
-                                const float sc0 = lds_f16(sk + T::SCALES + (krow * T::G32 + gr) * 2);
-                                const float sc1 = lds_f16(sk + T::SCALES + ((krow + 1) * T::G32 + gr) * 2);
-#pragma unroll
-                                for (int m = 0; m < MT; ++m) {
-                                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                    mma_bf16(acc, qf[m][2 * gr], k0, k1);
-                                    mma_bf16(acc, qf[m][2 * gr + 1], k2, k3);
-                                    s[m][n][0] = fmaf(acc[0], sc0, s[m][n][0]);
-                                    s[m][n][1] = fmaf(acc[1], sc1, s[m][n][1]);
-                                    s[m][n][2] = fmaf(acc[2], sc0, s[m][n][2]);
-                                    s[m][n][3] = fmaf(acc[3], sc1, s[m][n][3]);
-                                }
+                            for (int n = 0; n < NR; ++n) {
+                                uint32_t f[4];
+                                load_q2(n, gr, f);
+                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_bf16(acc, k0, f[0], f[1]);
+                                mma_bf16(acc, k1, f[2], f[3]);
+                                s[n][0] = fmaf(acc[0], f0, s[n][0]);
+                                s[n][1] = fmaf(acc[1], f0, s[n][1]);
+                                s[n][2] = fmaf(acc[2], f1, s[n][2]);
+                                s[n][3] = fmaf(acc[3], f1, s[n][3]);
                             }
                         }
                     }
-                    // ---- mask, running maximum, exponentials ----
-                    uint32_t vis[MT][2];  // bit k: key0 + k visible to the row
+                    // ---- mask, reference maximum, exponentials ----
+                    const bool masked = draft || key0 + 16 > valid;
+                    uint32_t vis[NR][2];  // draft tiles: bit k, key0 + k visible to the row
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                    for (int n = 0; n < NR; ++n)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            vis[m][h] = 0xffffu;
-                            if (!full) {
+                        for (int e = 0; e < 2; ++e) {
+                            vis[n][e] = 0xffffu;
+                            if (masked) {
                                 uint64_t w = valid >= 64 ? ~0ull : (1ull << valid) - 1;
                                 if (draft) {
-                                    const int t = t_of[m][h];
+                                    const int t = t_of[n][e];
                                     w &= t < 0 ? 0ull
                                          : a.ancestors ? __ldg(a.ancestors + (long long)b * a.n_draft + t) >> d0
                                                        : (t >= 63 ? ~0ull : (2ull << t) - 1) >> d0;
                                 }
-                                vis[m][h] = (uint32_t)(w >> key0) & 0xffffu;
+                                vis[n][e] = (uint32_t)(w >> key0) & 0xffffu;
                             }
                         }
+                    bool above = false;
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        float tm[2] = {-INFINITY, -INFINITY};
+                    for (int n = 0; n < NR; ++n) {
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                        for (int i = 0; i < 4; ++i) {
+                            s[n][i] = score(s[n][i]);
+                            if (masked && !((vis[n][i & 1] >> (kq + 8 * (i >> 1))) & 1u)) s[n][i] = -INFINITY;
+                        }
+                        above = above || fmaxf(s[n][0], s[n][2]) > mx[n][0] + 8.0f || fmaxf(s[n][1], s[n][3]) > mx[n][1] + 8.0f;
+                    }
+                    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float v = score(s[m][n][i]);
-                                if (!full && !((vis[m][i >> 1] >> (8 * n + 2 * c + (i & 1))) & 1u)) v = -INFINITY;
-                                s[m][n][i] = v;
-                                tm[i >> 1] = fmaxf(tm[i >> 1], v);
+                        for (int n = 0; n < NR; ++n) {
+                            float f[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float m = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+                                for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                                m = fmaxf(m, mx[n][e]);
+                                f[e] = m == -INFINITY ? 1.0f : ex2(mx[n][e] - m);
+                                mx[n][e] = m;
+                                sum[n][e] *= f[e];
                             }
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            tm[h] = fmaxf(tm[h], __shfl_xor_sync(0xffffffffu, tm[h], 1));
-                            tm[h] = fmaxf(tm[h], __shfl_xor_sync(0xffffffffu, tm[h], 2));
-                        }
-                        const float m0 = fmaxf(mx[m][0], tm[0]), m1 = fmaxf(mx[m][1], tm[1]);
-                        const float u0 = m0 == -INFINITY ? 0.0f : m0, u1 = m1 == -INFINITY ? 0.0f : m1;
-                        if (__any_sync(0xffffffffu, m0 != mx[m][0] || m1 != mx[m][1])) {
-                            const float f0 = ex2(mx[m][0] - u0), f1 = ex2(mx[m][1] - u1);
-                            sum[m][0] *= f0;
-                            sum[m][1] *= f1;
+                            for (int ds = 0; ds < KS; ++ds)
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                o[m][nt][0] *= f0;
-                                o[m][nt][1] *= f0;
-                                o[m][nt][2] *= f1;
-                                o[m][nt][3] *= f1;
-                            }
-                            mx[m][0] = m0;
-                            mx[m][1] = m1;
-                        }
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            s[m][n][0] = ex2(s[m][n][0] - u0);
-                            s[m][n][1] = ex2(s[m][n][1] - u0);
-                            s[m][n][2] = ex2(s[m][n][2] - u1);
-                            s[m][n][3] = ex2(s[m][n][3] - u1);
-                            sum[m][0] += s[m][n][0] + s[m][n][1];
-                            sum[m][1] += s[m][n][2] + s[m][n][3];
+                                for (int i = 0; i < 4; ++i) o[n][ds][i] *= f[i & 1];
                         }
                     }
-                    // ---- O += P V ----
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        const float u0 = mx[n][0] == -INFINITY ? 0.0f : mx[n][0], u1 = mx[n][1] == -INFINITY ? 0.0f : mx[n][1];
+                        s[n][0] = ex2(s[n][0] - u0);
+                        s[n][1] = ex2(s[n][1] - u1);
+                        s[n][2] = ex2(s[n][2] - u0);
+                        s[n][3] = ex2(s[n][3] - u1);
+                        sum[n][0] += s[n][0] + s[n][2];
+                        sum[n][1] += s[n][1] + s[n][3];
+                    }
+                    // ---- O^T += V^T P^T ----
                     if (!v_ready) {
                         ok = mbar_wait(smem_addr(&sh.full_v[st]), par, abort, kWait);
                         if (!ok) {
@@ -390,63 +442,61 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
                         __syncwarp();
                     }
                     if constexpr (!Q8) {
-                        uint32_t p[MT][4];
+                        uint32_t p[NR][2];
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            p[m][0] = pack_bf16(s[m][0][0], s[m][0][1]);
-                            p[m][1] = pack_bf16(s[m][0][2], s[m][0][3]);
-                            p[m][2] = pack_bf16(s[m][1][0], s[m][1][1]);
-                            p[m][3] = pack_bf16(s[m][1][2], s[m][1][3]);
+                        for (int n = 0; n < NR; ++n) {
+                            p[n][0] = movmatrix_trans(pack_bf16(s[n][0], s[n][1]));
+                            p[n][1] = movmatrix_trans(pack_bf16(s[n][2], s[n][3]));
                         }
 #pragma unroll
                         for (int ds = 0; ds < KS; ++ds) {
                             uint32_t vf[4];
-                            load_v_step<D>(sv, key0, ds, lane, vf);
+                            load_v_cols<D>(sv, key0, ds, lane, vf);
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) {
-                                mma_bf16(o[m][2 * ds], p[m], vf[0], vf[1]);
-                                mma_bf16(o[m][2 * ds + 1], p[m], vf[2], vf[3]);
-                            }
+                            for (int n = 0; n < NR; ++n) mma_bf16(o[n][ds], vf, p[n][0], p[n][1]);
                         }
                     } else {
+                        constexpr int G = D / 32;
                         const int kr[4] = {key0 + 2 * c, key0 + 2 * c + 1, key0 + 2 * c + 8, key0 + 2 * c + 9};
+                        uint32_t sc0[(G + 1) / 2], sc1[(G + 1) / 2];
+                        if (!draft) {
+                            load_scales<G>(sv + TileCfg<D, Q8>::SCALES + (key0 + kq) * G * 2, sc0);
+                            load_scales<G>(sv + TileCfg<D, Q8>::SCALES + (key0 + kq + 8) * G * 2, sc1);
+                        }
 #pragma unroll
-                        for (int gr = 0; gr < D / 32; ++gr) {
-                            uint32_t b0[4], b1[4];  // operands of the group's four 8-column tiles
-                            float sc[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+                        for (int gr = 0; gr < G; ++gr) {
+                            uint32_t v0[4], v1[4];  // operands of the group's two 16-column steps
+                            float f0 = 1.0f, f1 = 1.0f;
                             if (draft) {
                                 uint2 w[4];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) w[k] = lds64(sv + kr[k] * C::DROW + (32 * gr + 4 * rq0) * 2);
-                                b0[0] = __byte_perm(w[0].x, w[1].x, 0x5410);
-                                b0[1] = __byte_perm(w[0].x, w[1].x, 0x7632);
-                                b0[2] = __byte_perm(w[0].y, w[1].y, 0x5410);
-                                b0[3] = __byte_perm(w[0].y, w[1].y, 0x7632);
-                                b1[0] = __byte_perm(w[2].x, w[3].x, 0x5410);
-                                b1[1] = __byte_perm(w[2].x, w[3].x, 0x7632);
-                                b1[2] = __byte_perm(w[2].y, w[3].y, 0x5410);
-                                b1[3] = __byte_perm(w[2].y, w[3].y, 0x7632);
+                                for (int k = 0; k < 4; ++k) w[k] = lds64(sv + kr[k] * C::DROW + (32 * gr + 4 * kq) * 2);
+                                v0[0] = __byte_perm(w[0].x, w[1].x, 0x5410);
+                                v0[1] = __byte_perm(w[0].x, w[1].x, 0x7632);
+                                v0[2] = __byte_perm(w[2].x, w[3].x, 0x5410);
+                                v0[3] = __byte_perm(w[2].x, w[3].x, 0x7632);
+                                v1[0] = __byte_perm(w[0].y, w[1].y, 0x5410);
+                                v1[1] = __byte_perm(w[0].y, w[1].y, 0x7632);
+                                v1[2] = __byte_perm(w[2].y, w[3].y, 0x5410);
+                                v1[3] = __byte_perm(w[2].y, w[3].y, 0x7632);
                             } else {
                                 uint32_t w[4];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    w[k] = lds32(sv + q8_qs_off(kr[k], 32 * gr + 4 * rq0, D));
-                                    sc[k] = lds_f16(sv + TileCfg<D, Q8>::SCALES + (kr[k] * (D / 32) + gr) * 2);
-                                }
-                                int8x4_to_bf16(__byte_perm(w[0], w[1], 0x5140), b0[0], b0[1]);
-                                int8x4_to_bf16(__byte_perm(w[0], w[1], 0x7362), b0[2], b0[3]);
-                                int8x4_to_bf16(__byte_perm(w[2], w[3], 0x5140), b1[0], b1[1]);
-                                int8x4_to_bf16(__byte_perm(w[2], w[3], 0x7362), b1[2], b1[3]);
+                                for (int k = 0; k < 4; ++k) w[k] = lds32(sv + q8_qs_off(kr[k], 32 * gr + 4 * kq, D));
+                                int8x4_to_bf16(__byte_perm(w[0], w[1], 0x5140), v0[0], v0[1]);
+                                int8x4_to_bf16(__byte_perm(w[2], w[3], 0x5140), v0[2], v0[3]);
+                                int8x4_to_bf16(__byte_perm(w[0], w[1], 0x7362), v1[0], v1[1]);
+                                int8x4_to_bf16(__byte_perm(w[2], w[3], 0x7362), v1[2], v1[3]);
+                                f0 = scale_of(sc0, gr);
+                                f1 = scale_of(sc1, gr);
                             }
                             // the values' scales ride on the probabilities, which are rounded once either way
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) {
-                                const uint32_t p[4] = {pack_bf16(s[m][0][0] * sc[0], s[m][0][1] * sc[1]),
-                                                       pack_bf16(s[m][0][2] * sc[0], s[m][0][3] * sc[1]),
-                                                       pack_bf16(s[m][1][0] * sc[2], s[m][1][1] * sc[3]),
-                                                       pack_bf16(s[m][1][2] * sc[2], s[m][1][3] * sc[3])};
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) mma_bf16(o[m][4 * gr + e], p, b0[e], b1[e]);
+                            for (int n = 0; n < NR; ++n) {
+                                const uint32_t p0 = movmatrix_trans(pack_bf16(s[n][0] * f0, s[n][1] * f0));
+                                const uint32_t p1 = movmatrix_trans(pack_bf16(s[n][2] * f1, s[n][3] * f1));
+                                mma_bf16(o[n][2 * gr], v0, p0, p1);
+                                mma_bf16(o[n][2 * gr + 1], v1, p0, p1);
                             }
                         }
                     }
@@ -457,25 +507,17 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
                             bad &= bad - 1;
                             const uint16_t *v = a.v_draft + kv_row + (long long)(d0 + key0 + k) * hk * D;
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) {
+                            for (int n = 0; n < NR; ++n) {
                                 float pk[2];
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    float mine = 0.0f;
+                                for (int e = 0; e < 2; ++e)
+                                    pk[e] = __shfl_sync(0xffffffffu, k < 8 ? s[n][e] : s[n][e + 2], (k & 7) * 4 + c);
 #pragma unroll
-                                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                                        for (int e = 0; e < 2; ++e)
-                                            if (8 * n + 2 * c + e == k) mine = s[m][n][2 * h + e];
-                                    pk[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) | ((k & 7) >> 1));
-                                }
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
+                                for (int ds = 0; ds < KS; ++ds)
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) {
-                                        const float x = bf16_bits_to_f32(__ldg(v + o_col<Q8>(nt, c, i)));
-                                        if (!isfinite(x) && ((vis[m][i >> 1] >> k) & 1u))
-                                            o[m][nt][i] = fmaf(pk[i >> 1], x, o[m][nt][i]);
+                                        const float y = bf16_bits_to_f32(__ldg(v + o_col<Q8>(ds, kq, i)));
+                                        if (!isfinite(y) && ((vis[n][i & 1] >> k) & 1u)) o[n][ds][i] = fmaf(pk[i & 1], y, o[n][ds][i]);
                                     }
                             }
                         }
@@ -490,22 +532,24 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
             }
 
             // ---- join the key groups, write the rows ----
-            float scale_o[MT][2], l_tot[MT][2], m_tot[MT][2];
+            float scale_o[NR][2], l_tot[NR][2], m_tot[NR][2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float l = sum[m][h];
-                    l += __shfl_xor_sync(0xffffffffu, l, 1);
-                    l += __shfl_xor_sync(0xffffffffu, l, 2);
-                    if (c == 0) sml[wk * C::ROWS + (wr * MT + m) * 16 + rq0 + 8 * h] = make_float2(mx[m][h], l);
+                for (int e = 0; e < 2; ++e) {
+                    float l = sum[n][e];
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+                    if (kq == 0) sml[wk * C::ROWS + wrow + 8 * n + 2 * c + e] = make_float2(mx[n][e], l);
                 }
             asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
+            const bool whole = t0 == 0 && t1 == n_tiles;
+            const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = (wr * MT + m) * 16 + rq0 + 8 * h;
+                for (int e = 0; e < 2; ++e) {
+                    const int r = wrow + 8 * n + 2 * c + e;
                     float mt = -INFINITY, lt = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WK; ++w) mt = fmaxf(mt, sml[w * C::ROWS + r].x);
@@ -515,60 +559,40 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
                         const float2 ml = sml[w * C::ROWS + r];
                         lt += ml.y * ex2(ml.x - mu);
                     }
-                    m_tot[m][h] = mt;
-                    l_tot[m][h] = lt;
-                    scale_o[m][h] = ex2(mx[m][h] - mu);
-                }
-            const bool whole = t0 == 0 && t1 == n_tiles;
-            const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
-            if (wk == 0 && c == 0) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = (wr * MT + m) * 16 + rq0 + 8 * h;
-                        if (r >= rows) continue;
-                        if (whole) {
-                            if (a.lse) {
-                                const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
-                                const bool none = t_of[m][h] < 0 || l_tot[m][h] == 0.0f;
-                                a.lse[((long long)b * a.n_draft + t) * a.q_heads + hq] =
-                                    none ? -INFINITY : (m_tot[m][h] + __log2f(l_tot[m][h])) * 0.6931471805599453f;
-                            }
-                        } else {
-                            a.ws_ml[slot * C::ROWS + r] = make_float2(t_of[m][h] < 0 ? -INFINITY : m_tot[m][h],
-                                                                      t_of[m][h] < 0 ? 0.0f : l_tot[m][h]);
-                        }
+                    m_tot[n][e] = mt;
+                    l_tot[n][e] = lt;
+                    scale_o[n][e] = mx[n][e] == -INFINITY ? 0.0f : ex2(mx[n][e] - mu);
+                    if (whole) scale_o[n][e] = lt == 0.0f ? 0.0f : scale_o[n][e] / lt;
+                    if (wk != 0 || kq != 0 || r >= rows) continue;
+                    const bool off = t_of[n][e] < 0;
+                    if (!whole) {
+                        a.ws_ml[slot * C::ROWS + r] = off ? make_float2(-INFINITY, 0.0f) : make_float2(mt, lt);
+                    } else if (a.lse) {
+                        const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
+                        a.lse[((long long)b * a.n_draft + t) * a.q_heads + hq] =
+                            off || lt == 0.0f ? -INFINITY : (mt + __log2f(lt)) * 0.6931471805599453f;
                     }
-            }
+                }
             if (a.split && threadIdx.x == 0 && t0 == 0) {
                 const long long unit0 = base + (long long)u * n_tiles, last = unit0 + n_tiles - 1;
-                a.parts[b * units_per_req + u] =
-                    make_int2(blockIdx.x, (int)(((last + 1) * rg.ctas - 1) / rg.total));
+                a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)(((last + 1) * rg.ctas - 1) / rg.total));
             }
-            // rows' final factor: 1 / sum for whole units, none for parts
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (whole) scale_o[m][h] = l_tot[m][h] == 0.0f ? 0.0f : scale_o[m][h] / l_tot[m][h];
-                }
 #pragma unroll
             for (int cc = 0; cc < (D + kXCols - 1) / kXCols; ++cc) {
                 const int cols = min(kXCols, D - cc * kXCols);
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int n4 = 0; n4 < 4; ++n4) {
-                        const int nt = cc * 4 + n4;
-                        if (nt >= NT) continue;
+                    for (int d2 = 0; d2 < 2; ++d2) {
+                        const int ds = cc * 2 + d2;
+                        if (ds >= KS) continue;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int r = (wr * MT + m) * 16 + rq0 + 8 * (i >> 1);
-                            const int col = o_col<Q8>(nt, c, i) - cc * kXCols;
-                            // a row without keys of this warp has factor 0 (or 0 / 0 were there none at all)
-                            const float v = mx[m][i >> 1] == -INFINITY ? 0.0f : o[m][nt][i] * scale_o[m][i >> 1];
-                            xb[(wk * C::ROWS + r) * kXCols + ((col + 4 * r) & (kXCols - 1))] = v;
+                            const int r = wrow + 8 * n + 2 * c + (i & 1);
+                            const int col = o_col<Q8>(ds, kq, i) - cc * kXCols;
+                            // a warp without a key for the row has nothing (not 0 * its garbage)
+                            const float f = scale_o[n][i & 1];
+                            xb[(wk * C::ROWS + r) * kXCols + ((col + 4 * r) & (kXCols - 1))] = f == 0.0f ? 0.0f : o[n][ds][i] * f;
                         }
                     }
                 asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
@@ -603,11 +627,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, MT, WR, WK>::THREADS, Cfg<D, Q8, MT
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 7);
     if (warp == C::NW && !ok && lane == 0) {
         // leave no copy writing this CTA's shared memory: the last uses of every stage that were issued
-        for (int st = 0; st < NST; ++st) {
-            mbar_wait_drain(smem_addr(&sh.full_k[st]), 0, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.full_k[st]), 1, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.full_v[st]), 0, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.full_v[st]), 1, kWait / 64);
+        for (int i = 0; i < NST; ++i) {
+            mbar_wait_drain(smem_addr(&sh.full_k[i]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full_k[i]), 1, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full_v[i]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full_v[i]), 1, kWait / 64);
         }
     }
 }
@@ -620,6 +644,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
     const int rows_all = a.n_draft * a.group;
     const int row = blockIdx.x % rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
     const int bg = blockIdx.x / rows_all, b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
+    grid_wait();
     const int2 part = a.parts[bg * a.row_tiles + rt];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (part.x == part.y) return;
@@ -674,25 +699,28 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
 }
 
 // ---- host side ----
-// Row tiles: 16 rows are one warp's registers (32 up to head_dim 128); more rows take four warps' rows, so
-// that a tile of keys is read from shared memory once per 64 rows.
-enum class Shape { R16, R32, R64 };
+// Row tiles: a warp holds 8, 16 or (up to head_dim 128) 32 rows; more rows take four warps' 16, so that a tile
+// of keys is read from memory once per 64 rows.
+enum class Shape { R8, R16, R32, R64 };
 
 Shape shape_for(int head_dim, int rows) {
+    if (rows <= 8) return Shape::R8;
     if (rows <= 16) return Shape::R16;
     if (rows <= 32 && head_dim <= 128) return Shape::R32;
     return Shape::R64;
 }
-int tile_rows(Shape s) { return s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64; }
+int tile_rows(Shape s) { return s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64; }
 
-int ctas_per_sm(Shape s, int head_dim) { return rows_ctas(head_dim, s == Shape::R32 ? 2 : 1); }
+int ctas_per_sm(Shape s, int head_dim, bool q8) {
+    return rows_ctas(head_dim, q8, s == Shape::R8 ? 1 : s == Shape::R32 ? 4 : 2, s == Shape::R64 ? 4 : 1);
+}
 
 struct WsLayout {
     size_t parts, ml, o, total;
 };
 WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
     const Shape sh = shape_for(p.head_dim, rows);
-    const size_t slots = 2ull * sms * ctas_per_sm(sh, p.head_dim) * tile_rows(sh);
+    const size_t slots = 2ull * sms * ctas_per_sm(sh, p.head_dim, p.dtype == EKV_DTYPE_Q8_0) * tile_rows(sh);
     WsLayout w;
     w.parts = 0;
     w.ml = ((size_t)n_batch * p.kv_heads * rt * sizeof(int2) + 255) / 256 * 256;
@@ -701,26 +729,23 @@ WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
     return w;
 }
 
-template <int D, bool Q8, int MT, int WR, int WK>
+template <int D, bool Q8, int NR, int WR, int WK>
 int launch_rows(const TreeArgs &a, int grid, cudaStream_t s) {
-    using C = Cfg<D, Q8, MT, WR, WK>;
-    auto k = tree_rows_kernel<D, Q8, MT, WR, WK>;
-    // the base is rounded up to 1024 bytes inside the kernel
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return EKV_ERR_CUDA;
-    k<<<grid, C::THREADS, C::SMEM, s>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    note_launches(1);
-    return EKV_OK;
+    using C = Cfg<D, Q8, NR, WR, WK>;
+    static std::atomic<uint64_t> smem_done{0};
+    if (const int rc = allow_smem(tree_rows_kernel<D, Q8, NR, WR, WK>, C::SMEM, smem_done)) return rc;
+    return launch_after(tree_rows_kernel<D, Q8, NR, WR, WK>, grid, C::THREADS, C::SMEM, s, a);
 }
 
 template <int D, bool Q8>
 int launch_shape(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     switch (sh) {
-        case Shape::R16: return launch_rows<D, Q8, 1, 1, 4>(a, grid, s);
+        case Shape::R8: return launch_rows<D, Q8, 1, 1, 4>(a, grid, s);
+        case Shape::R16: return launch_rows<D, Q8, 2, 1, 4>(a, grid, s);
         case Shape::R32:
-            if constexpr (D <= 128) return launch_rows<D, Q8, 2, 1, 4>(a, grid, s);
+            if constexpr (D <= 128) return launch_rows<D, Q8, 4, 1, 4>(a, grid, s);
             return EKV_ERR_UNSUPPORTED;
-        default: return launch_rows<D, Q8, 1, 4, 1>(a, grid, s);
+        default: return launch_rows<D, Q8, 2, 4, 1>(a, grid, s);
     }
 }
 
@@ -735,10 +760,8 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     }
     if (rc || !a.split) return rc;
     const int rows = a.n_draft * a.group;
-    tree_merge_kernel<D><<<a.n_batch * a.pool.kv_heads * rows, kMergeWarps * 32, 0, s>>>(a, tile_rows(sh));
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    note_launches(1);
-    return EKV_OK;
+    return launch_after(tree_merge_kernel<D>, a.n_batch * a.pool.kv_heads * rows, kMergeWarps * 32, 0, s, a,
+                        tile_rows(sh));
 }
 
 }  // namespace
@@ -758,7 +781,7 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
     const WsLayout w = ws_layout(a.pool, a.n_batch, rows, a.row_tiles, sms);
     const int64_t unit_tiles = (max_len + kTile - 1) / kTile + 1;
-    const int full = sms * ctas_per_sm(sh, a.pool.head_dim);
+    const int full = sms * ctas_per_sm(sh, a.pool.head_dim, a.pool.dtype == EKV_DTYPE_Q8_0);
     // Units of one or two tiles are not worth a second launch; without a workspace a unit is one CTA's.
     a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2;
     int64_t grid = units;

@@ -3,6 +3,7 @@
 // with the scores s and the lse of ekv_tree_attention. Every key's sum is one CTA's, in a fixed order: no
 // atomics, the same result every time. K is read once, V not at all.
 #include <algorithm>
+#include <type_traits>
 
 #include "ekv_decode.cuh"
 
@@ -14,43 +15,46 @@ using namespace sm100;
 
 constexpr int kWarps = 4;  // 16 keys of a 64-key tile each
 constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kMaxStages = 8;
 
 template <int D, bool Q8>
 struct WCfg {
     using T = TileCfg<D, Q8>;
     static constexpr int STAGE = (T::KV_BYTES + 1023) / 1024 * 1024;
-    static constexpr int NST_64K = 65536 / STAGE;
-    static constexpr int NST = NST_64K < 3 ? 3 : NST_64K > 8 ? 8 : NST_64K;
-    static constexpr int QROW = 2 * D + 16;                  // bytes of a query row in shared memory
+    static constexpr int QROW = q_row_bytes<D>();
     static constexpr int QROWS = D > 128 ? 128 : 256;        // query rows held at a time
-    static constexpr int smem(int rows) { return NST * STAGE + rows * (QROW + 4) + 1024 + 1024; }
+    // two CTAs per SM: what their query rows leave of half an SM's shared memory holds tiles in flight
+    static constexpr int fixed(int rows) { return rows * (QROW + 4) + 1024 + 1024; }
+    static constexpr int stages(int rows) {
+        const int n = (112 * 1024 - fixed(rows)) / STAGE;
+        return n < 2 ? 2 : n > kMaxStages ? kMaxStages : n;
+    }
+    static constexpr int smem(int rows) { return stages(rows) * STAGE + fixed(rows); }
 };
 
-template <int NST>
 struct WShared {
-    uint64_t full[NST], empty[NST];
+    uint64_t full[kMaxStages], empty[kMaxStages];
     RangeScratch range;
     int abort;
 };
 
 template <int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs a, int q_rows) {
+__global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs a, int q_rows, int nst) {
     using C = WCfg<D, Q8>;
     using T = TileCfg<D, Q8>;
-    constexpr int NST = C::NST, KS = D / 16;
+    constexpr int KS = D / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    using Sh = WShared<NST>;
-    static_assert(sizeof(Sh) <= 1024, "barrier block");
-    Sh &sh = *(Sh *)(smem + NST * C::STAGE);
-    uint8_t *sq = smem + NST * C::STAGE + 1024;           // [q_rows] rows of C::QROW bytes
+    static_assert(sizeof(WShared) <= 1024, "barrier block");
+    WShared &sh = *(WShared *)(smem + nst * C::STAGE);
+    uint8_t *sq = smem + nst * C::STAGE + 1024;           // [q_rows] rows of C::QROW bytes
     float *slse = (float *)(sq + q_rows * C::QROW);       // [q_rows] lse in the log2 domain
     volatile int *abort = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int hk = a.pool.kv_heads, rows_all = a.n_draft * a.group;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NST; ++i) {
+        for (int i = 0; i < nst; ++i) {
             mbar_init(smem_addr(&sh.full[i]), 1);
             mbar_init(smem_addr(&sh.empty[i]), kWarps);
         }
@@ -65,11 +69,18 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
         }
         return r;
     };
+    grid_wait();
     const Range rg = find_range<kThreads>(a.n_batch, hk, sh.range, [&](int b) {
         return (request(b, false).n_prefix + kTile - 1) / kTile;
     });
 
-    int it = 0;
+    int st = 0, turn = 0;  // stage of the next tile, and how often the ring went round
+    auto advance = [&]() {
+        if (++st == nst) {
+            st = 0;
+            ++turn;
+        }
+    };
     bool ok = true;
     int b = rg.b;
     long long base = rg.base;
@@ -91,11 +102,10 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
             if (warp == kWarps) {
                 // ---- feeder ----
                 Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
-                for (int j = t0; j < t1; ++j, ++it) {
-                    const int st = it % NST;
+                for (int j = t0; j < t1; ++j, advance()) {
                     const Piece pc = next;
                     if (j + 1 < t1) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
-                    if (it >= NST) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), ((it / NST) - 1) & 1, abort, kWait);
+                    if (turn > 0) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort, kWait);
                     if (!ok) {
                         *abort = 1;
                         continue;
@@ -113,18 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 if (row < rows_all && t < rq.n_nodes)
                     v = __ldg((const uint4 *)(a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row -
                                                      t * a.group) * D) + u);
-                uint8_t *dst = sq + r * C::QROW;
-                if (Q8) {
-                    // columns 32 g + 8 c + 4 i + 2 h + {0, 1} go to place 32 g + 16 i + 2 c + 8 h
-                    const int g32 = u >> 2, cc = u & 3;
-                    uint32_t *d32 = (uint32_t *)(dst + 64 * g32);
-                    d32[cc] = v.x;
-                    d32[cc + 4] = v.y;
-                    d32[cc + 8] = v.z;
-                    d32[cc + 12] = v.w;
-                } else {
-                    *(uint4 *)(dst + 16 * u) = v;
-                }
+                store_q_unit<Q8>(sq + r * C::QROW, u, v);
             }
             for (int r = threadIdx.x; r < rows; r += kWarps * 32) {
                 const int row = c0 + r, t = row / a.group;
@@ -141,13 +140,19 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
             const int key_l = 16 * warp + 8 * ((rq0 >> 1) & 1) + 2 * c + (rq0 & 1);  // the key this lane writes (rq0 < 4)
             float *wrow = a.weights + ((long long)b * hk + g) * a.weight_stride;
-            for (int j = t0; j < t1; ++j, ++it) {
-                const int st = it % NST, par = (it / NST) & 1;
+            // the entry this lane adds to, a tile ahead
+            auto load_old = [&](int j) {
+                const int key = j * kTile + key_l;
+                return rq0 < 4 && key < rq.n_prefix && j < t1 && (c0 > 0 || a.decay != 0.0f) ? wrow[key] : 0.0f;
+            };
+            float next_old = load_old(t0);
+            for (int j = t0; j < t1; ++j, advance()) {
+                const int par = turn & 1;
                 const uint32_t sk = smem_addr(smem + st * C::STAGE);
                 const int key = j * kTile + key_l;
                 const bool writes = rq0 < 4 && key < rq.n_prefix;
-                float old = 0.0f;
-                if (writes && (c0 > 0 || a.decay != 0.0f)) old = wrow[key] * (c0 > 0 ? 1.0f : a.decay);
+                const float old = next_old;
+                next_old = load_old(j + 1);
                 ok = ok && mbar_wait(smem_addr(&sh.full[st]), par, abort, kWait);
                 if (!ok) {
                     *abort = 1;
@@ -155,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 }
                 const int key0 = 16 * warp;
                 uint32_t kf[KS][4];
+                float sc[Q8 ? KS / 2 : 1][2][2];  // scales of the lane's keys by group
                 if constexpr (!Q8) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) load_k_step<D>(sk, key0, ks, lane, kf[ks]);
@@ -166,67 +172,82 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                             const uint2 w = lds64(sk + q8_qs_off(key0 + 8 * n + rq0, 32 * gr + 8 * c, D));
                             int8x4_to_bf16(w.x, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
                             int8x4_to_bf16(w.y, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
+                            const int krow = key0 + 8 * n + 2 * c;
+                            sc[gr][n][0] = lds_f16(sk + T::SCALES + (krow * T::G32 + gr) * 2);
+                            sc[gr][n][1] = lds_f16(sk + T::SCALES + ((krow + 1) * T::G32 + gr) * 2);
                         }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.empty[st]));  // the keys are in registers
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys (n, e): 8 n + 2 c + e, rows of this lane
-                for (int r0 = 0; r0 < rows; r0 += 16) {
-                    float s[2][4];
+                // two 16-row tiles at a time: their products do not wait for one another
+                auto row_tiles = [&](auto count, int r0) {
+                    constexpr int M = decltype(count)::value;
+                    float s[M][2][4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int m = 0; m < M; ++m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.0f;
                     const uint32_t qa = smem_addr(sq) + (r0 + (lane & 15)) * C::QROW + (lane >> 4) * 16;
                     if constexpr (!Q8) {
 #pragma unroll
-                        for (int ks = 0; ks < KS; ++ks) {
-                            uint32_t qf[4];
-                            ldmatrix_x4(qf, qa + 32 * ks);
-                            mma_bf16(s[0], qf, kf[ks][0], kf[ks][1]);
-                            mma_bf16(s[1], qf, kf[ks][2], kf[ks][3]);
-                        }
+                        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                            for (int m = 0; m < M; ++m) {
+                                uint32_t qf[4];
+                                ldmatrix_x4(qf, qa + m * 16 * C::QROW + 32 * ks);
+                                mma_bf16(s[m][0], qf, kf[ks][0], kf[ks][1]);
+                                mma_bf16(s[m][1], qf, kf[ks][2], kf[ks][3]);
+                            }
                     } else {
 #pragma unroll
-                        for (int gr = 0; gr < KS / 2; ++gr) {
-                            uint32_t q0[4], q1[4];
-                            ldmatrix_x4(q0, qa + 64 * gr);
-                            ldmatrix_x4(q1, qa + 64 * gr + 32);
+                        for (int gr = 0; gr < KS / 2; ++gr)
 #pragma unroll
-                            for (int n = 0; n < 2; ++n) {
-                                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma_bf16(p, q0, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
-                                mma_bf16(p, q1, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
-                                const int krow = key0 + 8 * n + 2 * c;
-                                const float s0 = lds_f16(sk + T::SCALES + (krow * T::G32 + gr) * 2);
-                                const float s1 = lds_f16(sk + T::SCALES + ((krow + 1) * T::G32 + gr) * 2);
-                                s[n][0] = fmaf(p[0], s0, s[n][0]);
-                                s[n][1] = fmaf(p[1], s1, s[n][1]);
-                                s[n][2] = fmaf(p[2], s0, s[n][2]);
-                                s[n][3] = fmaf(p[3], s1, s[n][3]);
+                            for (int m = 0; m < M; ++m) {
+                                uint32_t q0[4], q1[4];
+                                ldmatrix_x4(q0, qa + m * 16 * C::QROW + 64 * gr);
+                                ldmatrix_x4(q1, qa + m * 16 * C::QROW + 64 * gr + 32);
+#pragma unroll
+                                for (int n = 0; n < 2; ++n) {
+                                    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                    mma_bf16(p, q0, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
+                                    mma_bf16(p, q1, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
+                                    s[m][n][0] = fmaf(p[0], sc[gr][n][0], s[m][n][0]);
+                                    s[m][n][1] = fmaf(p[1], sc[gr][n][1], s[m][n][1]);
+                                    s[m][n][2] = fmaf(p[2], sc[gr][n][0], s[m][n][2]);
+                                    s[m][n][3] = fmaf(p[3], sc[gr][n][1], s[m][n][3]);
+                                }
                             }
-                        }
                     }
-                    const float l0 = slse[r0 + rq0], l1 = slse[r0 + rq0 + 8];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int m = 0; m < M; ++m) {
+                        const float l0 = slse[r0 + 16 * m + rq0], l1 = slse[r0 + 16 * m + rq0 + 8];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            acc[2 * n + e] += ex2(score(s[n][e]) - l0) + ex2(score(s[n][2 + e]) - l1);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.empty[st]));
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                acc[2 * n + e] += ex2(score(s[m][n][e]) - l0) + ex2(score(s[m][n][2 + e]) - l1);
+                    }
+                };
+                int r0 = 0;
+#pragma unroll 1
+                for (; r0 + 32 <= rows; r0 += 32) row_tiles(std::integral_constant<int, 2>(), r0);
+                if (r0 < rows) row_tiles(std::integral_constant<int, 1>(), r0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int m = 4; m < 32; m <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], m);
                 const float mine = rq0 & 2 ? (rq0 & 1 ? acc[3] : acc[2]) : (rq0 & 1 ? acc[1] : acc[0]);
-                if (writes) wrow[key] = old + mine;
+                if (writes) wrow[key] = old * (c0 > 0 ? 1.0f : a.decay) + mine;
             }
         }
         x += t1 - t0;
     }
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 8);
     if (warp == kWarps && !ok && lane == 0) {
-        for (int st = 0; st < NST; ++st) {  // leave no copy writing this CTA's shared memory
+        for (int st = 0; st < nst; ++st) {  // leave no copy writing this CTA's shared memory
             mbar_wait_drain(smem_addr(&sh.full[st]), 0, kWait / 64);
             mbar_wait_drain(smem_addr(&sh.full[st]), 1, kWait / 64);
         }
@@ -239,16 +260,12 @@ int launch(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
     const int64_t rows = (int64_t)a.n_draft * a.group;
     const int q_rows = (int)std::min<int64_t>((rows + 15) / 16 * 16, C::QROWS);
     const int smem = C::smem(q_rows);
-    auto k = key_weights_kernel<D, Q8>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(C::QROWS)) != cudaSuccess)
-        return EKV_ERR_CUDA;
+    static std::atomic<uint64_t> smem_done{0};
+    if (const int rc = allow_smem(key_weights_kernel<D, Q8>, 227 * 1024, smem_done)) return rc;
     const int64_t tiles = (int64_t)a.n_batch * a.pool.kv_heads * ((max_len + kTile - 1) / kTile);
-    const int ctas = std::max(1, std::min(3, 226 * 1024 / (smem + 1024)));
+    const int ctas = smem > 112 * 1024 ? 1 : 2;
     const int grid = (int)std::min<int64_t>((int64_t)sms * ctas, std::max<int64_t>(1, tiles));
-    k<<<grid, kThreads, smem, s>>>(a, q_rows);
-    if (cudaGetLastError() != cudaSuccess) return EKV_ERR_CUDA;
-    note_launches(1);
-    return EKV_OK;
+    return launch_after(key_weights_kernel<D, Q8>, grid, kThreads, smem, s, a, q_rows, C::stages(q_rows));
 }
 
 template <int D>

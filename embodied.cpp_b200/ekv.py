@@ -218,13 +218,13 @@ def check(code, what="ekv"):
 
 
 def _ptr(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream(stream):
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    return s.cuda_stream
 
 
 @dataclass
