@@ -229,21 +229,25 @@ __device__ __forceinline__ Req load_req(const TreeArgs &a, int b, bool report) {
 
 // A flat order of all tiles of the call -- request, then unit (KV head, row tile), then tile -- is cut
 // into G = min(gridDim.x, T) equal ranges, whatever the requests' lengths: CTA c < G takes
-// [c T / G, (c + 1) T / G), at least one tile.
+// [c T / G, (c + 1) T / G), at least one tile. The launchers see to it that T < 2^31.
 struct Range {
-    long long total, lo, hi;  // T and this CTA's range
-    int ctas;                 // G
-    int b;                    // request that holds tile lo
-    long long base;           // first tile of request b
+    uint32_t total, lo, hi;  // T and this CTA's range
+    int ctas;                // G
+    int b;                   // request that holds tile lo
+    uint32_t base;           // first tile of request b
 };
 
 struct RangeScratch {
-    long long warp_sum[32];
-    long long base;
+    uint32_t warp_sum[32];
+    uint32_t base;
     int b;
 };
 
-__device__ __forceinline__ long long range_lo(long long total, int c, int g) { return total * c / g; }
+// floor(total * c / g) for c <= g <= 2^16, in 32 bits.
+__device__ __forceinline__ uint32_t range_lo(uint32_t total, uint32_t c, uint32_t g) {
+    const uint32_t q = total / g, r = total - q * g;
+    return c * q + c * r / g;
+}
 
 // All threads of the block (NT of them). tiles(b): tiles of one unit of request b.
 template <int NT, class Tiles>
@@ -251,49 +255,51 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = NT / 32;
     // inclusive scan of one chunk of NT requests; returns this thread's inclusive sum and the chunk's total
-    auto scan = [&](long long v, long long &chunk) {
+    auto scan = [&](uint32_t v, uint32_t &chunk) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         if (lane == 31) sh.warp_sum[warp] = v;
         __syncthreads();
-        long long before = 0;
+        uint32_t before = 0;
         chunk = 0;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const long long s = sh.warp_sum[w];
+            const uint32_t s = sh.warp_sum[w];
             if (w < warp) before += s;
             chunk += s;
         }
-        __syncthreads();
         return v + before;
     };
     Range r;
     r.total = 0;
-    long long v0 = tid < n_batch ? (long long)tiles(tid) * units_per_req : 0, incl0 = 0, chunk = 0;
+    const uint32_t v0 = tid < n_batch ? (uint32_t)(tiles(tid) * units_per_req) : 0u;
+    uint32_t incl0 = 0, chunk = 0;
     if (tid == 0) {
         sh.b = n_batch;
         sh.base = 0;
     }
     for (int b0 = 0; b0 < n_batch; b0 += NT) {
-        const long long v = b0 == 0 ? v0 : (b0 + tid < n_batch ? (long long)tiles(b0 + tid) * units_per_req : 0);
-        const long long incl = scan(v, chunk);
+        if (b0 > 0) __syncthreads();
+        const uint32_t v = b0 == 0 ? v0 : (b0 + tid < n_batch ? (uint32_t)(tiles(b0 + tid) * units_per_req) : 0u);
+        const uint32_t incl = scan(v, chunk);
         if (b0 == 0) incl0 = incl;
         r.total += chunk;
     }
-    r.ctas = (int)min((long long)gridDim.x, r.total);
+    r.ctas = (int)min(gridDim.x, r.total);
     r.lo = r.hi = r.total;
     if ((int)blockIdx.x < r.ctas) {
         r.lo = range_lo(r.total, blockIdx.x, r.ctas);
         r.hi = range_lo(r.total, blockIdx.x + 1, r.ctas);
     }
-    long long base = 0;
+    uint32_t base = 0;
     for (int b0 = 0; b0 < n_batch; b0 += NT) {
-        long long v = v0, incl = incl0;
+        uint32_t v = v0, incl = incl0;
         if (n_batch > NT) {
-            v = b0 + tid < n_batch ? (long long)tiles(b0 + tid) * units_per_req : 0;
+            __syncthreads();
+            v = b0 + tid < n_batch ? (uint32_t)(tiles(b0 + tid) * units_per_req) : 0u;
             incl = scan(v, chunk);
         }
         if (v > 0 && base + incl - v <= r.lo && r.lo < base + incl) {

@@ -29,6 +29,7 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
 }
 
 constexpr int kCopies = 4;   // histograms, by lane: weights share few exponents, so lanes meet in few bins
+constexpr int kList = 12288; // survivors listed in shared memory; where more move, each free slot searches for its own
 constexpr int kInRegs = 16;  // keys a thread keeps (16384 slots); longer rows are read again by each pass
 
 struct SelShared {
@@ -171,7 +172,8 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
 
     // ---- one bit per slot ----
     const int words = (n + 31) / 32;
-    uint32_t *sel = s_mem, *cnt = s_mem + a.max_words;  // chosen slots; ties, then survivors at or above keep before a word
+    uint32_t *sel = s_mem, *cnt = s_mem + a.max_words;  // chosen slots; ties, then free slots or survivors before a word
+    uint32_t *list = s_mem + 2 * a.max_words;           // [kList] survivors at or above keep
     each([&](int i, uint32_t k) {
         const uint32_t gt = __ballot_sync(0xffffffffu, i < n && (k & mask) > prefix);
         const uint32_t eq = __ballot_sync(0xffffffffu, i < n && (k & mask) == prefix);
@@ -208,35 +210,49 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     auto tail_bits = [&](int wd) {
         return wd < first_tail ? 0u : wd == first_tail ? sel[wd] & ~((1u << (a.keep & 31)) - 1u) : sel[wd];
     };
-    uint32_t tails = 0;
-    for (int w0 = first_tail; w0 < words; w0 += kSelThreads) {
+    // (cnt of a word below holds the free slots before it)
+    const uint32_t low_mask = (1u << (a.keep & 31)) - 1u;
+    uint32_t tails = 0, holes = 0;
+    for (int w0 = 0; w0 < words; w0 += kSelThreads) {
         const int wd = w0 + tid;
+        const uint32_t free_bits = wd >= words || wd > first_tail ? 0u : wd < first_tail ? ~sel[wd] : ~sel[wd] & low_mask;
+        const uint32_t tail = wd < words ? tail_bits(wd) : 0u;
         uint32_t total;
-        const uint32_t before = tails + block_scan(wd < words ? __popc(tail_bits(wd)) : 0u, sh, turn, total);
-        if (wd < words) cnt[wd] = before;
-        tails += total;
+        // both counts in one scan: each is at most 2^15 a round
+        const uint32_t before = block_scan(__popc(tail) << 16 | __popc(free_bits), sh, turn, total);
+        if (wd < words) cnt[wd] = wd <= first_tail ? holes + (before & 0xffffu) : tails + (before >> 16);
+        tails += total >> 16;
+        holes += total & 0xffffu;
     }
     __syncthreads();
-    // ---- free slots below keep, in order, take them ----
-    uint32_t holes = 0;
-    for (int i0 = 0; i0 < a.keep; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        const bool hole = i < a.keep && !((sel[i >> 5] >> (i & 31)) & 1u);
-        uint32_t total;
-        const uint32_t rank = holes + block_scan(hole ? 1u : 0u, sh, turn, total);
-        holes += total;
-        if (i >= a.keep) continue;
+    // ---- the survivors in order, and a free slot below keep for each ----
+    const bool listed = holes <= (uint32_t)kList;
+    if (listed) {
+        for (int i = (a.keep & ~31) + tid; i < 32 * words; i += kSelThreads) {
+            const int wd = i >> 5;
+            const uint32_t bits = tail_bits(wd);
+            if ((bits >> lane) & 1u) list[(wd == first_tail ? 0u : cnt[wd]) + __popc(bits & ((1u << lane) - 1u))] = i;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < a.keep; i += kSelThreads) {
+        const uint32_t chosen = sel[i >> 5];
         int from = i;
-        if (hole) {
-            int lo = first_tail, hi = words - 1;  // the last word with at most `rank` survivors before it
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (cnt[mid] <= rank) lo = mid;
-                else hi = mid - 1;
+        if (!((chosen >> (i & 31)) & 1u)) {
+            const uint32_t rank = cnt[i >> 5] + __popc(~chosen & ((1u << (i & 31)) - 1u));
+            if (listed) {
+                from = list[rank];
+            } else {
+                int lo = first_tail, hi = words - 1;  // the last word with at most `rank` survivors before it
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (cnt[mid] <= rank) lo = mid;
+                    else hi = mid - 1;
+                }
+                uint32_t bits = tail_bits(lo);
+                for (uint32_t k = rank - (lo == first_tail ? 0u : cnt[lo]); k; --k) bits &= bits - 1;
+                from = 32 * lo + __ffs(bits) - 1;
             }
-            uint32_t bits = tail_bits(lo);
-            for (uint32_t k = rank - cnt[lo]; k; --k) bits &= bits - 1;
-            from = 32 * lo + __ffs(bits) - 1;
         }
         kept[i] = from;
         const float wi = w[from];
@@ -325,9 +341,9 @@ int launch_evict(EvictArgs a, cudaStream_t s) {
     const int chunks = (a.keep + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
     if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
     a.max_words = (a.max_len + 31) / 32 + 1;
-    const size_t smem = (size_t)a.max_words * 2 * sizeof(uint32_t);
+    const size_t smem = ((size_t)a.max_words * 2 + kList) * sizeof(uint32_t);
     static std::atomic<uint64_t> smem_done{0};
-    if (const int rc = decode::allow_smem(evict_select_kernel, (EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 * (int)sizeof(uint32_t), smem_done))
+    if (const int rc = decode::allow_smem(evict_select_kernel, ((EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 + kList) * (int)sizeof(uint32_t), smem_done))
         return rc;
     if (const int rc = decode::launch_after(evict_select_kernel, (unsigned)n, kSelThreads, smem, s, a)) return rc;
     return decode::launch_after(evict_move_kernel, (unsigned)(n * chunks), kMoveWarps * 32, 0, s, a, chunks);

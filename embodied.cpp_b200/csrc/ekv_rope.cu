@@ -300,7 +300,8 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
     a.q_stride = q_stride;
     a.kv_stride = kv_stride;
     a.q_out = (uint16_t *)q_out;
-    a.rows_per_cta = (int)std::min<int64_t>(kMaxRows, std::max<int64_t>(1, (int64_t)max_rows * n_batch / (8 * sms)));
+    // as few rows as leave one wave of CTAs (4 per SM): a CTA's chain of dependent loads is not paid twice
+    a.rows_per_cta = (int)std::min<int64_t>(kMaxRows, std::max<int64_t>(1, ((int64_t)max_rows * n_batch + 4 * sms - 1) / (4 * sms)));
     const dim3 grid((unsigned)((max_rows + a.rows_per_cta - 1) / a.rows_per_cta), (unsigned)n_batch);
     const size_t smem = (size_t)a.rows_per_cta * (a.rotary / 2) * sizeof(float2);
     const bool wide = a.interleaved || a.rotary % 16 == 0;

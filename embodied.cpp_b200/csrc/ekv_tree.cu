@@ -21,7 +21,6 @@ namespace {
 using namespace decode;
 using namespace sm100;
 
-constexpr int kXCols = 32;  // columns that the key groups' outputs are joined in at a time
 
 // CTAs per SM: two where a thread's share of the output (8 * NR rows by D columns over a warp) leaves the
 // registers for it and two tiles in flight fit the shared memory of half an SM.
@@ -43,7 +42,10 @@ struct Cfg {
     static constexpr int STAGE_MIN = 2 * T::KV_BYTES, STAGE_DRAFT = Q8 ? 2 * DT * DROW : 0;
     static constexpr int STAGE = ((STAGE_MIN > STAGE_DRAFT ? STAGE_MIN : STAGE_DRAFT) + 1023) / 1024 * 1024;
     static constexpr int V_OFF = T::KV_BYTES, DRAFT_V_OFF = Q8 ? DT * DROW : T::KV_BYTES;
-    static constexpr int X_BYTES = WK * ROWS * kXCols * 4;
+    // columns that the key groups' outputs are joined in at a time: 16 KB of rows (or all columns)
+    static constexpr int X_FIT = WK * ROWS <= 32 ? 128 : WK * ROWS <= 64 ? 64 : 32;
+    static constexpr int X_COLS = X_FIT < D ? X_FIT : D <= 32 ? 32 : D <= 64 ? 64 : 128;
+    static constexpr int X_BYTES = WK * ROWS * X_COLS * 4;
     static constexpr int ML_BYTES = WK * ROWS * 8;
     // query rows in shared memory where the output's share of the registers leaves no room for them
     static constexpr bool Q_SMEM = D * NR > 256;
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
         rg.b = blockIdx.x / units_per_req;
         const int n = unit_tiles(load_req(a, rg.b, false));
         rg.base = 0;
-        rg.lo = (long long)(blockIdx.x - rg.b * units_per_req) * n;
+        rg.lo = (blockIdx.x - rg.b * units_per_req) * (uint32_t)n;
         rg.hi = rg.lo + n;
         rg.total = 0;
         rg.ctas = 0;
@@ -131,19 +133,19 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     };
     bool ok = true;
     int b = rg.b;
-    long long base = rg.base;
-    for (long long x = rg.lo; x < rg.hi && b < a.n_batch;) {
+    uint32_t base = rg.base;
+    for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
         const Req rq = load_req(a, b, warp == 0);
         const int n_tiles = unit_tiles(rq);
-        const long long span = (long long)n_tiles * units_per_req;
+        const uint32_t span = (uint32_t)n_tiles * units_per_req;
         if (x >= base + span) {
             base += span;
             ++b;
             continue;
         }
-        const int u = (int)((x - base) / n_tiles);
-        const int t0 = (int)((x - base) - (long long)u * n_tiles);
-        const int t1 = (int)min((long long)n_tiles, t0 + (rg.hi - x));
+        const int u = (int)((x - base) / (uint32_t)n_tiles);
+        const int t0 = (int)(x - base) - u * n_tiles;
+        const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
         const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * C::ROWS;
         const int rows = min(C::ROWS, rows_all - row0);
         const int p_tiles = (rq.n_prefix + kTile - 1) / kTile;
@@ -158,6 +160,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
         if (warp == C::NW) {
             // ---- feeder ----
             Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
+            if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
+                const unsigned long long end = base + (uint32_t)(u + 1) * n_tiles;
+                a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
+            }
             for (int j = t0; j < t1; ++j, advance()) {
                 const Piece pc = next;
                 if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
@@ -573,53 +579,52 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                             off || lt == 0.0f ? -INFINITY : (mt + __log2f(lt)) * 0.6931471805599453f;
                     }
                 }
-            if (a.split && threadIdx.x == 0 && t0 == 0) {
-                const long long unit0 = base + (long long)u * n_tiles, last = unit0 + n_tiles - 1;
-                a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)(((last + 1) * rg.ctas - 1) / rg.total));
-            }
+            constexpr int XC = C::X_COLS, ROUNDS = (D + XC - 1) / XC;
 #pragma unroll
-            for (int cc = 0; cc < (D + kXCols - 1) / kXCols; ++cc) {
-                const int cols = min(kXCols, D - cc * kXCols);
+            for (int cc = 0; cc < ROUNDS; ++cc) {
+                constexpr int q4_max = XC / 4;
+                const int q4 = min(XC, D - cc * XC) / 4;
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int d2 = 0; d2 < 2; ++d2) {
-                        const int ds = cc * 2 + d2;
+                    for (int d2 = 0; d2 < XC / 16; ++d2) {
+                        const int ds = cc * (XC / 16) + d2;
                         if (ds >= KS) continue;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int r = wrow + 8 * n + 2 * c + (i & 1);
-                            const int col = o_col<Q8>(ds, kq, i) - cc * kXCols;
+                            const int col = o_col<Q8>(ds, kq, i) - cc * XC;
                             // a warp without a key for the row has nothing (not 0 * its garbage)
                             const float f = scale_o[n][i & 1];
-                            xb[(wk * C::ROWS + r) * kXCols + ((col + 4 * r) & (kXCols - 1))] = f == 0.0f ? 0.0f : o[n][ds][i] * f;
+                            xb[(wk * C::ROWS + r) * XC + ((col + 4 * r) & (XC - 1))] = f == 0.0f ? 0.0f : o[n][ds][i] * f;
                         }
                     }
                 asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
-                for (int i = threadIdx.x; i < rows * (cols / 4); i += C::NC) {
-                    const int r = i / (cols / 4), col = (i - r * (cols / 4)) * 4;
+                for (int i = threadIdx.x; i < rows * q4; i += C::NC) {
+                    const int r = q4 == q4_max ? i / q4_max : i / q4, col = (i - r * q4) * 4;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int w = 0; w < WK; ++w) {
-                        const float4 y = *(const float4 *)&xb[(w * C::ROWS + r) * kXCols + ((col + 4 * r) & (kXCols - 1))];
+                        const float4 y = *(const float4 *)&xb[(w * C::ROWS + r) * XC + ((col + 4 * r) & (XC - 1))];
                         v.x += y.x;
                         v.y += y.y;
                         v.z += y.z;
                         v.w += y.w;
                     }
                     if (!whole) {
-                        *(float4 *)(a.ws_o + (slot * C::ROWS + r) * D + cc * kXCols + col) = v;
+                        *(float4 *)(a.ws_o + (slot * C::ROWS + r) * D + cc * XC + col) = v;
                         continue;
                     }
                     const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
                     if (t >= rq.n_nodes) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    const long long dst = (((long long)b * a.n_draft + t) * a.q_heads + hq) * D + cc * kXCols + col;
+                    const long long dst = (((long long)b * a.n_draft + t) * a.q_heads + hq) * D + cc * XC + col;
                     if (a.out_dtype == EKV_DTYPE_F32)
                         *(float4 *)((float *)a.out + dst) = v;
                     else
                         *(uint2 *)((uint16_t *)a.out + dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
+                // (the next unit's end has a barrier before these are written again)
+                if (cc + 1 < ROUNDS) asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
             }
         }
         x += t1 - t0;
@@ -637,65 +642,66 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
 }
 
 // One query row of a unit that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
-// The warps of the block take parts in turn, so a row of many parts is not one warp's chain.
-constexpr int kMergeWarps = 4;
+// Lanes look at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one
+// another; the warps of the block take rows of parts in turn.
+constexpr int kMergeWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const TreeArgs a, int rows_tile) {
     const int rows_all = a.n_draft * a.group;
     const int row = blockIdx.x % rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
     const int bg = blockIdx.x / rows_all, b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = row / a.group, hq = g * a.group + row - t * a.group;
+    const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
     grid_wait();
     const int2 part = a.parts[bg * a.row_tiles + rt];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (part.x == part.y) return;
-    __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
+    __shared__ float s_o[kMergeWarps][D];
     constexpr int PER = (D + 31) / 32;
-    float m = -INFINITY, l = 0.0f, o[PER];
+    auto slot_of = [&](int c) { return (2ll * c + (c == part.x ? 1 : 0)) * rows_tile + r; };
+    float m = -INFINITY;
+    for (int c = part.x + lane; c <= part.y; c += 32) m = fmaxf(m, a.ws_ml[slot_of(c)].x);
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    float l = 0.0f, o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) o[i] = 0.0f;
-    for (int c = part.x + warp; c <= part.y; c += kMergeWarps) {
-        const long long slot = (2ll * c + (c == part.x ? 1 : 0)) * rows_tile + r;
-        const float2 ml = a.ws_ml[slot];
-        float v[PER];
+    for (int c0 = part.x; c0 <= part.y; c0 += 32) {
+        float f = 0.0f;
+        if (c0 + lane <= part.y) {
+            const float2 ml = a.ws_ml[slot_of(c0 + lane)];
+            f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+            l += f * ml.y;
+        }
+        const int n = min(32, part.y + 1 - c0);
+#pragma unroll 4
+        for (int k = warp; k < n; k += kMergeWarps) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float *src = a.ws_o + slot_of(c0 + k) * D;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < D ? a.ws_o[slot * D + lane + 32 * i] : 0.0f;
-        const float mn = fmaxf(m, ml.x);
-        if (mn == -INFINITY) continue;
-        const float f = ex2(m - mn), h = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mn);
-        l = l * f + ml.y * h;
+            for (int i = 0; i < PER; ++i)
+                if (lane + 32 * i < D) {
+                    const float v = src[lane + 32 * i];
+                    o[i] += fk == 0.0f ? 0.0f : v * fk;  // (a part that saw nothing for the row)
+                }
+        }
+    }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] = o[i] * f + (h == 0.0f ? 0.0f : v[i] * h);
-        m = mn;
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
+    for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (lane + 32 * i < D) s_o[warp][lane + 32 * i] = o[i];
     __syncthreads();
-    float mt = -INFINITY, lt = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) mt = fmaxf(mt, s_m[w]);
-    float f[kMergeWarps];
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
-        f[w] = s_m[w] == -INFINITY ? 0.0f : ex2(s_m[w] - mt);
-        lt += s_l[w] * f[w];
-    }
-    const int t = row / a.group, hq = g * a.group + row - t * a.group;
-    const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
-    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     for (int d = threadIdx.x; d < D; d += kMergeWarps * 32) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) v += f[w] == 0.0f ? 0.0f : s_o[w][d] * f[w];
+        for (int w = 0; w < kMergeWarps; ++w) v += s_o[w][d];
         v *= inv;
         if (a.out_dtype == EKV_DTYPE_F32) ((float *)a.out)[at * D + d] = v;
         else ((uint16_t *)a.out)[at * D + d] = f32_to_bf16_bits(v);
     }
-    if (a.lse && threadIdx.x == 0) a.lse[at] = lt == 0.0f ? -INFINITY : (mt + __log2f(lt)) * 0.6931471805599453f;
+    if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host side ----
@@ -778,12 +784,14 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     a.row_tiles = (rows + tile_rows(sh) - 1) / tile_rows(sh);
     const int64_t units = (int64_t)a.n_batch * a.pool.kv_heads * a.row_tiles;
     const int64_t all_rows = (int64_t)a.n_batch * a.pool.kv_heads * rows;
-    if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
     const WsLayout w = ws_layout(a.pool, a.n_batch, rows, a.row_tiles, sms);
+    // (a request's tiles: 64 keys, and 64 or 32 drafts; the sums of a split call are 32-bit)
     const int64_t unit_tiles = (max_len + kTile - 1) / kTile + 1;
+    const int64_t most_tiles = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile + 2;
+    if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
     const int full = sms * ctas_per_sm(sh, a.pool.head_dim, a.pool.dtype == EKV_DTYPE_Q8_0);
     // Units of one or two tiles are not worth a second launch; without a workspace a unit is one CTA's.
-    a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2;
+    a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2 && units * most_tiles < INT32_MAX;
     int64_t grid = units;
     if (a.split) {
         grid = std::min<int64_t>(full, units * unit_tiles);

@@ -83,19 +83,19 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
     };
     bool ok = true;
     int b = rg.b;
-    long long base = rg.base;
-    for (long long x = rg.lo; x < rg.hi && b < a.n_batch;) {
+    uint32_t base = rg.base;
+    for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
         const Req rq = request(b, warp == 0);
         const int n_tiles = (rq.n_prefix + kTile - 1) / kTile;
-        const long long span = (long long)n_tiles * hk;
+        const uint32_t span = (uint32_t)n_tiles * hk;
         if (x >= base + span) {
             base += span;
             ++b;
             continue;
         }
-        const int g = (int)((x - base) / n_tiles);
-        const int t0 = (int)((x - base) - (long long)g * n_tiles);
-        const int t1 = (int)min((long long)n_tiles, t0 + (rg.hi - x));
+        const int g = (int)((x - base) / (uint32_t)n_tiles);
+        const int t0 = (int)(x - base) - g * n_tiles;
+        const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
 
         for (int c0 = 0; c0 < rows_all; c0 += q_rows) {
             const int rows = min(q_rows, (rows_all - c0 + 15) / 16 * 16);
@@ -262,6 +262,8 @@ int launch(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
     const int smem = C::smem(q_rows);
     static std::atomic<uint64_t> smem_done{0};
     if (const int rc = allow_smem(key_weights_kernel<D, Q8>, 227 * 1024, smem_done)) return rc;
+    const int64_t most = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile;
+    if ((int64_t)a.n_batch * a.pool.kv_heads * most > INT32_MAX) return EKV_ERR_UNSUPPORTED;
     const int64_t tiles = (int64_t)a.n_batch * a.pool.kv_heads * ((max_len + kTile - 1) / kTile);
     const int ctas = smem > 112 * 1024 ? 1 : 2;
     const int grid = (int)std::min<int64_t>((int64_t)sms * ctas, std::max<int64_t>(1, tiles));
