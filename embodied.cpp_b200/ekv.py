@@ -221,10 +221,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(stream):
+def _current_stream():
+    """The current torch stream's handle. torch.cuda.current_stream() makes a Stream object first, 3 us of a call that
+    may itself take 5; where torch has the raw query it is asked instead."""
+    global _current_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.cuda.current_device
+    if raw is not None:
+        _current_stream = lambda: raw(device())  # noqa: E731
+    else:
+        _current_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+    return _current_stream()
+
+
+def _stream(stream):
+    return _current_stream() if stream is None else stream.cuda_stream
 
 
 @dataclass
@@ -367,25 +378,16 @@ class Pool:
         """ekv_rope_append: turn q [rows, q_heads, head_dim] into q_out and k into the pages beside v ([rows, kv_heads,
         head_dim]), all bf16 and by source row. q, k and v may be slices of one [rows, columns] projection output:
         rows may be any distance apart, a row's heads are adjacent. Either pair may be left out."""
-        q_heads, q_stride = self._rows(q, self.cfg.head_dim, "q")
-        kv_heads, kv_stride = self._rows(k, self.cfg.head_dim, "k")
-        v_heads, v_stride = self._rows(v, self.cfg.head_dim, "v")
-        if (kv_heads, kv_stride) != (v_heads, v_stride) or (k is not None and kv_heads != self.cfg.kv_heads):
+        cfg = self.cfg
+        q_heads, q_stride = _rows(q, cfg.head_dim, "q")
+        kv = _rows(k, cfg.head_dim, "k")
+        if kv != _rows(v, cfg.head_dim, "v") or (k is not None and kv[0] != cfg.kv_heads):
             raise ValueError("k and v must have the pool's KV heads and the same distance from row to row")
-        if q is not None and (q_out is None or not q_out.is_contiguous() or q_out.shape != q.shape):
+        if q is not None and (q_out is None or q_out.shape != q.shape or not q_out.is_contiguous()):
             raise ValueError("q_out must be contiguous and of q's shape")
         check(lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), _ptr(seq_ids), _ptr(dst_pos), _ptr(n_rows),
                                   _ptr(src_row), max_rows, _ptr(positions), q_heads, _ptr(q), q_stride, _ptr(q_out),
-                                  _ptr(k), _ptr(v), kv_stride, _stream(stream)), "ekv_rope_append")
-
-    @staticmethod
-    def _rows(t, head_dim, name):
-        """Heads of a [rows, heads, head_dim] tensor and the elements from row to row; a row must be adjacent."""
-        if t is None:
-            return 0, 0
-        if t.dim() != 3 or t.shape[2] != head_dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != head_dim):
-            raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
-        return t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * head_dim
+                                  _ptr(k), _ptr(v), kv[1], _stream(stream)), "ekv_rope_append")
 
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
                     prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
@@ -468,6 +470,16 @@ def project_qkv_rope(pool: "Pool", layer, seq_ids, x, wq, wk, wv, positions, rop
     check(lib.ekv_project_qkv_rope(pool.h, layer, n_batch, _ptr(seq_ids), tokens, q_heads, hidden, _ptr(x), _ptr(wq),
                                    _ptr(wk), _ptr(wv), _ptr(positions), rope_base, _ptr(q_out), _ptr(k_out),
                                    _ptr(v_out), _stream(stream)), "ekv_project_qkv_rope")
+
+
+def _rows(t, head_dim, name):
+    """Heads of a [rows, heads, head_dim] tensor and the elements from row to row; a row must be adjacent."""
+    if t is None:
+        return 0, 0
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != head_dim or stride[2] != 1 or (shape[1] > 1 and stride[1] != head_dim):
+        raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
+    return shape[1], stride[0] if shape[0] > 1 else shape[1] * head_dim
 
 
 class DevArray:
