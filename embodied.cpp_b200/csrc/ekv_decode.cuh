@@ -63,6 +63,11 @@ int allow_smem(K k, int bytes, std::atomic<uint64_t> &done) {
     return EKV_OK;
 }
 
+// Bounded wait of a whole warp: the same answer in every lane, so that what follows may be warp-wide.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+    return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, abort, kDefaultWaitBudget));
+}
+
 constexpr int kTile = 64;                       // keys per tile
 constexpr long long kWait = kDefaultWaitBudget; // clock cycles a bounded wait gives up after
 
@@ -315,18 +320,19 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
 }
 
 // ---- copy-engine feeder ----
-// One lane's share of a 64-key tile of the paged prefix: lanes 0-15 copy K, 16-31 V, one run of rows
-// inside one block each (blocks hold a multiple of 8 rows, so a tile spans at most 9 of them).
+// One lane's share of a 64- or 128-key tile of the paged prefix: lanes 0-15 copy K, 16-31 V, one run of rows
+// inside one block each (blocks hold a multiple of 8 rows and tiles start at multiples of 64, so a tile of 128
+// spans at most 16 of them).
 struct Piece {
     const uint8_t *src;  // first row of the run (bf16: its row group; Q8_0: its int8 row), or null
     int row, n;          // first row inside the tile, rows (multiple of 8)
     int rib;             // first row inside the block
 };
 
-template <int D, bool Q8>
+template <int D, bool Q8, int TILE = kTile>
 __device__ __forceinline__ Piece find_piece(const TreeArgs &a, const Req &rq, int head, int key0, int lane) {
     const PoolView &p = a.pool;
-    const int valid = min(kTile, rq.n_prefix - key0), n8 = (valid + 7) & ~7;
+    const int valid = min(TILE, rq.n_prefix - key0), n8 = (valid + 7) & ~7;
     const int kv = lane >> 4, i = lane & 15;
     Piece pc;
     pc.src = nullptr;
@@ -371,6 +377,16 @@ __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, 
     } else {
         bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2), bar);
     }
+}
+
+// One side of a bf16 tile: the lanes with `mine` copy their runs to `dst` (completion on `bar`).
+template <int D>
+__device__ __forceinline__ void issue_half(const Piece &pc, uint32_t dst, uint32_t bar, bool mine, int lane) {
+    const uint32_t bytes = mine && pc.src ? (uint32_t)(pc.n * D * 2) : 0u;
+    const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
+    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, all);
+    __syncwarp();
+    if (bytes) sm100::bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, bytes, bar);
 }
 
 // A query row in shared memory: padded by 16 bytes, so that eight rows' 16-byte units fall in eight different

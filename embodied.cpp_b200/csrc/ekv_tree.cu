@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
             for (int j = t0; j < t1; ++j, advance()) {
                 const Piece pc = next;
                 if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
-                if (turn > 0) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort, kWait);
+                if (turn > 0) ok = ok && warp_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort);
                 if (!ok) {
                     *abort = 1;
                     continue;
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                 const int d0 = (j - p_tiles) * C::DT;
                 const int valid = draft ? min(C::DT, rq.n_nodes - d0) : min(kTile, rq.n_prefix - j * kTile);
                 const uint32_t sv = sk + (draft ? C::DRAFT_V_OFF : C::V_OFF);
-                ok = ok && mbar_wait(smem_addr(&sh.full_k[st]), par, abort, kWait);
+                ok = ok && warp_wait(smem_addr(&sh.full_k[st]), par, abort);
                 if (!ok) {
                     *abort = 1;
                     continue;
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     }
                     // ---- O^T += V^T P^T ----
                     if (!v_ready) {
-                        ok = mbar_wait(smem_addr(&sh.full_v[st]), par, abort, kWait);
+                        ok = warp_wait(smem_addr(&sh.full_v[st]), par, abort);
                         if (!ok) {
                             *abort = 1;
                             break;
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     }
                 }
                 if (ok && !v_ready) {  // no key of this tile is the warp's: still stay in step with the stage
-                    ok = mbar_wait(smem_addr(&sh.full_v[st]), par, abort, kWait);
+                    ok = warp_wait(smem_addr(&sh.full_v[st]), par, abort);
                     if (!ok) *abort = 1;
                 }
                 __syncwarp();
@@ -707,26 +707,29 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
 // ---- host side ----
 // Row tiles: a warp holds 8, 16 or (up to head_dim 128) 32 rows; more rows take four warps' 16, so that a tile
 // of keys is read from memory once per 64 rows.
-enum class Shape { R8, R16, R32, R64 };
+enum class Shape { R8, R16, R32, R64, Tile };
 
-Shape shape_for(int head_dim, int rows) {
+Shape shape_for(const PoolView &p, int rows) {
+    const int head_dim = p.head_dim;
+    if (tree_tile_fits(p, rows)) return Shape::Tile;
     if (rows <= 8) return Shape::R8;
     if (rows <= 16) return Shape::R16;
     if (rows <= 32 && head_dim <= 128) return Shape::R32;
     return Shape::R64;
 }
-int tile_rows(Shape s) { return s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64; }
+int tile_rows(Shape s) { return s == Shape::Tile ? kTreeTileRows : s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64; }
 
-int ctas_per_sm(Shape s, int head_dim, bool q8) {
-    return rows_ctas(head_dim, q8, s == Shape::R8 ? 1 : s == Shape::R32 ? 4 : 2, s == Shape::R64 ? 4 : 1);
+int grid_ctas(Shape s, const PoolView &p, int sms) {
+    if (s == Shape::Tile) return tree_tile_ctas(p, sms);
+    return sms * rows_ctas(p.head_dim, p.dtype == EKV_DTYPE_Q8_0, s == Shape::R8 ? 1 : s == Shape::R32 ? 4 : 2, s == Shape::R64 ? 4 : 1);
 }
 
 struct WsLayout {
     size_t parts, ml, o, total;
 };
 WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
-    const Shape sh = shape_for(p.head_dim, rows);
-    const size_t slots = 2ull * sms * ctas_per_sm(sh, p.head_dim, p.dtype == EKV_DTYPE_Q8_0) * tile_rows(sh);
+    const Shape sh = shape_for(p, rows);
+    const size_t slots = 2ull * grid_ctas(sh, p, sms) * tile_rows(sh);
     WsLayout w;
     w.parts = 0;
     w.ml = ((size_t)n_batch * p.kv_heads * rt * sizeof(int2) + 255) / 256 * 256;
@@ -758,7 +761,9 @@ int launch_shape(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
 template <int D>
 int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     int rc;
-    if (a.pool.dtype == EKV_DTYPE_Q8_0) {
+    if (sh == Shape::Tile) {
+        rc = launch_tree_tile(a, grid, s);
+    } else if (a.pool.dtype == EKV_DTYPE_Q8_0) {
         if constexpr (D % 32 == 0) rc = launch_shape<D, true>(a, sh, grid, s);
         else rc = EKV_ERR_UNSUPPORTED;
     } else {
@@ -774,13 +779,13 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
 
 size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, int sms) {
     const int rows = n_draft * (q_heads / p.kv_heads);
-    const int tr = tile_rows(shape_for(p.head_dim, rows));
+    const int tr = tile_rows(shape_for(p, rows));
     return ws_layout(p, n_batch, rows, (rows + tr - 1) / tr, sms).total;
 }
 
 int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s) {
     const int rows = a.n_draft * a.group;
-    const Shape sh = shape_for(a.pool.head_dim, rows);
+    const Shape sh = shape_for(a.pool, rows);
     a.row_tiles = (rows + tile_rows(sh) - 1) / tile_rows(sh);
     const int64_t units = (int64_t)a.n_batch * a.pool.kv_heads * a.row_tiles;
     const int64_t all_rows = (int64_t)a.n_batch * a.pool.kv_heads * rows;
@@ -789,7 +794,7 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     const int64_t unit_tiles = (max_len + kTile - 1) / kTile + 1;
     const int64_t most_tiles = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile + 2;
     if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
-    const int full = sms * ctas_per_sm(sh, a.pool.head_dim, a.pool.dtype == EKV_DTYPE_Q8_0);
+    const int full = grid_ctas(sh, a.pool, sms);
     // Units of one or two tiles are not worth a second launch; without a workspace a unit is one CTA's.
     a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2 && units * most_tiles < INT32_MAX;
     int64_t grid = units;

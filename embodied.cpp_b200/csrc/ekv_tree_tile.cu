@@ -1,0 +1,467 @@
+// ekv_tree_tile.cu -- draft-tree attention for many query rows per KV head (bf16 pools), on tcgen05.
+//
+// The same sums as ekv_tree.cu. From about 64 rows per cached key the tensor pipe bounds the call, not the
+// bytes, so 128 rows take the 5th-generation tensor cores: S = Q K^T with both operands in shared memory and S
+// in tensor memory, P = exp(S - m) as bf16 over S's own columns, O += P V with P read from tensor memory.
+// A CTA holds one 128-row tile: warps 0-3 are the softmax (a thread is a row), warp 4 issues the products,
+// warp 5 feeds K and V through the copy engine (pool tiles are canonical operands as they are stored). Up to
+// head_dim 128 two CTAs share an SM, 256 tensor-memory columns each: while one takes exponentials the other's
+// products run, so that a CTA needs neither a second S nor a second K/V stage. At head_dim 256 one CTA has two
+// of each and issues S(j + 1) before P V(j).
+#include "ekv_decode.cuh"
+
+namespace ekv {
+namespace {
+
+using namespace decode;
+using namespace sm100;
+
+template <int D>
+struct TCfg {
+    static constexpr int BN = D > 128 ? 64 : 128;  // keys per tile
+    static constexpr int NS = D > 128 ? 2 : 1;     // S buffers, and K and V stages
+    static constexpr int CTAS = D > 128 ? 1 : 2;
+    static constexpr uint32_t SBO = 16 * D;        // bytes between 8-row groups; chunks of 64 columns are 1024 apart
+    static constexpr uint32_t LAYOUT = 2;          // 128-byte swizzle
+    static constexpr int KV_BYTES = BN * D * 2;
+    static constexpr int Q_BYTES = kTreeTileRows * D * 2;
+    static constexpr int S_COL = 0, O_COL = BN * NS, COLS = D > 128 ? 512 : 256;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_SH = OFF_V + NS * KV_BYTES;
+    static constexpr int SMEM = OFF_SH + 1024 + 1024;
+    static_assert(O_COL + D <= COLS, "tensor memory");
+    static_assert(D % 64 == 0, "whole swizzle chunks");
+};
+
+struct TShared {
+    uint64_t k_full[2], v_full[2], s_full[2], p_full[2], v_done[2], q_ready, drained;
+    unsigned long long bad[2];  // drafted keys of the unit (even, odd) whose values are not all finite
+    uint32_t tmem;
+    int abort;
+    RangeScratch range;
+};
+
+constexpr int kRowWarps = 4, kTileThreads = (kRowWarps + 2) * 32;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Visible columns [0, 32) of a 32-column chunk that starts at key c0 of the tile: `word` has a bit per key.
+__device__ __forceinline__ uint32_t chunk_bits(unsigned long long word, int c0, int valid) {
+    const uint32_t w = c0 >= 64 ? 0xffffffffu : (uint32_t)(word >> c0);
+    const int n = valid - c0;
+    return n >= 32 ? w : n <= 0 ? 0u : w & ((1u << n) - 1u);
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(const TreeArgs a) {
+    using C = TCfg<D>;
+    constexpr int BN = C::BN, NS = C::NS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    TShared &sh = *(TShared *)(smem + C::OFF_SH);
+    static_assert(sizeof(TShared) <= 1024, "barrier block");
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hk = a.pool.kv_heads, units_per_req = hk * a.row_tiles;
+    const int rows_all = a.n_draft * a.group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_addr(&sh.k_full[i]), 1);
+            mbar_init(smem_addr(&sh.v_full[i]), 1);
+            mbar_init(smem_addr(&sh.s_full[i]), 1);
+            mbar_init(smem_addr(&sh.p_full[i]), kRowWarps);
+            mbar_init(smem_addr(&sh.v_done[i]), 1);
+        }
+        mbar_init(smem_addr(&sh.q_ready), kRowWarps);
+        mbar_init(smem_addr(&sh.drained), 1);
+        sh.abort = 0;
+        sh.bad[0] = sh.bad[1] = 0;
+        mbar_init_fence();
+    }
+    if (warp == kRowWarps) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
+    auto unit_tiles = [](const Req &r) { return max(1, (r.n_prefix + BN - 1) / BN + (r.n_nodes > 0 ? 1 : 0)); };
+    grid_wait();
+    grid_launch_next();
+    tc_fence_before();
+    Range rg;
+    if (a.split) {
+        rg = find_range<kTileThreads>(a.n_batch, units_per_req, sh.range,
+                                      [&](int b) { return unit_tiles(load_req(a, b, false)); });
+    } else {
+        __syncthreads();
+        rg.b = blockIdx.x / units_per_req;
+        const int n = unit_tiles(load_req(a, rg.b, false));
+        rg.base = 0;
+        rg.lo = (blockIdx.x - rg.b * units_per_req) * (uint32_t)n;
+        rg.hi = rg.lo + n;
+        rg.total = 0;
+        rg.ctas = 0;
+    }
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    int it = 0, unit_no = 0;  // tiles and units of this CTA so far
+    bool ok = true;
+    int b = rg.b;
+    uint32_t base = rg.base;
+    for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
+        const Req rq = load_req(a, b, warp == 0);
+        const int n_tiles = unit_tiles(rq);
+        const uint32_t span = (uint32_t)n_tiles * units_per_req;
+        if (x >= base + span) {
+            base += span;
+            ++b;
+            continue;
+        }
+        const int u = (int)((x - base) / (uint32_t)n_tiles);
+        const int t0 = (int)(x - base) - u * n_tiles;
+        const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
+        const int n = t1 - t0;
+        const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * kTreeTileRows;
+        const int rows = min(kTreeTileRows, rows_all - row0);
+        const int p_tiles = (rq.n_prefix + BN - 1) / BN;
+        const long long kv_row = ((long long)b * a.n_draft * hk + g) * D;
+
+        if (warp == kRowWarps + 1) {
+            // ---- feeder ----
+            Piece next = find_piece<D, false, BN>(a, rq, g, t0 * BN, lane);
+            if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
+                const unsigned long long end = base + (uint32_t)(u + 1) * n_tiles;
+                a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
+            }
+            for (int j = t0; j < t1; ++j, ++it) {
+                const int st = it % NS, par = (it / NS) & 1;
+                const Piece pc = next;
+                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, false, BN>(a, rq, g, (j + 1) * BN, lane);
+                const uint32_t sk = smem_addr(smem + C::OFF_K + st * C::KV_BYTES);
+                const uint32_t sv = smem_addr(smem + C::OFF_V + st * C::KV_BYTES);
+                const uint32_t bk = smem_addr(&sh.k_full[st]), bv = smem_addr(&sh.v_full[st]);
+                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.s_full[st]), par ^ 1, abort);  // K(it - NS) read
+                if (ok && j < p_tiles) issue_half<D>(pc, sk, bk, lane < 16, lane);
+                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.v_done[st]), par ^ 1, abort);  // V(it - NS) read
+                if (!ok) {
+                    *abort = 1;
+                    continue;
+                }
+                if (j < p_tiles) {
+                    issue_half<D>(pc, sv, bv, lane >= 16, lane);
+                    continue;
+                }
+                // drafted rows, from the caller's buffers
+                const int nd = rq.n_nodes;
+                constexpr int U = D / 8;
+                for (int i = lane; i < nd * U; i += 32) {
+                    const int r = i / U, col = (i - r * U) * 8;
+                    const long long src = kv_row + (long long)r * hk * D + col;
+                    const uint32_t off = bf16_off<D>(r, col);
+                    cp_async_16(sk + off, a.k_draft + src);
+                    cp_async_16(sv + off, a.v_draft + src);
+                }
+                cp_async_wait_all();
+                // values that are not finite leave the tile: 0 * inf would reach rows that may not see them
+                unsigned long long bad = 0;
+                for (int i = lane; i < nd * U; i += 32) {
+                    const int r = i / U, col = (i - r * U) * 8;
+                    uint16_t *w = (uint16_t *)(smem + C::OFF_V + st * C::KV_BYTES + bf16_off<D>(r, col));
+                    const uint4 v = *(const uint4 *)w;
+                    const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        any = any || (ww[e] & 0x7f80u) == 0x7f80u || (ww[e] & 0x7f800000u) == 0x7f800000u;
+                    if (any) {
+                        bad |= 1ull << r;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if ((w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
+                    }
+                }
+                const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
+                const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
+                if (lane == 0) sh.bad[unit_no & 1] = (unsigned long long)bhi << 32 | blo;
+                fence_proxy_async();  // read by the tensor core
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bk);
+                    mbar_arrive(bv);
+                }
+            }
+        } else if (warp == kRowWarps) {
+            // ---- products ----
+            if (lane == 0) {
+                const uint32_t id_s = idesc_f16(true, false, BN), id_o = idesc_f16(true, true, D);
+                const uint32_t q_addr = smem_addr(smem), k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
+                auto issue_s = [&](int i) {
+                    const int st = i % NS;
+                    if (!mbar_wait(smem_addr(&sh.k_full[st]), (i / NS) & 1, abort, kWait)) return false;
+                    tc_fence_after();
+                    const uint64_t qa = sdesc(q_addr, 16, C::SBO, C::LAYOUT);
+                    const uint64_t kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
+#pragma unroll
+                    for (int s4 = 0; s4 < D / 64; ++s4) {  // four 16-column steps of a 64-column chunk
+                        uint64_t av[4], bv[4];
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
+                            bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
+                        }
+                        mma_ss_x4<false>(tmem + C::S_COL + (uint32_t)(st * BN), av, bv, id_s, s4 > 0 ? 1u : 0u);
+                    }
+                    mma_commit(smem_addr(&sh.s_full[st]));
+                    return true;
+                };
+                auto issue_pv = [&](int i, bool first) {
+                    const int st = i % NS;
+                    if (!mbar_wait(smem_addr(&sh.v_full[st]), (i / NS) & 1, abort, kWait)) return false;
+                    if (!mbar_wait(smem_addr(&sh.p_full[st]), (i / NS) & 1, abort, kWait)) return false;
+                    tc_fence_after();
+                    const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
+#pragma unroll
+                    for (int s4 = 0; s4 < BN / 64; ++s4) {
+                        uint32_t av[4];
+                        uint64_t bv[4];
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            av[s] = tmem + C::S_COL + (uint32_t)(st * BN + (4 * s4 + s) * 8);
+                            bv[s] = vb + ((uint32_t)(4 * s4 + s) * 2u * C::SBO >> 4);
+                        }
+                        mma_ts_x4<false>(tmem + C::O_COL, av, bv, id_o, (first && s4 == 0) ? 0u : 1u);
+                    }
+                    mma_commit(smem_addr(&sh.v_done[st]));
+                    return true;
+                };
+                ok = ok && mbar_wait(smem_addr(&sh.q_ready), unit_no & 1, abort, kWait);
+                ok = ok && issue_s(it);
+                for (int i = 0; ok && i < n; ++i) {
+                    if (NS == 2 && i + 1 < n) ok = issue_s(it + i + 1);
+                    ok = ok && issue_pv(it + i, i == 0);
+                    if (NS == 1 && ok && i + 1 < n) ok = issue_s(it + i + 1);
+                }
+                if (!ok) *abort = 1;
+            }
+            it += n;
+        } else {
+            // ---- softmax: thread = row ----
+            const int r = threadIdx.x;
+            const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+            const int t = (row0 + r) / a.group;
+            const bool on = r < rows && t < rq.n_nodes;
+            // this warp's query rows to shared memory (the last unit's products are done: its O was read)
+            constexpr int U = D / 8;
+#pragma unroll 8
+            for (int i = lane; i < 32 * U; i += 32) {
+                const int rr = warp * 32 + i / U, uu = i % U, rw = row0 + rr, tt = rw / a.group;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (rr < rows && tt < rq.n_nodes)
+                    v = __ldg((const uint4 *)(a.q + (((long long)b * a.n_draft + tt) * a.q_heads + g * a.group + rw - tt * a.group) * D) + uu);
+                *(uint4 *)(smem + bf16_off<D>(rr, 8 * uu)) = v;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready));
+
+            const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
+            float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+            bool draft_seen = false;
+            unsigned long long word = ~0ull;
+            for (int i = 0; i < n; ++i, ++it) {
+                const int st = it % NS, par = (it / NS) & 1, j = t0 + i;
+                const bool draft = j >= p_tiles;
+                const int valid = draft ? rq.n_nodes : min(BN, rq.n_prefix - j * BN);
+                if (draft) {
+                    draft_seen = valid > 0;
+                    word = !on ? 0ull
+                           : a.ancestors ? __ldg(a.ancestors + (long long)b * a.n_draft + t)
+                                         : (t >= 63 ? ~0ull : (2ull << t) - 1);
+                }
+                const bool full = !draft && valid == BN;
+                ok = ok && warp_wait(smem_addr(&sh.s_full[st]), par, abort);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t s_col = tmem + lane_base + C::S_COL + (uint32_t)(st * BN);
+                // the row's maximum of the tile
+                float top = -INFINITY;
+#pragma unroll
+                for (int c0 = 0; c0 < BN; c0 += 32) {
+                    uint32_t s[32];
+                    tmem_load32(s_col + c0, s);
+                    if (!full) {
+                        const uint32_t bits = chunk_bits(word, c0, valid);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!((bits >> k) & 1u)) s[k] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) top = max3(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                }
+                const float mt = top == -INFINITY ? -INFINITY : CAP ? score(top) : top * a.scale_log2;
+                // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
+                const bool up = mt > m + 8.0f;
+                if (__any_sync(0xffffffffu, up)) {
+                    const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
+                    if (up) m = mt;
+                    l0 *= f;
+                    l1 *= f;
+                    if (i > 0) {
+                        const int pst = (it - 1) % NS;
+                        ok = warp_wait(smem_addr(&sh.v_done[pst]), ((it - 1) / NS) & 1, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            uint32_t o[32];
+                            tmem_load32(tmem + lane_base + C::O_COL + c0, o);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st32(tmem + lane_base + C::O_COL + c0, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int c0 = 0; c0 < BN; c0 += 32) {
+                    uint32_t s[32], p[16];
+                    tmem_load32(s_col + c0, s);
+                    const uint32_t bits = full ? 0xffffffffu : chunk_bits(word, c0, valid);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float e[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float v = __uint_as_float(s[2 * k + h]);
+                            e[h] = ex2(CAP ? score(v) + neg : fmaf(v, a.scale_log2, neg));
+                            if (!full && !((bits >> (2 * k + h)) & 1u)) e[h] = 0.0f;
+                        }
+                        l0 += e[0];
+                        l1 += e[1];
+                        p[k] = pack_bf16(e[0], e[1]);
+                    }
+                    tmem_st16(s_col + c0 / 2, p);
+                }
+                tmem_wait_st();
+                if (valid < BN) {  // rows past the last key hold whatever was there: 0 * that must be 0
+                    ok = warp_wait(smem_addr(&sh.v_full[st]), par, abort);
+                    if (!ok) break;
+                    for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += kRowWarps * 32)
+                        *(uint4 *)(smem + C::OFF_V + st * C::KV_BYTES + bf16_off<D>(e / U, (e % U) * 8)) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[st]));
+            }
+            if (ok && n > 0) {
+                ok = warp_wait(smem_addr(&sh.v_done[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
+                tc_fence_after();
+            }
+            if (!ok) *abort = 1;
+            if (ok) {
+                const bool whole = t0 == 0 && t1 == n_tiles;
+                const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
+                const float l = l0 + l1;
+                const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+                const int hq = g * a.group + (row0 + r) - t * a.group;
+                const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
+                if (r < rows) {
+                    if (!whole) a.ws_ml[slot * kTreeTileRows + r] = on ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+                    else if (a.lse) a.lse[at] = on && l != 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+                }
+                const unsigned long long bad = draft_seen ? sh.bad[unit_no & 1] : 0ull;
+                const uint32_t p_col = tmem + lane_base + C::S_COL + (uint32_t)(((it - 1) % NS) * BN);
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_load32(tmem + lane_base + C::O_COL + c0, o);
+                    // rare: drafted values that are not finite, for the rows that see them (the drafts are the
+                    // unit's last tile, so their P is still there)
+                    for (unsigned long long rest = bad; rest; rest &= rest - 1) {
+                        const int k = __ffsll((long long)rest) - 1;
+                        uint32_t pair;
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                                     : "=r"(pair)
+                                     : "r"(p_col + (uint32_t)(k >> 1))
+                                     : "memory");
+                        const float p = bf16_bits_to_f32((uint16_t)(k & 1 ? pair >> 16 : pair));
+                        const uint16_t *v = a.v_draft + kv_row + (long long)k * hk * D + c0;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float y = bf16_bits_to_f32(__ldg(v + e));
+                            if (!isfinite(y) && ((word >> k) & 1ull)) o[e] = __float_as_uint(fmaf(p, y, __uint_as_float(o[e])));
+                        }
+                    }
+                    if (r < rows) {
+                        // a row without a key has nothing (not 0 * what the columns hold)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = on && l != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+                        float *of = !whole ? a.ws_o + (slot * kTreeTileRows + r) * D + c0 : (float *)a.out + at * D + c0;
+                        if (!whole || a.out_dtype == EKV_DTYPE_F32) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *(uint4 *)(of + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        } else {
+                            uint16_t *ob = (uint16_t *)a.out + at * D + c0;
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    w[k] = pack_bf16(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1]));
+                                *(uint4 *)(ob + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();
+            }
+        }
+        ++unit_no;
+        x += n;
+    }
+    if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 11);
+    if (warp == kRowWarps + 1 && !ok && lane == 0) {
+        for (int i = 0; i < NS; ++i) {  // leave no copy writing this CTA's shared memory
+            mbar_wait_drain(smem_addr(&sh.k_full[i]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.k_full[i]), 1, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.v_full[i]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.v_full[i]), 1, kWait / 64);
+        }
+    }
+    if (warp == kRowWarps && lane == 0) {  // nor a product using its tensor memory
+        mma_commit(smem_addr(&sh.drained));
+        mbar_wait_drain(smem_addr(&sh.drained), 0, kWait);
+    }
+    __syncthreads();
+    if (warp == kRowWarps) tmem_dealloc(tmem, C::COLS);
+}
+
+template <int D, bool CAP>
+int launch(const TreeArgs &a, int grid, cudaStream_t s) {
+    static std::atomic<uint64_t> smem_done{0};
+    if (const int rc = allow_smem(tree_tile_kernel<D, CAP>, TCfg<D>::SMEM, smem_done)) return rc;
+    return launch_after(tree_tile_kernel<D, CAP>, grid, kTileThreads, TCfg<D>::SMEM, s, a);
+}
+
+}  // namespace
+
+bool tree_tile_fits(const PoolView &p, int rows) {
+    return p.dtype == EKV_DTYPE_BF16 && (p.head_dim == 64 || p.head_dim == 128 || p.head_dim == 256) && rows > 64;
+}
+
+int tree_tile_ctas(const PoolView &p, int sms) { return sms * (p.head_dim > 128 ? 1 : 2); }
+
+int launch_tree_tile(const TreeArgs &a, int grid, cudaStream_t s) {
+    const bool cap = a.cap_log2 != 0.0f;
+    switch (a.pool.head_dim) {
+        case 64: return cap ? launch<64, true>(a, grid, s) : launch<64, false>(a, grid, s);
+        case 128: return cap ? launch<128, true>(a, grid, s) : launch<128, false>(a, grid, s);
+        case 256: return cap ? launch<256, true>(a, grid, s) : launch<256, false>(a, grid, s);
+        default: return EKV_ERR_UNSUPPORTED;
+    }
+}
+
+}  // namespace ekv

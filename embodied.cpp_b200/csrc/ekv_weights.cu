@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 for (int j = t0; j < t1; ++j, advance()) {
                     const Piece pc = next;
                     if (j + 1 < t1) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
-                    if (turn > 0) ok = ok && mbar_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort, kWait);
+                    if (turn > 0) ok = ok && warp_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort);
                     if (!ok) {
                         *abort = 1;
                         continue;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 const bool writes = rq0 < 4 && key < rq.n_prefix;
                 const float old = next_old;
                 next_old = load_old(j + 1);
-                ok = ok && mbar_wait(smem_addr(&sh.full[st]), par, abort, kWait);
+                ok = ok && warp_wait(smem_addr(&sh.full[st]), par, abort);
                 if (!ok) {
                     *abort = 1;
                     continue;

@@ -98,6 +98,21 @@ def test_tree_long_ragged_capped(store, dim, cap):
     check_tree(c, q, kd, vd, out, lse, up=up, cap=cap, prefix_len=use)
 
 
+@pytest.mark.parametrize("store,dim", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("q8_0", 128)])
+@pytest.mark.parametrize("T,hq,cap,dtype", [(64, 8, 20.0, torch.bfloat16), (19, 8, 0.0, torch.float32), (43, 3, 0.0, torch.bfloat16)])
+def test_tree_wide_long_ragged(store, dim, T, hq, cap, dtype):
+    """Many rows per KV head over caches of several tiles: rising maxima, odd row counts, parts of units, an empty cache."""
+    lens = [3000, 0, 515, 129]
+    c = dc.Cache(lens, 2, dim, store=store, block=24, seed=11)
+    B = len(lens)
+    q, kd, vd = rand(8, B, T, 2 * hq, dim, scale=5.0), rand(9, B, T, 2, dim), rand(10, B, T, 2, dim)
+    nodes = [T, T - 1, 1, 0]
+    up = [dc.tree_words(T, 60 + b) for b in range(B)]
+    for ws in (True, False):
+        out, lse, _ = run_tree(c, q, kd, vd, nodes=nodes, up=dc.words(up), cap=cap, dtype=dtype, workspace=ws)
+        check_tree(c, q, kd, vd, out, lse, nodes=nodes, up=up, cap=cap)
+
+
 def test_tree_rows_that_see_nothing():
     """Ancestor words of zero over an empty cache, no nodes at all: 0 and -inf."""
     c = dc.Cache([0, 40, 0], 1, 64, seed=1)
