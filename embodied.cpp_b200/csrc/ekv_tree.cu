@@ -641,31 +641,35 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     }
 }
 
-// One query row of a unit that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
-// Lanes look at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one
-// another; the warps of the block take rows of parts in turn.
+// Rows of units that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c. Lanes look
+// at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one another.
+// WARPS = 1: a warp per row (8 rows a block), for calls of many rows, which have few parts each; WARPS = 8: the
+// block's warps take parts of one row in turn.
 constexpr int kMergeWarps = 8;
-template <int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const TreeArgs a, int rows_tile) {
+template <int D, int WARPS>
+__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const TreeArgs a, int rows_tile, int n_rows) {
     const int rows_all = a.n_draft * a.group;
-    const int row = blockIdx.x % rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
-    const int bg = blockIdx.x / rows_all, b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = WARPS == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int id = WARPS == 1 ? blockIdx.x * kMergeWarps + (threadIdx.x >> 5) : blockIdx.x;
+    if (id >= n_rows) return;
+    const int bg = id / rows_all, row = id - bg * rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
+    const int b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
     const int t = row / a.group, hq = g * a.group + row - t * a.group;
     const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
     grid_wait();
     const int2 part = a.parts[bg * a.row_tiles + rt];
     if (part.x == part.y) return;
-    __shared__ float s_o[kMergeWarps][D];
-    constexpr int PER = (D + 31) / 32;
+    __shared__ float4 s_o[WARPS == 1 ? 1 : kMergeWarps][D / 4];
+    constexpr int PER = (D + 127) / 128;  // float4 of a lane
     auto slot_of = [&](int c) { return (2ll * c + (c == part.x ? 1 : 0)) * rows_tile + r; };
     float m = -INFINITY;
     for (int c = part.x + lane; c <= part.y; c += 32) m = fmaxf(m, a.ws_ml[slot_of(c)].x);
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    float l = 0.0f, o[PER];
+    float l = 0.0f;
+    float4 o[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+    for (int i = 0; i < PER; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c0 = part.x; c0 <= part.y; c0 += 32) {
         float f = 0.0f;
         if (c0 + lane <= part.y) {
@@ -675,33 +679,51 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
         }
         const int n = min(32, part.y + 1 - c0);
 #pragma unroll 4
-        for (int k = warp; k < n; k += kMergeWarps) {
+        for (int k = warp; k < n; k += WARPS) {
             const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float *src = a.ws_o + slot_of(c0 + k) * D;
+            const float4 *src = (const float4 *)(a.ws_o + slot_of(c0 + k) * D);
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (lane + 32 * i < D) {
-                    const float v = src[lane + 32 * i];
-                    o[i] += fk == 0.0f ? 0.0f : v * fk;  // (a part that saw nothing for the row)
-                }
+            for (int i = 0; i < PER; ++i) {
+                if (lane + 32 * i >= D / 4) continue;
+                const float4 v = src[lane + 32 * i];
+                if (fk == 0.0f) continue;  // (a part that saw nothing for the row)
+                o[i].x = fmaf(v.x, fk, o[i].x);
+                o[i].y = fmaf(v.y, fk, o[i].y);
+                o[i].z = fmaf(v.z, fk, o[i].z);
+                o[i].w = fmaf(v.w, fk, o[i].w);
+            }
         }
     }
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i < D) s_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int d = threadIdx.x; d < D; d += kMergeWarps * 32) {
-        float v = 0.0f;
+    auto put = [&](int i, float4 v) {
+        v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        if (a.out_dtype == EKV_DTYPE_F32) ((float4 *)((float *)a.out + at * D))[i] = v;
+        else ((uint2 *)((uint16_t *)a.out + at * D))[i] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    };
+    if constexpr (WARPS == 1) {
 #pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) v += s_o[w][d];
-        v *= inv;
-        if (a.out_dtype == EKV_DTYPE_F32) ((float *)a.out)[at * D + d] = v;
-        else ((uint16_t *)a.out)[at * D + d] = f32_to_bf16_bits(v);
+        for (int i = 0; i < PER; ++i)
+            if (lane + 32 * i < D / 4) put(lane + 32 * i, o[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (lane + 32 * i < D / 4) s_o[warp][lane + 32 * i] = o[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < D / 4; i += kMergeWarps * 32) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kMergeWarps; ++w) {
+                v.x += s_o[w][i].x;
+                v.y += s_o[w][i].y;
+                v.z += s_o[w][i].z;
+                v.w += s_o[w][i].w;
+            }
+            put(i, v);
+        }
     }
-    if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+    if (a.lse && lane == 0 && warp == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host side ----
@@ -770,9 +792,11 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
         rc = launch_shape<D, false>(a, sh, grid, s);
     }
     if (rc || !a.split) return rc;
-    const int rows = a.n_draft * a.group;
-    return launch_after(tree_merge_kernel<D>, a.n_batch * a.pool.kv_heads * rows, kMergeWarps * 32, 0, s, a,
-                        tile_rows(sh));
+    const int n_rows = a.n_batch * a.pool.kv_heads * a.n_draft * a.group;
+    // a warp per row once that fills the SMs
+    if (n_rows >= 4 * kMergeWarps * grid)
+        return launch_after(tree_merge_kernel<D, 1>, (n_rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, s, a, tile_rows(sh), n_rows);
+    return launch_after(tree_merge_kernel<D, kMergeWarps>, n_rows, kMergeWarps * 32, 0, s, a, tile_rows(sh), n_rows);
 }
 
 }  // namespace

@@ -140,6 +140,8 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                 const uint32_t sk = smem_addr(smem + C::OFF_K + st * C::KV_BYTES);
                 const uint32_t sv = smem_addr(smem + C::OFF_V + st * C::KV_BYTES);
                 const uint32_t bk = smem_addr(&sh.k_full[st]), bv = smem_addr(&sh.v_full[st]);
+                if (pc.src && j < p_tiles)  // the stages are taken until the last tile's products are done: start the way from memory
+                    bulk_prefetch_l2(pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2));
                 if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.s_full[st]), par ^ 1, abort);  // K(it - NS) read
                 if (ok && j < p_tiles) issue_half<D>(pc, sk, bk, lane < 16, lane);
                 if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.v_done[st]), par ^ 1, abort);  // V(it - NS) read
@@ -151,38 +153,25 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     issue_half<D>(pc, sv, bv, lane >= 16, lane);
                     continue;
                 }
-                // drafted rows, from the caller's buffers
+                // drafted rows, from the caller's buffers: a lane keeps its 16-byte unit of the rows
                 const int nd = rq.n_nodes;
-                constexpr int U = D / 8;
-                for (int i = lane; i < nd * U; i += 32) {
-                    const int r = i / U, col = (i - r * U) * 8;
-                    const long long src = kv_row + (long long)r * hk * D + col;
-                    const uint32_t off = bf16_off<D>(r, col);
-                    cp_async_16(sk + off, a.k_draft + src);
-                    cp_async_16(sv + off, a.v_draft + src);
-                }
-                cp_async_wait_all();
-                // values that are not finite leave the tile: 0 * inf would reach rows that may not see them
-                unsigned long long bad = 0;
-                for (int i = lane; i < nd * U; i += 32) {
-                    const int r = i / U, col = (i - r * U) * 8;
-                    uint16_t *w = (uint16_t *)(smem + C::OFF_V + st * C::KV_BYTES + bf16_off<D>(r, col));
-                    const uint4 v = *(const uint4 *)w;
-                    const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
-                    bool any = false;
+                constexpr int U = D / 8, AT_ONCE = 32 / U > 0 ? 32 / U : 1;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        any = any || (ww[e] & 0x7f80u) == 0x7f80u || (ww[e] & 0x7f800000u) == 0x7f800000u;
-                    if (any) {
-                        bad |= 1ull << r;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if ((w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
+                for (int u0 = 0; u0 < U; u0 += 32) {
+                    const int uu = u0 + lane % (U < 32 ? U : 32), r0 = U < 32 ? lane / U : 0;
+                    const long long src = kv_row + (long long)r0 * hk * D + 8 * uu;
+                    const uint16_t *kp = a.k_draft + src, *vp = a.v_draft + src;
+                    const long long step = (long long)AT_ONCE * hk * D;
+#pragma unroll 8
+                    for (int r = r0; r < nd; r += AT_ONCE) {
+                        const uint32_t off = bf16_off<D>(r, 8 * uu);
+                        cp_async_16(sk + off, kp);
+                        cp_async_16(sv + off, vp);
+                        kp += step;
+                        vp += step;
                     }
                 }
-                const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
-                const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
-                if (lane == 0) sh.bad[unit_no & 1] = (unsigned long long)bhi << 32 | blo;
+                cp_async_wait_all();
                 fence_proxy_async();  // read by the tensor core
                 __syncwarp();
                 if (lane == 0) {
@@ -250,22 +239,29 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
             const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
             const int t = (row0 + r) / a.group;
             const bool on = r < rows && t < rq.n_nodes;
+            // (the unit before last is through; this one's scan comes after every warp's q_ready)
+            if (threadIdx.x == 0) sh.bad[unit_no & 1] = 0;
             // this warp's query rows to shared memory (the last unit's products are done: its O was read)
             constexpr int U = D / 8;
-#pragma unroll 8
-            for (int i = lane; i < 32 * U; i += 32) {
-                const int rr = warp * 32 + i / U, uu = i % U, rw = row0 + rr, tt = rw / a.group;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (rr < rows && tt < rq.n_nodes)
-                    v = __ldg((const uint4 *)(a.q + (((long long)b * a.n_draft + tt) * a.q_heads + g * a.group + rw - tt * a.group) * D) + uu);
-                *(uint4 *)(smem + bf16_off<D>(rr, 8 * uu)) = v;
+            {
+                const long long mine = (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (row0 + r) - t * a.group) * D;
+                const uint32_t live = __ballot_sync(0xffffffffu, on);
+#pragma unroll 16
+                for (int i = lane; i < 32 * U; i += 32) {
+                    const int rr = i / U, uu = i % U;  // row of the warp (one per 32 or 16 lanes), unit
+                    const long long row = __shfl_sync(0xffffffffu, mine, rr);
+                    const bool has = (live >> rr) & 1u;
+                    cp_async_16_or_zero(smem_addr(smem + bf16_off<D>(warp * 32 + rr, 8 * uu)), has ? a.q + row + 8 * uu : a.q, has);
+                }
+                cp_async_wait_all();
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready));
 
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
-            float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+            float m = -INFINITY;
+            uint64_t l0 = 0, l1 = 0;  // the row's sum, in four parts
             bool draft_seen = false;
             unsigned long long word = ~0ull;
             for (int i = 0; i < n; ++i, ++it) {
@@ -284,28 +280,34 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                 tc_fence_after();
                 const uint32_t s_col = tmem + lane_base + C::S_COL + (uint32_t)(st * BN);
                 // the row's maximum of the tile
-                float top = -INFINITY;
+                float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int c0 = 0; c0 < BN; c0 += 32) {
-                    uint32_t s[32];
-                    tmem_load32(s_col + c0, s);
+                for (int c0 = 0; c0 < BN; c0 += 64) {
+                    uint32_t s[32], s1[32];
+                    tmem_load32x2(s_col + c0, s_col + c0 + 32, s, s1);
                     if (!full) {
-                        const uint32_t bits = chunk_bits(word, c0, valid);
+                        const uint32_t bits = chunk_bits(word, c0, valid), bits1 = chunk_bits(word, c0 + 32, valid);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
+                        for (int k = 0; k < 32; ++k) {
                             if (!((bits >> k) & 1u)) s[k] = 0xff800000u;
+                            if (!((bits1 >> k) & 1u)) s1[k] = 0xff800000u;
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) top = max3(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                    for (int k = 0; k < 32; k += 2) {
+                        top = max3(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                        top1 = max3(top1, __uint_as_float(s1[k]), __uint_as_float(s1[k + 1]));
+                    }
                 }
+                top = fmaxf(top, top1);
                 const float mt = top == -INFINITY ? -INFINITY : CAP ? score(top) : top * a.scale_log2;
                 // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
                 const bool up = mt > m + 8.0f;
                 if (__any_sync(0xffffffffu, up)) {
                     const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
                     if (up) m = mt;
-                    l0 *= f;
-                    l1 *= f;
+                    l0 = fma_pair(l0, pair_of(f, f), 0);
+                    l1 = fma_pair(l1, pair_of(f, f), 0);
                     if (i > 0) {
                         const int pst = (it - 1) % NS;
                         ok = warp_wait(smem_addr(&sh.v_done[pst]), ((it - 1) / NS) & 1, abort);
@@ -323,6 +325,7 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     }
                 }
                 const float neg = m == -INFINITY ? 0.0f : -m;
+                const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
 #pragma unroll
                 for (int c0 = 0; c0 < BN; c0 += 32) {
                     uint32_t s[32], p[16];
@@ -330,16 +333,17 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     const uint32_t bits = full ? 0xffffffffu : chunk_bits(word, c0, valid);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float e[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float v = __uint_as_float(s[2 * k + h]);
-                            e[h] = ex2(CAP ? score(v) + neg : fmaf(v, a.scale_log2, neg));
-                            if (!full && !((bits >> (2 * k + h)) & 1u)) e[h] = 0.0f;
+                        float2 v = make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+                        if (CAP) v = make_float2(score(v.x) + neg, score(v.y) + neg);
+                        else v = of_pair(fma_pair(pair_of(v.x, v.y), scale2, neg2));
+                        v = make_float2(ex2(v.x), ex2(v.y));
+                        if (!full) {
+                            if (!((bits >> (2 * k)) & 1u)) v.x = 0.0f;
+                            if (!((bits >> (2 * k + 1)) & 1u)) v.y = 0.0f;
                         }
-                        l0 += e[0];
-                        l1 += e[1];
-                        p[k] = pack_bf16(e[0], e[1]);
+                        if (k & 1) l1 = add_pair(l1, pair_of(v.x, v.y));
+                        else l0 = add_pair(l0, pair_of(v.x, v.y));
+                        p[k] = pack_bf16(v.x, v.y);
                     }
                     tmem_st16(s_col + c0 / 2, p);
                 }
@@ -347,8 +351,26 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                 if (valid < BN) {  // rows past the last key hold whatever was there: 0 * that must be 0
                     ok = warp_wait(smem_addr(&sh.v_full[st]), par, abort);
                     if (!ok) break;
+                    uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
                     for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += kRowWarps * 32)
-                        *(uint4 *)(smem + C::OFF_V + st * C::KV_BYTES + bf16_off<D>(e / U, (e % U) * 8)) = make_uint4(0, 0, 0, 0);
+                        *(uint4 *)(vt + bf16_off<D>(e / U, (e % U) * 8)) = make_uint4(0, 0, 0, 0);
+                    // Drafted values that are not finite leave the tile: 0 * inf would reach rows that may not
+                    // see them. Rows that do get them at the end.
+                    for (int e = threadIdx.x; draft && e < valid * U; e += kRowWarps * 32) {
+                        uint16_t *w = (uint16_t *)(vt + bf16_off<D>(e / U, (e % U) * 8));
+                        const uint4 v = *(const uint4 *)w;
+                        const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+                        bool any = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            any = any || (ww[k] & 0x7f80u) == 0x7f80u || (ww[k] & 0x7f800000u) == 0x7f800000u;
+                        if (any) {
+                            atomicOr(&sh.bad[unit_no & 1], 1ull << (e / U));
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if ((w[k] & 0x7f80u) == 0x7f80u) w[k] = 0;
+                        }
+                    }
                     fence_proxy_async();
                 }
                 tc_fence_before();
@@ -363,7 +385,8 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
             if (ok) {
                 const bool whole = t0 == 0 && t1 == n_tiles;
                 const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
-                const float l = l0 + l1;
+                const float2 la = of_pair(l0), lb = of_pair(l1);
+                const float l = (la.x + lb.x) + (la.y + lb.y);
                 const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
                 const int hq = g * a.group + (row0 + r) - t * a.group;
                 const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
@@ -394,24 +417,30 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                             if (!isfinite(y) && ((word >> k) & 1ull)) o[e] = __float_as_uint(fmaf(p, y, __uint_as_float(o[e])));
                         }
                     }
-                    if (r < rows) {
-                        // a row without a key has nothing (not 0 * what the columns hold)
+                    // a row without a key has nothing (not 0 * what the columns hold)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = on && l != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
-                        float *of = !whole ? a.ws_o + (slot * kTreeTileRows + r) * D + c0 : (float *)a.out + at * D + c0;
-                        if (!whole || a.out_dtype == EKV_DTYPE_F32) {
+                    for (int e = 0; e < 32; ++e) o[e] = on && l != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+                    // through the warp's query rows, which are done with, so that whole rows of 128 bytes are
+                    // written: unit k of row i lies at unit k ^ (i & 7) of 128 bytes
+                    uint8_t *stage = smem + warp * 32 * D * 2;
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) *(uint4 *)(of + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int k = 0; k < 8; ++k)
+                        *(uint4 *)(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    __syncwarp();
+                    const int unit = lane & 7;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = 4 * k + (lane >> 3), rr = warp * 32 + i;
+                        const uint4 v = *(const uint4 *)(stage + i * 128 + ((unit ^ (i & 7)) << 4));
+                        const long long row = __shfl_sync(0xffffffffu, at, i);
+                        if (rr >= rows) continue;
+                        if (!whole) {
+                            *(uint4 *)(a.ws_o + (slot * kTreeTileRows + rr) * D + c0 + 4 * unit) = v;
+                        } else if (a.out_dtype == EKV_DTYPE_F32) {
+                            *(uint4 *)((float *)a.out + row * D + c0 + 4 * unit) = v;
                         } else {
-                            uint16_t *ob = (uint16_t *)a.out + at * D + c0;
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    w[k] = pack_bf16(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1]));
-                                *(uint4 *)(ob + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
+                            *(uint2 *)((uint16_t *)a.out + row * D + c0 + 4 * unit) =
+                                make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)), pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
                         }
                     }
                     __syncwarp();
