@@ -134,8 +134,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     bool ok = true;
     int b = rg.b;
     uint32_t base = rg.base;
+    Req rq{};
+    int rq_of = -1;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        const Req rq = load_req(a, b, warp == 0);
+        if (b != rq_of) rq = load_req(a, b, warp == 0), rq_of = b;
         const int n_tiles = unit_tiles(rq);
         const uint32_t span = (uint32_t)n_tiles * units_per_req;
         if (x >= base + span) {
@@ -733,16 +735,19 @@ enum class Shape { R8, R16, R32, R64, Tile };
 
 Shape shape_for(const PoolView &p, int rows) {
     const int head_dim = p.head_dim;
-    if (tree_tile_fits(p, rows)) return Shape::Tile;
+    if (tree_tile_rows(p, rows)) return Shape::Tile;
     if (rows <= 8) return Shape::R8;
     if (rows <= 16) return Shape::R16;
     if (rows <= 32 && head_dim <= 128) return Shape::R32;
     return Shape::R64;
 }
-int tile_rows(Shape s) { return s == Shape::Tile ? kTreeTileRows : s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64; }
+int tile_rows(Shape s, const PoolView &p, int rows) {
+    if (s == Shape::Tile) return tree_tile_rows(p, rows);
+    return s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64;
+}
 
-int grid_ctas(Shape s, const PoolView &p, int sms) {
-    if (s == Shape::Tile) return tree_tile_ctas(p, sms);
+int grid_ctas(Shape s, const PoolView &p, int rows, int sms) {
+    if (s == Shape::Tile) return tree_tile_ctas(p, rows, sms);
     return sms * rows_ctas(p.head_dim, p.dtype == EKV_DTYPE_Q8_0, s == Shape::R8 ? 1 : s == Shape::R32 ? 4 : 2, s == Shape::R64 ? 4 : 1);
 }
 
@@ -751,7 +756,7 @@ struct WsLayout {
 };
 WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
     const Shape sh = shape_for(p, rows);
-    const size_t slots = 2ull * grid_ctas(sh, p, sms) * tile_rows(sh);
+    const size_t slots = 2ull * grid_ctas(sh, p, rows, sms) * tile_rows(sh, p, rows);
     WsLayout w;
     w.parts = 0;
     w.ml = ((size_t)n_batch * p.kv_heads * rt * sizeof(int2) + 255) / 256 * 256;
@@ -792,25 +797,27 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
         rc = launch_shape<D, false>(a, sh, grid, s);
     }
     if (rc || !a.split) return rc;
+    const int tr = tile_rows(sh, a.pool, a.n_draft * a.group);
     const int n_rows = a.n_batch * a.pool.kv_heads * a.n_draft * a.group;
     // a warp per row once that fills the SMs
     if (n_rows >= 4 * kMergeWarps * grid)
-        return launch_after(tree_merge_kernel<D, 1>, (n_rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, s, a, tile_rows(sh), n_rows);
-    return launch_after(tree_merge_kernel<D, kMergeWarps>, n_rows, kMergeWarps * 32, 0, s, a, tile_rows(sh), n_rows);
+        return launch_after(tree_merge_kernel<D, 1>, (n_rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, s, a, tr, n_rows);
+    return launch_after(tree_merge_kernel<D, kMergeWarps>, n_rows, kMergeWarps * 32, 0, s, a, tr, n_rows);
 }
 
 }  // namespace
 
 size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, int sms) {
     const int rows = n_draft * (q_heads / p.kv_heads);
-    const int tr = tile_rows(shape_for(p, rows));
+    const int tr = tile_rows(shape_for(p, rows), p, rows);
     return ws_layout(p, n_batch, rows, (rows + tr - 1) / tr, sms).total;
 }
 
 int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s) {
     const int rows = a.n_draft * a.group;
     const Shape sh = shape_for(a.pool, rows);
-    a.row_tiles = (rows + tile_rows(sh) - 1) / tile_rows(sh);
+    const int tr = tile_rows(sh, a.pool, rows);
+    a.row_tiles = (rows + tr - 1) / tr;
     const int64_t units = (int64_t)a.n_batch * a.pool.kv_heads * a.row_tiles;
     const int64_t all_rows = (int64_t)a.n_batch * a.pool.kv_heads * rows;
     const WsLayout w = ws_layout(a.pool, a.n_batch, rows, a.row_tiles, sms);
@@ -818,7 +825,7 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     const int64_t unit_tiles = (max_len + kTile - 1) / kTile + 1;
     const int64_t most_tiles = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile + 2;
     if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
-    const int full = grid_ctas(sh, a.pool, sms);
+    const int full = grid_ctas(sh, a.pool, rows, sms);
     // Units of one or two tiles are not worth a second launch; without a workspace a unit is one CTA's.
     a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2 && units * most_tiles < INT32_MAX;
     int64_t grid = units;

@@ -3,11 +3,15 @@
 // The same sums as ekv_tree.cu. From about 64 rows per cached key the tensor pipe bounds the call, not the
 // bytes, so 128 rows take the 5th-generation tensor cores: S = Q K^T with both operands in shared memory and S
 // in tensor memory, P = exp(S - m) as bf16 over S's own columns, O += P V with P read from tensor memory.
-// A CTA holds one 128-row tile: warps 0-3 are the softmax (a thread is a row), warp 4 issues the products,
-// warp 5 feeds K and V through the copy engine (pool tiles are canonical operands as they are stored). Up to
-// head_dim 128 two CTAs share an SM, 256 tensor-memory columns each: while one takes exponentials the other's
-// products run, so that a CTA needs neither a second S nor a second K/V stage. At head_dim 256 one CTA has two
-// of each and issues S(j + 1) before P V(j).
+// Four warps are the softmax of a 128-row tile (a thread is a row), one warp issues the products, one feeds K
+// and V through the copy engine (pool tiles are canonical operands as they are stored).
+// Exponentials and products take about as long (128 keys of 128 rows at head_dim 128: 1024 cycles of each), so
+// two row tiles share an SM and while one takes exponentials the other's products run:
+//   RT = 2 (head_dim 64 or 128, more than 128 rows): one CTA holds two row tiles of a KV head, which read each
+//     K/V tile once between them; 256 tensor-memory columns each, two K/V stages.
+//   RT = 1 (up to 128 rows): two CTAs per SM of one row tile each, with one K/V stage.
+//   RT = 1 at head_dim 256: one CTA, whose output leaves tensor memory for two S tiles: S(j + 1) runs under the
+//     exponentials of S(j).
 #include "ekv_decode.cuh"
 
 namespace ekv {
@@ -16,31 +20,37 @@ namespace {
 using namespace decode;
 using namespace sm100;
 
-template <int D>
+template <int D, int RT>
 struct TCfg {
-    static constexpr int BN = D > 128 ? 64 : 128;  // keys per tile
-    static constexpr int NS = D > 128 ? 2 : 1;     // S buffers, and K and V stages
-    static constexpr int CTAS = D > 128 ? 1 : 2;
+    static constexpr int BN = D > 128 ? 64 : 128;            // keys per tile
+    static constexpr int NSB = D > 128 ? 2 : 1;              // S tiles per row tile
+    static constexpr int NS = D > 128 || RT == 2 ? 2 : 1;    // K and V stages
+    static constexpr int CTAS = D > 128 || RT == 2 ? 1 : 2;  // per SM
     static constexpr uint32_t SBO = 16 * D;        // bytes between 8-row groups; chunks of 64 columns are 1024 apart
     static constexpr uint32_t LAYOUT = 2;          // 128-byte swizzle
     static constexpr int KV_BYTES = BN * D * 2;
     static constexpr int Q_BYTES = kTreeTileRows * D * 2;
-    static constexpr int S_COL = 0, O_COL = BN * NS, COLS = D > 128 ? 512 : 256;
-    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_SH = OFF_V + NS * KV_BYTES;
+    static constexpr int SLOT_COLS = 256;          // tensor-memory columns from row tile to row tile
+    static constexpr int S_COL = 0, O_COL = BN * NSB, COLS = D > 128 ? 512 : SLOT_COLS * RT;
+    static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_SH = OFF_V + NS * KV_BYTES;
     static constexpr int SMEM = OFF_SH + 1024 + 1024;
-    static_assert(O_COL + D <= COLS, "tensor memory");
-    static_assert(D % 64 == 0, "whole swizzle chunks");
+    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = ROW_WARPS + 1, THREADS = (ROW_WARPS + 2) * 32;
+    static_assert(O_COL + D <= (D > 128 ? 512 : SLOT_COLS), "tensor memory");
+    static_assert(D % 64 == 0 && (RT == 1 || D <= 128), "whole swizzle chunks; two outputs fit");
 };
 
+// Phases: k_full, v_full, s_full and v_done go by the tile's stage (tile / NS), p_full by its S tile (tile / NSB).
 struct TShared {
-    uint64_t k_full[2], v_full[2], s_full[2], p_full[2], v_done[2], q_ready, drained;
+    uint64_t k_full[2], v_full[2];
+    uint64_t s_full[2][2];  // [row tile][stage] S done, and of the last row tile: K read
+    uint64_t v_done[2][2];  // [row tile][stage] P V done, and of the last row tile: V read
+    uint64_t p_full[2][2];  // [row tile][S tile] P written
+    uint64_t q_ready, drained;
     unsigned long long bad[2];  // drafted keys of the unit (even, odd) whose values are not all finite
     uint32_t tmem;
     int abort;
     RangeScratch range;
 };
-
-constexpr int kRowWarps = 4, kTileThreads = (kRowWarps + 2) * 32;
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -55,10 +65,10 @@ __device__ __forceinline__ uint32_t chunk_bits(unsigned long long word, int c0, 
     return n >= 32 ? w : n <= 0 ? 0u : w & ((1u << n) - 1u);
 }
 
-template <int D, bool CAP>
-__global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(const TreeArgs a) {
-    using C = TCfg<D>;
-    constexpr int BN = C::BN, NS = C::NS;
+template <int D, int RT, bool CAP>
+__global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_tile_kernel(const TreeArgs a) {
+    using C = TCfg<D, RT>;
+    constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, ROWS = RT * kTreeTileRows;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     TShared &sh = *(TShared *)(smem + C::OFF_SH);
@@ -72,24 +82,26 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_addr(&sh.k_full[i]), 1);
             mbar_init(smem_addr(&sh.v_full[i]), 1);
-            mbar_init(smem_addr(&sh.s_full[i]), 1);
-            mbar_init(smem_addr(&sh.p_full[i]), kRowWarps);
-            mbar_init(smem_addr(&sh.v_done[i]), 1);
+            for (int k = 0; k < 2; ++k) {
+                mbar_init(smem_addr(&sh.s_full[i][k]), 1);
+                mbar_init(smem_addr(&sh.v_done[i][k]), 1);
+                mbar_init(smem_addr(&sh.p_full[i][k]), 4);
+            }
         }
-        mbar_init(smem_addr(&sh.q_ready), kRowWarps);
+        mbar_init(smem_addr(&sh.q_ready), C::ROW_WARPS);
         mbar_init(smem_addr(&sh.drained), 1);
         sh.abort = 0;
         sh.bad[0] = sh.bad[1] = 0;
         mbar_init_fence();
     }
-    if (warp == kRowWarps) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
+    if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
     auto unit_tiles = [](const Req &r) { return max(1, (r.n_prefix + BN - 1) / BN + (r.n_nodes > 0 ? 1 : 0)); };
     grid_wait();
     grid_launch_next();
     tc_fence_before();
     Range rg;
     if (a.split) {
-        rg = find_range<kTileThreads>(a.n_batch, units_per_req, sh.range,
+        rg = find_range<C::THREADS>(a.n_batch, units_per_req, sh.range,
                                       [&](int b) { return unit_tiles(load_req(a, b, false)); });
     } else {
         __syncthreads();
@@ -108,8 +120,10 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
     bool ok = true;
     int b = rg.b;
     uint32_t base = rg.base;
+    Req rq{};
+    int rq_of = -1;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        const Req rq = load_req(a, b, warp == 0);
+        if (b != rq_of) rq = load_req(a, b, warp == 0), rq_of = b;
         const int n_tiles = unit_tiles(rq);
         const uint32_t span = (uint32_t)n_tiles * units_per_req;
         if (x >= base + span) {
@@ -121,12 +135,11 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
         const int t0 = (int)(x - base) - u * n_tiles;
         const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
         const int n = t1 - t0;
-        const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * kTreeTileRows;
-        const int rows = min(kTreeTileRows, rows_all - row0);
+        const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * ROWS;
         const int p_tiles = (rq.n_prefix + BN - 1) / BN;
         const long long kv_row = ((long long)b * a.n_draft * hk + g) * D;
 
-        if (warp == kRowWarps + 1) {
+        if (warp == C::FEED_WARP) {
             // ---- feeder ----
             Piece next = find_piece<D, false, BN>(a, rq, g, t0 * BN, lane);
             if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
@@ -142,9 +155,9 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                 const uint32_t bk = smem_addr(&sh.k_full[st]), bv = smem_addr(&sh.v_full[st]);
                 if (pc.src && j < p_tiles)  // the stages are taken until the last tile's products are done: start the way from memory
                     bulk_prefetch_l2(pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2));
-                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.s_full[st]), par ^ 1, abort);  // K(it - NS) read
+                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.s_full[RT - 1][st]), par ^ 1, abort);  // K(it - NS) read
                 if (ok && j < p_tiles) issue_half<D>(pc, sk, bk, lane < 16, lane);
-                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.v_done[st]), par ^ 1, abort);  // V(it - NS) read
+                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.v_done[RT - 1][st]), par ^ 1, abort);  // V(it - NS) read
                 if (!ok) {
                     *abort = 1;
                     continue;
@@ -179,16 +192,17 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     mbar_arrive(bv);
                 }
             }
-        } else if (warp == kRowWarps) {
+        } else if (warp == C::MMA_WARP) {
             // ---- products ----
             if (lane == 0) {
                 const uint32_t id_s = idesc_f16(true, false, BN), id_o = idesc_f16(true, true, D);
                 const uint32_t q_addr = smem_addr(smem), k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
-                auto issue_s = [&](int i) {
+                auto s_at = [&](int slot, int i) { return tmem + (uint32_t)(slot * C::SLOT_COLS + C::S_COL + (i % NSB) * BN); };
+                auto issue_s = [&](int slot, int i) {
                     const int st = i % NS;
                     if (!mbar_wait(smem_addr(&sh.k_full[st]), (i / NS) & 1, abort, kWait)) return false;
                     tc_fence_after();
-                    const uint64_t qa = sdesc(q_addr, 16, C::SBO, C::LAYOUT);
+                    const uint64_t qa = sdesc(q_addr + slot * C::Q_BYTES, 16, C::SBO, C::LAYOUT);
                     const uint64_t kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
 #pragma unroll
                     for (int s4 = 0; s4 < D / 64; ++s4) {  // four 16-column steps of a 64-column chunk
@@ -198,15 +212,15 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                             av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
                             bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
                         }
-                        mma_ss_x4<false>(tmem + C::S_COL + (uint32_t)(st * BN), av, bv, id_s, s4 > 0 ? 1u : 0u);
+                        mma_ss_x4<false>(s_at(slot, i), av, bv, id_s, s4 > 0 ? 1u : 0u);
                     }
-                    mma_commit(smem_addr(&sh.s_full[st]));
+                    mma_commit(smem_addr(&sh.s_full[slot][st]));
                     return true;
                 };
-                auto issue_pv = [&](int i, bool first) {
+                auto issue_pv = [&](int slot, int i, bool first) {
                     const int st = i % NS;
                     if (!mbar_wait(smem_addr(&sh.v_full[st]), (i / NS) & 1, abort, kWait)) return false;
-                    if (!mbar_wait(smem_addr(&sh.p_full[st]), (i / NS) & 1, abort, kWait)) return false;
+                    if (!mbar_wait(smem_addr(&sh.p_full[slot][i % NSB]), (i / NSB) & 1, abort, kWait)) return false;
                     tc_fence_after();
                     const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
 #pragma unroll
@@ -215,43 +229,50 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                         uint64_t bv[4];
 #pragma unroll
                         for (int s = 0; s < 4; ++s) {
-                            av[s] = tmem + C::S_COL + (uint32_t)(st * BN + (4 * s4 + s) * 8);
+                            av[s] = s_at(slot, i) + (uint32_t)((4 * s4 + s) * 8);
                             bv[s] = vb + ((uint32_t)(4 * s4 + s) * 2u * C::SBO >> 4);
                         }
-                        mma_ts_x4<false>(tmem + C::O_COL, av, bv, id_o, (first && s4 == 0) ? 0u : 1u);
+                        mma_ts_x4<false>(tmem + (uint32_t)(slot * C::SLOT_COLS + C::O_COL), av, bv, id_o, (first && s4 == 0) ? 0u : 1u);
                     }
-                    mma_commit(smem_addr(&sh.v_done[st]));
+                    mma_commit(smem_addr(&sh.v_done[slot][st]));
                     return true;
                 };
+                // An S tile is free once its P V was issued: the tensor pipe runs them in order.
                 ok = ok && mbar_wait(smem_addr(&sh.q_ready), unit_no & 1, abort, kWait);
-                ok = ok && issue_s(it);
+#pragma unroll
+                for (int slot = 0; slot < RT; ++slot) ok = ok && issue_s(slot, it);
                 for (int i = 0; ok && i < n; ++i) {
-                    if (NS == 2 && i + 1 < n) ok = issue_s(it + i + 1);
-                    ok = ok && issue_pv(it + i, i == 0);
-                    if (NS == 1 && ok && i + 1 < n) ok = issue_s(it + i + 1);
+                    if (NSB == 2 && i + 1 < n) ok = issue_s(0, it + i + 1);
+#pragma unroll
+                    for (int slot = 0; slot < RT; ++slot) {
+                        ok = ok && issue_pv(slot, it + i, i == 0);
+                        if (NSB == 1 && ok && i + 1 < n) ok = issue_s(slot, it + i + 1);
+                    }
                 }
                 if (!ok) *abort = 1;
             }
             it += n;
         } else {
             // ---- softmax: thread = row ----
-            const int r = threadIdx.x;
-            const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-            const int t = (row0 + r) / a.group;
+            const int slot = warp >> 2, r = (warp & 3) * 32 + lane, row00 = row0 + slot * kTreeTileRows;
+            const int rows = max(0, min(kTreeTileRows, rows_all - row00));
+            const uint32_t lane_base = ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(slot * C::SLOT_COLS);
+            uint8_t *sq = smem + slot * C::Q_BYTES;
+            const int t = (row00 + r) / a.group;
             const bool on = r < rows && t < rq.n_nodes;
             // (the unit before last is through; this one's scan comes after every warp's q_ready)
             if (threadIdx.x == 0) sh.bad[unit_no & 1] = 0;
             // this warp's query rows to shared memory (the last unit's products are done: its O was read)
             constexpr int U = D / 8;
             {
-                const long long mine = (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (row0 + r) - t * a.group) * D;
+                const long long mine = (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (row00 + r) - t * a.group) * D;
                 const uint32_t live = __ballot_sync(0xffffffffu, on);
 #pragma unroll 16
                 for (int i = lane; i < 32 * U; i += 32) {
                     const int rr = i / U, uu = i % U;  // row of the warp (one per 32 or 16 lanes), unit
                     const long long row = __shfl_sync(0xffffffffu, mine, rr);
                     const bool has = (live >> rr) & 1u;
-                    cp_async_16_or_zero(smem_addr(smem + bf16_off<D>(warp * 32 + rr, 8 * uu)), has ? a.q + row + 8 * uu : a.q, has);
+                    cp_async_16_or_zero(smem_addr(sq + bf16_off<D>((warp & 3) * 32 + rr, 8 * uu)), has ? a.q + row + 8 * uu : a.q, has);
                 }
                 cp_async_wait_all();
             }
@@ -275,10 +296,10 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                                          : (t >= 63 ? ~0ull : (2ull << t) - 1);
                 }
                 const bool full = !draft && valid == BN;
-                ok = ok && warp_wait(smem_addr(&sh.s_full[st]), par, abort);
+                ok = ok && warp_wait(smem_addr(&sh.s_full[slot][st]), par, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t s_col = tmem + lane_base + C::S_COL + (uint32_t)(st * BN);
+                const uint32_t s_col = tmem + lane_base + C::S_COL + (uint32_t)((it % NSB) * BN);
                 // the row's maximum of the tile
                 float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
@@ -310,7 +331,7 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     l1 = fma_pair(l1, pair_of(f, f), 0);
                     if (i > 0) {
                         const int pst = (it - 1) % NS;
-                        ok = warp_wait(smem_addr(&sh.v_done[pst]), ((it - 1) / NS) & 1, abort);
+                        ok = warp_wait(smem_addr(&sh.v_done[slot][pst]), ((it - 1) / NS) & 1, abort);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -348,15 +369,17 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     tmem_st16(s_col + c0 / 2, p);
                 }
                 tmem_wait_st();
-                if (valid < BN) {  // rows past the last key hold whatever was there: 0 * that must be 0
+                // rows past the last key hold whatever was there: 0 * that must be 0 (the second row tile's product
+                // comes after the first's)
+                if (valid < BN && slot == 0) {
                     ok = warp_wait(smem_addr(&sh.v_full[st]), par, abort);
                     if (!ok) break;
                     uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
-                    for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += kRowWarps * 32)
+                    for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += 128)
                         *(uint4 *)(vt + bf16_off<D>(e / U, (e % U) * 8)) = make_uint4(0, 0, 0, 0);
                     // Drafted values that are not finite leave the tile: 0 * inf would reach rows that may not
                     // see them. Rows that do get them at the end.
-                    for (int e = threadIdx.x; draft && e < valid * U; e += kRowWarps * 32) {
+                    for (int e = threadIdx.x; draft && e < valid * U; e += 128) {
                         uint16_t *w = (uint16_t *)(vt + bf16_off<D>(e / U, (e % U) * 8));
                         const uint4 v = *(const uint4 *)w;
                         const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
@@ -375,27 +398,27 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[st]));
+                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[slot][it % NSB]));
             }
             if (ok && n > 0) {
-                ok = warp_wait(smem_addr(&sh.v_done[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
+                ok = warp_wait(smem_addr(&sh.v_done[slot][(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
                 tc_fence_after();
             }
             if (!ok) *abort = 1;
             if (ok) {
                 const bool whole = t0 == 0 && t1 == n_tiles;
-                const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
+                const long long part = (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS + slot * kTreeTileRows;
                 const float2 la = of_pair(l0), lb = of_pair(l1);
                 const float l = (la.x + lb.x) + (la.y + lb.y);
                 const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-                const int hq = g * a.group + (row0 + r) - t * a.group;
+                const int hq = g * a.group + (row00 + r) - t * a.group;
                 const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
                 if (r < rows) {
-                    if (!whole) a.ws_ml[slot * kTreeTileRows + r] = on ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+                    if (!whole) a.ws_ml[part + r] = on ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
                     else if (a.lse) a.lse[at] = on && l != 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
                 }
                 const unsigned long long bad = draft_seen ? sh.bad[unit_no & 1] : 0ull;
-                const uint32_t p_col = tmem + lane_base + C::S_COL + (uint32_t)(((it - 1) % NS) * BN);
+                const uint32_t p_col = tmem + lane_base + C::S_COL + (uint32_t)(((it - 1) % NSB) * BN);
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     uint32_t o[32];
@@ -422,7 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     for (int e = 0; e < 32; ++e) o[e] = on && l != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
                     // through the warp's query rows, which are done with, so that whole rows of 128 bytes are
                     // written: unit k of row i lies at unit k ^ (i & 7) of 128 bytes
-                    uint8_t *stage = smem + warp * 32 * D * 2;
+                    uint8_t *stage = sq + (warp & 3) * 32 * D * 2;
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         *(uint4 *)(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
@@ -430,12 +453,12 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
                     const int unit = lane & 7;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const int i = 4 * k + (lane >> 3), rr = warp * 32 + i;
+                        const int i = 4 * k + (lane >> 3), rr = (warp & 3) * 32 + i;
                         const uint4 v = *(const uint4 *)(stage + i * 128 + ((unit ^ (i & 7)) << 4));
                         const long long row = __shfl_sync(0xffffffffu, at, i);
                         if (rr >= rows) continue;
                         if (!whole) {
-                            *(uint4 *)(a.ws_o + (slot * kTreeTileRows + rr) * D + c0 + 4 * unit) = v;
+                            *(uint4 *)(a.ws_o + (part + rr) * D + c0 + 4 * unit) = v;
                         } else if (a.out_dtype == EKV_DTYPE_F32) {
                             *(uint4 *)((float *)a.out + row * D + c0 + 4 * unit) = v;
                         } else {
@@ -452,7 +475,7 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
         x += n;
     }
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 11);
-    if (warp == kRowWarps + 1 && !ok && lane == 0) {
+    if (warp == C::FEED_WARP && !ok && lane == 0) {
         for (int i = 0; i < NS; ++i) {  // leave no copy writing this CTA's shared memory
             mbar_wait_drain(smem_addr(&sh.k_full[i]), 0, kWait / 64);
             mbar_wait_drain(smem_addr(&sh.k_full[i]), 1, kWait / 64);
@@ -460,35 +483,44 @@ __global__ void __launch_bounds__(kTileThreads, TCfg<D>::CTAS) tree_tile_kernel(
             mbar_wait_drain(smem_addr(&sh.v_full[i]), 1, kWait / 64);
         }
     }
-    if (warp == kRowWarps && lane == 0) {  // nor a product using its tensor memory
+    if (warp == C::MMA_WARP && lane == 0) {  // nor a product using its tensor memory
         mma_commit(smem_addr(&sh.drained));
         mbar_wait_drain(smem_addr(&sh.drained), 0, kWait);
     }
     __syncthreads();
-    if (warp == kRowWarps) tmem_dealloc(tmem, C::COLS);
+    if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
 }
 
-template <int D, bool CAP>
+template <int D, int RT>
 int launch(const TreeArgs &a, int grid, cudaStream_t s) {
-    static std::atomic<uint64_t> smem_done{0};
-    if (const int rc = allow_smem(tree_tile_kernel<D, CAP>, TCfg<D>::SMEM, smem_done)) return rc;
-    return launch_after(tree_tile_kernel<D, CAP>, grid, kTileThreads, TCfg<D>::SMEM, s, a);
+    using C = TCfg<D, RT>;
+    static std::atomic<uint64_t> done{0}, done_cap{0};
+    if (a.cap_log2 != 0.0f) {
+        if (const int rc = allow_smem(tree_tile_kernel<D, RT, true>, C::SMEM, done_cap)) return rc;
+        return launch_after(tree_tile_kernel<D, RT, true>, grid, C::THREADS, C::SMEM, s, a);
+    }
+    if (const int rc = allow_smem(tree_tile_kernel<D, RT, false>, C::SMEM, done)) return rc;
+    return launch_after(tree_tile_kernel<D, RT, false>, grid, C::THREADS, C::SMEM, s, a);
 }
 
 }  // namespace
 
-bool tree_tile_fits(const PoolView &p, int rows) {
-    return p.dtype == EKV_DTYPE_BF16 && (p.head_dim == 64 || p.head_dim == 128 || p.head_dim == 256) && rows > 64;
+int tree_tile_rows(const PoolView &p, int rows) {
+    if (p.dtype != EKV_DTYPE_BF16 || rows <= 64) return 0;
+    if (p.head_dim == 64 || p.head_dim == 128) return rows > kTreeTileRows ? 2 * kTreeTileRows : kTreeTileRows;
+    return p.head_dim == 256 ? kTreeTileRows : 0;
 }
 
-int tree_tile_ctas(const PoolView &p, int sms) { return sms * (p.head_dim > 128 ? 1 : 2); }
+int tree_tile_ctas(const PoolView &p, int rows, int sms) {
+    return sms * (p.head_dim <= 128 && rows <= kTreeTileRows ? 2 : 1);
+}
 
 int launch_tree_tile(const TreeArgs &a, int grid, cudaStream_t s) {
-    const bool cap = a.cap_log2 != 0.0f;
+    const bool two = a.n_draft * a.group > kTreeTileRows;
     switch (a.pool.head_dim) {
-        case 64: return cap ? launch<64, true>(a, grid, s) : launch<64, false>(a, grid, s);
-        case 128: return cap ? launch<128, true>(a, grid, s) : launch<128, false>(a, grid, s);
-        case 256: return cap ? launch<256, true>(a, grid, s) : launch<256, false>(a, grid, s);
+        case 64: return two ? launch<64, 2>(a, grid, s) : launch<64, 1>(a, grid, s);
+        case 128: return two ? launch<128, 2>(a, grid, s) : launch<128, 1>(a, grid, s);
+        case 256: return launch<256, 1>(a, grid, s);
         default: return EKV_ERR_UNSUPPORTED;
     }
 }

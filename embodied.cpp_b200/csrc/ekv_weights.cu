@@ -84,8 +84,10 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
     bool ok = true;
     int b = rg.b;
     uint32_t base = rg.base;
+    Req rq{};
+    int rq_of = -1;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        const Req rq = request(b, warp == 0);
+        if (b != rq_of) rq = request(b, warp == 0), rq_of = b;
         const int n_tiles = (rq.n_prefix + kTile - 1) / kTile;
         const uint32_t span = (uint32_t)n_tiles * hk;
         if (x >= base + span) {
