@@ -3,15 +3,17 @@
 // The same sums as ekv_tree.cu. From about 64 rows per cached key the tensor pipe bounds the call, not the
 // bytes, so 128 rows take the 5th-generation tensor cores: S = Q K^T with both operands in shared memory and S
 // in tensor memory, P = exp(S - m) as bf16 over S's own columns, O += P V with P read from tensor memory.
-// Four warps are the softmax of a 128-row tile (a thread is a row), one warp issues the products, one feeds K
+// Four warps are the softmax of a 128-row tile (a thread is a row) and one more issues its products; one feeds K
 // and V through the copy engine (pool tiles are canonical operands as they are stored).
-// Exponentials and products take about as long (128 keys of 128 rows at head_dim 128: 1024 cycles of each), so
-// two row tiles share an SM and while one takes exponentials the other's products run:
+// A row tile has two S tiles of 64 keys, so that S(j + 1) is computed under the exponentials of S(j); and
+// exponentials and products take about as long (64 keys of 128 rows at head_dim 128: 512 cycles of the one, 640 of
+// the other), so two row tiles share an SM and take turns on both pipes:
 //   RT = 2 (head_dim 64 or 128, more than 128 rows): one CTA holds two row tiles of a KV head, which read each
-//     K/V tile once between them; 256 tensor-memory columns each, two K/V stages.
-//   RT = 1 (up to 128 rows): two CTAs per SM of one row tile each, with one K/V stage.
-//   RT = 1 at head_dim 256: one CTA, whose output leaves tensor memory for two S tiles: S(j + 1) runs under the
-//     exponentials of S(j).
+//     K/V tile once between them; 256 tensor-memory columns each.
+//   RT = 1 (up to 128 rows): two CTAs per SM of one row tile each; at head_dim 256 one CTA, by its size.
+// With one S tile of 128 keys per row tile instead, the chain S, maximum, exponentials, P V left the tensor pipe
+// idle half of the time: 4300 cycles per 128 keys of two row tiles. With one issuing warp for both row tiles its
+// barrier waits, about 220 idle cycles each, took half: 5080 cycles.
 #include "ekv_decode.cuh"
 
 namespace ekv {
@@ -22,9 +24,8 @@ using namespace sm100;
 
 template <int D, int RT>
 struct TCfg {
-    static constexpr int BN = D > 128 ? 64 : 128;            // keys per tile
-    static constexpr int NSB = D > 128 ? 2 : 1;              // S tiles per row tile
-    static constexpr int NS = D > 128 || RT == 2 ? 2 : 1;    // K and V stages
+    static constexpr int BN = 64, NSB = 2;                   // keys per tile; S tiles per row tile
+    static constexpr int NS = RT == 2 || D == 64 ? 4 : 2;    // K and V stages
     static constexpr int CTAS = D > 128 || RT == 2 ? 1 : 2;  // per SM
     static constexpr uint32_t SBO = 16 * D;        // bytes between 8-row groups; chunks of 64 columns are 1024 apart
     static constexpr uint32_t LAYOUT = 2;          // 128-byte swizzle
@@ -34,19 +35,23 @@ struct TCfg {
     static constexpr int S_COL = 0, O_COL = BN * NSB, COLS = D > 128 ? 512 : SLOT_COLS * RT;
     static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_SH = OFF_V + NS * KV_BYTES;
     static constexpr int SMEM = OFF_SH + 1024 + 1024;
-    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = ROW_WARPS + 1, THREADS = (ROW_WARPS + 2) * 32;
+    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = ROW_WARPS + RT, THREADS = (FEED_WARP + 1) * 32;
     static_assert(O_COL + D <= (D > 128 ? 512 : SLOT_COLS), "tensor memory");
     static_assert(D % 64 == 0 && (RT == 1 || D <= 128), "whole swizzle chunks; two outputs fit");
 };
 
-// Phases: k_full, v_full, s_full and v_done go by the tile's stage (tile / NS), p_full by its S tile (tile / NSB).
+// Phases: full, s_full, v_done and v_clean go by the tile's stage (tile / NS), p_full by its S tile (tile / NSB),
+// q_ready by the CTA's unit. The two row tiles run at most NS tiles apart, as a stage is refilled after both.
 struct TShared {
-    uint64_t k_full[2], v_full[2];
-    uint64_t s_full[2][2];  // [row tile][stage] S done, and of the last row tile: K read
-    uint64_t v_done[2][2];  // [row tile][stage] P V done, and of the last row tile: V read
+    uint64_t full[4];       // K and V of the stage have landed
+    uint64_t s_full[2][4];  // [row tile][stage] S done
+    uint64_t v_done[2][4];  // [row tile][stage] P V done
     uint64_t p_full[2][2];  // [row tile][S tile] P written
-    uint64_t q_ready, drained;
-    unsigned long long bad[2];  // drafted keys of the unit (even, odd) whose values are not all finite
+    uint64_t q_ready[2];    // [row tile] query rows in shared memory
+    uint64_t v_clean[4];    // the first row tile's warps have made rows without a key zero and taken what is not
+                            // finite out of the drafts
+    uint64_t drained[2];
+    unsigned long long bad[8];  // [unit % 8] drafted keys of the unit whose values are not all finite
     uint32_t tmem;
     int abort;
     RangeScratch range;
@@ -79,19 +84,20 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     const int rows_all = a.n_draft * a.group;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&sh.k_full[i]), 1);
-            mbar_init(smem_addr(&sh.v_full[i]), 1);
-            for (int k = 0; k < 2; ++k) {
-                mbar_init(smem_addr(&sh.s_full[i][k]), 1);
-                mbar_init(smem_addr(&sh.v_done[i][k]), 1);
-                mbar_init(smem_addr(&sh.p_full[i][k]), 4);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(smem_addr(&sh.full[i]), 2);
+            mbar_init(smem_addr(&sh.v_clean[i]), 4);
+            for (int k = 0; k < RT; ++k) {
+                mbar_init(smem_addr(&sh.s_full[k][i]), 1);
+                mbar_init(smem_addr(&sh.v_done[k][i]), 1);
             }
         }
-        mbar_init(smem_addr(&sh.q_ready), C::ROW_WARPS);
-        mbar_init(smem_addr(&sh.drained), 1);
+        for (int k = 0; k < RT; ++k) {
+            for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 4);
+            mbar_init(smem_addr(&sh.q_ready[k]), 4);
+            mbar_init(smem_addr(&sh.drained[k]), 1);
+        }
         sh.abort = 0;
-        sh.bad[0] = sh.bad[1] = 0;
         mbar_init_fence();
     }
     if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
@@ -138,6 +144,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
         const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * ROWS;
         const int p_tiles = (rq.n_prefix + BN - 1) / BN;
         const long long kv_row = ((long long)b * a.n_draft * hk + g) * D;
+        auto tile_full = [&](int j) { return (j + 1) * BN <= rq.n_prefix; };
 
         if (warp == C::FEED_WARP) {
             // ---- feeder ----
@@ -152,18 +159,19 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 if (j + 1 < min(t1, p_tiles)) next = find_piece<D, false, BN>(a, rq, g, (j + 1) * BN, lane);
                 const uint32_t sk = smem_addr(smem + C::OFF_K + st * C::KV_BYTES);
                 const uint32_t sv = smem_addr(smem + C::OFF_V + st * C::KV_BYTES);
-                const uint32_t bk = smem_addr(&sh.k_full[st]), bv = smem_addr(&sh.v_full[st]);
-                if (pc.src && j < p_tiles)  // the stages are taken until the last tile's products are done: start the way from memory
+                const uint32_t bar = smem_addr(&sh.full[st]);
+                if (NS < 4 && pc.src && j < p_tiles)  // the stage may be taken for a while: start the way from memory
                     bulk_prefetch_l2(pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2));
-                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.s_full[RT - 1][st]), par ^ 1, abort);  // K(it - NS) read
-                if (ok && j < p_tiles) issue_half<D>(pc, sk, bk, lane < 16, lane);
-                if (it >= NS) ok = ok && warp_wait(smem_addr(&sh.v_done[RT - 1][st]), par ^ 1, abort);  // V(it - NS) read
+                if (it >= NS) {
+#pragma unroll
+                    for (int k = 0; k < RT; ++k) ok = ok && warp_wait(smem_addr(&sh.v_done[k][st]), par ^ 1, abort);
+                }
                 if (!ok) {
                     *abort = 1;
                     continue;
                 }
                 if (j < p_tiles) {
-                    issue_half<D>(pc, sv, bv, lane >= 16, lane);
+                    issue_piece<D, false, true>(a, pc, sk, sv, bar, bar, lane);
                     continue;
                 }
                 // drafted rows, from the caller's buffers: a lane keeps its 16-byte unit of the rows
@@ -188,19 +196,20 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 fence_proxy_async();  // read by the tensor core
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bk);
-                    mbar_arrive(bv);
+                    mbar_arrive(bar);
+                    mbar_arrive(bar);
                 }
             }
-        } else if (warp == C::MMA_WARP) {
+        } else if (warp >= C::MMA_WARP) {
             // ---- products ----
+            const int slot = warp - C::MMA_WARP;
             if (lane == 0) {
                 const uint32_t id_s = idesc_f16(true, false, BN), id_o = idesc_f16(true, true, D);
                 const uint32_t q_addr = smem_addr(smem), k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
-                auto s_at = [&](int slot, int i) { return tmem + (uint32_t)(slot * C::SLOT_COLS + C::S_COL + (i % NSB) * BN); };
-                auto issue_s = [&](int slot, int i) {
+                auto s_at = [&](int i) { return tmem + (uint32_t)(slot * C::SLOT_COLS + C::S_COL + (i % NSB) * BN); };
+                auto issue_s = [&](int i) {
                     const int st = i % NS;
-                    if (!mbar_wait(smem_addr(&sh.k_full[st]), (i / NS) & 1, abort, kWait)) return false;
+                    if (!mbar_wait(smem_addr(&sh.full[st]), (i / NS) & 1, abort, kWait)) return false;
                     tc_fence_after();
                     const uint64_t qa = sdesc(q_addr + slot * C::Q_BYTES, 16, C::SBO, C::LAYOUT);
                     const uint64_t kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
@@ -212,14 +221,13 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                             av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
                             bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
                         }
-                        mma_ss_x4<false>(s_at(slot, i), av, bv, id_s, s4 > 0 ? 1u : 0u);
+                        mma_ss_x4<false>(s_at(i), av, bv, id_s, s4 > 0 ? 1u : 0u);
                     }
                     mma_commit(smem_addr(&sh.s_full[slot][st]));
                     return true;
                 };
-                auto issue_pv = [&](int slot, int i, bool first) {
+                auto issue_pv = [&](int i, bool first) {
                     const int st = i % NS;
-                    if (!mbar_wait(smem_addr(&sh.v_full[st]), (i / NS) & 1, abort, kWait)) return false;
                     if (!mbar_wait(smem_addr(&sh.p_full[slot][i % NSB]), (i / NSB) & 1, abort, kWait)) return false;
                     tc_fence_after();
                     const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
@@ -229,7 +237,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                         uint64_t bv[4];
 #pragma unroll
                         for (int s = 0; s < 4; ++s) {
-                            av[s] = s_at(slot, i) + (uint32_t)((4 * s4 + s) * 8);
+                            av[s] = s_at(i) + (uint32_t)((4 * s4 + s) * 8);
                             bv[s] = vb + ((uint32_t)(4 * s4 + s) * 2u * C::SBO >> 4);
                         }
                         mma_ts_x4<false>(tmem + (uint32_t)(slot * C::SLOT_COLS + C::O_COL), av, bv, id_o, (first && s4 == 0) ? 0u : 1u);
@@ -237,17 +245,14 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     mma_commit(smem_addr(&sh.v_done[slot][st]));
                     return true;
                 };
-                // An S tile is free once its P V was issued: the tensor pipe runs them in order.
-                ok = ok && mbar_wait(smem_addr(&sh.q_ready), unit_no & 1, abort, kWait);
-#pragma unroll
-                for (int slot = 0; slot < RT; ++slot) ok = ok && issue_s(slot, it);
+                // S(j + 1) goes over P(j - 1), whose product was issued before: the tensor pipe runs them in order.
+                ok = ok && mbar_wait(smem_addr(&sh.q_ready[slot]), unit_no & 1, abort, kWait);
+                ok = ok && issue_s(it);
                 for (int i = 0; ok && i < n; ++i) {
-                    if (NSB == 2 && i + 1 < n) ok = issue_s(0, it + i + 1);
-#pragma unroll
-                    for (int slot = 0; slot < RT; ++slot) {
-                        ok = ok && issue_pv(slot, it + i, i == 0);
-                        if (NSB == 1 && ok && i + 1 < n) ok = issue_s(slot, it + i + 1);
-                    }
+                    if (i + 1 < n) ok = issue_s(it + i + 1);
+                    if (slot > 0 && !tile_full(t0 + i))
+                        ok = ok && mbar_wait(smem_addr(&sh.v_clean[(it + i) % NS]), ((it + i) / NS) & 1, abort, kWait);
+                    ok = ok && issue_pv(it + i, i == 0);
                 }
                 if (!ok) *abort = 1;
             }
@@ -260,8 +265,9 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             uint8_t *sq = smem + slot * C::Q_BYTES;
             const int t = (row00 + r) / a.group;
             const bool on = r < rows && t < rq.n_nodes;
-            // (the unit before last is through; this one's scan comes after every warp's q_ready)
-            if (threadIdx.x == 0) sh.bad[unit_no & 1] = 0;
+            // (units that the other row tile may still look at are at most NS back; this one's scan comes after every
+            // warp's q_ready)
+            if (threadIdx.x == 0) sh.bad[unit_no & 7] = 0;
             // this warp's query rows to shared memory (the last unit's products are done: its O was read)
             constexpr int U = D / 8;
             {
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready));
+            if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready[slot]));
 
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
             float m = -INFINITY;
@@ -295,30 +301,27 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                            : a.ancestors ? __ldg(a.ancestors + (long long)b * a.n_draft + t)
                                          : (t >= 63 ? ~0ull : (2ull << t) - 1);
                 }
-                const bool full = !draft && valid == BN;
+                const bool full = tile_full(j);
                 ok = ok && warp_wait(smem_addr(&sh.s_full[slot][st]), par, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t s_col = tmem + lane_base + C::S_COL + (uint32_t)((it % NSB) * BN);
+                const uint32_t s_col = tmem + lane_base + (uint32_t)(C::S_COL + (it % NSB) * BN);
                 // the row's maximum of the tile
+                uint32_t sa[32], sb[32];
+                tmem_load32x2(s_col, s_col + 32, sa, sb);
+                if (!full) {
+                    const uint32_t bits = chunk_bits(word, 0, valid), bits1 = chunk_bits(word, 32, valid);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        if (!((bits >> k) & 1u)) sa[k] = 0xff800000u;
+                        if (!((bits1 >> k) & 1u)) sb[k] = 0xff800000u;
+                    }
+                }
                 float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int c0 = 0; c0 < BN; c0 += 64) {
-                    uint32_t s[32], s1[32];
-                    tmem_load32x2(s_col + c0, s_col + c0 + 32, s, s1);
-                    if (!full) {
-                        const uint32_t bits = chunk_bits(word, c0, valid), bits1 = chunk_bits(word, c0 + 32, valid);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            if (!((bits >> k) & 1u)) s[k] = 0xff800000u;
-                            if (!((bits1 >> k) & 1u)) s1[k] = 0xff800000u;
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        top = max3(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-                        top1 = max3(top1, __uint_as_float(s1[k]), __uint_as_float(s1[k + 1]));
-                    }
+                for (int k = 0; k < 32; k += 2) {
+                    top = max3(top, __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]));
+                    top1 = max3(top1, __uint_as_float(sb[k]), __uint_as_float(sb[k + 1]));
                 }
                 top = fmaxf(top, top1);
                 const float mt = top == -INFINITY ? -INFINITY : CAP ? score(top) : top * a.scale_log2;
@@ -347,18 +350,16 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 }
                 const float neg = m == -INFINITY ? 0.0f : -m;
                 const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
-#pragma unroll
-                for (int c0 = 0; c0 < BN; c0 += 32) {
-                    uint32_t s[32], p[16];
-                    tmem_load32(s_col + c0, s);
-                    const uint32_t bits = full ? 0xffffffffu : chunk_bits(word, c0, valid);
+                // (a masked score is -inf, of which the exponential is 0; a capped one is not, so it is put back to 0)
+                auto to_p = [&](uint32_t (&s)[32], uint32_t bits, uint32_t col) {
+                    uint32_t p[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float2 v = make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
                         if (CAP) v = make_float2(score(v.x) + neg, score(v.y) + neg);
                         else v = of_pair(fma_pair(pair_of(v.x, v.y), scale2, neg2));
                         v = make_float2(ex2(v.x), ex2(v.y));
-                        if (!full) {
+                        if (CAP && !full) {
                             if (!((bits >> (2 * k)) & 1u)) v.x = 0.0f;
                             if (!((bits >> (2 * k + 1)) & 1u)) v.y = 0.0f;
                         }
@@ -366,13 +367,13 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                         else l0 = add_pair(l0, pair_of(v.x, v.y));
                         p[k] = pack_bf16(v.x, v.y);
                     }
-                    tmem_st16(s_col + c0 / 2, p);
-                }
+                    tmem_st16(col, p);
+                };
+                to_p(sa, full ? 0xffffffffu : chunk_bits(word, 0, valid), s_col);
+                to_p(sb, full ? 0xffffffffu : chunk_bits(word, 32, valid), s_col + 16);
                 tmem_wait_st();
-                // rows past the last key hold whatever was there: 0 * that must be 0 (the second row tile's product
-                // comes after the first's)
-                if (valid < BN && slot == 0) {
-                    ok = warp_wait(smem_addr(&sh.v_full[st]), par, abort);
+                if (!full && slot == 0) {  // rows past the last key hold whatever was there: 0 * that must be 0
+                    ok = warp_wait(smem_addr(&sh.full[st]), par, abort);
                     if (!ok) break;
                     uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
                     for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += 128)
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                         for (int k = 0; k < 4; ++k)
                             any = any || (ww[k] & 0x7f80u) == 0x7f80u || (ww[k] & 0x7f800000u) == 0x7f800000u;
                         if (any) {
-                            atomicOr(&sh.bad[unit_no & 1], 1ull << (e / U));
+                            atomicOr(&sh.bad[unit_no & 7], 1ull << (e / U));
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
                                 if ((w[k] & 0x7f80u) == 0x7f80u) w[k] = 0;
@@ -398,7 +399,10 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[slot][it % NSB]));
+                if (lane == 0) {
+                    mbar_arrive(smem_addr(&sh.p_full[slot][it % NSB]));
+                    if (RT == 2 && slot == 0) mbar_arrive(smem_addr(&sh.v_clean[st]));
+                }
             }
             if (ok && n > 0) {
                 ok = warp_wait(smem_addr(&sh.v_done[slot][(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     if (!whole) a.ws_ml[part + r] = on ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
                     else if (a.lse) a.lse[at] = on && l != 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
                 }
-                const unsigned long long bad = draft_seen ? sh.bad[unit_no & 1] : 0ull;
+                const unsigned long long bad = draft_seen ? sh.bad[unit_no & 7] : 0ull;
                 const uint32_t p_col = tmem + lane_base + C::S_COL + (uint32_t)(((it - 1) % NSB) * BN);
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
@@ -477,15 +481,13 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 11);
     if (warp == C::FEED_WARP && !ok && lane == 0) {
         for (int i = 0; i < NS; ++i) {  // leave no copy writing this CTA's shared memory
-            mbar_wait_drain(smem_addr(&sh.k_full[i]), 0, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.k_full[i]), 1, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.v_full[i]), 0, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.v_full[i]), 1, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full[i]), 0, kWait / 64);
+            mbar_wait_drain(smem_addr(&sh.full[i]), 1, kWait / 64);
         }
     }
-    if (warp == C::MMA_WARP && lane == 0) {  // nor a product using its tensor memory
-        mma_commit(smem_addr(&sh.drained));
-        mbar_wait_drain(smem_addr(&sh.drained), 0, kWait);
+    if (warp >= C::MMA_WARP && warp < C::FEED_WARP && lane == 0) {  // nor a product using its tensor memory
+        mma_commit(smem_addr(&sh.drained[warp - C::MMA_WARP]));
+        mbar_wait_drain(smem_addr(&sh.drained[warp - C::MMA_WARP]), 0, kWait);
     }
     __syncthreads();
     if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
