@@ -677,7 +677,7 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
     a.group = prm->q_heads / c.kv_heads;
     a.scale_log2 = prm->scale * log2e;
     a.cap_log2 = prm->softcap * log2e;
-    a.cap_in = prm->softcap > 0.0f ? 2.0f * log2e * prm->scale / prm->softcap : 0.0f;
+    a.cap_in = prm->softcap > 0.0f ? prm->scale / prm->softcap : 0.0f;
     a.seq_ids = prm->seq_ids;
     a.prefix_len = prm->prefix_len;
     a.n_nodes = prm->n_nodes;

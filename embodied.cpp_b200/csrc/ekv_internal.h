@@ -71,7 +71,7 @@ struct TreeArgs {
     int32_t layer, n_batch, n_draft, q_heads, group;
     float scale_log2;  // scale * log2(e)
     float cap_log2;    // softcap * log2(e), 0 = none
-    float cap_in;      // 2 * log2(e) * scale / softcap
+    float cap_in;      // scale / softcap
     int32_t out_dtype;
     const int32_t *seq_ids, *prefix_len, *n_nodes;
     const uint64_t *ancestors;  // [n_batch][n_draft], or null: a chain
@@ -82,7 +82,7 @@ struct TreeArgs {
     int32_t split;     // 0: CTA = unit
     int32_t row_tiles; // row tiles of one (request, KV head)
     int2 *parts;       // [units] first and last CTA of each unit
-    float2 *ws_ml;     // [2 * CTAs][rows] maximum (log2 domain) and sum
+    float4 *ws_ml;     // [2 * CTAs][rows] maximum (log2 domain), sum, sum of the rounded probabilities
     float *ws_o;       // [2 * CTAs][rows][D] unnormalised output
     // key weights
     float *weights;    // [n_batch][kv_heads][weight_stride]

@@ -4,6 +4,9 @@
 // drafted keys that t's ancestor word names:
 //   s_k = scale * q.k  (or cap * tanh(scale * q.k / cap)),  out = sum exp(s_k - m) v_k / sum exp(s_k - m),
 //   lse = m + ln sum exp(s_k - m).
+// Probabilities are rounded to bf16 for the products with V, so the output is divided by the sum of the rounded
+// ones (a row with one heavy key would carry that key's rounding otherwise); lse takes the sum before rounding.
+// Q8_0 caches round p times the value's scale, a different number per 32 columns, and divide by the plain sum.
 // One pass over the keys: a warp keeps the reference maximum m, the sum and the output of its rows in
 // registers (the running softmax of Milakov and Gimelshein 2018, with the output as in flash attention,
 // Dao et al. 2022). m moves only when a score is more than 2^8 above it; every quotient is exact about that.
@@ -46,7 +49,7 @@ struct Cfg {
     static constexpr int X_FIT = WK * ROWS <= 32 ? 128 : WK * ROWS <= 64 ? 64 : 32;
     static constexpr int X_COLS = X_FIT < D ? X_FIT : D <= 32 ? 32 : D <= 64 ? 64 : 128;
     static constexpr int X_BYTES = WK * ROWS * X_COLS * 4;
-    static constexpr int ML_BYTES = WK * ROWS * 8;
+    static constexpr int ML_BYTES = WK * ROWS * 16;
     // query rows in shared memory where the output's share of the registers leaves no room for them
     static constexpr bool Q_SMEM = D * NR > 256;
     static constexpr int Q_BYTES = Q_SMEM ? ROWS * q_row_bytes<D>() : 0;
@@ -82,7 +85,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float *xb = (float *)(smem + NST * C::STAGE);                   // [WK][ROWS][kXCols]
-    float2 *sml = (float2 *)(smem + NST * C::STAGE + C::X_BYTES);   // [WK][ROWS]
+    float4 *sml = (float4 *)(smem + NST * C::STAGE + C::X_BYTES);   // [WK][ROWS]: maximum, sum, rounded sum
     using Sh = Shared<NST>;
     static_assert(sizeof(Sh) <= 1024, "barrier block");
     Sh &sh = *(Sh *)(smem + NST * C::STAGE + C::X_BYTES + C::ML_BYTES);
@@ -268,11 +271,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                 }
             };
             float o[NR][KS][4];  // O^T: columns o_col(ds, kq, i), row 2 c + (i & 1)
-            float mx[NR][2], sum[NR][2];
+            float mx[NR][2], sum[NR][2], rsum[NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 mx[n][0] = mx[n][1] = -INFINITY;
-                sum[n][0] = sum[n][1] = 0.0f;
+                sum[n][0] = sum[n][1] = rsum[n][0] = rsum[n][1] = 0.0f;
 #pragma unroll
                 for (int ds = 0; ds < KS; ++ds)
 #pragma unroll
@@ -405,6 +408,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                                 f[e] = m == -INFINITY ? 1.0f : ex2(mx[n][e] - m);
                                 mx[n][e] = m;
                                 sum[n][e] *= f[e];
+                                rsum[n][e] *= f[e];
                             }
 #pragma unroll
                             for (int ds = 0; ds < KS; ++ds)
@@ -453,8 +457,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                         uint32_t p[NR][2];
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
-                            p[n][0] = movmatrix_trans(pack_bf16(s[n][0], s[n][1]));
-                            p[n][1] = movmatrix_trans(pack_bf16(s[n][2], s[n][3]));
+                            const uint32_t w0 = pack_bf16(s[n][0], s[n][1]), w1 = pack_bf16(s[n][2], s[n][3]);
+                            rsum[n][0] += __uint_as_float(w0 << 16) + __uint_as_float(w1 << 16);
+                            rsum[n][1] += __uint_as_float(w0 & 0xffff0000u) + __uint_as_float(w1 & 0xffff0000u);
+                            p[n][0] = movmatrix_trans(w0);
+                            p[n][1] = movmatrix_trans(w1);
                         }
 #pragma unroll
                         for (int ds = 0; ds < KS; ++ds) {
@@ -540,15 +547,18 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
             }
 
             // ---- join the key groups, write the rows ----
-            float scale_o[NR][2], l_tot[NR][2], m_tot[NR][2];
+            float scale_o[NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float l = sum[n][e];
+                    float l = sum[n][e], lr = Q8 ? sum[n][e] : rsum[n][e];
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-                    if (kq == 0) sml[wk * C::ROWS + wrow + 8 * n + 2 * c + e] = make_float2(mx[n][e], l);
+                    for (int x = 4; x < 32; x <<= 1) {
+                        l += __shfl_xor_sync(0xffffffffu, l, x);
+                        lr += __shfl_xor_sync(0xffffffffu, lr, x);
+                    }
+                    if (kq == 0) sml[wk * C::ROWS + wrow + 8 * n + 2 * c + e] = make_float4(mx[n][e], l, lr, 0.0f);
                 }
             asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
             const bool whole = t0 == 0 && t1 == n_tiles;
@@ -558,23 +568,23 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int r = wrow + 8 * n + 2 * c + e;
-                    float mt = -INFINITY, lt = 0.0f;
+                    float mt = -INFINITY, lt = 0.0f, lr = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WK; ++w) mt = fmaxf(mt, sml[w * C::ROWS + r].x);
                     const float mu = mt == -INFINITY ? 0.0f : mt;
 #pragma unroll
                     for (int w = 0; w < WK; ++w) {
-                        const float2 ml = sml[w * C::ROWS + r];
-                        lt += ml.y * ex2(ml.x - mu);
+                        const float4 ml = sml[w * C::ROWS + r];
+                        const float f = ex2(ml.x - mu);
+                        lt += ml.y * f;
+                        lr += ml.z * f;
                     }
-                    m_tot[n][e] = mt;
-                    l_tot[n][e] = lt;
                     scale_o[n][e] = mx[n][e] == -INFINITY ? 0.0f : ex2(mx[n][e] - mu);
-                    if (whole) scale_o[n][e] = lt == 0.0f ? 0.0f : scale_o[n][e] / lt;
+                    if (whole) scale_o[n][e] = lr == 0.0f ? 0.0f : scale_o[n][e] / lr;
                     if (wk != 0 || kq != 0 || r >= rows) continue;
                     const bool off = t_of[n][e] < 0;
                     if (!whole) {
-                        a.ws_ml[slot * C::ROWS + r] = off ? make_float2(-INFINITY, 0.0f) : make_float2(mt, lt);
+                        a.ws_ml[slot * C::ROWS + r] = off ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(mt, lt, lr, 0.0f);
                     } else if (a.lse) {
                         const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
                         a.lse[((long long)b * a.n_draft + t) * a.q_heads + hq] =
@@ -668,16 +678,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
     for (int c = part.x + lane; c <= part.y; c += 32) m = fmaxf(m, a.ws_ml[slot_of(c)].x);
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    float l = 0.0f;
+    float l = 0.0f, lr = 0.0f;
     float4 o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c0 = part.x; c0 <= part.y; c0 += 32) {
         float f = 0.0f;
         if (c0 + lane <= part.y) {
-            const float2 ml = a.ws_ml[slot_of(c0 + lane)];
+            const float4 ml = a.ws_ml[slot_of(c0 + lane)];
             f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
             l += f * ml.y;
+            lr += f * ml.z;
         }
         const int n = min(32, part.y + 1 - c0);
 #pragma unroll 4
@@ -697,8 +708,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
         }
     }
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int x = 1; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, x);
+        lr += __shfl_xor_sync(0xffffffffu, lr, x);
+    }
+    const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
     auto put = [&](int i, float4 v) {
         v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         if (a.out_dtype == EKV_DTYPE_F32) ((float4 *)((float *)a.out + at * D))[i] = v;
@@ -760,7 +774,7 @@ WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
     WsLayout w;
     w.parts = 0;
     w.ml = ((size_t)n_batch * p.kv_heads * rt * sizeof(int2) + 255) / 256 * 256;
-    w.o = w.ml + slots * sizeof(float2);
+    w.o = w.ml + slots * sizeof(float4);
     w.total = w.o + slots * p.head_dim * sizeof(float);
     return w;
 }
@@ -832,7 +846,7 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     if (a.split) {
         grid = std::min<int64_t>(full, units * unit_tiles);
         a.parts = (int2 *)ws;
-        a.ws_ml = (float2 *)((uint8_t *)ws + w.ml);
+        a.ws_ml = (float4 *)((uint8_t *)ws + w.ml);
         a.ws_o = (float *)((uint8_t *)ws + w.o);
     }
     switch (a.pool.head_dim) {

@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
             float m = -INFINITY;
-            uint64_t l0 = 0, l1 = 0;  // the row's sum, in four parts
+            uint64_t l0 = 0, l1 = 0, lr = 0;  // the row's sum in four parts, and the rounded probabilities' in two
             bool draft_seen = false;
             unsigned long long word = ~0ull;
             for (int i = 0; i < n; ++i, ++it) {
@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     if (up) m = mt;
                     l0 = fma_pair(l0, pair_of(f, f), 0);
                     l1 = fma_pair(l1, pair_of(f, f), 0);
+                    lr = fma_pair(lr, pair_of(f, f), 0);
                     if (i > 0) {
                         const int pst = (it - 1) % NS;
                         ok = warp_wait(smem_addr(&sh.v_done[slot][pst]), ((it - 1) / NS) & 1, abort);
@@ -366,6 +367,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                         if (k & 1) l1 = add_pair(l1, pair_of(v.x, v.y));
                         else l0 = add_pair(l0, pair_of(v.x, v.y));
                         p[k] = pack_bf16(v.x, v.y);
+                        lr = add_pair(lr, pair_of(__uint_as_float(p[k] << 16), __uint_as_float(p[k] & 0xffff0000u)));
                     }
                     tmem_st16(col, p);
                 };
@@ -412,13 +414,13 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             if (ok) {
                 const bool whole = t0 == 0 && t1 == n_tiles;
                 const long long part = (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS + slot * kTreeTileRows;
-                const float2 la = of_pair(l0), lb = of_pair(l1);
-                const float l = (la.x + lb.x) + (la.y + lb.y);
-                const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+                const float2 la = of_pair(l0), lb = of_pair(l1), lc = of_pair(lr);
+                const float l = (la.x + lb.x) + (la.y + lb.y), lrow = lc.x + lc.y;
+                const float f = !whole ? 1.0f : lrow == 0.0f ? 0.0f : 1.0f / lrow;
                 const int hq = g * a.group + (row00 + r) - t * a.group;
                 const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
                 if (r < rows) {
-                    if (!whole) a.ws_ml[part + r] = on ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+                    if (!whole) a.ws_ml[part + r] = on ? make_float4(m, l, lrow, 0.0f) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
                     else if (a.lse) a.lse[at] = on && l != 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
                 }
                 const unsigned long long bad = draft_seen ? sh.bad[unit_no & 7] : 0ull;
