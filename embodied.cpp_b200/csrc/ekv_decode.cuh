@@ -345,29 +345,54 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
 }
 
 // ---- copy-engine feeder ----
-// One lane's share of a 64- or 128-key tile of the paged prefix: lanes 0-15 copy K, 16-31 V, one run of rows
-// inside one block each (blocks hold a multiple of 8 rows and tiles start at multiples of 64, so a tile of 128
-// spans at most 16 of them).
+// One lane's share of a 64-key tile of the paged prefix: lanes 0-15 copy K, 16-31 V, one run of rows inside one
+// block each (blocks hold a multiple of 8 rows, so a tile spans at most 9 of them).
 struct Piece {
     const uint8_t *src;  // first row of the run (bf16: its row group; Q8_0: its int8 row), or null
     int row, n;          // first row inside the tile, rows (multiple of 8)
     int rib;             // first row inside the block
 };
 
-template <int D, bool Q8, int TILE = kTile>
-__device__ __forceinline__ Piece find_piece(const TreeArgs &a, const Req &rq, int head, int key0, int lane) {
+// Block ids of a window of the request's table, in shared memory: read from global memory tile by tile, their
+// latency bounded the feeder (one 16 KB tile per 0.9 us). Used by one warp.
+constexpr int kTableWindow = 128;
+struct TableWindow {
+    int *blocks;  // [kTableWindow], -1 where the table's entry is no block
+    int seq, lo, n;
+    __device__ __forceinline__ void reset(int *mem) {
+        blocks = mem;
+        seq = -1;
+        lo = n = 0;
+    }
+    // Entries [first, last] of the request, of which all up to `end` will be wanted in turn.
+    __device__ __forceinline__ void want(const PoolView &p, int sq, int first, int last, int end, int lane) {
+        if (sq == seq && first >= lo && last < lo + n) return;
+        __syncwarp();
+        seq = sq;
+        lo = first;
+        n = min(kTableWindow, end + 1 - first);
+        for (int i = lane; i < n; i += 32) blocks[i] = lookup_block(p, sq, first + i);
+        __syncwarp();
+    }
+};
+
+template <int D, bool Q8>
+__device__ __forceinline__ Piece find_piece(const TreeArgs &a, const Req &rq, int head, int key0, TableWindow &tw, int lane) {
     const PoolView &p = a.pool;
-    const int valid = min(TILE, rq.n_prefix - key0), n8 = (valid + 7) & ~7;
+    const int valid = min(kTile, rq.n_prefix - key0), n8 = (valid + 7) & ~7;
     const int kv = lane >> 4, i = lane & 15;
     Piece pc;
     pc.src = nullptr;
     pc.row = pc.n = pc.rib = 0;
+    if (valid <= 0) return pc;
     const int bt = p.block_tokens;
-    const int blk0 = p.bt_shift >= 0 ? key0 >> p.bt_shift : key0 / bt;
+    auto block_of = [&](int pos) { return p.bt_shift >= 0 ? pos >> p.bt_shift : pos / bt; };
+    const int blk0 = block_of(key0);
+    tw.want(p, rq.seq, blk0, block_of(key0 + valid - 1), block_of(rq.n_prefix - 1), lane);
     const int e = blk0 + i;
     const int r0 = max(key0, e * bt), r1 = min(key0 + n8, (e + 1) * bt);
     if (r1 <= r0) return pc;
-    const int blk = lookup_block(p, rq.seq, e);
+    const int blk = tw.blocks[e - tw.lo];
     if (blk < 0) return pc;
     pc.row = r0 - key0;
     pc.n = r1 - r0;
@@ -402,16 +427,6 @@ __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, 
     } else {
         bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2), bar);
     }
-}
-
-// One side of a bf16 tile: the lanes with `mine` copy their runs to `dst` (completion on `bar`).
-template <int D>
-__device__ __forceinline__ void issue_half(const Piece &pc, uint32_t dst, uint32_t bar, bool mine, int lane) {
-    const uint32_t bytes = mine && pc.src ? (uint32_t)(pc.n * D * 2) : 0u;
-    const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
-    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, all);
-    __syncwarp();
-    if (bytes) sm100::bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, bytes, bar);
 }
 
 // A query row in shared memory: padded by 16 bytes, so that eight rows' 16-byte units fall in eight different

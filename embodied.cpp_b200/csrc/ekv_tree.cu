@@ -68,6 +68,7 @@ struct Shared {
     unsigned long long bad[NST];  // drafted keys of the stage whose values are not all finite
     RangeScratch range;
     int abort;
+    int table[kTableWindow];
 };
 
 // Column of output accumulator (16-column step ds, element i) of lane row kq. Q8_0 kernels take the columns of a
@@ -135,6 +136,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
         }
     };
     bool ok = true;
+    TableWindow tw;  // (the feeder's)
+    tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
     Req rq{};
@@ -164,14 +167,14 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
 
         if (warp == C::NW) {
             // ---- feeder ----
-            Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
+            Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, tw, lane);
             if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
                 const unsigned long long end = base + (uint32_t)(u + 1) * n_tiles;
                 a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
             }
             for (int j = t0; j < t1; ++j, advance()) {
                 const Piece pc = next;
-                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
+                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, tw, lane);
                 if (turn > 0) ok = ok && warp_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort);
                 if (!ok) {
                     *abort = 1;

@@ -24,7 +24,7 @@ using namespace sm100;
 
 template <int D, int RT>
 struct TCfg {
-    static constexpr int BN = 64, NSB = 2;                   // keys per tile; S tiles per row tile
+    static constexpr int BN = kTile, NSB = 2;                   // keys per tile; S tiles per row tile
     static constexpr int NS = RT == 2 || D == 64 ? 4 : 2;    // K and V stages
     static constexpr int CTAS = D > 128 || RT == 2 ? 1 : 2;  // per SM
     static constexpr uint32_t SBO = 16 * D;        // bytes between 8-row groups; chunks of 64 columns are 1024 apart
@@ -55,6 +55,7 @@ struct TShared {
     uint32_t tmem;
     int abort;
     RangeScratch range;
+    int table[kTableWindow];
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -124,6 +125,8 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 
     int it = 0, unit_no = 0;  // tiles and units of this CTA so far
     bool ok = true;
+    TableWindow tw;  // (the feeder's)
+    tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
     Req rq{};
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 
         if (warp == C::FEED_WARP) {
             // ---- feeder ----
-            Piece next = find_piece<D, false, BN>(a, rq, g, t0 * BN, lane);
+            Piece next = find_piece<D, false>(a, rq, g, t0 * BN, tw, lane);
             if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
                 const unsigned long long end = base + (uint32_t)(u + 1) * n_tiles;
                 a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             for (int j = t0; j < t1; ++j, ++it) {
                 const int st = it % NS, par = (it / NS) & 1;
                 const Piece pc = next;
-                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, false, BN>(a, rq, g, (j + 1) * BN, lane);
+                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, false>(a, rq, g, (j + 1) * BN, tw, lane);
                 const uint32_t sk = smem_addr(smem + C::OFF_K + st * C::KV_BYTES);
                 const uint32_t sv = smem_addr(smem + C::OFF_V + st * C::KV_BYTES);
                 const uint32_t bar = smem_addr(&sh.full[st]);

@@ -36,6 +36,7 @@ struct WShared {
     uint64_t full[kMaxStages], empty[kMaxStages];
     RangeScratch range;
     int abort;
+    int table[kTableWindow];
 };
 
 template <int D, bool Q8>
@@ -82,6 +83,8 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
         }
     };
     bool ok = true;
+    TableWindow tw;  // (the feeder's)
+    tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
     Req rq{};
@@ -103,10 +106,10 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
             const int rows = min(q_rows, (rows_all - c0 + 15) / 16 * 16);
             if (warp == kWarps) {
                 // ---- feeder ----
-                Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, lane);
+                Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, tw, lane);
                 for (int j = t0; j < t1; ++j, advance()) {
                     const Piece pc = next;
-                    if (j + 1 < t1) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, lane);
+                    if (j + 1 < t1) next = find_piece<D, Q8>(a, rq, g, (j + 1) * kTile, tw, lane);
                     if (turn > 0) ok = ok && warp_wait(smem_addr(&sh.empty[st]), (turn - 1) & 1, abort);
                     if (!ok) {
                         *abort = 1;
@@ -118,14 +121,21 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
             }
             // ---- query rows c0 .. c0 + rows to shared memory, in the products' column order ----
             asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");  // the last rows are done with
-            for (int i = threadIdx.x; i < rows * (D / 8); i += kWarps * 32) {
-                const int r = i / (D / 8), u = i - r * (D / 8);
-                const int row = c0 + r, t = row / a.group;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < rows_all && t < rq.n_nodes)
-                    v = __ldg((const uint4 *)(a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row -
-                                                     t * a.group) * D) + u);
-                store_q_unit<Q8>(sq + r * C::QROW, u, v);
+            {
+                // a warp takes 32 / U rows at a time, a lane one 16-byte unit (or two) of them
+                constexpr int U = D / 8, UL = U < 32 ? U : 32, PER = 32 / UL;
+                const int sub = lane / UL;
+#pragma unroll 4
+                for (int r = warp * PER + sub; r < rows; r += kWarps * PER) {
+                    const int row = c0 + r, t = row / a.group;
+                    const bool on = sub < PER && row < rows_all && t < rq.n_nodes;
+                    const uint4 *src = (const uint4 *)(a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group) * D);
+#pragma unroll
+                    for (int u = lane % UL; u < U; u += UL) {
+                        const uint4 v = on ? __ldg(src + u) : make_uint4(0, 0, 0, 0);
+                        if (sub < PER) store_q_unit<Q8>(sq + r * C::QROW, u, v);
+                    }
+                }
             }
             for (int r = threadIdx.x; r < rows; r += kWarps * 32) {
                 const int row = c0 + r, t = row / a.group;
