@@ -99,7 +99,7 @@ __device__ __forceinline__ int log2_of(int pow2) { return 31 - __clz(pow2); }
 // ---- matrix instructions ----
 // D[16x8] += A[16x16] * B[16x8], bf16 operands, f32 accumulators.
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -224,9 +224,17 @@ struct ScoreFn {
     float scale_log2;  // scale * log2(e)
     float cap_log2;    // cap * log2(e), 0 = no cap
     float cap_in;      // scale / cap
-    __device__ __forceinline__ float operator()(float s) const {
-        if (cap_log2 == 0.0f) return s * scale_log2;
-        return cap_log2 * tanhf(s * cap_in);
+    __device__ __forceinline__ float capped(float s) const { return cap_log2 * tanhf(s * cap_in); }
+    // N scores in place, behind one branch
+    template <int N>
+    __device__ __forceinline__ void operator()(float (&s)[N]) const {
+        if (cap_log2 == 0.0f) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] *= scale_log2;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = capped(s[i]);
+        }
     }
 };
 
@@ -429,44 +437,53 @@ __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, 
     }
 }
 
-// A query row in shared memory: padded by 16 bytes, so that eight rows' 16-byte units fall in eight different
-// bank groups; in the column order of the products (q_col).
-template <int D>
-__host__ __device__ constexpr int q_row_bytes() { return 2 * D + 16; }
+// Bytes of a query row in shared memory, padded so that the operand loads below meet different banks: eight rows'
+// 16-byte units (bf16), or two rows' 64 bytes (Q8_0).
+template <int D, bool Q8>
+__host__ __device__ constexpr int q_row_bytes() { return 2 * D + (Q8 ? 64 : 16); }
 
-// 16 bytes (columns 8 u .. 8 u + 7) of a query row to their places.
-template <bool Q8>
-__device__ __forceinline__ void store_q_unit(uint8_t *row, int u, uint4 v) {
-    if (!Q8) {
-        *(uint4 *)(row + 16 * u) = v;
-        return;
+// Query operands of column steps 2 i and 2 i + 1 of the eight rows at `rows` (shared-memory address of the first).
+template <int D, bool Q8>
+__device__ __forceinline__ void load_q_steps(uint32_t rows, int i, int lane, uint32_t (&f)[4]) {
+    if (Q8) {
+        // in q_col's order a lane's columns of a 32-column group are 16 adjacent bytes
+        const uint4 v = lds128(rows + (lane >> 2) * q_row_bytes<D, Q8>() + 64 * i + (lane & 3) * 16);
+        f[0] = v.x;
+        f[1] = v.y;
+        f[2] = v.z;
+        f[3] = v.w;
+    } else {
+        ldmatrix_x4(f, rows + (lane & 7) * q_row_bytes<D, Q8>() + 64 * i + (lane >> 3) * 16);
     }
-    // columns 32 g + 8 c + 4 i + 2 h + {0, 1} go to places 32 g + 16 i + 8 h + 2 c + {0, 1}
-    uint32_t *d = (uint32_t *)(row + 64 * (u >> 2)) + (u & 3);
-    d[0] = v.x;
-    d[4] = v.y;
-    d[8] = v.z;
-    d[12] = v.w;
+}
+
+// A warp's share (row `first`, first + step, ...) of n query rows to shared memory; `src(row)`: the row's elements,
+// or null for a row of zeros. Wait with cp_async_wait_all().
+template <int D, bool Q8, class Src>
+__device__ __forceinline__ void stage_q_rows(uint32_t dst, int n, const uint16_t *any, int first, int step, int lane, Src src) {
+    // 32 / U rows at a time, a lane one 16-byte unit (or two) of them
+    constexpr int U = D / 8, UL = U < 32 ? U : 32, PER = 32 / UL;
+    const int sub = lane / UL;
+#pragma unroll 4
+    for (int r = first * PER + sub; r < n; r += step * PER) {
+        const uint16_t *row = src(r);
+#pragma unroll
+        for (int u = lane % UL; u < U; u += UL)
+            if (sub < PER) cp_async_16_or_zero(dst + r * q_row_bytes<D, Q8>() + 16 * u, row ? row + 8 * u : any, row != nullptr);
+    }
 }
 
 // ---- scores of one warp's 16 keys ----
 // Column order of the matrix products. bf16 caches: natural. Q8_0 caches: step 2 g + i of group g (32
 // columns) gives lane c of a quad the columns 32 g + 8 c + 4 i + {0, 1 | 2, 3}, so that a lane reads its
-// 8 bytes of a group in one load; query rows are loaded in the same order, and a product does not depend
+// 8 bytes of a group in one load; the query operands are taken in the same order, and a product does not depend
 // on it.
 template <bool Q8>
 __device__ __forceinline__ int q_col(int step, int c, int half) {
     return Q8 ? 32 * (step >> 1) + 8 * c + 4 * (step & 1) + 2 * half : 16 * step + 2 * c + 8 * half;
 }
 
-// B operands of one 16-key x 16-column step of a bf16 tile: b[0..1] keys 0-7, b[2..3] keys 8-15.
-template <int D>
-__device__ __forceinline__ void load_k_step(uint32_t tile, int key0, int step, int lane, uint32_t (&b)[4]) {
-    const int row = key0 + (lane & 7) + ((lane >> 4) << 3);
-    ldmatrix_x4(b, tile + bf16_off<D>(row, 16 * step + ((lane >> 3) & 1) * 8));
-}
-
-// A operand of the same step: keys are its rows.
+// A operand of one 16-key x 16-column step of a bf16 tile: keys are its rows.
 template <int D>
 __device__ __forceinline__ void load_k_rows(uint32_t tile, int key0, int step, int lane, uint32_t (&a)[4]) {
     ldmatrix_x4(a, tile + bf16_off<D>(key0 + (lane & 15), 16 * step + (lane >> 4) * 8));

@@ -52,7 +52,7 @@ struct Cfg {
     static constexpr int ML_BYTES = WK * ROWS * 16;
     // query rows in shared memory where the output's share of the registers leaves no room for them
     static constexpr bool Q_SMEM = D * NR > 256;
-    static constexpr int Q_BYTES = Q_SMEM ? ROWS * q_row_bytes<D>() : 0;
+    static constexpr int Q_BYTES = Q_SMEM ? ROWS * q_row_bytes<D, Q8>() : 0;
     static constexpr int FIXED = X_BYTES + ML_BYTES + Q_BYTES + 1024 + 1024;
     static constexpr int CTAS = rows_ctas(D, Q8, NR, WR);
     static constexpr int BUDGET = CTAS == 2 ? 112 * 1024 : 220 * 1024;
@@ -253,17 +253,14 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                 }
             }
             if constexpr (C::Q_SMEM) {  // the last rows were done with at the barriers of their end
-                for (int i = threadIdx.x; i < C::ROWS * (D / 8); i += C::NC) {
-                    const int rr = i / (D / 8), uu = i - rr * (D / 8);
-                    const uint16_t *src = q_row(row0 + rr);
-                    store_q_unit<Q8>(sq + rr * q_row_bytes<D>(), uu, src ? __ldg((const uint4 *)src + uu) : make_uint4(0, 0, 0, 0));
-                }
+                stage_q_rows<D, Q8>(smem_addr(sq), C::ROWS, a.q, warp, C::NW, lane, [&](int r) { return q_row(row0 + r); });
+                cp_async_wait_all();
                 asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
             }
             // operands of steps 2 i and 2 i + 1 (D is a multiple of 32 where they come from shared memory)
             auto load_q2 = [&](int n, int i, uint32_t (&f)[4]) {
                 if constexpr (C::Q_SMEM) {
-                    ldmatrix_x4(f, smem_addr(sq) + (wrow + 8 * n + (lane & 7)) * q_row_bytes<D>() + 64 * i + (lane >> 3) * 16);
+                    load_q_steps<D, Q8>(smem_addr(sq) + (wrow + 8 * n) * q_row_bytes<D, Q8>(), i, lane, f);
                 } else {
                     f[0] = qf[n][2 * i][0];
                     f[1] = qf[n][2 * i][1];
@@ -389,11 +386,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                             }
                         }
                     bool above = false;
+                    score(*(float(*)[4 * NR])s);
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[n][i] = score(s[n][i]);
                             if (masked && !((vis[n][i & 1] >> (kq + 8 * (i >> 1))) & 1u)) s[n][i] = -INFINITY;
                         }
                         above = above || fmaxf(s[n][0], s[n][2]) > mx[n][0] + 8.0f || fmaxf(s[n][1], s[n][3]) > mx[n][1] + 8.0f;

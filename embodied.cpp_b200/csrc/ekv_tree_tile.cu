@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     top1 = max3(top1, __uint_as_float(sb[k]), __uint_as_float(sb[k + 1]));
                 }
                 top = fmaxf(top, top1);
-                const float mt = top == -INFINITY ? -INFINITY : CAP ? score(top) : top * a.scale_log2;
+                const float mt = top == -INFINITY ? -INFINITY : CAP ? score.capped(top) : top * a.scale_log2;
                 // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
                 const bool up = mt > m + 8.0f;
                 if (__any_sync(0xffffffffu, up)) {
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float2 v = make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-                        if (CAP) v = make_float2(score(v.x) + neg, score(v.y) + neg);
+                        if (CAP) v = make_float2(score.capped(v.x) + neg, score.capped(v.y) + neg);
                         else v = of_pair(fma_pair(pair_of(v.x, v.y), scale2, neg2));
                         v = make_float2(ex2(v.x), ex2(v.y));
                         if (CAP && !full) {

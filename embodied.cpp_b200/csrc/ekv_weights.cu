@@ -2,6 +2,8 @@
 //   w[b][h][k] = decay * w[b][h][k] + sum over rows r of KV head h of exp(s_rk - lse_r)
 // with the scores s and the lse of ekv_tree_attention. Every key's sum is one CTA's, in a fixed order: no
 // atomics, the same result every time. K is read once, V not at all.
+// Keys are the rows of the products (S^T = K Q^T), so that a lane holds two keys and sums over query rows in its own
+// registers; with query rows as rows, twelve shuffles per tile made the consumer the bound (97 us for 16 x 16k keys).
 #include <algorithm>
 #include <type_traits>
 
@@ -21,7 +23,7 @@ template <int D, bool Q8>
 struct WCfg {
     using T = TileCfg<D, Q8>;
     static constexpr int STAGE = (T::KV_BYTES + 1023) / 1024 * 1024;
-    static constexpr int QROW = q_row_bytes<D>();
+    static constexpr int QROW = q_row_bytes<D, Q8>();
     static constexpr int QROWS = D > 128 ? 128 : 256;        // query rows held at a time
     // two CTAs per SM: what their query rows leave of half an SM's shared memory holds tiles in flight
     static constexpr int fixed(int rows) { return rows * (QROW + 4) + 1024 + 1024; }
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
         const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
 
         for (int c0 = 0; c0 < rows_all; c0 += q_rows) {
-            const int rows = min(q_rows, (rows_all - c0 + 15) / 16 * 16);
+            const int rows = min(q_rows, (rows_all - c0 + 7) / 8 * 8);
             if (warp == kWarps) {
                 // ---- feeder ----
                 Piece next = find_piece<D, Q8>(a, rq, g, t0 * kTile, tw, lane);
@@ -115,28 +117,23 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                         *abort = 1;
                         continue;
                     }
+                    // the weights that this tile adds to: from memory to L2 while the tile is on its way (3 lines of 128
+                    // bytes hold 64 of them at any alignment)
+                    if (lane < 3 && (c0 > 0 || a.decay != 0.0f)) {
+                        const float *w = a.weights + ((long long)b * hk + g) * a.weight_stride + j * kTile + lane * 32;
+                        if (j * kTile + lane * 32 < rq.n_prefix) asm volatile("prefetch.global.L2 [%0];" ::"l"(w));
+                    }
                     issue_piece<D, Q8, false>(a, pc, smem_addr(smem + st * C::STAGE), 0, smem_addr(&sh.full[st]), 0, lane);
                 }
                 continue;
             }
             // ---- query rows c0 .. c0 + rows to shared memory, in the products' column order ----
             asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");  // the last rows are done with
-            {
-                // a warp takes 32 / U rows at a time, a lane one 16-byte unit (or two) of them
-                constexpr int U = D / 8, UL = U < 32 ? U : 32, PER = 32 / UL;
-                const int sub = lane / UL;
-#pragma unroll 4
-                for (int r = warp * PER + sub; r < rows; r += kWarps * PER) {
-                    const int row = c0 + r, t = row / a.group;
-                    const bool on = sub < PER && row < rows_all && t < rq.n_nodes;
-                    const uint4 *src = (const uint4 *)(a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group) * D);
-#pragma unroll
-                    for (int u = lane % UL; u < U; u += UL) {
-                        const uint4 v = on ? __ldg(src + u) : make_uint4(0, 0, 0, 0);
-                        if (sub < PER) store_q_unit<Q8>(sq + r * C::QROW, u, v);
-                    }
-                }
-            }
+            stage_q_rows<D, Q8>(smem_addr(sq), rows, a.q, warp, kWarps, lane, [&](int r) -> const uint16_t * {
+                const int row = c0 + r, t = row / a.group;
+                if (row >= rows_all || t >= rq.n_nodes) return nullptr;
+                return a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group) * D;
+            });
             for (int r = threadIdx.x; r < rows; r += kWarps * 32) {
                 const int row = c0 + r, t = row / a.group;
                 float l = INFINITY;  // no such row, or one that saw nothing: weight 0
@@ -146,23 +143,24 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 }
                 slse[r] = l;
             }
+            cp_async_wait_all();
             asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
 
-            const int rq0 = lane >> 2, c = lane & 3;
+            const int kq = lane >> 2, c = lane & 3;  // keys kq and kq + 8, query rows 2 c and 2 c + 1 of a lane's elements
             const ScoreFn score{a.scale_log2, a.cap_log2, a.cap_in};
-            const int key_l = 16 * warp + 8 * ((rq0 >> 1) & 1) + 2 * c + (rq0 & 1);  // the key this lane writes (rq0 < 4)
+            const int key_l = 16 * warp + kq + 8 * (c & 1);  // the key this lane writes (c < 2)
             float *wrow = a.weights + ((long long)b * hk + g) * a.weight_stride;
             // the entry this lane adds to, a tile ahead
             auto load_old = [&](int j) {
                 const int key = j * kTile + key_l;
-                return rq0 < 4 && key < rq.n_prefix && j < t1 && (c0 > 0 || a.decay != 0.0f) ? wrow[key] : 0.0f;
+                return c < 2 && key < rq.n_prefix && j < t1 && (c0 > 0 || a.decay != 0.0f) ? wrow[key] : 0.0f;
             };
             float next_old = load_old(t0);
             for (int j = t0; j < t1; ++j, advance()) {
                 const int par = turn & 1;
                 const uint32_t sk = smem_addr(smem + st * C::STAGE);
                 const int key = j * kTile + key_l;
-                const bool writes = rq0 < 4 && key < rq.n_prefix;
+                const bool writes = c < 2 && key < rq.n_prefix;
                 const float old = next_old;
                 next_old = load_old(j + 1);
                 ok = ok && warp_wait(smem_addr(&sh.full[st]), par, abort);
@@ -172,86 +170,90 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 }
                 const int key0 = 16 * warp;
                 uint32_t kf[KS][4];
-                float sc[Q8 ? KS / 2 : 1][2][2];  // scales of the lane's keys by group
+                uint32_t sc0[Q8 ? (T::G32 + 1) / 2 : 1], sc1[Q8 ? (T::G32 + 1) / 2 : 1];  // scales of keys kq, kq + 8
                 if constexpr (!Q8) {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) load_k_step<D>(sk, key0, ks, lane, kf[ks]);
+                    for (int ks = 0; ks < KS; ++ks) load_k_rows<D>(sk, key0, ks, lane, kf[ks]);
                 } else {
 #pragma unroll
-                    for (int gr = 0; gr < KS / 2; ++gr)
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            const uint2 w = lds64(sk + q8_qs_off(key0 + 8 * n + rq0, 32 * gr + 8 * c, D));
-                            int8x4_to_bf16(w.x, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
-                            int8x4_to_bf16(w.y, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
-                            const int krow = key0 + 8 * n + 2 * c;
-                            sc[gr][n][0] = lds_f16(sk + T::SCALES + (krow * T::G32 + gr) * 2);
-                            sc[gr][n][1] = lds_f16(sk + T::SCALES + ((krow + 1) * T::G32 + gr) * 2);
-                        }
+                    for (int gr = 0; gr < KS / 2; ++gr) {
+                        const uint2 w0 = lds64(sk + q8_qs_off(key0 + kq, 32 * gr + 8 * c, D));
+                        const uint2 w1 = lds64(sk + q8_qs_off(key0 + kq + 8, 32 * gr + 8 * c, D));
+                        int8x4_to_bf16(w0.x, kf[2 * gr][0], kf[2 * gr][2]);
+                        int8x4_to_bf16(w1.x, kf[2 * gr][1], kf[2 * gr][3]);
+                        int8x4_to_bf16(w0.y, kf[2 * gr + 1][0], kf[2 * gr + 1][2]);
+                        int8x4_to_bf16(w1.y, kf[2 * gr + 1][1], kf[2 * gr + 1][3]);
+                    }
+                    load_scales<T::G32>(sk + T::SCALES + (key0 + kq) * T::G32 * 2, sc0);
+                    load_scales<T::G32>(sk + T::SCALES + (key0 + kq + 8) * T::G32 * 2, sc1);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&sh.empty[st]));  // the keys are in registers
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys (n, e): 8 n + 2 c + e, rows of this lane
-                // two 16-row tiles at a time: their products do not wait for one another
+                float acc0 = 0.0f, acc1 = 0.0f;
+                // M tiles of eight query rows at a time: their products do not wait for one another
                 auto row_tiles = [&](auto count, int r0) {
                     constexpr int M = decltype(count)::value;
-                    float s[M][2][4];
+                    float s[M][2][4];  // even and odd column steps (Q8_0: one sum of scaled groups)
 #pragma unroll
                     for (int m = 0; m < M; ++m)
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                        for (int i = 0; i < 4; ++i) s[m][0][i] = s[m][1][i] = 0.0f;
+                    const uint32_t qa = smem_addr(sq) + r0 * C::QROW;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.0f;
-                    const uint32_t qa = smem_addr(sq) + (r0 + (lane & 15)) * C::QROW + (lane >> 4) * 16;
-                    if constexpr (!Q8) {
+                    for (int i = 0; i < (KS + 1) / 2; ++i) {
+                        uint32_t f[M][4];
 #pragma unroll
-                        for (int ks = 0; ks < KS; ++ks)
+                        for (int m = 0; m < M; ++m) load_q_steps<D, Q8>(qa + m * 8 * C::QROW, i, lane, f[m]);
+                        if constexpr (!Q8) {
+#pragma unroll
+                            for (int m = 0; m < M; ++m) mma_bf16(s[m][0], kf[2 * i], f[m][0], f[m][1]);
+                            if (2 * i + 1 < KS) {
+#pragma unroll
+                                for (int m = 0; m < M; ++m) mma_bf16(s[m][1], kf[2 * i + 1], f[m][2], f[m][3]);
+                            }
+                        } else {
+                            float p[M][4];
 #pragma unroll
                             for (int m = 0; m < M; ++m) {
-                                uint32_t qf[4];
-                                ldmatrix_x4(qf, qa + m * 16 * C::QROW + 32 * ks);
-                                mma_bf16(s[m][0], qf, kf[ks][0], kf[ks][1]);
-                                mma_bf16(s[m][1], qf, kf[ks][2], kf[ks][3]);
+                                p[m][0] = p[m][1] = p[m][2] = p[m][3] = 0.0f;
+                                mma_bf16(p[m], kf[2 * i], f[m][0], f[m][1]);
                             }
-                    } else {
 #pragma unroll
-                        for (int gr = 0; gr < KS / 2; ++gr)
+                            for (int m = 0; m < M; ++m) mma_bf16(p[m], kf[2 * i + 1], f[m][2], f[m][3]);
+                            const float f0 = scale_of(sc0, i), f1 = scale_of(sc1, i);
 #pragma unroll
                             for (int m = 0; m < M; ++m) {
-                                uint32_t q0[4], q1[4];
-                                ldmatrix_x4(q0, qa + m * 16 * C::QROW + 64 * gr);
-                                ldmatrix_x4(q1, qa + m * 16 * C::QROW + 64 * gr + 32);
-#pragma unroll
-                                for (int n = 0; n < 2; ++n) {
-                                    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                    mma_bf16(p, q0, kf[2 * gr][2 * n], kf[2 * gr][2 * n + 1]);
-                                    mma_bf16(p, q1, kf[2 * gr + 1][2 * n], kf[2 * gr + 1][2 * n + 1]);
-                                    s[m][n][0] = fmaf(p[0], sc[gr][n][0], s[m][n][0]);
-                                    s[m][n][1] = fmaf(p[1], sc[gr][n][1], s[m][n][1]);
-                                    s[m][n][2] = fmaf(p[2], sc[gr][n][0], s[m][n][2]);
-                                    s[m][n][3] = fmaf(p[3], sc[gr][n][1], s[m][n][3]);
-                                }
+                                s[m][0][0] = fmaf(p[m][0], f0, s[m][0][0]);
+                                s[m][0][1] = fmaf(p[m][1], f0, s[m][0][1]);
+                                s[m][0][2] = fmaf(p[m][2], f1, s[m][0][2]);
+                                s[m][0][3] = fmaf(p[m][3], f1, s[m][0][3]);
                             }
+                        }
                     }
+                    float x[M][4];
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[m][k] = s[m][0][k] + s[m][1][k];
+                    score(*(float(*)[4 * M])x);
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
-                        const float l0 = slse[r0 + 16 * m + rq0], l1 = slse[r0 + 16 * m + rq0 + 8];
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                acc[2 * n + e] += ex2(score(s[m][n][e]) - l0) + ex2(score(s[m][n][2 + e]) - l1);
+                        const float2 l = *(const float2 *)&slse[r0 + 8 * m + 2 * c];
+                        acc0 += ex2(x[m][0] - l.x) + ex2(x[m][1] - l.y);
+                        acc1 += ex2(x[m][2] - l.x) + ex2(x[m][3] - l.y);
                     }
                 };
                 int r0 = 0;
 #pragma unroll 1
-                for (; r0 + 32 <= rows; r0 += 32) row_tiles(std::integral_constant<int, 2>(), r0);
-                if (r0 < rows) row_tiles(std::integral_constant<int, 1>(), r0);
+                for (; r0 + 32 <= rows; r0 += 32) row_tiles(std::integral_constant<int, 4>(), r0);
+#pragma unroll 1
+                for (; r0 < rows; r0 += 8) row_tiles(std::integral_constant<int, 1>(), r0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int m = 4; m < 32; m <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], m);
-                const float mine = rq0 & 2 ? (rq0 & 1 ? acc[3] : acc[2]) : (rq0 & 1 ? acc[1] : acc[0]);
+                for (int m = 1; m < 4; m <<= 1) {
+                    acc0 += __shfl_xor_sync(0xffffffffu, acc0, m);
+                    acc1 += __shfl_xor_sync(0xffffffffu, acc1, m);
+                }
+                const float mine = c & 1 ? acc1 : acc0;
                 if (writes) wrow[key] = old * (c0 > 0 ? 1.0f : a.decay) + mine;
             }
         }
@@ -270,7 +272,7 @@ template <int D, bool Q8>
 int launch(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
     using C = WCfg<D, Q8>;
     const int64_t rows = (int64_t)a.n_draft * a.group;
-    const int q_rows = (int)std::min<int64_t>((rows + 15) / 16 * 16, C::QROWS);
+    const int q_rows = (int)std::min<int64_t>((rows + 7) / 8 * 8, C::QROWS);
     const int smem = C::smem(q_rows);
     static std::atomic<uint64_t> smem_done{0};
     if (const int rc = allow_smem(key_weights_kernel<D, Q8>, 227 * 1024, smem_done)) return rc;
