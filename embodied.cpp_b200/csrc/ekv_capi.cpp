@@ -675,6 +675,8 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
     a.n_draft = prm->n_draft;
     a.q_heads = prm->q_heads;
     a.group = prm->q_heads / c.kv_heads;
+    a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);  // (not used at 1, where it is 2^32)
+    if ((int64_t)EKV_MAX_DRAFT * a.group * a.group >= 1ll << 32) return EKV_ERR_UNSUPPORTED;
     a.scale_log2 = prm->scale * log2e;
     a.cap_log2 = prm->softcap * log2e;
     a.cap_in = prm->softcap > 0.0f ? prm->scale / prm->softcap : 0.0f;

@@ -273,12 +273,14 @@ struct Range {
     int ctas;                // G
     int b;                   // request that holds tile lo
     uint32_t base;           // first tile of request b
+    Req req;                 // request b
 };
 
 struct RangeScratch {
     uint32_t warp_sum[32];
     uint32_t base;
     int b;
+    Req req;
 };
 
 // floor(total * c / g) for c <= g <= 2^16, in 32 bits.
@@ -287,9 +289,14 @@ __device__ __forceinline__ uint32_t range_lo(uint32_t total, uint32_t c, uint32_
     return c * q + c * r / g;
 }
 
-// All threads of the block (NT of them). tiles(b): tiles of one unit of request b.
-template <int NT, class Tiles>
-__device__ __forceinline__ Range find_range(int n_batch, int units_per_req, RangeScratch &sh, Tiles tiles) {
+// floor(row / group) for the row of a unit: row * group < 2^32 (checked at the call), group_mul = ceil(2^32 / group).
+__device__ __forceinline__ int row_token(const TreeArgs &a, int row) {
+    return a.group == 1 ? row : (int)__umulhi((uint32_t)row, a.group_mul);
+}
+
+// All threads of the block (NT of them). request(b): request b; tiles(r): tiles of one unit of a request.
+template <int NT, class Request, class Tiles>
+__device__ __forceinline__ Range find_range(int n_batch, int units_per_req, RangeScratch &sh, Request request, Tiles tiles) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = NT / 32;
     // inclusive scan of one chunk of NT requests; returns this thread's inclusive sum and the chunk's total
@@ -313,7 +320,9 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
     };
     Range r;
     r.total = 0;
-    const uint32_t v0 = tid < n_batch ? (uint32_t)(tiles(tid) * units_per_req) : 0u;
+    Req mine{};
+    if (tid < n_batch) mine = request(tid);
+    const uint32_t v0 = tid < n_batch ? (uint32_t)(tiles(mine) * units_per_req) : 0u;
     uint32_t incl0 = 0, chunk = 0;
     if (tid == 0) {
         sh.b = n_batch;
@@ -321,7 +330,7 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
     }
     for (int b0 = 0; b0 < n_batch; b0 += NT) {
         if (b0 > 0) __syncthreads();
-        const uint32_t v = b0 == 0 ? v0 : (b0 + tid < n_batch ? (uint32_t)(tiles(b0 + tid) * units_per_req) : 0u);
+        const uint32_t v = b0 == 0 ? v0 : (b0 + tid < n_batch ? (uint32_t)(tiles(request(b0 + tid)) * units_per_req) : 0u);
         const uint32_t incl = scan(v, chunk);
         if (b0 == 0) incl0 = incl;
         r.total += chunk;
@@ -337,18 +346,21 @@ __device__ __forceinline__ Range find_range(int n_batch, int units_per_req, Rang
         uint32_t v = v0, incl = incl0;
         if (n_batch > NT) {
             __syncthreads();
-            v = b0 + tid < n_batch ? (uint32_t)(tiles(b0 + tid) * units_per_req) : 0u;
+            if (b0 + tid < n_batch) mine = request(b0 + tid);
+            v = b0 + tid < n_batch ? (uint32_t)(tiles(mine) * units_per_req) : 0u;
             incl = scan(v, chunk);
         }
         if (v > 0 && base + incl - v <= r.lo && r.lo < base + incl) {
             sh.b = b0 + tid;
             sh.base = base + incl - v;
+            sh.req = mine;
         }
         base += chunk;
     }
     __syncthreads();
     r.b = sh.b;
     r.base = sh.base;
+    r.req = sh.req;
     return r;
 }
 
@@ -409,16 +421,17 @@ __device__ __forceinline__ Piece find_piece(const TreeArgs &a, const Req &rq, in
     return pc;
 }
 
-// Issue the lane's copies of a tile whose K lands at `dst_k` (completion on bar_k) and V at `dst_v`.
-// With WITH_V false only K is copied.
+// Issue the lane's copies of a tile whose K lands at `dst_k` (completion on bar_k) and V at `dst_v`; lane 0 arrives on
+// both. With WITH_V false only K is copied.
 template <int D, bool Q8, bool WITH_V>
 __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, uint32_t dst_k, uint32_t dst_v,
                                             uint32_t bar_k, uint32_t bar_v, int lane) {
     using C = TileCfg<D, Q8>;
     using namespace sm100;
+    constexpr int ROW = Q8 ? D : 2 * D, SROW = C::G32 * 2;  // bytes of a row, and of its scales
     const bool is_v = lane >= 16;
     const bool on = pc.src != nullptr && (WITH_V || !is_v);
-    const uint32_t bytes = !on ? 0u : Q8 ? (uint32_t)(pc.n * (D + C::G32 * 2)) : (uint32_t)(pc.n * D * 2);
+    const uint32_t bytes = !on ? 0u : (uint32_t)(pc.n * (ROW + (Q8 ? SROW : 0)));
     const uint32_t kb = __reduce_add_sync(0xffffffffu, is_v ? 0u : bytes);
     const uint32_t vb = WITH_V ? __reduce_add_sync(0xffffffffu, is_v ? bytes : 0u) : 0u;
     if (lane == 0) {
@@ -428,13 +441,10 @@ __device__ __forceinline__ void issue_piece(const TreeArgs &a, const Piece &pc, 
     __syncwarp();
     if (!on) return;
     const uint32_t dst = is_v ? dst_v : dst_k, bar = is_v ? bar_v : bar_k;
-    if (Q8) {
-        bulk_g2s(dst + pc.row * D, pc.src + pc.rib * D, (uint32_t)(pc.n * D), bar);
-        bulk_g2s(dst + C::SCALES + pc.row * C::G32 * 2, pc.src + (int64_t)a.pool.block_tokens * D + pc.rib * C::G32 * 2,
-                 (uint32_t)(pc.n * C::G32 * 2), bar);
-    } else {
-        bulk_g2s(dst + pc.row * D * 2, pc.src + pc.rib * D * 2, (uint32_t)(pc.n * D * 2), bar);
-    }
+    bulk_g2s(dst + pc.row * ROW, pc.src + pc.rib * ROW, (uint32_t)(pc.n * ROW), bar);
+    if (Q8)
+        bulk_g2s(dst + C::SCALES + pc.row * SROW, pc.src + (int64_t)a.pool.block_tokens * D + pc.rib * SROW,
+                 (uint32_t)(pc.n * SROW), bar);
 }
 
 // Bytes of a query row in shared memory, padded so that the operand loads below meet different banks: eight rows'

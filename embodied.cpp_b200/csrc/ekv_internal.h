@@ -69,6 +69,7 @@ struct AttnArgs {
 struct TreeArgs {
     PoolView pool;
     int32_t layer, n_batch, n_draft, q_heads, group;
+    uint32_t group_mul;  // ceil(2^32 / group) (group > 1)
     float scale_log2;  // scale * log2(e)
     float cap_log2;    // softcap * log2(e), 0 = none
     float cap_in;      // scale / softcap

@@ -116,11 +116,12 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     grid_launch_next();  // the merge's blocks may take their places; they wait for this grid's end
     if (a.split) {
         rg = find_range<C::THREADS>(a.n_batch, units_per_req, sh.range,
-                                    [&](int b) { return unit_tiles(load_req(a, b, false)); });
+                                    [&](int b) { return load_req(a, b, blockIdx.x == 0); }, unit_tiles);
     } else {
         __syncthreads();
         rg.b = blockIdx.x / units_per_req;
-        const int n = unit_tiles(load_req(a, rg.b, false));
+        rg.req = load_req(a, rg.b, threadIdx.x == 0);
+        const int n = unit_tiles(rg.req);
         rg.base = 0;
         rg.lo = (blockIdx.x - rg.b * units_per_req) * (uint32_t)n;
         rg.hi = rg.lo + n;
@@ -140,10 +141,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
-    Req rq{};
-    int rq_of = -1;  // the request that rq describes
+    Req rq = rg.req;
+    int rq_of = b;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        if (b != rq_of) rq = load_req(a, b, warp == 0), rq_of = b;
+        if (b != rq_of) rq = load_req(a, b, false), rq_of = b;
         const int n_tiles = unit_tiles(rq);
         const uint32_t span = (uint32_t)n_tiles * units_per_req;
         if (x >= base + span) {
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
         const long long kv_row = ((long long)b * a.n_draft * hk + g) * D;  // drafted token 0 of this head
         // query row r of the unit, or null where it does not take part
         auto q_row = [&](int r) -> const uint16_t * {
-            const int t = r / a.group;
+            const int t = row_token(a, r);
             if (r >= rows_all || t >= rq.n_nodes) return nullptr;
             return a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (r - t * a.group)) * D;
         };
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
             for (int n = 0; n < NR; ++n) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = row0 + wrow + 8 * n + 2 * c + e, t = r / a.group;
+                    const int r = row0 + wrow + 8 * n + 2 * c + e, t = row_token(a, r);
                     t_of[n][e] = r < rows_all && t < rq.n_nodes ? t : -1;
                 }
                 if constexpr (!C::Q_SMEM) {
@@ -473,15 +474,28 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     } else {
                         constexpr int G = D / 32;
                         const int kr[4] = {key0 + 2 * c, key0 + 2 * c + 1, key0 + 2 * c + 8, key0 + 2 * c + 9};
-                        uint32_t sc0[(G + 1) / 2], sc1[(G + 1) / 2];
-                        if (!draft) {
-                            load_scales<G>(sv + TileCfg<D, Q8>::SCALES + (key0 + kq) * G * 2, sc0);
-                            load_scales<G>(sv + TileCfg<D, Q8>::SCALES + (key0 + kq + 8) * G * 2, sc1);
+                        uint32_t sc[4][(G + 1) / 2];
+                        if (!draft)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) load_scales<G>(sv + TileCfg<D, Q8>::SCALES + kr[k] * G * 2, sc[k]);
+                        // the probabilities of row kq and keys kr, from the keys' lanes: as two bf16 each, which hold
+                        // 16 bits of them, through the 16-bit transpose
+                        float pt[NR][4];
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) {
+                            const uint32_t h0 = pack_bf16(s[n][0], s[n][1]), h1 = pack_bf16(s[n][2], s[n][3]);
+                            const uint32_t l0 = pack_bf16(s[n][0] - __uint_as_float(h0 << 16), s[n][1] - __uint_as_float(h0 & 0xffff0000u));
+                            const uint32_t l1 = pack_bf16(s[n][2] - __uint_as_float(h1 << 16), s[n][3] - __uint_as_float(h1 & 0xffff0000u));
+                            const uint32_t a0 = movmatrix_trans(h0), a1 = movmatrix_trans(h1), b0 = movmatrix_trans(l0), b1 = movmatrix_trans(l1);
+                            pt[n][0] = __uint_as_float(a0 << 16) + __uint_as_float(b0 << 16);
+                            pt[n][1] = __uint_as_float(a0 & 0xffff0000u) + __uint_as_float(b0 & 0xffff0000u);
+                            pt[n][2] = __uint_as_float(a1 << 16) + __uint_as_float(b1 << 16);
+                            pt[n][3] = __uint_as_float(a1 & 0xffff0000u) + __uint_as_float(b1 & 0xffff0000u);
                         }
 #pragma unroll
                         for (int gr = 0; gr < G; ++gr) {
                             uint32_t v0[4], v1[4];  // operands of the group's two 16-column steps
-                            float f0 = 1.0f, f1 = 1.0f;
+                            float f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
                             if (draft) {
                                 uint2 w[4];
 #pragma unroll
@@ -502,14 +516,14 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                                 int8x4_to_bf16(__byte_perm(w[2], w[3], 0x5140), v0[2], v0[3]);
                                 int8x4_to_bf16(__byte_perm(w[0], w[1], 0x7362), v1[0], v1[1]);
                                 int8x4_to_bf16(__byte_perm(w[2], w[3], 0x7362), v1[2], v1[3]);
-                                f0 = scale_of(sc0, gr);
-                                f1 = scale_of(sc1, gr);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) f[k] = scale_of(sc[k], gr);
                             }
                             // the values' scales ride on the probabilities, which are rounded once either way
 #pragma unroll
                             for (int n = 0; n < NR; ++n) {
-                                const uint32_t p0 = movmatrix_trans(pack_bf16(s[n][0] * f0, s[n][1] * f0));
-                                const uint32_t p1 = movmatrix_trans(pack_bf16(s[n][2] * f1, s[n][3] * f1));
+                                const uint32_t p0 = pack_bf16(pt[n][0] * f[0], pt[n][1] * f[1]);
+                                const uint32_t p1 = pack_bf16(pt[n][2] * f[2], pt[n][3] * f[3]);
                                 mma_bf16(o[n][2 * gr], v0, p0, p1);
                                 mma_bf16(o[n][2 * gr + 1], v1, p0, p1);
                             }
@@ -586,7 +600,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     if (!whole) {
                         a.ws_ml[slot * C::ROWS + r] = off ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(mt, lt, lr, 0.0f);
                     } else if (a.lse) {
-                        const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
+                        const int t = row_token(a, row0 + r), hq = g * a.group + (row0 + r) - t * a.group;
                         a.lse[((long long)b * a.n_draft + t) * a.q_heads + hq] =
                             off || lt == 0.0f ? -INFINITY : (mt + __log2f(lt)) * 0.6931471805599453f;
                     }
@@ -627,7 +641,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                         *(float4 *)(a.ws_o + (slot * C::ROWS + r) * D + cc * XC + col) = v;
                         continue;
                     }
-                    const int t = (row0 + r) / a.group, hq = g * a.group + (row0 + r) - t * a.group;
+                    const int t = row_token(a, row0 + r), hq = g * a.group + (row0 + r) - t * a.group;
                     if (t >= rq.n_nodes) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     const long long dst = (((long long)b * a.n_draft + t) * a.q_heads + hq) * D + cc * XC + col;
                     if (a.out_dtype == EKV_DTYPE_F32)
@@ -666,7 +680,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
     if (id >= n_rows) return;
     const int bg = id / rows_all, row = id - bg * rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
     const int b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
-    const int t = row / a.group, hq = g * a.group + row - t * a.group;
+    const int t = row_token(a, row), hq = g * a.group + row - t * a.group;
     const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
     grid_wait();
     const int2 part = a.parts[bg * a.row_tiles + rt];

@@ -109,11 +109,12 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     Range rg;
     if (a.split) {
         rg = find_range<C::THREADS>(a.n_batch, units_per_req, sh.range,
-                                      [&](int b) { return unit_tiles(load_req(a, b, false)); });
+                                      [&](int b) { return load_req(a, b, blockIdx.x == 0); }, unit_tiles);
     } else {
         __syncthreads();
         rg.b = blockIdx.x / units_per_req;
-        const int n = unit_tiles(load_req(a, rg.b, false));
+        rg.req = load_req(a, rg.b, threadIdx.x == 0);
+        const int n = unit_tiles(rg.req);
         rg.base = 0;
         rg.lo = (blockIdx.x - rg.b * units_per_req) * (uint32_t)n;
         rg.hi = rg.lo + n;
@@ -129,10 +130,10 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
-    Req rq{};
-    int rq_of = -1;  // the request that rq describes
+    Req rq = rg.req;
+    int rq_of = b;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        if (b != rq_of) rq = load_req(a, b, warp == 0), rq_of = b;
+        if (b != rq_of) rq = load_req(a, b, false), rq_of = b;
         const int n_tiles = unit_tiles(rq);
         const uint32_t span = (uint32_t)n_tiles * units_per_req;
         if (x >= base + span) {
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             const int rows = max(0, min(kTreeTileRows, rows_all - row00));
             const uint32_t lane_base = ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(slot * C::SLOT_COLS);
             uint8_t *sq = smem + slot * C::Q_BYTES;
-            const int t = (row00 + r) / a.group;
+            const int t = row_token(a, row00 + r);
             const bool on = r < rows && t < rq.n_nodes;
             // (units that the other row tile may still look at are at most NS back; this one's scan comes after every
             // warp's q_ready)

@@ -73,9 +73,9 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
         return r;
     };
     grid_wait();
-    const Range rg = find_range<kThreads>(a.n_batch, hk, sh.range, [&](int b) {
-        return (request(b, false).n_prefix + kTile - 1) / kTile;
-    });
+    const Range rg = find_range<kThreads>(
+        a.n_batch, hk, sh.range, [&](int b) { return request(b, blockIdx.x == 0); },
+        [](const Req &r) { return (r.n_prefix + kTile - 1) / kTile; });
 
     int st = 0, turn = 0;  // stage of the next tile, and how often the ring went round
     auto advance = [&]() {
@@ -89,10 +89,10 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
     tw.reset(sh.table);
     int b = rg.b;
     uint32_t base = rg.base;
-    Req rq{};
-    int rq_of = -1;  // the request that rq describes
+    Req rq = rg.req;
+    int rq_of = b;  // the request that rq describes
     for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
-        if (b != rq_of) rq = request(b, warp == 0), rq_of = b;
+        if (b != rq_of) rq = request(b, true), rq_of = b;
         const int n_tiles = (rq.n_prefix + kTile - 1) / kTile;
         const uint32_t span = (uint32_t)n_tiles * hk;
         if (x >= base + span) {
@@ -130,12 +130,12 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
             // ---- query rows c0 .. c0 + rows to shared memory, in the products' column order ----
             asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");  // the last rows are done with
             stage_q_rows<D, Q8>(smem_addr(sq), rows, a.q, warp, kWarps, lane, [&](int r) -> const uint16_t * {
-                const int row = c0 + r, t = row / a.group;
+                const int row = c0 + r, t = row_token(a, row);
                 if (row >= rows_all || t >= rq.n_nodes) return nullptr;
                 return a.q + (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group) * D;
             });
             for (int r = threadIdx.x; r < rows; r += kWarps * 32) {
-                const int row = c0 + r, t = row / a.group;
+                const int row = c0 + r, t = row_token(a, row);
                 float l = INFINITY;  // no such row, or one that saw nothing: weight 0
                 if (row < rows_all && t < rq.n_nodes) {
                     l = a.lse[((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group] * 1.4426950408889634f;
