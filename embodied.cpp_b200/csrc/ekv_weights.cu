@@ -18,6 +18,7 @@ using namespace sm100;
 constexpr int kWarps = 4;  // 16 keys of a 64-key tile each
 constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kMaxStages = 8;
+constexpr int kRowTiles = 2;  // tiles of eight query rows whose products run side by side
 
 template <int D, bool Q8>
 struct WCfg {
@@ -25,10 +26,12 @@ struct WCfg {
     static constexpr int STAGE = (T::KV_BYTES + 1023) / 1024 * 1024;
     static constexpr int QROW = q_row_bytes<D, Q8>();
     static constexpr int QROWS = D > 128 ? 128 : 256;        // query rows held at a time
-    // two CTAs per SM: what their query rows leave of half an SM's shared memory holds tiles in flight
+    // CTAs per SM by their registers (the keys' 16 rows are D / 4 of them); what their query rows leave of the shared
+    // memory holds tiles in flight
+    static constexpr int CTAS = D > 128 ? 2 : 3, ROOM = (CTAS == 2 ? 112 : 74) * 1024;
     static constexpr int fixed(int rows) { return rows * (QROW + 4) + 1024 + 1024; }
     static constexpr int stages(int rows) {
-        const int n = (112 * 1024 - fixed(rows)) / STAGE;
+        const int n = (ROOM - fixed(rows)) / STAGE;
         return n < 2 ? 2 : n > kMaxStages ? kMaxStages : n;
     }
     static constexpr int smem(int rows) { return stages(rows) * STAGE + fixed(rows); }
@@ -42,7 +45,7 @@ struct WShared {
 };
 
 template <int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs a, int q_rows, int nst) {
+__global__ void __launch_bounds__(kThreads, WCfg<D, Q8>::CTAS) key_weights_kernel(const TreeArgs a, int q_rows, int nst) {
     using C = WCfg<D, Q8>;
     using T = TileCfg<D, Q8>;
     constexpr int KS = D / 16;
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 2) key_weights_kernel(const TreeArgs
                 };
                 int r0 = 0;
 #pragma unroll 1
-                for (; r0 + 32 <= rows; r0 += 32) row_tiles(std::integral_constant<int, 4>(), r0);
+                for (; r0 + 8 * kRowTiles <= rows; r0 += 8 * kRowTiles) row_tiles(std::integral_constant<int, kRowTiles>(), r0);
 #pragma unroll 1
                 for (; r0 < rows; r0 += 8) row_tiles(std::integral_constant<int, 1>(), r0);
 #pragma unroll
@@ -279,7 +282,7 @@ int launch(const TreeArgs &a, int max_len, int sms, cudaStream_t s) {
     const int64_t most = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile;
     if ((int64_t)a.n_batch * a.pool.kv_heads * most > INT32_MAX) return EKV_ERR_UNSUPPORTED;
     const int64_t tiles = (int64_t)a.n_batch * a.pool.kv_heads * ((max_len + kTile - 1) / kTile);
-    const int ctas = smem > 112 * 1024 ? 1 : 2;
+    const int ctas = std::min(C::CTAS, 227 * 1024 / (smem + 1024));
     const int grid = (int)std::min<int64_t>((int64_t)sms * ctas, std::max<int64_t>(1, tiles));
     return launch_after(key_weights_kernel<D, Q8>, grid, kThreads, smem, s, a, q_rows, C::stages(q_rows));
 }

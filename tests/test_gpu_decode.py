@@ -27,6 +27,8 @@ def run_tree(c, q, kd, vd, *, nodes=None, up=None, cap=0.0, dtype=torch.bfloat16
     out = torch.full((B, T, hq, d), 77.0, dtype=dtype, device="cuda")
     lse = torch.full((B, T, hq), 77.0, device="cuda")
     ws = torch.full((c.pool.tree_attention_workspace_size(prm),), 255, dtype=torch.uint8, device="cuda") if workspace else None
+    if stream is not None:  # the buffers were filled on the current one
+        stream.wait_stream(torch.cuda.current_stream())
     c.pool.tree_attention(prm, q, kd, vd, out, lse, ws, stream=stream)
     torch.cuda.synchronize()
     assert c.pool.status() == 0
