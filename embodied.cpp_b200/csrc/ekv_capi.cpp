@@ -773,7 +773,7 @@ int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t s
     a.weights_out = prm->weights_out;
     a.positions_out = prm->positions_out;
     a.max_len = (int32_t)std::min<int64_t>((int64_t)c.max_blocks_per_seq * c.block_tokens, EKV_MAX_EVICT_TOKENS);
-    return ekv::launch_evict(a, (cudaStream_t)stream);
+    return ekv::launch_evict(a, max_len, (cudaStream_t)stream);
 }
 
 }  // extern "C"

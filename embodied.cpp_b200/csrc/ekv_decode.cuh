@@ -29,23 +29,31 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 __device__ __forceinline__ void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <class... P, class... A>
-int launch_after(void (*k)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
+int launch_clusters_after(int cluster, void (*k)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
     c.blockDim = dim3((unsigned)threads);
     c.dynamicSmemBytes = smem;
     c.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = at;
-    c.numAttrs = 1;
+    c.numAttrs = cluster > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&c, k, P(args)...) != cudaSuccess) {
         cudaGetLastError();
         return EKV_ERR_CUDA;
     }
     note_launches(1);
     return EKV_OK;
+}
+
+template <class... P, class... A>
+int launch_after(void (*k)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
+    return launch_clusters_after(1, k, grid, threads, smem, s, args...);
 }
 
 // Dynamic shared memory above 48 KB, asked for once per kernel and device (`done`: the devices asked on).
@@ -164,6 +172,10 @@ __device__ __forceinline__ float lds_f16(uint32_t addr) {
     uint16_t v;
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
     return f16_bits_to_f32(v);
+}
+// 16 bytes to another CTA's shared memory (address from mapa_shared).
+__device__ __forceinline__ void stc128(uint32_t addr, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");

@@ -7,7 +7,8 @@
 // disjoint, so rows move in any order.
 //   evict_select_kernel  one CTA per (layer, request, KV head): the keep-th largest key by radix selection on
 //                        its bits, one bit per slot for the choice, then a slot for each survivor
-//   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed
+//   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed (the CTA that chose them,
+//                        where they are few)
 #include <algorithm>
 
 #include "ekv_decode.cuh"
@@ -19,6 +20,7 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;  // 11 bits of the key at a time: 11, 11, 10
 constexpr int kMoveWarps = 8;
+constexpr int64_t kMoveHere = 256 * 1024;  // bytes that one CTA moves itself
 
 // Larger is kept first. Protected rows are above every weight, NaN is below.
 __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
@@ -63,9 +65,80 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, SelShared &sh, int &t
     return s - v + __shfl_sync(0xffffffffu, w, warp) - mine;
 }
 
+// A warp's 32 slots of (layer, request, KV head) lbh: those whose row comes from elsewhere get it, K and V.
+struct MoveShared {
+    const uint8_t *src[32];
+    uint8_t *dst[32];
+    int rows[32];  // row inside the source block << 16 | inside the destination block
+};
+__device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0, int from, MoveShared &ms) {
+    const PoolView &p = a.pool;
+    const int h = lbh % p.kv_heads, lb = lbh / p.kv_heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
+    const int lane = threadIdx.x & 31, slot = slot0 + lane;
+    const int seq = a.seq_ids[b];
+    bool move = slot < a.keep && from >= 0 && from != slot;
+    int bs = -1, bd = -1;
+    if (move) {
+        bs = lookup_block(p, seq, from / p.block_tokens);
+        bd = lookup_block(p, seq, slot / p.block_tokens);
+        move = bs >= 0 && bd >= 0;
+    }
+    const uint32_t moving = __ballot_sync(0xffffffffu, move);
+    if (!moving) return;
+    const int n = __popc(moving);
+    if (move) {
+        const int i = __popc(moving & ((1u << lane) - 1u));
+        ms.src[i] = p.prefix + prefix_tile_index(p, layer, bs, 0, h) * p.tile_bytes;
+        ms.dst[i] = p.prefix + prefix_tile_index(p, layer, bd, 0, h) * p.tile_bytes;
+        ms.rows[i] = from % p.block_tokens << 16 | slot % p.block_tokens;
+    }
+    __syncwarp();
+    const int D = p.head_dim;
+    const int64_t kv_bytes = (int64_t)p.kv_heads * p.tile_bytes;
+    const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
+    const int per = q8 ? D / 16 : D / 8, units = 2 * per;  // 16-byte units of a row, K then V
+    // A lane keeps one unit of the row; where a row has at most 16 units, several rows are taken at a time.
+    const int wlog = decode::log2_of(p.swz_bytes);
+    const int at_once = units <= 16 ? 32 / units : 1, sub = units <= 16 ? lane / units : 0;
+    constexpr int UNROLL = 8;
+    for (int u0 = units <= 16 ? lane - sub * units : lane; u0 < units; u0 += 32) {
+        if (sub >= at_once) break;
+        const int u = u0 >= per ? u0 - per : u0;
+        const int64_t kv = u0 >= per ? kv_bytes : 0;
+        for (int m0 = sub; m0 < n; m0 += at_once * UNROLL) {
+            uint4 v[UNROLL];
+#pragma unroll
+            for (int j = 0; j < UNROLL; ++j) {
+                const int m = m0 + j * at_once;
+                if (m >= n) continue;
+                const int rs = ms.rows[m] >> 16;
+                v[j] = *(const uint4 *)(ms.src[m] + kv + (q8 ? q8_qs_off(rs, 16 * u, D) : decode::bf16_off_any(rs, 8 * u, D, wlog)));
+            }
+#pragma unroll
+            for (int j = 0; j < UNROLL; ++j) {
+                const int m = m0 + j * at_once;
+                if (m >= n) continue;
+                const int rd = ms.rows[m] & 0xffff;
+                *(uint4 *)(ms.dst[m] + kv + (q8 ? q8_qs_off(rd, 16 * u, D) : decode::bf16_off_any(rd, 8 * u, D, wlog))) = v[j];
+            }
+        }
+    }
+    const int g = q8 ? D / 32 : 0;
+    for (int i = lane; i < n * 2 * g; i += 32) {
+        const int m = i / (2 * g);
+        int u = i - m * 2 * g;
+        const int64_t base = (u >= g ? kv_bytes : 0) + (int64_t)p.block_tokens * D;
+        if (u >= g) u -= g;
+        const int rs = ms.rows[m] >> 16, rd = ms.rows[m] & 0xffff;
+        *(uint16_t *)(ms.dst[m] + base + (rd * g + u) * 2) = *(const uint16_t *)(ms.src[m] + base + (rs * g + u) * 2);
+    }
+    __syncwarp();
+}
+
 __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t s_mem[];
-    __shared__ SelShared sh;
+    __shared__ __align__(16) SelShared sh;
+    static_assert(sizeof(sh.hist) >= sizeof(MoveShared) * kSelThreads / 32, "the moves' tables fit the histograms");
     int turn = 0;
     decode::grid_wait();
     decode::grid_launch_next();
@@ -235,8 +308,11 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
         }
         __syncthreads();
     }
-    for (int i = tid; i < a.keep; i += kSelThreads) {
-        const uint32_t chosen = sel[i >> 5];
+    MoveShared *ms = (MoveShared *)&sh.hist[0][0];  // (the histograms are done with)
+    for (int i0 = 0; i0 < a.keep; i0 += kSelThreads) {
+        const int i = i0 + tid;
+        const bool in = i < a.keep;
+        const uint32_t chosen = in ? sel[i >> 5] : 0xffffffffu;
         int from = i;
         if (!((chosen >> (i & 31)) & 1u)) {
             const uint32_t rank = cnt[i >> 5] + __popc(~chosen & ((1u << (i & 31)) - 1u));
@@ -254,98 +330,43 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
                 from = 32 * lo + __ffs(bits) - 1;
             }
         }
-        kept[i] = from;
-        const float wi = w[from];
-        const int32_t pi = pos ? pos[from] : from;
-        if (w_out) w_out[i] = wi;
-        if (p_out) p_out[i] = pi;
+        if (in) {
+            kept[i] = from;
+            const float wi = w[from];
+            const int32_t pi = pos ? pos[from] : from;
+            if (w_out) w_out[i] = wi;
+            if (p_out) p_out[i] = pi;
+        }
+        if (a.move_here) move_rows(a, lbh, i0 + (tid & ~31), in ? from : -1, ms[tid >> 5]);
     }
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a, int chunks) {
-    __shared__ const uint8_t *s_src[kMoveWarps][32];
-    __shared__ uint8_t *s_dst[kMoveWarps][32];
-    __shared__ int s_rows[kMoveWarps][32];  // row inside the source block << 16 | inside the destination block
-    const PoolView &p = a.pool;
+    __shared__ MoveShared ms[kMoveWarps];
     decode::grid_wait();
-    const int lbh = blockIdx.x / chunks, chunk = blockIdx.x - lbh * chunks;
-    const int h = lbh % p.kv_heads, lb = lbh / p.kv_heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int slot = (chunk * kMoveWarps + warp) * 32 + lane;
-    const int seq = a.seq_ids[b];
-    int from = slot;
-    if (slot < a.keep) from = a.kept[(int64_t)lbh * a.keep + slot];
-    bool move = slot < a.keep && from >= 0 && from != slot;
-    int bs = -1, bd = -1;
-    if (move) {
-        bs = lookup_block(p, seq, from / p.block_tokens);
-        bd = lookup_block(p, seq, slot / p.block_tokens);
-        move = bs >= 0 && bd >= 0;
-    }
-    const uint32_t moving = __ballot_sync(0xffffffffu, move);
-    if (!moving) return;
-    const int n = __popc(moving);
-    if (move) {
-        const int i = __popc(moving & ((1u << lane) - 1u));
-        s_src[warp][i] = p.prefix + prefix_tile_index(p, layer, bs, 0, h) * p.tile_bytes;
-        s_dst[warp][i] = p.prefix + prefix_tile_index(p, layer, bd, 0, h) * p.tile_bytes;
-        s_rows[warp][i] = from % p.block_tokens << 16 | slot % p.block_tokens;
-    }
-    __syncwarp();
-    const int D = p.head_dim;
-    const int64_t kv_bytes = (int64_t)p.kv_heads * p.tile_bytes;
-    const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
-    const int per = q8 ? D / 16 : D / 8, units = 2 * per;  // 16-byte units of a row, K then V
-    // A lane keeps one unit of the row; where a row has at most 16 units, several rows are taken at a time.
-    const int wlog = decode::log2_of(p.swz_bytes);
-    const int at_once = units <= 16 ? 32 / units : 1, sub = units <= 16 ? lane / units : 0;
-    constexpr int UNROLL = 8;
-    for (int u0 = units <= 16 ? lane - sub * units : lane; u0 < units; u0 += 32) {
-        if (sub >= at_once) break;
-        const int u = u0 >= per ? u0 - per : u0;
-        const int64_t kv = u0 >= per ? kv_bytes : 0;
-        for (int m0 = sub; m0 < n; m0 += at_once * UNROLL) {
-            uint4 v[UNROLL];
-#pragma unroll
-            for (int j = 0; j < UNROLL; ++j) {
-                const int m = m0 + j * at_once;
-                if (m >= n) continue;
-                const int rs = s_rows[warp][m] >> 16;
-                v[j] = *(const uint4 *)(s_src[warp][m] + kv + (q8 ? q8_qs_off(rs, 16 * u, D) : decode::bf16_off_any(rs, 8 * u, D, wlog)));
-            }
-#pragma unroll
-            for (int j = 0; j < UNROLL; ++j) {
-                const int m = m0 + j * at_once;
-                if (m >= n) continue;
-                const int rd = s_rows[warp][m] & 0xffff;
-                *(uint4 *)(s_dst[warp][m] + kv + (q8 ? q8_qs_off(rd, 16 * u, D) : decode::bf16_off_any(rd, 8 * u, D, wlog))) = v[j];
-            }
-        }
-    }
-    if (!q8) return;
-    const int g = D / 32;
-    for (int i = lane; i < n * 2 * g; i += 32) {
-        const int m = i / (2 * g);
-        int u = i - m * 2 * g;
-        const int64_t base = (u >= g ? kv_bytes : 0) + (int64_t)p.block_tokens * D;
-        if (u >= g) u -= g;
-        const int rs = s_rows[warp][m] >> 16, rd = s_rows[warp][m] & 0xffff;
-        *(uint16_t *)(s_dst[warp][m] + base + (rd * g + u) * 2) = *(const uint16_t *)(s_src[warp][m] + base + (rs * g + u) * 2);
-    }
+    const int lbh = blockIdx.x / chunks, warp = threadIdx.x >> 5;
+    const int slot0 = ((blockIdx.x - lbh * chunks) * kMoveWarps + warp) * 32, slot = slot0 + (threadIdx.x & 31);
+    move_rows(a, lbh, slot0, slot < a.keep ? a.kept[(int64_t)lbh * a.keep + slot] : -1, ms[warp]);
 }
 
 }  // namespace
 
-int launch_evict(EvictArgs a, cudaStream_t s) {
+int launch_evict(EvictArgs a, int max_live, cudaStream_t s) {
     const int64_t n = (int64_t)a.n_layers * a.n_batch * a.pool.kv_heads;
     const int chunks = (a.keep + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
     if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
     a.max_words = (a.max_len + 31) / 32 + 1;
+    // At most max_live - keep rows of each (layer, request, KV head) move: few are moved by the CTA that chose them, which
+    // saves a launch and its tail; more are spread over the GPU. 18 x 100 rows of 544 bytes: 12.6 us with a second launch,
+    // 9.6 without.
+    const int64_t most = (int64_t)std::max(0, max_live - a.keep) * 2 * a.pool.tile_bytes / a.pool.block_tokens;
+    a.move_here = most <= kMoveHere;
     const size_t smem = ((size_t)a.max_words * 2 + kList) * sizeof(uint32_t);
     static std::atomic<uint64_t> smem_done{0};
     if (const int rc = decode::allow_smem(evict_select_kernel, ((EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 + kList) * (int)sizeof(uint32_t), smem_done))
         return rc;
     if (const int rc = decode::launch_after(evict_select_kernel, (unsigned)n, kSelThreads, smem, s, a)) return rc;
+    if (a.move_here) return EKV_OK;
     return decode::launch_after(evict_move_kernel, (unsigned)(n * chunks), kMoveWarps * 32, 0, s, a, chunks);
 }
 

@@ -80,7 +80,8 @@ struct TreeArgs {
     void *out;
     float *lse;        // attention: written, or null; key weights: read
     // attention: partial results of units cut between CTAs
-    int32_t split;     // 0: CTA = unit
+    int32_t split;     // CTAs take equal ranges of the call's tiles; 0: a unit is one cluster's
+    int32_t cluster;   // (split == 0) CTAs of a cluster
     int32_t row_tiles; // row tiles of one (request, KV head)
     int2 *parts;       // [units] first and last CTA of each unit
     float4 *ws_ml;     // [2 * CTAs][rows] maximum (log2 domain), sum, sum of the rounded probabilities
@@ -103,7 +104,7 @@ struct EvictArgs {
     float *weights_out;
     int32_t *positions_out;
     int32_t max_len;    // slots that the selection has room for
-    int32_t max_words;  // (set by the launcher)
+    int32_t max_words, move_here;  // (set by the launcher)
 };
 
 constexpr long long kDefaultWaitBudget = 4000000000LL;  // clock cycles, about 2 s
@@ -173,7 +174,8 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
                        const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
                        const void *v, int64_t kv_stride, int sms, cudaStream_t s);
 // Eviction by weight (ekv_evict.cu)
-int launch_evict(EvictArgs a, cudaStream_t s);
+// max_live: the longest live sequence (which only decides how the rows are moved)
+int launch_evict(EvictArgs a, int max_live, cudaStream_t s);
 // combine key-split partial outputs (head_dim of the pool) into a.out
 int launch_merge_splits(const AttnArgs &a, int n_qtiles, cudaStream_t s);
 #ifdef EKV_TRACE

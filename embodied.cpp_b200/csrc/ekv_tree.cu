@@ -31,6 +31,8 @@ constexpr int rows_ctas(int d, bool q8, int nr, int wr) {
     return d * nr > 256 || wr * 8 * nr > 64 || (d > 128 && !q8) || (d > 128 && wr > 1) ? 1 : 2;
 }
 
+constexpr int kMaxCluster = 8;
+
 // WR row groups of 8 * NR rows times WK groups of 64 / WK keys: one warp each, and one feeder warp.
 template <int D, bool Q8, int NR, int WR, int WK>
 struct Cfg {
@@ -53,7 +55,11 @@ struct Cfg {
     // query rows in shared memory where the output's share of the registers leaves no room for them
     static constexpr bool Q_SMEM = D * NR > 256;
     static constexpr int Q_BYTES = Q_SMEM ? ROWS * q_row_bytes<D, Q8>() : 0;
-    static constexpr int FIXED = X_BYTES + ML_BYTES + Q_BYTES + 1024 + 1024;
+    // what the CTAs of a cluster send one another: this CTA's share of the unit's outputs and all rows' maxima and
+    // sums, from each of them (few rows only: a large unit is better split)
+    static constexpr bool CLUSTERS = ROWS * D <= 2048;
+    static constexpr int P_BYTES = CLUSTERS ? ROWS * D * 4 + kMaxCluster * (ROWS + 1) * 16 : 0;
+    static constexpr int FIXED = X_BYTES + ML_BYTES + Q_BYTES + P_BYTES + 1024 + 1024;
     static constexpr int CTAS = rows_ctas(D, Q8, NR, WR);
     static constexpr int BUDGET = CTAS == 2 ? 112 * 1024 : 220 * 1024;
     static constexpr int NST_FIT = (BUDGET - FIXED) / STAGE;
@@ -91,6 +97,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     static_assert(sizeof(Sh) <= 1024, "barrier block");
     Sh &sh = *(Sh *)(smem + NST * C::STAGE + C::X_BYTES + C::ML_BYTES);
     uint8_t *sq = smem + NST * C::STAGE + C::X_BYTES + C::ML_BYTES + 1024;  // [ROWS] query rows (Q_SMEM)
+    float4 *part_o = (float4 *)(sq + C::Q_BYTES);                       // [cluster][its share of the unit's float4 outputs]
+    float4 *part_ml = part_o + C::ROWS * D / 4 + kMaxCluster;           // [cluster][ROWS]
     volatile int *abort = &sh.abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -111,6 +119,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     auto unit_tiles = [](const Req &r) {
         return max(1, (r.n_prefix + kTile - 1) / kTile + (r.n_nodes + C::DT - 1) / C::DT);
     };
+    // without the split a cluster of CTAs takes one unit's tiles in equal parts and joins its outputs through their
+    // shared memory
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
+    if (C::CLUSTERS && a.cluster > 1) cluster_arrive_relaxed();  // (waited for before anything is sent)
     Range rg;
     grid_wait();
     grid_launch_next();  // the merge's blocks may take their places; they wait for this grid's end
@@ -119,13 +131,9 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                                     [&](int b) { return load_req(a, b, blockIdx.x == 0); }, unit_tiles);
     } else {
         __syncthreads();
-        rg.b = blockIdx.x / units_per_req;
-        rg.req = load_req(a, rg.b, threadIdx.x == 0);
-        const int n = unit_tiles(rg.req);
-        rg.base = 0;
-        rg.lo = (blockIdx.x - rg.b * units_per_req) * (uint32_t)n;
-        rg.hi = rg.lo + n;
-        rg.total = 0;
+        rg.b = unit / units_per_req;
+        rg.req = load_req(a, rg.b, threadIdx.x == 0 && rank == 0);
+        rg.base = rg.lo = rg.hi = rg.total = 0;
         rg.ctas = 0;
     }
 
@@ -143,18 +151,18 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     uint32_t base = rg.base;
     Req rq = rg.req;
     int rq_of = b;  // the request that rq describes
-    for (uint32_t x = rg.lo; x < rg.hi && b < a.n_batch;) {
+    for (uint32_t x = rg.lo; (x < rg.hi || !a.split) && b < a.n_batch;) {
         if (b != rq_of) rq = load_req(a, b, false), rq_of = b;
         const int n_tiles = unit_tiles(rq);
         const uint32_t span = (uint32_t)n_tiles * units_per_req;
-        if (x >= base + span) {
+        if (a.split && x >= base + span) {
             base += span;
             ++b;
             continue;
         }
-        const int u = (int)((x - base) / (uint32_t)n_tiles);
-        const int t0 = (int)(x - base) - u * n_tiles;
-        const int t1 = min(n_tiles, t0 + (int)(rg.hi - x));
+        const int u = a.split ? (int)((x - base) / (uint32_t)n_tiles) : unit - b * units_per_req;
+        const int t0 = a.split ? (int)(x - base) - u * n_tiles : rank * n_tiles / a.cluster;
+        const int t1 = a.split ? min(n_tiles, t0 + (int)(rg.hi - x)) : (rank + 1) * n_tiles / a.cluster;
         const int g = u / a.row_tiles, row0 = (u - g * a.row_tiles) * C::ROWS;
         const int rows = min(C::ROWS, rows_all - row0);
         const int p_tiles = (rq.n_prefix + kTile - 1) / kTile;
@@ -561,6 +569,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
             }
 
             // ---- join the key groups, write the rows ----
+            if (C::CLUSTERS && a.cluster > 1) {  // the other CTAs have started
+                __syncwarp();
+                cluster_wait();
+            }
             float scale_o[NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n)
@@ -575,7 +587,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     if (kq == 0) sml[wk * C::ROWS + wrow + 8 * n + 2 * c + e] = make_float4(mx[n][e], l, lr, 0.0f);
                 }
             asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
-            const bool whole = t0 == 0 && t1 == n_tiles;
+            const bool joins = C::CLUSTERS && a.cluster > 1, whole = t0 == 0 && t1 == n_tiles && !joins;
             const long long slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
 #pragma unroll
             for (int n = 0; n < NR; ++n)
@@ -597,7 +609,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                     if (whole) scale_o[n][e] = lr == 0.0f ? 0.0f : scale_o[n][e] / lr;
                     if (wk != 0 || kq != 0 || r >= rows) continue;
                     const bool off = t_of[n][e] < 0;
-                    if (!whole) {
+                    if (joins) {
+                        const uint32_t at = smem_addr(part_ml + rank * C::ROWS + r);
+                        for (int k = 0; k < a.cluster; ++k)
+                            stc128(mapa_shared(at, k), off ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(mt, lt, lr, 0.0f));
+                    } else if (!whole) {
                         a.ws_ml[slot * C::ROWS + r] = off ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(mt, lt, lr, 0.0f);
                     } else if (a.lse) {
                         const int t = row_token(a, row0 + r), hq = g * a.group + (row0 + r) - t * a.group;
@@ -605,6 +621,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                             off || lt == 0.0f ? -INFINITY : (mt + __log2f(lt)) * 0.6931471805599453f;
                     }
                 }
+            const int share = (rows * (D / 4) + a.cluster - 1) / a.cluster;  // float4 outputs that a CTA of the cluster writes
             constexpr int XC = C::X_COLS, ROUNDS = (D + XC - 1) / XC;
 #pragma unroll
             for (int cc = 0; cc < ROUNDS; ++cc) {
@@ -637,6 +654,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                         v.z += y.z;
                         v.w += y.w;
                     }
+                    if (joins) {  // to the CTA that writes it
+                        const int item = r * (D / 4) + (cc * XC + col) / 4, to = item / share;
+                        stc128(mapa_shared(smem_addr(part_o + rank * share + item - to * share), to), v);
+                        continue;
+                    }
                     if (!whole) {
                         *(float4 *)(a.ws_o + (slot * C::ROWS + r) * D + cc * XC + col) = v;
                         continue;
@@ -653,6 +675,39 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                 if (cc + 1 < ROUNDS) asm volatile("bar.sync 1, %0;" ::"n"(C::NC) : "memory");
             }
         }
+        if constexpr (C::CLUSTERS)
+            if (a.cluster > 1) {
+                // out = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k over the cluster's CTAs k
+                __syncwarp();
+                if (warp == C::NW) cluster_wait();
+                cluster_sync();  // everyone's parts are here
+                const int share = (rows * (D / 4) + a.cluster - 1) / a.cluster;
+                for (int i = threadIdx.x; i < share && rank * share + i < rows * (D / 4); i += C::THREADS) {
+                    const int item = rank * share + i, r = item / (D / 4), col = (item - r * (D / 4)) * 4;
+                    float m = -INFINITY, l = 0.0f, lr = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int k = 0; k < a.cluster; ++k) m = fmaxf(m, part_ml[k * C::ROWS + r].x);
+                    for (int k = 0; k < a.cluster; ++k) {
+                        const float4 ml = part_ml[k * C::ROWS + r], y = part_o[k * share + i];
+                        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+                        l += f * ml.y;
+                        lr += f * ml.z;
+                        if (f == 0.0f) continue;  // (a part that saw nothing for the row)
+                        v.x = fmaf(y.x, f, v.x);
+                        v.y = fmaf(y.y, f, v.y);
+                        v.z = fmaf(y.z, f, v.z);
+                        v.w = fmaf(y.w, f, v.w);
+                    }
+                    const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+                    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                    const int t = row_token(a, row0 + r), hq = g * a.group + (row0 + r) - t * a.group;
+                    const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
+                    if (a.out_dtype == EKV_DTYPE_F32) *(float4 *)((float *)a.out + at * D + col) = v;
+                    else *(uint2 *)((uint16_t *)a.out + at * D + col) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                    if (a.lse && col == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+                }
+            }
+        if (!a.split) break;
         x += t1 - t0;
     }
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 7);
@@ -798,7 +853,7 @@ int launch_rows(const TreeArgs &a, int grid, cudaStream_t s) {
     using C = Cfg<D, Q8, NR, WR, WK>;
     static std::atomic<uint64_t> smem_done{0};
     if (const int rc = allow_smem(tree_rows_kernel<D, Q8, NR, WR, WK>, C::SMEM, smem_done)) return rc;
-    return launch_after(tree_rows_kernel<D, Q8, NR, WR, WK>, grid, C::THREADS, C::SMEM, s, a);
+    return launch_clusters_after(a.cluster, tree_rows_kernel<D, Q8, NR, WR, WK>, grid, C::THREADS, C::SMEM, s, a);
 }
 
 template <int D, bool Q8>
@@ -854,15 +909,31 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     const int64_t most_tiles = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile + 2;
     if (units > INT32_MAX || all_rows > INT32_MAX) return EKV_ERR_INVALID_ARG;
     const int full = grid_ctas(sh, a.pool, rows, sms);
-    // Units of one or two tiles are not worth a second launch; without a workspace a unit is one CTA's.
-    a.split = ws != nullptr && ws_bytes >= w.total && unit_tiles > 2 && units * most_tiles < INT32_MAX;
-    int64_t grid = units;
+    // Three ways to share the work: a CTA per unit (one or two tiles, or many units without a workspace); a cluster of
+    // CTAs per unit; CTAs with equal ranges of all tiles and a second kernel that joins the parts. The last is the most
+    // even one, but its second launch costs about 3.4 us, the time of `worth` tiles: one token over 816 keys takes 9.2 us
+    // with it and 6.4 as a cluster of eight.
+    const bool can_split = ws != nullptr && ws_bytes >= w.total && units * most_tiles < INT32_MAX;
+    const int64_t even = (units * unit_tiles + full - 1) / full;  // tiles per CTA when split
+    const int64_t worth = a.pool.dtype == EKV_DTYPE_Q8_0 ? 1 : 3;
+    a.split = 0;
+    a.cluster = 1;
+    if (unit_tiles > 2) {
+        int c = 1;
+        const bool few = sh != Shape::Tile && tr * a.pool.head_dim <= 2048;  // what Cfg::CLUSTERS has room for
+        if (few)
+            while (c < kMaxCluster && 2 * c <= unit_tiles && units * 2 * c <= full) c *= 2;
+        if (c > 1 && (!can_split || (unit_tiles + c - 1) / c <= even + worth)) a.cluster = c;
+        else a.split = can_split;
+    }
+    int64_t grid = units * a.cluster;
     if (a.split) {
         grid = std::min<int64_t>(full, units * unit_tiles);
         a.parts = (int2 *)ws;
         a.ws_ml = (float4 *)((uint8_t *)ws + w.ml);
         a.ws_o = (float *)((uint8_t *)ws + w.o);
     }
+    if (grid > INT32_MAX) return EKV_ERR_INVALID_ARG;
     switch (a.pool.head_dim) {
         case 48: return launch_dim<48>(a, sh, (int)grid, s);
         case 64: return launch_dim<64>(a, sh, (int)grid, s);
