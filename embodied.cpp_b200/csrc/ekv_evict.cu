@@ -7,8 +7,11 @@
 // disjoint, so rows move in any order.
 //   evict_select_kernel  one CTA per (layer, request, KV head): the keep-th largest key by radix selection on
 //                        its bits, one bit per slot for the choice, then a slot for each survivor
-//   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed (the CTA that chose them,
-//                        where they are few)
+//   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed
+// Bounds and figures: the move is bound by DRAM (64 rows of 16384 slots cut to 8192, head_dim 128 bf16: 38 us where the
+// bytes alone would take 31), the selection by its barriers and the latency of its loads, not by bytes (15 us for those
+// 64 rows, whose weights and positions would take 1.3). Moving the rows in the CTA that chose them saved the second
+// launch on the host but left a third of the SMs to move everything: 14.0 us against 13.3 for 18 rows of 1100 slots.
 #include <algorithm>
 
 #include "ekv_decode.cuh"
@@ -17,17 +20,17 @@
 namespace ekv {
 namespace {
 
-constexpr int kSelThreads = 1024;
+// Threads of a selection: 512 for rows of up to kFewSlots slots, whose barriers cost more than their keys (18 rows of
+// 1100 slots, the move included: 11.7 us, against 12.8 with 256 threads and 12.6 with 1024), else 1024.
+constexpr int kFewThreads = 512, kManyThreads = 1024, kFewSlots = 4096;
 constexpr int kBins = 2048;  // 11 bits of the key at a time: 11, 11, 10
 constexpr int kMoveWarps = 8;
-constexpr int64_t kMoveHere = 256 * 1024;  // bytes that one CTA moves itself
 
 // Larger is kept first. Protected rows are above every weight, NaN is below.
 __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
-    if (safe) return 0xffffffffu;
-    if (w != w) return 0u;
     const uint32_t b = __float_as_uint(w + 0.0f);  // -0 counts as 0
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    return safe ? 0xffffffffu : w != w ? 0u : k;
 }
 
 constexpr int kCopies = 4;   // histograms, by lane: weights share few exponents, so lanes meet in few bins
@@ -54,7 +57,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, SelShared &sh, int &t
     }
     if (lane == 31) sums[warp] = s;
     __syncthreads();
-    uint32_t w = sums[lane];
+    uint32_t w = lane < (int)blockDim.x / 32 ? sums[lane] : 0u;
     const uint32_t mine = __shfl_sync(0xffffffffu, w, warp);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -71,17 +74,22 @@ struct MoveShared {
     uint8_t *dst[32];
     int rows[32];  // row inside the source block << 16 | inside the destination block
 };
-__device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0, int from, MoveShared &ms) {
+template <class From>
+__device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0, From from_of, MoveShared &ms) {
     const PoolView &p = a.pool;
     const int h = lbh % p.kv_heads, lb = lbh / p.kv_heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
     const int lane = threadIdx.x & 31, slot = slot0 + lane;
+    // What the selection does not write is read while it still runs: it let this grid start after its own wait.
     const int seq = a.seq_ids[b];
-    bool move = slot < a.keep && from >= 0 && from != slot;
-    int bs = -1, bd = -1;
+    const bool real = slot < a.keep && seq >= 0 && seq < p.max_seqs && slot < p.seq_lens[seq];
+    const int bd = real ? lookup_block(p, seq, slot / p.block_tokens) : -1;
+    decode::grid_wait();
+    const int from = bd >= 0 ? from_of(slot) : -1;
+    bool move = from >= 0 && from != slot;
+    int bs = -1;
     if (move) {
         bs = lookup_block(p, seq, from / p.block_tokens);
-        bd = lookup_block(p, seq, slot / p.block_tokens);
-        move = bs >= 0 && bd >= 0;
+        move = bs >= 0;
     }
     const uint32_t moving = __ballot_sync(0xffffffffu, move);
     if (!moving) return;
@@ -97,6 +105,21 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0
     const int64_t kv_bytes = (int64_t)p.kv_heads * p.tile_bytes;
     const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
     const int per = q8 ? D / 16 : D / 8, units = 2 * per;  // 16-byte units of a row, K then V
+    // Q8_0 scales, 2 bytes each: the first of them on their way before the rows
+    const int g = q8 ? D / 32 : 0, n_scales = n * 2 * g;
+    constexpr int EARLY = 4;
+    auto scale_at = [&](int i, bool to) -> uint16_t * {
+        const int m = i / (2 * g);
+        int u = i - m * 2 * g;
+        const int64_t base = (u >= g ? kv_bytes : 0) + (int64_t)p.block_tokens * D;
+        if (u >= g) u -= g;
+        return to ? (uint16_t *)(ms.dst[m] + base + ((ms.rows[m] & 0xffff) * g + u) * 2)
+                  : (uint16_t *)(ms.src[m] + base + ((ms.rows[m] >> 16) * g + u) * 2);
+    };
+    uint16_t early[EARLY];
+#pragma unroll
+    for (int j = 0; j < EARLY; ++j)
+        if (lane + 32 * j < n_scales) early[j] = *scale_at(lane + 32 * j, false);
     // A lane keeps one unit of the row; where a row has at most 16 units, several rows are taken at a time.
     const int wlog = decode::log2_of(p.swz_bytes);
     const int at_once = units <= 16 ? 32 / units : 1, sub = units <= 16 ? lane / units : 0;
@@ -123,29 +146,40 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0
             }
         }
     }
-    const int g = q8 ? D / 32 : 0;
-    for (int i = lane; i < n * 2 * g; i += 32) {
-        const int m = i / (2 * g);
-        int u = i - m * 2 * g;
-        const int64_t base = (u >= g ? kv_bytes : 0) + (int64_t)p.block_tokens * D;
-        if (u >= g) u -= g;
-        const int rs = ms.rows[m] >> 16, rd = ms.rows[m] & 0xffff;
-        *(uint16_t *)(ms.dst[m] + base + (rd * g + u) * 2) = *(const uint16_t *)(ms.src[m] + base + (rs * g + u) * 2);
-    }
+#pragma unroll
+    for (int j = 0; j < EARLY; ++j)
+        if (lane + 32 * j < n_scales) *scale_at(lane + 32 * j, true) = early[j];
+    for (int i = lane + 32 * EARLY; i < n_scales; i += 32) *scale_at(i, true) = *scale_at(i, false);
     __syncwarp();
 }
 
+template <int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t s_mem[];
     __shared__ __align__(16) SelShared sh;
-    static_assert(sizeof(sh.hist) >= sizeof(MoveShared) * kSelThreads / 32, "the moves' tables fit the histograms");
     int turn = 0;
     decode::grid_wait();
     decode::grid_launch_next();
     const int hk = a.pool.kv_heads;
     const int lbh = blockIdx.x, b = (lbh / hk) % a.n_batch;
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seq = a.seq_ids[b];
+    const float *w = a.weights + (int64_t)lbh * a.weight_stride;
+    const int32_t *pos = a.positions ? a.positions + (int64_t)lbh * a.weight_stride : nullptr;
+    // The row is asked for before its length is known: the sequence's id and length are two reads one after the other.
+    // All of a thread's loads come first: with the test of each key between them a row of 16384 took 10 us to read.
+    const int ahead = a.row_hint <= kInRegs * kSelThreads ? a.row_hint : 0;
+    uint32_t keys[kInRegs], ages[kInRegs];
+#pragma unroll
+    for (int j = 0; j < kInRegs; ++j) {
+        const int i = tid + j * kSelThreads;
+        keys[j] = i < ahead ? __float_as_uint(__ldg(w + i)) : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < kInRegs; ++j) {
+        const int i = tid + j * kSelThreads;
+        ages[j] = pos && i < ahead ? (uint32_t)__ldg(pos + i) : (uint32_t)i;
+    }
     int n = 0;
     if (seq < 0 || seq >= a.pool.max_seqs) {
         if (tid == 0) report_error(a.pool.status, DEV_ERR_BAD_SEQ, b, seq, 10);
@@ -156,8 +190,6 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
             n = 0;
         }
     }
-    const float *w = a.weights + (int64_t)lbh * a.weight_stride;
-    const int32_t *pos = a.positions ? a.positions + (int64_t)lbh * a.weight_stride : nullptr;
     int32_t *kept = a.kept + (int64_t)lbh * a.keep;
     float *w_out = a.weights_out ? a.weights_out + (int64_t)lbh * a.out_stride : nullptr;
     int32_t *p_out = a.positions_out ? a.positions_out + (int64_t)lbh * a.out_stride : nullptr;
@@ -180,16 +212,13 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     }
 
     // ---- the keep-th largest key, from its upper bits down ----
-    const bool in_regs = n <= kInRegs * kSelThreads;
-    uint32_t keys[kInRegs];
-    if (in_regs) {
+    const bool in_regs = n <= ahead;
 #pragma unroll
-        for (int j = 0; j < kInRegs; ++j) {
-            const int i = tid + j * kSelThreads;
-            keys[j] = i < n ? key_of(i) : 0u;
-        }
+    for (int j = 0; j < kInRegs; ++j) {
+        const int age = (int)ages[j];
+        keys[j] = evict_key(__uint_as_float(keys[j]), age < a.first || age >= recent_from);
     }
-    // f(slot, key) for this thread's slots tid, tid + 1024, ...
+    // f(slot, key) for this thread's slots tid, tid + kSelThreads, ...
     auto each = [&](auto f) {
         if (in_regs) {
 #pragma unroll
@@ -205,35 +234,57 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     uint32_t prefix = 0, mask = 0;
     uint32_t need = (uint32_t)a.keep;  // how many of the keys that match `prefix` are kept
     bool all = false;                  // every key that matches is kept
+    for (int i = tid; i < kCopies * kBins / 2; i += kSelThreads) ((uint2 *)&sh.hist[0][0])[i] = make_uint2(0, 0);
+    __syncthreads();
 #pragma unroll 1
     for (int pass = 0; pass < 3 && !all; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digits = pass == 2 ? 1024u : 2048u;
-        for (int i = tid; i < kCopies * kBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
-        __syncthreads();
         each([&](int i, uint32_t k) {
             if (i < n && (k & mask) == prefix) atomicAdd(&sh.hist[lane % kCopies][(k >> shift) & (digits - 1)], 1u);
         });
         __syncthreads();
-        // digits from the top: thread t holds digits 2 (1023 - t) + 1 and 2 (1023 - t)
-        const int d = 2 * (kSelThreads - 1 - tid);
-        uint32_t hi = 0, lo = 0;
+        // digits from the top: thread t holds the PER digits from PER (threads - 1 - t); cleared for the next pass
+        constexpr int PER = kBins / kSelThreads;
+        struct __align__(4 * PER) Digits {
+            uint32_t n[PER];
+        };
+        const int d = PER * (kSelThreads - 1 - tid);
+        uint32_t cnt[PER], sum = 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) cnt[e] = 0;
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
-            const uint2 h = *(const uint2 *)&sh.hist[c][d];
-            lo += h.x;
-            hi += h.y;
+            Digits *h = (Digits *)&sh.hist[c][d];
+            const Digits v = *h;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) cnt[e] += v.n[e];
+            *h = Digits{};
         }
-        uint32_t total;
-        const uint32_t before = block_scan(hi + lo, sh, turn, total);
-        if (before < need && need <= before + hi) {
-            sh.digit = d + 1;
-            sh.above = before;
-            sh.count = hi;
-        } else if (before + hi < need && need <= before + hi + lo) {
-            sh.digit = d;
-            sh.above = before + hi;
-            sh.count = lo;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sum += cnt[e];
+        // only the warp in which the count reaches `need` looks closer
+        const uint32_t mine = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) sh.warp_sum[0][warp] = mine;
+        __syncthreads();
+        const uint32_t above = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_sum[0][lane] : 0u);  // (warp 0: none)
+        if (above < need && need <= above + mine) {
+            uint32_t s = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            uint32_t before = above + s - sum;
+#pragma unroll
+            for (int e = PER - 1; e >= 0; --e) {
+                if (before < need && need <= before + cnt[e]) {
+                    sh.digit = d + e;
+                    sh.above = before;
+                    sh.count = cnt[e];
+                }
+                before += cnt[e];
+            }
         }
         __syncthreads();
         prefix |= sh.digit << shift;
@@ -308,11 +359,8 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
         }
         __syncthreads();
     }
-    MoveShared *ms = (MoveShared *)&sh.hist[0][0];  // (the histograms are done with)
-    for (int i0 = 0; i0 < a.keep; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        const bool in = i < a.keep;
-        const uint32_t chosen = in ? sel[i >> 5] : 0xffffffffu;
+    for (int i = tid; i < a.keep; i += kSelThreads) {
+        const uint32_t chosen = sel[i >> 5];
         int from = i;
         if (!((chosen >> (i & 31)) & 1u)) {
             const uint32_t rank = cnt[i >> 5] + __popc(~chosen & ((1u << (i & 31)) - 1u));
@@ -330,23 +378,19 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
                 from = 32 * lo + __ffs(bits) - 1;
             }
         }
-        if (in) {
-            kept[i] = from;
-            const float wi = w[from];
-            const int32_t pi = pos ? pos[from] : from;
-            if (w_out) w_out[i] = wi;
-            if (p_out) p_out[i] = pi;
-        }
-        if (a.move_here) move_rows(a, lbh, i0 + (tid & ~31), in ? from : -1, ms[tid >> 5]);
+        kept[i] = from;
+        const float wi = w[from];
+        const int32_t pi = pos ? pos[from] : from;
+        if (w_out) w_out[i] = wi;
+        if (p_out) p_out[i] = pi;
     }
 }
 
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a, int chunks) {
     __shared__ MoveShared ms[kMoveWarps];
-    decode::grid_wait();
     const int lbh = blockIdx.x / chunks, warp = threadIdx.x >> 5;
-    const int slot0 = ((blockIdx.x - lbh * chunks) * kMoveWarps + warp) * 32, slot = slot0 + (threadIdx.x & 31);
-    move_rows(a, lbh, slot0, slot < a.keep ? a.kept[(int64_t)lbh * a.keep + slot] : -1, ms[warp]);
+    const int slot0 = ((blockIdx.x - lbh * chunks) * kMoveWarps + warp) * 32;
+    move_rows(a, lbh, slot0, [&](int slot) { return a.kept[(int64_t)lbh * a.keep + slot]; }, ms[warp]);
 }
 
 }  // namespace
@@ -356,17 +400,18 @@ int launch_evict(EvictArgs a, int max_live, cudaStream_t s) {
     const int chunks = (a.keep + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
     if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
     a.max_words = (a.max_len + 31) / 32 + 1;
-    // At most max_live - keep rows of each (layer, request, KV head) move: few are moved by the CTA that chose them, which
-    // saves a launch and its tail; more are spread over the GPU. 18 x 100 rows of 544 bytes: 12.6 us with a second launch,
-    // 9.6 without.
-    const int64_t most = (int64_t)std::max(0, max_live - a.keep) * 2 * a.pool.tile_bytes / a.pool.block_tokens;
-    a.move_here = most <= kMoveHere;
     const size_t smem = ((size_t)a.max_words * 2 + kList) * sizeof(uint32_t);
-    static std::atomic<uint64_t> smem_done{0};
-    if (const int rc = decode::allow_smem(evict_select_kernel, ((EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 + kList) * (int)sizeof(uint32_t), smem_done))
-        return rc;
-    if (const int rc = decode::launch_after(evict_select_kernel, (unsigned)n, kSelThreads, smem, s, a)) return rc;
-    if (a.move_here) return EKV_OK;
+    // The longest live sequence picks the form and how much of a row is read ahead: any sequence is right with either.
+    a.row_hint = (int)std::min<int64_t>(std::min(max_live, a.max_len), a.weight_stride);
+    const bool few = max_live <= kFewSlots;
+    static std::atomic<uint64_t> few_done{0}, many_done{0};
+    const int most_smem = ((EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 + kList) * (int)sizeof(uint32_t);
+    int rc = few ? decode::allow_smem(evict_select_kernel<kFewThreads>, most_smem, few_done)
+                 : decode::allow_smem(evict_select_kernel<kManyThreads>, most_smem, many_done);
+    if (!rc)
+        rc = few ? decode::launch_after(evict_select_kernel<kFewThreads>, (unsigned)n, kFewThreads, smem, s, a)
+                 : decode::launch_after(evict_select_kernel<kManyThreads>, (unsigned)n, kManyThreads, smem, s, a);
+    if (rc) return rc;
     return decode::launch_after(evict_move_kernel, (unsigned)(n * chunks), kMoveWarps * 32, 0, s, a, chunks);
 }
 

@@ -104,7 +104,7 @@ struct EvictArgs {
     float *weights_out;
     int32_t *positions_out;
     int32_t max_len;    // slots that the selection has room for
-    int32_t max_words, move_here;  // (set by the launcher)
+    int32_t max_words, row_hint;  // (set by the launcher)
 };
 
 constexpr long long kDefaultWaitBudget = 4000000000LL;  // clock cycles, about 2 s
@@ -174,7 +174,7 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
                        const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
                        const void *v, int64_t kv_stride, int sms, cudaStream_t s);
 // Eviction by weight (ekv_evict.cu)
-// max_live: the longest live sequence (which only decides how the rows are moved)
+// max_live: the longest live sequence
 int launch_evict(EvictArgs a, int max_live, cudaStream_t s);
 // combine key-split partial outputs (head_dim of the pool) into a.out
 int launch_merge_splits(const AttnArgs &a, int n_qtiles, cudaStream_t s);

@@ -221,6 +221,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _dense(*tensors):
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise ValueError("arrays by slot or row must be contiguous")
+
+
 def _current_stream():
     """The current torch stream's handle. torch.cuda.current_stream() makes a Stream object first, 3 us of a call that
     may itself take 5; where torch has the raw query it is asked instead."""
@@ -410,6 +416,7 @@ class Pool:
 
     def key_weights(self, params: TreeParams, q, lse, weights, decay=1.0, stream=None):
         """ekv_key_weights: weights [n_batch, kv_heads, stride] f32 = decay * weights + what the rows give each key."""
+        _dense(lse, weights)
         check(lib.ekv_key_weights(self.h, C.byref(params), _ptr(q), _ptr(lse), _ptr(weights), weights.shape[-1], decay,
                                   _stream(stream)), "ekv_key_weights")
 
@@ -418,6 +425,9 @@ class Pool:
         """ekv_evict_by_weight: weights (and positions) [n_layers, n_batch, kv_heads, stride], kept int32 [n_layers,
         n_batch, kv_heads, keep]; weights_out and positions_out have one stride of their own, or are the inputs."""
         outs = [t for t in (weights_out, positions_out) if t is not None]
+        _dense(weights, kept, positions, *outs)
+        if len({t.shape[-1] for t in outs}) > 1 or (positions is not None and positions.shape != weights.shape):
+            raise ValueError("weights and positions have one stride, and so have the outputs")
         p = EvictParams(layer0, n_layers, seq_ids.numel(), keep, first, recent, seq_ids.data_ptr(),
                         None if seen is None else seen.data_ptr(), weights.data_ptr(),
                         None if positions is None else positions.data_ptr(), weights.shape[-1], kept.data_ptr(),

@@ -391,7 +391,7 @@ typedef struct ekv_evict_params {
     const int32_t *seen;        /* device [n_batch] tokens seen so far; NULL: the sequence length        */
     const float *weights;       /* device [n_layers][n_batch][kv_heads][weight_stride], by slot          */
     const int32_t *positions;   /* the token position in each slot, same layout; NULL: the slot          */
-    int64_t weight_stride;      /* at least the longest sequence                                       */
+    int64_t weight_stride;      /* at least the longest sequence; whole rows of it may be read         */
     int32_t *kept;              /* out [n_layers][n_batch][kv_heads][keep]: the slot each row came from   */
     float *weights_out;         /* out [n_layers][n_batch][kv_heads][out_stride], or NULL; may be weights */
     int32_t *positions_out;     /* out, same layout, or NULL; may be positions                          */
