@@ -260,6 +260,7 @@ class Pool:
         h = C.c_void_p()
         check(lib.ekv_pool_create(C.byref(self.cfg), C.byref(h)), "ekv_pool_create")
         self.h = h
+        self.head_dim, self.kv_heads = head_dim, kv_heads  # (a field of cfg takes as long as a small check)
 
     def close(self):
         if self.h:
@@ -384,16 +385,25 @@ class Pool:
         """ekv_rope_append: turn q [rows, q_heads, head_dim] into q_out and k into the pages beside v ([rows, kv_heads,
         head_dim]), all bf16 and by source row. q, k and v may be slices of one [rows, columns] projection output:
         rows may be any distance apart, a row's heads are adjacent. Either pair may be left out."""
-        cfg = self.cfg
-        q_heads, q_stride = _rows(q, cfg.head_dim, "q")
-        kv = _rows(k, cfg.head_dim, "k")
-        if kv != _rows(v, cfg.head_dim, "v") or (k is not None and kv[0] != cfg.kv_heads):
-            raise ValueError("k and v must have the pool's KV heads and the same distance from row to row")
-        if q is not None and (q_out is None or q_out.shape != q.shape or not q_out.is_contiguous()):
-            raise ValueError("q_out must be contiguous and of q's shape")
-        check(lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), _ptr(seq_ids), _ptr(dst_pos), _ptr(n_rows),
-                                  _ptr(src_row), max_rows, _ptr(positions), q_heads, _ptr(q), q_stride, _ptr(q_out),
-                                  _ptr(k), _ptr(v), kv[1], _stream(stream)), "ekv_rope_append")
+        q_heads = q_stride = kv_stride = 0
+        qp = q_to = kp = vp = seqs = dst = None
+        if q is not None:
+            q_heads, q_stride = _rows(q, self.head_dim, "q")
+            if q_out is None or q_out.shape != q.shape or not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous and of q's shape")
+            qp, q_to = q.data_ptr(), q_out.data_ptr()
+        if k is not None or v is not None:
+            if k is None or v is None or k.shape != v.shape or k.stride() != v.stride():
+                raise ValueError("k and v must have one shape and the same distance from row to row")
+            kv_heads, kv_stride = _rows(k, self.head_dim, "k and v")
+            if kv_heads != self.kv_heads:
+                raise ValueError("k and v must have the pool's KV heads")
+            kp, vp, seqs, dst = k.data_ptr(), v.data_ptr(), _ptr(seq_ids), _ptr(dst_pos)
+        code = lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), seqs, dst, n_rows.data_ptr(), src_row.data_ptr(),
+                                   max_rows, positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride,
+                                   _stream(stream))
+        if code:
+            check(code, "ekv_rope_append")
 
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
                     prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
@@ -484,12 +494,11 @@ def project_qkv_rope(pool: "Pool", layer, seq_ids, x, wq, wk, wv, positions, rop
 
 def _rows(t, head_dim, name):
     """Heads of a [rows, heads, head_dim] tensor and the elements from row to row; a row must be adjacent."""
-    if t is None:
-        return 0, 0
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[2] != head_dim or stride[2] != 1 or (shape[1] > 1 and stride[1] != head_dim):
-        raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
-    return shape[1], stride[0] if shape[0] > 1 else shape[1] * head_dim
+    if t.dim() == 3:
+        (rows, heads, dim), (to_row, to_head, to_col) = t.shape, t.stride()
+        if dim == head_dim and to_col == 1 and (to_head == dim or heads <= 1):
+            return heads, to_row if rows > 1 else heads * dim
+    raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
 
 
 class DevArray:
