@@ -722,29 +722,118 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
     }
 }
 
-// Rows of units that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c. Lanes look
-// at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one another.
-// WARPS = 1: a warp per row (8 rows a block), for calls of many rows, which have few parts each; WARPS = 8: the
-// block's warps take parts of one row in turn.
-constexpr int kMergeWarps = 8;
-template <int D, int WARPS>
-__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const TreeArgs a, int rows_tile, int n_rows) {
-    const int rows_all = a.n_draft * a.group;
-    const int warp = WARPS == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int id = WARPS == 1 ? blockIdx.x * kMergeWarps + (threadIdx.x >> 5) : blockIdx.x;
-    if (id >= n_rows) return;
-    const int bg = id / rows_all, row = id - bg * rows_all, rt = row / rows_tile, r = row - rt * rows_tile;
-    const int b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads;
-    const int t = row_token(a, row), hq = g * a.group + row - t * a.group;
-    const long long at = ((long long)b * a.n_draft + t) * a.q_heads + hq;
+// Rows of units that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c. Two forms: a
+// warp for four rows, whose parts are the same, so that 8 rows of parts are on their way at a time; or, where that
+// leaves SMs empty, a block for one row, its warps taking parts in turn.
+constexpr int kMergeWarps = 8, kMergeRows = 4;
+
+struct MergeRow {  // one of a group's rows: where its result goes, and its parts
+    int bg, rt, r;
+    long long at;
+};
+__device__ __forceinline__ MergeRow merge_row(const TreeArgs &a, int bg, int row, int rows_tile) {
+    MergeRow m;
+    m.bg = bg;
+    m.rt = row / rows_tile;
+    m.r = row - m.rt * rows_tile;
+    const int b = bg / a.pool.kv_heads, g = bg - b * a.pool.kv_heads, t = row_token(a, row);
+    m.at = ((long long)b * a.n_draft + t) * a.q_heads + g * a.group + row - t * a.group;
+    return m;
+}
+template <int D>
+__device__ __forceinline__ void merge_put(const TreeArgs &a, long long at, int i, float4 v, float inv) {
+    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    if (a.out_dtype == EKV_DTYPE_F32) ((float4 *)((float *)a.out + at * D))[i] = v;
+    else ((uint2 *)((uint16_t *)a.out + at * D))[i] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+__device__ __forceinline__ void merge_add(float4 &o, const float4 &v, float f) {
+    if (f == 0.0f) return;  // (a part that saw nothing for the row: its output may be anything)
+    o.x = fmaf(v.x, f, o.x);
+    o.y = fmaf(v.y, f, o.y);
+    o.z = fmaf(v.z, f, o.z);
+    o.w = fmaf(v.w, f, o.w);
+}
+
+// Part c of row r of a unit whose first CTA is `first`.
+__device__ __forceinline__ long long part_row(int c, int first, int rows_tile, int r) {
+    return (2ll * c + (c == first ? 1 : 0)) * rows_tile + r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_rows_kernel(const TreeArgs a, int rows_tile, int n_groups) {
+    constexpr int R = kMergeRows, PARTS = 32 / R, PER = (D + 127) / 128;  // float4 of a lane
+    const int lane = threadIdx.x & 31, id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    if (id >= n_groups) return;
+    const int rows_all = a.n_draft * a.group, groups = (rows_all + R - 1) / R;
+    const int bg = id / groups, row0 = (id - bg * groups) * R, rows = min(R, rows_all - row0);
+    const int sub = min(lane % R, rows - 1);  // (rows of a group are in one row tile: its size is a multiple of 8)
+    const MergeRow mine = merge_row(a, bg, row0 + sub, rows_tile);
+    const int r0 = mine.r - sub;
     grid_wait();
-    const int2 part = a.parts[bg * a.row_tiles + rt];
+    const int2 part = a.parts[bg * a.row_tiles + mine.rt];
     if (part.x == part.y) return;
-    __shared__ float4 s_o[WARPS == 1 ? 1 : kMergeWarps][D / 4];
-    constexpr int PER = (D + 127) / 128;  // float4 of a lane
-    auto slot_of = [&](int c) { return (2ll * c + (c == part.x ? 1 : 0)) * rows_tile + r; };
     float m = -INFINITY;
-    for (int c = part.x + lane; c <= part.y; c += 32) m = fmaxf(m, a.ws_ml[slot_of(c)].x);
+    for (int c = part.x + lane / R; c <= part.y; c += PARTS) m = fmaxf(m, a.ws_ml[part_row(c, part.x, rows_tile, mine.r)].x);
+#pragma unroll
+    for (int x = R; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    float l = 0.0f, lr = 0.0f;
+    float4 o[R][PER];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[k][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c0 = part.x; c0 <= part.y; c0 += PARTS) {
+        float f = 0.0f;
+        const int c = c0 + lane / R;
+        if (c <= part.y) {
+            const float4 ml = a.ws_ml[part_row(c, part.x, rows_tile, mine.r)];
+            f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+            l += f * ml.y;
+            lr += f * ml.z;
+        }
+        const int n = min(PARTS, part.y + 1 - c0);
+#pragma unroll 2
+        for (int k = 0; k < n; ++k) {
+            const float4 *src = (const float4 *)(a.ws_o + part_row(c0 + k, part.x, rows_tile, r0) * D);
+#pragma unroll
+            for (int rr = 0; rr < R; ++rr) {
+                const float fk = __shfl_sync(0xffffffffu, f, k * R + rr);
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (rr < rows && lane + 32 * i < D / 4) merge_add(o[rr][i], src[rr * (D / 4) + lane + 32 * i], fk);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = R; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, x);
+        lr += __shfl_xor_sync(0xffffffffu, lr, x);
+    }
+    const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        const float iv = __shfl_sync(0xffffffffu, inv, rr);
+        const long long at = __shfl_sync(0xffffffffu, mine.at, rr);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (rr < rows && lane + 32 * i < D / 4) merge_put<D>(a, at, lane + 32 * i, o[rr][i], iv);
+    }
+    if (a.lse && lane < rows) a.lse[mine.at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+// Lanes look at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one another.
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const TreeArgs a, int rows_tile) {
+    const int rows_all = a.n_draft * a.group, bg = blockIdx.x / rows_all;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const MergeRow mr = merge_row(a, bg, blockIdx.x - bg * rows_all, rows_tile);
+    grid_wait();
+    const int2 part = a.parts[bg * a.row_tiles + mr.rt];
+    if (part.x == part.y) return;
+    __shared__ float4 s_o[kMergeWarps][D / 4];
+    constexpr int PER = (D + 127) / 128;  // float4 of a lane
+    float m = -INFINITY;
+    for (int c = part.x + lane; c <= part.y; c += 32) m = fmaxf(m, a.ws_ml[part_row(c, part.x, rows_tile, mr.r)].x);
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     float l = 0.0f, lr = 0.0f;
@@ -754,26 +843,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
     for (int c0 = part.x; c0 <= part.y; c0 += 32) {
         float f = 0.0f;
         if (c0 + lane <= part.y) {
-            const float4 ml = a.ws_ml[slot_of(c0 + lane)];
+            const float4 ml = a.ws_ml[part_row(c0 + lane, part.x, rows_tile, mr.r)];
             f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
             l += f * ml.y;
             lr += f * ml.z;
         }
         const int n = min(32, part.y + 1 - c0);
 #pragma unroll 4
-        for (int k = warp; k < n; k += WARPS) {
+        for (int k = warp; k < n; k += kMergeWarps) {
             const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float4 *src = (const float4 *)(a.ws_o + slot_of(c0 + k) * D);
+            const float4 *src = (const float4 *)(a.ws_o + part_row(c0 + k, part.x, rows_tile, mr.r) * D);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (lane + 32 * i >= D / 4) continue;
-                const float4 v = src[lane + 32 * i];
-                if (fk == 0.0f) continue;  // (a part that saw nothing for the row)
-                o[i].x = fmaf(v.x, fk, o[i].x);
-                o[i].y = fmaf(v.y, fk, o[i].y);
-                o[i].z = fmaf(v.z, fk, o[i].z);
-                o[i].w = fmaf(v.w, fk, o[i].w);
-            }
+            for (int i = 0; i < PER; ++i)
+                if (lane + 32 * i < D / 4) merge_add(o[i], src[lane + 32 * i], fk);
         }
     }
 #pragma unroll
@@ -782,33 +864,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
         lr += __shfl_xor_sync(0xffffffffu, lr, x);
     }
     const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-    auto put = [&](int i, float4 v) {
-        v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-        if (a.out_dtype == EKV_DTYPE_F32) ((float4 *)((float *)a.out + at * D))[i] = v;
-        else ((uint2 *)((uint16_t *)a.out + at * D))[i] = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-    };
-    if constexpr (WARPS == 1) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < D / 4) put(lane + 32 * i, o[i]);
-    } else {
+    for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i < D / 4) s_o[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < D / 4; i += kMergeWarps * 32) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < D / 4) s_o[warp][lane + 32 * i] = o[i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < D / 4; i += kMergeWarps * 32) {
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < kMergeWarps; ++w) {
-                v.x += s_o[w][i].x;
-                v.y += s_o[w][i].y;
-                v.z += s_o[w][i].z;
-                v.w += s_o[w][i].w;
-            }
-            put(i, v);
-        }
+        for (int w = 0; w < kMergeWarps; ++w) merge_add(v, s_o[w][i], 1.0f);
+        merge_put<D>(a, mr.at, i, v, inv);
     }
-    if (a.lse && lane == 0 && warp == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+    if (a.lse && lane == 0 && warp == 0) a.lse[mr.at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- host side ----
@@ -881,11 +947,12 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     }
     if (rc || !a.split) return rc;
     const int tr = tile_rows(sh, a.pool, a.n_draft * a.group);
-    const int n_rows = a.n_batch * a.pool.kv_heads * a.n_draft * a.group;
-    // a warp per row once that fills the SMs
-    if (n_rows >= 4 * kMergeWarps * grid)
-        return launch_after(tree_merge_kernel<D, 1>, (n_rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, s, a, tr, n_rows);
-    return launch_after(tree_merge_kernel<D, kMergeWarps>, n_rows, kMergeWarps * 32, 0, s, a, tr, n_rows);
+    const int rows = a.n_draft * a.group, n_rows = a.n_batch * a.pool.kv_heads * rows;
+    if (n_rows >= 2 * kMergeWarps * grid) {
+        const int n_groups = a.n_batch * a.pool.kv_heads * ((rows + kMergeRows - 1) / kMergeRows);
+        return launch_after(tree_merge_rows_kernel<D>, (n_groups + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, s, a, tr, n_groups);
+    }
+    return launch_after(tree_merge_kernel<D>, n_rows, kMergeWarps * 32, 0, s, a, tr);
 }
 
 }  // namespace
