@@ -695,7 +695,7 @@ size_t ekv_tree_attention_workspace_size(const ekv_pool *p, const ekv_tree_param
     if (!p || !prm || prm->n_batch <= 0 || prm->n_draft <= 0 || prm->n_draft > EKV_MAX_DRAFT || prm->q_heads <= 0 ||
         prm->q_heads % p->cfg.kv_heads)
         return 0;
-    return ekv::tree_workspace(p->view, prm->n_batch, prm->n_draft, prm->q_heads, p->sms);
+    return ekv::tree_workspace(p->view, prm->n_batch, prm->n_draft, prm->q_heads, prm->softcap > 0.0f, p->sms);
 }
 
 int ekv_tree_attention(ekv_pool *p, const ekv_tree_params *prm, const void *q, const void *k_draft, const void *v_draft,

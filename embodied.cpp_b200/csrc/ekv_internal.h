@@ -155,13 +155,13 @@ int launch_project_qkv(const PoolView &p, int layer, int n_batch, const int32_t 
                        float rope_base, void *q_out, void *k_out, void *v_out, cudaStream_t s);
 // Draft-tree attention (ekv_tree.cu). The workspace size depends on the call's shape alone; max_len, an
 // upper bound of the cached lengths, only sizes the grid.
-size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, int sms);
+size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, bool capped, int sms);
 int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s);
 // The same for many rows per KV head, on the tcgen05 tensor cores (ekv_tree_tile.cu): bf16 pools at head_dim 64, 128
 // or 256. tree_tile_rows() rows per unit (0: these rows are not for it); the caller lays out the workspace for
 // tree_tile_ctas() CTAs.
 constexpr int kTreeTileRows = 128;
-int tree_tile_rows(const PoolView &p, int rows);
+int tree_tile_rows(const PoolView &p, int rows, bool capped);
 int tree_tile_ctas(const PoolView &p, int rows, int sms);
 int launch_tree_tile(const TreeArgs &a, int grid, cudaStream_t s);
 // Key weights (ekv_weights.cu)

@@ -879,19 +879,20 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
 
 // ---- host side ----
 // Row tiles: a warp holds 8, 16 or (up to head_dim 128) 32 rows; more rows take four warps' 16, so that a tile
-// of keys is read from memory once per 64 rows.
+// of keys is read from memory once per 64 rows. Many rows of bf16 pages go to the 5th-generation tensor cores
+// (tree_tile_rows()).
 enum class Shape { R8, R16, R32, R64, Tile };
 
-Shape shape_for(const PoolView &p, int rows) {
+Shape shape_for(const PoolView &p, int rows, bool capped) {
     const int head_dim = p.head_dim;
-    if (tree_tile_rows(p, rows)) return Shape::Tile;
+    if (tree_tile_rows(p, rows, capped)) return Shape::Tile;
     if (rows <= 8) return Shape::R8;
     if (rows <= 16) return Shape::R16;
     if (rows <= 32 && head_dim <= 128) return Shape::R32;
     return Shape::R64;
 }
-int tile_rows(Shape s, const PoolView &p, int rows) {
-    if (s == Shape::Tile) return tree_tile_rows(p, rows);
+int tile_rows(Shape s, const PoolView &p, int rows, bool capped) {
+    if (s == Shape::Tile) return tree_tile_rows(p, rows, capped);
     return s == Shape::R8 ? 8 : s == Shape::R16 ? 16 : s == Shape::R32 ? 32 : 64;
 }
 
@@ -903,9 +904,9 @@ int grid_ctas(Shape s, const PoolView &p, int rows, int sms) {
 struct WsLayout {
     size_t parts, ml, o, total;
 };
-WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int rt, int sms) {
-    const Shape sh = shape_for(p, rows);
-    const size_t slots = 2ull * grid_ctas(sh, p, rows, sms) * tile_rows(sh, p, rows);
+WsLayout ws_layout(const PoolView &p, int n_batch, int rows, bool capped, int rt, int sms) {
+    const Shape sh = shape_for(p, rows, capped);
+    const size_t slots = 2ull * grid_ctas(sh, p, rows, sms) * tile_rows(sh, p, rows, capped);
     WsLayout w;
     w.parts = 0;
     w.ml = ((size_t)n_batch * p.kv_heads * rt * sizeof(int2) + 255) / 256 * 256;
@@ -930,7 +931,9 @@ int launch_shape(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
         case Shape::R32:
             if constexpr (D <= 128) return launch_rows<D, Q8, 4, 1, 4>(a, grid, s);
             return EKV_ERR_UNSUPPORTED;
-        default: return launch_rows<D, Q8, 2, 4, 1>(a, grid, s);
+        default:  // (bf16 at head_dim 128: 33 rows and more are the tile kernel's)
+            if constexpr (Q8 || D != 128) return launch_rows<D, Q8, 2, 4, 1>(a, grid, s);
+            return EKV_ERR_UNSUPPORTED;
     }
 }
 
@@ -946,7 +949,7 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
         rc = launch_shape<D, false>(a, sh, grid, s);
     }
     if (rc || !a.split) return rc;
-    const int tr = tile_rows(sh, a.pool, a.n_draft * a.group);
+    const int tr = tile_rows(sh, a.pool, a.n_draft * a.group, a.cap_log2 != 0.0f);
     const int rows = a.n_draft * a.group, n_rows = a.n_batch * a.pool.kv_heads * rows;
     if (n_rows >= 2 * kMergeWarps * grid) {
         const int n_groups = a.n_batch * a.pool.kv_heads * ((rows + kMergeRows - 1) / kMergeRows);
@@ -957,20 +960,21 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
 
 }  // namespace
 
-size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, int sms) {
+size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, bool capped, int sms) {
     const int rows = n_draft * (q_heads / p.kv_heads);
-    const int tr = tile_rows(shape_for(p, rows), p, rows);
-    return ws_layout(p, n_batch, rows, (rows + tr - 1) / tr, sms).total;
+    const int tr = tile_rows(shape_for(p, rows, capped), p, rows, capped);
+    return ws_layout(p, n_batch, rows, capped, (rows + tr - 1) / tr, sms).total;
 }
 
 int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s) {
     const int rows = a.n_draft * a.group;
-    const Shape sh = shape_for(a.pool, rows);
-    const int tr = tile_rows(sh, a.pool, rows);
+    const bool capped = a.cap_log2 != 0.0f;
+    const Shape sh = shape_for(a.pool, rows, capped);
+    const int tr = tile_rows(sh, a.pool, rows, capped);
     a.row_tiles = (rows + tr - 1) / tr;
     const int64_t units = (int64_t)a.n_batch * a.pool.kv_heads * a.row_tiles;
     const int64_t all_rows = (int64_t)a.n_batch * a.pool.kv_heads * rows;
-    const WsLayout w = ws_layout(a.pool, a.n_batch, rows, a.row_tiles, sms);
+    const WsLayout w = ws_layout(a.pool, a.n_batch, rows, capped, a.row_tiles, sms);
     // (a request's tiles: 64 keys, and 64 or 32 drafts; the sums of a split call are 32-bit)
     const int64_t unit_tiles = (max_len + kTile - 1) / kTile + 1;
     const int64_t most_tiles = ((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens + kTile - 1) / kTile + 2;

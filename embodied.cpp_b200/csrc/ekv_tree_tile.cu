@@ -1,7 +1,7 @@
 // ekv_tree_tile.cu -- draft-tree attention for many query rows per KV head (bf16 pools), on tcgen05.
 //
-// The same sums as ekv_tree.cu. From about 64 rows per cached key the tensor pipe bounds the call, not the
-// bytes, so 128 rows take the 5th-generation tensor cores: S = Q K^T with both operands in shared memory and S
+// The same sums as ekv_tree.cu. With many rows per cached key the products bound the call, not the bytes, so row
+// tiles of 128 take the 5th-generation tensor cores (from 17 rows on: tree_tile_rows()): S = Q K^T with both operands in shared memory and S
 // in tensor memory, P = exp(S - m) as bf16 over S's own columns, O += P V with P read from tensor memory.
 // Four warps are the softmax of a 128-row tile (a thread is a row) and one more issues its products; one feeds K
 // and V through the copy engine (pool tiles are canonical operands as they are stored).
@@ -269,6 +269,8 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             uint8_t *sq = smem + slot * C::Q_BYTES;
             const int t = row_token(a, row00 + r);
             const bool on = r < rows && t < rq.n_nodes;
+            // a warp without a row leaves P as it is: its products go to rows of O that nobody reads
+            const bool live = __any_sync(0xffffffffu, on);
             // (units that the other row tile may still look at are at most NS back; this one's scan comes after every
             // warp's q_ready)
             if (threadIdx.x == 0) sh.bad[unit_no & 7] = 0;
@@ -310,74 +312,76 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t s_col = tmem + lane_base + (uint32_t)(C::S_COL + (it % NSB) * BN);
-                // the row's maximum of the tile
-                uint32_t sa[32], sb[32];
-                tmem_load32x2(s_col, s_col + 32, sa, sb);
-                if (!full) {
-                    const uint32_t bits = chunk_bits(word, 0, valid), bits1 = chunk_bits(word, 32, valid);
+                if (live) {
+                    // the row's maximum of the tile
+                    uint32_t sa[32], sb[32];
+                    tmem_load32x2(s_col, s_col + 32, sa, sb);
+                    if (!full) {
+                        const uint32_t bits = chunk_bits(word, 0, valid), bits1 = chunk_bits(word, 32, valid);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        if (!((bits >> k) & 1u)) sa[k] = 0xff800000u;
-                        if (!((bits1 >> k) & 1u)) sb[k] = 0xff800000u;
+                        for (int k = 0; k < 32; ++k) {
+                            if (!((bits >> k) & 1u)) sa[k] = 0xff800000u;
+                            if (!((bits1 >> k) & 1u)) sb[k] = 0xff800000u;
+                        }
                     }
-                }
-                float top = -INFINITY, top1 = -INFINITY;
+                    float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    top = max3(top, __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]));
-                    top1 = max3(top1, __uint_as_float(sb[k]), __uint_as_float(sb[k + 1]));
-                }
-                top = fmaxf(top, top1);
-                const float mt = top == -INFINITY ? -INFINITY : CAP ? score.capped(top) : top * a.scale_log2;
-                // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
-                const bool up = mt > m + 8.0f;
-                if (__any_sync(0xffffffffu, up)) {
-                    const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
-                    if (up) m = mt;
-                    l0 = fma_pair(l0, pair_of(f, f), 0);
-                    l1 = fma_pair(l1, pair_of(f, f), 0);
-                    lr = fma_pair(lr, pair_of(f, f), 0);
-                    if (i > 0) {
-                        const int pst = (it - 1) % NS;
-                        ok = warp_wait(smem_addr(&sh.v_done[slot][pst]), ((it - 1) / NS) & 1, abort);
-                        if (!ok) break;
-                        tc_fence_after();
+                    for (int k = 0; k < 32; k += 2) {
+                        top = max3(top, __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]));
+                        top1 = max3(top1, __uint_as_float(sb[k]), __uint_as_float(sb[k + 1]));
+                    }
+                    top = fmaxf(top, top1);
+                    const float mt = top == -INFINITY ? -INFINITY : CAP ? score.capped(top) : top * a.scale_log2;
+                    // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
+                    const bool up = mt > m + 8.0f;
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
+                        if (up) m = mt;
+                        l0 = fma_pair(l0, pair_of(f, f), 0);
+                        l1 = fma_pair(l1, pair_of(f, f), 0);
+                        lr = fma_pair(lr, pair_of(f, f), 0);
+                        if (i > 0) {
+                            const int pst = (it - 1) % NS;
+                            ok = warp_wait(smem_addr(&sh.v_done[slot][pst]), ((it - 1) / NS) & 1, abort);
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_load32(tmem + lane_base + C::O_COL + c0, o);
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t o[32];
+                                tmem_load32(tmem + lane_base + C::O_COL + c0, o);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tmem_st32(tmem + lane_base + C::O_COL + c0, o);
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tmem_st32(tmem + lane_base + C::O_COL + c0, o);
+                            }
+                            tmem_wait_st();
                         }
-                        tmem_wait_st();
                     }
+                    const float neg = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
+                    // (a masked score is -inf, of which the exponential is 0; a capped one is not, so it is put back to 0)
+                    auto to_p = [&](uint32_t (&s)[32], uint32_t bits, uint32_t col) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float2 v = make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+                            if (CAP) v = make_float2(score.capped(v.x) + neg, score.capped(v.y) + neg);
+                            else v = of_pair(fma_pair(pair_of(v.x, v.y), scale2, neg2));
+                            v = make_float2(ex2(v.x), ex2(v.y));
+                            if (CAP && !full) {
+                                if (!((bits >> (2 * k)) & 1u)) v.x = 0.0f;
+                                if (!((bits >> (2 * k + 1)) & 1u)) v.y = 0.0f;
+                            }
+                            if (k & 1) l1 = add_pair(l1, pair_of(v.x, v.y));
+                            else l0 = add_pair(l0, pair_of(v.x, v.y));
+                            p[k] = pack_bf16(v.x, v.y);
+                            lr = add_pair(lr, pair_of(__uint_as_float(p[k] << 16), __uint_as_float(p[k] & 0xffff0000u)));
+                        }
+                        tmem_st16(col, p);
+                    };
+                    to_p(sa, full ? 0xffffffffu : chunk_bits(word, 0, valid), s_col);
+                    to_p(sb, full ? 0xffffffffu : chunk_bits(word, 32, valid), s_col + 16);
+                    tmem_wait_st();
                 }
-                const float neg = m == -INFINITY ? 0.0f : -m;
-                const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
-                // (a masked score is -inf, of which the exponential is 0; a capped one is not, so it is put back to 0)
-                auto to_p = [&](uint32_t (&s)[32], uint32_t bits, uint32_t col) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        float2 v = make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-                        if (CAP) v = make_float2(score.capped(v.x) + neg, score.capped(v.y) + neg);
-                        else v = of_pair(fma_pair(pair_of(v.x, v.y), scale2, neg2));
-                        v = make_float2(ex2(v.x), ex2(v.y));
-                        if (CAP && !full) {
-                            if (!((bits >> (2 * k)) & 1u)) v.x = 0.0f;
-                            if (!((bits >> (2 * k + 1)) & 1u)) v.y = 0.0f;
-                        }
-                        if (k & 1) l1 = add_pair(l1, pair_of(v.x, v.y));
-                        else l0 = add_pair(l0, pair_of(v.x, v.y));
-                        p[k] = pack_bf16(v.x, v.y);
-                        lr = add_pair(lr, pair_of(__uint_as_float(p[k] << 16), __uint_as_float(p[k] & 0xffff0000u)));
-                    }
-                    tmem_st16(col, p);
-                };
-                to_p(sa, full ? 0xffffffffu : chunk_bits(word, 0, valid), s_col);
-                to_p(sb, full ? 0xffffffffu : chunk_bits(word, 32, valid), s_col + 16);
-                tmem_wait_st();
                 if (!full && slot == 0) {  // rows past the last key hold whatever was there: 0 * that must be 0
                     ok = warp_wait(smem_addr(&sh.full[st]), par, abort);
                     if (!ok) break;
@@ -513,8 +517,15 @@ int launch(const TreeArgs &a, int grid, cudaStream_t s) {
 
 }  // namespace
 
-int tree_tile_rows(const PoolView &p, int rows) {
-    if (p.dtype != EKV_DTYPE_BF16 || rows <= 64) return 0;
+// Where this form begins, measured over pools of 800 to 4096 keys and 1 to 16 requests. Scores without a cap: from 17
+// rows of a KV head (16 requests of 4096 keys, 8 KV heads: 24 rows 71 -> 46 us at head_dim 64, 90 -> 69 at 128, 131 -> 80
+// at 256; with 16 rows the rows kernel is ahead, 62 against 67 at head_dim 128). A cap costs a thread 64 tanhf a tile here,
+// which the rows kernel spreads over all lanes: from 33 rows (head_dim 128: 24 rows 103 against 119 us, 48 rows 170
+// against 116), and from 65 at head_dim 64 (48 rows: 25 against 24 us in a middling call, but 20 against 25 with 39 ragged
+// ones).
+int tree_tile_rows(const PoolView &p, int rows, bool capped) {
+    const int below = !capped ? 16 : p.head_dim == 64 ? 64 : 32;
+    if (p.dtype != EKV_DTYPE_BF16 || rows <= below) return 0;
     if (p.head_dim == 64 || p.head_dim == 128) return rows > kTreeTileRows ? 2 * kTreeTileRows : kTreeTileRows;
     return p.head_dim == 256 ? kTreeTileRows : 0;
 }
