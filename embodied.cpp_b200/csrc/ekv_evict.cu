@@ -8,9 +8,9 @@
 //   evict_select_kernel  one CTA per (layer, request, KV head): the keep-th largest key by radix selection on
 //                        its bits, one bit per slot for the choice, then a slot for each survivor
 //   evict_move_kernel    a warp per 32 slots moves the K and V rows of those that changed
-// Bounds and figures: the move is bound by DRAM (64 rows of 16384 slots cut to 8192, head_dim 128 bf16: 38 us where the
-// bytes alone would take 31), the selection by its barriers and the latency of its loads, not by bytes (15 us for those
-// 64 rows, whose weights and positions would take 1.3). Moving the rows in the CTA that chose them saved the second
+// Bounds and figures: the move is bound by DRAM (64 rows of 16384 slots cut to 4096, head_dim 128 bf16: 38 us where the
+// bytes alone would take 31), the selection by its instructions and barriers, not by bytes (14 us for those 64 rows,
+// whose weights would take 0.6). Moving the rows in the CTA that chose them saved the second
 // launch on the host but left a third of the SMs to move everything: 14.0 us against 13.3 for 18 rows of 1100 slots.
 #include <algorithm>
 
@@ -21,10 +21,12 @@ namespace ekv {
 namespace {
 
 // Threads of a selection: 512 for rows of up to kFewSlots slots, whose barriers cost more than their keys (18 rows of
-// 1100 slots, the move included: 11.7 us, against 12.8 with 256 threads and 12.6 with 1024), else 1024.
+// 1100 slots, the move included: 11.7 us, against 12.8 with 256 threads and 12.6 with 1024, all with 8 moving warps), else 1024.
 constexpr int kFewThreads = 512, kManyThreads = 1024, kFewSlots = 4096;
 constexpr int kBins = 2048;  // 11 bits of the key at a time: 11, 11, 10
-constexpr int kMoveWarps = 8;
+// Warps of a moving CTA: few, so that the last wave of CTAs is a short one (64 rows of 16384 slots cut to 4096, the
+// selection included: 56.0 us with 8 warps, 54.1 with 2).
+constexpr int kMoveWarps = 2;
 
 // Larger is kept first. Protected rows are above every weight, NaN is below.
 __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
@@ -298,35 +300,41 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     const int words = (n + 31) / 32;
     uint32_t *sel = s_mem, *cnt = s_mem + a.max_words;  // chosen slots; ties, then free slots or survivors before a word
     uint32_t *list = s_mem + 2 * a.max_words;           // [kList] survivors at or above keep
-    each([&](int i, uint32_t k) {
-        const uint32_t gt = __ballot_sync(0xffffffffu, i < n && (k & mask) > prefix);
-        const uint32_t eq = __ballot_sync(0xffffffffu, i < n && (k & mask) == prefix);
-        const int wd = i >> 5;
-        if (lane == 0 && wd < words) {
-            sel[wd] = gt;
-            cnt[wd] = eq;
-        }
-    });
-    __syncthreads();
-    uint32_t ties = 0;
-    for (int w0 = 0; w0 < words; w0 += kSelThreads) {
-        const int wd = w0 + tid;
-        const uint32_t eq = wd < words ? cnt[wd] : 0u;
-        uint32_t total;
-        uint32_t rank = ties + block_scan(__popc(eq), sh, turn, total);
-        if (eq && rank < need) {
-            uint32_t take = need - rank, e = eq, got = 0;
-            if (take >= (uint32_t)__popc(eq)) {
-                got = eq;
-            } else {
-                for (; take; --take) {
-                    got |= e & (0u - e);
-                    e &= e - 1;
-                }
+    if (all) {  // (the usual case: no tie at the last place)
+        each([&](int i, uint32_t k) {
+            const uint32_t in = __ballot_sync(0xffffffffu, i < n && (k & mask) >= prefix);
+            if (lane == 0 && i < n) sel[i >> 5] = in;
+        });
+    } else {
+        each([&](int i, uint32_t k) {
+            const uint32_t gt = __ballot_sync(0xffffffffu, i < n && (k & mask) > prefix);
+            const uint32_t eq = __ballot_sync(0xffffffffu, i < n && (k & mask) == prefix);
+            if (lane == 0 && i < n) {
+                sel[i >> 5] = gt;
+                cnt[i >> 5] = eq;
             }
-            sel[wd] |= got;
+        });
+        __syncthreads();
+        uint32_t ties = 0;
+        for (int w0 = 0; w0 < words; w0 += kSelThreads) {
+            const int wd = w0 + tid;
+            const uint32_t eq = wd < words ? cnt[wd] : 0u;
+            uint32_t total;
+            uint32_t rank = ties + block_scan(__popc(eq), sh, turn, total);
+            if (eq && rank < need) {
+                uint32_t take = need - rank, e = eq, got = 0;
+                if (take >= (uint32_t)__popc(eq)) {
+                    got = eq;
+                } else {
+                    for (; take; --take) {
+                        got |= e & (0u - e);
+                        e &= e - 1;
+                    }
+                }
+                sel[wd] |= got;
+            }
+            ties += total;
         }
-        ties += total;
     }
     __syncthreads();
     // ---- survivors at or above keep before each word ----
@@ -352,10 +360,11 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     // ---- the survivors in order, and a free slot below keep for each ----
     const bool listed = holes <= (uint32_t)kList;
     if (listed) {
-        for (int i = (a.keep & ~31) + tid; i < 32 * words; i += kSelThreads) {
-            const int wd = i >> 5;
-            const uint32_t bits = tail_bits(wd);
-            if ((bits >> lane) & 1u) list[(wd == first_tail ? 0u : cnt[wd]) + __popc(bits & ((1u << lane) - 1u))] = i;
+        for (int i = 4 * first_tail + tid; i < 4 * words; i += kSelThreads) {  // eight slots each
+            const int wd = i >> 2, lo = 8 * (i & 3);
+            const uint32_t word = tail_bits(wd);
+            uint32_t at = (wd == first_tail ? 0u : cnt[wd]) + __popc(word & ((1u << lo) - 1u));
+            for (uint32_t bits = (word >> lo) & 0xffu; bits; bits &= bits - 1) list[at++] = 32 * wd + lo + __ffs(bits) - 1;
         }
         __syncthreads();
     }
