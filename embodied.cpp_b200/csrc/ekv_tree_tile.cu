@@ -14,6 +14,11 @@
 // With one S tile of 128 keys per row tile instead, the chain S, maximum, exponentials, P V left the tensor pipe
 // idle half of the time: 4300 cycles per 128 keys of two row tiles. With one issuing warp for both row tiles its
 // barrier waits, about 220 idle cycles each, took half: 5080 cycles.
+// Bound and figures: 8 requests of 8192 keys, 8 KV heads of 128 columns, 256 rows each (62 GFLOP, 258 MB) take 72 us and
+// 11 of the join, 750 TFLOP/s. 64 keys of two row tiles take 1980 cycles of the products' 1280: no pipe is full (tensor
+// memory and cores 55%, exponentials 41%, issue 45%), the softmax warps' chain of waits and tensor-memory reads is what
+// is left. Loading S of the next tile under the exponentials, with P in columns of its own, made it longer (2300 cycles);
+// exponentials and sums in a fixed order, or row tiles half a tile apart, changed nothing.
 #include "ekv_decode.cuh"
 
 namespace ekv {
