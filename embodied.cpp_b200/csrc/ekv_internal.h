@@ -158,8 +158,8 @@ int launch_project_qkv(const PoolView &p, int layer, int n_batch, const int32_t 
 size_t tree_workspace(const PoolView &p, int n_batch, int n_draft, int q_heads, bool capped, int sms);
 int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s);
 // The same for many rows per KV head, on the tcgen05 tensor cores (ekv_tree_tile.cu): bf16 pools at head_dim 64, 128
-// or 256. tree_tile_rows() rows per unit (0: these rows are not for it); the caller lays out the workspace for
-// tree_tile_ctas() CTAs.
+// or 256, Q8_0 pools at 64 or 128. tree_tile_rows() rows per unit (0: these rows are not for it); the caller lays out
+// the workspace for tree_tile_ctas() CTAs.
 constexpr int kTreeTileRows = 128;
 int tree_tile_rows(const PoolView &p, int rows, bool capped);
 int tree_tile_ctas(const PoolView &p, int rows, int sms);

@@ -17,8 +17,8 @@
 // Bound and figures: with up to 16 rows of a KV head the bytes: 16 requests of 16 k keys, 8 KV heads of 128 columns in
 // bf16 (976 MB), 4 rows each, take 151 us, 6.5 TB/s, 99% of the measured copy rate. Short caches are bound by the chain
 // launch, lengths, block ids, first tile, a few tiles, join: one token over 816 keys 8.4 us, 64 requests of 816 Q8_0 keys
-// 19 us where their bytes take 4.1. More rows of Q8_0 caches are bound by the matrix instructions of one warp per
-// scheduler: 32 rows of 16 requests of 4096 keys, 8 KV heads of 128 columns, 173 us.
+// 19 us where their bytes take 4.1. More rows are bound by the matrix instructions of one or two warps per
+// scheduler, and are the tile kernel's but for Q8_0 at head_dim 256, head_dim 48 and some capped calls.
 #include <algorithm>
 
 #include "ekv_decode.cuh"
@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const Tree
 
 // ---- host side ----
 // Row tiles: a warp holds 8, 16 or (up to head_dim 128) 32 rows; more rows take four warps' 16, so that a tile
-// of keys is read from memory once per 64 rows. Many rows of bf16 pages go to the 5th-generation tensor cores
+// of keys is read from memory once per 64 rows. More rows mostly go to the 5th-generation tensor cores
 // (tree_tile_rows()).
 enum class Shape { R8, R16, R32, R64, Tile };
 

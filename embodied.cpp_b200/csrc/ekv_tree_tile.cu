@@ -1,4 +1,4 @@
-// ekv_tree_tile.cu -- draft-tree attention for many query rows per KV head (bf16 pools), on tcgen05.
+// ekv_tree_tile.cu -- draft-tree attention for many query rows per KV head, on tcgen05.
 //
 // The same sums as ekv_tree.cu. With many rows per cached key the products bound the call, not the bytes, so row
 // tiles of 128 take the 5th-generation tensor cores (from 17 rows on: tree_tile_rows()): S = Q K^T with both operands in shared memory and S
@@ -27,28 +27,43 @@ namespace {
 using namespace decode;
 using namespace sm100;
 
-template <int D, int RT>
+// Q8: pages of 8-bit blocks. A value of one, int8 times an f16 scale, has up to 19 significant bits, so K and V are two
+// bf16 tiles each, the value rounded and what that left (2^-17 of it at most is lost), and each product is two: the
+// scores stay as exact as the rows kernel's. Eight warps make them from the blocks that the feeder brought, K before V,
+// so that S of the next tile waits neither for V nor behind the product before it (one barrier for both: 204 us instead
+// of 158 for 32 rows of 16 requests of 4096 keys, 8 KV heads of 128 columns), and Q lies in tensor memory (152 us). 64 keys
+// take 4200 cycles of an SM: 2600 of conversion, and products at half their rate beside its shared-memory writes.
+template <int D, int RT, bool Q8>
 struct TCfg {
     static constexpr int BN = kTile, NSB = 2;                   // keys per tile; S tiles per row tile
-    static constexpr int NS = RT == 2 || D == 64 ? 4 : 2;    // K and V stages
-    static constexpr int CTAS = D > 128 || RT == 2 ? 1 : 2;  // per SM
+    static constexpr int NS = RT == 2 || D == 64 ? 4 : 2;          // K and V stages
+    static constexpr int CTAS = D > 128 || RT == 2 || Q8 ? 1 : 2;  // per SM
     static constexpr uint32_t SBO = 16 * D;        // bytes between 8-row groups; chunks of 64 columns are 1024 apart
     static constexpr uint32_t LAYOUT = 2;          // 128-byte swizzle
-    static constexpr int KV_BYTES = BN * D * 2;
+    static constexpr int PARTS = Q8 ? 2 : 1;       // of K and V
+    static constexpr int PART_BYTES = BN * D * 2, KV_BYTES = PARTS * PART_BYTES;
+    static constexpr int NR = Q8 ? 3 : 1;          // stages of blocks as they are stored, K then V (Q8)
+    static constexpr int RAW_KV = (TileCfg<D, true>::KV_BYTES + 127) / 128 * 128;
     static constexpr int Q_BYTES = kTreeTileRows * D * 2;
     static constexpr int SLOT_COLS = 256;          // tensor-memory columns from row tile to row tile
-    static constexpr int S_COL = 0, O_COL = BN * NSB, COLS = D > 128 ? 512 : SLOT_COLS * RT;
-    static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_SH = OFF_V + NS * KV_BYTES;
-    static constexpr int SMEM = OFF_SH + 1024 + 1024;
-    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = ROW_WARPS + RT, THREADS = (FEED_WARP + 1) * 32;
+    static constexpr int S_COL = 0, O_COL = BN * NSB, Q_COL = O_COL + D;
+    static constexpr int COLS = D > 128 || (Q8 && D == 128) ? 512 : SLOT_COLS * RT;
+    static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES;
+    static constexpr int OFF_RAW = OFF_V + NS * KV_BYTES, OFF_SH = OFF_RAW + (Q8 ? (NR * 2 * RAW_KV + 1023) / 1024 * 1024 : 0);
+    static constexpr int SMEM = OFF_SH + 2048 + 1024;
+    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = ROW_WARPS + RT;
+    static constexpr int CONV_WARP = FEED_WARP + 1, CONV_WARPS = Q8 ? 8 : 0, THREADS = (CONV_WARP + CONV_WARPS) * 32;
     static_assert(O_COL + D <= (D > 128 ? 512 : SLOT_COLS), "tensor memory");
     static_assert(D % 64 == 0 && (RT == 1 || D <= 128), "whole swizzle chunks; two outputs fit");
+    static_assert(!Q8 || (RT == 1 && D <= 128), "shared memory");
 };
 
 // Phases: full, s_full, v_done and v_clean go by the tile's stage (tile / NS), p_full by its S tile (tile / NSB),
 // q_ready by the CTA's unit. The two row tiles run at most NS tiles apart, as a stage is refilled after both.
 struct TShared {
-    uint64_t full[4];       // K and V of the stage have landed
+    uint64_t full[4];       // K and V of the stage have landed (Q8: K)
+    uint64_t full_v[4];     // Q8: V
+    uint64_t raw_full[3], raw_empty[3];  // blocks have landed; are converted
     uint64_t s_full[2][4];  // [row tile][stage] S done
     uint64_t v_done[2][4];  // [row tile][stage] P V done
     uint64_t p_full[2][2];  // [row tile][S tile] P written
@@ -76,14 +91,51 @@ __device__ __forceinline__ uint32_t chunk_bits(unsigned long long word, int c0, 
     return n >= 32 ? w : n <= 0 ? 0u : w & ((1u << n) - 1u);
 }
 
-template <int D, int RT, bool CAP>
-__global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_tile_kernel(const TreeArgs a) {
-    using C = TCfg<D, RT>;
+// A Q8_0 block's rows as two bf16 tiles: 16 columns at a time, four of them and two rows in every eight lanes, which
+// then write to eight different 16-byte columns of the swizzled rows.
+template <int D, int THREADS>
+__device__ __forceinline__ void convert_tile(const uint8_t *raw, uint8_t *dst, int part_bytes, int valid, int thread) {
+    constexpr int U = D / 16;
+#pragma unroll 2
+    for (int e = thread; e < kTile * U; e += THREADS) {
+        const int rest = e >> 3, u = (rest % (U / 4)) * 4 + (e & 3), row = rest / (U / 4) * 2 + ((e >> 2) & 1);
+        uint32_t hi[8] = {}, lo[8] = {};
+        if (row < valid) {
+            const uint4 v = *(const uint4 *)(raw + q8_qs_off(row, 16 * u, D));
+            const float d = __half2float(*(const __half *)(raw + TileCfg<D, true>::SCALES + (row * (D / 32) + (u >> 1)) * 2));
+            const bool finite = fabsf(d) < INFINITY;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t q[2];
+                int8x4_to_bf16(w[i], q[0], q[1]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint64_t x = fma_pair(pair_of(__uint_as_float(q[k] << 16), __uint_as_float(q[k] & 0xffff0000u)), pair_of(d, d), 0);
+                    const uint32_t h = pack_bf16(of_pair(x).x, of_pair(x).y);
+                    const float2 r = of_pair(fma_pair(pair_of(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), pair_of(-1.0f, -1.0f), x));
+                    hi[2 * i + k] = h;
+                    lo[2 * i + k] = finite ? pack_bf16(r.x, r.y) : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t off = bf16_off<D>(row, 16 * u + 8 * k);
+            *(uint4 *)(dst + off) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+            *(uint4 *)(dst + part_bytes + off) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+        }
+    }
+}
+
+template <int D, int RT, bool Q8, bool CAP>
+__global__ void __launch_bounds__(TCfg<D, RT, Q8>::THREADS, TCfg<D, RT, Q8>::CTAS) tree_tile_kernel(const TreeArgs a) {
+    using C = TCfg<D, RT, Q8>;
     constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, ROWS = RT * kTreeTileRows;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     TShared &sh = *(TShared *)(smem + C::OFF_SH);
-    static_assert(sizeof(TShared) <= 1024, "barrier block");
+    static_assert(sizeof(TShared) <= 2048, "barrier block");
     volatile int *abort = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int hk = a.pool.kv_heads, units_per_req = hk * a.row_tiles;
@@ -91,7 +143,8 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(smem_addr(&sh.full[i]), 2);
+            mbar_init(smem_addr(&sh.full[i]), Q8 ? C::CONV_WARPS : 2);
+            if (Q8) mbar_init(smem_addr(&sh.full_v[i]), C::CONV_WARPS);
             mbar_init(smem_addr(&sh.v_clean[i]), 4);
             for (int k = 0; k < RT; ++k) {
                 mbar_init(smem_addr(&sh.s_full[k][i]), 1);
@@ -102,6 +155,10 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 4);
             mbar_init(smem_addr(&sh.q_ready[k]), 4);
             mbar_init(smem_addr(&sh.drained[k]), 1);
+        }
+        for (int i = 0; Q8 && i < C::NR; ++i) {
+            mbar_init(smem_addr(&sh.raw_full[i]), 2);
+            mbar_init(smem_addr(&sh.raw_empty[i]), C::CONV_WARPS);
         }
         sh.abort = 0;
         mbar_init_fence();
@@ -130,6 +187,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     const uint32_t tmem = sh.tmem;
 
     int it = 0, unit_no = 0;  // tiles and units of this CTA so far
+    int raw_it = 0;           // tiles of blocks (the feeder's and the converters')
     bool ok = true;
     TableWindow tw;  // (the feeder's)
     tw.reset(sh.table);
@@ -157,7 +215,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
 
         if (warp == C::FEED_WARP) {
             // ---- feeder ----
-            Piece next = find_piece<D, false>(a, rq, g, t0 * BN, tw, lane);
+            Piece next = find_piece<D, Q8>(a, rq, g, t0 * BN, tw, lane);
             if (a.split && lane == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
                 const unsigned long long end = base + (uint32_t)(u + 1) * n_tiles;
                 a.parts[b * units_per_req + u] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
@@ -165,7 +223,20 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             for (int j = t0; j < t1; ++j, ++it) {
                 const int st = it % NS, par = (it / NS) & 1;
                 const Piece pc = next;
-                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, false>(a, rq, g, (j + 1) * BN, tw, lane);
+                if (j + 1 < min(t1, p_tiles)) next = find_piece<D, Q8>(a, rq, g, (j + 1) * BN, tw, lane);
+                if constexpr (Q8) {
+                    if (j >= p_tiles) continue;  // (drafted rows are the converters')
+                    const int rs = raw_it % C::NR;
+                    if (raw_it >= C::NR) ok = ok && warp_wait(smem_addr(&sh.raw_empty[rs]), (raw_it / C::NR - 1) & 1, abort);
+                    if (!ok) {
+                        *abort = 1;
+                        continue;
+                    }
+                    const uint32_t raw = smem_addr(smem + C::OFF_RAW + rs * 2 * C::RAW_KV), bar = smem_addr(&sh.raw_full[rs]);
+                    issue_piece<D, true, true>(a, pc, raw, raw + C::RAW_KV, bar, bar, lane);
+                    ++raw_it;
+                    continue;
+                }
                 const uint32_t sk = smem_addr(smem + C::OFF_K + st * C::KV_BYTES);
                 const uint32_t sv = smem_addr(smem + C::OFF_V + st * C::KV_BYTES);
                 const uint32_t bar = smem_addr(&sh.full[st]);
@@ -209,6 +280,45 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     mbar_arrive(bar);
                 }
             }
+        } else if (Q8 && warp >= C::CONV_WARP) {
+            // ---- converters: K of a tile once S of the tile before it in its stage is done, V once that tile's P V is ----
+            const int thread = threadIdx.x - C::CONV_WARP * 32;
+            for (int j = t0; j < t1; ++j, ++it) {
+                const int st = it % NS, rs = raw_it % C::NR;
+                const bool draft = j >= p_tiles;
+                const int valid = draft ? rq.n_nodes : min(BN, rq.n_prefix - j * BN);
+                const uint8_t *raw = smem + C::OFF_RAW + rs * 2 * C::RAW_KV;
+                if (!draft) ok = ok && warp_wait(smem_addr(&sh.raw_full[rs]), (raw_it / C::NR) & 1, abort);
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v) {
+                    const uint32_t before = smem_addr(v ? &sh.v_done[0][st] : &sh.s_full[0][st]);
+                    if (it >= NS) ok = ok && warp_wait(before, (it / NS - 1) & 1, abort);
+                    if (!ok) break;
+                    uint8_t *dst = smem + (v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES;
+                    if (!draft) {
+                        convert_tile<D, C::CONV_WARPS * 32>(raw + v * C::RAW_KV, dst, C::PART_BYTES, valid, thread);
+                    } else {  // bf16 already: one part; rows past the last are zero
+                        constexpr int U = D / 8;
+                        const uint16_t *rows = (v ? a.v_draft : a.k_draft) + kv_row;
+                        for (int e = thread; e < BN * U; e += C::CONV_WARPS * 32) {
+                            const int r = e / U, u = e % U;
+                            *(uint4 *)(dst + bf16_off<D>(r, 8 * u)) =
+                                r < valid ? *(const uint4 *)(rows + (long long)r * hk * D + 8 * u) : make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_proxy_async();  // read by the tensor core
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(v ? &sh.full_v[st] : &sh.full[st]));
+                }
+                if (!ok) {
+                    *abort = 1;
+                    continue;
+                }
+                if (!draft) {
+                    if (lane == 0) mbar_arrive(smem_addr(&sh.raw_empty[rs]));
+                    ++raw_it;
+                }
+            }
         } else if (warp >= C::MMA_WARP) {
             // ---- products ----
             const int slot = warp - C::MMA_WARP;
@@ -216,6 +326,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 const uint32_t id_s = idesc_f16(true, false, BN), id_o = idesc_f16(true, true, D);
                 const uint32_t q_addr = smem_addr(smem), k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
                 auto s_at = [&](int i) { return tmem + (uint32_t)(slot * C::SLOT_COLS + C::S_COL + (i % NSB) * BN); };
+                auto parts_of = [&](int i) { return t0 + i - it >= p_tiles ? 1 : C::PARTS; };  // (drafts have one)
                 auto issue_s = [&](int i) {
                     const int st = i % NS;
                     if (!mbar_wait(smem_addr(&sh.full[st]), (i / NS) & 1, abort, kWait)) return false;
@@ -223,14 +334,22 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     const uint64_t qa = sdesc(q_addr + slot * C::Q_BYTES, 16, C::SBO, C::LAYOUT);
                     const uint64_t kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
 #pragma unroll
-                    for (int s4 = 0; s4 < D / 64; ++s4) {  // four 16-column steps of a 64-column chunk
-                        uint64_t av[4], bv[4];
+                    for (int part = 0; part < C::PARTS; ++part) {
+                        if (part >= parts_of(i)) break;
 #pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
-                            bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
+                        for (int s4 = 0; s4 < D / 64; ++s4) {  // four 16-column steps of a 64-column chunk
+                            uint64_t av[4], bv[4];
+                            uint32_t qt[4];
+#pragma unroll
+                            for (int s = 0; s < 4; ++s) {
+                                av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
+                                qt[s] = tmem + (uint32_t)(C::Q_COL + (4 * s4 + s) * 8);
+                                bv[s] = kb + ((uint32_t)(part * C::PART_BYTES + s4 * 1024 + s * 32) >> 4);
+                            }
+                            const uint32_t add = s4 > 0 || part > 0 ? 1u : 0u;
+                            if constexpr (Q8) mma_ts_x4<false>(s_at(i), qt, bv, id_s, add);
+                            else mma_ss_x4<false>(s_at(i), av, bv, id_s, add);
                         }
-                        mma_ss_x4<false>(s_at(i), av, bv, id_s, s4 > 0 ? 1u : 0u);
                     }
                     mma_commit(smem_addr(&sh.s_full[slot][st]));
                     return true;
@@ -238,18 +357,20 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                 auto issue_pv = [&](int i, bool first) {
                     const int st = i % NS;
                     if (!mbar_wait(smem_addr(&sh.p_full[slot][i % NSB]), (i / NSB) & 1, abort, kWait)) return false;
+                    if (Q8 && !mbar_wait(smem_addr(&sh.full_v[st]), (i / NS) & 1, abort, kWait)) return false;
                     tc_fence_after();
                     const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
 #pragma unroll
-                    for (int s4 = 0; s4 < BN / 64; ++s4) {
+                    for (int part = 0; part < C::PARTS; ++part) {
+                        if (part >= parts_of(i)) break;
                         uint32_t av[4];
                         uint64_t bv[4];
 #pragma unroll
                         for (int s = 0; s < 4; ++s) {
-                            av[s] = s_at(i) + (uint32_t)((4 * s4 + s) * 8);
-                            bv[s] = vb + ((uint32_t)(4 * s4 + s) * 2u * C::SBO >> 4);
+                            av[s] = s_at(i) + (uint32_t)(s * 8);
+                            bv[s] = vb + (((uint32_t)s * 2u * C::SBO + part * C::PART_BYTES) >> 4);
                         }
-                        mma_ts_x4<false>(tmem + (uint32_t)(slot * C::SLOT_COLS + C::O_COL), av, bv, id_o, (first && s4 == 0) ? 0u : 1u);
+                        mma_ts_x4<false>(tmem + (uint32_t)(slot * C::SLOT_COLS + C::O_COL), av, bv, id_o, first && part == 0 ? 0u : 1u);
                     }
                     mma_commit(smem_addr(&sh.v_done[slot][st]));
                     return true;
@@ -283,15 +404,34 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
             constexpr int U = D / 8;
             {
                 const long long mine = (((long long)b * a.n_draft + t) * a.q_heads + g * a.group + (row00 + r) - t * a.group) * D;
-                const uint32_t live = __ballot_sync(0xffffffffu, on);
+                if constexpr (Q8) {
+                    // to tensor memory: the converters' writes leave the shared memory no time to be read twice a product
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint4 v = on ? *(const uint4 *)(a.q + mine + 64 * c + 8 * k) : make_uint4(0, 0, 0, 0);
+                            w[4 * k] = v.x;
+                            w[4 * k + 1] = v.y;
+                            w[4 * k + 2] = v.z;
+                            w[4 * k + 3] = v.w;
+                        }
+                        tmem_st32(tmem + lane_base + C::Q_COL + 32 * c, w);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                } else {
+                    const uint32_t live = __ballot_sync(0xffffffffu, on);
 #pragma unroll 16
-                for (int i = lane; i < 32 * U; i += 32) {
-                    const int rr = i / U, uu = i % U;  // row of the warp (one per 32 or 16 lanes), unit
-                    const long long row = __shfl_sync(0xffffffffu, mine, rr);
-                    const bool has = (live >> rr) & 1u;
-                    cp_async_16_or_zero(smem_addr(sq + bf16_off<D>((warp & 3) * 32 + rr, 8 * uu)), has ? a.q + row + 8 * uu : a.q, has);
+                    for (int i = lane; i < 32 * U; i += 32) {
+                        const int rr = i / U, uu = i % U;  // row of the warp (one per 32 or 16 lanes), unit
+                        const long long row = __shfl_sync(0xffffffffu, mine, rr);
+                        const bool has = (live >> rr) & 1u;
+                        cp_async_16_or_zero(smem_addr(sq + bf16_off<D>((warp & 3) * 32 + rr, 8 * uu)), has ? a.q + row + 8 * uu : a.q, has);
+                    }
+                    cp_async_wait_all();
                 }
-                cp_async_wait_all();
             }
             fence_proxy_async();
             __syncwarp();
@@ -388,7 +528,7 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
                     tmem_wait_st();
                 }
                 if (!full && slot == 0) {  // rows past the last key hold whatever was there: 0 * that must be 0
-                    ok = warp_wait(smem_addr(&sh.full[st]), par, abort);
+                    ok = warp_wait(smem_addr(Q8 ? &sh.full_v[st] : &sh.full[st]), par, abort);
                     if (!ok) break;
                     uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
                     for (int e = max(0, valid) * U + threadIdx.x; e < BN * U; e += 128)
@@ -495,9 +635,10 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     }
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 11);
     if (warp == C::FEED_WARP && !ok && lane == 0) {
-        for (int i = 0; i < NS; ++i) {  // leave no copy writing this CTA's shared memory
-            mbar_wait_drain(smem_addr(&sh.full[i]), 0, kWait / 64);
-            mbar_wait_drain(smem_addr(&sh.full[i]), 1, kWait / 64);
+        for (int i = 0; i < (Q8 ? C::NR : NS); ++i) {  // leave no copy writing this CTA's shared memory
+            const uint32_t bar = smem_addr(Q8 ? &sh.raw_full[i] : &sh.full[i]);
+            mbar_wait_drain(bar, 0, kWait / 64);
+            mbar_wait_drain(bar, 1, kWait / 64);
         }
     }
     if (warp >= C::MMA_WARP && warp < C::FEED_WARP && lane == 0) {  // nor a product using its tensor memory
@@ -508,16 +649,16 @@ __global__ void __launch_bounds__(TCfg<D, RT>::THREADS, TCfg<D, RT>::CTAS) tree_
     if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
 }
 
-template <int D, int RT>
+template <int D, int RT, bool Q8 = false>
 int launch(const TreeArgs &a, int grid, cudaStream_t s) {
-    using C = TCfg<D, RT>;
+    using C = TCfg<D, RT, Q8>;
     static std::atomic<uint64_t> done{0}, done_cap{0};
     if (a.cap_log2 != 0.0f) {
-        if (const int rc = allow_smem(tree_tile_kernel<D, RT, true>, C::SMEM, done_cap)) return rc;
-        return launch_after(tree_tile_kernel<D, RT, true>, grid, C::THREADS, C::SMEM, s, a);
+        if (const int rc = allow_smem(tree_tile_kernel<D, RT, Q8, true>, C::SMEM, done_cap)) return rc;
+        return launch_after(tree_tile_kernel<D, RT, Q8, true>, grid, C::THREADS, C::SMEM, s, a);
     }
-    if (const int rc = allow_smem(tree_tile_kernel<D, RT, false>, C::SMEM, done)) return rc;
-    return launch_after(tree_tile_kernel<D, RT, false>, grid, C::THREADS, C::SMEM, s, a);
+    if (const int rc = allow_smem(tree_tile_kernel<D, RT, Q8, false>, C::SMEM, done)) return rc;
+    return launch_after(tree_tile_kernel<D, RT, Q8, false>, grid, C::THREADS, C::SMEM, s, a);
 }
 
 }  // namespace
@@ -527,19 +668,29 @@ int launch(const TreeArgs &a, int grid, cudaStream_t s) {
 // at 256; with 16 rows the rows kernel is ahead, 62 against 67 at head_dim 128). A cap costs a thread 64 tanhf a tile here,
 // which the rows kernel spreads over all lanes: from 33 rows (head_dim 128: 24 rows 103 against 119 us, 48 rows 170
 // against 116), and from 65 at head_dim 64 (48 rows: 25 against 24 us in a middling call, but 20 against 25 with 39 ragged
-// ones).
+// ones). Q8_0 at head_dim 64 and 128, the same calls: 32 rows 102 -> 97 and 172 -> 152 us, 256 rows 505 -> 184 and
+// 826 -> 297; with a cap from 65 (head_dim 128: 48 rows 258 against 323 us, 256 rows 957 against 591). At head_dim 256 two
+// parts of K and V do not fit the shared memory.
 int tree_tile_rows(const PoolView &p, int rows, bool capped) {
-    const int below = !capped ? 16 : p.head_dim == 64 ? 64 : 32;
-    if (p.dtype != EKV_DTYPE_BF16 || rows <= below) return 0;
+    const int below = !capped ? 16 : p.head_dim == 64 || p.dtype == EKV_DTYPE_Q8_0 ? 64 : 32;
+    if (rows <= below) return 0;
+    if (p.dtype != EKV_DTYPE_BF16) return p.head_dim == 64 || p.head_dim == 128 ? kTreeTileRows : 0;
     if (p.head_dim == 64 || p.head_dim == 128) return rows > kTreeTileRows ? 2 * kTreeTileRows : kTreeTileRows;
     return p.head_dim == 256 ? kTreeTileRows : 0;
 }
 
 int tree_tile_ctas(const PoolView &p, int rows, int sms) {
-    return sms * (p.head_dim <= 128 && rows <= kTreeTileRows ? 2 : 1);
+    return sms * (p.dtype == EKV_DTYPE_BF16 && p.head_dim <= 128 && rows <= kTreeTileRows ? 2 : 1);
 }
 
 int launch_tree_tile(const TreeArgs &a, int grid, cudaStream_t s) {
+    if (a.pool.dtype == EKV_DTYPE_Q8_0) {
+        switch (a.pool.head_dim) {
+            case 64: return launch<64, 1, true>(a, grid, s);
+            case 128: return launch<128, 1, true>(a, grid, s);
+            default: return EKV_ERR_UNSUPPORTED;
+        }
+    }
     const bool two = a.n_draft * a.group > kTreeTileRows;
     switch (a.pool.head_dim) {
         case 64: return two ? launch<64, 2>(a, grid, s) : launch<64, 1>(a, grid, s);
