@@ -40,8 +40,9 @@ struct SmallDiv {
 struct RopeArgs {
     PoolView pool;
     int32_t layer, n_batch, max_rows, rows_per_cta, q_heads, interleaved, rotary;
-    int32_t per;  // units (items of the odd forms) of a turned head
-    SmallDiv div_per, div_q, div_kv, div_v;
+    int32_t per;       // units of a turned head
+    int32_t per_item;  // items of a query head that is turned in place in the odd form, else 0
+    SmallDiv div_per, div_item, div_q, div_kv, div_v;
     float magnitude;
     const double *turns;
     const int32_t *seq_ids, *dst_pos, *n_rows, *src_row, *positions;
@@ -105,7 +106,36 @@ __device__ __forceinline__ void turn_unit(const RopeArgs &a, Unit r, int u, cons
     put(d + h, make_uint4(q[0], q[1], q[2], q[3]));
 }
 
-// Element i of the odd forms (split pairs that are not whole 16-byte units): i < n / 2 a pair, then the rest.
+// The odd form: split pairs that are not whole 16-byte units. Columns 8 u .. 8 u + 7 of the result, whose partners are
+// read one by one: 9 of 32 units where 66 of 256 columns turn (8 x 2000 rows of 16 such heads and v: 222 -> 131 us against
+// pair by pair; 64 columns, in whole units: 73).
+__device__ __forceinline__ uint4 odd_unit(const RopeArgs &a, const uint16_t *src, int u, const float2 *cs) {
+    const uint4 own = *(const uint4 *)(src + 8 * u);
+    const int n = a.rotary, h = n / 2;
+    if (8 * u >= n) return own;
+    uint16_t partner[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = 8 * u + e;
+        partner[e] = d < n ? src[d < h ? d + h : d - h] : (uint16_t)0;
+    }
+    const uint32_t w[4] = {own.x, own.y, own.z, own.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = 8 * u + e;
+        const uint32_t x = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+        uint32_t y = x;
+        if (d < h) y = rot_pair(x | (uint32_t)partner[e] << 16, cs[d]) & 0xffffu;
+        else if (d < n) y = rot_pair((uint32_t)partner[e] | x << 16, cs[d - h]) >> 16;
+        if (e & 1) r[e >> 1] |= y << 16;
+        else r[e >> 1] = y;
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Element i of a head that is turned in place in the odd form, where nobody else may have written what a pair reads:
+// i < n / 2 a pair, then the rest.
 template <class Put>
 __device__ __forceinline__ void rot_item(const RopeArgs &a, const uint16_t *src, int i, const float2 *cs, Put put) {
     const int h = a.rotary / 2;
@@ -164,9 +194,10 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
     }
     __syncthreads();
     // Items of the CTA's rows: (row, head, unit) of q, then of k, then of v, kLoads of them in flight per thread.
-    const int per = a.per, hk = p.kv_heads;
+    const int hk = p.kv_heads;
     if (a.q) {
-        const int total = nr * a.q_heads * per;
+        const bool items = !WIDE && a.per_item > 0;
+        const int per = items ? a.per_item : a.per, total = nr * a.q_heads * per;
         for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kLoads) {
             Unit x[kLoads];
             int rr[kLoads], uu[kLoads];
@@ -176,19 +207,21 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
                 const int i = i0 + j * kThreads;
                 rr[j] = -1;
                 if (i >= total) continue;
-                const int hr = a.div_per(i), r = a.div_q(hr), h = hr - r * a.q_heads;
+                const int hr = items ? a.div_item(i) : a.div_per(i), r = a.div_q(hr), h = hr - r * a.q_heads;
                 rr[j] = r;
                 uu[j] = i - hr * per;
                 const uint16_t *src = a.q + (row0 + r) * a.q_stride + h * D;
                 at[j] = ((row0 + r) * a.q_heads + h) * D;
                 if (WIDE) x[j] = load_unit(a, src, uu[j]);
-                else rot_item(a, src, uu[j], s_cs + r * half, [&](int d, uint16_t v) { a.q_out[at[j] + d] = v; });
+                else if (items) rot_item(a, src, uu[j], s_cs + r * half, [&](int d, uint16_t v) { a.q_out[at[j] + d] = v; });
+                else x[j].x = odd_unit(a, src, uu[j], s_cs + r * half);
             }
-            if constexpr (WIDE) {
 #pragma unroll
-                for (int j = 0; j < kLoads; ++j)
-                    if (rr[j] >= 0)
-                        turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, [&](int d, uint4 v) { *(uint4 *)(a.q_out + at[j] + d) = v; });
+            for (int j = 0; j < kLoads; ++j) {
+                if (rr[j] < 0 || items) continue;
+                auto put = [&](int d, uint4 v) { *(uint4 *)(a.q_out + at[j] + d) = v; };
+                if constexpr (WIDE) turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, put);
+                else put(8 * uu[j], x[j].x);
             }
         }
     }
@@ -225,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
         }
         return;
     }
-    const int total_k = nr * hk * per;
+    const int per = a.per, total_k = nr * hk * per;
     for (int i0 = threadIdx.x; i0 < total_k; i0 += kThreads * kLoads) {
         Unit x[kLoads];
         int rr[kLoads], uu[kLoads];
@@ -242,18 +275,14 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
             const uint16_t *src = a.k + (row0 + r) * a.kv_stride + h * D;
             tile[j] = p.prefix + prefix_tile_index(p, a.layer, s_blk[r], 0, h) * p.tile_bytes;
             if (WIDE) x[j] = load_unit(a, src, uu[j]);
-            else
-                rot_item(a, src, uu[j], s_cs + r * half, [&](int d, uint16_t v) {
-                    *(uint16_t *)(tile[j] + decode::bf16_off_any(s_rib[r], d, D, wlog)) = v;
-                });
+            else x[j].x = odd_unit(a, src, uu[j], s_cs + r * half);
         }
-        if constexpr (WIDE) {
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                if (rr[j] >= 0)
-                    turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, [&](int d, uint4 v) {
-                        *(uint4 *)(tile[j] + decode::bf16_off_any(s_rib[rr[j]], d, D, wlog)) = v;
-                    });
+        for (int j = 0; j < kLoads; ++j) {
+            if (rr[j] < 0) continue;
+            auto put = [&](int d, uint4 v) { *(uint4 *)(tile[j] + decode::bf16_off_any(s_rib[rr[j]], d, D, wlog)) = v; };
+            if constexpr (WIDE) turn_unit(a, x[j], uu[j], s_cs + rr[j] * half, put);
+            else put(8 * uu[j], x[j].x);
         }
     }
     const int pv = D / 8, total_v = nr * hk * pv;
@@ -309,10 +338,12 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
     const size_t smem = (size_t)a.rows_per_cta * (a.rotary / 2) * sizeof(float2);
     const bool wide = a.interleaved || a.rotary % 16 == 0;
     const int D = p.head_dim;
-    a.per = !wide ? a.rotary / 2 + D - a.rotary : a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8;
-    if ((int64_t)kMaxRows * std::max(q_heads, p.kv_heads) * D * std::max({a.per, q_heads, p.kv_heads, D / 8}) >= 1ll << 32)
+    a.per = !wide || a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8;
+    a.per_item = !wide && q == q_out ? D - a.rotary / 2 : 0;
+    if ((int64_t)kMaxRows * std::max(q_heads, p.kv_heads) * D * std::max({a.per, a.per_item, q_heads, p.kv_heads, D / 8}) >= 1ll << 32)
         return EKV_ERR_UNSUPPORTED;
     a.div_per = SmallDiv((uint32_t)a.per);
+    a.div_item = SmallDiv((uint32_t)std::max(1, a.per_item));
     a.div_q = SmallDiv((uint32_t)std::max(1, q_heads));
     a.div_kv = SmallDiv((uint32_t)p.kv_heads);
     a.div_v = SmallDiv((uint32_t)(D / 8));

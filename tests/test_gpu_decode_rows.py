@@ -45,3 +45,18 @@ def test_tree_scales_that_are_not_finite_stay_hidden():
     for use in ([160, 50], [131, 1]):
         out, lse, _ = run_tree(c, q, kd, vd, prefix_len=use)
         check_tree(c, q, kd, vd, out, lse, prefix_len=use)
+
+
+@pytest.mark.parametrize("rotary", [2, 18, 34, 66, 126, 64])
+def test_rope_in_place_is_the_same(rotary):
+    """Turning q where it lies gives the bits of turning it elsewhere, in the odd split form too."""
+    import ekv
+    c = dc.Cache([40, 9], 2, 128, seed=1)
+    rope = ekv.Rope(rotary_dims=rotary)
+    q = rand(51, 49, 6, 128)
+    pos = dc.ints(list(range(100, 149)))
+    args = (None, None, dc.ints([40, 9]), dc.ints([0, 40]), 40, pos)
+    out = torch.empty_like(q)
+    c.pool.rope_append(rope, 0, *args, q=q, q_out=out)
+    c.pool.rope_append(rope, 0, *args, q=q, q_out=q)
+    assert torch.equal(q.view(torch.int16), out.view(torch.int16)) and c.pool.status() == 0
