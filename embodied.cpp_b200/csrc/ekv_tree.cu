@@ -6,7 +6,8 @@
 //   lse = m + ln sum exp(s_k - m).
 // Probabilities are rounded to bf16 for the products with V, so the output is divided by the sum of the rounded
 // ones (a row with one heavy key would carry that key's rounding otherwise); lse takes the sum before rounding.
-// Q8_0 caches round p times the value's scale, a different number per 32 columns, and divide by the plain sum.
+// Q8_0 caches take p times the value's scale, a different number per 32 columns, as two bf16 parts and divide by the plain
+// sum. (As one part, one heavy key's 32 columns were all off by up to 2^-9 whatever the output's type.)
 // One pass over the keys: a warp keeps the reference maximum m, the sum and the output of its rows in
 // registers (the running softmax of Milakov and Gimelshein 2018, with the output as in flash attention,
 // Dao et al. 2022). m moves only when a score is more than 2^8 above it; every quotient is exact about that.
@@ -17,7 +18,7 @@
 // Bound and figures: with up to 16 rows of a KV head the bytes: 16 requests of 16 k keys, 8 KV heads of 128 columns in
 // bf16 (976 MB), 4 rows each, take 151 us, 6.5 TB/s, 99% of the measured copy rate. Short caches are bound by the chain
 // launch, lengths, block ids, first tile, a few tiles, join: one token over 816 keys 8.4 us, 64 requests of 816 Q8_0 keys
-// 19 us where their bytes take 4.1. More rows are bound by the matrix instructions of one or two warps per
+// 20 us where their bytes take 4.1. More rows are bound by the matrix instructions of one or two warps per
 // scheduler, and are the tile kernel's but for Q8_0 at head_dim 256, head_dim 48 and some capped calls.
 #include <algorithm>
 
@@ -532,13 +533,24 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) f[k] = scale_of(sc[k], gr);
                             }
-                            // the values' scales ride on the probabilities, which are rounded once either way
+                            // The values' scales ride on the probabilities, as two bf16 parts: one part would put a whole
+                            // group of 32 columns off by the same 2^-9. An infinite scale has no remainder (inf - inf), and
+                            // any finite number serves for it. The second part's products cost 3 to 10% of a call: 64 requests
+                            // of 816 keys, 256 columns, 8 rows 18.9 -> 19.8 us, 512 rows 557 -> 612.
 #pragma unroll
                             for (int n = 0; n < NR; ++n) {
-                                const uint32_t p0 = pack_bf16(pt[n][0] * f[0], pt[n][1] * f[1]);
-                                const uint32_t p1 = pack_bf16(pt[n][2] * f[2], pt[n][3] * f[3]);
+                                const uint64_t x01 = fma_pair(pair_of(pt[n][0], pt[n][1]), pair_of(f[0], f[1]), 0);
+                                const uint64_t x23 = fma_pair(pair_of(pt[n][2], pt[n][3]), pair_of(f[2], f[3]), 0);
+                                const uint32_t p0 = pack_bf16(of_pair(x01).x, of_pair(x01).y), p1 = pack_bf16(of_pair(x23).x, of_pair(x23).y);
+                                const uint64_t minus = pair_of(-1.0f, -1.0f);
+                                const float2 d0 = of_pair(fma_pair(pair_of(__uint_as_float(p0 << 16), __uint_as_float(p0 & 0xffff0000u)), minus, x01));
+                                const float2 d1 = of_pair(fma_pair(pair_of(__uint_as_float(p1 << 16), __uint_as_float(p1 & 0xffff0000u)), minus, x23));
+                                const float r[4] = {fminf(d0.x, 3e38f), fminf(d0.y, 3e38f), fminf(d1.x, 3e38f), fminf(d1.y, 3e38f)};
+                                const uint32_t r0 = pack_bf16(r[0], r[1]), r1 = pack_bf16(r[2], r[3]);
                                 mma_bf16(o[n][2 * gr], v0, p0, p1);
                                 mma_bf16(o[n][2 * gr + 1], v1, p0, p1);
+                                mma_bf16(o[n][2 * gr], v0, r0, r1);
+                                mma_bf16(o[n][2 * gr + 1], v1, r0, r1);
                             }
                         }
                     }
@@ -991,7 +1003,7 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     // Three ways to share the work: a CTA per unit (one or two tiles, or many units without a workspace); a cluster of
     // CTAs per unit; CTAs with equal ranges of all tiles and a second kernel that joins the parts. The last is the most
     // even one, but its second launch costs about 3.4 us, the time of `worth` tiles: one token over 816 keys takes 9.3 us
-    // with it and 8.4 as a cluster of eight, 64 requests of an 8-bit cache 22 and 19.
+    // with it and 8.4 as a cluster of eight, 64 requests of an 8-bit cache 22 and 20.
     const bool can_split = ws != nullptr && ws_bytes >= w.total && units * most_tiles < INT32_MAX;
     const int64_t even = (units * unit_tiles + full - 1) / full;  // tiles per CTA when split
     const int64_t worth = a.pool.dtype == EKV_DTYPE_Q8_0 ? 1 : 3;
