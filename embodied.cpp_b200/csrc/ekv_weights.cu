@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(kThreads, WCfg<D, Q8>::CTAS) key_weights_kerne
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&sh.empty[st]));  // the keys are in registers
-                float acc0 = 0.0f, acc1 = 0.0f;
+                float acc0, acc1;
                 // M tiles of eight query rows at a time: their products do not wait for one another
-                auto row_tiles = [&](auto count, int r0) {
+                auto row_tiles = [&](auto count, auto checked, int r0) {
                     constexpr int M = decltype(count)::value;
                     float s[M][2][4];  // even and odd column steps (Q8_0: one sum of scaled groups)
 #pragma unroll
@@ -246,21 +246,36 @@ __global__ void __launch_bounds__(kThreads, WCfg<D, Q8>::CTAS) key_weights_kerne
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
                         const float2 l = *(const float2 *)&slse[r0 + 8 * m + 2 * c];
+                        if constexpr (decltype(checked)::value) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if ((k & 1 ? l.y : l.x) == INFINITY) x[m][k] = -INFINITY;
+                        }
                         acc0 += ex2(x[m][0] - l.x) + ex2(x[m][1] - l.y);
                         acc1 += ex2(x[m][2] - l.x) + ex2(x[m][3] - l.y);
                     }
                 };
-                int r0 = 0;
+                // the sum of key key_l over all rows (checked: tile by tile, in the same order)
+                auto sum_rows = [&](auto checked) {
+                    acc0 = acc1 = 0.0f;
+                    int r0 = 0;
+                    if constexpr (!decltype(checked)::value)
 #pragma unroll 1
-                for (; r0 + 8 * kRowTiles <= rows; r0 += 8 * kRowTiles) row_tiles(std::integral_constant<int, kRowTiles>(), r0);
+                        for (; r0 + 8 * kRowTiles <= rows; r0 += 8 * kRowTiles) row_tiles(std::integral_constant<int, kRowTiles>(), checked, r0);
 #pragma unroll 1
-                for (; r0 < rows; r0 += 8) row_tiles(std::integral_constant<int, 1>(), r0);
+                    for (; r0 < rows; r0 += 8) row_tiles(std::integral_constant<int, 1>(), checked, r0);
 #pragma unroll
-                for (int m = 1; m < 4; m <<= 1) {
-                    acc0 += __shfl_xor_sync(0xffffffffu, acc0, m);
-                    acc1 += __shfl_xor_sync(0xffffffffu, acc1, m);
-                }
-                const float mine = c & 1 ? acc1 : acc0;
+                    for (int m = 1; m < 4; m <<= 1) {
+                        acc0 += __shfl_xor_sync(0xffffffffu, acc0, m);
+                        acc1 += __shfl_xor_sync(0xffffffffu, acc1, m);
+                    }
+                    return c & 1 ? acc1 : acc0;
+                };
+                // Rows that do not count have lse inf, and a number less inf is nothing. A key that is not finite has no
+                // number with them: a sum that came out NaN is taken again without them. (With that select in every sum
+                // 16 x 16 k keys took 86.8 us instead of 84.8, 256 rows 79.8 instead of 76.8.)
+                float mine = sum_rows(std::false_type());
+                if (__any_sync(0xffffffffu, writes && mine != mine)) mine = sum_rows(std::true_type());
                 if (writes) wrow[key] = old * (c0 > 0 ? 1.0f : a.decay) + mine;
             }
         }

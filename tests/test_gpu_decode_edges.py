@@ -1,10 +1,12 @@
 """Decoding operators where inputs are not finite, and what rounding may not cost. Shapes, checks and tolerances not derived
 here are those of test_gpu_decode.py."""
+import math
+
 import pytest
 import torch
 
 import decode_cases as dc
-from test_gpu_decode import check_tree, rand, run_tree
+from test_gpu_decode import STORES, check_tree, rand, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +43,48 @@ def test_tree_values_beyond_their_scale(dim, T, hq):
     out, lse, _ = run_tree(c, q, kd, vd)
     assert torch.isinf(out[..., 32:64]).all() and torch.isnan(out[..., 6]).all()
     check_tree(c, q, kd, vd, out, lse)
+
+
+@pytest.mark.parametrize("store,dim", STORES)
+@pytest.mark.parametrize("T,hq", [(1, 4), (3, 5), (9, 8)])
+def test_key_weights_of_rows_that_do_not_count(store, dim, T, hq):
+    """Keys that are not finite get nothing from rows that add nothing: tokens at or above n_nodes, rows with lse -inf, and
+    what fills up the kernel's tiles of rows."""
+    n = 90
+    c = dc.Cache([n, n, n], 1, dim, store=store, seed=2)
+    bad = torch.full((3, 1, dim), float("nan"), dtype=torch.bfloat16, device="cuda")
+    bad[1], bad[2] = float("inf"), 1e8
+    c.pool.append(0, c.seq_ids, dc.ints([4] * 3), dc.ints([3] * 3), dc.ints([0] * 3), 3, bad, bad)
+    q = rand(91, 3, T, hq, dim)
+    nodes = [0, T, max(0, T - 1)]
+    prm = c.pool.tree_params(layer=0, seq_ids=c.seq_ids, n_draft=T, q_heads=hq, scale=0.125, n_nodes=dc.ints(nodes))
+    lse = torch.full((3, T, hq), -math.inf, device="cuda")
+    lse[:, nodes[2]:] = 1.0  # (only of request 2 are these tokens beyond the last)
+    lse[1] = -math.inf
+    w = torch.rand(3, 1, n, generator=torch.Generator().manual_seed(1)).cuda()
+    old = w.clone()
+    c.pool.key_weights(prm, q, lse, w, 1.0)
+    torch.cuda.synchronize()
+    assert c.pool.status() == 0
+    assert torch.equal(w, old)
+
+
+@pytest.mark.parametrize("dim", [48, 64, 128, 256])
+@pytest.mark.parametrize("T,hq", [(1, 3), (5, 3), (17, 2)])
+def test_key_weights_of_a_key_far_below(dim, T, hq):
+    """A key of -infinity that every row takes to a score of -inf: weight 0, not the 0 * inf of rows that are not there."""
+    c = dc.Cache([70], 1, dim, seed=6)
+    bad = torch.zeros(1, 1, dim, dtype=torch.bfloat16, device="cuda")
+    bad[0, 0, 2] = float("-inf")
+    c.pool.append(0, c.seq_ids, dc.ints([9]), dc.ints([1]), dc.ints([0]), 1, bad, bad)
+    q = rand(92, 1, T, hq, dim)
+    q[..., 2] = 1.0
+    prm = c.pool.tree_params(layer=0, seq_ids=c.seq_ids, n_draft=T, q_heads=hq, scale=0.125, n_nodes=dc.ints([T]))
+    s = torch.einsum("thd,kd->thk", q[0].double(), c.rows(0)[0][:, 0].double()) * 0.125
+    lse = torch.logsumexp(s, -1).float()[None]
+    w = torch.zeros(1, 1, 70, device="cuda")
+    c.pool.key_weights(prm, q, lse, w, 0.0)
+    torch.cuda.synchronize()
+    want = torch.exp(s - lse[0].double()[..., None]).sum((0, 1))
+    assert want[9] == 0 and w[0, 0, 9] == 0
+    assert ((w[0, 0].double() - want).abs() <= 1e-4 * want).all()
