@@ -227,6 +227,30 @@ def _dense(*tensors):
             raise ValueError("arrays by slot or row must be contiguous")
 
 
+_bf16 = _f32 = None  # torch's types, once a call has met a tensor
+
+
+def _check_rows(*rows):
+    """(tensor, elements, f32?, name) each: raises unless the tensor holds that many adjacent elements of bf16 (or of its
+    bits) or f32. The calls ask for the usual case in line first: this takes 2 us of a call that may itself take 9."""
+    global _bf16, _f32
+    import torch
+    _bf16, _f32 = torch.bfloat16, torch.float32
+    for t, n, f32, name in rows:
+        types = (_f32,) if f32 else (_bf16, torch.int16, torch.uint16)
+        if t is not None and not (t.is_contiguous() and t.numel() >= n and t.dtype in types):
+            raise ValueError(f"{name} must be {n} adjacent {'f32' if f32 else 'bf16'} values or more, in one piece")
+
+
+def _index(t, n, size, name):
+    """The pointer of an index array (a tensor, or a DevArray of the library) of at least n elements of `size` bytes."""
+    if t is None:
+        return None
+    if t.numel() < n or (hasattr(t, "is_contiguous") and not (t.is_contiguous() and t.element_size() == size)):
+        raise ValueError(f"{name} must be {n} adjacent {8 * size}-bit integers or more, in one piece")
+    return t.data_ptr()
+
+
 def _current_stream():
     """The current torch stream's handle. torch.cuda.current_stream() makes a Stream object first, 3 us of a call that
     may itself take 5; where torch has the raw query it is asked instead."""
@@ -407,10 +431,10 @@ class Pool:
 
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
                     prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
-        p = TreeParams(layer, seq_ids.numel(), n_draft, q_heads, scale, softcap, out_dtype, 0, seq_ids.data_ptr(),
-                       None if prefix_len is None else prefix_len.data_ptr(),
-                       None if n_nodes is None else n_nodes.data_ptr(),
-                       None if ancestors is None else ancestors.data_ptr())
+        n = seq_ids.numel()
+        p = TreeParams(layer, n, n_draft, q_heads, scale, softcap, out_dtype, 0, _index(seq_ids, n, 4, "seq_ids"),
+                       _index(prefix_len, n, 4, "prefix_len"), _index(n_nodes, n, 4, "n_nodes"),
+                       _index(ancestors, n * n_draft, 8, "ancestors"))
         p._keep = (seq_ids, prefix_len, n_nodes, ancestors)
         return p
 
@@ -419,16 +443,40 @@ class Pool:
 
     def tree_attention(self, params: TreeParams, q, k_draft, v_draft, out, lse=None, workspace=None, stream=None):
         """ekv_tree_attention: q [n_batch, n_draft, q_heads, head_dim], k_draft / v_draft [n_batch, n_draft, kv_heads,
-        head_dim] bf16 over the cached prefix; out like q (bf16 or f32), lse f32 [n_batch, n_draft, q_heads]."""
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        check(lib.ekv_tree_attention(self.h, C.byref(params), _ptr(q), _ptr(k_draft), _ptr(v_draft), _ptr(out), _ptr(lse),
-                                     _ptr(workspace), ws_bytes, _stream(stream)), "ekv_tree_attention")
+        head_dim] bf16 over the cached prefix; out like q (bf16 or f32), lse f32 [n_batch, n_draft, q_heads]. All in one
+        piece: a slice of a projection needs .contiguous() first."""
+        rows, dim = params.n_batch * params.n_draft, self.head_dim
+        heads = rows * params.q_heads
+        n, m, f32 = heads * dim, rows * self.kv_heads * dim, params.out_dtype == DTYPE_F32
+        bf16 = _bf16
+        if not (q.dtype is bf16 and k_draft.dtype is bf16 and v_draft.dtype is bf16 and out.dtype is (_f32 if f32 else bf16)
+                and q.is_contiguous() and k_draft.is_contiguous() and v_draft.is_contiguous() and out.is_contiguous()
+                and q.numel() >= n and k_draft.numel() >= m and v_draft.numel() >= m and out.numel() >= n
+                and (lse is None or lse.dtype is _f32 and lse.is_contiguous() and lse.numel() >= heads)):
+            _check_rows((q, n, False, "q"), (k_draft, m, False, "k_draft"), (v_draft, m, False, "v_draft"), (out, n, f32, "out"),
+                        (lse, heads, True, "lse"))
+        ws_bytes = 0
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be in one piece")
+            ws_bytes = workspace.numel() * workspace.element_size()
+        code = lib.ekv_tree_attention(self.h, C.byref(params), q.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(),
+                                      out.data_ptr(), _ptr(lse), _ptr(workspace), ws_bytes, _stream(stream))
+        if code:
+            check(code, "ekv_tree_attention")
 
     def key_weights(self, params: TreeParams, q, lse, weights, decay=1.0, stream=None):
-        """ekv_key_weights: weights [n_batch, kv_heads, stride] f32 = decay * weights + what the rows give each key."""
-        _dense(lse, weights)
-        check(lib.ekv_key_weights(self.h, C.byref(params), _ptr(q), _ptr(lse), _ptr(weights), weights.shape[-1], decay,
-                                  _stream(stream)), "ekv_key_weights")
+        """ekv_key_weights: weights [n_batch, kv_heads, stride] f32 = decay * weights + what the rows give each key; q and
+        lse as ekv_tree_attention got and gave them."""
+        heads, stride = params.n_batch * params.n_draft * params.q_heads, weights.shape[-1]
+        n, m = heads * self.head_dim, params.n_batch * self.kv_heads * stride
+        if not (q.dtype is _bf16 and lse.dtype is _f32 and weights.dtype is _f32 and q.is_contiguous() and lse.is_contiguous()
+                and weights.is_contiguous() and q.numel() >= n and lse.numel() >= heads and weights.numel() >= m):
+            _check_rows((q, n, False, "q"), (lse, heads, True, "lse"), (weights, m, True, "weights"))
+        code = lib.ekv_key_weights(self.h, C.byref(params), q.data_ptr(), lse.data_ptr(), weights.data_ptr(), stride, decay,
+                                   _stream(stream))
+        if code:
+            check(code, "ekv_key_weights")
 
     def evict_by_weight(self, layer0, n_layers, seq_ids, weights, *, keep, first, recent, kept, weights_out=None,
                         positions=None, positions_out=None, seen=None, stream=None):

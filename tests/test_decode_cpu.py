@@ -143,3 +143,62 @@ def test_python_checks_of_rope_rows():
         p.rope_append(rope, 0, n, n, n, n, 3, n, q=x, q_out=x[:2])
     with pytest.raises(ValueError):
         p.rope_append(rope, 0, n, n, n, n, 3, n, k=x, v=x)  # 4 KV heads, the pool has 2
+
+
+class NoStream:
+    cuda_stream = 0
+
+
+def test_python_checks_of_tree_layouts():
+    """tree_attention and key_weights read and write adjacent rows: slices of a projection, short buffers and other types are
+    refused; what passes reaches the library (which has no device here)."""
+    torch = pytest.importorskip("torch")
+    p = pool()
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    ids = torch.zeros(3, dtype=torch.int32)
+    prm = p.tree_params(layer=0, seq_ids=ids, n_draft=2, q_heads=4, scale=0.125)
+    proj = bf(6, 8, 64)  # q, k and v of one projection: 4 + 2 + 2 heads
+    q, k, v = proj.split([4, 2, 2], 1)
+    good = dict(q=q.contiguous(), k=k.contiguous(), v=v.contiguous(), out=bf(3, 2, 4, 64), lse=torch.zeros(3, 2, 4))
+
+    def tree(ws=None, params=prm, **kw):
+        a = {**good, **kw}
+        p.tree_attention(params, a["q"], a["k"], a["v"], a["out"], a["lse"], ws, stream=NoStream)
+
+    def weights(w=None, **kw):
+        a = {**good, **kw}
+        p.key_weights(prm, a["q"], a["lse"], torch.zeros(3, 2, 100) if w is None else w, stream=NoStream)
+
+    for call in (tree, weights, lambda: tree(lse=None), lambda: tree(ws=torch.zeros(64, dtype=torch.uint8)), lambda: tree(q=bf(5, 2, 4, 64))):
+        with pytest.raises(ekv.EkvError) as e:
+            call()
+        assert e.value.code == ekv.ERR_UNSUPPORTED
+    for kw in (dict(q=q), dict(k=k), dict(v=v), dict(out=bf(3, 2, 64, 4).transpose(2, 3)), dict(lse=torch.zeros(3, 4, 2).transpose(1, 2)),
+               dict(q=bf(5, 4, 64)), dict(k=bf(5, 2, 64)), dict(v=bf(5, 2, 64)), dict(out=bf(3, 2, 3, 64)), dict(lse=torch.zeros(3, 2, 3)),
+               dict(q=torch.zeros(3, 2, 4, 64)), dict(k=torch.zeros(6, 2, 64)), dict(v=good["v"].half()), dict(out=torch.zeros(3, 2, 4, 64)),
+               dict(lse=bf(3, 2, 4)), dict(ws=torch.zeros(64, 2, dtype=torch.uint8).T)):
+        with pytest.raises(ValueError):
+            tree(**kw)
+    f32 = p.tree_params(layer=0, seq_ids=ids, n_draft=2, q_heads=4, scale=0.125, out_dtype=ekv.DTYPE_F32)
+    with pytest.raises(ValueError):
+        tree(params=f32)
+    with pytest.raises(ekv.EkvError):
+        tree(params=f32, out=torch.zeros(3, 2, 4, 64))
+    for kw in (dict(q=q), dict(q=bf(5, 4, 64)), dict(lse=torch.zeros(3, 2, 3)), dict(w=torch.zeros(3, 100, 2).transpose(1, 2)),
+               dict(w=torch.zeros(2, 2, 100)), dict(w=bf(3, 2, 100)), dict(lse=torch.zeros(3, 4, 2).transpose(1, 2))):
+        with pytest.raises(ValueError):
+            weights(**kw)
+
+
+def test_python_checks_of_tree_params():
+    torch = pytest.importorskip("torch")
+    p = pool()
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    good = dict(seq_ids=i32(3), prefix_len=i32(3), n_nodes=i32(4), ancestors=torch.zeros(3, 2, dtype=torch.int64))
+    p.tree_params(layer=0, n_draft=2, q_heads=4, scale=1.0, **good)
+    for kw in (dict(seq_ids=i32(3, 2)[:, 0]), dict(prefix_len=i32(2)), dict(prefix_len=i32(6)[::2]), dict(n_nodes=i32(2)),
+               dict(seq_ids=torch.zeros(3, dtype=torch.int64)), dict(n_nodes=torch.zeros(3, dtype=torch.int64)),
+               dict(ancestors=torch.zeros(3, 4, dtype=torch.int64)[:, :2]), dict(ancestors=i32(3, 2)),
+               dict(ancestors=torch.zeros(3, 1, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            p.tree_params(layer=0, n_draft=2, q_heads=4, scale=1.0, **{**good, **kw})
