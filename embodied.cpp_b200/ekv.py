@@ -221,34 +221,33 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _dense(*tensors):
-    for t in tensors:
-        if t is not None and not t.is_contiguous():
-            raise ValueError("arrays by slot or row must be contiguous")
-
-
-_bf16 = _f32 = None  # torch's types, once a call has met a tensor
+_bf16 = _f32 = _i32 = None  # torch's types, once a call has met a tensor
 
 
 def _check_rows(*rows):
     """(tensor, elements, f32?, name) each: raises unless the tensor holds that many adjacent elements of bf16 (or of its
     bits) or f32. The calls ask for the usual case in line first: this takes 2 us of a call that may itself take 9."""
-    global _bf16, _f32
+    global _bf16, _f32, _i32
     import torch
-    _bf16, _f32 = torch.bfloat16, torch.float32
+    _bf16, _f32, _i32 = torch.bfloat16, torch.float32, torch.int32
     for t, n, f32, name in rows:
         types = (_f32,) if f32 else (_bf16, torch.int16, torch.uint16)
         if t is not None and not (t.is_contiguous() and t.numel() >= n and t.dtype in types):
             raise ValueError(f"{name} must be {n} adjacent {'f32' if f32 else 'bf16'} values or more, in one piece")
 
 
-def _index(t, n, size, name):
-    """The pointer of an index array (a tensor, or a DevArray of the library) of at least n elements of `size` bytes."""
+def _index(t, n, name, bits=32):
+    """The pointer of an integer array (a tensor, or a DevArray of the library) of at least n elements."""
     if t is None:
         return None
-    if t.numel() < n or (hasattr(t, "is_contiguous") and not (t.is_contiguous() and t.element_size() == size)):
-        raise ValueError(f"{name} must be {n} adjacent {8 * size}-bit integers or more, in one piece")
+    if t.numel() < n or (hasattr(t, "is_contiguous") and not (t.is_contiguous() and t.dtype in _ints(bits))):
+        raise ValueError(f"{name} must be {n} adjacent {bits}-bit integers or more, in one piece")
     return t.data_ptr()
+
+
+def _ints(bits):
+    import torch
+    return (torch.int32, torch.uint32) if bits == 32 else (torch.int64, torch.uint64)
 
 
 def _current_stream():
@@ -432,9 +431,9 @@ class Pool:
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
                     prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
         n = seq_ids.numel()
-        p = TreeParams(layer, n, n_draft, q_heads, scale, softcap, out_dtype, 0, _index(seq_ids, n, 4, "seq_ids"),
-                       _index(prefix_len, n, 4, "prefix_len"), _index(n_nodes, n, 4, "n_nodes"),
-                       _index(ancestors, n * n_draft, 8, "ancestors"))
+        p = TreeParams(layer, n, n_draft, q_heads, scale, softcap, out_dtype, 0, _index(seq_ids, n, "seq_ids"),
+                       _index(prefix_len, n, "prefix_len"), _index(n_nodes, n, "n_nodes"),
+                       _index(ancestors, n * n_draft, "ancestors", 64))
         p._keep = (seq_ids, prefix_len, n_nodes, ancestors)
         return p
 
@@ -482,16 +481,36 @@ class Pool:
                         positions=None, positions_out=None, seen=None, stream=None):
         """ekv_evict_by_weight: weights (and positions) [n_layers, n_batch, kv_heads, stride], kept int32 [n_layers,
         n_batch, kv_heads, keep]; weights_out and positions_out have one stride of their own, or are the inputs."""
-        outs = [t for t in (weights_out, positions_out) if t is not None]
-        _dense(weights, kept, positions, *outs)
-        if len({t.shape[-1] for t in outs}) > 1 or (positions is not None and positions.shape != weights.shape):
+        n, stride = seq_ids.numel(), weights.shape[-1]
+        rows, out_stride = n_layers * n * self.kv_heads, 0
+        if weights_out is not None:
+            out_stride = weights_out.shape[-1]
+        elif positions_out is not None:
+            out_stride = positions_out.shape[-1]
+        if (positions_out is not None and positions_out.shape[-1] != out_stride
+                or positions is not None and positions.shape[-1] != stride):
             raise ValueError("weights and positions have one stride, and so have the outputs")
-        p = EvictParams(layer0, n_layers, seq_ids.numel(), keep, first, recent, seq_ids.data_ptr(),
-                        None if seen is None else seen.data_ptr(), weights.data_ptr(),
-                        None if positions is None else positions.data_ptr(), weights.shape[-1], kept.data_ptr(),
+        if kept.shape[-1] != keep and kept.dim() > 1:
+            raise ValueError("kept must be [n_layers, n_batch, kv_heads, keep]")
+        m, i32, f32 = rows * out_stride, _i32, _f32
+        if not (kept.dtype is i32 and kept.is_contiguous() and kept.numel() >= rows * keep
+                and (seq_ids.__class__ is DevArray or seq_ids.dtype is i32 and seq_ids.is_contiguous())
+                and weights.dtype is f32 and weights.is_contiguous() and weights.numel() >= rows * stride
+                and (weights_out is None or weights_out.dtype is f32 and weights_out.is_contiguous() and weights_out.numel() >= m)
+                and (positions is None or positions.dtype is i32 and positions.is_contiguous() and positions.numel() >= rows * stride)
+                and (positions_out is None or positions_out.dtype is i32 and positions_out.is_contiguous() and positions_out.numel() >= m)
+                and (seen is None or seen.__class__ is not DevArray and seen.dtype is i32 and seen.is_contiguous() and seen.numel() >= n)):
+            _check_rows((weights, rows * stride, True, "weights"), (weights_out, m, True, "weights_out"))
+            for t, size, name in ((kept, rows * keep, "kept"), (positions, rows * stride, "positions"),
+                                  (positions_out, m, "positions_out"), (seen, n, "seen"), (seq_ids, n, "seq_ids")):
+                _index(t, size, name)
+        p = EvictParams(layer0, n_layers, n, keep, first, recent, seq_ids.data_ptr(), None if seen is None else seen.data_ptr(),
+                        weights.data_ptr(), None if positions is None else positions.data_ptr(), stride, kept.data_ptr(),
                         None if weights_out is None else weights_out.data_ptr(),
-                        None if positions_out is None else positions_out.data_ptr(), outs[0].shape[-1] if outs else 0)
-        check(lib.ekv_evict_by_weight(self.h, C.byref(p), _stream(stream)), "ekv_evict_by_weight")
+                        None if positions_out is None else positions_out.data_ptr(), out_stride)
+        code = lib.ekv_evict_by_weight(self.h, C.byref(p), _stream(stream))
+        if code:
+            check(code, "ekv_evict_by_weight")
 
 
 class Rope:

@@ -196,9 +196,39 @@ def test_python_checks_of_tree_params():
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     good = dict(seq_ids=i32(3), prefix_len=i32(3), n_nodes=i32(4), ancestors=torch.zeros(3, 2, dtype=torch.int64))
     p.tree_params(layer=0, n_draft=2, q_heads=4, scale=1.0, **good)
+    p.tree_params(layer=0, n_draft=2, q_heads=4, scale=1.0, **{**good, "seq_ids": ekv.DevArray(P, 3)})
     for kw in (dict(seq_ids=i32(3, 2)[:, 0]), dict(prefix_len=i32(2)), dict(prefix_len=i32(6)[::2]), dict(n_nodes=i32(2)),
                dict(seq_ids=torch.zeros(3, dtype=torch.int64)), dict(n_nodes=torch.zeros(3, dtype=torch.int64)),
                dict(ancestors=torch.zeros(3, 4, dtype=torch.int64)[:, :2]), dict(ancestors=i32(3, 2)),
                dict(ancestors=torch.zeros(3, 1, dtype=torch.int64))):
         with pytest.raises(ValueError):
             p.tree_params(layer=0, n_draft=2, q_heads=4, scale=1.0, **{**good, **kw})
+
+
+def test_python_checks_of_evict_buffers():
+    """What the eviction reads and writes has room for all layers, requests and KV heads, in the layout that it is written in."""
+    torch = pytest.importorskip("torch")
+    p = pool()  # 2 layers, 2 KV heads
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    good = dict(seq_ids=i32(3), weights=torch.zeros(2, 3, 2, 100), kept=i32(2, 3, 2, 32), weights_out=torch.zeros(2, 3, 2, 40),
+                positions=i32(2, 3, 2, 100), positions_out=i32(2, 3, 2, 40), seen=i32(3))
+
+    def call(**kw):
+        a = {**good, **kw}
+        p.evict_by_weight(0, 2, a.pop("seq_ids"), a.pop("weights"), keep=32, first=4, recent=8, stream=NoStream, **a)
+
+    for kw in (dict(), dict(weights_out=None, positions_out=None), dict(positions=None), dict(seen=None), dict(kept=i32(384)),
+               dict(seq_ids=ekv.DevArray(P, 3)), dict(seq_ids=ekv.DevArray(P, 3), seen=ekv.DevArray(P, 3)),
+               dict(weights_out=good["weights"], positions_out=good["positions"])):
+        with pytest.raises(ekv.EkvError) as e:
+            call(**kw)
+        assert e.value.code == ekv.ERR_UNSUPPORTED, kw
+    for kw in (dict(kept=i32(2, 3, 2, 31)), dict(kept=i32(2, 3, 2, 40)), dict(kept=i32(1, 3, 2, 32)), dict(kept=torch.zeros(2, 3, 2, 32)),
+               dict(weights=torch.zeros(1, 3, 2, 100), positions=i32(1, 3, 2, 100)), dict(weights=i32(2, 3, 2, 100)),
+               dict(positions=torch.zeros(2, 3, 2, 100)), dict(positions=i32(2, 3, 2, 99)), dict(weights_out=torch.zeros(2, 3, 1, 40)),
+               dict(weights_out=i32(2, 3, 2, 40)), dict(positions_out=i32(2, 2, 2, 40)), dict(positions_out=i32(2, 3, 2, 41)),
+               dict(positions_out=torch.zeros(2, 3, 2, 40)), dict(seen=i32(2)), dict(seen=torch.zeros(3, dtype=torch.int64)),
+               dict(seq_ids=i32(3, 2)[:, 0]), dict(seq_ids=torch.zeros(3, dtype=torch.int64)), dict(seen=ekv.DevArray(P, 2)),
+               dict(weights=torch.zeros(2, 3, 100, 2).transpose(2, 3))):
+        with pytest.raises(ValueError):
+            call(**kw)
