@@ -88,3 +88,35 @@ def test_key_weights_of_a_key_far_below(dim, T, hq):
     want = torch.exp(s - lse[0].double()[..., None]).sum((0, 1))
     assert want[9] == 0 and w[0, 0, 9] == 0
     assert ((w[0, 0].double() - want).abs() <= 1e-4 * want).all()
+
+
+@pytest.mark.parametrize("store", ["bf16", "q8_0"])
+def test_evict_resize_and_attend_with_a_short_request(store):
+    """The whole turn over a batch in which one request has fewer tokens than are kept: it stays as it is, the others are cut,
+    and attention sees the rows that stayed and no slot besides. The pages that a request would gain hold NaN."""
+    lens, keep = [300, 41, 100, 101], 100
+    c = dc.Cache(lens, 2, 64, store=store, block=16, seed=8, spare=8, width=25)
+    junk = c.pool.seq_create()
+    c.pool.seq_resize(junk, 8 * 16)
+    c.pool.sync()
+    nan = torch.full((128, 2, 64), float("inf" if store == "q8_0" else "nan"), dtype=torch.bfloat16, device="cuda")
+    c.pool.append(0, dc.ints([junk]), dc.ints([0]), dc.ints([128]), dc.ints([0]), 128, nan, nan)
+    c.pool.seq_free(junk)
+    before = [c.rows(b) for b in range(4)]
+    w = torch.rand(1, 4, 2, 300, generator=torch.Generator().manual_seed(5)).cuda()
+    kept = torch.empty(1, 4, 2, keep, dtype=torch.int32, device="cuda")
+    c.pool.evict_by_weight(0, 1, c.seq_ids, w, keep=keep, first=4, recent=8, kept=kept)
+    for b, s in enumerate(c.seqs):
+        if c.lens[b] > keep:
+            c.pool.seq_resize(s, keep)
+            c.lens[b] = keep
+    c.pool.sync()
+    assert [c.pool.seq_get(s).n_tokens for s in c.seqs] == [100, 41, 100, 100]
+    q, kd, vd = rand(101, 4, 3, 4, 64), rand(102, 4, 3, 2, 64), rand(103, 4, 3, 2, 64)
+    out, lse, _ = run_tree(c, q, kd, vd)
+    check_tree(c, q, kd, vd, out, lse)
+    for b in range(4):  # and the rows in use are those that were kept
+        for x, y in zip(before[b], c.rows(b)):
+            for h in range(2):
+                at = kept[0, b, h, :c.lens[b]].long()
+                assert torch.equal(y[:, h], x[at, h])
