@@ -749,10 +749,15 @@ int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t s
     if (((uintptr_t)prm->weights | (uintptr_t)prm->kept | (uintptr_t)prm->positions | (uintptr_t)prm->weights_out |
          (uintptr_t)prm->positions_out) & 3)
         return EKV_ERR_INVALID_ARG;
-    int max_len = 0;
-    for (const ekv_pool::Seq &s : p->seqs)
-        if (s.live) max_len = std::max(max_len, s.n_tokens);
-    if (max_len > EKV_MAX_EVICT_TOKENS) return EKV_ERR_RANGE;
+    // Which sequences the call means is known on the device, where one that is too long is reported. Here the call is
+    // refused when its distinct sequences cannot all be short enough.
+    int max_len = 0, fit = 0, too_long = 0;
+    for (const ekv_pool::Seq &s : p->seqs) {
+        if (!s.live) continue;
+        max_len = std::max(max_len, s.n_tokens);
+        (s.n_tokens > EKV_MAX_EVICT_TOKENS ? too_long : fit)++;
+    }
+    if (too_long > 0 && prm->n_batch > fit) return EKV_ERR_RANGE;
     const DeviceScope dev_scope(p);
     if (const int e = dev_scope.rc()) return e;
     ekv::EvictArgs a{};

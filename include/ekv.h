@@ -380,7 +380,7 @@ int ekv_tree_attention(ekv_pool *pool, const ekv_tree_params *p, const void *q, 
 int ekv_key_weights(ekv_pool *pool, const ekv_tree_params *p, const void *q, const float *lse, float *weights,
                     int64_t weight_stride, float decay, ekv_stream_t stream);
 
-#define EKV_MAX_EVICT_TOKENS (1 << 19) /* longest sequence ekv_evict_by_weight takes */
+#define EKV_MAX_EVICT_TOKENS (1 << 19) /* longest sequence ekv_evict_by_weight takes; others may be longer */
 typedef struct ekv_evict_params {
     int32_t layer0, n_layers;   /* the layers [layer0, layer0 + n_layers)                              */
     int32_t n_batch;

@@ -232,3 +232,19 @@ def test_python_checks_of_evict_buffers():
                dict(weights=torch.zeros(2, 3, 100, 2).transpose(2, 3))):
         with pytest.raises(ValueError):
             call(**kw)
+
+
+def test_evict_range_is_of_the_calls_sequences():
+    """A sequence beyond the limit that the call does not need does not refuse it."""
+    p = pool(n_blocks=3000, block_tokens=256, max_blocks_per_seq=3000)
+    seqs = [p.seq_create() for _ in range(4)]
+    p.seq_resize(seqs[1], ekv.MAX_EVICT_TOKENS + 1)
+
+    def call(n):
+        e = ekv.EvictParams(0, 1, n, 32, 4, 8, P, None, P, None, 1 << 20, P, None, None, 0)
+        return L.ekv_evict_by_weight(p.h, C.byref(e), None)
+
+    assert call(3) == ekv.ERR_UNSUPPORTED
+    assert call(4) == ekv.ERR_RANGE
+    p.seq_resize(seqs[1], ekv.MAX_EVICT_TOKENS)
+    assert call(4) == ekv.ERR_UNSUPPORTED

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import decode_cases as dc
+import ekv
 from test_gpu_decode import STORES, check_tree, rand, run_tree
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +121,20 @@ def test_evict_resize_and_attend_with_a_short_request(store):
             for h in range(2):
                 at = kept[0, b, h, :c.lens[b]].long()
                 assert torch.equal(y[:, h], x[at, h])
+
+
+def test_evict_beside_a_sequence_beyond_the_limit():
+    """A sequence longer than any eviction takes, which the call does not name, changes nothing; named, it is reported."""
+    n = ekv.MAX_EVICT_TOKENS + 1
+    c = dc.Cache([300, n, 90], 1, 16, block=256, seed=3)
+    w = torch.rand(1, 2, 1, 300, generator=torch.Generator().manual_seed(6)).cuda()
+    kept = torch.empty(1, 2, 1, 80, dtype=torch.int32, device="cuda")
+    c.pool.evict_by_weight(0, 1, dc.ints([c.seqs[0], c.seqs[2]]), w, keep=80, first=4, recent=8, kept=kept)
+    torch.cuda.synchronize()
+    assert c.pool.status() == 0
+    for b, m in enumerate((300, 90)):
+        assert kept[0, b, 0].tolist() == dc.evict(w[0, b, 0, :m].tolist(), m, 80, 4, 8)
+    long = torch.rand(1, 1, 1, n, generator=torch.Generator().manual_seed(7)).cuda()
+    c.pool.evict_by_weight(0, 1, dc.ints([c.seqs[1]]), long, keep=80, first=4, recent=8, kept=kept)
+    torch.cuda.synchronize()
+    assert c.pool.status() == ekv.DEV_ERR_BAD_POS
