@@ -37,7 +37,9 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool safe) {
 
 constexpr int kCopies = 4;   // histograms, by lane: weights share few exponents, so lanes meet in few bins
 constexpr int kList = 12288; // survivors listed in shared memory; where more move, each free slot searches for its own
-constexpr int kInRegs = 16;  // keys a thread keeps (16384 slots); longer rows are read again by each pass
+// Keys a thread keeps (16384 slots); longer rows are read again by each pass: 64 rows cut to 4096 take 54 us from 16000 slots,
+// 63 from 17000, 130 from 60000, 16 rows 560 from 400000.
+constexpr int kInRegs = 16;
 
 struct SelShared {
     uint32_t hist[kCopies][kBins];
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
     const int32_t *pos = a.positions ? a.positions + (int64_t)lbh * a.weight_stride : nullptr;
     // The row is asked for before its length is known: the sequence's id and length are two reads one after the other.
     // All of a thread's loads come first: with the test of each key between them a row of 16384 took 10 us to read.
-    const int ahead = a.row_hint <= kInRegs * kSelThreads ? a.row_hint : 0;
+    const int ahead = min(a.row_hint, kInRegs * kSelThreads);
     uint32_t keys[kInRegs], ages[kInRegs];
 #pragma unroll
     for (int j = 0; j < kInRegs; ++j) {
@@ -410,9 +412,12 @@ int launch_evict(EvictArgs a, int max_live, cudaStream_t s) {
     if (n * chunks > INT32_MAX) return EKV_ERR_INVALID_ARG;
     a.max_words = (a.max_len + 31) / 32 + 1;
     const size_t smem = ((size_t)a.max_words * 2 + kList) * sizeof(uint32_t);
-    // The longest live sequence picks the form and how much of a row is read ahead: any sequence is right with either.
+    // The longest live sequence and the stride bound the rows of the call, which are known on the device: they pick the form
+    // and how much of a row is read ahead, and any sequence is right with either. A longer sequence that is not of the call
+    // counts only where the stride has room for it: 18 rows of 1100 slots 9.6 us, 10.8 with a stride of 20480 and such a
+    // sequence beside them; 64 rows of 16000 slots 54 us either way.
     a.row_hint = (int)std::min<int64_t>(std::min(max_live, a.max_len), a.weight_stride);
-    const bool few = max_live <= kFewSlots;
+    const bool few = a.row_hint <= kFewSlots;
     static std::atomic<uint64_t> few_done{0}, many_done{0};
     const int most_smem = ((EKV_MAX_EVICT_TOKENS / 32 + 1) * 2 + kList) * (int)sizeof(uint32_t);
     int rc = few ? decode::allow_smem(evict_select_kernel<kFewThreads>, most_smem, few_done)

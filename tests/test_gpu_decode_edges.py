@@ -7,7 +7,7 @@ import torch
 
 import decode_cases as dc
 import ekv
-from test_gpu_decode import STORES, check_tree, rand, run_tree
+from test_gpu_decode import STORES, check_evict, check_tree, rand, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,18 @@ def test_evict_beside_a_sequence_beyond_the_limit():
     c.pool.evict_by_weight(0, 1, dc.ints([c.seqs[1]]), long, keep=80, first=4, recent=8, kept=kept)
     torch.cuda.synchronize()
     assert c.pool.status() == ekv.DEV_ERR_BAD_POS
+
+
+@pytest.mark.parametrize("lens", [[1100, 4096], [4097, 300], [16384, 16385, 16383, 200]])
+@pytest.mark.parametrize("stride", [0, 21000])
+def test_evict_rows_shorter_than_what_is_read_ahead(lens, stride):
+    """Rows on both sides of what the selection holds in registers, with strides as long as the rows and longer, beside an idle
+    sequence that is longer still."""
+    c = dc.Cache(lens, 1, 16, block=256, seed=4, spare=84, width=84)
+    c.pool.seq_resize(c.pool.seq_create(), 20500)
+    c.pool.sync()
+    w = torch.rand(1, len(lens), 1, max(max(lens), stride), generator=torch.Generator().manual_seed(9)).cuda()
+    w[..., ::5] = 0.5
+    pos = torch.arange(w.shape[-1], dtype=torch.int32, device="cuda").flip(0).repeat(1, len(lens), 1, 1).contiguous()
+    check_evict(c, w, 150, 4, 20)
+    check_evict(c, w, 1000, 4, 20, positions=pos, seen=[w.shape[-1]] * len(lens))
