@@ -740,6 +740,7 @@ int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t s
         return EKV_ERR_INVALID_ARG;
     if (prm->keep <= 0 || prm->first < 0 || prm->recent < 0 || (int64_t)prm->first + prm->recent > prm->keep)
         return EKV_ERR_INVALID_ARG;
+    if (prm->keep > INT32_MAX - 4096) return EKV_ERR_RANGE;  // the kernels count slots past it in 32 bits
     if (prm->weight_stride < 0 || ((prm->weights_out || prm->positions_out) && prm->out_stride < prm->keep))
         return EKV_ERR_INVALID_ARG;
     // in place only where slot i is the same entry on both sides

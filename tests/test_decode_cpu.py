@@ -248,3 +248,11 @@ def test_evict_range_is_of_the_calls_sequences():
     assert call(4) == ekv.ERR_RANGE
     p.seq_resize(seqs[1], ekv.MAX_EVICT_TOKENS)
     assert call(4) == ekv.ERR_UNSUPPORTED
+
+
+def test_evict_keep_near_the_end_of_32_bits():
+    """Slot counters run up to a block of threads past keep; nothing is launched where that is beyond 32 bits."""
+    p = pool()
+    for keep, code in ((2 ** 31 - 1, ekv.ERR_RANGE), (2 ** 31 - 1024, ekv.ERR_RANGE), (2 ** 30, ekv.ERR_UNSUPPORTED)):
+        e = ekv.EvictParams(0, 2, 3, keep, 4, 8, P, None, P, None, 100, P, None, None, 0)
+        assert L.ekv_evict_by_weight(p.h, C.byref(e), None) == code
