@@ -412,7 +412,10 @@ extern "C" int ekv_rope_create(const ekv_rope_config *c, ekv_rope **out) {
         }
         const size_t bytes = (size_t)(c->rotary_dims / 2) * sizeof(double);
         int rc = cudaMalloc((void **)&r->dev_turns, bytes) == cudaSuccess ? EKV_OK : EKV_ERR_ALLOC;
-        if (!rc && cudaMemcpy(r->dev_turns, turns, bytes, cudaMemcpyHostToDevice) != cudaSuccess) rc = EKV_ERR_CUDA;
+        // (the copy of pageable memory may return before it has landed, and other streams do not wait for this one)
+        if (!rc && (cudaMemcpy(r->dev_turns, turns, bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
+                    cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess))
+            rc = EKV_ERR_CUDA;
         if (rc && r->dev_turns) cudaFree(r->dev_turns);
         if (rc) cudaGetLastError();
         if (prev != c->device) cudaSetDevice(prev);

@@ -7,7 +7,7 @@ import torch
 
 import decode_cases as dc
 import ekv
-from test_gpu_decode import STORES, check_evict, check_tree, rand, run_tree
+from test_gpu_decode import STORES, check_evict, check_tree, close_turned, rand, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,19 @@ def test_evict_rows_shorter_than_what_is_read_ahead(lens, stride):
     pos = torch.arange(w.shape[-1], dtype=torch.int32, device="cuda").flip(0).repeat(1, len(lens), 1, 1).contiguous()
     check_evict(c, w, 150, 4, 20)
     check_evict(c, w, 1000, 4, 20, positions=pos, seen=[w.shape[-1]] * len(lens))
+
+
+def test_rope_is_ready_when_it_is_made():
+    """A handle's frequencies are on the device when the call that makes it returns, whatever stream uses them first."""
+    c = dc.Cache([64], 1, 256, seed=1)
+    q, pos, out = rand(111, 32, 4, 256), dc.ints(range(32)), torch.empty(32, 4, 256, dtype=torch.bfloat16, device="cuda")
+    n, at = dc.ints([32]), dc.ints([0])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for i in range(50):
+        rope = ekv.Rope(rotary_dims=256, freq_base=100.0 + i)
+        c.pool.rope_append(rope, 0, None, None, n, at, 32, pos, q=q, q_out=out, stream=side)
+        side.synchronize()
+        want, size = dc.rope(q, pos, dc.rope_table(256, 100.0 + i), 256, False)
+        close_turned(out, want, size)
+        rope.close()
