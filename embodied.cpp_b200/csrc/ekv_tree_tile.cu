@@ -163,10 +163,11 @@ __global__ void __launch_bounds__(TCfg<D, RT, Q8>::THREADS, TCfg<D, RT, Q8>::CTA
         sh.abort = 0;
         mbar_init_fence();
     }
-    if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
     auto unit_tiles = [](const Req &r) { return max(1, (r.n_prefix + BN - 1) / BN + (r.n_nodes > 0 ? 1 : 0)); };
     grid_wait();
-    grid_launch_next();
+    // Tensor memory is taken between the two launch points: before the wait this CTA could hold columns that a CTA of the
+    // kernel it waits for still has to get, and after the signal a CTA of the next kernel could hold this one's.
+    if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
     tc_fence_before();
     Range rg;
     if (a.split) {
@@ -184,7 +185,8 @@ __global__ void __launch_bounds__(TCfg<D, RT, Q8>::THREADS, TCfg<D, RT, Q8>::CTA
         rg.ctas = 0;
     }
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = sh.tmem;  // (there is a barrier in either branch)
+    grid_launch_next();
 
     int it = 0, unit_no = 0;  // tiles and units of this CTA so far
     int raw_it = 0;           // tiles of blocks (the feeder's and the converters')

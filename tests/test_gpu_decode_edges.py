@@ -169,3 +169,22 @@ def test_rope_is_ready_when_it_is_made():
         want, size = dc.rope(q, pos, dc.rope_table(256, 100.0 + i), 256, False)
         close_turned(out, want, size)
         rope.close()
+
+
+def test_tree_calls_that_start_under_one_another():
+    """Calls of many rows over pools of several widths, a hundred in a row without a wait between them (each kernel starts while
+    the one before it drains, and holds tensor memory of its own): every result is that of the call alone."""
+    calls = []
+    for store, dim, T in (("bf16", 64, 6), ("bf16", 256, 6), ("q8_0", 128, 6), ("bf16", 64, 40), ("bf16", 128, 6), ("q8_0", 64, 40)):
+        c = dc.Cache([200, 90, 0], 2, dim, store=store, seed=dim)
+        q, kd, vd = rand(121, 3, T, 8, dim), rand(122, 3, T, 2, dim), rand(123, 3, T, 2, dim)
+        for ws in (False, True):
+            out, lse, prm = run_tree(c, q, kd, vd, workspace=ws)
+            room = torch.empty(c.pool.tree_attention_workspace_size(prm), dtype=torch.uint8, device="cuda") if ws else None
+            calls.append((c, prm, q, kd, vd, torch.zeros_like(out), torch.zeros_like(lse), room, out, lse))
+    for _ in range(10):
+        for c, prm, q, kd, vd, out, lse, room, _, _ in calls:
+            c.pool.tree_attention(prm, q, kd, vd, out, lse, room)
+    torch.cuda.synchronize()
+    for c, prm, q, kd, vd, out, lse, room, want, want_lse in calls:
+        assert c.pool.status() == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
