@@ -655,6 +655,10 @@ int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_
                                    q_heads, q, q_stride, q_out, k, v, kv_stride, p->sms, (cudaStream_t)stream);
 }
 
+// Rows of a KV head times its query heads, EKV_MAX_DRAFT * group^2, are 32-bit in the kernels.
+static bool group_too_large(int group) { return group >= 8192; }
+static_assert(EKV_MAX_DRAFT * 8191ll * 8191 < 1ll << 32, "rows times query heads");
+
 // Checks what attention and key weights share, and the longest live sequence (which only sizes grids).
 static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const void *q, ekv::TreeArgs &a, int &max_len) {
     if (!p || !prm || !q || !prm->seq_ids) return EKV_ERR_INVALID_ARG;
@@ -663,11 +667,13 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
         prm->q_heads % c.kv_heads)
         return EKV_ERR_INVALID_ARG;
     if (prm->n_draft > EKV_MAX_DRAFT) return EKV_ERR_RANGE;
-    if (!(prm->scale > 0.0f) || !std::isfinite(prm->scale) || !(prm->softcap >= 0.0f) || !std::isfinite(prm->softcap))
+    const float log2e = 1.4426950408889634f;
+    if (!(prm->scale > 0.0f) || !std::isfinite(prm->scale * log2e) || !(prm->softcap >= 0.0f) || !std::isfinite(prm->softcap * log2e))
         return EKV_ERR_INVALID_ARG;
+    const float cap_in = prm->softcap > 0.0f ? prm->scale / prm->softcap : 0.0f;
+    if (!std::isfinite(cap_in)) return EKV_ERR_INVALID_ARG;  // (0 * inf for a score of 0)
     if (((uintptr_t)q | ((uintptr_t)prm->ancestors << 1)) & 15) return EKV_ERR_INVALID_ARG;
     if (c.head_dim != 48 && c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return EKV_ERR_UNSUPPORTED;
-    const float log2e = 1.4426950408889634f;
     a = ekv::TreeArgs{};
     a.pool = p->view;
     a.layer = prm->layer;
@@ -676,10 +682,10 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
     a.q_heads = prm->q_heads;
     a.group = prm->q_heads / c.kv_heads;
     a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);  // (not used at 1, where it is 2^32)
-    if ((int64_t)EKV_MAX_DRAFT * a.group * a.group >= 1ll << 32) return EKV_ERR_UNSUPPORTED;
+    if (group_too_large(a.group)) return EKV_ERR_UNSUPPORTED;
     a.scale_log2 = prm->scale * log2e;
     a.cap_log2 = prm->softcap * log2e;
-    a.cap_in = prm->softcap > 0.0f ? prm->scale / prm->softcap : 0.0f;
+    a.cap_in = cap_in;
     a.seq_ids = prm->seq_ids;
     a.prefix_len = prm->prefix_len;
     a.n_nodes = prm->n_nodes;
@@ -693,7 +699,7 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
 
 size_t ekv_tree_attention_workspace_size(const ekv_pool *p, const ekv_tree_params *prm) {
     if (!p || !prm || prm->n_batch <= 0 || prm->n_draft <= 0 || prm->n_draft > EKV_MAX_DRAFT || prm->q_heads <= 0 ||
-        prm->q_heads % p->cfg.kv_heads)
+        prm->q_heads % p->cfg.kv_heads || group_too_large(prm->q_heads / p->cfg.kv_heads))
         return 0;
     return ekv::tree_workspace(p->view, prm->n_batch, prm->n_draft, prm->q_heads, prm->softcap > 0.0f, p->sms);
 }

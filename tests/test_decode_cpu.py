@@ -256,3 +256,16 @@ def test_evict_keep_near_the_end_of_32_bits():
     for keep, code in ((2 ** 31 - 1, ekv.ERR_RANGE), (2 ** 31 - 1024, ekv.ERR_RANGE), (2 ** 30, ekv.ERR_UNSUPPORTED)):
         e = ekv.EvictParams(0, 2, 3, keep, 4, 8, P, None, P, None, 100, P, None, None, 0)
         assert L.ekv_evict_by_weight(p.h, C.byref(e), None) == code
+
+
+def test_tree_scales_and_heads_whose_products_overflow():
+    """A scale, a cap or their quotient that is infinite in f32 (a score of 0 would be NaN), and head counts beyond 32 bits."""
+    p = pool()
+    for kw in (dict(scale=3e38), dict(softcap=3e38), dict(softcap=1e-45), dict(scale=1e20, softcap=1e-20)):
+        assert tree(p, tree_params(**kw)) == ekv.ERR_INVALID_ARG, kw
+    for kw in (dict(scale=2e38), dict(softcap=1e-30), dict(softcap=2e38)):
+        assert tree(p, tree_params(**kw)) == ekv.ERR_UNSUPPORTED, kw
+    huge = tree_params(q_heads=2 ** 31 - 2, n_draft=64)
+    assert tree(p, huge) == ekv.ERR_UNSUPPORTED
+    assert L.ekv_tree_attention_workspace_size(p.h, C.byref(huge)) == 0
+    assert L.ekv_tree_attention_workspace_size(p.h, C.byref(tree_params(q_heads=2 * 8191))) > 0
