@@ -340,7 +340,9 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
     const int D = p.head_dim;
     a.per = !wide || a.interleaved ? D / 8 : a.rotary / 16 + (D - a.rotary) / 8;
     a.per_item = !wide && q == q_out ? D - a.rotary / 2 : 0;
-    if ((int64_t)kMaxRows * std::max(q_heads, p.kv_heads) * D * std::max({a.per, a.per_item, q_heads, p.kv_heads, D / 8}) >= 1ll << 32)
+    // (as two comparisons: the whole product passes 64 bits from 2^28 heads on)
+    const int64_t items = (int64_t)kMaxRows * std::max(q_heads, p.kv_heads) * D;
+    if (items >= 1ll << 32 || items * std::max({a.per, a.per_item, q_heads, p.kv_heads, D / 8}) >= 1ll << 32)
         return EKV_ERR_UNSUPPORTED;
     a.div_per = SmallDiv((uint32_t)a.per);
     a.div_item = SmallDiv((uint32_t)std::max(1, a.per_item));

@@ -188,3 +188,14 @@ def test_tree_calls_that_start_under_one_another():
     torch.cuda.synchronize()
     for c, prm, q, kd, vd, out, lse, room, want, want_lse in calls:
         assert c.pool.status() == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("heads", [2 ** 13, 2 ** 29, 2 ** 30, 2 ** 31 - 1])
+def test_rope_refuses_heads_beyond_its_divisions(heads):
+    """Nothing is launched for head counts whose items are beyond the kernel's 32-bit divisions, also where the check's own
+    product would pass 64 bits."""
+    c = dc.Cache([4], 1, 16, seed=1)
+    rope, one, q = ekv.Rope(rotary_dims=16), dc.ints([0]), torch.zeros(64, dtype=torch.bfloat16, device="cuda")
+    code = ekv.lib.ekv_rope_append(c.pool.h, rope.h, 0, 1, None, None, one.data_ptr(), one.data_ptr(), 1, one.data_ptr(), heads,
+                                   q.data_ptr(), 0, q.data_ptr(), None, None, 0, None)
+    assert code == ekv.ERR_UNSUPPORTED
