@@ -168,11 +168,6 @@ __device__ __forceinline__ float scale_of(const uint32_t (&s)[N], int g) {
     const __half2 h = *(const __half2 *)&s[g >> 1];
     return g & 1 ? __high2float(h) : __low2float(h);
 }
-__device__ __forceinline__ float lds_f16(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return f16_bits_to_f32(v);
-}
 // 16 bytes to another CTA's shared memory (address from mapa_shared).
 __device__ __forceinline__ void stc128(uint32_t addr, float4 v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
