@@ -12,6 +12,31 @@ from test_gpu_decode import STORES, check_evict, check_tree, close_turned, rand,
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("store,dim", STORES)
+@pytest.mark.parametrize("T,hq", [(1, 4), (3, 5), (6, 4), (45, 4)])
+@pytest.mark.parametrize("cap", [0.0, 9.0])
+def test_tree_rows_without_a_number_stay_so(store, dim, T, hq, cap):
+    """A row whose every score is NaN (its query is, or the one key that it sees) gives NaN, as the formula does, not the 0
+    and -inf of a row that sees nothing; short and long caches, with the cache cut into parts and without."""
+    lens = [0, 0, 40, 900, 5000]
+    c = dc.Cache(lens, 1, dim, store=store, seed=dim)
+    B = len(lens)
+    q, kd, vd = rand(61, B, T, hq, dim), rand(62, B, T, 1, dim), rand(63, B, T, 1, dim)
+    q[0, 0, 1, 3] = float("nan")
+    kd[1, T - 1, 0, 5] = float("nan")
+    q[2:, T - 1, hq - 1, 7] = float("nan")
+    q[4, T // 2] = float("nan")
+    up = [[1 << t for t in range(T)] for _ in range(B)]
+    for ws in (True, False):
+        for nodes in ([T] * B, [T, T, 0, max(1, T - 1), T]):
+            out, lse, _ = run_tree(c, q, kd, vd, up=dc.words(up), nodes=nodes, cap=cap, workspace=ws)
+            check_tree(c, q, kd, vd, out, lse, up=up, nodes=nodes, cap=cap)
+            for b in range(B):
+                n = torch.isnan(out[b]).any(-1)
+                assert torch.equal(n, torch.isnan(lse[b])) and n[nodes[b]:].sum() == 0
+            assert torch.isnan(out[0, 0, 1]).all() and torch.isnan(out[1, T - 1]).all() and torch.isnan(out[4, T // 2]).all()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("T,hq", [(1, 1), (1, 8), (2, 8), (3, 6), (9, 8), (32, 8)])
 @pytest.mark.parametrize("cap", [0.0, 6.0])
