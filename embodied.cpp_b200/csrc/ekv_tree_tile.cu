@@ -463,8 +463,10 @@ __global__ void __launch_bounds__(TCfg<D, RT, Q8>::THREADS, TCfg<D, RT, Q8>::CTA
                     // the row's maximum of the tile
                     uint32_t sa[32], sb[32];
                     tmem_load32x2(s_col, s_col + 32, sa, sb);
+                    bool sees = true;  // (a cap makes a score of an infinite product, which is no mask)
                     if (!full) {
                         const uint32_t bits = chunk_bits(word, 0, valid), bits1 = chunk_bits(word, 32, valid);
+                        sees = (bits | bits1) != 0;
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
                             if (!((bits >> k) & 1u)) sa[k] = 0xff800000u;
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(TCfg<D, RT, Q8>::THREADS, TCfg<D, RT, Q8>::CTA
                         top1 = max3(top1, __uint_as_float(sb[k]), __uint_as_float(sb[k + 1]));
                     }
                     top = fmaxf(top, top1);
-                    const float mt = top == -INFINITY ? -INFINITY : CAP ? score.capped(top) : top * a.scale_log2;
+                    const float mt = (CAP ? !sees : top == -INFINITY) ? -INFINITY : CAP ? score.capped(top) : top * a.scale_log2;
                     // m moves when the tile is more than 2^8 above it; O follows once P V(j - 1) has landed
                     const bool up = mt > m + 8.0f;
                     if (__any_sync(0xffffffffu, up)) {

@@ -224,3 +224,28 @@ def test_rope_refuses_heads_beyond_its_divisions(heads):
     code = ekv.lib.ekv_rope_append(c.pool.h, rope.h, 0, 1, None, None, one.data_ptr(), one.data_ptr(), 1, one.data_ptr(), heads,
                                    q.data_ptr(), 0, q.data_ptr(), None, None, 0, None)
     assert code == ekv.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("T,hq", [(1, 4), (20, 4), (40, 4)])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_tree_capped_scores_of_infinity(dim, T, hq, sign):
+    """cap * tanh takes an infinite product to -cap or cap, a score like any other: where every visible key has it the output
+    is the values' mean and lse is that score plus the logarithm of their number."""
+    lens = [70, 1, 640, 5000]
+    c = dc.Cache(lens, 1, dim, seed=7)
+    q, kd, vd = rand(171, 4, T, hq, dim), rand(172, 4, T, 1, dim), rand(173, 4, T, 1, dim)
+    q[..., 3] = sign
+    k = rand(174, max(lens), 1, dim)
+    k[..., 3] = kd[..., 3] = float("inf")
+    v = rand(175, max(lens), 1, dim)
+    for b, n in enumerate(lens):
+        c.pool.append(0, dc.ints([c.seqs[b]]), dc.ints([0]), dc.ints([n]), dc.ints([0]), n, k, v)
+    up = [[1 << t if t % 2 else 0 for t in range(T)] for _ in range(4)]
+    for ws in (True, False):
+        out, lse, _ = run_tree(c, q, kd, vd, up=dc.words(up), cap=5.0, workspace=ws)
+        check_tree(c, q, kd, vd, out, lse, up=up, cap=5.0)
+        for b, n in enumerate(lens):
+            for t in range(T):
+                want = sign * 5.0 + math.log(n + t % 2)
+                assert ((lse[b, t] - want).abs() < 1e-4).all()
