@@ -659,7 +659,7 @@ int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_
 static bool group_too_large(int group) { return group >= 8192; }
 static_assert(EKV_MAX_DRAFT * 8191ll * 8191 < 1ll << 32, "rows times query heads");
 
-// Checks what attention and key weights share, and the longest live sequence (which only sizes grids).
+// Checks what attention and key weights share, and the longest prefix to expect (which only sizes grids).
 static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const void *q, ekv::TreeArgs &a, int &max_len) {
     if (!p || !prm || !q || !prm->seq_ids) return EKV_ERR_INVALID_ARG;
     const ekv_pool_config &c = p->cfg;
@@ -667,6 +667,7 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
         prm->q_heads % c.kv_heads)
         return EKV_ERR_INVALID_ARG;
     if (prm->n_draft > EKV_MAX_DRAFT) return EKV_ERR_RANGE;
+    if (prm->max_prefix < 0) return EKV_ERR_INVALID_ARG;
     const float log2e = 1.4426950408889634f;
     if (!(prm->scale > 0.0f) || !std::isfinite(prm->scale * log2e) || !(prm->softcap >= 0.0f) || !std::isfinite(prm->softcap * log2e))
         return EKV_ERR_INVALID_ARG;
@@ -694,6 +695,7 @@ static int fill_tree_args(const ekv_pool *p, const ekv_tree_params *prm, const v
     max_len = 0;
     for (const ekv_pool::Seq &s : p->seqs)
         if (s.live) max_len = std::max(max_len, s.n_tokens);
+    if (prm->max_prefix > 0) max_len = std::min(max_len, prm->max_prefix);
     return EKV_OK;
 }
 

@@ -1003,7 +1003,9 @@ int launch_tree_attention(TreeArgs a, int max_len, void *ws, size_t ws_bytes, in
     // Three ways to share the work: a CTA per unit (one or two tiles, or many units without a workspace); a cluster of
     // CTAs per unit; CTAs with equal ranges of all tiles and a second kernel that joins the parts. The last is the most
     // even one, but its second launch costs about 3.4 us, the time of `worth` tiles: one token over 816 keys takes 9.3 us
-    // with it and 8.4 as a cluster of eight, 64 requests of an 8-bit cache 22 and 20.
+    // with it and 8.4 as a cluster of eight, 64 requests of an 8-bit cache 22 and 20. max_len stands for the call's lengths,
+    // which are on the device: where an idle sequence of 60000 tokens makes it too long the split is taken for the clusters'
+    // calls as well (that token 9.9 us, the 64 requests 23.5, in bf16 18.8 for 13.5); the caller's max_prefix puts it right.
     const bool can_split = ws != nullptr && ws_bytes >= w.total && units * most_tiles < INT32_MAX;
     const int64_t even = (units * unit_tiles + full - 1) / full;  // tiles per CTA when split
     const int64_t worth = a.pool.dtype == EKV_DTYPE_Q8_0 ? 1 : 3;

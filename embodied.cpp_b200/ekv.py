@@ -95,7 +95,7 @@ class RopeConfig(C.Structure):
 
 class TreeParams(C.Structure):
     _fields_ = [("layer", C.c_int32), ("n_batch", C.c_int32), ("n_draft", C.c_int32), ("q_heads", C.c_int32),
-                ("scale", C.c_float), ("softcap", C.c_float), ("out_dtype", C.c_int32), ("reserved", C.c_int32),
+                ("scale", C.c_float), ("softcap", C.c_float), ("out_dtype", C.c_int32), ("max_prefix", C.c_int32),
                 ("seq_ids", C.c_void_p), ("prefix_len", C.c_void_p), ("n_nodes", C.c_void_p), ("ancestors", C.c_void_p)]
 
 
@@ -429,9 +429,11 @@ class Pool:
             check(code, "ekv_rope_append")
 
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
-                    prefix_len=None, n_nodes=None, ancestors=None) -> TreeParams:
+                    prefix_len=None, n_nodes=None, ancestors=None, max_prefix=0) -> TreeParams:
+        """What ekv_tree_attention and ekv_key_weights share. max_prefix, the longest cached prefix of the call, is worth
+        giving where the pool holds longer sequences that are not of the call."""
         n = seq_ids.numel()
-        p = TreeParams(layer, n, n_draft, q_heads, scale, softcap, out_dtype, 0, _index(seq_ids, n, "seq_ids"),
+        p = TreeParams(layer, n, n_draft, q_heads, scale, softcap, out_dtype, max_prefix, _index(seq_ids, n, "seq_ids"),
                        _index(prefix_len, n, "prefix_len"), _index(n_nodes, n, "n_nodes"),
                        _index(ancestors, n * n_draft, "ancestors", 64))
         p._keep = (seq_ids, prefix_len, n_nodes, ancestors)

@@ -349,7 +349,8 @@ typedef struct ekv_tree_params {
     float scale;
     float softcap;          /* > 0: scores are softcap * tanh(scale * q.k / softcap); 0: scale * q.k    */
     int32_t out_dtype;      /* EKV_DTYPE_BF16 or EKV_DTYPE_F32                                        */
-    int32_t reserved;
+    int32_t max_prefix;     /* longest cached prefix of the call where the caller knows it; 0: the longest live sequence of
+                               the pool stands for it. It picks how the work is shared; no result hangs on it     */
     /* device arrays; NULL selects the default                                                        */
     const int32_t *seq_ids;     /* [n_batch], required                                                */
     const int32_t *prefix_len;  /* [n_batch] cached keys used; default: the sequence length            */

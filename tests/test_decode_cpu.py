@@ -269,3 +269,9 @@ def test_tree_scales_and_heads_whose_products_overflow():
     assert tree(p, huge) == ekv.ERR_UNSUPPORTED
     assert L.ekv_tree_attention_workspace_size(p.h, C.byref(huge)) == 0
     assert L.ekv_tree_attention_workspace_size(p.h, C.byref(tree_params(q_heads=2 * 8191))) > 0
+
+
+def test_tree_max_prefix_refusals():
+    p = pool()
+    assert tree(p, tree_params(max_prefix=-1)) == ekv.ERR_INVALID_ARG
+    assert tree(p, tree_params(max_prefix=1)) == tree(p, tree_params(max_prefix=2 ** 31 - 1)) == ekv.ERR_UNSUPPORTED

@@ -73,6 +73,31 @@ def test_tree_workspaces_of_every_size(store, dim, T, hq):
         check_tree(c, q, kd, vd, out, lse)
 
 
+@pytest.mark.parametrize("store,dim,T,hq", [("bf16", 128, 1, 8), ("bf16", 64, 20, 4), ("q8_0", 256, 3, 8), ("q8_0", 128, 20, 4)])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_tree_prefixes_beyond_or_below_what_was_said(store, dim, T, hq, workspace):
+    """max_prefix picks how the work is shared and nothing else: far too small, right and far too large, beside an idle
+    sequence that is longer than all."""
+    c = dc.Cache([2100, 40, 0, 700], 1, dim, store=store, block=64, seed=2, spare=160, width=160)
+    c.pool.seq_resize(c.pool.seq_create(), 10000)
+    c.pool.sync()
+    q, kd, vd = rand(181, 4, T, hq, dim), rand(182, 4, T, 1, dim), rand(183, 4, T, 1, dim)
+    for said in (0, 1, 100, 700, 2100, 2 ** 31 - 1):
+        prm = c.pool.tree_params(layer=0, seq_ids=c.seq_ids, n_draft=T, q_heads=hq, scale=1 / math.sqrt(dim), max_prefix=said)
+        room = torch.empty(c.pool.tree_attention_workspace_size(prm), dtype=torch.uint8, device="cuda") if workspace else None
+        out, lse = torch.full_like(q, 9.0), torch.full((4, T, hq), 9.0, device="cuda")
+        c.pool.tree_attention(prm, q, kd, vd, out, lse, room)
+        w = torch.zeros(4, 1, 2100, device="cuda")
+        c.pool.key_weights(prm, q, lse, w, 0.0)
+        torch.cuda.synchronize()
+        assert c.pool.status() == 0
+        check_tree(c, q, kd, vd, out, lse)
+        for b, n in enumerate(c.lens):
+            s, _ = dc.tree_scores(q[b].double(), c.rows(b)[0].double(), 1 / math.sqrt(dim), 0.0)
+            want = torch.exp(s - lse[b].double()[..., None]).sum((0, 1))
+            assert ((w[b, 0, :n].double() - want).abs() <= 1e-4 * want).all() and (w[b, 0, n:] == 0).all()
+
+
 def test_two_streams_with_workspaces_of_their_own():
     """Calls of two pools, and of one pool, side by side on two streams: the bits of the calls alone."""
     calls = []
