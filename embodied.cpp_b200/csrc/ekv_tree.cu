@@ -4,10 +4,13 @@
 // drafted keys that t's ancestor word names:
 //   s_k = scale * q.k  (or cap * tanh(scale * q.k / cap)),  out = sum exp(s_k - m) v_k / sum exp(s_k - m),
 //   lse = m + ln sum exp(s_k - m).
-// Probabilities are rounded to bf16 for the products with V, so the output is divided by the sum of the rounded
-// ones (a row with one heavy key would carry that key's rounding otherwise); lse takes the sum before rounding.
-// Q8_0 caches take p times the value's scale, a different number per 32 columns, as two bf16 parts and divide by the plain
-// sum. (As one part, one heavy key's 32 columns were all off by up to 2^-9 whatever the output's type.)
+// For bf16 outputs over bf16 pages probabilities are rounded to bf16 for the products with V, and the output is divided by
+// the sum of the rounded ones (a row with one heavy key would carry that key's rounding otherwise); lse takes the sum before
+// rounding. For f32 outputs the probabilities, and over 8-bit pages p times the value's scale, a different number per 32
+// columns, are two bf16 parts each, and the output is divided by the plain sum: off by 2^-16 of sum p |v| instead of 2^-8.
+// The second parts cost 0 to 8% of an f32 call: 16 requests of 16 k keys 163.0 -> 163.2 us, 64 requests of 816 keys of 256
+// columns 13.5 -> 14.6. 8-bit pages take them for bf16 outputs too: as one part, a heavy key's 32 columns were all off by up to
+// 2^-8.
 // One pass over the keys: a warp keeps the reference maximum m, the sum and the output of its rows in
 // registers (the running softmax of Milakov and Gimelshein 2018, with the output as in flash attention,
 // Dao et al. 2022). m moves only when a score is more than 2^8 above it; every quotient is exact about that.
@@ -90,10 +93,12 @@ __device__ __forceinline__ int o_col(int ds, int kq, int i) {
     return Q8 ? 32 * (ds >> 1) + 4 * kq + 2 * (ds & 1) + (i >> 1) : 16 * ds + kq + 8 * (i >> 1);
 }
 
-template <int D, bool Q8, int NR, int WR, int WK>
+// FINE (f32 outputs): probabilities as two bf16 parts for the products with V, over 8-bit pages always.
+template <int D, bool Q8, bool FINE, int NR, int WR, int WK>
 __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR, WR, WK>::CTAS)
     tree_rows_kernel(const TreeArgs a) {
     using C = Cfg<D, Q8, NR, WR, WK>;
+    static_assert(FINE || !Q8, "8-bit pages have one form");
     constexpr int NST = C::NST, KS = D / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -469,12 +474,19 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                         __syncwarp();
                     }
                     if constexpr (!Q8) {
-                        uint32_t p[NR][2];
+                        uint32_t p[NR][2], pl[FINE ? NR : 1][2];  // P^T, and what its rounding left
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
                             const uint32_t w0 = pack_bf16(s[n][0], s[n][1]), w1 = pack_bf16(s[n][2], s[n][3]);
-                            rsum[n][0] += __uint_as_float(w0 << 16) + __uint_as_float(w1 << 16);
-                            rsum[n][1] += __uint_as_float(w0 & 0xffff0000u) + __uint_as_float(w1 & 0xffff0000u);
+                            const float h[4] = {__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
+                                                __uint_as_float(w1 & 0xffff0000u)};
+                            if constexpr (FINE) {
+                                pl[n][0] = movmatrix_trans(pack_bf16(s[n][0] - h[0], s[n][1] - h[1]));
+                                pl[n][1] = movmatrix_trans(pack_bf16(s[n][2] - h[2], s[n][3] - h[3]));
+                            } else {
+                                rsum[n][0] += h[0] + h[2];
+                                rsum[n][1] += h[1] + h[3];
+                            }
                             p[n][0] = movmatrix_trans(w0);
                             p[n][1] = movmatrix_trans(w1);
                         }
@@ -484,6 +496,10 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                             load_v_cols<D>(sv, key0, ds, lane, vf);
 #pragma unroll
                             for (int n = 0; n < NR; ++n) mma_bf16(o[n][ds], vf, p[n][0], p[n][1]);
+                            if constexpr (FINE) {
+#pragma unroll
+                                for (int n = 0; n < NR; ++n) mma_bf16(o[n][ds], vf, pl[n][0], pl[n][1]);
+                            }
                         }
                     } else {
                         constexpr int G = D / 32;
@@ -534,7 +550,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
                                 for (int k = 0; k < 4; ++k) f[k] = scale_of(sc[k], gr);
                             }
                             // The values' scales ride on the probabilities, as two bf16 parts: one part would put a whole
-                            // group of 32 columns off by the same 2^-9. An infinite scale has no remainder (inf - inf), and
+                            // group of 32 columns off by the same 2^-8. An infinite scale has no remainder (inf - inf), and
                             // any finite number serves for it. The second part's products cost 3 to 10% of a call: 64 requests
                             // of 816 keys, 256 columns, 8 rows 18.9 -> 19.8 us, 512 rows 557 -> 612.
 #pragma unroll
@@ -595,7 +611,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8, NR, WR, WK>::THREADS, Cfg<D, Q8, NR
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float l = sum[n][e], lr = Q8 ? sum[n][e] : rsum[n][e];
+                    float l = sum[n][e], lr = FINE ? sum[n][e] : rsum[n][e];
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) {
                         l += __shfl_xor_sync(0xffffffffu, l, x);
@@ -932,24 +948,24 @@ WsLayout ws_layout(const PoolView &p, int n_batch, int rows, bool capped, int rt
     return w;
 }
 
-template <int D, bool Q8, int NR, int WR, int WK>
+template <int D, bool Q8, bool FINE, int NR, int WR, int WK>
 int launch_rows(const TreeArgs &a, int grid, cudaStream_t s) {
     using C = Cfg<D, Q8, NR, WR, WK>;
     static std::atomic<uint64_t> smem_done{0};
-    if (const int rc = allow_smem(tree_rows_kernel<D, Q8, NR, WR, WK>, C::SMEM, smem_done)) return rc;
-    return launch_clusters_after(a.cluster, tree_rows_kernel<D, Q8, NR, WR, WK>, grid, C::THREADS, C::SMEM, s, a);
+    if (const int rc = allow_smem(tree_rows_kernel<D, Q8, FINE, NR, WR, WK>, C::SMEM, smem_done)) return rc;
+    return launch_clusters_after(a.cluster, tree_rows_kernel<D, Q8, FINE, NR, WR, WK>, grid, C::THREADS, C::SMEM, s, a);
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool FINE>
 int launch_shape(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     switch (sh) {
-        case Shape::R8: return launch_rows<D, Q8, 1, 1, 4>(a, grid, s);
-        case Shape::R16: return launch_rows<D, Q8, 2, 1, 4>(a, grid, s);
+        case Shape::R8: return launch_rows<D, Q8, FINE, 1, 1, 4>(a, grid, s);
+        case Shape::R16: return launch_rows<D, Q8, FINE, 2, 1, 4>(a, grid, s);
         case Shape::R32:
-            if constexpr (D <= 128) return launch_rows<D, Q8, 4, 1, 4>(a, grid, s);
+            if constexpr (D <= 128) return launch_rows<D, Q8, FINE, 4, 1, 4>(a, grid, s);
             return EKV_ERR_UNSUPPORTED;
         default:  // (bf16 at head_dim 128: 33 rows and more are the tile kernel's)
-            if constexpr (Q8 || D != 128) return launch_rows<D, Q8, 2, 4, 1>(a, grid, s);
+            if constexpr (Q8 || D != 128) return launch_rows<D, Q8, FINE, 2, 4, 1>(a, grid, s);
             return EKV_ERR_UNSUPPORTED;
     }
 }
@@ -960,10 +976,10 @@ int launch_dim(const TreeArgs &a, Shape sh, int grid, cudaStream_t s) {
     if (sh == Shape::Tile) {
         rc = launch_tree_tile(a, grid, s);
     } else if (a.pool.dtype == EKV_DTYPE_Q8_0) {
-        if constexpr (D % 32 == 0) rc = launch_shape<D, true>(a, sh, grid, s);
+        if constexpr (D % 32 == 0) rc = launch_shape<D, true, true>(a, sh, grid, s);
         else rc = EKV_ERR_UNSUPPORTED;
     } else {
-        rc = launch_shape<D, false>(a, sh, grid, s);
+        rc = a.out_dtype == EKV_DTYPE_F32 ? launch_shape<D, false, true>(a, sh, grid, s) : launch_shape<D, false, false>(a, sh, grid, s);
     }
     if (rc || !a.split) return rc;
     const int tr = tile_rows(sh, a.pool, a.n_draft * a.group, a.cap_log2 != 0.0f);

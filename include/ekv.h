@@ -348,7 +348,8 @@ typedef struct ekv_tree_params {
     int32_t q_heads;        /* a multiple of the pool's kv_heads                                      */
     float scale;
     float softcap;          /* > 0: scores are softcap * tanh(scale * q.k / softcap); 0: scale * q.k    */
-    int32_t out_dtype;      /* EKV_DTYPE_BF16 or EKV_DTYPE_F32                                        */
+    int32_t out_dtype;      /* EKV_DTYPE_BF16, or EKV_DTYPE_F32: probabilities then keep 16 bits for the products
+                               with V (8 for bf16 outputs)                                            */
     int32_t max_prefix;     /* longest cached prefix of the call where the caller knows it; 0: the longest live sequence of
                                the pool stands for it. It picks how the work is shared; no result hangs on it     */
     /* device arrays; NULL selects the default                                                        */

@@ -42,8 +42,8 @@ def test_tree_rows_without_a_number_stay_so(store, dim, T, hq, cap):
 @pytest.mark.parametrize("cap", [0.0, 6.0])
 def test_tree_weighted_mean_of_equal_values(dim, T, hq, cap):
     """Where every key holds the same 8-bit row, the output is that row whatever the probabilities. Tolerance: a
-    probability as two bf16 parts is off by 2^-17, its product with the value's scale (or the value as two parts) by another
-    2^-17, the sums of up to 200 terms by 200 * 2^-24; the rest of 2^-14 is room."""
+    probability as two bf16 parts is off by 2^-16, its product with the value's scale (or the value as two parts) by another
+    2^-16, the sums of up to 200 terms by 200 * 2^-24; the rest of 2^-14 is room."""
     lens = [1, 2, 17, 200]
     c = dc.Cache(lens, 1, dim, store="q8_0", seed=3)
     row = rand(71, 1, 1, dim)
@@ -249,3 +249,25 @@ def test_tree_capped_scores_of_infinity(dim, T, hq, sign):
             for t in range(T):
                 want = sign * 5.0 + math.log(n + t % 2)
                 assert ((lse[b, t] - want).abs() < 1e-4).all()
+
+
+@pytest.mark.parametrize("store,dim", STORES)
+@pytest.mark.parametrize("T,hq", [(1, 1), (1, 8), (3, 4), (5, 4), (9, 4), (40, 4)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_tree_f32_outputs(store, dim, T, hq, cap):
+    """An f32 output is more than a bf16 one with zeros behind it. Tolerance, of A = sum p |v|: a probability as two bf16 parts
+    is off by 2^-16, over 8-bit pages its product with the value's scale, or the value as two parts, by another 2^-16 (2^-14
+    leaves twice that), sums of n terms by n 2^-24, and an error e of a score moves numerator and denominator by e: head_dim *
+    2^-24 * sum |q k|, and 2e-5 for cap and exponential."""
+    lens = [1, 2, 5, 300, 2500]
+    c = dc.Cache(lens, 1, dim, store=store, block=32, seed=dim)
+    q, kd, vd = rand(191, 5, T, hq, dim), rand(192, 5, T, 1, dim), rand(193, 5, T, 1, dim)
+    up = [dc.tree_words(T, b) for b in range(5)]
+    for ws in (True, False):
+        out, _, _ = run_tree(c, q, kd, vd, up=dc.words(up), cap=cap, dtype=torch.float32, workspace=ws)
+        for b, n in enumerate(lens):
+            k, v = c.rows(b)
+            want, _, size, most = dc.tree_attention(q[b], k, v, kd[b], vd[b], up[b], T, 1 / math.sqrt(dim), cap)
+            e = dim * 2 ** -24 * most + 2e-5
+            off = (out[b].double() - want).abs() - size * (2 ** -14 + (n + T) * 2 ** -24 + 2 * e[..., None])
+            assert not (off > 0).any(), (b, ((out[b].double() - want).abs() / size).max().item())
