@@ -51,9 +51,11 @@ struct RopeArgs {
     uint16_t *q_out;
 };
 
-__device__ __forceinline__ uint32_t rot_pair(uint32_t lo_hi, float2 cs) {  // an interleaved pair in one word
+// An interleaved pair in one word. Which product is rounded and which is part of the sum is said, so that every form gives
+// the same bits: left to the compiler it differed from form to form, and two of 10^7 values with it.
+__device__ __forceinline__ uint32_t rot_pair(uint32_t lo_hi, float2 cs) {
     const float x = bf16_bits_to_f32((uint16_t)lo_hi), y = bf16_bits_to_f32((uint16_t)(lo_hi >> 16));
-    const uint32_t a = f32_to_bf16_bits(x * cs.x - y * cs.y), b = f32_to_bf16_bits(x * cs.y + y * cs.x);
+    const uint32_t a = f32_to_bf16_bits(__fmaf_rn(x, cs.x, -__fmul_rn(y, cs.y))), b = f32_to_bf16_bits(__fmaf_rn(x, cs.y, __fmul_rn(y, cs.x)));
     return a | b << 16;
 }
 
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
     }
     for (int i = threadIdx.x; i < nr * half; i += kThreads) {
         const int r = i / half, j = i - r * half;
-        const double t = (double)a.positions[row0 + r] * a.turns[j];
+        const double t = __dmul_rn((double)a.positions[row0 + r], a.turns[j]);
         float sn, cn;
         sincospif(2.0f * (float)(t - rint(t)), &sn, &cn);
         s_cs[i] = make_float2(cn * a.magnitude, sn * a.magnitude);

@@ -271,3 +271,34 @@ def test_tree_f32_outputs(store, dim, T, hq, cap):
             e = dim * 2 ** -24 * most + 2e-5
             off = (out[b].double() - want).abs() - size * (2 ** -14 + (n + T) * 2 ** -24 + 2 * e[..., None])
             assert not (off > 0).any(), (b, ((out[b].double() - want).abs() / size).max().item())
+
+
+@pytest.mark.parametrize("store", ["bf16", "q8_0"])
+@pytest.mark.parametrize("rotary", [64, 34, 18])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_has_one_rounding(store, rotary, interleaved):
+    """A turned value has the same bits whichever form of the kernel turns it: out of place, in place, and on the way into the
+    pages (40 million values: of those whose last bit of f32 hangs on the order of the products, some fall on a bf16 tie)."""
+    n, heads, dim = 4000, 4, 64
+    pools = []
+    for _ in range(2):
+        p = ekv.Pool(dtype=ekv.DTYPE_Q8_0 if store == "q8_0" else ekv.DTYPE_BF16, block_tokens=16, n_blocks=250, kv_heads=heads, head_dim=dim,
+                     max_seqs=1, max_blocks_per_seq=250)
+        p.seq_resize(p.seq_create(), n)
+        p.sync()
+        pools.append(p)
+    rope, zero, count = ekv.Rope(rotary_dims=rotary, interleaved=interleaved), dc.ints([0]), dc.ints([n])
+    size = n * heads * (dim * 2 if store == "bf16" else dim // 32 * 34)
+    g = torch.Generator("cuda").manual_seed(rotary)
+    for _ in range(40):
+        k = torch.randn(n, heads, dim, device="cuda", generator=g).bfloat16()
+        pos = torch.randint(0, 1 << 20, (n,), device="cuda", dtype=torch.int32, generator=g)
+        out, there = torch.empty_like(k), k.clone()
+        pools[0].rope_append(rope, 0, zero, zero, count, zero, n, pos, q=k, q_out=out, k=k, v=k)
+        pools[0].rope_append(rope, 0, None, None, count, zero, n, pos, q=there, q_out=there)
+        pools[1].append(0, zero, zero, count, zero, n, out, k)
+        assert torch.equal(out.view(torch.int16), there.view(torch.int16))
+        got, want = ([torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(2)] for _ in range(2))
+        pools[0].gather(0, 0, 0, n, ekv.GATHER_NATIVE, *got)
+        pools[1].gather(0, 0, 0, n, ekv.GATHER_NATIVE, *want)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
