@@ -4,9 +4,10 @@
 // turns, pos * (f_i / 2 pi) in 64 bits, reduced to its fraction, and only then rounded to 32: at position
 // 100000 a 32-bit product would be off by 0.004 radians. One CTA computes the sines of its rows once and uses
 // them for every head; the rest is a stream of 16-byte loads and stores.
-// Bound: DRAM. 32 k rows of 48 heads of 128 columns (700 MB read and written) take 118 us, 5.9 TB/s, 91% of the measured
-// copy rate; 3 k rows of 10 heads of 256 (31 MB) 9.2 us, half of it the dependent loads before the stream (rows of the
-// request, their positions, the sines); one row 3.6 us.
+// Bound: DRAM. On the device 32 k rows of 48 heads of 128 columns (700 MB read and written) take 118 us, 5.9 TB/s, 91% of the
+// measured copy rate (125 us, 85%, as calls with inputs that change); 3 k rows of 10 heads of 256 (31 MB) 9.1 us, half of it
+// the dependent loads before the stream (rows of the request, their positions, the sines); one row 3.7 us. 8-bit pages are
+// written a 32-column group a thread, read column by column: 233 us for the 32 k rows' like, whose bytes take 113.
 #include <algorithm>
 #include <cmath>
 #include <new>

@@ -5,9 +5,9 @@
 // Keys are the rows of the products (S^T = K Q^T), so that a lane holds two keys and sums over query rows in its own
 // registers; with query rows as rows, twelve shuffles per tile made the consumer the bound (97 us for 16 x 16k keys).
 // Bound and figures: the bytes of K up to about 16 rows of a KV head: 16 requests of 16 k keys, 8 KV heads of 128 columns
-// in bf16 (503 MB), 4 rows each, take 87 us, 5.8 TB/s, 89% of the measured copy rate. With more rows the matrix
+// in bf16 (503 MB), 4 rows each, take 85 us on the device, 5.9 TB/s, 90% of the measured copy rate. With more rows the matrix
 // instructions and one exponential per row and key: 256 rows over 8 requests of 4096 such keys 77 us (a tcgen05 form
-// would have 15 of exponentials and 11 of products). 132 rows over 4 requests of 4 k Q8_0 keys: 15.6 us.
+// would have 15 of exponentials and 11 of products). 132 rows over 4 requests of 4 k Q8_0 keys: 15.2 us.
 #include <algorithm>
 #include <type_traits>
 
