@@ -184,17 +184,21 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const Evic
         const int i = tid + j * kSelThreads;
         ages[j] = pos && i < ahead ? (uint32_t)__ldg(pos + i) : (uint32_t)i;
     }
-    int n = 0;
+    int n = -1;
     if (seq < 0 || seq >= a.pool.max_seqs) {
         if (tid == 0) report_error(a.pool.status, DEV_ERR_BAD_SEQ, b, seq, 10);
     } else {
         n = a.pool.seq_lens[seq];
         if (n > a.weight_stride || n > a.max_len) {
             if (tid == 0) report_error(a.pool.status, DEV_ERR_BAD_POS, seq, n, 10);
-            n = 0;
+            n = -1;
         }
     }
     int32_t *kept = a.kept + (int64_t)lbh * a.keep;
+    if (n < 0) {  // reported: no row moves, and weights and positions, which may be the call's own inputs, stay
+        for (int i = tid; i < a.keep; i += kSelThreads) kept[i] = -1;
+        return;
+    }
     float *w_out = a.weights_out ? a.weights_out + (int64_t)lbh * a.out_stride : nullptr;
     int32_t *p_out = a.positions_out ? a.positions_out + (int64_t)lbh * a.out_stride : nullptr;
     const int recent_from = (a.seen ? a.seen[b] : n) - a.recent;

@@ -403,6 +403,8 @@ typedef struct ekv_evict_params {
  * tokens the rows of largest weight stay (ties: the lower slot; NaN goes first). Rows that stay below slot
  * `keep` stay in place; the i-th free slot takes the i-th row that stays from above, K and V. kept, weights_out
  * and positions_out describe slots 0 .. keep - 1 afterwards (-1, 0, -1 at or past a shorter sequence's end).
+ * A sequence that cannot be cut (unknown, or longer than the stride or the limit) is reported through the pool's
+ * status: its kept is -1 and nothing else of it changes.
  * Lengths do not change here: once every layer is done call ekv_seq_resize(pool, seq, keep) for every sequence that
  * was longer than keep, which frees the blocks (a shorter one would grow by slots that nothing was written to, and
  * they would count as keys). Order among slots is not kept, which attention over turned keys does not see. */

@@ -302,3 +302,23 @@ def test_rope_has_one_rounding(store, rotary, interleaved):
         pools[0].gather(0, 0, 0, n, ekv.GATHER_NATIVE, *got)
         pools[1].gather(0, 0, 0, n, ekv.GATHER_NATIVE, *want)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_evict_leaves_what_it_reports():
+    """A sequence that the call cannot cut keeps its weights and positions also where the outputs are the inputs; the others of
+    the call are cut."""
+    c = dc.Cache([100, 70, 90], 1, 64, seed=1)
+    w = torch.rand(1, 3, 1, 95, generator=torch.Generator().manual_seed(2)).cuda()  # (the first is longer than that)
+    pos = torch.arange(95, dtype=torch.int32, device="cuda").repeat(1, 3, 1, 1).contiguous()
+    old, rows = w.clone(), [c.rows(b) for b in range(3)]
+    kept = torch.zeros(1, 3, 1, 60, dtype=torch.int32, device="cuda")
+    ids = dc.ints([c.seqs[0], c.seqs[1], 999])
+    c.pool.evict_by_weight(0, 1, ids, w, keep=60, first=2, recent=5, kept=kept, weights_out=w, positions=pos, positions_out=pos)
+    torch.cuda.synchronize()
+    assert c.pool.status() in (ekv.DEV_ERR_BAD_POS, ekv.DEV_ERR_BAD_SEQ)
+    for b in (0, 2):
+        assert (kept[0, b] == -1).all() and torch.equal(w[0, b], old[0, b]) and pos[0, b, 0].tolist() == list(range(95))
+        for x, y in zip(rows[b], c.rows(b)):
+            assert torch.equal(x, y)
+    want = dc.evict(old[0, 1, 0, :70].tolist(), 70, 60, 2, 5)
+    assert kept[0, 1, 0].tolist() == want and torch.equal(w[0, 1, 0, :60], old[0, 1, 0][torch.tensor(want, device="cuda")])
