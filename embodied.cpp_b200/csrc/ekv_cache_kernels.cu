@@ -30,7 +30,7 @@ __device__ __forceinline__ bool prefix_dest(const PoolView &p, int layer, int se
         report_error(p.status, DEV_ERR_BAD_POS, seq, pos, p.seq_lens[seq]);
         return false;
     }
-    blk = lookup_block(p, seq, pos / p.block_tokens);
+    blk = lookup_block_to_write(p, seq, pos / p.block_tokens);
     rib = pos % p.block_tokens;
     return blk >= 0;
 }

@@ -40,6 +40,19 @@ void mark_dirty(ekv_pool *p, int32_t id) {
     p->any_dirty = true;
 }
 
+// Blocks in and out of sequences: a block is free again when its last holder lets it go.
+int32_t take_lowest_block(ekv_pool *p) {
+    const int32_t b = *p->free_blocks.begin();
+    p->free_blocks.erase(p->free_blocks.begin());
+    p->holders[(size_t)b] = 1;
+    return b;
+}
+void release_block(ekv_pool *p, int32_t b) {
+    const int32_t left = --p->holders[(size_t)b];
+    if (left == 0) p->free_blocks.insert(b);
+    if (left == 1) p->unshared = p->any_dirty = true;  // its last holder may write it again: known at the next sync
+}
+
 // Makes the pool's device current for one entry point and restores the caller's current device when
 // the entry point returns (a library inside a host such as a ggml backend must not move its device).
 class DeviceScope {
@@ -145,6 +158,12 @@ int ekv_pool_create(const ekv_pool_config *cfg, ekv_pool **out) {
     v.max_blocks_per_seq = c.max_blocks_per_seq;
     v.suffix_rows = (c.suffix_tokens + 15) / 16 * 16;
     v.swz_bytes = ekv::swizzle_bytes_for(c.head_dim);
+    try {
+        p->holders.assign((size_t)c.n_blocks, 0);
+    } catch (const std::bad_alloc &) {
+        delete p;
+        return EKV_ERR_ALLOC;
+    }
     v.bt_shift = -1;
     for (int sh = 0; sh < 16; ++sh)
         if ((1 << sh) == c.block_tokens) v.bt_shift = sh;
@@ -191,6 +210,7 @@ int ekv_pool_create(const ekv_pool_config *cfg, ekv_pool **out) {
     v.prefix = base;
     v.suffix = base + p->bytes_prefix;
     v.block_tables = (int32_t *)(base + p->bytes_prefix + p->bytes_suffix);
+    v.write_tables = v.block_tables;
     v.seq_lens = (int32_t *)(base + p->bytes_prefix + p->bytes_suffix + bytes_tables);
     v.status = (int32_t *)(base + p->bytes_prefix + p->bytes_suffix + bytes_tables + bytes_lens);
 
@@ -218,6 +238,7 @@ int ekv_pool_destroy(ekv_pool *p) {
     cudaDeviceSynchronize();
     if (p->h_status) cudaFreeHost(p->h_status);
     if (p->dev_base) cudaFree(p->dev_base);
+    if (p->dev_write_tables) cudaFree(p->dev_write_tables);
     delete p;
     return EKV_OK;
 }
@@ -254,29 +275,57 @@ int ekv_pool_status(ekv_pool *p, int32_t *code, ekv_stream_t stream) {
     return EKV_OK;
 }
 
+// Upload the rows of changed sequences, adjacent ones together.
+static int upload_dirty(ekv_pool *p, cudaStream_t s) {
+    const int32_t W = p->cfg.max_blocks_per_seq;
+    // Pageable sources: cudaMemcpyAsync stages them before returning, so the host vectors may
+    // change right after this call.
+    std::vector<int32_t> rows, lens;
+    for (int32_t id = 0; id < p->cfg.max_seqs;) {
+        if (!p->dirty[(size_t)id]) {
+            ++id;
+            continue;
+        }
+        int32_t end = id;
+        rows.clear();
+        lens.clear();
+        for (; end < p->cfg.max_seqs && p->dirty[(size_t)end]; ++end) {
+            const ekv_pool::Seq &q = p->seqs[(size_t)end];
+            rows.insert(rows.end(), q.blocks.begin(), q.blocks.end());
+            rows.resize((size_t)(end - id + 1) * W, -1);
+            lens.push_back(q.live ? q.n_tokens : 0);
+        }
+        const size_t n = (size_t)(end - id), at = (size_t)id * W;
+        if (cudaMemcpyAsync(p->view.block_tables + at, rows.data(), n * W * 4, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+            cudaMemcpyAsync(p->view.seq_lens + id, lens.data(), n * 4, cudaMemcpyHostToDevice, s) != cudaSuccess)
+            return EKV_ERR_CUDA;
+        if (p->dev_write_tables) {
+            for (int32_t &b : rows)
+                if (b >= 0 && p->holders[(size_t)b] > 1) b = -1;
+            if (cudaMemcpyAsync(p->dev_write_tables + at, rows.data(), n * W * 4, cudaMemcpyHostToDevice, s) != cudaSuccess)
+                return EKV_ERR_CUDA;
+        }
+        std::fill(p->dirty.begin() + id, p->dirty.begin() + end, (uint8_t)0);
+        id = end;
+    }
+    return EKV_OK;
+}
+
 int ekv_pool_sync(ekv_pool *p, ekv_stream_t stream) {
     if (!p) return EKV_ERR_INVALID_ARG;
     if (!p->any_dirty || p->cfg.device < 0) return EKV_OK;
     const DeviceScope dev_scope(p);
     if (const int e = dev_scope.rc()) return e;
-    cudaStream_t s = (cudaStream_t)stream;
-    const int32_t W = p->cfg.max_blocks_per_seq;
-    // Pageable sources: cudaMemcpyAsync stages them before returning, so the host vectors may
-    // change right after this call.
-    std::vector<int32_t> row((size_t)W);
-    for (int32_t id = 0; id < p->cfg.max_seqs; ++id) {
-        if (!p->dirty[(size_t)id]) continue;
-        const ekv_pool::Seq &q = p->seqs[(size_t)id];
-        std::fill(row.begin(), row.end(), -1);
-        std::copy(q.blocks.begin(), q.blocks.end(), row.begin());
-        const int32_t len = q.live ? q.n_tokens : 0;
-        if (cudaMemcpyAsync(p->view.block_tables + (size_t)id * W, row.data(), (size_t)W * 4,
-                            cudaMemcpyHostToDevice, s) != cudaSuccess ||
-            cudaMemcpyAsync(p->view.seq_lens + id, &len, 4, cudaMemcpyHostToDevice, s) != cudaSuccess)
-            return EKV_ERR_CUDA;
-        p->dirty[(size_t)id] = 0;
+    if (p->unshared && p->dev_write_tables) {
+        for (int32_t id = 0; id < p->cfg.max_seqs; ++id)
+            if (p->seqs[(size_t)id].live && p->seqs[(size_t)id].forked) p->dirty[(size_t)id] = 1;
     }
-    p->any_dirty = false;
+    try {
+        if (const int rc = upload_dirty(p, (cudaStream_t)stream)) return rc;
+    } catch (const std::bad_alloc &) {
+        return EKV_ERR_ALLOC;
+    }
+    p->any_dirty = p->unshared = false;
     return EKV_OK;
 }
 
@@ -287,6 +336,7 @@ int ekv_seq_create(ekv_pool *p, int32_t *seq_id) {
     p->free_seq_ids.erase(p->free_seq_ids.begin());
     ekv_pool::Seq &q = p->seqs[(size_t)id];
     q.live = true;
+    q.forked = false;
     q.n_tokens = 0;
     q.blocks.clear();
     q.pred_lo = q.pred_hi = 0;
@@ -298,7 +348,7 @@ int ekv_seq_create(ekv_pool *p, int32_t *seq_id) {
 int ekv_seq_free(ekv_pool *p, int32_t id) {
     if (!valid_seq(p, id)) return EKV_ERR_NO_SEQ;
     ekv_pool::Seq &q = p->seqs[(size_t)id];
-    for (int32_t b : q.blocks) p->free_blocks.insert(b);
+    for (int32_t b : q.blocks) release_block(p, b);
     q.blocks.clear();
     q.n_tokens = 0;
     q.pred_lo = q.pred_hi = 0;
@@ -317,12 +367,9 @@ int ekv_seq_resize(ekv_pool *p, int32_t id, int32_t n_tokens) {
     const int32_t have = (int32_t)q.blocks.size();
     if (need > have) {
         if ((int32_t)p->free_blocks.size() < need - have) return EKV_ERR_POOL_EXHAUSTED;
-        for (int32_t i = have; i < need; ++i) {
-            q.blocks.push_back(*p->free_blocks.begin());
-            p->free_blocks.erase(p->free_blocks.begin());
-        }
+        for (int32_t i = have; i < need; ++i) q.blocks.push_back(take_lowest_block(p));
     } else {
-        for (int32_t i = need; i < have; ++i) p->free_blocks.insert(q.blocks[(size_t)i]);
+        for (int32_t i = need; i < have; ++i) release_block(p, q.blocks[(size_t)i]);
         q.blocks.resize((size_t)need);
     }
     q.n_tokens = n_tokens;
@@ -345,9 +392,12 @@ int ekv_seq_set_blocks(ekv_pool *p, int32_t id, const int32_t *blocks, int32_t n
         if (!seen.insert(b).second) return EKV_ERR_INVALID_ARG;
         if (!own.count(b) && !p->free_blocks.count(b)) return EKV_ERR_POOL_EXHAUSTED;
     }
-    for (int32_t b : q.blocks) p->free_blocks.insert(b);
+    for (int32_t b : q.blocks) release_block(p, b);
     q.blocks.assign(blocks, blocks + n_blocks);
-    for (int32_t b : q.blocks) p->free_blocks.erase(b);
+    for (int32_t b : q.blocks) {
+        p->free_blocks.erase(b);
+        ++p->holders[(size_t)b];
+    }
     q.n_tokens = n_tokens;
     q.pred_lo = q.pred_hi = 0;
     mark_dirty(p, id);
@@ -358,7 +408,7 @@ int ekv_seq_evict_front(ekv_pool *p, int32_t id, int32_t n_blocks) {
     if (!valid_seq(p, id)) return EKV_ERR_NO_SEQ;
     ekv_pool::Seq &q = p->seqs[(size_t)id];
     if (n_blocks < 0 || n_blocks > (int32_t)q.blocks.size()) return EKV_ERR_RANGE;
-    for (int32_t i = 0; i < n_blocks; ++i) p->free_blocks.insert(q.blocks[(size_t)i]);
+    for (int32_t i = 0; i < n_blocks; ++i) release_block(p, q.blocks[(size_t)i]);
     q.blocks.erase(q.blocks.begin(), q.blocks.begin() + n_blocks);
     const int32_t shift = n_blocks * p->cfg.block_tokens;
     q.n_tokens = std::max(0, q.n_tokens - shift);
@@ -367,6 +417,184 @@ int ekv_seq_evict_front(ekv_pool *p, int32_t id, int32_t n_blocks) {
     clamp_pred(q);
     mark_dirty(p, id);
     return EKV_OK;
+}
+
+int ekv_seq_drop_blocks(ekv_pool *p, int32_t id, int32_t first, int32_t n_blocks) {
+    if (!valid_seq(p, id)) return EKV_ERR_NO_SEQ;
+    ekv_pool::Seq &q = p->seqs[(size_t)id];
+    const int32_t have = (int32_t)q.blocks.size();
+    if (first < 0 || n_blocks < 0 || first > have || n_blocks > have - first) return EKV_ERR_RANGE;
+    // (a table reaches no further than 2^31 tokens: ekv_seq_resize and ekv_seq_set_blocks count them in 32 bits)
+    const int64_t bt = p->cfg.block_tokens;
+    const int32_t lo = (int32_t)std::min<int64_t>(q.n_tokens, first * bt), hi = (int32_t)std::min<int64_t>(q.n_tokens, (first + n_blocks) * bt);
+    if (q.pred_hi > q.pred_lo && q.pred_lo < hi && q.pred_hi > lo) return EKV_ERR_UNSUPPORTED;  // predicted tokens: ekv_seq_clear_pred
+    for (int32_t i = first; i < first + n_blocks; ++i) release_block(p, q.blocks[(size_t)i]);
+    q.blocks.erase(q.blocks.begin() + first, q.blocks.begin() + first + n_blocks);
+    q.n_tokens -= hi - lo;
+    if (q.pred_lo >= hi) {
+        q.pred_lo -= hi - lo;
+        q.pred_hi -= hi - lo;
+    }
+    clamp_pred(q);
+    mark_dirty(p, id);
+    return EKV_OK;
+}
+
+// The writers' own tables, from the first fork on: which blocks a sequence alone holds.
+static int make_write_tables(ekv_pool *p) {
+    if (p->cfg.device < 0 || p->dev_write_tables) return EKV_OK;
+    const size_t bytes = (size_t)p->cfg.max_seqs * p->cfg.max_blocks_per_seq * 4;
+    if (cudaMalloc((void **)&p->dev_write_tables, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        p->dev_write_tables = nullptr;
+        return EKV_ERR_ALLOC;
+    }
+    p->bytes_total += bytes;
+    p->view.write_tables = p->dev_write_tables;
+    for (int32_t id = 0; id < p->cfg.max_seqs; ++id) p->dirty[(size_t)id] = 1;
+    p->any_dirty = true;
+    return EKV_OK;
+}
+
+// The copies count the 16-byte units of a block, all layers, in 32 bits.
+static bool copies_too_large(const ekv_pool *p) {
+    return (int64_t)p->cfg.n_layers * 2 * p->cfg.kv_heads > (1ll << 34) / p->view.tile_bytes;
+}
+
+static int fork_sequences(ekv_pool *p, int32_t n, const int32_t *parents, const int32_t *n_tokens, int32_t *children, cudaStream_t s) {
+    const int32_t bt = p->cfg.block_tokens;
+    const bool device = p->cfg.device >= 0;
+    std::vector<ekv::BlockCopy> copies;
+    std::vector<ekv::ForkedSeq> forks;
+    std::vector<int32_t> dst;
+    copies.reserve(ekv::kMaxForks);
+    forks.reserve(ekv::kMaxForks);
+    dst.reserve(ekv::kMaxForks);
+    std::vector<std::vector<int32_t>> tables((size_t)n);
+    for (int32_t i = 0; i < n; ++i) tables[(size_t)i].reserve((size_t)blocks_for(p, n_tokens[i]));
+    if (device) {
+        if (const int rc = make_write_tables(p)) return rc;
+        // The kernel reads the parents' tables and writes the children's. (Blocks that are no longer shared may wait: so marked,
+        // they are refused to writers, no more.)
+        std::set<int32_t>::const_iterator id = p->free_seq_ids.begin();
+        for (int32_t i = 0; i < n; ++i) p->dirty[(size_t)*id++] = 0;
+        if (const int rc = upload_dirty(p, s)) {
+            p->any_dirty = true;
+            id = p->free_seq_ids.begin();
+            for (int32_t i = 0; i < n; ++i) p->dirty[(size_t)*id++] = 1;
+            return rc;
+        }
+        p->any_dirty = p->unshared;
+    }
+    for (int32_t i = 0; i < n; ++i) {
+        ekv_pool::Seq &from = p->seqs[(size_t)parents[i]];
+        const int32_t full = n_tokens[i] / bt, rest = n_tokens[i] % bt;
+        int32_t tail = -1;
+        std::vector<int32_t> &blocks = tables[(size_t)i];
+        blocks.assign(from.blocks.begin(), from.blocks.begin() + full);
+        for (int32_t b : blocks) ++p->holders[(size_t)b];
+        if (rest) {
+            tail = take_lowest_block(p);
+            blocks.push_back(tail);
+            const int32_t src = from.blocks[(size_t)full], rows = (rest + 7) / 8 * 8;
+            if (!copies.empty() && copies.back().src == src && copies.back().rows == rows) ++copies.back().n_dst;  // a sibling
+            else copies.push_back({src, rows, (int32_t)dst.size(), 1});
+            dst.push_back(tail);
+        }
+        const int32_t id = *p->free_seq_ids.begin();
+        p->free_seq_ids.erase(p->free_seq_ids.begin());
+        ekv_pool::Seq &q = p->seqs[(size_t)id];
+        q.live = q.forked = from.forked = true;
+        q.n_tokens = n_tokens[i];
+        q.blocks.swap(blocks);
+        q.pred_lo = q.pred_hi = 0;
+        children[i] = id;
+        if (!device) {
+            mark_dirty(p, id);
+            continue;
+        }
+        forks.push_back({parents[i], id, full, tail, n_tokens[i]});
+        if ((int32_t)forks.size() < ekv::kMaxForks && i + 1 < n) continue;
+        const int rc = ekv::launch_pages(p->view, copies.data(), (int)copies.size(), dst.data(), (int)dst.size(), forks.data(),
+                                         (int)forks.size(), p->sms, s);
+        if (rc) {  // back to the parents alone; the next sync writes their tables again
+            for (int32_t k = 0; k <= i; ++k) {
+                ekv_seq_free(p, children[k]);
+                mark_dirty(p, parents[k]);
+                children[k] = -1;
+            }
+            return rc;
+        }
+        copies.clear();
+        forks.clear();
+        dst.clear();
+    }
+    return EKV_OK;
+}
+
+int ekv_seq_fork(ekv_pool *p, int32_t n, const int32_t *parents, const int32_t *n_tokens, int32_t *children, ekv_stream_t stream) {
+    if (!p || n < 0 || (n > 0 && (!parents || !n_tokens || !children))) return EKV_ERR_INVALID_ARG;
+    if (copies_too_large(p)) return EKV_ERR_UNSUPPORTED;
+    int64_t tails = 0;
+    for (int32_t i = 0; i < n; ++i) {
+        if (!valid_seq(p, parents[i])) return EKV_ERR_NO_SEQ;
+        if (n_tokens[i] < 0 || n_tokens[i] > p->seqs[(size_t)parents[i]].n_tokens) return EKV_ERR_RANGE;
+        tails += n_tokens[i] % p->cfg.block_tokens != 0;
+    }
+    if ((int64_t)p->free_seq_ids.size() < n || (int64_t)p->free_blocks.size() < tails) return EKV_ERR_POOL_EXHAUSTED;
+    if (n == 0) return EKV_OK;
+    const DeviceScope dev_scope(p);
+    if (p->cfg.device >= 0 && dev_scope.rc()) return dev_scope.rc();
+    try {
+        return fork_sequences(p, n, parents, n_tokens, children, (cudaStream_t)stream);
+    } catch (const std::bad_alloc &) {  // (every allocation comes before the first change, but for the freed sequences' marks)
+        std::set<int32_t>::const_iterator id = p->free_seq_ids.begin();
+        for (int32_t i = 0; i < n; ++i) mark_dirty(p, *id++);
+        return EKV_ERR_ALLOC;
+    }
+}
+
+int ekv_seq_own(ekv_pool *p, int32_t id, int32_t pos0, int32_t n_tokens, ekv_stream_t stream) {
+    if (!valid_seq(p, id)) return EKV_ERR_NO_SEQ;
+    if (copies_too_large(p)) return EKV_ERR_UNSUPPORTED;
+    ekv_pool::Seq &q = p->seqs[(size_t)id];
+    const int32_t bt = p->cfg.block_tokens, have = (int32_t)q.blocks.size();
+    if (pos0 < 0 || n_tokens < 0 || (int64_t)pos0 + n_tokens > (int64_t)have * bt) return EKV_ERR_RANGE;
+    if (n_tokens == 0) return EKV_OK;
+    const int32_t first = pos0 / bt, last = (int32_t)(((int64_t)pos0 + n_tokens - 1) / bt);
+    int32_t shared = 0;
+    for (int32_t i = first; i <= last; ++i) shared += p->holders[(size_t)q.blocks[(size_t)i]] > 1;
+    if (shared == 0) {
+        // what was shared once may still be marked so on the device
+        return p->unshared ? ekv_pool_sync(p, stream) : EKV_OK;
+    }
+    if ((int32_t)p->free_blocks.size() < shared) return EKV_ERR_POOL_EXHAUSTED;
+    const DeviceScope dev_scope(p);
+    if (p->cfg.device >= 0 && dev_scope.rc()) return dev_scope.rc();
+    int rc = EKV_OK;
+    int32_t at = first;
+    while (at <= last && !rc) {
+        // some copies at a time: their launch comes first, so that a failure leaves the sequence as it was
+        ekv::BlockCopy copies[ekv::kMaxForks];
+        int32_t dst[ekv::kMaxForks], entry[ekv::kMaxForks];
+        int n = 0;
+        std::set<int32_t>::const_iterator next = p->free_blocks.begin();
+        for (; at <= last && n < ekv::kMaxForks; ++at) {
+            if (p->holders[(size_t)q.blocks[(size_t)at]] <= 1) continue;
+            copies[n] = {q.blocks[(size_t)at], bt, n, 1};
+            entry[n] = at;
+            dst[n++] = *next++;
+        }
+        if (p->cfg.device >= 0 && n > 0)
+            rc = ekv::launch_pages(p->view, copies, n, dst, n, nullptr, 0, p->sms, (cudaStream_t)stream);
+        for (int i = 0; i < n && !rc; ++i) {
+            q.blocks[(size_t)entry[i]] = take_lowest_block(p);  // (dst[i])
+            release_block(p, copies[i].src);
+        }
+        mark_dirty(p, id);
+    }
+    if (p->cfg.device >= 0 && !rc) rc = ekv_pool_sync(p, stream);
+    return rc;
 }
 
 int ekv_seq_append_tokens(ekv_pool *p, int32_t id, int32_t n_tokens, int32_t pred) {
@@ -395,7 +623,7 @@ int ekv_seq_clear_pred(ekv_pool *p, int32_t id) {
         return ekv_seq_resize(p, id, lo);  // truncation cannot fail
     }
     if (lo % bt || hi % bt) return EKV_ERR_UNSUPPORTED;
-    for (int32_t i = lo / bt; i < hi / bt; ++i) p->free_blocks.insert(q.blocks[(size_t)i]);
+    for (int32_t i = lo / bt; i < hi / bt; ++i) release_block(p, q.blocks[(size_t)i]);
     q.blocks.erase(q.blocks.begin() + lo / bt, q.blocks.begin() + hi / bt);
     q.n_tokens -= hi - lo;
     q.pred_lo = q.pred_hi = 0;
@@ -630,10 +858,11 @@ int ekv_append_suffix_attention(ekv_pool *p, const ekv_attn_params *prm, const v
     return ekv::launch_attention_tc(a, s, ekv::TcKernel::Auto);
 }
 
-int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_batch, const int32_t *seq_ids,
-                    const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int32_t max_rows,
-                    const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
-                    const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream) {
+// Checks of a rotary append, which also fills in the strides of adjacent rows.
+static int check_rope_append(const ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_batch, const int32_t *seq_ids,
+                             const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int32_t max_rows,
+                             const int32_t *positions, int32_t q_heads, const void *q, int64_t &q_stride, const void *q_out,
+                             const void *k, const void *v, int64_t &kv_stride) {
     if (!p || !rope || !n_rows || !src_row || !positions) return EKV_ERR_INVALID_ARG;
     if ((q == nullptr) != (q_out == nullptr) || (k == nullptr) != (v == nullptr) || (!q && !k)) return EKV_ERR_INVALID_ARG;
     if (k && (!seq_ids || !dst_pos)) return EKV_ERR_INVALID_ARG;
@@ -647,11 +876,39 @@ int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_
     if ((q && (q_stride < q_row || q_stride % 8)) || (k && (kv_stride < kv_row || kv_stride % 8))) return EKV_ERR_INVALID_ARG;
     if (q && q == q_out && q_stride != q_row) return EKV_ERR_INVALID_ARG;
     if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) return EKV_ERR_INVALID_ARG;
+    return EKV_OK;
+}
+
+int ekv_rope_append(ekv_pool *p, const ekv_rope *rope, int32_t layer, int32_t n_batch, const int32_t *seq_ids,
+                    const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int32_t max_rows,
+                    const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
+                    const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream) {
+    if (const int rc = check_rope_append(p, rope, layer, n_batch, seq_ids, dst_pos, n_rows, src_row, max_rows, positions, q_heads, q,
+                                         q_stride, q_out, k, v, kv_stride))
+        return rc;
     if (n_batch == 0 || max_rows == 0) return EKV_OK;
-    if (ekv::rope_device(rope) != c.device) return EKV_ERR_INVALID_ARG;
+    if (ekv::rope_device(rope) != p->cfg.device) return EKV_ERR_INVALID_ARG;
     const DeviceScope dev_scope(p);
     if (const int e = dev_scope.rc()) return e;
     return ekv::launch_rope_append(p->view, rope, layer, n_batch, seq_ids, dst_pos, n_rows, src_row, max_rows, positions,
+                                   q_heads, q, q_stride, q_out, k, v, kv_stride, p->sms, (cudaStream_t)stream);
+}
+
+int ekv_norm_rope_append(ekv_pool *p, const ekv_rope *rope, const ekv_head_norm *norm, int32_t layer, int32_t n_batch,
+                         const int32_t *seq_ids, const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row,
+                         int32_t max_rows, const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
+                         const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream) {
+    if (!norm || !(norm->eps >= 0.0f) || !std::isfinite(norm->eps) || !std::isfinite(norm->weight_offset)) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)norm->q_weight | (uintptr_t)norm->k_weight) & 15) return EKV_ERR_INVALID_ARG;
+    if (const int rc = check_rope_append(p, rope, layer, n_batch, seq_ids, dst_pos, n_rows, src_row, max_rows, positions, q_heads, q,
+                                         q_stride, q_out, k, v, kv_stride))
+        return rc;
+    if (norm->weight_dtype != EKV_DTYPE_F32 && norm->weight_dtype != EKV_DTYPE_BF16) return EKV_ERR_UNSUPPORTED;
+    if (n_batch == 0 || max_rows == 0) return EKV_OK;
+    if (ekv::rope_device(rope) != p->cfg.device) return EKV_ERR_INVALID_ARG;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    return ekv::launch_norm_rope_append(p->view, rope, norm, layer, n_batch, seq_ids, dst_pos, n_rows, src_row, max_rows, positions,
                                    q_heads, q, q_stride, q_out, k, v, kv_stride, p->sms, (cudaStream_t)stream);
 }
 
@@ -788,6 +1045,27 @@ int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t s
     a.positions_out = prm->positions_out;
     a.max_len = (int32_t)std::min<int64_t>((int64_t)c.max_blocks_per_seq * c.block_tokens, EKV_MAX_EVICT_TOKENS);
     return ekv::launch_evict(a, max_len, (cudaStream_t)stream);
+}
+
+int ekv_compact(ekv_pool *p, const ekv_compact_params *prm, ekv_stream_t stream) {
+    if (!p || !prm || !prm->seq_ids || !prm->n_keep || !prm->slots) return EKV_ERR_INVALID_ARG;
+    const ekv_pool_config &c = p->cfg;
+    if (prm->layer0 < 0 || prm->n_layers <= 0 || prm->n_layers > c.n_layers - prm->layer0 || prm->n_batch < 0 || prm->slot_stride < 0)
+        return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)prm->seq_ids | (uintptr_t)prm->n_keep | (uintptr_t)prm->slots) & 3) return EKV_ERR_INVALID_ARG;
+    if (prm->n_batch == 0 || prm->slot_stride == 0) return EKV_OK;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    ekv::CompactArgs a{};
+    a.pool = p->view;
+    a.layer0 = prm->layer0;
+    a.n_layers = prm->n_layers;
+    a.n_batch = prm->n_batch;
+    a.seq_ids = prm->seq_ids;
+    a.n_keep = prm->n_keep;
+    a.slots = prm->slots;
+    a.slot_stride = prm->slot_stride;
+    return ekv::launch_compact(a, p->sms, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -164,18 +164,21 @@ __device__ __forceinline__ SeqKeys resolve_seq(const PoolView &p, int use_prefix
     return r;
 }
 
-// Physical block of table entry `idx` of `seq`, or -1 (and an error report) when out of range.
-__device__ __forceinline__ int lookup_block(const PoolView &p, int seq, int idx) {
+// Physical block of entry `idx` of `seq` in one of the pool's tables, or -1 (and an error report) when out of range.
+__device__ __forceinline__ int lookup_in(const PoolView &p, const int32_t *tables, int seq, int idx) {
     if (idx < 0 || idx >= p.max_blocks_per_seq) {
         report_error(p.status, DEV_ERR_BAD_POS, seq, idx, 0);
         return -1;
     }
-    const int blk = p.block_tables[(int64_t)seq * p.max_blocks_per_seq + idx];
+    const int blk = tables[(int64_t)seq * p.max_blocks_per_seq + idx];
     if (blk < 0 || blk >= p.n_blocks) {
         report_error(p.status, DEV_ERR_BAD_BLOCK, seq, idx, blk);
         return -1;
     }
     return blk;
 }
+__device__ __forceinline__ int lookup_block(const PoolView &p, int seq, int idx) { return lookup_in(p, p.block_tables, seq, idx); }
+// The same for a block that will be written: one that several sequences share is an error.
+__device__ __forceinline__ int lookup_block_to_write(const PoolView &p, int seq, int idx) { return lookup_in(p, p.write_tables, seq, idx); }
 
 }  // namespace ekv

@@ -93,7 +93,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int lbh, int slot0
     int bs = -1;
     if (move) {
         bs = lookup_block(p, seq, from / p.block_tokens);
-        move = bs >= 0;
+        move = bs >= 0 && (p.write_tables == p.block_tables || lookup_block_to_write(p, seq, slot / p.block_tokens) >= 0);
     }
     const uint32_t moving = __ballot_sync(0xffffffffu, move);
     if (!moving) return;

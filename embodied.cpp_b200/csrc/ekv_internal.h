@@ -16,8 +16,12 @@ struct ekv_pool {
     void *dev_base = nullptr;
     size_t bytes_total = 0, bytes_prefix = 0, bytes_suffix = 0;
     std::set<int32_t> free_blocks;  // lowest index first
+    std::vector<int32_t> holders;   // per block: sequences that hold it (0: free)
+    int32_t *dev_write_tables = nullptr;  // made by the first fork (PoolView::write_tables)
+    bool unshared = false;          // a block went from two holders to one since the last sync
     struct Seq {
         bool live = false;
+        bool forked = false;               // it was forked, or came from a fork
         int32_t n_tokens = 0;
         std::vector<int32_t> blocks;
         int32_t pred_lo = 0, pred_hi = 0;  // predicted tokens [pred_lo, pred_hi), empty when equal
@@ -28,6 +32,13 @@ struct ekv_pool {
     bool any_dirty = false;
     int32_t *h_status = nullptr;   // pinned, 4 ints
     int sms = 148;                 // SM count of the pool's device (key-split sizing)
+};
+
+struct ekv_rope {
+    int32_t device, interleaved, rotary;
+    float magnitude;
+    double freq[128];      // radians per position of each pair
+    double *dev_turns;     // the same in turns, on the device
 };
 
 namespace ekv {
@@ -173,6 +184,31 @@ int launch_rope_append(const PoolView &p, const ekv_rope *rope, int layer, int n
                        const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int max_rows,
                        const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
                        const void *v, int64_t kv_stride, int sms, cudaStream_t s);
+// The same with RMS norms of the q and k heads (ekv_norm_rope.cu)
+int launch_norm_rope_append(const PoolView &p, const ekv_rope *rope, const ekv_head_norm *norm, int layer, int n_batch,
+                            const int32_t *seq_ids, const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row, int max_rows,
+                            const int32_t *positions, int q_heads, const void *q, int64_t q_stride, void *q_out, const void *k,
+                            const void *v, int64_t kv_stride, int sms, cudaStream_t s);
+// Copies of blocks and children's tables (ekv_pages.cu). A copy: rows [0, rows) (a multiple of 8) of block `src` of every
+// layer go to `n_dst` blocks, the entries dst[first ..]. A child: its table row, the first n_full entries the parent's, then
+// `tail` (-1: none), and its length.
+struct BlockCopy {
+    int32_t src, rows, first, n_dst;
+};
+struct ForkedSeq {
+    int32_t parent, child, n_full, tail, n_tokens;
+};
+constexpr int kMaxForks = 256;  // copies, destinations and children of one launch
+int launch_pages(const PoolView &p, const BlockCopy *copies, int n_copies, const int32_t *dst, int n_dst, const ForkedSeq *children,
+                 int n_children, int sms, cudaStream_t s);
+// Rows that stay move together (ekv_pages.cu)
+struct CompactArgs {
+    PoolView pool;
+    int32_t layer0, n_layers, n_batch;
+    const int32_t *seq_ids, *n_keep, *slots;
+    int64_t slot_stride;
+};
+int launch_compact(const CompactArgs &a, int sms, cudaStream_t s);
 // Eviction by weight (ekv_evict.cu)
 // max_live: the longest live sequence
 int launch_evict(EvictArgs a, int max_live, cudaStream_t s);

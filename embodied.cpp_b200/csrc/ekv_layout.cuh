@@ -25,6 +25,8 @@ struct PoolView {
     uint8_t *prefix;          // prefix arena
     uint8_t *suffix;          // suffix arena
     int32_t *block_tables;    // [max_seqs][max_blocks_per_seq]
+    int32_t *write_tables;    // what writers go by: block_tables, until a sequence of the pool is forked; then a table
+                              // of its own, -1 where a block belongs to several sequences
     int32_t *seq_lens;        // [max_seqs]
     int32_t *status;          // [4]
     int32_t dtype;            // EKV_DTYPE_BF16 / EKV_DTYPE_Q8_0

@@ -15,13 +15,6 @@
 #include "ekv_decode.cuh"
 #include "ekv_internal.h"
 
-struct ekv_rope {
-    int32_t device, interleaved, rotary;
-    float magnitude;
-    double freq[128];      // radians per position of each pair
-    double *dev_turns;     // the same in turns, on the device
-};
-
 namespace ekv {
 namespace {
 
@@ -183,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeArgs a)
         } else if (pos < 0 || pos >= p.seq_lens[seq]) {
             report_error(p.status, DEV_ERR_BAD_POS, seq, pos, p.seq_lens[seq]);
         } else {
-            blk = lookup_block(p, seq, pos / p.block_tokens);
+            blk = lookup_block_to_write(p, seq, pos / p.block_tokens);
         }
         s_blk[threadIdx.x] = blk;
         s_rib[threadIdx.x] = pos < 0 ? 0 : pos % p.block_tokens;

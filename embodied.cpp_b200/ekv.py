@@ -106,6 +106,16 @@ class EvictParams(C.Structure):
                 ("weights_out", C.c_void_p), ("positions_out", C.c_void_p), ("out_stride", C.c_int64)]
 
 
+class CompactParams(C.Structure):
+    _fields_ = [("layer0", C.c_int32), ("n_layers", C.c_int32), ("n_batch", C.c_int32), ("reserved", C.c_int32),
+                ("seq_ids", C.c_void_p), ("n_keep", C.c_void_p), ("slots", C.c_void_p), ("slot_stride", C.c_int64)]
+
+
+class HeadNormConfig(C.Structure):
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int32),
+                ("after_rotation", C.c_int32), ("weight_offset", C.c_float), ("eps", C.c_float)]
+
+
 class Tensor(C.Structure):
     """ekv_tensor: a ggml-ordered strided device tensor (ne[0] fastest, nb in bytes)."""
     _fields_ = [("data", C.c_void_p), ("type", C.c_int32), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
@@ -124,7 +134,8 @@ EXPORTED = [
     "ekv_flow_step_f32", "ekv_guidance_f32", "ekv_sched_create", "ekv_sched_destroy", "ekv_sched_submit",
     "ekv_sched_begin_tick", "ekv_sched_end_tick", "ekv_sched_stats", "ekv_project_qkv_rope",
     "ekv_rope_create", "ekv_rope_destroy", "ekv_rope_get", "ekv_rope_append", "ekv_tree_attention_workspace_size",
-    "ekv_tree_attention", "ekv_key_weights", "ekv_evict_by_weight",
+    "ekv_tree_attention", "ekv_key_weights", "ekv_evict_by_weight", "ekv_norm_rope_append", "ekv_seq_drop_blocks",
+    "ekv_seq_fork", "ekv_seq_own", "ekv_compact",
 ]
 NOALLOC_SCRATCH_BYTES = 16 << 20  # EKV_NOALLOC_SCRATCH_BYTES
 
@@ -191,6 +202,12 @@ def _load():
         "ekv_tree_attention": ([vp, C.POINTER(TreeParams), vp, vp, vp, vp, vp, vp, C.c_size_t, vp], C.c_int),
         "ekv_key_weights": ([vp, C.POINTER(TreeParams), vp, vp, vp, C.c_int64, C.c_float, vp], C.c_int),
         "ekv_evict_by_weight": ([vp, C.POINTER(EvictParams), vp], C.c_int),
+        "ekv_norm_rope_append": ([vp, vp, C.POINTER(HeadNormConfig), i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, C.c_int64, vp, vp,
+                                  vp, C.c_int64, vp], C.c_int),
+        "ekv_seq_drop_blocks": ([vp, i32, i32, i32], C.c_int),
+        "ekv_seq_fork": ([vp, i32, pi32, pi32, pi32, vp], C.c_int),
+        "ekv_seq_own": ([vp, i32, i32, i32, vp], C.c_int),
+        "ekv_compact": ([vp, C.POINTER(CompactParams), vp], C.c_int),
         "ekv_version": ([], C.c_char_p),
         "ekv_launch_count": ([], C.c_uint64),
         "ekv_strerror": ([C.c_int], C.c_char_p),
@@ -328,6 +345,28 @@ class Pool:
     def seq_evict_front(self, seq, n_blocks):
         check(lib.ekv_seq_evict_front(self.h, seq, n_blocks), "ekv_seq_evict_front")
 
+    def seq_drop_blocks(self, seq, first, n_blocks):
+        """ekv_seq_drop_blocks: blocks [first, first + n_blocks) leave the sequence; later tokens move down."""
+        check(lib.ekv_seq_drop_blocks(self.h, seq, first, n_blocks), "ekv_seq_drop_blocks")
+
+    def seq_fork(self, parents, n_tokens, stream=None) -> list:
+        """ekv_seq_fork: one new sequence for each entry, the first n_tokens[i] tokens of sequence parents[i]; whole blocks
+        are shared, the last, partial one is copied. Needs no sync()."""
+        n = len(parents)
+        if len(n_tokens) != n:
+            raise ValueError("one length for each parent")
+        ints = C.c_int32 * n
+        children = ints()
+        code = lib.ekv_seq_fork(self.h, n, ints(*parents), ints(*n_tokens), children,
+                                None if self.cfg.device < 0 else _stream(stream))
+        if code:
+            check(code, "ekv_seq_fork")
+        return children[:]
+
+    def seq_own(self, seq, pos0, n_tokens, stream=None):
+        """ekv_seq_own: shared blocks under positions [pos0, pos0 + n_tokens) become copies that the sequence may write."""
+        check(lib.ekv_seq_own(self.h, seq, pos0, n_tokens, None if self.cfg.device < 0 else _stream(stream)), "ekv_seq_own")
+
     def seq_append_tokens(self, seq, n_tokens, pred=False):
         check(lib.ekv_seq_append_tokens(self.h, seq, n_tokens, 1 if pred else 0), "ekv_seq_append_tokens")
 
@@ -408,8 +447,17 @@ class Pool:
         """ekv_rope_append: turn q [rows, q_heads, head_dim] into q_out and k into the pages beside v ([rows, kv_heads,
         head_dim]), all bf16 and by source row. q, k and v may be slices of one [rows, columns] projection output:
         rows may be any distance apart, a row's heads are adjacent. Either pair may be left out."""
+        q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
+        code = lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), None if kp is None else _ptr(seq_ids),
+                                   None if kp is None else _ptr(dst_pos), n_rows.data_ptr(), src_row.data_ptr(), max_rows,
+                                   positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride, _stream(stream))
+        if code:
+            check(code, "ekv_rope_append")
+
+    def _rope_rows(self, q, q_out, k, v):
+        """Heads, pointers and row distances of a rotary append's rows."""
         q_heads = q_stride = kv_stride = 0
-        qp = q_to = kp = vp = seqs = dst = None
+        qp = q_to = kp = vp = None
         if q is not None:
             q_heads, q_stride = _rows(q, self.head_dim, "q")
             if q_out is None or q_out.shape != q.shape or not q_out.is_contiguous():
@@ -421,12 +469,24 @@ class Pool:
             kv_heads, kv_stride = _rows(k, self.head_dim, "k and v")
             if kv_heads != self.kv_heads:
                 raise ValueError("k and v must have the pool's KV heads")
-            kp, vp, seqs, dst = k.data_ptr(), v.data_ptr(), _ptr(seq_ids), _ptr(dst_pos)
-        code = lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), seqs, dst, n_rows.data_ptr(), src_row.data_ptr(),
-                                   max_rows, positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride,
-                                   _stream(stream))
+            kp, vp = k.data_ptr(), v.data_ptr()
+        return q_heads, qp, q_stride, q_to, kp, vp, kv_stride
+
+    def norm_rope_append(self, rope, norm, layer, seq_ids, dst_pos, n_rows, src_row, max_rows, positions, *, q=None, q_out=None,
+                         k=None, v=None, stream=None):
+        """ekv_norm_rope_append: rope_append with an RMS norm (HeadNorm) of every q and k head before its rotation, or after."""
+        if norm.dim not in (0, self.head_dim):
+            raise ValueError("the norm's weights must have head_dim values")
+        q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
+        for t in (q, q_out, k, v):
+            if t is not None and t.dtype is not norm.bf16:
+                raise ValueError("q, q_out, k and v must be bf16")
+        code = lib.ekv_norm_rope_append(self.h, rope.h, norm.ref, layer, n_rows.numel(), None if kp is None else seq_ids.data_ptr(),
+                                        None if kp is None else dst_pos.data_ptr(), n_rows.data_ptr(), src_row.data_ptr(),
+                                        max_rows, positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride,
+                                        _stream(stream))
         if code:
-            check(code, "ekv_rope_append")
+            check(code, "ekv_norm_rope_append")
 
     def tree_params(self, *, layer, seq_ids, n_draft, q_heads, scale, softcap=0.0, out_dtype=DTYPE_BF16,
                     prefix_len=None, n_nodes=None, ancestors=None, max_prefix=0) -> TreeParams:
@@ -513,6 +573,41 @@ class Pool:
         code = lib.ekv_evict_by_weight(self.h, C.byref(p), _stream(stream))
         if code:
             check(code, "ekv_evict_by_weight")
+
+
+    def compact(self, layer0, n_layers, seq_ids, slots, n_keep, stream=None):
+        """ekv_compact: slot i of sequence seq_ids[b] gets the row of slot slots[b, i], for i below n_keep[b], in the layers from
+        layer0 on. slots int32 [n_batch, stride], ascending; call seq_resize(seq, n_keep) afterwards."""
+        n = seq_ids.numel()
+        if slots.dim() != 2 or slots.shape[0] != n:
+            raise ValueError("slots must be [n_batch, stride]")
+        stride = slots.shape[1]
+        p = CompactParams(layer0, n_layers, n, 0, _index(seq_ids, n, "seq_ids"), _index(n_keep, n, "n_keep"),
+                          _index(slots, n * stride, "slots"), stride)
+        code = lib.ekv_compact(self.h, C.byref(p), _stream(stream))
+        if code:
+            check(code, "ekv_compact")
+
+
+class HeadNorm:
+    """RMS norms of q and k heads for norm_rope_append (ekv_head_norm): weights of head_dim values, bf16 or f32 (None: ones),
+    weight_offset added to them (1 where they are stored as differences from 1), before the rotation or after it."""
+
+    def __init__(self, *, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0, after_rotation=False):
+        import torch
+        given = [w for w in (q_weight, k_weight) if w is not None]
+        for w in given:
+            if w.dtype not in (torch.float32, torch.bfloat16) or w.dim() != 1 or not w.is_contiguous():
+                raise ValueError("weights must be one adjacent row of bf16 or f32 values")
+        if len({(w.dtype, w.numel()) for w in given}) > 1:
+            raise ValueError("q_weight and k_weight must have one type and length")
+        self.dim = given[0].numel() if given else 0
+        self.bf16 = torch.bfloat16
+        self._keep = given
+        self.cfg = HeadNormConfig(_ptr(q_weight), _ptr(k_weight),
+                                  DTYPE_BF16 if given and given[0].dtype is torch.bfloat16 else DTYPE_F32,
+                                  1 if after_rotation else 0, weight_offset, eps)
+        self.ref = C.byref(self.cfg)
 
 
 class Rope:

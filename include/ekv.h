@@ -111,6 +111,29 @@ int ekv_seq_set_blocks(ekv_pool *pool, int32_t seq_id, const int32_t *blocks, in
  * the role of LingBotKVCache::allocate_slots_into's oldest-id eviction,
  * models/lingbot_va.cpp:8806-8825). Later tokens move down by n_blocks*block_tokens. */
 int ekv_seq_evict_front(ekv_pool *pool, int32_t seq_id, int32_t n_blocks);
+/* Drop blocks [first, first + n_blocks) of the sequence's table, free ones to the pool: what lies between the first tokens and a
+ * sliding window, say. Later tokens move down by n_blocks*block_tokens (fewer where the last block was not full).
+ * EKV_ERR_UNSUPPORTED where predicted tokens lie in them. */
+int ekv_seq_drop_blocks(ekv_pool *pool, int32_t seq_id, int32_t first, int32_t n_blocks);
+/* ---- sequences that share blocks ----
+ * A block may belong to several sequences; it is free once the last of them lets it go, by whichever call. Shared blocks are
+ * read by all and written by none: from the pool's first fork on, ekv_append, ekv_rope_append, ekv_norm_rope_append,
+ * ekv_evict_by_weight and ekv_compact report a row that would go into one (ekv_pool_status: 1) and do not write it. Calls that
+ * were captured into a graph before the pool's first fork do not look. No counterpart in the reference. */
+/* For each i < n a new sequence children[i], the first n_tokens[i] tokens of sequence parents[i] in every layer (host arrays; a
+ * parent may be named any number of times). Whole blocks are shared. Of a last, partial block the child gets a copy of the rows
+ * in use, in whole groups of eight, so that parent and children append to blocks of their own. Suffix slots and predicted marks
+ * are not taken over. The children's tables and lengths, and those of sequences that changed before, are on the device for what
+ * follows on `stream`: no ekv_pool_sync is needed. (Blocks whose other holders have let them go stay closed to writers until the
+ * next ekv_pool_sync or ekv_seq_own.) EKV_ERR_POOL_EXHAUSTED leaves the pool unchanged. The pool's first fork
+ * allocates device memory: not under stream capture, nor is any other (the host hands out the blocks). */
+int ekv_seq_fork(ekv_pool *pool, int32_t n, const int32_t *parents, const int32_t *n_tokens, int32_t *children,
+                 ekv_stream_t stream);
+/* Copies of the shared blocks that hold positions [pos0, pos0 + n_tokens) of the sequence, which is then their only holder and
+ * may write them (before rows of a fork are overwritten, evicted by weight or compacted, or after a fork was cut shorter and
+ * before it grows again). The table is uploaded. EKV_ERR_POOL_EXHAUSTED leaves the pool unchanged. */
+int ekv_seq_own(ekv_pool *pool, int32_t seq_id, int32_t pos0, int32_t n_tokens, ekv_stream_t stream);
+
 /* ---- predicted tokens (LingBot-VA's rollout appends predicted K/V, attends, then rolls them back
  * before the clean K/V of the same chunk are appended: LingBotKVCache::update_with_workspace's
  * is_pred, restore and clear_pred, models/lingbot_va.cpp:8853-8886, 8946-8966). A sequence holds at
@@ -340,6 +363,22 @@ int ekv_rope_append(ekv_pool *pool, const ekv_rope *rope, int32_t layer, int32_t
                     const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
                     const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream);
 
+typedef struct ekv_head_norm {
+    const void *q_weight;   /* device [head_dim], or NULL: ones                                       */
+    const void *k_weight;
+    int32_t weight_dtype;   /* EKV_DTYPE_F32 or EKV_DTYPE_BF16                                         */
+    int32_t after_rotation; /* 0: heads are normed, then turned; 1: turned, then normed                */
+    float weight_offset;    /* added to every weight: 1 where the weights are stored as differences from 1 */
+    float eps;
+} ekv_head_norm;
+/* ekv_rope_append with an RMS norm of every q and k head: x / sqrt(mean(x^2) + eps) * (weight + weight_offset) over the head's
+ * columns, before or after its rotation, in 32 bits and rounded to bf16 once. v passes as it is. Everything else as
+ * ekv_rope_append; weights 16-byte aligned. */
+int ekv_norm_rope_append(ekv_pool *pool, const ekv_rope *rope, const ekv_head_norm *norm, int32_t layer, int32_t n_batch,
+                         const int32_t *seq_ids, const int32_t *dst_pos, const int32_t *n_rows, const int32_t *src_row,
+                         int32_t max_rows, const int32_t *positions, int32_t q_heads, const void *q, int64_t q_stride, void *q_out,
+                         const void *k, const void *v, int64_t kv_stride, ekv_stream_t stream);
+
 #define EKV_MAX_DRAFT 64
 typedef struct ekv_tree_params {
     int32_t layer;
@@ -409,6 +448,22 @@ typedef struct ekv_evict_params {
  * was longer than keep, which frees the blocks (a shorter one would grow by slots that nothing was written to, and
  * they would count as keys). Order among slots is not kept, which attention over turned keys does not see. */
 int ekv_evict_by_weight(ekv_pool *pool, const ekv_evict_params *p, ekv_stream_t stream);
+
+typedef struct ekv_compact_params {
+    int32_t layer0, n_layers;   /* the layers [layer0, layer0 + n_layers)                              */
+    int32_t n_batch;
+    int32_t reserved;
+    const int32_t *seq_ids;     /* device [n_batch], distinct                                         */
+    const int32_t *n_keep;      /* device [n_batch] slots that stay                                   */
+    const int32_t *slots;       /* device [n_batch][slot_stride]: the slots that stay, ascending         */
+    int64_t slot_stride;
+} ekv_compact_params;
+/* Move the rows that stay together, K and V of every KV head: slot i of the sequence gets the row of slot slots[b][i], for i below
+ * n_keep[b]. Order among rows is kept, and slots at or above n_keep[b] keep what they hold. Lengths do not change here: call
+ * ekv_seq_resize(pool, seq, n_keep) afterwards. Rows keep the positions that they were turned by. An entry that is not above the
+ * one before it, or not a slot of the sequence, is reported through the pool's status and its row does not move; so is a request
+ * whose n_keep is not in 0 .. slot_stride, or above the sequence's length, of which nothing moves. */
+int ekv_compact(ekv_pool *pool, const ekv_compact_params *p, ekv_stream_t stream);
 
 /* ---- ggml op surface: GGML_OP_FLASH_ATTN_EXT on strided device tensors ----
  * Replaces ggml_flash_attn_ext (models/hy_vla.cpp:376-378, :439-441, :460, :492, :859 (GQA, mask);
