@@ -998,6 +998,63 @@ int ekv_key_weights(ekv_pool *p, const ekv_tree_params *prm, const void *q, cons
     return ekv::launch_key_weights(a, max_len, p->sms, (cudaStream_t)stream);
 }
 
+// Rows of a KV head times its query heads are 32-bit in the kernels, and so are a KV head's rows.
+static bool window_rows_fit(const ekv_window_params *prm, const ekv_pool *p) {
+    const int64_t group = prm->q_heads / p->cfg.kv_heads;
+    return group < 8192 && (prm->max_rows + 256ll) * group < (1ll << 32) / group && prm->max_rows * group < INT32_MAX - 512;
+}
+
+size_t ekv_window_attention_workspace_size(const ekv_pool *p, const ekv_window_params *prm) {
+    if (!p || !prm || prm->n_batch <= 0 || prm->max_rows <= 0 || prm->q_heads <= 0 || prm->q_heads % p->cfg.kv_heads ||
+        !window_rows_fit(prm, p))
+        return 0;
+    return ekv::window_workspace(p->view, prm->n_batch, prm->max_rows, prm->q_heads, p->sms);
+}
+
+int ekv_window_attention(ekv_pool *p, const ekv_window_params *prm, const void *q, int64_t q_stride, void *out, void *workspace,
+                         size_t workspace_bytes, ekv_stream_t stream) {
+    if (!p || !prm || !q || !out || q == out || !prm->seq_ids || !prm->dst_pos || !prm->n_rows || !prm->src_row) return EKV_ERR_INVALID_ARG;
+    const ekv_pool_config &c = p->cfg;
+    if (prm->layer < 0 || prm->layer >= c.n_layers || prm->n_batch < 0 || prm->max_rows < 0 || prm->q_heads <= 0 || prm->q_heads % c.kv_heads)
+        return EKV_ERR_INVALID_ARG;
+    if (prm->window < 0 || prm->sinks < 0 || prm->max_len < 0) return EKV_ERR_INVALID_ARG;
+    const float log2e = 1.4426950408889634f;
+    if (!(prm->scale > 0.0f) || !std::isfinite(prm->scale * log2e)) return EKV_ERR_INVALID_ARG;
+    const int64_t row = (int64_t)prm->q_heads * c.head_dim;
+    if (q_stride == 0) q_stride = row;
+    if (q_stride < row || q_stride % 8) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) return EKV_ERR_INVALID_ARG;
+    if (((uintptr_t)prm->seq_ids | (uintptr_t)prm->dst_pos | (uintptr_t)prm->n_rows | (uintptr_t)prm->src_row) & 3) return EKV_ERR_INVALID_ARG;
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return EKV_ERR_UNSUPPORTED;
+    if (!window_rows_fit(prm, p)) return EKV_ERR_UNSUPPORTED;
+    if (prm->n_batch == 0 || prm->max_rows == 0) return EKV_OK;
+    const DeviceScope dev_scope(p);
+    if (const int e = dev_scope.rc()) return e;
+    ekv::WindowArgs a{};
+    a.pool = p->view;
+    a.layer = prm->layer;
+    a.n_batch = prm->n_batch;
+    a.q_heads = prm->q_heads;
+    a.group = prm->q_heads / c.kv_heads;
+    a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);  // (not used at 1, where it is 2^32)
+    a.max_rows = prm->max_rows;
+    a.window = prm->window > 0 ? prm->window : INT32_MAX;
+    a.sinks = prm->sinks;
+    a.scale_log2 = prm->scale * log2e;
+    a.seq_ids = prm->seq_ids;
+    a.dst_pos = prm->dst_pos;
+    a.n_rows = prm->n_rows;
+    a.src_row = prm->src_row;
+    a.q = (const uint16_t *)q;
+    a.q_stride = q_stride;
+    a.out = (uint16_t *)out;
+    int max_len = 0;
+    for (const ekv_pool::Seq &s : p->seqs)
+        if (s.live) max_len = std::max(max_len, s.n_tokens);
+    if (prm->max_len > 0) max_len = std::min(max_len, prm->max_len);
+    return ekv::launch_window_attention(a, max_len, workspace, workspace_bytes, p->sms, (cudaStream_t)stream);
+}
+
 int ekv_evict_by_weight(ekv_pool *p, const ekv_evict_params *prm, ekv_stream_t stream) {
     if (!p || !prm || !prm->seq_ids || !prm->weights || !prm->kept) return EKV_ERR_INVALID_ARG;
     const ekv_pool_config &c = p->cfg;

@@ -103,6 +103,27 @@ struct TreeArgs {
     float decay;
 };
 
+// An attention of appended rows with a sliding window and first tokens that stay visible.
+struct WindowArgs {
+    PoolView pool;
+    int32_t layer, n_batch, q_heads, group, max_rows;
+    uint32_t group_mul;  // ceil(2^32 / group) (group > 1)
+    int32_t window;      // a row sees its own slot and the window - 1 before it (2^31 - 1: all before it)
+    int32_t sinks;       // and slots below this
+    float scale_log2;    // scale * log2(e)
+    const int32_t *seq_ids, *dst_pos, *n_rows, *src_row;
+    const uint16_t *q;
+    int64_t q_stride;    // elements per source row
+    uint16_t *out;
+    // units: (request, row tile, KV head); partial results of units cut between CTAs
+    int32_t row_tiles;   // row tiles of one (request, KV head)
+    int32_t split;       // CTAs take equal ranges of the call's tiles; 0: whole units
+    int32_t cluster;     // (rows kernel, split == 0) CTAs of a unit
+    int2 *parts;         // [units] first and last CTA of each unit
+    float4 *ws_ml;       // [2 * CTAs][rows] maximum (log2 domain), sum of the rounded probabilities
+    float *ws_o;         // [2 * CTAs][rows][D] unnormalised output
+};
+
 // An eviction (ekv_evict_params, with the pool).
 struct EvictArgs {
     PoolView pool;
@@ -209,6 +230,13 @@ struct CompactArgs {
     int64_t slot_stride;
 };
 int launch_compact(const CompactArgs &a, int sms, cudaStream_t s);
+// Windowed attention (ekv_window.cu: few rows of a KV head, and the choice; ekv_window_tile.cu: more, on tcgen05). The workspace
+// size depends on the call's shape alone; max_len, an upper bound of the slots that rows see, only sizes grids.
+size_t window_workspace(const PoolView &p, int n_batch, int max_rows, int q_heads, int sms);
+int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s);
+int window_tile_rows(int head_dim);  // rows of a unit of the tile kernel
+int window_tile_keys(int head_dim);  // keys of one of its tiles
+int launch_window_tile(const WindowArgs &a, int grid, cudaStream_t s);
 // Eviction by weight (ekv_evict.cu)
 // max_live: the longest live sequence
 int launch_evict(EvictArgs a, int max_live, cudaStream_t s);

@@ -111,6 +111,12 @@ class CompactParams(C.Structure):
                 ("seq_ids", C.c_void_p), ("n_keep", C.c_void_p), ("slots", C.c_void_p), ("slot_stride", C.c_int64)]
 
 
+class WindowParams(C.Structure):
+    _fields_ = [("layer", C.c_int32), ("n_batch", C.c_int32), ("q_heads", C.c_int32), ("max_rows", C.c_int32),
+                ("window", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("max_len", C.c_int32),
+                ("seq_ids", C.c_void_p), ("dst_pos", C.c_void_p), ("n_rows", C.c_void_p), ("src_row", C.c_void_p)]
+
+
 class HeadNormConfig(C.Structure):
     _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int32),
                 ("after_rotation", C.c_int32), ("weight_offset", C.c_float), ("eps", C.c_float)]
@@ -135,7 +141,7 @@ EXPORTED = [
     "ekv_sched_begin_tick", "ekv_sched_end_tick", "ekv_sched_stats", "ekv_project_qkv_rope",
     "ekv_rope_create", "ekv_rope_destroy", "ekv_rope_get", "ekv_rope_append", "ekv_tree_attention_workspace_size",
     "ekv_tree_attention", "ekv_key_weights", "ekv_evict_by_weight", "ekv_norm_rope_append", "ekv_seq_drop_blocks",
-    "ekv_seq_fork", "ekv_seq_own", "ekv_compact",
+    "ekv_seq_fork", "ekv_seq_own", "ekv_compact", "ekv_window_attention_workspace_size", "ekv_window_attention",
 ]
 NOALLOC_SCRATCH_BYTES = 16 << 20  # EKV_NOALLOC_SCRATCH_BYTES
 
@@ -204,6 +210,8 @@ def _load():
         "ekv_evict_by_weight": ([vp, C.POINTER(EvictParams), vp], C.c_int),
         "ekv_norm_rope_append": ([vp, vp, C.POINTER(HeadNormConfig), i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, C.c_int64, vp, vp,
                                   vp, C.c_int64, vp], C.c_int),
+        "ekv_window_attention_workspace_size": ([vp, C.POINTER(WindowParams)], C.c_size_t),
+        "ekv_window_attention": ([vp, C.POINTER(WindowParams), vp, C.c_int64, vp, vp, C.c_size_t, vp], C.c_int),
         "ekv_seq_drop_blocks": ([vp, i32, i32, i32], C.c_int),
         "ekv_seq_fork": ([vp, i32, pi32, pi32, pi32, vp], C.c_int),
         "ekv_seq_own": ([vp, i32, i32, i32, vp], C.c_int),
@@ -574,6 +582,41 @@ class Pool:
         if code:
             check(code, "ekv_evict_by_weight")
 
+
+    def window_params(self, *, layer, seq_ids, dst_pos, n_rows, src_row, max_rows, q_heads, scale, window=0, sinks=0,
+                      max_len=0) -> WindowParams:
+        """What ekv_window_attention is asked: rows as ekv_append's (dst_pos, n_rows, src_row), a window (0: none) and the number
+        of first slots that stay visible. max_len, the longest sequence of the call, is worth giving where the pool holds longer
+        ones that are not of the call."""
+        n = seq_ids.numel()
+        p = WindowParams(layer, n, q_heads, max_rows, window, sinks, scale, max_len, _index(seq_ids, n, "seq_ids"),
+                         _index(dst_pos, n, "dst_pos"), _index(n_rows, n, "n_rows"), _index(src_row, n, "src_row"))
+        p._keep = (seq_ids, dst_pos, n_rows, src_row)
+        p.heads = q_heads
+        return p
+
+    def window_attention_workspace_size(self, params: WindowParams) -> int:
+        return lib.ekv_window_attention_workspace_size(self.h, C.byref(params))
+
+    def window_attention(self, params: WindowParams, q, out, workspace=None, stream=None):
+        """ekv_window_attention: q bf16 [rows, q_heads, head_dim], its rows any distance apart (a slice of a projection), out
+        bf16 of q's shape, in one piece."""
+        heads, stride = _rows(q, self.head_dim, "q")
+        if heads != params.heads or q.dtype is not out.dtype or not out.is_contiguous() or out.shape != q.shape:
+            raise ValueError("q must have params' query heads, and out must be contiguous and of q's shape and type")
+        if q.dtype is not _bf16:
+            import torch
+            if q.dtype is not torch.bfloat16:
+                raise ValueError("q and out must be bf16")
+        ws_bytes = 0
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be in one piece")
+            ws_bytes = workspace.numel() * workspace.element_size()
+        code = lib.ekv_window_attention(self.h, C.byref(params), q.data_ptr(), stride, out.data_ptr(), _ptr(workspace), ws_bytes,
+                                        _stream(stream))
+        if code:
+            check(code, "ekv_window_attention")
 
     def compact(self, layer0, n_layers, seq_ids, slots, n_keep, stream=None):
         """ekv_compact: slot i of sequence seq_ids[b] gets the row of slot slots[b, i], for i below n_keep[b], in the layers from

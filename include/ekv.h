@@ -421,6 +421,36 @@ int ekv_tree_attention(ekv_pool *pool, const ekv_tree_params *p, const void *q, 
 int ekv_key_weights(ekv_pool *pool, const ekv_tree_params *p, const void *q, const float *lse, float *weights,
                     int64_t weight_stride, float decay, ekv_stream_t stream);
 
+typedef struct ekv_window_params {
+    int32_t layer;
+    int32_t n_batch;
+    int32_t q_heads;        /* a multiple of the pool's kv_heads                                      */
+    int32_t max_rows;       /* bounds every n_rows[i]                                                 */
+    int32_t window;         /* a row sees its own slot and the window - 1 before it; 0: every slot before it */
+    int32_t sinks;          /* first slots that every later row sees, whatever the window              */
+    float scale;
+    int32_t max_len;        /* longest sequence of the call where the caller knows it; 0: the longest live sequence of the pool
+                               stands for it. It picks how the work is shared; no result hangs on it     */
+    /* device arrays of n_batch entries, as ekv_append and ekv_rope_append take them                   */
+    const int32_t *seq_ids;
+    const int32_t *dst_pos; /* slot of the request's first row                                        */
+    const int32_t *n_rows;  /* its rows                                                               */
+    const int32_t *src_row; /* where they start in q and out                                          */
+} ekv_window_params;
+/* Bytes of workspace with which ekv_window_attention shares a few long requests over all SMs. */
+size_t ekv_window_attention_workspace_size(const ekv_pool *pool, const ekv_window_params *p);
+/* Causal attention of rows whose K and V are in the pages already: whole prompts, chunks of them, or one token each. Row r of request
+ * i (row src_row[i] + r of q and out) is the token at slot p = dst_pos[i] + r of sequence seq_ids[i]; it sees the slots k <= p with
+ * k > p - window or k < sinks. Where blocks behind the window were dropped (ekv_seq_drop_blocks), slots are those that are left. q is
+ * bf16 rows of q_heads x head_dim, q_stride elements from row to row (a multiple of 8; 0: rows are adjacent), out bf16 [rows][q_heads]
+ * [head_dim] and not q; query head h reads KV head h / (q_heads / kv_heads). Rows of a request that the pool cannot serve (unknown
+ * sequence, slots past its length) are 0 and reported through the pool's status; rows of out that belong to no request stay. What a
+ * row does not see does not reach it, whatever it holds. head_dim 64, 128 or 256. Q8_0 pools: calls of more than 16 rows of a KV head
+ * (max_rows * q_heads / kv_heads) compute in f16, and report (5) a query beyond its range, or a block whose scale is above 515 or not
+ * finite, which counts as 0. Without a workspace (or with a smaller one) units are not cut. Pointers 16-byte aligned. */
+int ekv_window_attention(ekv_pool *pool, const ekv_window_params *p, const void *q, int64_t q_stride, void *out, void *workspace,
+                         size_t workspace_bytes, ekv_stream_t stream);
+
 #define EKV_MAX_EVICT_TOKENS (1 << 19) /* longest sequence ekv_evict_by_weight takes; others may be longer */
 typedef struct ekv_evict_params {
     int32_t layer0, n_layers;   /* the layers [layer0, layer0 + n_layers)                              */
