@@ -119,7 +119,9 @@ struct WindowArgs {
     int32_t row_tiles;   // row tiles of one (request, KV head)
     int32_t split;       // CTAs take equal ranges of the call's tiles; 0: whole units
     int32_t cluster;     // (rows kernel, split == 0) CTAs of a unit
-    int2 *parts;         // [units] first and last CTA of each unit
+    int2 *parts;         // rows kernel: [units] first and last CTA of each unit
+    int4 *cuts;          // tile kernel: [CTAs] the unit that the CTA begins and others end (request * row tiles + row tile, KV head, last
+                         // CTA, 1), or 0
     float4 *ws_ml;       // [2 * CTAs][rows] maximum (log2 domain), sum of the rounded probabilities
     float *ws_o;         // [2 * CTAs][rows][D] unnormalised output
 };

@@ -566,17 +566,28 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
 // Rows of units that several CTAs took parts of: out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c, a warp for each row. Lanes look
 // at 32 parts' maxima and sums at once, so that the parts' rows are read without waiting for one another.
 constexpr int kMergeWarps = 8;
+constexpr int kMaxRangeRequests = 4096;  // (their places take 16 KB of the tile kernel's shared memory)
 
 template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) window_merge_kernel(const WindowArgs a, int unit_rows) {
     const int lane = threadIdx.x & 31, blocks = unit_rows / kMergeWarps;
     const int unit = blockIdx.x / blocks, r = (blockIdx.x - unit * blocks) * kMergeWarps + (threadIdx.x >> 5);
-    const int hk = a.pool.kv_heads, flat = unit / hk, g = unit - flat * hk, b = flat / a.row_tiles, rt = flat - b * a.row_tiles;
-    const int row = rt * unit_rows + r;
+    // a unit (rows kernel), or the one that CTA `unit` began (tile kernel)
+    const int hk = a.pool.kv_heads;
+    int flat = unit / hk, g = unit - flat * hk;
+    int2 part = make_int2(unit, 0);
     grid_wait();
+    if (a.cuts) {
+        const int4 cut = a.cuts[unit];
+        if (cut.w == 0) return;
+        flat = cut.x;
+        g = cut.y;
+        part.y = cut.z;
+    }
+    const int b = flat / a.row_tiles, row = (flat - b * a.row_tiles) * unit_rows + r;
     const WinReq rq = load_win_req(a, b, false);
     if (rq.seq < 0 || row >= rq.n * a.group) return;
-    const int2 part = a.parts[unit];
+    if (!a.cuts) part = a.parts[unit];
     if (part.x == part.y) return;
     constexpr int PER = (D + 127) / 128;  // float4 of a lane
     auto part_row = [&](int c) { return (2ll * c + (c == part.x ? 1 : 0)) * unit_rows + r; };
@@ -634,7 +645,8 @@ struct WsLayout {
 WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int sms) {
     const size_t ur = (size_t)unit_rows(p, rows), slots = 2 * (size_t)full_grid(p, rows, sms) * ur, row_tiles = ((size_t)rows + ur - 1) / ur;
     WsLayout w;
-    w.ml = ((size_t)n_batch * p.kv_heads * row_tiles * sizeof(int2) + 255) / 256 * 256;
+    const size_t joins = few_rows(rows) ? (size_t)n_batch * p.kv_heads * row_tiles * sizeof(int2) : slots / ur / 2 * sizeof(int4);
+    w.ml = (joins + 255) / 256 * 256;
     w.o = w.ml + slots * sizeof(float4);
     w.total = w.o + slots * p.head_dim * sizeof(float);
     return w;
@@ -656,7 +668,7 @@ int launch_dim(const WindowArgs &a, int rows, int grid, cudaStream_t s) {
     else if (rows <= 8) rc = q8 ? launch_rows<D, true, 1>(a, grid, s) : launch_rows<D, false, 1>(a, grid, s);
     else rc = q8 ? launch_rows<D, true, 2>(a, grid, s) : launch_rows<D, false, 2>(a, grid, s);
     if (rc || !a.split) return rc;
-    const int ur = unit_rows(a.pool, rows), units = a.n_batch * a.row_tiles * a.pool.kv_heads;
+    const int ur = unit_rows(a.pool, rows), units = a.cuts ? grid : a.n_batch * a.row_tiles * a.pool.kv_heads;
     return launch_after(window_merge_kernel<D>, units * (ur / kMergeWarps), kMergeWarps * 32, 0, s, a, ur);
 }
 
@@ -677,7 +689,7 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
     const int64_t tokens = std::min<int64_t>(a.max_rows, (ur + a.group - 1) / a.group + 1);
     auto tiles = [&](int64_t len) { return (std::min<int64_t>(len, (int64_t)a.window + tokens + a.sinks) + 16 + keys - 1) / keys; };
     const int64_t unit_tiles = tiles(max_len), most_tiles = tiles((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens) + 1;
-    const bool can_split = ws != nullptr && ws_bytes >= w.total && units * most_tiles < INT32_MAX;
+    const bool can_split = ws != nullptr && ws_bytes >= w.total && units * (most_tiles + 3) < INT32_MAX;
     a.split = 0;
     a.cluster = 1;
     int64_t grid;
@@ -695,12 +707,13 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
         }
         grid = a.split ? std::min<int64_t>(full, units * unit_tiles) : units * a.cluster;
     } else {
-        const int64_t whole = (units + full - 1) / full * unit_tiles, even = (units * unit_tiles + full - 1) / full;
-        a.split = can_split && even + 4 < whole;
-        grid = a.split ? std::min<int64_t>(full, units * unit_tiles) : std::min<int64_t>(full, units);
+        // Equal ranges of all tiles wherever there is room for the join; every CTA looks through the requests for its own.
+        a.split = can_split && a.n_batch <= kMaxRangeRequests;
+        grid = std::min<int64_t>(full, a.split ? units * (unit_tiles + 3) : units);
     }
     if (a.split) {
         a.parts = (int2 *)ws;
+        a.cuts = few_rows(rows) ? nullptr : (int4 *)ws;
         a.ws_ml = (float4 *)((uint8_t *)ws + w.ml);
         a.ws_o = (float *)((uint8_t *)ws + w.o);
     }

@@ -4,6 +4,8 @@
 // moves only when a score is 2^8 above it. S = Q K^T with both operands in shared memory and S in tensor memory, P in 16 bits over
 // S's own columns, O += P V with P read from tensor memory. P is rounded to bf16 (bf16 pages) and the row divided by the sum of the
 // rounded ones; over 8-bit pages operands are f16 (a value's int8 times its scale keeps 11 bits, P too).
+#include <type_traits>
+
 #include "ekv_window.cuh"
 
 namespace ekv {
@@ -15,47 +17,65 @@ using namespace window;
 
 constexpr int kTileRows = 128;  // rows of a row tile: the lanes of tensor memory
 
-// head_dim 64 and 128: two row tiles (slots) of a KV head share an SM and each K/V tile of 128 keys. While one slot's exponentials
-// run, the other's products do. head_dim 256: one row tile, 64 keys, two S tiles, as two outputs do not fit the tensor memory.
+// head_dim 64 and 128: two row tiles (slots) of a KV head share an SM and each K/V tile; head_dim 256: one, as two outputs do not fit the
+// tensor memory. A slot has two S tiles, so that the scores of the next tile are there when the exponentials of one are done.
 template <int D, bool Q8>
 struct WCfg {
     static constexpr int RT = D > 128 ? 1 : 2;
-    static constexpr int BN = D > 128 ? 64 : 128;     // keys per tile
-    static constexpr int NSB = D > 128 ? 2 : 1;       // S tiles of a row tile
-    static constexpr int NS = D == 64 ? 4 : 2;        // K and V stages
-    static constexpr int KPW = BN / 2;                // keys of a tile per softmax warp: two warps share 32 rows
+    static constexpr int BN = 64;                     // keys per tile
+    static constexpr int NSB = 2;                     // S tiles of a row tile
+    // K and V stages. 8-bit pages: one (two), as they are filled from the blocks as stored, which have room to be on their way instead
+    static constexpr int NS = D <= 128 ? (Q8 ? 2 : 4) : (Q8 ? 1 : 2);
+    static constexpr int NSF = NS > NSB ? NS : NSB;   // barriers of S: a tile's S may be done while S of the one before is not read
+    // a reference that is 2^LIMIT too low does not move: P and what is summed are floating point numbers, and only their range counts
+    static constexpr float LIMIT = Q8 ? 8.0f : 24.0f;
     static constexpr uint32_t SBO = 16 * D, LAYOUT = 2;
     static constexpr int KV_BYTES = BN * D * 2, Q_BYTES = kTileRows * D * 2;
-    static constexpr int RK = 8192 / D;               // Q8: keys of a piece of blocks as they are stored
-    static constexpr int NR = 3, RAW = RK * D + RK * (D / 32) * 2;
+    static constexpr int NR = D == 64 ? 6 : 5, RAW = BN * D + BN * (D / 32) * 2;  // Q8: tiles of K, of V as they are stored
     static constexpr int S_COL = 0, O_COL = BN * NSB, SLOT_COLS = 256, COLS = 512;
     static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_RAW = OFF_V + NS * KV_BYTES;
     static constexpr int OFF_SH = OFF_RAW + (Q8 ? (NR * RAW + 1023) / 1024 * 1024 : 0);
-    static constexpr int SHARED = 4096 + RT * 2 * kTileRows * 4, SMEM = OFF_SH + SHARED + 1024;
-    static constexpr int ROW_WARPS = 8 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = MMA_WARP + RT;
-    // bf16: K's feeder, V's feeder, and a warp that looks at V; Q8: one feeder, and converters
-    static constexpr int SCRUB_WARP = FEED_WARP + 2, CONV_WARP = FEED_WARP + 1, CONV_WARPS = RT == 1 ? 8 : 4;
-    static constexpr int THREADS = (Q8 ? CONV_WARP + CONV_WARPS : SCRUB_WARP + 1) * 32;
+    static constexpr int OFF_BAD = OFF_SH + 2048, SHARED = 2048 + (Q8 ? 0 : 8192), SMEM = OFF_SH + SHARED + 1024;
+    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = MMA_WARP + RT;
+    // bf16: K's feeder, V's feeder, and four warps that look at V; Q8: one feeder, and converters
+    static constexpr int SCRUB_WARP = FEED_WARP + 2, SCRUB_WARPS = 4, CONV_WARP = FEED_WARP + 1, CONV_WARPS = RT == 1 ? 8 : 4;
+    static constexpr int WARPS = Q8 ? CONV_WARP + CONV_WARPS : SCRUB_WARP + SCRUB_WARPS, THREADS = (WARPS + 3) / 4 * 128;
     static_assert(O_COL + D <= (RT == 2 ? SLOT_COLS : COLS) && SMEM <= 232448, "tensor memory, shared memory");
 };
 
-constexpr int kBadTiles = 10;  // a unit has at most ten tiles that only some of its rows see: three of 128 keys around 256 tokens'
-                               // own slots, three around the window's end, two around the first tokens, and the last one
-constexpr int kBadUnits = 8;   // V is looked at no more than the stages' tiles ahead of the rows
+constexpr int kBadChunks = 56;  // four for each tile that only some rows of a unit see: at most 13 for 256 tokens (five around their own
+                                // slots, six around the window's end, one each where the first tokens and the keys end)
+constexpr int kBadUnits = 16;   // V is looked at no more than the stages' four tiles ahead of the rows, by four warps that are no more than
+                                // that apart: the unit eight on may be made empty
+
+// Where a CTA's range of a split call begins, and where it ends (Units).
+struct RangeStart {
+    int b, g, rt;      // the unit that holds place x
+    uint32_t at;       // its first place
+    uint32_t x, hi, total;
+    int ctas;
+};
 
 struct WShared {
     uint64_t full_k[4], full_v[4];       // K, V of the stage are there
-    uint64_t raw_full[3], raw_empty[3];  // Q8: a piece has landed; is converted
-    uint64_t s_full[2][4];               // [slot][stage] S done
+    uint64_t raw_full[6], raw_empty[6];  // Q8: a tile of K or V has landed; is converted
+    uint64_t s_full[2][4];               // [slot][tile % NSF] S done
     uint64_t v_free[4];                  // both slots' P V done, and (bf16) the tile looked at
     uint64_t p_full[2][2];               // [slot][S tile] P written
     uint64_t q_ready[2], o_done[2], drained[2];
+    uint64_t turn[2];                    // [slot] it may issue its next group of products
     uint64_t v_clean[4];                 // V of a tile that only some rows see holds finite values
-    uint32_t bad[kBadUnits][kBadTiles][4];  // [unit % kBadUnits] its keys that did not
-    int bad_key[kBadUnits][kBadTiles], n_bad[kBadUnits];
     uint32_t tmem;
     int abort;
     RangeScratch range;
+    RangeStart start;
+};
+
+// [unit % kBadUnits] keys whose values are not all finite, 32 to an entry
+struct WBad {
+    int n[kBadUnits];
+    uint32_t keys[kBadUnits][kBadChunks];
+    int first[kBadUnits][kBadChunks];
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -64,24 +84,41 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Two warps that share 32 rows (64 threads of a named barrier). Both take the same way through these whatever else fails, so that
-// neither is left waiting.
-__device__ __forceinline__ bool pair_any(int id, bool x) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((uint32_t)x), "r"(id)
-        : "memory");
-    return r != 0;
+// One lane of a converged warp. With `lane == 0` in its place the compiler guards each tcgen05.mma by itself against lanes that
+// differ: 80 to 110 cycles an instruction, more than most of them run, so that issuing bound the kernel.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
 
-// Where a unit is, and its keys.
-struct Unit {
-    int b, g, row0, rows_all;  // request, KV head, first row, the request's rows
-    WinReq rq;
-};
+__device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at)
+                 : "memory");
+}
+
+// N x 32 columns of tensor memory, one wait for all of them.
+__device__ __forceinline__ void tmem_load32_nowait(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+}
+// (names the registers, so that none of them is read before it)
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 
 // The blocks' int8 rows as f16 values, rounded once; rows past `valid` are zero. Scales that leave the f16 range with them are
 // reported, their values 0.
@@ -89,7 +126,7 @@ template <int D, int ROWS, int THREADS>
 __device__ __forceinline__ bool convert_piece(const uint8_t *raw, uint8_t *dst, int row0, int valid, int thread) {
     constexpr int U = D / 16;
     bool fits = true;
-#pragma unroll 2
+#pragma unroll 4
     for (int e = thread; e < ROWS * U; e += THREADS) {
         // four 16-byte columns and two rows in every eight lanes, which then write to eight different columns of the swizzled rows
         const int rest = e >> 3, u = (rest % (U / 4)) * 4 + (e & 3), row = rest / (U / 4) * 2 + ((e >> 2) & 1);
@@ -118,388 +155,464 @@ __device__ __forceinline__ bool convert_piece(const uint8_t *raw, uint8_t *dst, 
     return fits;
 }
 
-template <int D, bool Q8>
-__global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(const WindowArgs a) {
-    using C = WCfg<D, Q8>;
-    constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, RT = C::RT, ROWS = RT * kTileRows, KPW = C::KPW;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    WShared &sh = *(WShared *)(smem + C::OFF_SH);
-    static_assert(sizeof(WShared) <= 4096, "barrier block");
-    float *const s_x = (float *)(smem + C::OFF_SH + 4096);  // [slot][warp of the pair][row]
-    volatile int *abort = &sh.abort;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = a.pool.kv_heads;
-
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) {
-            mbar_init(smem_addr(&sh.full_k[i]), Q8 ? C::CONV_WARPS : 1);
-            mbar_init(smem_addr(&sh.full_v[i]), Q8 ? C::CONV_WARPS : 1);
-            mbar_init(smem_addr(&sh.v_free[i]), Q8 ? RT : RT + 1);
-            mbar_init(smem_addr(&sh.v_clean[i]), 1);
-            for (int k = 0; k < RT; ++k) mbar_init(smem_addr(&sh.s_full[k][i]), 1);
-        }
-        for (int k = 0; k < RT; ++k) {
-            for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 8);
-            mbar_init(smem_addr(&sh.q_ready[k]), 8);
-            mbar_init(smem_addr(&sh.o_done[k]), 1);
-            mbar_init(smem_addr(&sh.drained[k]), 1);
-        }
-        for (int i = 0; Q8 && i < C::NR; ++i) {
-            mbar_init(smem_addr(&sh.raw_full[i]), 1);
-            mbar_init(smem_addr(&sh.raw_empty[i]), C::CONV_WARPS);
-        }
-        sh.abort = 0;
-        mbar_init_fence();
-    }
-    // request b's row tile t, without its tiles (units in the flat order of a split: request, row tile, KV head)
-    const int n_tiles_rt = a.row_tiles;
-    auto tiles_of = [&](const WinReq &r, int rt) {
-        const int row0 = rt * ROWS, rows_all = r.n * a.group;
-        if (row0 >= rows_all) return 0;
+// ---- the units of a CTA, in the same order in every warp ----
+// split: the range [x, hi) of all tiles in the order request, KV head, row tile, tile, where a unit counts kUnitCost tiles more for
+// what it costs beside them (query rows, the first tile's way, the end): without that the CTA of a long prompt's first rows took half
+// as long again. The row tiles of a head follow one another, so that a CTA finds most of a window in L2: with the heads innermost the
+// windows of all CTAs' heads did not fit it (8 prompts of 4096 tokens, a window of 1024: 980 us).
+// Else whole units, the longest (a request's last rows) first, back and forth over the CTAs.
+constexpr int kUnitCost = 3;
+template <int ROWS, int BN>
+struct Units {
+    int rt, round;     // row tile (split); rounds over the CTAs so far
+    uint32_t at, x, hi;
+    int b, g, row0;    // the unit: request, KV head, first row
+    int rq_of;         // the request that rq describes
+    WinReq rq;
+    int n_tiles, t0, t1;  // its tiles, and this CTA's
+    static __device__ __forceinline__ int tiles_of(const WindowArgs &a, const WinReq &r, int rt) {
+        const int row0 = rt * ROWS;
+        if (row0 >= r.n * a.group) return 0;
         const Span sp(a, r, row_token(a, row0), last_token(a, row0, ROWS, r.n));
         return max(1, (sp.keys + BN - 1) / BN);
-    };
-    grid_wait();
-    // (tensor memory between the two launch points: ekv_tree_tile.cu says why)
-    if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
-    tc_fence_before();
-    Range rg;
-    rg.b = 0;
-    rg.base = rg.lo = rg.hi = rg.total = 0;
-    rg.ctas = 0;
-    if (a.split) {
-        rg = find_range<C::THREADS>(
-            a.n_batch * n_tiles_rt, hk, sh.range,
-            [&](int i) {
-                const WinReq r = load_win_req(a, i / n_tiles_rt, false);
-                return Req{0, tiles_of(r, i % n_tiles_rt), 0};
-            },
-            [](const Req &r) { return r.n_prefix; });
-    } else {
-        __syncthreads();
     }
-    tc_fence_after();
-    const uint32_t tmem = sh.tmem;  // (there is a barrier in either branch)
-    grid_launch_next();
-
-    // ---- the units of this CTA, in the same order in every warp ----
-    // split: the tiles [rg.lo, rg.hi); else whole units, the longest (a request's last rows) first, back and forth over the CTAs
-    const int n_flat = a.n_batch * n_tiles_rt;
-    int flat = rg.b, round = 0;
-    uint32_t base = rg.base, x = rg.lo;
-    Unit u;
-    int t0 = 0, t1 = 0, n_tiles = 0;
-    // flat: request * row tiles + row tile (split), or the place in the order of units
-    auto next_unit = [&]() -> bool {
+    static __device__ __forceinline__ uint32_t cost_of(const WindowArgs &a, const WinReq &r, int rt) {
+        const int n = tiles_of(a, r, rt);
+        return n > 0 ? (uint32_t)(n + kUnitCost) : 0u;
+    }
+    __device__ __forceinline__ Units(const RangeStart &s) : rt(s.rt), round(0), at(s.at), x(s.x), hi(s.hi), b(s.b), g(s.g), rq_of(-1) {}
+    __device__ __forceinline__ bool next(const WindowArgs &a, bool report) {
+        const int hk = a.pool.kv_heads;
         if (a.split) {
-            for (; x < rg.hi && flat < n_flat; ++flat) {
-                u.b = flat / n_tiles_rt;
-                const int rt = flat - u.b * n_tiles_rt;
-                u.rq = load_win_req(a, u.b, false);
-                n_tiles = tiles_of(u.rq, rt);
-                const uint32_t span = (uint32_t)n_tiles * hk;
-                if (x >= base + span) {
-                    base += span;
+            while (x < hi && b < a.n_batch) {
+                if (rq_of != b) rq = load_win_req(a, b, false), rq_of = b;
+                n_tiles = tiles_of(a, rq, rt);
+                if (n_tiles == 0) {  // the request has no more rows: its next head, or the next request
+                    rt = 0;
+                    if (++g == hk || rq.n == 0) {
+                        g = 0;
+                        ++b;
+                    }
                     continue;
                 }
-                u.g = (int)((x - base) / (uint32_t)n_tiles);
-                t0 = (int)(x - base) - u.g * n_tiles;
-                t1 = min(n_tiles, t0 + (int)(rg.hi - x));
-                u.row0 = rt * ROWS;
-                u.rows_all = u.rq.n * a.group;
-                x += t1 - t0;
-                return true;
+                const uint32_t cost = (uint32_t)(n_tiles + kUnitCost);
+                if (x >= at + cost) {
+                    at += cost;
+                    ++rt;
+                    continue;
+                }
+                const int from = (int)(x - at), to = (int)min(cost, from + (hi - x));
+                x += to - from;
+                t0 = max(0, from - kUnitCost);
+                t1 = to - kUnitCost;
+                row0 = rt * ROWS;
+                if (t1 > t0) return true;  // (not only what a unit costs beside its tiles)
             }
             return false;
         }
-        const long long all = (long long)n_flat * hk;
+        const int all = a.n_batch * a.row_tiles * hk;  // (below 2^31: checked at the launch)
         for (;;) {
-            const long long at = (long long)round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            if ((long long)round * gridDim.x >= all) return false;
+            const long long from = (long long)round * gridDim.x, place = from + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            if (from >= all) return false;
             ++round;
-            if (at >= all) continue;
-            const int rest = (int)(at / hk), rt = n_tiles_rt - 1 - rest / a.n_batch;
-            u.g = (int)(at - (long long)rest * hk);
-            u.b = rest - rest / a.n_batch * a.n_batch;
-            u.rq = load_win_req(a, u.b, warp == 0 && rt == 0 && u.g == 0 && lane == 0);
-            n_tiles = tiles_of(u.rq, rt);
+            if (place >= all) continue;
+            const int rest = (int)place / hk, k = rest / a.n_batch;
+            rt = a.row_tiles - 1 - k;
+            g = (int)place - rest * hk;
+            b = rest - k * a.n_batch;
+            rq = load_win_req(a, b, report && rt == 0 && g == 0);
+            n_tiles = tiles_of(a, rq, rt);
             if (n_tiles == 0) continue;
-            u.row0 = rt * ROWS;
-            u.rows_all = u.rq.n * a.group;
+            row0 = rt * ROWS;
             t0 = 0;
             t1 = n_tiles;
             return true;
         }
-    };
-    if (a.split && blockIdx.x == 0)  // (whoever has a request's unit does not report it: the first CTA looks at all)
-        for (int b = threadIdx.x; b < a.n_batch; b += C::THREADS) load_win_req(a, b, true);
+    }
+    __device__ __forceinline__ int rows(const WindowArgs &a) const { return min(ROWS, rq.n * a.group - row0); }
+    __device__ __forceinline__ Span span(const WindowArgs &a) const {
+        return Span(a, rq, row_token(a, row0), last_token(a, row0, ROWS, rq.n));
+    }
+};
 
-    bool ok = true, fits = true;
-    int it = 0;       // tiles of this CTA so far
-    int unit_no = 0;  // units so far
-    int raw_it = 0;   // Q8: pieces so far
-    int live_it[1] = {0};  // tiles so far that this slot had rows for (products and softmax)
-    int live_units = 0;
-    uint32_t clean_phase = 0;  // v_clean, a bit per stage
-
-    while (next_unit()) {
-        const int n = t1 - t0;
-        const Span sp(a, u.rq, row_token(a, u.row0), last_token(a, u.row0, ROWS, u.rq.n));
-        const int rows_here = min(ROWS, u.rows_all - u.row0);
-        auto unit_sees = [&](int j) { return sp.all_see(a, j * BN, BN); };
-
-        if (warp >= C::FEED_WARP && warp < (Q8 ? C::CONV_WARP : C::SCRUB_WARP)) {
-            // ---- feeders ----
-            auto want = [](int, int) {};
-            auto block = [&](int e) { return lookup_block(a.pool, u.rq.seq, e); };
-            const int64_t v_from_k = (int64_t)hk * a.pool.tile_bytes;
-            if constexpr (!Q8) {
-                const bool is_v = warp != C::FEED_WARP;
-                Run next = find_run<BN>(a, sp, u.g, t0 * BN, lane, want, block);
-                for (int j = t0; j < t1; ++j, ++it) {
-                    const int st = it % NS, par = (it / NS) & 1;
-                    const Run r = next;
-                    if (j + 1 < t1) next = find_run<BN>(a, sp, u.g, (j + 1) * BN, lane, want, block);
-                    if (it >= NS) {
-                        if (is_v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), par ^ 1, abort);
-#pragma unroll
-                        for (int k = 0; k < RT; ++k)
-                            if (!is_v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][st]), par ^ 1, abort);
-                    }
-                    if (!ok) {
-                        *abort = 1;
-                        continue;
-                    }
-                    const uint32_t dst = smem_addr(smem + (is_v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES);
-                    const uint32_t bar = smem_addr(is_v ? &sh.full_v[st] : &sh.full_k[st]);
-                    const uint32_t bytes = r.src ? (uint32_t)(r.n * 2 * D) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, all);
-                    __syncwarp();
-                    if (r.src) bulk_g2s(dst + r.row * 2 * D, r.src + (is_v ? v_from_k : 0) + r.rib * 2 * D, bytes, bar);
-                }
-            } else {
-                constexpr int PIECES = BN / C::RK;  // of K, then of V
-                for (int j = t0; j < t1; ++j)
-                    for (int pc = 0; pc < 2 * PIECES; ++pc, ++raw_it) {
-                        const bool is_v = pc >= PIECES;
-                        const int key = j * BN + (pc - (is_v ? PIECES : 0)) * C::RK, rs = raw_it % C::NR;
-                        const Run r = find_run<C::RK>(a, sp, u.g, key, lane, want, block);
-                        if (raw_it >= C::NR) ok = ok && warp_wait(smem_addr(&sh.raw_empty[rs]), (raw_it / C::NR - 1) & 1, abort);
-                        if (!ok) {
-                            *abort = 1;
-                            continue;
-                        }
-                        const uint32_t dst = smem_addr(smem + C::OFF_RAW + rs * C::RAW), bar = smem_addr(&sh.raw_full[rs]);
-                        const uint32_t bytes = r.src ? (uint32_t)(r.n * (D + D / 16)) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
-                        if (lane == 0) mbar_arrive_expect_tx(bar, all);
-                        __syncwarp();
-                        if (!r.src) continue;
-                        const uint8_t *src = r.src + (is_v ? v_from_k : 0);
-                        bulk_g2s(dst + r.row * D, src + r.rib * D, (uint32_t)(r.n * D), bar);
-                        bulk_g2s(dst + C::RK * D + r.row * (D / 16), src + (int64_t)a.pool.block_tokens * D + r.rib * (D / 16),
-                                 (uint32_t)(r.n * (D / 16)), bar);
-                    }
-            }
-        } else if (Q8 && warp >= C::CONV_WARP) {
-            // ---- converters ----
-            constexpr int PIECES = BN / C::RK;
-            const int thread = threadIdx.x - C::CONV_WARP * 32;
-            for (int j = t0; j < t1; ++j, ++it) {
+template <int D, bool Q8>
+__device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u) {
+    using C = WCfg<D, Q8>;
+    constexpr int BN = C::BN, NS = C::NS, RT = C::RT;
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = a.pool.kv_heads;
+    bool ok = true;
+    [[maybe_unused]] int it = 0, raw_it = 0;  // tiles, and (Q8) pieces, of this CTA so far
+    while (u.next(a, false)) {
+        const Span sp = u.span(a);
+        // ---- feeders ----
+        auto want = [](int, int) {};
+        auto block = [&](int e) { return lookup_block(a.pool, u.rq.seq, e); };
+        const int64_t v_from_k = (int64_t)hk * a.pool.tile_bytes;
+        if constexpr (!Q8) {
+            const bool is_v = warp != C::FEED_WARP;
+            Run next = find_run<BN>(a, sp, u.g, u.t0 * BN, lane, want, block);
+            for (int j = u.t0; j < u.t1; ++j, ++it) {
                 const int st = it % NS, par = (it / NS) & 1;
-                for (int pc = 0; pc < 2 * PIECES; ++pc, ++raw_it) {
-                    const bool is_v = pc >= PIECES;
-                    const int row0 = (pc - (is_v ? PIECES : 0)) * C::RK, rs = raw_it % C::NR;
-                    if (row0 == 0 && it >= NS) {  // the stage is free
-                        if (is_v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), par ^ 1, abort);
+                const Run r = next;
+                if (j + 1 < u.t1) next = find_run<BN>(a, sp, u.g, (j + 1) * BN, lane, want, block);
+                if (it >= NS) {
+                    if (is_v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), par ^ 1, abort);
 #pragma unroll
-                        for (int k = 0; k < RT; ++k)
-                            if (!is_v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][st]), par ^ 1, abort);
-                    }
-                    ok = ok && warp_wait(smem_addr(&sh.raw_full[rs]), (raw_it / C::NR) & 1, abort);
-                    if (!ok) {
-                        *abort = 1;
-                        continue;
-                    }
-                    fits &= convert_piece<D, C::RK, C::CONV_WARPS * 32>(smem + C::OFF_RAW + rs * C::RAW, smem + (is_v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES,
-                                                                       row0, sp.keys - j * BN - row0, thread);
-                    fence_proxy_async();  // read by the tensor core; the piece's next contents come through the copy engine
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_addr(&sh.raw_empty[rs]));
-                        if (row0 + C::RK == BN) mbar_arrive(smem_addr(is_v ? &sh.full_v[st] : &sh.full_k[st]));
-                    }
+                    for (int k = 0; k < RT; ++k)
+                        if (!is_v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][(it - NS) % C::NSF]), ((it - NS) / C::NSF) & 1, abort);
                 }
-            }
-        } else if (!Q8 && warp == C::SCRUB_WARP) {
-            // ---- values that are not finite leave the tiles that only some rows see: 0 * inf would reach the others ----
-            const int ub = unit_no % kBadUnits;
-            if (lane == 0) sh.n_bad[ub] = 0;
-            for (int j = t0; j < t1; ++j, ++it) {
-                // (every tile is waited for and let go, whether it is looked at or not: a barrier's parity tells two phases apart)
-                const int st = it % NS;
-                ok = ok && warp_wait(smem_addr(&sh.full_v[st]), (it / NS) & 1, abort);
                 if (!ok) {
                     *abort = 1;
                     continue;
                 }
-                if (unit_sees(j)) {
-                    if (lane == 0) mbar_arrive(smem_addr(&sh.v_free[st]));
-                    continue;
-                }
-                uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
-                constexpr int U = D / 8;
-                const int valid = min(BN, sp.keys - j * BN);
-                uint32_t bad[4] = {};
-                for (int e = lane; e < BN * U; e += 32) {
-                    const int r = e / U;
-                    uint4 *at = (uint4 *)(vt + bf16_off<D>(r, (e % U) * 8));
-                    if (r >= valid) {
-                        *at = make_uint4(0, 0, 0, 0);
+                const uint32_t dst = smem_addr(smem + (is_v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES);
+                const uint32_t bar = smem_addr(is_v ? &sh.full_v[st] : &sh.full_k[st]);
+                const uint32_t bytes = r.src ? (uint32_t)(r.n * 2 * D) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
+                if (lane == 0) mbar_arrive_expect_tx(bar, all);
+                __syncwarp();
+                if (r.src) bulk_g2s(dst + r.row * 2 * D, r.src + (is_v ? v_from_k : 0) + r.rib * 2 * D, bytes, bar);
+            }
+        } else {
+            Run next = find_run<BN>(a, sp, u.g, u.t0 * BN, lane, want, block);
+            for (int j = u.t0; j < u.t1; ++j) {
+                const Run r = next;
+                if (j + 1 < u.t1) next = find_run<BN>(a, sp, u.g, (j + 1) * BN, lane, want, block);
+                for (int v = 0; v < 2; ++v, ++raw_it) {  // K, then V
+                    const int rs = raw_it % C::NR;
+                    if (raw_it >= C::NR) ok = ok && warp_wait(smem_addr(&sh.raw_empty[rs]), (raw_it / C::NR - 1) & 1, abort);
+                    if (!ok) {
+                        *abort = 1;
                         continue;
                     }
-                    const uint4 v = *at;
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    const uint32_t dst = smem_addr(smem + C::OFF_RAW + rs * C::RAW), bar = smem_addr(&sh.raw_full[rs]);
+                    const uint32_t bytes = r.src ? (uint32_t)(r.n * (D + D / 16)) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, all);
+                    __syncwarp();
+                    if (!r.src) continue;
+                    const uint8_t *src = r.src + (v ? v_from_k : 0);
+                    bulk_g2s(dst + r.row * D, src + r.rib * D, (uint32_t)(r.n * D), bar);
+                    bulk_g2s(dst + BN * D + r.row * (D / 16), src + (int64_t)a.pool.block_tokens * D + r.rib * (D / 16),
+                             (uint32_t)(r.n * (D / 16)), bar);
+                }
+            }
+        }
+    }
+    if (!ok && lane == 0) {
+        // leave no copy writing this CTA's shared memory
+        for (int i = 0; i < (Q8 ? C::NR : NS); ++i) {
+            const uint32_t bar = smem_addr(Q8 ? &sh.raw_full[i] : warp == C::FEED_WARP ? &sh.full_k[i] : &sh.full_v[i]);
+            mbar_wait_drain(bar, 0, kWait / 64);
+            mbar_wait_drain(bar, 1, kWait / 64);
+        }
+    }
+    return ok;
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ bool convert(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u) {
+    using C = WCfg<D, Q8>;
+    constexpr int BN = C::BN, NS = C::NS, RT = C::RT;
+    volatile int *abort = &sh.abort;
+    const int lane = threadIdx.x & 31;
+    bool ok = true;
+    int it = 0;  // tiles of this CTA so far
+    int raw_it = 0;  // pieces so far
+    bool fits = true;
+    while (u.next(a, false)) {
+        const Span sp = u.span(a);
+        // ---- converters ----
+        const int thread = threadIdx.x - C::CONV_WARP * 32;
+        for (int j = u.t0; j < u.t1; ++j, ++it) {
+            const int st = it % NS;
+#pragma unroll 1
+            for (int v = 0; v < 2; ++v, ++raw_it) {
+                const int rs = raw_it % C::NR;
+                if (it >= NS) {  // the stage is free
+                    if (v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), (it / NS - 1) & 1, abort);
+#pragma unroll
+                    for (int k = 0; k < RT; ++k)
+                        if (!v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][(it - NS) % C::NSF]), ((it - NS) / C::NSF) & 1, abort);
+                }
+                ok = ok && warp_wait(smem_addr(&sh.raw_full[rs]), (raw_it / C::NR) & 1, abort);
+                if (!ok) {
+                    *abort = 1;
+                    continue;
+                }
+                fits &= convert_piece<D, BN, C::CONV_WARPS * 32>(smem + C::OFF_RAW + rs * C::RAW, smem + (v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES, 0,
+                                                                sp.keys - j * BN, thread);
+                fence_proxy_async();  // read by the tensor core; the next blocks come through the copy engine
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_addr(&sh.raw_empty[rs]));
+                    mbar_arrive(smem_addr(v ? &sh.full_v[st] : &sh.full_k[st]));
+                }
+            }
+        }
+    }
+    if (!__all_sync(0xffffffffu, fits) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, 0, 15);
+    return ok;
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ bool look_at_values(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u) {
+    using C = WCfg<D, Q8>;
+    constexpr int BN = C::BN, NS = C::NS;
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool ok = true;
+    int it = 0;  // tiles of this CTA so far
+    int unit_no = 0;
+    while (u.next(a, false)) {
+        const Span sp = u.span(a);
+        auto unit_sees = [&](int j) { return sp.all_see(a, j * BN, BN); };
+        // ---- values that are not finite leave the tiles that only some rows see: 0 * inf would reach the others ----
+        WBad &found = *(WBad *)(smem + C::OFF_BAD);
+        const int ub = unit_no % kBadUnits;
+        if (warp == C::SCRUB_WARP && lane == 0) found.n[(unit_no + kBadUnits / 2) % kBadUnits] = 0;
+        for (int j = u.t0; j < u.t1; ++j, ++it) {
+            // (every tile is waited for and let go, whether it is looked at or not: a barrier's parity tells two phases apart)
+            const int st = it % NS;
+            ok = ok && warp_wait(smem_addr(&sh.full_v[st]), (it / NS) & 1, abort);
+            if (!ok) {
+                *abort = 1;
+                continue;
+            }
+            if (unit_sees(j)) {
+                if (lane == 0) mbar_arrive(smem_addr(&sh.v_free[st]));
+                continue;
+            }
+            // a warp takes BN / 4 keys, a lane up to eight units of them at a time
+            uint8_t *vt = smem + C::OFF_V + st * C::KV_BYTES;
+            constexpr int U = D / 8, KEYS = BN / C::SCRUB_WARPS, PER = KEYS * U / 32, STEP = PER < 8 ? PER : 8;
+            static_assert(PER % STEP == 0 && KEYS <= 32 && KEYS * U % 32 == 0, "whole steps inside the warp's keys");
+            const int first = (warp - C::SCRUB_WARP) * KEYS, valid = min(BN, sp.keys - j * BN);
+            uint32_t bad = 0;
+#pragma unroll 1
+            for (int e0 = 0; e0 < PER; e0 += STEP) {
+                uint4 v[STEP];
+#pragma unroll
+                for (int e = 0; e < STEP; ++e) {
+                    const int i = (e0 + e) * 32 + lane;
+                    v[e] = *(const uint4 *)(vt + bf16_off<D>(first + i / U, (i % U) * 8));
+                }
+#pragma unroll
+                for (int e = 0; e < STEP; ++e) {
+                    const int i = (e0 + e) * 32 + lane, r = first + i / U;
+                    uint32_t w[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
                     bool any = false;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) any = any || (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
-                    if (!any) continue;
+                    if (r < valid && !any) continue;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
-                        if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
-                        if (r >> 5 == k) bad[k] |= 1u << (r & 31);
+                        if ((w[k] & 0x7f80u) == 0x7f80u || r >= valid) w[k] &= 0xffff0000u;
+                        if ((w[k] & 0x7f800000u) == 0x7f800000u || r >= valid) w[k] &= 0xffffu;
                     }
-                    *at = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bad[k] = __reduce_or_sync(0xffffffffu, bad[k]);
-                if ((bad[0] | bad[1] | bad[2] | bad[3]) && lane == 0 && sh.n_bad[ub] < kBadTiles) {
-                    const int i = sh.n_bad[ub];
-                    for (int k = 0; k < 4; ++k) sh.bad[ub][i][k] = bad[k];
-                    sh.bad_key[ub][i] = j * BN;
-                    sh.n_bad[ub] = i + 1;
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_addr(&sh.v_clean[st]));
-                    mbar_arrive(smem_addr(&sh.v_free[st]));
+                    if (r < valid) bad |= 1u << (r - first);
+                    *(uint4 *)(vt + bf16_off<D>(r, (i % U) * 8)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-        } else if (warp >= C::MMA_WARP) {
-            // ---- products ----
-            const int slot = warp - C::MMA_WARP;
-            const bool live = rows_here > slot * kTileRows && u.rq.seq >= 0;
+            bad = __reduce_or_sync(0xffffffffu, bad);
+            if (bad && lane == 0) {
+                const int i = atomicAdd(&found.n[ub], 1);
+                if (i < kBadChunks) {
+                    found.keys[ub][i] = bad;
+                    found.first[ub][i] = j * BN + first;
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
             if (lane == 0) {
-                const uint32_t id_s = idesc_f16(!Q8, false, BN), id_o = idesc_f16(!Q8, true, D);
-                const uint32_t q_addr = smem_addr(smem) + slot * C::Q_BYTES, k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
-                const uint32_t cols = tmem + (uint32_t)(slot * C::SLOT_COLS);
-                auto issue_s = [&](int i) {  // tile i of the unit
-                    const int at = it + i, st = at % NS;
-                    if (!mbar_wait(smem_addr(&sh.full_k[st]), (at / NS) & 1, abort, kWait)) return false;
-                    if (!live) {
-                        mbar_arrive(smem_addr(&sh.s_full[slot][st]));
-                        return true;
-                    }
-                    tc_fence_after();
-                    const uint32_t s_at = cols + (uint32_t)(C::S_COL + ((live_it[0] + i) % NSB) * BN);
-                    const uint64_t qa = sdesc(q_addr, 16, C::SBO, C::LAYOUT), kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
-#pragma unroll
-                    for (int s4 = 0; s4 < D / 64; ++s4) {
-                        uint64_t av[4], bv[4];
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
-                            bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
-                        }
-                        mma_ss_x4<false>(s_at, av, bv, id_s, s4 > 0 ? 1u : 0u);
-                    }
-                    mma_commit(smem_addr(&sh.s_full[slot][st]));
-                    return true;
-                };
-                auto issue_pv = [&](int i) {
-                    const int at = it + i, st = at % NS;
-                    if (live && !mbar_wait(smem_addr(&sh.p_full[slot][(live_it[0] + i) % NSB]), ((live_it[0] + i) / NSB) & 1, abort, kWait)) return false;
-                    if (!mbar_wait(smem_addr(&sh.full_v[st]), (at / NS) & 1, abort, kWait)) return false;
-                    if (!Q8 && !unit_sees(t0 + i)) {
-                        if (!mbar_wait(smem_addr(&sh.v_clean[st]), (clean_phase >> st) & 1u, abort, kWait)) return false;
-                        clean_phase ^= 1u << st;
-                    }
-                    if (!live) {
-                        mbar_arrive(smem_addr(&sh.v_free[st]));
-                        return true;
-                    }
-                    tc_fence_after();
-                    const uint32_t p_at = cols + (uint32_t)(C::S_COL + ((live_it[0] + i) % NSB) * BN);
-                    const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
-#pragma unroll
-                    for (int s4 = 0; s4 < BN / 64; ++s4) {
-                        uint32_t av[4];
-                        uint64_t bv[4];
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            const int k = 4 * s4 + s;  // 16 keys; P of a warp's keys starts where their S did
-                            av[s] = p_at + (uint32_t)(16 * k / KPW * KPW + 16 * k % KPW / 2);
-                            bv[s] = vb + ((uint32_t)(k * 2 * C::SBO) >> 4);
-                        }
-                        mma_ts_x4<false>(cols + C::O_COL, av, bv, id_o, i > 0 || s4 > 0 ? 1u : 0u);
-                    }
-                    mma_commit(smem_addr(&sh.v_free[st]));
-                    return true;
-                };
-                // S(j + NSB) goes over P(j), whose product is issued before it: the tensor pipe runs them in order
-                if (live) ok = ok && mbar_wait(smem_addr(&sh.q_ready[slot]), live_units & 1, abort, kWait);
-                for (int i = 0; ok && i < min(NSB, n); ++i) ok = issue_s(i);
-                for (int i = 0; ok && i < n; ++i) {
-                    ok = issue_pv(i);
-                    if (ok && i + NSB < n) ok = issue_s(i + NSB);
-                }
-                if (live) mma_commit(smem_addr(&sh.o_done[slot]));
-                if (!ok) *abort = 1;
+                mbar_arrive(smem_addr(&sh.v_clean[st]));
+                mbar_arrive(smem_addr(&sh.v_free[st]));
             }
-            it += n;
-            if (live) {
-                live_it[0] += n;
-                ++live_units;
+        }
+        ++unit_no;
+    }
+    return ok;
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ bool products(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u, uint32_t tmem) {
+    using C = WCfg<D, Q8>;
+    constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, RT = C::RT;
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool ok = true;
+    int it = 0, live_units = 0;  // tiles of this CTA so far; units that this slot had rows for
+    [[maybe_unused]] int turns = 0;
+    [[maybe_unused]] uint32_t clean_phase = 0;  // v_clean, a bit per stage
+    while (u.next(a, false)) {
+        const int n = u.t1 - u.t0;
+        const Span sp = u.span(a);
+        auto unit_sees = [&](int j) { return sp.all_see(a, j * BN, BN); };
+        // ---- products ----
+        const int slot = warp - C::MMA_WARP;
+        const bool live = u.rows(a) > slot * kTileRows && u.rq.seq >= 0;
+        const uint32_t id_s = idesc_f16(!Q8, false, BN), id_o = idesc_f16(!Q8, true, D);
+        const uint32_t q_addr = smem_addr(smem) + slot * C::Q_BYTES, k_addr = smem_addr(smem + C::OFF_K), v_addr = smem_addr(smem + C::OFF_V);
+        const uint32_t cols = tmem + (uint32_t)(slot * C::SLOT_COLS);
+        // A group is P V of a tile and S of the one NSB after it, which goes over that P: the tensor pipe runs them in order. Each
+        // group is waited for as a whole, and the slots' groups take turns: with both threads issuing as they could, the pipe
+        // took their products alternately, so that both slots had their S at the same time and then waited for the
+        // exponential unit together (5800 cycles a tile).
+        auto ready_s = [&](int i) { return warp_wait(smem_addr(&sh.full_k[(it + i) % NS]), ((it + i) / NS) & 1, abort); };
+        auto issue_s = [&](int i) {
+            const int at = it + i, st = at % NS;
+            if (!live) {
+                mbar_arrive(smem_addr(&sh.s_full[slot][at % C::NSF]));
+                return;
             }
-        } else {
-            // ---- softmax: thread = row and half of the tile's keys ----
-            const int slot = warp >> 3, quarter = warp & 3, half = (warp >> 2) & 1, r = quarter * 32 + lane;
-            const int row = u.row0 + slot * kTileRows + r, t = row_token(a, row), id = 1 + slot * 4 + quarter;
-            const bool slot_live = rows_here > slot * kTileRows && u.rq.seq >= 0;
-            const bool on = row < u.rows_all;
-            const int64_t src_row = (int64_t)a.src_row[u.b] + t;
-            const int head = u.g * a.group + row - t * a.group;
-            if (!slot_live) {
-                for (int i = 0; i < n; ++i, ++it) ok = ok && warp_wait(smem_addr(&sh.s_full[slot][it % NS]), (it / NS) & 1, abort);
-                if (!ok) *abort = 1;
-                if (u.rq.seq < 0 && on && t0 == 0) {  // a refused request's rows are 0
-                    for (int c = half * D / 2; c < (half + 1) * D / 2; c += 8)
-                        *(uint4 *)(a.out + (src_row * a.q_heads + head) * D + c) = make_uint4(0, 0, 0, 0);
+            const uint32_t s_at = cols + (uint32_t)(C::S_COL + (at % NSB) * BN);
+            const uint64_t qa = sdesc(q_addr, 16, C::SBO, C::LAYOUT), kb = sdesc(k_addr + st * C::KV_BYTES, 16, C::SBO, C::LAYOUT);
+#pragma unroll
+            for (int s4 = 0; s4 < D / 64; ++s4) {
+                uint64_t av[4], bv[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    av[s] = qa + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
+                    bv[s] = kb + ((uint32_t)(s4 * 1024 + s * 32) >> 4);
                 }
-                ++unit_no;
+                mma_ss_x4<false>(s_at, av, bv, id_s, s4 > 0 ? 1u : 0u);
+            }
+            mma_commit(smem_addr(&sh.s_full[slot][at % C::NSF]));
+        };
+        auto ready_pv = [&](int i) {
+            const int at = it + i, st = at % NS;
+            if (!warp_wait(smem_addr(&sh.full_v[st]), (at / NS) & 1, abort)) return false;
+            if (!Q8 && !unit_sees(u.t0 + i)) {
+                if (!warp_wait(smem_addr(&sh.v_clean[st]), (clean_phase >> st) & 1u, abort)) return false;
+                clean_phase ^= 1u << st;
+            }
+            return warp_wait(smem_addr(&sh.p_full[slot][at % NSB]), (at / NSB) & 1, abort);
+        };
+        auto issue_pv = [&](int i) {
+            const int at = it + i, st = at % NS;
+            if (!live) {
+                mbar_arrive(smem_addr(&sh.v_free[st]));
+                return;
+            }
+            const uint32_t p_at = cols + (uint32_t)(C::S_COL + (at % NSB) * BN);
+            const uint64_t vb = sdesc(v_addr + st * C::KV_BYTES, 1024, C::SBO, C::LAYOUT);
+#pragma unroll
+            for (int s4 = 0; s4 < BN / 64; ++s4) {
+                uint32_t av[4];
+                uint64_t bv[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int k = 4 * s4 + s;  // 16 keys
+                    av[s] = p_at + (uint32_t)(8 * k);
+                    bv[s] = vb + ((uint32_t)(k * 2 * C::SBO) >> 4);
+                }
+                mma_ts_x4<false>(cols + C::O_COL, av, bv, id_o, i > 0 || s4 > 0 ? 1u : 0u);
+            }
+            mma_commit(smem_addr(&sh.v_free[st]));
+        };
+        if (live) ok = ok && warp_wait(smem_addr(&sh.q_ready[slot]), live_units & 1, abort);
+        for (int i = -NSB; ok && i < n; ++i) {
+            const bool pv = i >= 0, next_s = i + NSB < n;
+            if (RT == 1) {
+                // (K may come from a stage whose V waits for this P V)
+                if (pv) ok = ready_pv(i);
+                tc_fence_after();
+                if (ok && pv && elect_one()) issue_pv(i);
+                __syncwarp();
+                if (next_s) ok = ok && ready_s(i + NSB);
+                tc_fence_after();
+                if (ok && next_s && elect_one()) issue_s(i + NSB);
+                __syncwarp();
                 continue;
             }
-            const uint32_t lane_base = ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * C::SLOT_COLS);
-            const bool live = __any_sync(0xffffffffu, on);  // (a pair's two warps have the same rows)
-            float *const mine = s_x + (slot * 2 + half) * kTileRows, *const other = s_x + (slot * 2 + (half ^ 1)) * kTileRows;
-            {
-                // query rows: this warp those of its lane quarter's half
-                constexpr int U = D / 8;
-                uint8_t *sq = smem + slot * C::Q_BYTES;
-                const long long at = (long long)src_row * a.q_stride + (long long)head * D;
-                const uint32_t have = __ballot_sync(0xffffffffu, on);
+            if (next_s) ok = ready_s(i + NSB);
+            if (pv) ok = ok && ready_pv(i);
+            // (the first slot's first turn is free)
+            ok = ok && warp_wait(smem_addr(&sh.turn[slot]), (turns + (slot == 0 ? 1 : 0)) & 1, abort);
+            ++turns;
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                if (pv) issue_pv(i);
+                if (next_s) issue_s(i + NSB);
+                mbar_arrive(smem_addr(&sh.turn[slot ^ 1]));
+            }
+            __syncwarp();
+        }
+        if (live && elect_one()) mma_commit(smem_addr(&sh.o_done[slot]));
+        __syncwarp();
+        if (!ok) *abort = 1;
+        it += n;
+        if (live) ++live_units;
+    }
+    // no product is left that uses the tensor memory
+    if (elect_one()) mma_commit(smem_addr(&sh.drained[warp - C::MMA_WARP]));
+    __syncwarp();
+    mbar_wait_drain(smem_addr(&sh.drained[warp - C::MMA_WARP]), 0, kWait);
+    return ok;
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u, uint32_t tmem, int ctas, uint32_t total) {
+    using C = WCfg<D, Q8>;
+    constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, RT = C::RT, ROWS = RT * kTileRows;
+    volatile int *abort = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // thread = row: all keys of a tile are its own, so that rows need nothing from one another
+    const int slot = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * C::SLOT_COLS);
+    bool ok = true, fits = true;
+    int it = 0, unit_no = 0;  // tiles and units of this CTA so far
+    int live_units = 0;       // units that this slot had rows for
+    int4 cut = make_int4(0, 0, 0, 0);  // the unit that this CTA begins and others end: row tile, KV head, last CTA
+    while (u.next(a, warp == 0 && lane == 0)) {
+        const int n = u.t1 - u.t0;
+        const Span sp = u.span(a);
+        auto unit_sees = [&](int j) { return sp.all_see(a, j * BN, BN); };
+        const int row = u.row0 + slot * kTileRows + r, t = row_token(a, row);
+        const bool slot_live = u.rows(a) > slot * kTileRows && u.rq.seq >= 0;
+        const bool on = row < u.rq.n * a.group;
+        const long long out_at = (((int64_t)a.src_row[u.b] + t) * a.q_heads + u.g * a.group + row - t * a.group) * D;
+        if (!slot_live) {
+            // in step with the tiles all the same: a barrier's parity tells two phases apart, so nobody may fall behind
+            for (int i = 0; i < n; ++i, ++it) {
+                ok = ok && warp_wait(smem_addr(&sh.s_full[slot][it % C::NSF]), (it / C::NSF) & 1, abort);
+                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[slot][it % NSB]));
+            }
+            if (!ok) *abort = 1;
+            if (u.rq.seq < 0 && on && u.t0 == 0)  // a refused request's rows are 0
+                for (int c = 0; c < D; c += 8) *(uint4 *)(a.out + out_at + c) = make_uint4(0, 0, 0, 0);
+            ++unit_no;
+            continue;
+        }
+        const bool live = __any_sync(0xffffffffu, on);
+        uint8_t *const mine = smem + slot * C::Q_BYTES + quarter * (C::Q_BYTES / 4);  // this warp's 32 query rows
+        {
+            constexpr int U = D / 8;
+            const long long q_at = ((long long)a.src_row[u.b] + t) * a.q_stride + (long long)(u.g * a.group + row - t * a.group) * D;
+            const uint32_t have = __ballot_sync(0xffffffffu, on);
+            if constexpr (!Q8) {
 #pragma unroll 8
-                for (int i = lane; i < 16 * U; i += 32) {
-                    const int rr = half * 16 + i / U, uu = i % U;
-                    const long long from = __shfl_sync(0xffffffffu, at, rr);
+                for (int i = lane; i < 32 * U; i += 32) {
+                    const int rr = i / U, uu = i % U;
+                    const long long from = __shfl_sync(0xffffffffu, q_at, rr);
                     const bool has = (have >> rr) & 1u;
-                    uint8_t *to = sq + bf16_off<D>(quarter * 32 + rr, 8 * uu);
-                    if constexpr (!Q8) {
-                        cp_async_16_or_zero(smem_addr(to), has ? a.q + from + 8 * uu : a.q, has);
-                    } else {
-                        const uint4 v = has ? *(const uint4 *)(a.q + from + 8 * uu) : make_uint4(0, 0, 0, 0);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    cp_async_16_or_zero(smem_addr(mine + bf16_off<D>(rr, 8 * uu)), has ? a.q + from + 8 * uu : a.q, has);
+                }
+            } else {
+                // to f16, eight loads on their way at a time
+#pragma unroll 1
+                for (int i0 = lane; i0 < 32 * U; i0 += 256) {
+                    uint4 v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = i0 + 32 * e, rr = i / U, uu = i % U;
+                        const long long from = __shfl_sync(0xffffffffu, q_at, rr);
+                        v[e] = (have >> rr) & 1u ? *(const uint4 *)(a.q + from + 8 * uu) : make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = i0 + 32 * e, rr = i / U, uu = i % U;
+                        const uint32_t w[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
                         uint32_t o[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -508,181 +621,295 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
                             const __half2 h = __floats2half2_rn(lo, hi);
                             o[k] = *(const uint32_t *)&h;
                         }
-                        *(uint4 *)to = make_uint4(o[0], o[1], o[2], o[3]);
+                        *(uint4 *)(mine + bf16_off<D>(rr, 8 * uu)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 }
-                if (!Q8) cp_async_wait_all();
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready[slot]));
             }
-            float m = -INFINITY;
-            uint64_t l0 = 0, l1 = 0;  // the row's sum over this warp's keys
-            const int p = u.rq.pos0 + t;
-            for (int i = 0; i < n; ++i, ++it) {
-                const int st = it % NS, j = t0 + i, sb = (live_it[0] + i) % NSB;
-                ok = ok && warp_wait(smem_addr(&sh.s_full[slot][st]), (it / NS) & 1, abort);
-                if (!ok) *abort = 1;
-                tc_fence_after();
-                const uint32_t s_col = tmem + lane_base + (uint32_t)(C::S_COL + sb * BN + half * KPW);
-                if (live) {
-                    uint32_t s[KPW];
-                    if constexpr (KPW == 64) tmem_load32x2(s_col, s_col + 32, *(uint32_t(*)[32])s, *(uint32_t(*)[32])(s + 32));
-                    else tmem_load32(s_col, *(uint32_t(*)[32])s);
-                    if (!unit_sees(j)) {
-#pragma unroll
-                        for (int c = 0; c < KPW; c += 32) {
-                            const uint32_t bits = on ? seen_bits(a, sp, p, j * BN + half * KPW + c) : 0u;
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!((bits >> k) & 1u)) s[c + k] = 0xff800000u;
-                        }
-                    }
-                    float top = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < KPW; k += 4) {
-                        top = max3(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-                        top1 = max3(top1, __uint_as_float(s[k + 2]), __uint_as_float(s[k + 3]));
-                    }
-                    top = fmaxf(top, top1);
-                    const float mt = top == -INFINITY ? -INFINITY : top * a.scale_log2;
-                    // m moves when a score of either warp's keys is more than 2^8 above it
-                    if (pair_any(id, mt > m + 8.0f)) {
-                        mine[r] = mt;
-                        pair_sync(id);
-                        const float mn = fmaxf(mt, other[r]);
-                        const bool up = mn > m + 8.0f;
-                        const float f = up ? ex2(m - mn) : 1.0f;  // (0 for the first)
-                        if (up) m = mn;
-                        l0 = fma_pair(l0, pair_of(f, f), 0);
-                        l1 = fma_pair(l1, pair_of(f, f), 0);
-                        if (i > 0 && __any_sync(0xffffffffu, up)) {
-                            // O of the tiles before is complete: with one S tile because S came after it, with two it is waited for
-                            if (NSB > 1) {
-                                ok = ok && warp_wait(smem_addr(&sh.v_free[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
-                                tc_fence_after();
-                            }
-#pragma unroll 1
-                            for (int c0 = half * D / 2; c0 < (half + 1) * D / 2; c0 += 32) {
-                                uint32_t o[32];
-                                tmem_load32(tmem + lane_base + C::O_COL + c0, o);
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                tmem_st32(tmem + lane_base + C::O_COL + c0, o);
-                            }
-                        }
-                    }
-                    const float neg = m == -INFINITY ? 0.0f : -m;
-                    const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
-#pragma unroll
-                    for (int c = 0; c < KPW; c += 32) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            float2 v = of_pair(fma_pair(pair_of(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, neg2));
-                            v = make_float2(ex2(v.x), ex2(v.y));
-                            uint64_t add;
-                            if constexpr (Q8) {
-                                const __half2 h = __floats2half2_rn(v.x, v.y);
-                                w[k] = *(const uint32_t *)&h;
-                                add = pair_of(v.x, v.y);
-                            } else {
-                                w[k] = pack_bf16(v.x, v.y);
-                                add = pair_of(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
-                            }
-                            if (k & 1) l1 = add_pair(l1, add);
-                            else l0 = add_pair(l0, add);
-                        }
-                        tmem_st16(s_col + c / 2, w);
-                    }
-                    tmem_wait_st();
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[slot][sb]));
-            }
-            live_it[0] += n;
-            ok = ok && warp_wait(smem_addr(&sh.o_done[slot]), live_units & 1, abort);
-            ++live_units;
+            if (!Q8) cp_async_wait_all();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready[slot]));
+        }
+        float m = -INFINITY;
+        uint64_t l0 = 0, l1 = 0;  // the row's sum
+        const int p = u.rq.pos0 + t;
+        const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
+        for (int i = 0; i < n; ++i, ++it) {
+            const int j = u.t0 + i, sb = it % NSB;
+            ok = ok && warp_wait(smem_addr(&sh.s_full[slot][it % C::NSF]), (it / C::NSF) & 1, abort);
             if (!ok) *abort = 1;
             tc_fence_after();
-            const float2 la = of_pair(l0), lb = of_pair(l1);
-            const float part_l = (la.x + la.y) + (lb.x + lb.y);
             if (live) {
-                pair_sync(id);  // (maxima have been read)
-                mine[r] = part_l;
-                pair_sync(id);
-            }
-            if (ok && live) {
-                const float l = part_l + other[r];
-                const bool whole = t0 == 0 && t1 == n_tiles;
-                const long long part = (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS + slot * kTileRows + r;
-                if (!whole && half == 0 && on) a.ws_ml[part] = make_float4(m, l, 0.0f, 0.0f);
-                const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-                const int ub = unit_no % kBadUnits, n_bad = Q8 ? 0 : *(volatile int *)&sh.n_bad[ub];
-                uint16_t *const out = a.out + (src_row * a.q_heads + head) * D;
-#pragma unroll 1
-                for (int c0 = half * D / 2; c0 < (half + 1) * D / 2; c0 += 32) {
-                    uint32_t o[32];
-                    __syncwarp();
-                    tmem_load32(tmem + lane_base + C::O_COL + c0, o);
-                    // rare: values that are not finite, for the rows that see them
-#pragma unroll 1
-                    for (int i = 0; i < n_bad; ++i)
-#pragma unroll 1
-                        for (int k = 0; k < BN; ++k) {
-                            if (!((sh.bad[ub][i][k >> 5] >> (k & 31)) & 1u)) continue;
-                            const int key = sh.bad_key[ub][i] + k, slot_k = sp.slot(key);
-                            if (!on || !(seen_bits(a, sp, p, key) & 1u)) continue;
-                            const int e = slot_k / a.pool.block_tokens, blk = lookup_block(a.pool, u.rq.seq, e);
-                            if (blk < 0) continue;
-                            const uint8_t *tile = a.pool.prefix + prefix_tile_index(a.pool, a.layer, blk, 1, u.g) * a.pool.tile_bytes;
+                const uint32_t s_col = lane_base + (uint32_t)(C::S_COL + sb * BN);
+                const bool all_see = unit_sees(j);
+                // the row's scores, all in registers
+                uint32_t s[BN / 32][32];
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) {
-                                const float y = bf16_bits_to_f32(*(const uint16_t *)(tile + bf16_off<D>(slot_k - e * a.pool.block_tokens, c0 + c)));
-                                if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
-                            }
+                for (int c = 0; c < BN / 32; ++c) tmem_load32_nowait(s_col + 32 * c, s[c]);
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) tmem_wait_ld32(s[c]);
+                if (!all_see) {
+#pragma unroll
+                    for (int c = 0; c < BN / 32; ++c) {
+                        const uint32_t bits = on ? seen_bits(a, sp, p, j * BN + 32 * c) : 0u;
+                        if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!((bits >> k) & 1u)) s[c][k] = 0xff800000u;
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) tops[k / 2 % 4] = max3(tops[k / 2 % 4], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+                const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], -INFINITY);
+                const float mt = top == -INFINITY ? -INFINITY : top * a.scale_log2;
+                const bool up = mt > m + C::LIMIT;
+                if (__any_sync(0xffffffffu, up)) {  // (a unit's first tile, hardly ever later)
+                    const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
+                    if (up) m = mt;
+                    l0 = fma_pair(l0, pair_of(f, f), 0);
+                    l1 = fma_pair(l1, pair_of(f, f), 0);
+                    if (i > 0) {
+                        // O of the tiles before is complete: with one S tile because S came after it, with two it is waited for
+                        if (NSB > 1) {
+                            ok = ok && warp_wait(smem_addr(&sh.v_free[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
+                            tc_fence_after();
                         }
-                    // a row without a key has nothing (not 0 * what the columns hold)
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 8) {
+                            uint32_t o[8];
+                            tmem_load8(lane_base + C::O_COL + c0, o);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = l != 0.0f ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
-                    if (on && !whole) {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4) *(uint4 *)(a.ws_o + part * D + c0 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                    } else if (on) {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(o[k + 2 * e]), __uint_as_float(o[k + 2 * e + 1]));
-                            *(uint4 *)(out + c0 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st8(lane_base + C::O_COL + c0, o);
                         }
                     }
                 }
-                __syncwarp();
-            }
-            if (a.split && threadIdx.x == 0 && t0 == 0) {  // the CTAs of this unit: tile x is CTA ((x + 1) G - 1) / T's
-                const unsigned long long end = (unsigned long long)base + (uint32_t)(u.g + 1) * (uint32_t)n_tiles;
-                a.parts[(long long)flat * hk + u.g] = make_int2(blockIdx.x, (int)((end * rg.ctas - 1) / rg.total));
+                const float neg = m == -INFINITY ? 0.0f : -m;
+                const uint64_t neg2 = pair_of(neg, neg);
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float2 v = of_pair(fma_pair(pair_of(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), scale2, neg2));
+                        v = make_float2(ex2(v.x), ex2(v.y));
+                        uint64_t add;
+                        if constexpr (Q8) {
+                            const __half2 h = __floats2half2_rn(v.x, v.y);
+                            w[k] = *(const uint32_t *)&h;
+                            add = pair_of(v.x, v.y);
+                        } else {
+                            w[k] = pack_bf16(v.x, v.y);
+                            add = pair_of(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+                        }
+                        if (k & 1) l1 = add_pair(l1, add);
+                        else l0 = add_pair(l0, add);
+                    }
+                    tmem_st16(s_col + 16 * c, w);
+                }
+                tmem_wait_st();
             }
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[slot][sb]));
         }
+        ok = ok && warp_wait(smem_addr(&sh.o_done[slot]), live_units & 1, abort);
+        ++live_units;
+        if (!ok) *abort = 1;
+        tc_fence_after();
+        if (ok && live) {
+            const float2 la = of_pair(l0), lb = of_pair(l1);
+            const float l = (la.x + la.y) + (lb.x + lb.y);
+            const bool whole = u.t0 == 0 && u.t1 == u.n_tiles;
+            const long long part = (2ll * blockIdx.x + (u.t0 == 0 ? 1 : 0)) * ROWS + slot * kTileRows + r;
+            if (!whole && on) a.ws_ml[part] = make_float4(m, l, 0.0f, 0.0f);
+            const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const int ub = unit_no % kBadUnits, n_bad = Q8 ? 0 : min(kBadChunks, *(volatile int *)&((WBad *)(smem + C::OFF_BAD))->n[ub]);
+            const uint32_t have = __ballot_sync(0xffffffffu, on);
+            // through the warp's query rows, which are done with, their 16-byte units at unit ^ row, so that whole runs of a row are
+            // written together (with a thread for a row's stores an end took 7500 cycles)
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                tmem_load32(lane_base + C::O_COL + c0, o);
+                // rare: values that are not finite, for the rows that see them
+#pragma unroll 1
+                for (int i = 0; i < n_bad; ++i)
+#pragma unroll 1
+                    for (uint32_t bits = ((WBad *)(smem + C::OFF_BAD))->keys[ub][i]; bits; bits &= bits - 1) {
+                        const int key = ((WBad *)(smem + C::OFF_BAD))->first[ub][i] + __ffs(bits) - 1, slot_k = sp.slot(key);
+                        if (!on || !(seen_bits(a, sp, p, key) & 1u)) continue;
+                        const int e = slot_k / a.pool.block_tokens, blk = lookup_block(a.pool, u.rq.seq, e);
+                        if (blk < 0) continue;
+                        const uint8_t *tile = a.pool.prefix + prefix_tile_index(a.pool, a.layer, blk, 1, u.g) * a.pool.tile_bytes;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const float y = bf16_bits_to_f32(*(const uint16_t *)(tile + bf16_off<D>(slot_k - e * a.pool.block_tokens, c0 + c)));
+                            if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
+                        }
+                    }
+                // a row without a key has nothing (not 0 * what the columns hold)
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = l != 0.0f ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
+                if (!whole) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        *(uint4 *)(mine + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = 4 * k + (lane >> 3), unit = lane & 7;
+                        if ((have >> i) & 1u)
+                            *(uint4 *)(a.ws_o + (part - lane + i) * D + c0 + 4 * unit) = *(const uint4 *)(mine + i * 128 + ((unit ^ (i & 7)) << 4));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = pack_bf16(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
+                        *(uint4 *)(mine + lane * 2 * D + (((c0 / 8 + k) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (whole) {
+                constexpr int U = D / 8;
+#pragma unroll 8
+                for (int k = 0; k < U; ++k) {
+                    const int e = k * 32 + lane, i = e / U, unit = e % U;
+                    const long long to = __shfl_sync(0xffffffffu, out_at, i);
+                    if ((have >> i) & 1u) *(uint4 *)(a.out + to + 8 * unit) = *(const uint4 *)(mine + i * 2 * D + ((unit ^ (i & 7)) << 4));
+                }
+                __syncwarp();
+            }
+        }
+        if (a.split && u.t0 == 0 && u.t1 < u.n_tiles) {  // cut, and this is the first of its CTAs: place x is CTA ((x + 1) G - 1) / T's
+            const unsigned long long end = (unsigned long long)u.at + (uint32_t)(u.n_tiles + kUnitCost);
+            cut = make_int4(u.b * a.row_tiles + u.rt, u.g, (int)((end * ctas - 1) / total), 1);
+        }
+        tc_fence_before();
         ++unit_no;
     }
-    if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 15);
+    if (a.split && threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
     if (!__all_sync(0xffffffffu, fits) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, warp, 15);
-    if (warp >= C::FEED_WARP && warp < (Q8 ? C::CONV_WARP : C::SCRUB_WARP) && !ok && lane == 0) {
-        // leave no copy writing this CTA's shared memory
-        for (int i = 0; i < (Q8 ? C::NR : NS); ++i) {
-            const uint32_t bar = smem_addr(Q8 ? &sh.raw_full[i] : warp == C::FEED_WARP ? &sh.full_k[i] : &sh.full_v[i]);
-            mbar_wait_drain(bar, 0, kWait / 64);
-            mbar_wait_drain(bar, 1, kWait / 64);
+    return ok;
+}
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(const WindowArgs a) {
+    using C = WCfg<D, Q8>;
+    constexpr int NS = C::NS, NSB = C::NSB, RT = C::RT;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    WShared &sh = *(WShared *)(smem + C::OFF_SH);
+    static_assert(sizeof(WShared) <= 2048 && sizeof(WBad) <= 8192, "barrier block");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = a.pool.kv_heads;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(smem_addr(&sh.full_k[i]), Q8 ? C::CONV_WARPS : 1);
+            mbar_init(smem_addr(&sh.full_v[i]), Q8 ? C::CONV_WARPS : 1);
+            mbar_init(smem_addr(&sh.v_free[i]), Q8 ? RT : RT + C::SCRUB_WARPS);
+            mbar_init(smem_addr(&sh.v_clean[i]), C::SCRUB_WARPS);
+        }
+        for (int k = 0; k < RT; ++k) {
+            for (int i = 0; i < C::NSF; ++i) mbar_init(smem_addr(&sh.s_full[k][i]), 1);
+            for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 4);
+            mbar_init(smem_addr(&sh.q_ready[k]), 4);
+            mbar_init(smem_addr(&sh.o_done[k]), 1);
+            mbar_init(smem_addr(&sh.drained[k]), 1);
+            mbar_init(smem_addr(&sh.turn[k]), 1);
+        }
+        for (int i = 0; Q8 && i < C::NR; ++i) {
+            mbar_init(smem_addr(&sh.raw_full[i]), 1);
+            mbar_init(smem_addr(&sh.raw_empty[i]), C::CONV_WARPS);
+        }
+        sh.abort = 0;
+        if constexpr (!Q8)
+            for (int i = 0; i < kBadUnits; ++i) ((WBad *)(smem + C::OFF_BAD))->n[i] = 0;
+        mbar_init_fence();
+    }
+    grid_wait();
+    // (tensor memory between the two launch points: ekv_tree_tile.cu says why)
+    if (warp == C::MMA_WARP) tmem_alloc(smem_addr(&sh.tmem), C::COLS);
+    tc_fence_before();
+    using U = Units<RT * kTileRows, C::BN>;
+    RangeStart start{};
+    if (a.split) {
+        // a head's places of each request, a warp per request, in shared memory that nothing else uses yet
+        uint32_t *const places = (uint32_t *)smem;
+        constexpr int WARPS = C::THREADS / 32;
+        for (int b = warp; b < a.n_batch; b += WARPS) {
+            const WinReq rq = load_win_req(a, b, blockIdx.x == 0 && lane == 0);
+            uint32_t sum = 0;
+            for (int rt = lane; rt < a.row_tiles; rt += 32) sum += U::cost_of(a, rq, rt);
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) places[b] = sum;
+        }
+        __syncthreads();
+        const Range rg = find_range<C::THREADS>(
+            a.n_batch, hk, sh.range, [&](int i) { return Req{0, (int)places[i], 0}; }, [](const Req &r) { return r.n_prefix; });
+        start.x = rg.lo;
+        start.hi = rg.hi;
+        start.total = rg.total;
+        start.ctas = rg.ctas;
+        start.b = rg.b;
+        if (warp == 0 && rg.lo < rg.hi) {
+            // the head, and its row tile: 32 row tiles' places at a time
+            const uint32_t head = places[rg.b];
+            start.g = (int)((rg.lo - rg.base) / head);
+            start.at = rg.base + start.g * head;
+            const WinReq rq = load_win_req(a, rg.b, false);
+            for (int rt0 = 0;; rt0 += 32) {
+                const uint32_t cost = U::cost_of(a, rq, rt0 + lane);
+                uint32_t incl = cost;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const uint32_t here = __ballot_sync(0xffffffffu, rg.lo < start.at + incl);
+                if (here || rt0 + 32 >= a.row_tiles) {
+                    const int l = here ? __ffs(here) - 1 : 31;
+                    start.rt = rt0 + l;
+                    start.at += __shfl_sync(0xffffffffu, incl - cost, l);
+                    break;
+                }
+                start.at += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) sh.start = start;
+        }
+        __syncthreads();
+        if (rg.lo < rg.hi) start = sh.start;
+        __syncthreads();  // (query rows go where the places are)
+    } else {
+        __syncthreads();
+    }
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;  // (there is a barrier in either branch)
+    grid_launch_next();
+
+    const U u(start);
+    bool ok = true;
+    if (warp < C::ROW_WARPS) {
+        ok = softmax<D, Q8>(a, smem, sh, u, tmem, start.ctas, start.total);
+    } else {
+        if (warp < C::FEED_WARP) {
+            ok = products<D, Q8>(a, smem, sh, u, tmem);
+        } else if constexpr (Q8) {
+            if (warp < C::CONV_WARP) ok = feed<D, true>(a, smem, sh, u);
+            else if (warp < C::WARPS) ok = convert<D, true>(a, smem, sh, u);
+        } else {
+            if (warp < C::SCRUB_WARP) ok = feed<D, false>(a, smem, sh, u);
+            else if (warp < C::WARPS) ok = look_at_values<D, false>(a, smem, sh, u);
         }
     }
-    if (warp >= C::MMA_WARP && warp < C::FEED_WARP && lane == 0) {  // nor a product using its tensor memory
-        mma_commit(smem_addr(&sh.drained[warp - C::MMA_WARP]));
-        mbar_wait_drain(smem_addr(&sh.drained[warp - C::MMA_WARP]), 0, kWait);
-    }
+    if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 15);
     __syncthreads();
     if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
 }
@@ -698,7 +925,7 @@ int launch_form(const WindowArgs &a, int grid, cudaStream_t s) {
 }  // namespace
 
 int window_tile_rows(int head_dim) { return (head_dim > 128 ? 1 : 2) * kTileRows; }
-int window_tile_keys(int head_dim) { return head_dim > 128 ? 64 : 128; }
+int window_tile_keys(int) { return 64; }
 
 int launch_window_tile(const WindowArgs &a, int grid, cudaStream_t s) {
     const bool q8 = a.pool.dtype == EKV_DTYPE_Q8_0;
