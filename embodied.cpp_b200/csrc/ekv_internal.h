@@ -237,7 +237,8 @@ int launch_compact(const CompactArgs &a, int sms, cudaStream_t s);
 size_t window_workspace(const PoolView &p, int n_batch, int max_rows, int q_heads, int sms);
 int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s);
 int window_tile_rows(int head_dim);  // rows of a unit of the tile kernel
-int window_tile_keys(int head_dim);  // keys of one of its tiles
+int window_tile_keys();              // keys of one of its tiles
+constexpr int kWindowUnitCost = 4;   // and the tiles that it costs beside its own
 int launch_window_tile(const WindowArgs &a, int grid, cudaStream_t s);
 // Eviction by weight (ekv_evict.cu)
 // max_live: the longest live sequence

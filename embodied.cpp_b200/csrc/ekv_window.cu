@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
         const int t1 = a.split ? min(n_tiles, t0 + (int)(rg.hi - x)) : (rank + 1) * n_tiles / a.cluster;
         const int rows = rq.n * a.group;
         const Span sp = span_of(rq);
-        const int64_t src_row = rq.n > 0 ? (int64_t)a.src_row[b] : 0;
+        const int64_t src_row = rq.src;
         // query row r of the unit, or null where it does not take part
         auto q_row = [&](int r) -> const uint16_t * {
             const int t = row_token(a, r);
@@ -679,7 +679,7 @@ size_t window_workspace(const PoolView &p, int n_batch, int max_rows, int q_head
 }
 
 int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes, int sms, cudaStream_t s) {
-    const int rows = a.max_rows * a.group, ur = unit_rows(a.pool, rows), keys = few_rows(rows) ? kTile : window_tile_keys(a.pool.head_dim);
+    const int rows = a.max_rows * a.group, ur = unit_rows(a.pool, rows), keys = few_rows(rows) ? kTile : window_tile_keys();
     a.row_tiles = (rows + ur - 1) / ur;
     const int64_t units = (int64_t)a.n_batch * a.row_tiles * a.pool.kv_heads;
     if (units * (ur / kMergeWarps) > INT32_MAX) return EKV_ERR_INVALID_ARG;
@@ -689,7 +689,7 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
     const int64_t tokens = std::min<int64_t>(a.max_rows, (ur + a.group - 1) / a.group + 1);
     auto tiles = [&](int64_t len) { return (std::min<int64_t>(len, (int64_t)a.window + tokens + a.sinks) + 16 + keys - 1) / keys; };
     const int64_t unit_tiles = tiles(max_len), most_tiles = tiles((int64_t)a.pool.max_blocks_per_seq * a.pool.block_tokens) + 1;
-    const bool can_split = ws != nullptr && ws_bytes >= w.total && units * (most_tiles + 3) < INT32_MAX;
+    const bool can_split = ws != nullptr && ws_bytes >= w.total && units * (most_tiles + kWindowUnitCost) < INT32_MAX;
     a.split = 0;
     a.cluster = 1;
     int64_t grid;
@@ -709,7 +709,7 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
     } else {
         // Equal ranges of all tiles wherever there is room for the join; every CTA looks through the requests for its own.
         a.split = can_split && a.n_batch <= kMaxRangeRequests;
-        grid = std::min<int64_t>(full, a.split ? units * (unit_tiles + 3) : units);
+        grid = std::min<int64_t>(full, a.split ? units * (unit_tiles + kWindowUnitCost) : units);
     }
     if (a.split) {
         a.parts = (int2 *)ws;

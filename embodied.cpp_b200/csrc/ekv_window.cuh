@@ -13,7 +13,7 @@ namespace window {
 
 // One request of the call: `n` rows' tokens from slot pos0 on; seq < 0: refused, its rows become 0.
 struct WinReq {
-    int seq, pos0, n;
+    int seq, pos0, n, src;  // src: its first row in q and out
 };
 
 __device__ __forceinline__ WinReq load_win_req(const WindowArgs &a, int b, bool report) {
@@ -21,6 +21,7 @@ __device__ __forceinline__ WinReq load_win_req(const WindowArgs &a, int b, bool 
     r.seq = a.seq_ids[b];
     r.pos0 = a.dst_pos[b];
     r.n = min(max(a.n_rows[b], 0), a.max_rows);
+    r.src = a.src_row[b];
     if (r.n == 0) return r;
     if (r.seq < 0 || r.seq >= a.pool.max_seqs) {
         if (report) report_error(a.pool.status, DEV_ERR_BAD_SEQ, b, r.seq, 14);

@@ -1,10 +1,21 @@
 // ekv_window_tile.cu -- windowed attention of many rows per KV head (prompts, chunks) on tcgen05.
 //
 // out = sum_k p_k v_k / sum_k p_k with p_k = exp(scale q.k - m) over the keys a row sees (ekv_window.cuh), m a running reference that
-// moves only when a score is 2^8 above it. S = Q K^T with both operands in shared memory and S in tensor memory, P in 16 bits over
-// S's own columns, O += P V with P read from tensor memory. P is rounded to bf16 (bf16 pages) and the row divided by the sum of the
-// rounded ones; over 8-bit pages operands are f16 (a value's int8 times its scale keeps 11 bits, P too).
-#include <type_traits>
+// moves only when a score is 2^24 (8-bit pages: 2^8) above it. S = Q K^T with both operands in shared memory and S in tensor memory, P in
+// 16 bits over S's own columns, O += P V with P read from tensor memory. P is rounded to bf16 (bf16 pages) and the row divided by the
+// sum of the rounded ones; over 8-bit pages operands are f16 (a value's int8 times its scale keeps 11 bits, P too).
+//
+// Roles of a CTA's warps, each in step with the CTA's tiles by its own count: feed (K, V), convert (8-bit pages, K and V apart) or
+// look_at_values (bf16), products (a warp per row tile), softmax (a thread per row; head_dim 256: two). What bounds it: a row
+// tile's chain of scores, maximum, exponentials, P, next products. Two row tiles fill it for the special-function unit (1024 of a
+// 64-key tile's 2450 cycles) and the tensor pipe (1300 of them); a unit's end and beginning take 9000 cycles, beside 12 tiles of a
+// window of 1024 a quarter.
+// 32 / 8 heads of 128: a prompt of 16384 tokens 2305 us (954 TFLOP/s of the products that rows see, 60% of a measured bf16 product), over
+// 8-bit pages 2555; 8 prompts of up to 4096, window 1024 and 4 first tokens: 660 us (600), over 8-bit pages 775. 8 / 1 heads of 256, 8192
+// tokens: 300 us (915).
+// Measured and left out, the first two figures again: 128 keys a tile with one S tile 2386 and 773 us; two warps to a row in place
+// of one for head_dim 128 2654 and 718 (for 256, where one row tile leaves the schedulers a warp each, 343 instead of 396); a part of
+// the exponentials by polynomial 2333 and 645 (an eighth), 2448 and 711 (a quarter).
 
 #include "ekv_window.cuh"
 
@@ -31,15 +42,22 @@ struct WCfg {
     static constexpr float LIMIT = Q8 ? 8.0f : 24.0f;
     static constexpr uint32_t SBO = 16 * D, LAYOUT = 2;
     static constexpr int KV_BYTES = BN * D * 2, Q_BYTES = kTileRows * D * 2;
-    static constexpr int NR = D == 64 ? 6 : 5, RAW = BN * D + BN * (D / 32) * 2;  // Q8: tiles of K, of V as they are stored
+    static constexpr int NR = D > 128 ? 2 : 4, RAW = BN * D + BN * (D / 32) * 2;  // Q8: tiles of K, and of V, as they are stored
     static constexpr int S_COL = 0, O_COL = BN * NSB, SLOT_COLS = 256, COLS = 512;
     static constexpr int OFF_K = RT * Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_RAW = OFF_V + NS * KV_BYTES;
-    static constexpr int OFF_SH = OFF_RAW + (Q8 ? (NR * RAW + 1023) / 1024 * 1024 : 0);
-    static constexpr int OFF_BAD = OFF_SH + 2048, SHARED = 2048 + (Q8 ? 0 : 8192), SMEM = OFF_SH + SHARED + 1024;
-    static constexpr int ROW_WARPS = 4 * RT, MMA_WARP = ROW_WARPS, FEED_WARP = MMA_WARP + RT;
-    // bf16: K's feeder, V's feeder, and four warps that look at V; Q8: one feeder, and converters
-    static constexpr int SCRUB_WARP = FEED_WARP + 2, SCRUB_WARPS = 4, CONV_WARP = FEED_WARP + 1, CONV_WARPS = RT == 1 ? 8 : 4;
-    static constexpr int WARPS = Q8 ? CONV_WARP + CONV_WARPS : SCRUB_WARP + SCRUB_WARPS, THREADS = (WARPS + 3) / 4 * 128;
+    static constexpr int OFF_SH = OFF_RAW + (Q8 ? (2 * NR * RAW + 1023) / 1024 * 1024 : 0);
+    static constexpr int OFF_X = OFF_SH + 2048, OFF_BAD = OFF_X + RT * 2 * kTileRows * 4, SHARED = OFF_BAD - OFF_SH + (Q8 ? 0 : 8192);
+    static constexpr int SMEM = OFF_SH + SHARED + 1024;
+    static constexpr int SHARE = RT == 1 ? 2 : 1;  // softmax warps of 32 rows
+    static constexpr int ROW_WARPS = 4 * SHARE * RT, MMA_WARP = ROW_WARPS, FEED_WARP = MMA_WARP + RT;
+    // K's feeder, V's feeder; bf16: four warps that look at V; Q8: four that convert K, four that convert V
+    static constexpr int SCRUB_WARP = FEED_WARP + 2, SCRUB_WARPS = 4, CONV_WARP = FEED_WARP + 2, CONV_WARPS = 4;
+    static constexpr int WARPS = Q8 ? CONV_WARP + 2 * CONV_WARPS : SCRUB_WARP + SCRUB_WARPS, THREADS = WARPS * 32;
+    // 8-bit pages, two row tiles: 20 warps leave 96 registers to a thread at launch, and a row's 64 scores take more. (With two warps in
+    // place of four for each conversion there is room for 128; 16384 tokens of head_dim 128 then took 2960 us instead of 2620.)
+    static constexpr bool SPLIT_REGS = Q8 && RT == 2;
+    static constexpr int ROW_REGS = 136, OTHER_REGS = 64;
+    static_assert(!SPLIT_REGS || (THREADS == 640 && 256 * ROW_REGS + 384 * OTHER_REGS <= 640 * 96), "registers");
     static_assert(O_COL + D <= (RT == 2 ? SLOT_COLS : COLS) && SMEM <= 232448, "tensor memory, shared memory");
 };
 
@@ -58,7 +76,7 @@ struct RangeStart {
 
 struct WShared {
     uint64_t full_k[4], full_v[4];       // K, V of the stage are there
-    uint64_t raw_full[6], raw_empty[6];  // Q8: a tile of K or V has landed; is converted
+    uint64_t raw_full[2][4], raw_empty[2][4];  // Q8: [K, V] a tile has landed; is converted
     uint64_t s_full[2][4];               // [slot][tile % NSF] S done
     uint64_t v_free[4];                  // both slots' P V done, and (bf16) the tile looked at
     uint64_t p_full[2][2];               // [slot][S tile] P written
@@ -84,6 +102,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// The two warps that share rows (named barrier id): any of their lanes' x; both there.
+__device__ __forceinline__ bool pair_any(int id, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)x), "r"(id)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+
 // One lane of a converged warp. With `lane == 0` in its place the compiler guards each tcgen05.mma by itself against lanes that
 // differ: 80 to 110 cycles an instruction, more than most of them run, so that issuing bound the kernel.
 __device__ __forceinline__ bool elect_one() {
@@ -99,31 +129,27 @@ __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t (&r)[8]) {
                  : "memory");
 }
 
-// N x 32 columns of tensor memory, one wait for all of them.
-__device__ __forceinline__ void tmem_load32_nowait(uint32_t at, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(at)
-        : "memory");
-}
-// (names the registers, so that none of them is read before it)
-__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
+// Lane i of four has unit k of row i in x[k], and gets unit i of row k: four rows' 64 bytes each in one store of the four lanes.
+__device__ __forceinline__ void transpose4(uint4 (&x)[4], int lane) {
+    auto swap = [&](uint4 &a, uint4 &b, int m) {  // the upper lane's a for the lower one's b
+        const bool up = lane & m;
+        uint4 give = up ? a : b;
+        give.x = __shfl_xor_sync(0xffffffffu, give.x, m);
+        give.y = __shfl_xor_sync(0xffffffffu, give.y, m);
+        give.z = __shfl_xor_sync(0xffffffffu, give.z, m);
+        give.w = __shfl_xor_sync(0xffffffffu, give.w, m);
+        (up ? a : b) = give;
+    };
+    swap(x[0], x[1], 1);
+    swap(x[2], x[3], 1);
+    swap(x[0], x[2], 2);
+    swap(x[1], x[3], 2);
 }
 
 // The blocks' int8 rows as f16 values, rounded once; rows past `valid` are zero. Scales that leave the f16 range with them are
 // reported, their values 0.
 template <int D, int ROWS, int THREADS>
-__device__ __forceinline__ bool convert_piece(const uint8_t *raw, uint8_t *dst, int row0, int valid, int thread) {
+__device__ __forceinline__ bool convert_tile(const uint8_t *raw, uint8_t *dst, int valid, int thread) {
     constexpr int U = D / 16;
     bool fits = true;
 #pragma unroll 4
@@ -150,7 +176,7 @@ __device__ __forceinline__ bool convert_piece(const uint8_t *raw, uint8_t *dst, 
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-            *(uint4 *)(dst + bf16_off<D>(row0 + row, 16 * u + 8 * k)) = make_uint4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+            *(uint4 *)(dst + bf16_off<D>(row, 16 * u + 8 * k)) = make_uint4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
     }
     return fits;
 }
@@ -158,10 +184,10 @@ __device__ __forceinline__ bool convert_piece(const uint8_t *raw, uint8_t *dst, 
 // ---- the units of a CTA, in the same order in every warp ----
 // split: the range [x, hi) of all tiles in the order request, KV head, row tile, tile, where a unit counts kUnitCost tiles more for
 // what it costs beside them (query rows, the first tile's way, the end): without that the CTA of a long prompt's first rows took half
-// as long again. The row tiles of a head follow one another, so that a CTA finds most of a window in L2: with the heads innermost the
-// windows of all CTAs' heads did not fit it (8 prompts of 4096 tokens, a window of 1024: 980 us).
+// as long again (8192 tokens of head_dim 256: 367 us at 2, 294 at 4, 300 at 8). The row tiles of a head follow one another, so that a CTA
+// finds most of a window in L2: with the heads innermost the windows of all CTAs' heads did not fit it.
 // Else whole units, the longest (a request's last rows) first, back and forth over the CTAs.
-constexpr int kUnitCost = 3;
+constexpr int kUnitCost = kWindowUnitCost;
 template <int ROWS, int BN>
 struct Units {
     int rt, round;     // row tile (split); rounds over the CTAs so far
@@ -242,7 +268,8 @@ __device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared
     volatile int *abort = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = a.pool.kv_heads;
     bool ok = true;
-    [[maybe_unused]] int it = 0, raw_it = 0;  // tiles, and (Q8) pieces, of this CTA so far
+    const bool is_v = warp != C::FEED_WARP;
+    int it = 0;  // tiles of this CTA so far
     while (u.next(a, false)) {
         const Span sp = u.span(a);
         // ---- feeders ----
@@ -250,7 +277,6 @@ __device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared
         auto block = [&](int e) { return lookup_block(a.pool, u.rq.seq, e); };
         const int64_t v_from_k = (int64_t)hk * a.pool.tile_bytes;
         if constexpr (!Q8) {
-            const bool is_v = warp != C::FEED_WARP;
             Run next = find_run<BN>(a, sp, u.g, u.t0 * BN, lane, want, block);
             for (int j = u.t0; j < u.t1; ++j, ++it) {
                 const int st = it % NS, par = (it / NS) & 1;
@@ -275,33 +301,30 @@ __device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared
             }
         } else {
             Run next = find_run<BN>(a, sp, u.g, u.t0 * BN, lane, want, block);
-            for (int j = u.t0; j < u.t1; ++j) {
+            for (int j = u.t0; j < u.t1; ++j, ++it) {
+                const int rs = it % C::NR;
                 const Run r = next;
                 if (j + 1 < u.t1) next = find_run<BN>(a, sp, u.g, (j + 1) * BN, lane, want, block);
-                for (int v = 0; v < 2; ++v, ++raw_it) {  // K, then V
-                    const int rs = raw_it % C::NR;
-                    if (raw_it >= C::NR) ok = ok && warp_wait(smem_addr(&sh.raw_empty[rs]), (raw_it / C::NR - 1) & 1, abort);
-                    if (!ok) {
-                        *abort = 1;
-                        continue;
-                    }
-                    const uint32_t dst = smem_addr(smem + C::OFF_RAW + rs * C::RAW), bar = smem_addr(&sh.raw_full[rs]);
-                    const uint32_t bytes = r.src ? (uint32_t)(r.n * (D + D / 16)) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, all);
-                    __syncwarp();
-                    if (!r.src) continue;
-                    const uint8_t *src = r.src + (v ? v_from_k : 0);
-                    bulk_g2s(dst + r.row * D, src + r.rib * D, (uint32_t)(r.n * D), bar);
-                    bulk_g2s(dst + BN * D + r.row * (D / 16), src + (int64_t)a.pool.block_tokens * D + r.rib * (D / 16),
-                             (uint32_t)(r.n * (D / 16)), bar);
+                if (it >= C::NR) ok = ok && warp_wait(smem_addr(&sh.raw_empty[is_v][rs]), (it / C::NR - 1) & 1, abort);
+                if (!ok) {
+                    *abort = 1;
+                    continue;
                 }
+                const uint32_t dst = smem_addr(smem + C::OFF_RAW + (is_v * C::NR + rs) * C::RAW), bar = smem_addr(&sh.raw_full[is_v][rs]);
+                const uint32_t bytes = r.src ? (uint32_t)(r.n * (D + D / 16)) : 0u, all = __reduce_add_sync(0xffffffffu, bytes);
+                if (lane == 0) mbar_arrive_expect_tx(bar, all);
+                __syncwarp();
+                if (!r.src) continue;
+                const uint8_t *src = r.src + (is_v ? v_from_k : 0);
+                bulk_g2s(dst + r.row * D, src + r.rib * D, (uint32_t)(r.n * D), bar);
+                bulk_g2s(dst + BN * D + r.row * (D / 16), src + (int64_t)a.pool.block_tokens * D + r.rib * (D / 16), (uint32_t)(r.n * (D / 16)), bar);
             }
         }
     }
     if (!ok && lane == 0) {
         // leave no copy writing this CTA's shared memory
         for (int i = 0; i < (Q8 ? C::NR : NS); ++i) {
-            const uint32_t bar = smem_addr(Q8 ? &sh.raw_full[i] : warp == C::FEED_WARP ? &sh.full_k[i] : &sh.full_v[i]);
+            const uint32_t bar = smem_addr(Q8 ? &sh.raw_full[is_v][i] : is_v ? &sh.full_v[i] : &sh.full_k[i]);
             mbar_wait_drain(bar, 0, kWait / 64);
             mbar_wait_drain(bar, 1, kWait / 64);
         }
@@ -314,39 +337,32 @@ __device__ __forceinline__ bool convert(const WindowArgs &a, uint8_t *smem, WSha
     using C = WCfg<D, Q8>;
     constexpr int BN = C::BN, NS = C::NS, RT = C::RT;
     volatile int *abort = &sh.abort;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, thread = threadIdx.x - C::CONV_WARP * 32, is_v = thread >= C::CONV_WARPS * 32;
     bool ok = true;
     int it = 0;  // tiles of this CTA so far
-    int raw_it = 0;  // pieces so far
     bool fits = true;
     while (u.next(a, false)) {
         const Span sp = u.span(a);
-        // ---- converters ----
-        const int thread = threadIdx.x - C::CONV_WARP * 32;
         for (int j = u.t0; j < u.t1; ++j, ++it) {
-            const int st = it % NS;
-#pragma unroll 1
-            for (int v = 0; v < 2; ++v, ++raw_it) {
-                const int rs = raw_it % C::NR;
-                if (it >= NS) {  // the stage is free
-                    if (v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), (it / NS - 1) & 1, abort);
+            const int st = it % NS, rs = it % C::NR;
+            if (it >= NS) {  // the stage is free
+                if (is_v) ok = ok && warp_wait(smem_addr(&sh.v_free[st]), (it / NS - 1) & 1, abort);
 #pragma unroll
-                    for (int k = 0; k < RT; ++k)
-                        if (!v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][(it - NS) % C::NSF]), ((it - NS) / C::NSF) & 1, abort);
-                }
-                ok = ok && warp_wait(smem_addr(&sh.raw_full[rs]), (raw_it / C::NR) & 1, abort);
-                if (!ok) {
-                    *abort = 1;
-                    continue;
-                }
-                fits &= convert_piece<D, BN, C::CONV_WARPS * 32>(smem + C::OFF_RAW + rs * C::RAW, smem + (v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES, 0,
-                                                                sp.keys - j * BN, thread);
-                fence_proxy_async();  // read by the tensor core; the next blocks come through the copy engine
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_addr(&sh.raw_empty[rs]));
-                    mbar_arrive(smem_addr(v ? &sh.full_v[st] : &sh.full_k[st]));
-                }
+                for (int k = 0; k < RT; ++k)
+                    if (!is_v) ok = ok && warp_wait(smem_addr(&sh.s_full[k][(it - NS) % C::NSF]), ((it - NS) / C::NSF) & 1, abort);
+            }
+            ok = ok && warp_wait(smem_addr(&sh.raw_full[is_v][rs]), (it / C::NR) & 1, abort);
+            if (!ok) {
+                *abort = 1;
+                continue;
+            }
+            fits &= convert_tile<D, BN, C::CONV_WARPS * 32>(smem + C::OFF_RAW + (is_v * C::NR + rs) * C::RAW, smem + (is_v ? C::OFF_V : C::OFF_K) + st * C::KV_BYTES,
+                                                           sp.keys - j * BN, thread & (C::CONV_WARPS * 32 - 1));
+            fence_proxy_async();  // read by the tensor core; the next blocks come through the copy engine
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_addr(&sh.raw_empty[is_v][rs]));
+                mbar_arrive(smem_addr(is_v ? &sh.full_v[st] : &sh.full_k[st]));
             }
         }
     }
@@ -502,7 +518,7 @@ __device__ __forceinline__ bool products(const WindowArgs &a, uint8_t *smem, WSh
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     const int k = 4 * s4 + s;  // 16 keys
-                    av[s] = p_at + (uint32_t)(8 * k);
+                    av[s] = p_at + (uint32_t)(32 * (k / 2) + 8 * (k % 2));  // (32 keys' P over their own scores)
                     bv[s] = vb + ((uint32_t)(k * 2 * C::SBO) >> 4);
                 }
                 mma_ts_x4<false>(cols + C::O_COL, av, bv, id_o, i > 0 || s4 > 0 ? 1u : 0u);
@@ -557,22 +573,71 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
     constexpr int BN = C::BN, NS = C::NS, NSB = C::NSB, RT = C::RT, ROWS = RT * kTileRows;
     volatile int *abort = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // thread = row: all keys of a tile are its own, so that rows need nothing from one another
-    const int slot = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    // thread = row and 32 keys of a tile: two warps share 32 rows. A warp for all 64 keys waits for its own results (for the exponentials
+    // alone 1.5 times what the special-function unit takes), and four to a scheduler fill one another's waits.
+    constexpr int SHARE = C::SHARE, KEYS = BN / SHARE;
+    const int slot = warp / (4 * SHARE), half = SHARE > 1 ? (warp >> 2) & 1 : 0, quarter = warp & 3, r = quarter * 32 + lane;
+    [[maybe_unused]] const int id = 1 + slot * 4 + quarter;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * C::SLOT_COLS);
+    [[maybe_unused]] float *const x_mine = (float *)(smem + C::OFF_X) + (slot * 2 + half) * kTileRows + r, *const x_other = (float *)(smem + C::OFF_X) + (slot * 2 + 1 - half) * kTileRows + r;
     bool ok = true, fits = true;
     int it = 0, unit_no = 0;  // tiles and units of this CTA so far
     int live_units = 0;       // units that this slot had rows for
     int4 cut = make_int4(0, 0, 0, 0);  // the unit that this CTA begins and others end: row tile, KV head, last CTA
-    while (u.next(a, warp == 0 && lane == 0)) {
+    // The unit's query rows of this warp: half of the 16-byte units of 32 rows, on their way, and there. A unit's rows are fetched as
+    // soon as the products of the unit before are done, and the first scores run beside that unit's end.
+    uint8_t *const q_rows = smem + slot * C::Q_BYTES + quarter * (C::Q_BYTES / 4);
+    constexpr int QU = D / 8;
+    auto q_fetch = [&](const auto &v) {
+        const int row = v.row0 + slot * kTileRows + r, t = row_token(a, row);
+        const long long q_at = ((long long)v.rq.src + t) * a.q_stride + (long long)(v.g * a.group + row - t * a.group) * D;
+        const uint32_t have = __ballot_sync(0xffffffffu, row < v.rq.n * a.group);
+#pragma unroll 8
+        for (int k = 0; k < QU / SHARE; ++k) {
+            const int i = (k * SHARE + half) * 32 + lane, rr = i / QU, uu = i % QU;
+            const long long from = __shfl_sync(0xffffffffu, q_at, rr);
+            const bool has = (have >> rr) & 1u;
+            cp_async_16_or_zero(smem_addr(q_rows + bf16_off<D>(rr, 8 * uu)), has ? a.q + from + 8 * uu : a.q, has);
+        }
+    };
+    auto q_there = [&] {
+        cp_async_wait_all();
+        if constexpr (Q8) {  // as f16, each lane what it fetched
+#pragma unroll 2
+            for (int k = 0; k < QU / SHARE; ++k) {
+                const int i = (k * SHARE + half) * 32 + lane;
+                uint4 *const at = (uint4 *)(q_rows + bf16_off<D>(i / QU, 8 * (i % QU)));
+                const uint4 v = *at;
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float lo = __uint_as_float(w[e] << 16), hi = __uint_as_float(w[e] & 0xffff0000u);
+                    fits = fits && fabsf(lo) <= 65504.0f && fabsf(hi) <= 65504.0f;
+                    const __half2 h = __floats2half2_rn(lo, hi);
+                    o[e] = *(const uint32_t *)&h;
+                }
+                *at = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready[slot]));
+    };
+    auto has_rows = [&](const auto &v) { return v.rows(a) > slot * kTileRows && v.rq.seq >= 0; };
+    const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
+    bool more = u.next(a, warp == 0 && lane == 0);
+    if (more && has_rows(u)) {
+        q_fetch(u);
+        q_there();
+    }
+    while (more) {
         const int n = u.t1 - u.t0;
         const Span sp = u.span(a);
-        auto unit_sees = [&](int j) { return sp.all_see(a, j * BN, BN); };
         const int row = u.row0 + slot * kTileRows + r, t = row_token(a, row);
-        const bool slot_live = u.rows(a) > slot * kTileRows && u.rq.seq >= 0;
         const bool on = row < u.rq.n * a.group;
-        const long long out_at = (((int64_t)a.src_row[u.b] + t) * a.q_heads + u.g * a.group + row - t * a.group) * D;
-        if (!slot_live) {
+        const long long out_at = (((int64_t)u.rq.src + t) * a.q_heads + u.g * a.group + row - t * a.group) * D;
+        if (!has_rows(u)) {
             // in step with the tiles all the same: a barrier's parity tells two phases apart, so nobody may fall behind
             for (int i = 0; i < n; ++i, ++it) {
                 ok = ok && warp_wait(smem_addr(&sh.s_full[slot][it % C::NSF]), (it / C::NSF) & 1, abort);
@@ -580,79 +645,34 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
             }
             if (!ok) *abort = 1;
             if (u.rq.seq < 0 && on && u.t0 == 0)  // a refused request's rows are 0
-                for (int c = 0; c < D; c += 8) *(uint4 *)(a.out + out_at + c) = make_uint4(0, 0, 0, 0);
+                for (int c = half * D / SHARE; c < (half + 1) * D / SHARE; c += 8) *(uint4 *)(a.out + out_at + c) = make_uint4(0, 0, 0, 0);
             ++unit_no;
+            more = u.next(a, warp == 0 && lane == 0);
+            if (more && has_rows(u)) {
+                q_fetch(u);
+                q_there();
+            }
             continue;
         }
         const bool live = __any_sync(0xffffffffu, on);
-        uint8_t *const mine = smem + slot * C::Q_BYTES + quarter * (C::Q_BYTES / 4);  // this warp's 32 query rows
-        {
-            constexpr int U = D / 8;
-            const long long q_at = ((long long)a.src_row[u.b] + t) * a.q_stride + (long long)(u.g * a.group + row - t * a.group) * D;
-            const uint32_t have = __ballot_sync(0xffffffffu, on);
-            if constexpr (!Q8) {
-#pragma unroll 8
-                for (int i = lane; i < 32 * U; i += 32) {
-                    const int rr = i / U, uu = i % U;
-                    const long long from = __shfl_sync(0xffffffffu, q_at, rr);
-                    const bool has = (have >> rr) & 1u;
-                    cp_async_16_or_zero(smem_addr(mine + bf16_off<D>(rr, 8 * uu)), has ? a.q + from + 8 * uu : a.q, has);
-                }
-            } else {
-                // to f16, eight loads on their way at a time
-#pragma unroll 1
-                for (int i0 = lane; i0 < 32 * U; i0 += 256) {
-                    uint4 v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int i = i0 + 32 * e, rr = i / U, uu = i % U;
-                        const long long from = __shfl_sync(0xffffffffu, q_at, rr);
-                        v[e] = (have >> rr) & 1u ? *(const uint4 *)(a.q + from + 8 * uu) : make_uint4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int i = i0 + 32 * e, rr = i / U, uu = i % U;
-                        const uint32_t w[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
-                        uint32_t o[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float lo = __uint_as_float(w[k] << 16), hi = __uint_as_float(w[k] & 0xffff0000u);
-                            fits = fits && fabsf(lo) <= 65504.0f && fabsf(hi) <= 65504.0f;
-                            const __half2 h = __floats2half2_rn(lo, hi);
-                            o[k] = *(const uint32_t *)&h;
-                        }
-                        *(uint4 *)(mine + bf16_off<D>(rr, 8 * uu)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
-                }
-            }
-            if (!Q8) cp_async_wait_all();
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&sh.q_ready[slot]));
-        }
         float m = -INFINITY;
-        uint64_t l0 = 0, l1 = 0;  // the row's sum
+        uint64_t l0 = 0, l1 = 0;  // the row's sum over this warp's keys
         const int p = u.rq.pos0 + t;
-        const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
         for (int i = 0; i < n; ++i, ++it) {
-            const int j = u.t0 + i, sb = it % NSB;
+            const int sb = it % NSB, key = (u.t0 + i) * BN + KEYS * half;
             ok = ok && warp_wait(smem_addr(&sh.s_full[slot][it % C::NSF]), (it / C::NSF) & 1, abort);
             if (!ok) *abort = 1;
             tc_fence_after();
             if (live) {
-                const uint32_t s_col = lane_base + (uint32_t)(C::S_COL + sb * BN);
-                const bool all_see = unit_sees(j);
-                // the row's scores, all in registers
-                uint32_t s[BN / 32][32];
+                const uint32_t s_col = lane_base + (uint32_t)(C::S_COL + sb * BN + KEYS * half);
+                uint32_t s[KEYS / 32][32];
+                if constexpr (KEYS == 64) tmem_load32x2(s_col, s_col + 32, s[0], s[1]);
+                else tmem_load32(s_col, s[0]);
+                if (!sp.all_see(a, key, KEYS)) {
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_load32_nowait(s_col + 32 * c, s[c]);
-#pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_wait_ld32(s[c]);
-                if (!all_see) {
-#pragma unroll
-                    for (int c = 0; c < BN / 32; ++c) {
-                        const uint32_t bits = on ? seen_bits(a, sp, p, j * BN + 32 * c) : 0u;
-                        if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
+                    for (int c = 0; c < KEYS / 32; ++c) {
+                        const uint32_t bits = on ? seen_bits(a, sp, p, key + 32 * c) : 0u;
+                        if (KEYS > 32 && __all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
                             if (!((bits >> k) & 1u)) s[c][k] = 0xff800000u;
@@ -660,25 +680,32 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                 }
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c)
+                for (int c = 0; c < KEYS / 32; ++c)
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) tops[k / 2 % 4] = max3(tops[k / 2 % 4], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
                 const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], -INFINITY);
                 const float mt = top == -INFINITY ? -INFINITY : top * a.scale_log2;
-                const bool up = mt > m + C::LIMIT;
-                if (__any_sync(0xffffffffu, up)) {  // (a unit's first tile, hardly ever later)
-                    const float f = up ? ex2(m - mt) : 1.0f;  // (0 for the first)
-                    if (up) m = mt;
+                bool any;
+                if constexpr (SHARE > 1) any = pair_any(id, mt > m + C::LIMIT);
+                else any = __any_sync(0xffffffffu, mt > m + C::LIMIT);
+                if (any) {  // (a unit's first tile, hardly ever later)
+                    float both = mt;
+                    if constexpr (SHARE > 1) {
+                        *x_mine = mt;
+                        pair_sync(id);
+                        both = fmaxf(mt, *x_other);
+                    }
+                    const bool up = both > m + C::LIMIT;
+                    const float f = up ? ex2(m - both) : 1.0f;  // (0 for the first)
+                    if (up) m = both;
                     l0 = fma_pair(l0, pair_of(f, f), 0);
                     l1 = fma_pair(l1, pair_of(f, f), 0);
                     if (i > 0) {
-                        // O of the tiles before is complete: with one S tile because S came after it, with two it is waited for
-                        if (NSB > 1) {
-                            ok = ok && warp_wait(smem_addr(&sh.v_free[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
-                            tc_fence_after();
-                        }
+                        // O of the tiles before is complete when V of the last one is free
+                        ok = ok && warp_wait(smem_addr(&sh.v_free[(it - 1) % NS]), ((it - 1) / NS) & 1, abort);
+                        tc_fence_after();
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 8) {
+                        for (int c0 = half * D / SHARE; c0 < (half + 1) * D / SHARE; c0 += 8) {
                             uint32_t o[8];
                             tmem_load8(lane_base + C::O_COL + c0, o);
 #pragma unroll
@@ -690,7 +717,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                 const float neg = m == -INFINITY ? 0.0f : -m;
                 const uint64_t neg2 = pair_of(neg, neg);
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
+                for (int c = 0; c < KEYS / 32; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
@@ -708,7 +735,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                         if (k & 1) l1 = add_pair(l1, add);
                         else l0 = add_pair(l0, add);
                     }
-                    tmem_st16(s_col + 16 * c, w);
+                    tmem_st16(s_col + 32 * c, w);
                 }
                 tmem_wait_st();
             }
@@ -720,21 +747,32 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
         ++live_units;
         if (!ok) *abort = 1;
         tc_fence_after();
-        if (ok && live) {
+        // the unit's end: the next one's query rows are fetched beside it
+        const auto last = u;
+        const bool whole = u.t0 == 0 && u.t1 == u.n_tiles;
+        if (a.split && u.t0 == 0 && u.t1 < u.n_tiles) {  // cut, and this is the first of its CTAs: place x is CTA ((x + 1) G - 1) / T's
+            const unsigned long long end = (unsigned long long)u.at + (uint32_t)(u.n_tiles + kUnitCost);
+            cut = make_int4(u.b * a.row_tiles + u.rt, u.g, (int)((end * ctas - 1) / total), 1);
+        }
+        more = u.next(a, warp == 0 && lane == 0);
+        const bool fetch = more && has_rows(u);
+        if (fetch) q_fetch(u);
+        if (live) {
             const float2 la = of_pair(l0), lb = of_pair(l1);
-            const float l = (la.x + la.y) + (lb.x + lb.y);
-            const bool whole = u.t0 == 0 && u.t1 == u.n_tiles;
-            const long long part = (2ll * blockIdx.x + (u.t0 == 0 ? 1 : 0)) * ROWS + slot * kTileRows + r;
-            if (!whole && on) a.ws_ml[part] = make_float4(m, l, 0.0f, 0.0f);
+            float l = (la.x + la.y) + (lb.x + lb.y);
+            if constexpr (SHARE > 1) {
+                *x_mine = l;  // (the other warp has read the maximum: its P is in O)
+                pair_sync(id);
+                l = half ? *x_other + l : l + *x_other;
+            }
+            const long long part = (2ll * blockIdx.x + (last.t0 == 0 ? 1 : 0)) * ROWS + slot * kTileRows + r;
+            if (!whole && on && half == 0) a.ws_ml[part] = make_float4(m, l, 0.0f, 0.0f);
             const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             const int ub = unit_no % kBadUnits, n_bad = Q8 ? 0 : min(kBadChunks, *(volatile int *)&((WBad *)(smem + C::OFF_BAD))->n[ub]);
             const uint32_t have = __ballot_sync(0xffffffffu, on);
-            // through the warp's query rows, which are done with, their 16-byte units at unit ^ row, so that whole runs of a row are
-            // written together (with a thread for a row's stores an end took 7500 cycles)
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
+            for (int c0 = half * D / SHARE; ok && c0 < (half + 1) * D / SHARE; c0 += 32) {
                 uint32_t o[32];
-                __syncwarp();
                 tmem_load32(lane_base + C::O_COL + c0, o);
                 // rare: values that are not finite, for the rows that see them
 #pragma unroll 1
@@ -743,55 +781,47 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                     for (uint32_t bits = ((WBad *)(smem + C::OFF_BAD))->keys[ub][i]; bits; bits &= bits - 1) {
                         const int key = ((WBad *)(smem + C::OFF_BAD))->first[ub][i] + __ffs(bits) - 1, slot_k = sp.slot(key);
                         if (!on || !(seen_bits(a, sp, p, key) & 1u)) continue;
-                        const int e = slot_k / a.pool.block_tokens, blk = lookup_block(a.pool, u.rq.seq, e);
+                        const int e = slot_k / a.pool.block_tokens, blk = lookup_block(a.pool, last.rq.seq, e);
                         if (blk < 0) continue;
-                        const uint8_t *tile = a.pool.prefix + prefix_tile_index(a.pool, a.layer, blk, 1, u.g) * a.pool.tile_bytes;
+                        const uint8_t *tile = a.pool.prefix + prefix_tile_index(a.pool, a.layer, blk, 1, last.g) * a.pool.tile_bytes;
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
                             const float y = bf16_bits_to_f32(*(const uint16_t *)(tile + bf16_off<D>(slot_k - e * a.pool.block_tokens, c0 + c)));
                             if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
                         }
                     }
-                // a row without a key has nothing (not 0 * what the columns hold)
+                // (a row without a key: its P were 0, and so are its columns, as the values that some rows do not see are finite)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = l != 0.0f ? __float_as_uint(__uint_as_float(o[k]) * f) : 0u;
+                for (int k = 0; k < 32; k += 2) {
+                    const float2 y = of_pair(fma_pair(pair_of(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), pair_of(f, f), 0));
+                    o[k] = __float_as_uint(y.x);
+                    o[k + 1] = __float_as_uint(y.y);
+                }
                 if (!whole) {
+                    if (on)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        *(uint4 *)(mine + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int i = 4 * k + (lane >> 3), unit = lane & 7;
-                        if ((have >> i) & 1u)
-                            *(uint4 *)(a.ws_o + (part - lane + i) * D + c0 + 4 * unit) = *(const uint4 *)(mine + i * 128 + ((unit ^ (i & 7)) << 4));
-                    }
+                        for (int k = 0; k < 8; ++k) *(uint4 *)(a.ws_o + part * D + c0 + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 } else {
+                    uint4 x[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        uint32_t x[4];
+                        uint32_t y[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = pack_bf16(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
-                        *(uint4 *)(mine + lane * 2 * D + (((c0 / 8 + k) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                        for (int e = 0; e < 4; ++e) y[e] = pack_bf16(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
+                        x[k] = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                    transpose4(x, lane);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int i = (lane & ~3) + k;
+                        const long long to = __shfl_sync(0xffffffffu, out_at, i);
+                        if ((have >> i) & 1u) *(uint4 *)(a.out + to + c0 + 8 * (lane & 3)) = x[k];
                     }
                 }
-            }
-            __syncwarp();
-            if (whole) {
-                constexpr int U = D / 8;
-#pragma unroll 8
-                for (int k = 0; k < U; ++k) {
-                    const int e = k * 32 + lane, i = e / U, unit = e % U;
-                    const long long to = __shfl_sync(0xffffffffu, out_at, i);
-                    if ((have >> i) & 1u) *(uint4 *)(a.out + to + 8 * unit) = *(const uint4 *)(mine + i * 2 * D + ((unit ^ (i & 7)) << 4));
-                }
-                __syncwarp();
+                if (fetch && c0 == half * D / SHARE) q_there();
             }
         }
-        if (a.split && u.t0 == 0 && u.t1 < u.n_tiles) {  // cut, and this is the first of its CTAs: place x is CTA ((x + 1) G - 1) / T's
-            const unsigned long long end = (unsigned long long)u.at + (uint32_t)(u.n_tiles + kUnitCost);
-            cut = make_int4(u.b * a.row_tiles + u.rt, u.g, (int)((end * ctas - 1) / total), 1);
-        }
+        if (fetch && !(live && ok)) q_there();
         tc_fence_before();
         ++unit_no;
     }
@@ -819,15 +849,15 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
         }
         for (int k = 0; k < RT; ++k) {
             for (int i = 0; i < C::NSF; ++i) mbar_init(smem_addr(&sh.s_full[k][i]), 1);
-            for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 4);
-            mbar_init(smem_addr(&sh.q_ready[k]), 4);
+            for (int i = 0; i < NSB; ++i) mbar_init(smem_addr(&sh.p_full[k][i]), 4 * C::SHARE);
+            mbar_init(smem_addr(&sh.q_ready[k]), 4 * C::SHARE);
             mbar_init(smem_addr(&sh.o_done[k]), 1);
             mbar_init(smem_addr(&sh.drained[k]), 1);
             mbar_init(smem_addr(&sh.turn[k]), 1);
         }
-        for (int i = 0; Q8 && i < C::NR; ++i) {
-            mbar_init(smem_addr(&sh.raw_full[i]), 1);
-            mbar_init(smem_addr(&sh.raw_empty[i]), C::CONV_WARPS);
+        for (int i = 0; Q8 && i < 2 * C::NR; ++i) {
+            mbar_init(smem_addr(&sh.raw_full[i / C::NR][i % C::NR]), 1);
+            mbar_init(smem_addr(&sh.raw_empty[i / C::NR][i % C::NR]), C::CONV_WARPS);
         }
         sh.abort = 0;
         if constexpr (!Q8)
@@ -897,8 +927,10 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
     const U u(start);
     bool ok = true;
     if (warp < C::ROW_WARPS) {
+        if constexpr (C::SPLIT_REGS) warpgroup_reg_alloc<C::ROW_REGS>();
         ok = softmax<D, Q8>(a, smem, sh, u, tmem, start.ctas, start.total);
     } else {
+        if constexpr (C::SPLIT_REGS) warpgroup_reg_dealloc<C::OTHER_REGS>();
         if (warp < C::FEED_WARP) {
             ok = products<D, Q8>(a, smem, sh, u, tmem);
         } else if constexpr (Q8) {
@@ -925,7 +957,7 @@ int launch_form(const WindowArgs &a, int grid, cudaStream_t s) {
 }  // namespace
 
 int window_tile_rows(int head_dim) { return (head_dim > 128 ? 1 : 2) * kTileRows; }
-int window_tile_keys(int) { return 64; }
+int window_tile_keys() { return 64; }
 
 int launch_window_tile(const WindowArgs &a, int grid, cudaStream_t s) {
     const bool q8 = a.pool.dtype == EKV_DTYPE_Q8_0;
