@@ -10,6 +10,7 @@
 // the copy engine. P is rounded to bf16 and the row divided by the sum of the rounded ones; over 8-bit pages p times the value's scale
 // is two bf16 parts, so that a heavy key's 32 columns are not all off by the same 2^-8.
 #include <algorithm>
+#include <type_traits>
 
 #include "ekv_window.cuh"
 
@@ -653,23 +654,64 @@ WsLayout ws_layout(const PoolView &p, int n_batch, int rows, int sms) {
 }
 
 template <int D, bool Q8, int NR>
+int rows_smem() {
+    static std::atomic<uint64_t> done{0};
+    return allow_smem(window_rows_kernel<D, Q8, NR>, FCfg<D, Q8, NR>::SMEM, done);
+}
+
+template <int D, bool Q8, int NR>
 int launch_rows(const WindowArgs &a, int grid, cudaStream_t s) {
     using C = FCfg<D, Q8, NR>;
-    static std::atomic<uint64_t> done{0};
-    if (const int rc = allow_smem(window_rows_kernel<D, Q8, NR>, C::SMEM, done)) return rc;
+    if (const int rc = rows_smem<D, Q8, NR>()) return rc;
     return launch_clusters_after(a.cluster, window_rows_kernel<D, Q8, NR>, grid, C::THREADS, C::SMEM, s, a);
 }
 
-template <int D>
-int launch_dim(const WindowArgs &a, int rows, int grid, cudaStream_t s) {
-    int rc;
-    const bool q8 = a.pool.dtype == EKV_DTYPE_Q8_0;
-    if (!few_rows(rows)) rc = launch_window_tile(a, grid, s);
-    else if (rows <= 8) rc = q8 ? launch_rows<D, true, 1>(a, grid, s) : launch_rows<D, false, 1>(a, grid, s);
-    else rc = q8 ? launch_rows<D, true, 2>(a, grid, s) : launch_rows<D, false, 2>(a, grid, s);
-    if (rc || !a.split) return rc;
-    const int ur = unit_rows(a.pool, rows), units = a.cuts ? grid : a.n_batch * a.row_tiles * a.pool.kv_heads;
-    return launch_after(window_merge_kernel<D>, units * (ur / kMergeWarps), kMergeWarps * 32, 0, s, a, ur);
+// Clusters of 2^(i + 1) CTAs that run at the same time on the current device (asked once: it depends on how many SMs each part of the
+// device has; 0 where that cannot be asked).
+template <int D, bool Q8, int NR>
+int rows_clusters(int i) {
+    using C = FCfg<D, Q8, NR>;
+    static std::atomic<int> known[64][3];  // 1 + their number
+    int dev = 0, n = 0;
+    if (!C::CLUSTERS || cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || rows_smem<D, Q8, NR>()) return 0;
+    std::atomic<int> &k = known[dev][i];
+    if (const int have = k.load(std::memory_order_relaxed)) return have - 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(2u << i);
+    c.blockDim = dim3((unsigned)C::THREADS);
+    c.dynamicSmemBytes = C::SMEM;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2u << i;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, window_rows_kernel<D, Q8, NR>, &c) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    k.store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+// f with head_dim, 8-bit pages, and groups of eight rows (0: the tile kernel) as types.
+template <class F>
+int with_form(const PoolView &p, int rows, F f) {
+    const bool q8 = p.dtype == EKV_DTYPE_Q8_0;
+    auto dim = [&](auto d) {
+        using D = decltype(d);
+        using T = std::true_type;
+        using N = std::false_type;
+        if (!few_rows(rows)) return f(d, N{}, std::integral_constant<int, 0>{});
+        if (rows <= 8) return q8 ? f(D{}, T{}, std::integral_constant<int, 1>{}) : f(D{}, N{}, std::integral_constant<int, 1>{});
+        return q8 ? f(D{}, T{}, std::integral_constant<int, 2>{}) : f(D{}, N{}, std::integral_constant<int, 2>{});
+    };
+    switch (p.head_dim) {
+        case 64: return dim(std::integral_constant<int, 64>{});
+        case 128: return dim(std::integral_constant<int, 128>{});
+        case 256: return dim(std::integral_constant<int, 256>{});
+        default: return EKV_ERR_UNSUPPORTED;
+    }
 }
 
 }  // namespace
@@ -694,16 +736,31 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
     a.cluster = 1;
     int64_t grid;
     if (few_rows(rows)) {
-        // As launch_tree_attention: a cluster of CTAs per unit, or equal ranges of all tiles and a join, which costs about as much as
-        // `worth` tiles.
-        const int64_t even = (units * unit_tiles + full - 1) / full;
-        const int64_t worth = a.pool.dtype == EKV_DTYPE_Q8_0 ? 1 : 3;
-        if (unit_tiles > 2) {
-            int c = 1;
-            if (ur * a.pool.head_dim <= 2048)
-                while (c < kMaxCluster && 2 * c <= unit_tiles && units * 2 * c <= full) c *= 2;
-            if (c > 1 && (!can_split || (unit_tiles + c - 1) / c <= even + worth)) a.cluster = c;
-            else a.split = can_split;
+        // A cluster of CTAs per unit, or equal ranges of all tiles and a join; times in tiles. A call costs `fixed` beside its
+        // tiles, the join `worth`, which grows with the parts of a unit: 64 requests of 17 tiles of head_dim 256, bf16 22.1 us with clusters of 2, 33.1 with 4 (which run in two
+        // turns), 29.9 with a join; 16 of them 13.4 with clusters of 4, 21.7 with 8 (two turns) and with a join. 8-bit pages: 32 requests
+        // 37.1, 23.7, 17.9, 15.3 with 1, 2, 4, 8, 24.1 with a join; 128 of 17 tiles 32.9 with 2, 39.9 with 1, 39.1 with a join; one of 65 tiles
+        // 22.6 with 8, 33.4 with a join of 65 parts. 128 units of 129 tiles of head_dim 128, bf16: 84 with clusters of 2, 92 with a join.
+        const bool q8 = a.pool.dtype == EKV_DTYPE_Q8_0;
+        const int64_t even = (units * unit_tiles + full - 1) / full, parts = (unit_tiles + even - 1) / std::max<int64_t>(1, even);
+        const int64_t fixed = q8 ? 4 : 8, worth = q8 ? std::max<int64_t>(7, 5 + parts / 7) : std::max<int64_t>(10, 8 + parts / 4);
+        int64_t best = (units + full - 1) / full * (fixed + unit_tiles);
+        for (int i = 0; i < 3 && (2 << i) <= unit_tiles; ++i) {
+            const int c = 2 << i;
+            const int64_t fit = with_form(a.pool, rows, [&](auto d, auto q, auto nr) {
+                if constexpr (decltype(nr)::value > 0) return rows_clusters<decltype(d)::value, decltype(q)::value, decltype(nr)::value>(i);
+                else return 0;
+            });
+            if (fit <= 0) break;
+            const int64_t cost = (units + fit - 1) / fit * (fixed + (unit_tiles + c - 1) / c);
+            if (cost < best) {
+                best = cost;
+                a.cluster = c;
+            }
+        }
+        if (can_split && fixed + even + worth < best) {
+            a.split = 1;
+            a.cluster = 1;
         }
         grid = a.split ? std::min<int64_t>(full, units * unit_tiles) : units * a.cluster;
     } else {
@@ -718,12 +775,15 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
         a.ws_o = (float *)((uint8_t *)ws + w.o);
     }
     if (grid > INT32_MAX) return EKV_ERR_INVALID_ARG;
-    switch (a.pool.head_dim) {
-        case 64: return launch_dim<64>(a, rows, (int)grid, s);
-        case 128: return launch_dim<128>(a, rows, (int)grid, s);
-        case 256: return launch_dim<256>(a, rows, (int)grid, s);
-        default: return EKV_ERR_UNSUPPORTED;
-    }
+    return with_form(a.pool, rows, [&](auto d, auto q, auto nr) {
+        constexpr int D = decltype(d)::value, NR = decltype(nr)::value;
+        int rc;
+        if constexpr (NR > 0) rc = launch_rows<D, decltype(q)::value, NR>(a, (int)grid, s);
+        else rc = launch_window_tile(a, (int)grid, s);
+        if (rc || !a.split) return rc;
+        const int n_units = a.cuts ? (int)grid : (int)units;
+        return launch_after(window_merge_kernel<D>, n_units * (ur / kMergeWarps), kMergeWarps * 32, 0, s, a, ur);
+    });
 }
 
 }  // namespace ekv

@@ -10,7 +10,7 @@
 // tile's chain of scores, maximum, exponentials, P, next products. Two row tiles fill it for the special-function unit (1024 of a
 // 64-key tile's 2450 cycles) and the tensor pipe (1300 of them); a unit's end and beginning take 9000 cycles, beside 12 tiles of a
 // window of 1024 a quarter.
-// 32 / 8 heads of 128: a prompt of 16384 tokens 2305 us (954 TFLOP/s of the products that rows see, 60% of a measured bf16 product), over
+// 32 / 8 heads of 128: a prompt of 16384 tokens 2305 us (954 TFLOP/s of the products that rows see, 56% of a measured bf16 product), over
 // 8-bit pages 2555; 8 prompts of up to 4096, window 1024 and 4 first tokens: 660 us (600), over 8-bit pages 775. 8 / 1 heads of 256, 8192
 // tokens: 300 us (915).
 // Measured and left out, the first two figures again: 128 keys a tile with one S tile 2386 and 773 us; two warps to a row in place
