@@ -104,6 +104,7 @@ struct TreeArgs {
 };
 
 // An attention of appended rows with a sliding window and first tokens that stay visible.
+constexpr int32_t kCutUnits = 1, kWholeUnits = 2;
 struct WindowArgs {
     PoolView pool;
     int32_t layer, n_batch, q_heads, group, max_rows;
@@ -117,7 +118,7 @@ struct WindowArgs {
     uint16_t *out;
     // units: (request, row tile, KV head); partial results of units cut between CTAs
     int32_t row_tiles;   // row tiles of one (request, KV head)
-    int32_t split;       // CTAs take equal ranges of the call's tiles; 0: whole units
+    int32_t split;       // CTAs take equal ranges of the call's tiles: kCutUnits, or (tile kernel) kWholeUnits; 0: a unit, or units, each
     int32_t cluster;     // (rows kernel, split == 0) CTAs of a unit
     int2 *parts;         // rows kernel: [units] first and last CTA of each unit
     int4 *cuts;          // tile kernel: [CTAs] the unit that the CTA begins and others end (request * row tiles + row tile, KV head, last

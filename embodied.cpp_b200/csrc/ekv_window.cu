@@ -759,16 +759,25 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
             }
         }
         if (can_split && fixed + even + worth < best) {
-            a.split = 1;
+            a.split = kCutUnits;
             a.cluster = 1;
         }
         grid = a.split ? std::min<int64_t>(full, units * unit_tiles) : units * a.cluster;
     } else {
-        // Equal ranges of all tiles wherever there is room for the join; every CTA looks through the requests for its own.
-        a.split = can_split && a.n_batch <= kMaxRangeRequests;
-        grid = std::min<int64_t>(full, a.split ? units * (unit_tiles + kWindowUnitCost) : units);
+        // Up to four units a CTA: whole ones, the longest first. More: ranges of whole units, which know how many rows the requests have
+        // (32 requests of 100 to 500 rows: 197 us, the longest first 262). Cut ranges where the longest CTA would have more than 40 tiles
+        // above the even share, or 16 where none has two units: cutting costs 25 us, for the parts' way through memory and the join.
+        // Whole in order, whole by ranges, cut: 64 requests of 77 rows, a window of 300 (1.7 units a CTA): 25, 35, 40 us; a prompt of 4096
+        // tokens (3.5) 166, 208, 197; 3 prompts of up to 2048 (5.2) 126, 99, 112; 8 of up to 4096, a window of 1024 (28) 680, 633, 655;
+        // 5 requests of 200 rows, a window of 2000 (0.3) 46, 49, 26; one prompt of 16384 (14) 2419, 2568, 2383.
+        const int64_t cost = unit_tiles + kWindowUnitCost;
+        const bool ranges = a.n_batch <= kMaxRangeRequests && units * (most_tiles + kWindowUnitCost) < INT32_MAX;
+        const int64_t over = ((units + full - 1) / full * full - units) * cost / full;
+        if (ranges && can_split && over > (units > full ? 40 : 16)) a.split = kCutUnits;
+        else if (ranges && units > 4 * full) a.split = kWholeUnits;
+        grid = std::min<int64_t>(full, a.split == kCutUnits ? units * cost : units);
     }
-    if (a.split) {
+    if (a.split == kCutUnits) {
         a.parts = (int2 *)ws;
         a.cuts = few_rows(rows) ? nullptr : (int4 *)ws;
         a.ws_ml = (float4 *)((uint8_t *)ws + w.ml);
@@ -780,7 +789,7 @@ int launch_window_attention(WindowArgs a, int max_len, void *ws, size_t ws_bytes
         int rc;
         if constexpr (NR > 0) rc = launch_rows<D, decltype(q)::value, NR>(a, (int)grid, s);
         else rc = launch_window_tile(a, (int)grid, s);
-        if (rc || !a.split) return rc;
+        if (rc || a.split != kCutUnits) return rc;
         const int n_units = a.cuts ? (int)grid : (int)units;
         return launch_after(window_merge_kernel<D>, n_units * (ur / kMergeWarps), kMergeWarps * 32, 0, s, a, ur);
     });

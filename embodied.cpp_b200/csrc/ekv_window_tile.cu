@@ -182,10 +182,11 @@ __device__ __forceinline__ bool convert_tile(const uint8_t *raw, uint8_t *dst, i
 }
 
 // ---- the units of a CTA, in the same order in every warp ----
-// split: the range [x, hi) of all tiles in the order request, KV head, row tile, tile, where a unit counts kUnitCost tiles more for
+// kCutUnits: the range [x, hi) of all tiles in the order request, KV head, row tile, tile, where a unit counts kUnitCost tiles more for
 // what it costs beside them (query rows, the first tile's way, the end): without that the CTA of a long prompt's first rows took half
 // as long again (8192 tokens of head_dim 256: 367 us at 2, 294 at 4, 300 at 8). The row tiles of a head follow one another, so that a CTA
 // finds most of a window in L2: with the heads innermost the windows of all CTAs' heads did not fit it.
+// kWholeUnits: the same ranges, but a unit belongs to the CTA whose range its middle is in.
 // Else whole units, the longest (a request's last rows) first, back and forth over the CTAs.
 constexpr int kUnitCost = kWindowUnitCost;
 template <int ROWS, int BN>
@@ -210,7 +211,7 @@ struct Units {
     __device__ __forceinline__ bool next(const WindowArgs &a, bool report) {
         const int hk = a.pool.kv_heads;
         if (a.split) {
-            while (x < hi && b < a.n_batch) {
+            while ((x < hi || a.split == kWholeUnits) && b < a.n_batch) {
                 if (rq_of != b) rq = load_win_req(a, b, false), rq_of = b;
                 n_tiles = tiles_of(a, rq, rt);
                 if (n_tiles == 0) {  // the request has no more rows: its next head, or the next request
@@ -226,6 +227,20 @@ struct Units {
                     at += cost;
                     ++rt;
                     continue;
+                }
+                if (a.split == kWholeUnits) {
+                    // those whose middle is in the range
+                    const uint32_t middle = at + cost / 2;
+                    if (middle >= hi) return false;
+                    if (middle < x) {
+                        x = at + cost;
+                        continue;
+                    }
+                    x = at + cost;
+                    row0 = rt * ROWS;
+                    t0 = 0;
+                    t1 = n_tiles;
+                    return true;
                 }
                 const int from = (int)(x - at), to = (int)min(cost, from + (hi - x));
                 x += to - from;
@@ -750,7 +765,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
         // the unit's end: the next one's query rows are fetched beside it
         const auto last = u;
         const bool whole = u.t0 == 0 && u.t1 == u.n_tiles;
-        if (a.split && u.t0 == 0 && u.t1 < u.n_tiles) {  // cut, and this is the first of its CTAs: place x is CTA ((x + 1) G - 1) / T's
+        if (u.t0 == 0 && u.t1 < u.n_tiles) {  // cut, and this is the first of its CTAs: place x is CTA ((x + 1) G - 1) / T's
             const unsigned long long end = (unsigned long long)u.at + (uint32_t)(u.n_tiles + kUnitCost);
             cut = make_int4(u.b * a.row_tiles + u.rt, u.g, (int)((end * ctas - 1) / total), 1);
         }
@@ -825,7 +840,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
         tc_fence_before();
         ++unit_no;
     }
-    if (a.split && threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
+    if (a.split == kCutUnits && threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
     if (!__all_sync(0xffffffffu, fits) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, warp, 15);
     return ok;
 }
