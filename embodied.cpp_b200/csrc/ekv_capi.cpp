@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstring>
 #include <new>
+#include <set>
 
 #include "ekv_internal.h"
 
@@ -42,8 +43,7 @@ void mark_dirty(ekv_pool *p, int32_t id) {
 
 // Blocks in and out of sequences: a block is free again when its last holder lets it go.
 int32_t take_lowest_block(ekv_pool *p) {
-    const int32_t b = *p->free_blocks.begin();
-    p->free_blocks.erase(p->free_blocks.begin());
+    const int32_t b = p->free_blocks.take();
     p->holders[(size_t)b] = 1;
     return b;
 }
@@ -182,10 +182,10 @@ int ekv_pool_create(const ekv_pool_config *cfg, ekv_pool **out) {
     if (c.device < 0) {
         // Host-only pool: block tables and sequences without device memory (for testing the
         // allocator where no GPU is present). Data operations on it fail with EKV_ERR_UNSUPPORTED.
-        for (int32_t b = 0; b < c.n_blocks; ++b) p->free_blocks.insert(p->free_blocks.end(), b);
+        p->free_blocks.fill(c.n_blocks);
         p->seqs.resize((size_t)c.max_seqs);
         p->dirty.assign((size_t)c.max_seqs, 0);
-        for (int32_t s = 0; s < c.max_seqs; ++s) p->free_seq_ids.insert(p->free_seq_ids.end(), s);
+        p->free_seq_ids.fill(c.max_seqs);
         *out = p;
         return EKV_OK;
     }
@@ -214,10 +214,10 @@ int ekv_pool_create(const ekv_pool_config *cfg, ekv_pool **out) {
     v.seq_lens = (int32_t *)(base + p->bytes_prefix + p->bytes_suffix + bytes_tables);
     v.status = (int32_t *)(base + p->bytes_prefix + p->bytes_suffix + bytes_tables + bytes_lens);
 
-    for (int32_t b = 0; b < c.n_blocks; ++b) p->free_blocks.insert(p->free_blocks.end(), b);
+    p->free_blocks.fill(c.n_blocks);
     p->seqs.resize((size_t)c.max_seqs);
     p->dirty.assign((size_t)c.max_seqs, 0);
-    for (int32_t s = 0; s < c.max_seqs; ++s) p->free_seq_ids.insert(p->free_seq_ids.end(), s);
+    p->free_seq_ids.fill(c.max_seqs);
     if (cudaDeviceSynchronize() != cudaSuccess) {
         cudaFreeHost(p->h_status);
         cudaFree(p->dev_base);
@@ -332,8 +332,7 @@ int ekv_pool_sync(ekv_pool *p, ekv_stream_t stream) {
 int ekv_seq_create(ekv_pool *p, int32_t *seq_id) {
     if (!p || !seq_id) return EKV_ERR_INVALID_ARG;
     if (p->free_seq_ids.empty()) return EKV_ERR_POOL_EXHAUSTED;
-    const int32_t id = *p->free_seq_ids.begin();
-    p->free_seq_ids.erase(p->free_seq_ids.begin());
+    const int32_t id = p->free_seq_ids.take();
     ekv_pool::Seq &q = p->seqs[(size_t)id];
     q.live = true;
     q.forked = false;
@@ -390,7 +389,7 @@ int ekv_seq_set_blocks(ekv_pool *p, int32_t id, const int32_t *blocks, int32_t n
         const int32_t b = blocks[i];
         if (b < 0 || b >= p->cfg.n_blocks) return EKV_ERR_INVALID_ARG;
         if (!seen.insert(b).second) return EKV_ERR_INVALID_ARG;
-        if (!own.count(b) && !p->free_blocks.count(b)) return EKV_ERR_POOL_EXHAUSTED;
+        if (!own.count(b) && !p->free_blocks.has(b)) return EKV_ERR_POOL_EXHAUSTED;
     }
     for (int32_t b : q.blocks) release_block(p, b);
     q.blocks.assign(blocks, blocks + n_blocks);
@@ -470,18 +469,21 @@ static int fork_sequences(ekv_pool *p, int32_t n, const int32_t *parents, const 
     copies.reserve(ekv::kMaxForks);
     forks.reserve(ekv::kMaxForks);
     dst.reserve(ekv::kMaxForks);
-    std::vector<std::vector<int32_t>> tables((size_t)n);
-    for (int32_t i = 0; i < n; ++i) tables[(size_t)i].reserve((size_t)blocks_for(p, n_tokens[i]));
+    for (int32_t i = 0, id = 0; i < n; ++i, ++id) {
+        id = p->free_seq_ids.next(id);
+        p->seqs[(size_t)id].blocks.reserve((size_t)blocks_for(p, n_tokens[i]));
+    }
     if (device) {
         if (const int rc = make_write_tables(p)) return rc;
         // The kernel reads the parents' tables and writes the children's. (Blocks that are no longer shared may wait: so marked,
         // they are refused to writers, no more.)
-        std::set<int32_t>::const_iterator id = p->free_seq_ids.begin();
-        for (int32_t i = 0; i < n; ++i) p->dirty[(size_t)*id++] = 0;
+        auto mark = [&](uint8_t to) {
+            for (int32_t i = 0, id = 0; i < n; ++i, ++id) p->dirty[(size_t)(id = p->free_seq_ids.next(id))] = to;
+        };
+        mark(0);
         if (const int rc = upload_dirty(p, s)) {
             p->any_dirty = true;
-            id = p->free_seq_ids.begin();
-            for (int32_t i = 0; i < n; ++i) p->dirty[(size_t)*id++] = 1;
+            mark(1);
             return rc;
         }
         p->any_dirty = p->unshared;
@@ -490,7 +492,9 @@ static int fork_sequences(ekv_pool *p, int32_t n, const int32_t *parents, const 
         ekv_pool::Seq &from = p->seqs[(size_t)parents[i]];
         const int32_t full = n_tokens[i] / bt, rest = n_tokens[i] % bt;
         int32_t tail = -1;
-        std::vector<int32_t> &blocks = tables[(size_t)i];
+        const int32_t id = p->free_seq_ids.take();
+        ekv_pool::Seq &q = p->seqs[(size_t)id];
+        std::vector<int32_t> &blocks = q.blocks;
         blocks.assign(from.blocks.begin(), from.blocks.begin() + full);
         for (int32_t b : blocks) ++p->holders[(size_t)b];
         if (rest) {
@@ -501,12 +505,8 @@ static int fork_sequences(ekv_pool *p, int32_t n, const int32_t *parents, const 
             else copies.push_back({src, rows, (int32_t)dst.size(), 1});
             dst.push_back(tail);
         }
-        const int32_t id = *p->free_seq_ids.begin();
-        p->free_seq_ids.erase(p->free_seq_ids.begin());
-        ekv_pool::Seq &q = p->seqs[(size_t)id];
         q.live = q.forked = from.forked = true;
         q.n_tokens = n_tokens[i];
-        q.blocks.swap(blocks);
         q.pred_lo = q.pred_hi = 0;
         children[i] = id;
         if (!device) {
@@ -548,8 +548,7 @@ int ekv_seq_fork(ekv_pool *p, int32_t n, const int32_t *parents, const int32_t *
     try {
         return fork_sequences(p, n, parents, n_tokens, children, (cudaStream_t)stream);
     } catch (const std::bad_alloc &) {  // (every allocation comes before the first change, but for the freed sequences' marks)
-        std::set<int32_t>::const_iterator id = p->free_seq_ids.begin();
-        for (int32_t i = 0; i < n; ++i) mark_dirty(p, *id++);
+        for (int32_t i = 0, id = 0; i < n; ++i, ++id) mark_dirty(p, id = p->free_seq_ids.next(id));
         return EKV_ERR_ALLOC;
     }
 }
@@ -578,12 +577,12 @@ int ekv_seq_own(ekv_pool *p, int32_t id, int32_t pos0, int32_t n_tokens, ekv_str
         ekv::BlockCopy copies[ekv::kMaxForks];
         int32_t dst[ekv::kMaxForks], entry[ekv::kMaxForks];
         int n = 0;
-        std::set<int32_t>::const_iterator next = p->free_blocks.begin();
+        int32_t next = -1;
         for (; at <= last && n < ekv::kMaxForks; ++at) {
             if (p->holders[(size_t)q.blocks[(size_t)at]] <= 1) continue;
             copies[n] = {q.blocks[(size_t)at], bt, n, 1};
             entry[n] = at;
-            dst[n++] = *next++;
+            dst[n++] = next = p->free_blocks.next(next + 1);
         }
         if (p->cfg.device >= 0 && n > 0)
             rc = ekv::launch_pages(p->view, copies, n, dst, n, nullptr, 0, p->sms, (cudaStream_t)stream);

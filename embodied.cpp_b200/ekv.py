@@ -341,7 +341,9 @@ class Pool:
         return s.value
 
     def seq_free(self, seq):
-        check(lib.ekv_seq_free(self.h, seq), "ekv_seq_free")
+        code = lib.ekv_seq_free(self.h, seq)
+        if code:
+            check(code, "ekv_seq_free")
 
     def seq_resize(self, seq, n_tokens):
         check(lib.ekv_seq_resize(self.h, seq, n_tokens), "ekv_seq_resize")
