@@ -1037,7 +1037,9 @@ int ekv_window_attention(ekv_pool *p, const ekv_window_params *prm, const void *
     a.group = prm->q_heads / c.kv_heads;
     a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);  // (not used at 1, where it is 2^32)
     a.max_rows = prm->max_rows;
-    a.window = prm->window > 0 ? prm->window : INT32_MAX;
+    // (no sequence is that long, and slots less the window stay inside 32 bits for every key of a row's tiles)
+    constexpr int32_t all = INT32_MAX - 1024;
+    a.window = prm->window > 0 ? std::min(prm->window, all) : all;
     a.sinks = prm->sinks;
     a.scale_log2 = prm->scale * log2e;
     a.seq_ids = prm->seq_ids;

@@ -157,7 +157,7 @@ struct WindowArgs {
     PoolView pool;
     int32_t layer, n_batch, q_heads, group, max_rows;
     uint32_t group_mul;  // ceil(2^32 / group) (group > 1)
-    int32_t window;      // a row sees its own slot and the window - 1 before it (2^31 - 1: all before it)
+    int32_t window;      // a row sees its own slot and the window - 1 before it (no window: more than any sequence has)
     int32_t sinks;       // and slots below this
     float scale_log2;    // scale * log2(e)
     const int32_t *seq_ids, *dst_pos, *n_rows, *src_row;

@@ -1,5 +1,8 @@
 """Windowed attention on the GPU: how calls are shared over the SMs. The formula and its tolerances are those of test_gpu_window.py."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -150,3 +153,46 @@ def test_scores_far_apart():
             # f32 sums of products up to M are off by 2^-24 of it for each of log2(128) + 1 steps and the scale: 2^-20 M, twice
             tol = tolerance("bf16", call.many, size, most) + torch.expm1(most * 2 ** -19) * size
             assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("store", ["bf16", "q8_0"])
+@pytest.mark.parametrize("rows", [1, 50])
+def test_the_largest_windows_and_first_tokens(store, rows):
+    """Windows and numbers of first tokens up to what their type holds: every slot up to the row's own."""
+    call = Call([300, 0], [rows, rows], 4, 2, 64, store=store, window=0, seed=6)
+    want = call.run()
+    call.check(want)
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (0, 2 ** 31 - 1), (5, 2 ** 31 - 1), (1, 100000)):
+        got = call.run(window=window, sinks=sinks)
+        call.check(got)
+
+
+CAPTURE_FIRST = """
+import math, sys
+import torch
+import decode_cases as dc, ekv
+from test_gpu_window import Call
+rows, dim, store = int(sys.argv[1]), int(sys.argv[2]), sys.argv[3]
+call = Call([1500, 900], [rows, rows], 8, 1, dim, store=store, window=1200, sinks=4)
+prm = call.c.pool.window_params(layer=0, seq_ids=call.c.seq_ids, dst_pos=dc.ints(call.past), n_rows=call.n_rows, src_row=call.src, max_rows=rows,
+                                q_heads=8, scale=1 / math.sqrt(dim), window=1200, sinks=4)
+ws = torch.empty(call.c.pool.window_attention_workspace_size(prm), dtype=torch.uint8, device="cuda")
+out, s = torch.zeros_like(call.q), torch.cuda.Stream()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    call.c.pool.window_attention(prm, call.q, out, ws)
+g.replay()
+torch.cuda.synchronize()
+call.check(out)
+assert torch.equal(out, call.run())
+print("done")
+"""
+
+
+@pytest.mark.parametrize("rows,dim,store", [(1, 256, "bf16"), (1, 128, "q8_0"), (60, 128, "bf16")])
+def test_the_first_call_of_a_process_is_captured(rows, dim, store):
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(os.path.abspath(ekv.__file__)), os.environ.get("PYTHONPATH", "")]))
+    r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST, str(rows), str(dim), store], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
