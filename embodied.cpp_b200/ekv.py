@@ -465,18 +465,22 @@ class Pool:
             check(code, "ekv_rope_append")
 
     def _rope_rows(self, q, q_out, k, v):
-        """Heads, pointers and row distances of a rotary append's rows."""
+        """Heads, pointers and row distances of a rotary append's rows. (Shapes and distances are asked for once: each takes 0.2 us.)"""
         q_heads = q_stride = kv_stride = 0
         qp = q_to = kp = vp = None
         if q is not None:
-            q_heads, q_stride = _rows(q, self.head_dim, "q")
-            if q_out is None or q_out.shape != q.shape or not q_out.is_contiguous():
+            shape = q.shape
+            q_heads, q_stride = _rows_of(shape, q.stride(), self.head_dim, "q")
+            if q_out is None or q_out.shape != shape or not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous and of q's shape")
             qp, q_to = q.data_ptr(), q_out.data_ptr()
         if k is not None or v is not None:
-            if k is None or v is None or k.shape != v.shape or k.stride() != v.stride():
+            if k is None or v is None:
                 raise ValueError("k and v must have one shape and the same distance from row to row")
-            kv_heads, kv_stride = _rows(k, self.head_dim, "k and v")
+            shape, steps = k.shape, k.stride()
+            if shape != v.shape or steps != v.stride():
+                raise ValueError("k and v must have one shape and the same distance from row to row")
+            kv_heads, kv_stride = _rows_of(shape, steps, self.head_dim, "k and v")
             if kv_heads != self.kv_heads:
                 raise ValueError("k and v must have the pool's KV heads")
             kp, vp = k.data_ptr(), v.data_ptr()
@@ -488,9 +492,9 @@ class Pool:
         if norm.dim not in (0, self.head_dim):
             raise ValueError("the norm's weights must have head_dim values")
         q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
-        for t in (q, q_out, k, v):
-            if t is not None and t.dtype is not norm.bf16:
-                raise ValueError("q, q_out, k and v must be bf16")
+        bf16 = norm.bf16
+        if not ((qp is None or q.dtype is bf16 and q_out.dtype is bf16) and (kp is None or k.dtype is bf16 and v.dtype is bf16)):
+            raise ValueError("q, q_out, k and v must be bf16")
         code = lib.ekv_norm_rope_append(self.h, rope.h, norm.ref, layer, n_rows.numel(), None if kp is None else seq_ids.data_ptr(),
                                         None if kp is None else dst_pos.data_ptr(), n_rows.data_ptr(), src_row.data_ptr(),
                                         max_rows, positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride,
@@ -703,8 +707,13 @@ def project_qkv_rope(pool: "Pool", layer, seq_ids, x, wq, wk, wv, positions, rop
 
 def _rows(t, head_dim, name):
     """Heads of a [rows, heads, head_dim] tensor and the elements from row to row; a row must be adjacent."""
-    if t.dim() == 3:
-        (rows, heads, dim), (to_row, to_head, to_col) = t.shape, t.stride()
+    return _rows_of(t.shape, t.stride(), head_dim, name)
+
+
+def _rows_of(shape, steps, head_dim, name):
+    if len(shape) == 3:
+        rows, heads, dim = shape
+        to_row, to_head, to_col = steps
         if dim == head_dim and to_col == 1 and (to_head == dim or heads <= 1):
             return heads, to_row if rows > 1 else heads * dim
     raise ValueError(f"{name} must be [rows, heads, {head_dim}] with adjacent heads")
