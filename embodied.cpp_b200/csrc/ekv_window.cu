@@ -44,6 +44,49 @@ struct FCfg {
     static_assert(NST >= 2, "two stages");
 };
 
+// Block ids of the entries that a request's rows see, in the order of their keys: the first `front` entries of its table, then those from
+// the window's on, as one list, of which kTableWindow are in shared memory. (Two lists, read 32 entries at a time, took 2.3 us before the
+// first tile of a row with a window of 1024 and blocks of 16 was on its way; one, with all loads at once, 1.) Used by one warp.
+struct SeenBlocks {
+    int *blocks;
+    int request, front, skip, lo, n;
+    __device__ __forceinline__ void reset(int *mem) {
+        blocks = mem;
+        request = -1;
+    }
+    __device__ __forceinline__ int place(int entry) const { return entry < front ? entry : entry - skip; }
+    // Entries [first, last] of the request, of which all up to `end` will be wanted in turn.
+    __device__ __forceinline__ void want(const PoolView &p, int b, int seq, const Span &sp, int first, int last, int end, int lane) {
+        if (b != request) {
+            auto entry = [&](int slot) { return p.bt_shift >= 0 ? slot >> p.bt_shift : slot / p.block_tokens; };
+            request = b;
+            front = sp.front > 0 ? entry(sp.front - 1) + 1 : 0;
+            skip = max(0, entry(sp.lo) - front);
+            n = 0;
+        }
+        first = place(first);
+        if (n > 0 && first >= lo && place(last) < lo + n) return;
+        __syncwarp();
+        lo = first;
+        n = min(kTableWindow, place(end) + 1 - first);
+        int e[kTableWindow / 32], v[kTableWindow / 32];
+#pragma unroll
+        for (int j = 0; j < kTableWindow / 32; ++j) {
+            const int i = first + lane + 32 * j;
+            e[j] = i < front ? i : i + skip;
+            v[j] = lane + 32 * j < n && e[j] < p.max_blocks_per_seq ? p.block_tables[(int64_t)seq * p.max_blocks_per_seq + e[j]] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kTableWindow / 32; ++j) {
+            if (lane + 32 * j >= n) continue;
+            const bool fine = v[j] >= 0 && v[j] < p.n_blocks;
+            if (!fine) report_error(p.status, DEV_ERR_BAD_BLOCK, seq, e[j], v[j]);
+            blocks[lane + 32 * j] = fine ? v[j] : -1;
+        }
+        __syncwarp();
+    }
+};
+
 template <int NST>
 struct FShared {
     uint64_t full_k[NST], full_v[NST], empty[NST];
@@ -115,8 +158,8 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
         }
     };
     bool ok = true;
-    TableWindow tw;  // (the feeder's)
-    tw.reset(sh.table);
+    SeenBlocks seen;  // (the feeder's)
+    seen.reset(sh.table);
     uint32_t base = rg.base;
     WinReq rq{-1, 0, 0};
     int rq_of = -1;
@@ -147,8 +190,8 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
             const int last_entry = rq.seq >= 0 ? sp.last / a.pool.block_tokens : 0;
             auto find = [&](int j) {
                 return find_run<kTile>(
-                    a, sp, g, j * kTile, lane & 15, [&](int e0, int e1) { tw.want(a.pool, rq.seq, e0, e1, max(e1, last_entry), lane); },
-                    [&](int e) { return tw.blocks[e - tw.lo]; });
+                    a, sp, g, j * kTile, lane & 15, [&](int e0, int e1) { seen.want(a.pool, b, rq.seq, sp, e0, e1, last_entry, lane); },
+                    [&](int e) { return seen.blocks[seen.place(e) - seen.lo]; });
             };
             Run next{nullptr, 0, 0, 0};
             if (t0 < t1) next = find(t0);  // (a request without rows has no tiles, and its slots mean nothing)
@@ -335,6 +378,76 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
                     ok = warp_wait(smem_addr(&sh.full_v[st]), par, abort);
                     if (!ok) *abort = 1;
                     if constexpr (!Q8) {
+                        if (masked) {
+                            // 0 * inf would reach rows that do not see a value. So the values of keys that no row sees become 0, and
+                            // those that are not finite of keys that some rows see (rare) go to those rows one by one. In shared
+                            // memory, of which the warp's keys are its own, so that the products below have one form: with this among
+                            // them a first masked tile waited for 4000 cycles of instructions.
+                            uint32_t some = 0, every = 0xffffu;
+#pragma unroll
+                            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    if (p_of[n][e] >= 0) {
+                                        some |= vis[n][e];
+                                        every &= vis[n][e];
+                                    }
+                            some = __reduce_or_sync(0xffffffffu, some);
+                            const bool differ = __reduce_and_sync(0xffffffffu, every) != some;
+                            constexpr int U = D / 8;
+                            uint8_t *const vt = smem + st * C::STAGE + C::V_OFF;
+                            auto marks = [](const uint4 &v) {  // its values that are not finite, a bit each
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                uint32_t m = 0;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) m |= ((w[k] & 0x7f80u) == 0x7f80u ? 1u : 0u) << 2 * k | ((w[k] & 0x7f800000u) == 0x7f800000u ? 2u : 0u) << 2 * k;
+                                return m;
+                            };
+                            uint32_t bad = 0;
+#pragma unroll 4
+                            for (int i = lane; i < 16 * U; i += 32) {
+                                uint4 *const at = (uint4 *)(vt + bf16_off<D>(key0 + i / U, i % U * 8));
+                                if (!((some >> (i / U)) & 1u)) *at = make_uint4(0, 0, 0, 0);
+                                else if (differ) bad |= marks(*at);
+                            }
+                            if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll 1
+                                for (int i = lane; i < 16 * U; i += 32) {
+                                    uint4 *const at = (uint4 *)(vt + bf16_off<D>(key0 + i / U, i % U * 8));
+                                    uint4 v = *at;
+                                    const uint32_t m = marks(v);
+                                    for (uint32_t lanes = __ballot_sync(0xffffffffu, m != 0); lanes; lanes &= lanes - 1) {
+                                        const int from = __ffs(lanes) - 1, key = __shfl_sync(0xffffffffu, i, from) / U, unit = __shfl_sync(0xffffffffu, i, from) % U;
+                                        const uint32_t w[4] = {__shfl_sync(0xffffffffu, v.x, from), __shfl_sync(0xffffffffu, v.y, from),
+                                                               __shfl_sync(0xffffffffu, v.z, from), __shfl_sync(0xffffffffu, v.w, from)};
+                                        const uint32_t of = __shfl_sync(0xffffffffu, m, from);
+#pragma unroll
+                                        for (int k = 0; k < 8; ++k) {
+                                            if (kq != k || !((of >> k) & 1u)) continue;  // column 8 unit + k is this lane's
+                                            const float y = __uint_as_float(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+#pragma unroll
+                                            for (int ds = 0; ds < KS; ++ds)
+#pragma unroll
+                                                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                                                    for (int x = 0; x < 4; ++x)
+                                                        if (unit == 2 * ds + (x >> 1) && ((vis[n][x & 1] >> key) & 1u)) o[n][ds][x] += y;
+                                        }
+                                    }
+                                    if (m & 1u) v.x &= 0xffff0000u;
+                                    if (m & 2u) v.x &= 0xffffu;
+                                    if (m & 4u) v.y &= 0xffff0000u;
+                                    if (m & 8u) v.y &= 0xffffu;
+                                    if (m & 16u) v.z &= 0xffff0000u;
+                                    if (m & 32u) v.z &= 0xffffu;
+                                    if (m & 64u) v.w &= 0xffff0000u;
+                                    if (m & 128u) v.w &= 0xffffu;
+                                    if (m) *at = v;
+                                }
+                            }
+                            fence_proxy_async();  // the next tile comes here through the copy engine
+                            __syncwarp();
+                        }
                         uint32_t pr[NR][2];
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
@@ -348,35 +461,6 @@ __global__ void __launch_bounds__(FCfg<D, Q8, NR>::THREADS, FCfg<D, Q8, NR>::CTA
                         for (int ds = 0; ds < KS; ++ds) {
                             uint32_t vf[4];
                             load_v_cols<D>(sv, key0, ds, lane, vf);
-                            if (masked) {
-                                // Values that are not finite leave the product: 0 * inf would reach rows that do not see them. Rows
-                                // that do get them one by one (rare). Element (i, h): key 2 c + h + 8 (i >> 1), column kq + 8 (i & 1).
-                                bool any = false;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) any = any || (vf[i] & 0x7f80u) == 0x7f80u || (vf[i] & 0x7f800000u) == 0x7f800000u;
-                                if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                                        for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-                                            for (int from = 0; from < 4; ++from) {
-                                                const uint32_t w = __shfl_sync(0xffffffffu, vf[i], (lane & ~3) + from);
-                                                const float y = __uint_as_float(h ? w & 0xffff0000u : w << 16);
-                                                const int k = 2 * from + h + 8 * (i >> 1);
-#pragma unroll
-                                                for (int n = 0; n < NR; ++n)
-#pragma unroll
-                                                    for (int e = 0; e < 2; ++e)
-                                                        if (!isfinite(y) && ((vis[n][e] >> k) & 1u)) o[n][ds][e + 2 * (i & 1)] += y;
-                                            }
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        if ((vf[i] & 0x7f80u) == 0x7f80u) vf[i] &= 0xffff0000u;
-                                        if ((vf[i] & 0x7f800000u) == 0x7f800000u) vf[i] &= 0xffffu;
-                                    }
-                                }
-                            }
 #pragma unroll
                             for (int n = 0; n < NR; ++n) mma_bf16(o[n][ds], vf, pr[n][0], pr[n][1]);
                         }
