@@ -10,10 +10,10 @@
 // tile's chain of scores, maximum, exponentials, P, next products. Two row tiles fill it for the special-function unit (1024 of a
 // 64-key tile's 2450 cycles) and the tensor pipe (1300 of them); a unit's end and beginning take 9000 cycles, beside 12 tiles of a
 // window of 1024 a quarter.
-// 32 / 8 heads of 128: a prompt of 16384 tokens 2305 us (954 TFLOP/s of the products that rows see, 56% of a measured bf16 product), over
-// 8-bit pages 2555; 8 prompts of up to 4096, window 1024 and 4 first tokens: 660 us (600), over 8-bit pages 775. 8 / 1 heads of 256, 8192
-// tokens: 300 us (915).
-// Measured and left out, the first two figures again: 128 keys a tile with one S tile 2386 and 773 us; two warps to a row in place
+// 32 / 8 heads of 128: a prompt of 16384 tokens 2284 us (963 TFLOP/s of the products that rows see, 57% of a measured bf16 product), over
+// 8-bit pages 2561; 8 prompts of up to 4096, window 1024 and 4 first tokens: 625 us (639), over 8-bit pages 764. 8 / 1 heads of 256, 8192
+// tokens: 298 us (923).
+// Measured and left out, the first prompt's and the eight's times, which were 2335 and 637 us then: 128 keys a tile with one S tile 2386 and 773 us; two warps to a row in place
 // of one for head_dim 128 2654 and 718 (for 256, where one row tile leaves the schedulers a warp each, 343 instead of 396); a part of
 // the exponentials by polynomial 2333 and 645 (an eighth), 2448 and 711 (a quarter).
 
@@ -607,7 +607,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
         const int row = v.row0 + slot * kTileRows + r, t = row_token(a, row);
         const long long q_at = ((long long)v.rq.src + t) * a.q_stride + (long long)(v.g * a.group + row - t * a.group) * D;
         const uint32_t have = __ballot_sync(0xffffffffu, row < v.rq.n * a.group);
-#pragma unroll 8
+#pragma unroll 2  // (more is slower: the end of a unit waits for its instructions)
         for (int k = 0; k < QU / SHARE; ++k) {
             const int i = (k * SHARE + half) * 32 + lane, rr = i / QU, uu = i % QU;
             const long long from = __shfl_sync(0xffffffffu, q_at, rr);
