@@ -13,9 +13,9 @@
 // 32 / 8 heads of 128: a prompt of 16384 tokens 2284 us (963 TFLOP/s of the products that rows see, 57% of a measured bf16 product), over
 // 8-bit pages 2561; 8 prompts of up to 4096, window 1024 and 4 first tokens: 625 us (639), over 8-bit pages 764. 8 / 1 heads of 256, 8192
 // tokens: 298 us (923).
-// Measured and left out, the first prompt's and the eight's times, which were 2335 and 637 us then: 128 keys a tile with one S tile 2386 and 773 us; two warps to a row in place
-// of one for head_dim 128 2654 and 718 (for 256, where one row tile leaves the schedulers a warp each, 343 instead of 396); a part of
-// the exponentials by polynomial 2333 and 645 (an eighth), 2448 and 711 (a quarter).
+// Measured and left out, with the first prompt's and the eight's times, which were 2335 and 637 us then: 128 keys a tile with one S tile
+// 2386 and 773; two warps to a row in place of one for head_dim 128 2654 and 718 (for 256, where one row tile leaves the schedulers a
+// warp each, 343 instead of 396); a part of the exponentials by polynomial 2333 and 645 (an eighth), 2448 and 711 (a quarter).
 
 #include "ekv_window.cuh"
 
