@@ -108,6 +108,7 @@ int launch_pages_n(const PoolView &p, const BlockCopy *copies, int n_copies, con
 
 // ---- compaction ----
 constexpr int kRowLoads = 16;   // 16-byte units of a thread and chunk
+constexpr int kListLoads = 8;   // entries of a thread and round, while rows stay
 constexpr int kMaxCluster = 8;
 
 // Where a row of the chunk comes from and goes to: tiles, and rows inside them. A row that stays has to < 0, and a source that
@@ -153,8 +154,11 @@ __device__ __forceinline__ void store_row_scales(uint8_t *dst, int bytes, const 
 // EVEN: a row's units divide the threads, so that a thread keeps to one unit of its rows.
 template <bool Q8, bool EVEN>
 __global__ void __launch_bounds__(kThreads, 2) compact_kernel(const CompactArgs a, int cluster) {
+    __shared__ int s_off[2];
     __shared__ Move s_moves[3][kThreads];  // (three: a thread may store a chunk while another resolves the one after the next)
     const PoolView &p = a.pool;
+    if (threadIdx.x < 2) s_off[threadIdx.x] = INT32_MAX;
+    __syncthreads();
     decode::grid_wait();
     const int strip = blockIdx.x / cluster, rank = blockIdx.x - strip * cluster, tid = threadIdx.x;
     const int heads = 2 * p.kv_heads, kvh = strip % heads, lb = strip / heads, b = lb % a.n_batch, layer = a.layer0 + lb / a.n_batch;
@@ -170,14 +174,27 @@ __global__ void __launch_bounds__(kThreads, 2) compact_kernel(const CompactArgs 
         return;
     }
     const int32_t *slots = a.slots + (int64_t)b * a.slot_stride;
-    // rows below `first` stay where they are: a search of 256 steps at a time
+    // Rows below `first` stay where they are. Every entry is looked at, up to the first that is not its own place: a list may be in order
+    // again behind one that is not, and that one is to be reported. (60 000 rows of which 59 000 stay: 14 us; a search that trusted the
+    // list took 5.)
     int first = 0;
-    for (int span = n; span > 0;) {
-        const int step = (span + kThreads - 1) / kThreads;
-        const int64_t i = first + (tid + 1ll) * step - 1;  // the last row of the thread's part
-        const int whole = __syncthreads_count(i < first + span && __ldg(slots + i) == i);
-        first += whole * step;
-        span = step == 1 ? 0 : min(step, n - first);
+    for (int round = 0; first < n; ++round) {
+        int at[kListLoads], off = INT32_MAX;
+#pragma unroll
+        for (int j = 0; j < kListLoads; ++j) at[j] = tid + j * kThreads < n - first ? __ldg(slots + first + tid + j * kThreads) : -1;
+#pragma unroll
+        for (int j = kListLoads - 1; j >= 0; --j)
+            if (tid + j * kThreads < n - first && at[j] != first + tid + j * kThreads) off = tid + j * kThreads;
+        off = __reduce_min_sync(0xffffffffu, off);
+        // (two, in turn: a thread may look at one round's while another is in the next)
+        if (off != INT32_MAX && (tid & 31) == 0) atomicMin(&s_off[round & 1], off);
+        __syncthreads();
+        off = s_off[round & 1];
+        if (off != INT32_MAX) {
+            first += off;
+            break;
+        }
+        first += min(n - first, kThreads * kListLoads);
     }
     const int D = p.head_dim, wlog = decode::log2_of(p.swz_bytes), bt = p.block_tokens;
     const int per = Q8 ? D / 16 : D / 8;  // units of a row

@@ -263,6 +263,53 @@ def test_compact_reports_bad_lists():
     assert torch.equal(bytes_of(c.pool, 0, c.seqs[0], 2).view(2, 2, -1), want[:, [5, 6]])
 
 
+def in_place_again(n, **at):
+    """0 .. n - 1 with some entries replaced."""
+    x = list(range(n))
+    for i, s in at.items():
+        x[int(i[1:])] = s
+    return x
+
+
+@pytest.mark.parametrize("store", ["bf16", "q8_0"])
+@pytest.mark.parametrize("slots", [in_place_again(5, _1=7), [0, 0, 2, 3], [0, 1, 1, 3], in_place_again(5, _0=-2), in_place_again(6, _2=700),
+                                   in_place_again(256, _100=650), in_place_again(600, _100=650), in_place_again(600, _101=99, _300=640),
+                                   in_place_again(690, _255=256, _256=255), in_place_again(513, _511=2 ** 31 - 1)])
+def test_compact_reports_bad_entries_before_rows_in_place(store, slots):
+    """An entry that is out of order, or a row that moves before it, is seen where later rows are in their places again."""
+    n, lens = len(slots), [700, 700]
+    c = dc.Cache(lens, 2, 64, store=store, block=16, layers=2, seed=8)
+    before = {(layer, s): bytes_of(c.pool, layer, s, 700).view(2, 700, -1) for layer in range(2) for s in c.seqs}
+    good = list(range(0, 2 * n, 2))[:350]
+    lists = [slots, good + [0] * (n - len(good))]
+    c.pool.compact(0, 2, c.seq_ids, dc.ints(lists), dc.ints([n, len(good[:n])]))
+    assert c.pool.status() == ekv.DEV_ERR_BAD_POS
+    for (layer, s), rows in before.items():
+        want = rows.clone()
+        if s == c.seqs[0]:
+            for i, x in enumerate(slots):
+                if x >= i and x < 700 and x > (slots[i - 1] if i else -1):
+                    want[:, i] = rows[:, x]
+        else:
+            want[:, :len(good[:n])] = rows[:, good[:n]]
+        assert torch.equal(bytes_of(c.pool, layer, s, 700).view(2, 700, -1), want)
+
+
+@pytest.mark.parametrize("n", [0, 1, 255, 256, 257, 4096, 4097, 9000])
+@pytest.mark.parametrize("first", [0, 1, 255, 256, 4095, 4096, 8191, 8999])
+def test_compact_behind_rows_in_place(n, first):
+    """Rows before the first that moves stay, however many they are."""
+    c = dc.Cache([10000], 1, 32, store="q8_0", block=64, layers=1, seed=8)
+    lists = [i if i < first else i + 3 + i % 7 // 6 for i in range(n)]
+    lists = sorted(set(lists))
+    rows = bytes_of(c.pool, 0, c.seqs[0], 10000).view(2, 10000, -1)
+    c.pool.compact(0, 1, c.seq_ids, dc.ints([lists + [0]]), dc.ints([len(lists)]))
+    assert c.pool.status() == 0
+    want = rows.clone()
+    want[:, :len(lists)] = rows[:, lists]
+    assert torch.equal(bytes_of(c.pool, 0, c.seqs[0], 10000).view(2, 10000, -1), want)
+
+
 def test_compact_replayed_and_on_another_stream():
     c = dc.Cache([600, 300], 2, 128, block=32, layers=2, seed=6)
     lists = [kept_slots(600, 1, 0.8)[:300], kept_slots(300, 2, 0.9)[:200]]
