@@ -559,14 +559,12 @@ int ekv_seq_own(ekv_pool *p, int32_t id, int32_t pos0, int32_t n_tokens, ekv_str
     ekv_pool::Seq &q = p->seqs[(size_t)id];
     const int32_t bt = p->cfg.block_tokens, have = (int32_t)q.blocks.size();
     if (pos0 < 0 || n_tokens < 0 || (int64_t)pos0 + n_tokens > (int64_t)have * bt) return EKV_ERR_RANGE;
-    if (n_tokens == 0) return EKV_OK;
+    if (n_tokens == 0) return ekv_pool_sync(p, stream);
     const int32_t first = pos0 / bt, last = (int32_t)(((int64_t)pos0 + n_tokens - 1) / bt);
     int32_t shared = 0;
     for (int32_t i = first; i <= last; ++i) shared += p->holders[(size_t)q.blocks[(size_t)i]] > 1;
-    if (shared == 0) {
-        // what was shared once may still be marked so on the device
-        return p->unshared ? ekv_pool_sync(p, stream) : EKV_OK;
-    }
+    // (what was shared once may still be marked so on the device, and the sequence may have grown)
+    if (shared == 0) return ekv_pool_sync(p, stream);
     if ((int32_t)p->free_blocks.size() < shared) return EKV_ERR_POOL_EXHAUSTED;
     const DeviceScope dev_scope(p);
     if (p->cfg.device >= 0 && dev_scope.rc()) return dev_scope.rc();

@@ -131,7 +131,8 @@ int ekv_seq_fork(ekv_pool *pool, int32_t n, const int32_t *parents, const int32_
                  ekv_stream_t stream);
 /* Copies of the shared blocks that hold positions [pos0, pos0 + n_tokens) of the sequence, which is then their only holder and
  * may write them (before rows of a fork are overwritten, evicted by weight or compacted, or after a fork was cut shorter and
- * before it grows again). The table is uploaded. EKV_ERR_POOL_EXHAUSTED leaves the pool unchanged. */
+ * before it grows again). Changed tables are uploaded as by ekv_pool_sync, whether or not a block was shared.
+ * EKV_ERR_POOL_EXHAUSTED leaves the pool unchanged. */
 int ekv_seq_own(ekv_pool *pool, int32_t seq_id, int32_t pos0, int32_t n_tokens, ekv_stream_t stream);
 
 /* ---- predicted tokens (LingBot-VA's rollout appends predicted K/V, attends, then rolls them back

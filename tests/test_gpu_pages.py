@@ -167,6 +167,23 @@ def test_own_copies_many_blocks_of_every_layer():
         assert torch.equal(bytes_of(p, layer, kid, 2405), want[layer]) and not torch.equal(bytes_of(p, layer, 0, 2405), want[layer])
 
 
+def test_own_uploads_the_table():
+    """What follows ekv_seq_own sees the sequence's length and blocks, whether or not a block was shared."""
+    c = cache([40, 20], 1, 64, block=16, layers=1)
+    p = c.pool
+    kid, = p.seq_fork([0], [40])
+    k, v = rand(1, 30, 1, 64), rand(2, 30, 1, 64)
+    for seq, pos, n in ((kid, 40, 30), (0, 40, 5), (1, 20, 28)):
+        p.seq_resize(seq, pos + n)
+        p.seq_own(seq, pos, n)  # blocks of its own
+        p.append(0, dc.ints([seq]), dc.ints([pos]), dc.ints([n]), dc.ints([0]), n, k, v)
+        assert p.status() == 0, seq
+    p.seq_resize(kid, 75)
+    p.seq_own(kid, 75, 0)  # no block at all
+    p.append(0, dc.ints([kid]), dc.ints([70]), dc.ints([5]), dc.ints([0]), 5, k, v)
+    assert p.status() == 0
+
+
 def test_evict_with_shared_blocks():
     """Rows move where the sequence owns the blocks they go to; a move into a shared block is reported."""
     c = cache([64], 1, 64, block=16, layers=1)
