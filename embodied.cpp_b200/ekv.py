@@ -270,6 +270,27 @@ def _index(t, n, name, bits=32):
     return t.data_ptr()
 
 
+def _rope_index(seq_ids, dst_pos, n_rows, src_row, positions, rows, append):
+    """Requests of a rotary append and the pointers of its arrays: 32-bit integers, one for each request, positions for each of
+    `rows` rows. (As _index asks, but the usual case in line: five calls of it take 3 us of one that takes 9, this 1.)"""
+    global _i32
+    n, i32 = n_rows.numel(), _i32
+    try:
+        # (of one element there is no distance to the next)
+        if (n_rows.dtype is i32 and src_row.dtype is i32 and positions.dtype is i32 and src_row.numel() >= n and positions.numel() >= rows
+                and (n == 1 or n_rows.is_contiguous() and src_row.is_contiguous()) and (rows == 1 or positions.is_contiguous())):
+            if not append:
+                return n, None, None, n_rows.data_ptr(), src_row.data_ptr(), positions.data_ptr()
+            if (seq_ids.dtype is i32 and dst_pos.dtype is i32 and seq_ids.numel() >= n and dst_pos.numel() >= n
+                    and (n == 1 or seq_ids.is_contiguous() and dst_pos.is_contiguous())):
+                return n, seq_ids.data_ptr(), dst_pos.data_ptr(), n_rows.data_ptr(), src_row.data_ptr(), positions.data_ptr()
+    except AttributeError:  # (an array of the library, or none: the call refuses it)
+        pass
+    _i32 = _ints(32)[0]
+    return (n, _index(seq_ids, n, "seq_ids") if append else None, _index(dst_pos, n, "dst_pos") if append else None,
+            _index(n_rows, n, "n_rows"), _index(src_row, n, "src_row"), _index(positions, rows, "positions"))
+
+
 def _ints(bits):
     import torch
     return (torch.int32, torch.uint32) if bits == 32 else (torch.int64, torch.uint64)
@@ -457,19 +478,21 @@ class Pool:
         """ekv_rope_append: turn q [rows, q_heads, head_dim] into q_out and k into the pages beside v ([rows, kv_heads,
         head_dim]), all bf16 and by source row. q, k and v may be slices of one [rows, columns] projection output:
         rows may be any distance apart, a row's heads are adjacent. Either pair may be left out."""
-        q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
-        code = lib.ekv_rope_append(self.h, rope.h, layer, n_rows.numel(), None if kp is None else _ptr(seq_ids),
-                                   None if kp is None else _ptr(dst_pos), n_rows.data_ptr(), src_row.data_ptr(), max_rows,
-                                   positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride, _stream(stream))
+        _, q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
+        # (positions may end with the last row that a request uses, which only the device knows)
+        n, seqs, dst, counts, src, pos = _rope_index(seq_ids, dst_pos, n_rows, src_row, positions, 0, kp is not None)
+        code = lib.ekv_rope_append(self.h, rope.h, layer, n, seqs, dst, counts, src, max_rows, pos, q_heads, qp, q_stride, q_to, kp, vp,
+                                   kv_stride, _stream(stream))
         if code:
             check(code, "ekv_rope_append")
 
     def _rope_rows(self, q, q_out, k, v):
-        """Heads, pointers and row distances of a rotary append's rows. (Shapes and distances are asked for once: each takes 0.2 us.)"""
-        q_heads = q_stride = kv_stride = 0
+        """Rows, heads, pointers and row distances of a rotary append. (Shapes and distances are asked for once: each takes 0.2 us.)"""
+        rows = q_heads = q_stride = kv_stride = 0
         qp = q_to = kp = vp = None
         if q is not None:
             shape = q.shape
+            rows = shape[0]
             q_heads, q_stride = _rows_of(shape, q.stride(), self.head_dim, "q")
             if q_out is None or q_out.shape != shape or not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous and of q's shape")
@@ -484,21 +507,22 @@ class Pool:
             if kv_heads != self.kv_heads:
                 raise ValueError("k and v must have the pool's KV heads")
             kp, vp = k.data_ptr(), v.data_ptr()
-        return q_heads, qp, q_stride, q_to, kp, vp, kv_stride
+            rows = max(rows, shape[0])
+        return rows, q_heads, qp, q_stride, q_to, kp, vp, kv_stride
 
     def norm_rope_append(self, rope, norm, layer, seq_ids, dst_pos, n_rows, src_row, max_rows, positions, *, q=None, q_out=None,
                          k=None, v=None, stream=None):
-        """ekv_norm_rope_append: rope_append with an RMS norm (HeadNorm) of every q and k head before its rotation, or after."""
+        """ekv_norm_rope_append: rope_append with an RMS norm (HeadNorm) of every q and k head before its rotation, or after. positions
+        has a value for every row of q and k."""
         if norm.dim not in (0, self.head_dim):
             raise ValueError("the norm's weights must have head_dim values")
-        q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
+        rows, q_heads, qp, q_stride, q_to, kp, vp, kv_stride = self._rope_rows(q, q_out, k, v)
         bf16 = norm.bf16
         if not ((qp is None or q.dtype is bf16 and q_out.dtype is bf16) and (kp is None or k.dtype is bf16 and v.dtype is bf16)):
             raise ValueError("q, q_out, k and v must be bf16")
-        code = lib.ekv_norm_rope_append(self.h, rope.h, norm.ref, layer, n_rows.numel(), None if kp is None else seq_ids.data_ptr(),
-                                        None if kp is None else dst_pos.data_ptr(), n_rows.data_ptr(), src_row.data_ptr(),
-                                        max_rows, positions.data_ptr(), q_heads, qp, q_stride, q_to, kp, vp, kv_stride,
-                                        _stream(stream))
+        n, seqs, dst, counts, src, pos = _rope_index(seq_ids, dst_pos, n_rows, src_row, positions, rows, kp is not None)
+        code = lib.ekv_norm_rope_append(self.h, rope.h, norm.ref, layer, n, seqs, dst, counts, src, max_rows, pos, q_heads, qp, q_stride,
+                                        q_to, kp, vp, kv_stride, _stream(stream))
         if code:
             check(code, "ekv_norm_rope_append")
 

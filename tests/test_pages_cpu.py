@@ -223,3 +223,58 @@ def test_norm_rope_append_refusals():
     assert call(norm=dict(weight_dtype=ekv.DTYPE_F16)) == ekv.ERR_UNSUPPORTED
     assert call(pl=pool(head_dim=48)) == ekv.ERR_INVALID_ARG  # more rotated columns than a head has
     assert L.ekv_norm_rope_append(p.h, rope.h, None, 0, 1, P, P, P, P, 1, P, 4, P, 0, P, P, P, 0, None) == ekv.ERR_INVALID_ARG
+
+
+class NoStream:
+    cuda_stream = 0
+
+
+@pytest.mark.parametrize("how", ["rope", "norm"])
+def test_rotary_appends_refuse_other_index_arrays(how):
+    """Arrays of another integer type, with gaps, or too short for the requests or rows would be read wrongly, or past their ends."""
+    torch = pytest.importorskip("torch")
+    p, rope, norm = pool(), ekv.Rope(device=-1, rotary_dims=64), ekv.HeadNorm()
+    kv_heads = p.cfg.kv_heads
+    q = torch.zeros(9, 4, 64, dtype=torch.bfloat16)
+    k = torch.zeros(9, kv_heads, 64, dtype=torch.bfloat16)
+    good = dict(seq_ids=torch.zeros(3, dtype=torch.int32), dst_pos=torch.zeros(4, dtype=torch.int32), n_rows=torch.zeros(3, dtype=torch.int32),
+                src_row=torch.zeros(3, dtype=torch.int32), positions=torch.zeros(9, dtype=torch.int32))
+
+    def call(rows, **kw):
+        a = {**good, **kw}
+        args = (0, a["seq_ids"], a["dst_pos"], a["n_rows"], a["src_row"], 3, a["positions"])
+        if how == "rope":
+            p.rope_append(rope, *args, **rows, stream=NoStream)
+        else:
+            p.norm_rope_append(rope, norm, *args, **rows, stream=NoStream)
+
+    for rows in (dict(q=q, q_out=q), dict(k=k, v=k), dict(q=q, q_out=q, k=k, v=k)):
+        for kw in ({}, {name: t.to(torch.uint32) for name, t in good.items()}, dict(positions=torch.zeros(30, dtype=torch.int32)),
+                   dict(seq_ids=ekv.DevArray(0x10000, 3), dst_pos=ekv.DevArray(0x10000, 3))):
+            with pytest.raises(ekv.EkvError) as e:
+                call(rows, **kw)
+            assert e.value.code == ekv.ERR_UNSUPPORTED  # no device: the arrays have passed
+        append = "k" in rows
+        for name in good:
+            if name in ("seq_ids", "dst_pos") and not append:
+                with pytest.raises(ekv.EkvError) as e:  # not looked at
+                    call(rows, **{name: None})
+                assert e.value.code == ekv.ERR_UNSUPPORTED
+                continue
+            n = good[name].numel()
+            bad = [torch.zeros(n, dtype=torch.int64), torch.zeros(n), torch.zeros(2 * n, dtype=torch.int32)[::2]]
+            if name in ("seq_ids", "dst_pos"):
+                bad += [torch.zeros(2, dtype=torch.int32), ekv.DevArray(0x10000, 2)]
+            if name == "src_row":
+                bad.append(torch.zeros(2, dtype=torch.int32))
+            if name == "n_rows":
+                bad.append(torch.zeros(5, dtype=torch.int32))  # more requests than the other arrays have
+            if name == "positions" and how == "norm":
+                bad += [torch.zeros(8, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)]
+            for t in bad:
+                with pytest.raises(ValueError):
+                    call(rows, **{name: t})
+        if append:
+            with pytest.raises(ekv.EkvError) as e:
+                call(rows, seq_ids=None)
+            assert e.value.code == ekv.ERR_INVALID_ARG
