@@ -40,6 +40,10 @@ struct WCfg {
     static constexpr int NSF = NS > NSB ? NS : NSB;   // barriers of S: a tile's S may be done while S of the one before is not read
     // a reference that is 2^LIMIT too low does not move: P and what is summed are floating point numbers, and only their range counts
     static constexpr float LIMIT = Q8 ? 8.0f : 24.0f;
+    // f16 ends at 2^16 and has steps of 2^-24 below 2^-14: P is 2^HEADROOM times what it stands for, as its sum is, so that a key is off by
+    // 2^-32 of its row's largest at most and not by 2^-25 (one heavy key before 60 000 light ones, 26 bits below it: those were lost)
+    static constexpr float HEADROOM = Q8 ? 7.0f : 0.0f;
+    static_assert(!Q8 || LIMIT + HEADROOM < 16.0f, "P in f16");
     static constexpr uint32_t SBO = 16 * D, LAYOUT = 2;
     static constexpr int KV_BYTES = BN * D * 2, Q_BYTES = kTileRows * D * 2;
     static constexpr int NR = D > 128 ? 2 : 4, RAW = BN * D + BN * (D / 32) * 2;  // Q8: tiles of K, and of V, as they are stored
@@ -729,7 +733,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                         }
                     }
                 }
-                const float neg = m == -INFINITY ? 0.0f : -m;
+                const float neg = m == -INFINITY ? 0.0f : C::HEADROOM - m;
                 const uint64_t neg2 = pair_of(neg, neg);
 #pragma unroll
                 for (int c = 0; c < KEYS / 32; ++c) {

@@ -262,3 +262,29 @@ def test_values_beyond_f16():
     call.c.pool.append(0, call.c.seq_ids, dc.ints([7]), dc.ints([1]), dc.ints([0]), 1, k, v)
     call.run()
     assert call.c.pool.status() == ekv.DEV_ERR_F16_RANGE
+
+
+@pytest.mark.parametrize("dim,rows,hq", [(64, 20, 1), (128, 3, 8), (256, 40, 1)])
+@pytest.mark.parametrize("below", [14.0, 18.0, 19.5])
+def test_many_small_keys_behind_a_heavy_one(dim, rows, hq, below):
+    """8-bit pages, many rows: the output is made of probabilities far below the row's largest, whose value is 0. P is f16 with 7 bits of
+    headroom: a key is off by half of the smallest step at most, 2^-25 of 2^7, 2^-32 of the row's largest, beside the relative terms
+    (values are at most 1)."""
+    past = 60000
+    call = Call([past], [rows], hq, 1, dim, store="q8_0", block=64, seed=1)
+    n = past + rows
+    k, v = torch.zeros(n, 1, dim, device="cuda").bfloat16(), torch.ones(n, 1, dim, device="cuda").bfloat16()
+    k[0, 0, 3] = 1.0
+    v[0] = 0.0
+    v[n // 2:] = -0.5
+    call.c.pool.append(0, call.c.seq_ids, dc.ints([0]), dc.ints([n]), dc.ints([0]), n, k, v)
+    call.q.zero_()
+    call.q[:, :, 3] = below * math.sqrt(dim)
+    kk, vv = call.c.rows(0)
+    want, size, most = formula(call.q, kk, vv, past, 0, 0)
+    for ws in (True, False):
+        got = call.run(ws).double()
+        assert call.c.pool.status() == 0
+        tol = (2 ** -8 + 5 * 2 ** -11) * size + torch.expm1(2 * 2 ** -11 * most) * size + n * 2 ** -32
+        err = (got - want).abs()
+        assert (err <= tol).all()
