@@ -49,6 +49,10 @@ struct Span {
         keys = r.seq < 0 ? 0 : front + last + 1 - lo;
     }
     __device__ __forceinline__ int slot(int key) const { return key < front ? key : key - front + lo; }
+    // Keys that no row sees, as runs begin and end at multiples of eight rows: n_hidden from `hidden` on, behind the first tokens and before
+    // the first row's window.
+    __device__ __forceinline__ int hidden(const WindowArgs &a) const { return min(a.sinks, max(0, first - a.window + 1) - lo + front); }
+    __device__ __forceinline__ int n_hidden(const WindowArgs &a) const { return max(0, first - a.window + 1) - lo + front - hidden(a); }
     // Every row sees all of keys [key, key + n).
     __device__ __forceinline__ bool all_see(const WindowArgs &a, int key, int n) const {
         if (key < front) return key + n <= min(front, a.sinks);  // (lo > front: all before the first row)

@@ -89,6 +89,7 @@ struct WShared {
     uint64_t v_clean[4];                 // V of a tile that only some rows see holds finite values
     uint32_t tmem;
     int abort;
+    int unfit;  // Q8: a scale of some tile's
     RangeScratch range;
     RangeStart start;
 };
@@ -150,8 +151,10 @@ __device__ __forceinline__ void transpose4(uint4 (&x)[4], int lane) {
     swap(x[1], x[3], 2);
 }
 
-// The blocks' int8 rows as f16 values, rounded once; rows past `valid` are zero. Scales that leave the f16 range with them are
-// reported, their values 0.
+__device__ __forceinline__ bool scale_fits(uint16_t bits) { return fabsf(f16_bits_to_f32(bits)) <= 515.0f; }
+
+// The blocks' int8 rows as f16 values, rounded once; rows past `valid` are zero. Values whose scale leaves the f16 range with them are 0;
+// false where there are any.
 template <int D, int ROWS, int THREADS>
 __device__ __forceinline__ bool convert_tile(const uint8_t *raw, uint8_t *dst, int valid, int thread) {
     constexpr int U = D / 16;
@@ -164,7 +167,7 @@ __device__ __forceinline__ bool convert_tile(const uint8_t *raw, uint8_t *dst, i
         if (row < valid) {
             const uint4 v = *(const uint4 *)(raw + q8_qs_off(row, 16 * u, D));
             const uint16_t bits = *(const uint16_t *)(raw + ROWS * D + (row * (D / 32) + (u >> 1)) * 2);
-            const bool ok = fabsf(f16_bits_to_f32(bits)) <= 515.0f;
+            const bool ok = scale_fits(bits);
             fits = fits && ok;
             const __half2 d = __half2half2(__ushort_as_half(ok ? bits : (uint16_t)0)), base = __half2half2(__ushort_as_half(0x6480));  // 1152
             const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
@@ -351,6 +354,30 @@ __device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared
     return ok;
 }
 
+// Whether the scales that the rows of this CTA's units see fit, one lane a key. Asked once some tile's did not: tiles hold up to 14 rows
+// that no row sees. (Told apart where a tile is converted, they cost 2 to 4% of a prompt; here, up to 1%.)
+template <int D, class U>
+__device__ __forceinline__ bool seen_scales_fit(const WindowArgs &a, U u, int bn, int lane) {
+    const PoolView &p = a.pool;
+    bool fits = true;
+    while (u.next(a, false)) {
+        const Span sp = u.span(a);
+        const int hidden = sp.hidden(a), n_hidden = sp.n_hidden(a), end = min(u.t1 * bn, sp.keys);
+#pragma unroll 1
+        for (int key = u.t0 * bn + lane; key < end; key += 32) {
+            if ((uint32_t)(key - hidden) < (uint32_t)n_hidden) continue;
+            const int slot = sp.slot(key), e = slot / p.block_tokens, blk = lookup_block(p, u.rq.seq, e);
+            if (blk < 0) continue;
+#pragma unroll 1
+            for (int i = 0; i < 2 * (D / 32); ++i) {
+                const uint8_t *tile = p.prefix + prefix_tile_index(p, a.layer, blk, i & 1, u.g) * p.tile_bytes;
+                fits = fits && scale_fits(((const uint16_t *)(tile + (int64_t)p.block_tokens * D))[(slot - e * p.block_tokens) * (D / 32) + (i >> 1)]);
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, fits);
+}
+
 template <int D, bool Q8>
 __device__ __forceinline__ bool convert(const WindowArgs &a, uint8_t *smem, WShared &sh, Units<WCfg<D, Q8>::RT * kTileRows, WCfg<D, Q8>::BN> u) {
     using C = WCfg<D, Q8>;
@@ -385,7 +412,7 @@ __device__ __forceinline__ bool convert(const WindowArgs &a, uint8_t *smem, WSha
             }
         }
     }
-    if (!__all_sync(0xffffffffu, fits) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, 0, 15);
+    if (!fits) sh.unfit = 1;
     return ok;
 }
 
@@ -878,7 +905,7 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
             mbar_init(smem_addr(&sh.raw_full[i / C::NR][i % C::NR]), 1);
             mbar_init(smem_addr(&sh.raw_empty[i / C::NR][i % C::NR]), C::CONV_WARPS);
         }
-        sh.abort = 0;
+        sh.abort = sh.unfit = 0;
         if constexpr (!Q8)
             for (int i = 0; i < kBadUnits; ++i) ((WBad *)(smem + C::OFF_BAD))->n[i] = 0;
         mbar_init_fence();
@@ -933,10 +960,12 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
             }
             if (lane == 0) sh.start = start;
         }
+        if (threadIdx.x == 0 && rg.lo >= rg.hi) sh.start = start;
         __syncthreads();
-        if (rg.lo < rg.hi) start = sh.start;
+        start = sh.start;
         __syncthreads();  // (query rows go where the places are)
     } else {
+        if (threadIdx.x == 0) sh.start = start;
         __syncthreads();
     }
     tc_fence_after();
@@ -963,6 +992,8 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
     if (!ok && lane == 0) report_error(a.pool.status, DEV_ERR_TIMEOUT, blockIdx.x, warp, 15);
     __syncthreads();
     if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
+    if constexpr (Q8)
+        if (warp == 0 && sh.unfit && !seen_scales_fit<D>(a, U(sh.start), C::BN, lane) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, 0, 15);
 }
 
 template <int D, bool Q8>

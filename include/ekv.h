@@ -448,7 +448,7 @@ size_t ekv_window_attention_workspace_size(const ekv_pool *pool, const ekv_windo
  * sequence, slots past its length) are 0 and reported through the pool's status; rows of out that belong to no request stay. What a
  * row does not see does not reach it, whatever it holds. head_dim 64, 128 or 256. Q8_0 pools: calls of more than 16 rows of a KV head
  * (max_rows * q_heads / kv_heads) compute in f16, and report (5) a query beyond its range, or a block whose scale is above 515 or not
- * finite, which counts as 0; a key's weight is off by up to 2^-32 of its row's largest there, beside f16's 2^-11 of itself. Without a workspace (or with a smaller one) units are not cut. Pointers 16-byte aligned. */
+ * finite and that some row sees, which counts as 0; a key's weight is off by up to 2^-32 of its row's largest there, beside f16's 2^-11 of itself. Without a workspace (or with a smaller one) units are not cut. Pointers 16-byte aligned. */
 int ekv_window_attention(ekv_pool *pool, const ekv_window_params *p, const void *q, int64_t q_stride, void *out, void *workspace,
                          size_t workspace_bytes, ekv_stream_t stream);
 

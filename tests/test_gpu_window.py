@@ -288,3 +288,37 @@ def test_many_small_keys_behind_a_heavy_one(dim, rows, hq, below):
         tol = (2 ** -8 + 5 * 2 ** -11) * size + torch.expm1(2 * 2 ** -11 * most) * size + n * 2 ** -32
         err = (got - want).abs()
         assert (err <= tol).all()
+
+
+class Bytes:
+    def __init__(self, pool):
+        self.__cuda_array_interface__ = dict(shape=(int(pool.info().bytes_prefix),), typestr="|u1", version=2, data=(int(pool.info().prefix_base), False))
+
+
+def set_scale(call, kv, slot, group, value):
+    """The stored scale of 32 values of K (0) or V (1): a pool of one layer and KV head."""
+    pool, dim, bt = call.c.pool, call.c.dim, call.c.block
+    block = pool.seq_get(call.c.seqs[0]).blocks[slot // bt]
+    at = (2 * block + kv) * (bt * dim // 32 * 34) + bt * dim + (slot % bt * (dim // 32) + group) * 2
+    torch.as_tensor(Bytes(pool), device="cuda")[at:at + 2] = torch.tensor([value], dtype=torch.float16, device="cuda").view(torch.uint8)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,hq", [(1, 8), (7, 2), (40, 4), (300, 1)])
+@pytest.mark.parametrize("window,sinks", [(90, 3), (93, 0), (320, 5), (331, 8), (1, 0)])
+def test_hidden_scales_do_not_leak(dim, rows, hq, window, sinks):
+    """Infinite and NaN scales of 8-bit rows that no query row sees reach neither the output nor the status: between the first tokens and
+    the window, next to them and far from them."""
+    past = 335
+    call = Call([past], [rows], hq, 1, dim, store="q8_0", window=window, sinks=sinks, seed=9)
+    hidden = [s for s in range(past + rows) if sinks <= s <= past - window]
+    want = [call.run(ws) for ws in (True, False)]
+    assert call.c.pool.status() == 0
+    for i, slot in enumerate(sorted(set(hidden[:9] + hidden[::17] + hidden[-9:]))):
+        for kv in range(2):
+            set_scale(call, kv, slot, (i + kv) % (dim // 32), (math.inf, math.nan, -math.inf, 6e4, math.nan)[(i + kv) % 5])
+    rows_now = [x[hidden] for x in call.c.rows(0)]
+    assert not hidden or not any(torch.isfinite(x).all() for x in rows_now)
+    for ws, x in zip((True, False), want):
+        assert torch.equal(call.run(ws), x)
+        assert call.c.pool.status() == 0
