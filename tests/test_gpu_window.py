@@ -322,3 +322,40 @@ def test_hidden_scales_do_not_leak(dim, rows, hq, window, sinks):
     for ws, x in zip((True, False), want):
         assert torch.equal(call.run(ws), x)
         assert call.c.pool.status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,hq", [(1, 8), (7, 2), (4, 4), (40, 4), (300, 1)])
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan])
+def test_values_with_scales_that_are_not_finite(dim, rows, hq, scale):
+    """They reach the rows that see them and no others. With many rows they count as 0 and are reported."""
+    past, window, sinks = 330, 90, 3
+    call = Call([past], [rows], hq, 1, dim, store="q8_0", window=window, sinks=sinks, seed=10)
+    end = past + rows
+    want = [call.run(ws) for ws in (True, False)]
+    see = seen(past, rows, window, sinks)
+    last = dim // 32 - 1
+    slots = {2: 0, past - 20: 1, past - window + 3: 0, past - window + 1: last, end - 1: 1}
+    if rows > 3:
+        slots[past + 3] = last
+    hit = torch.zeros(rows, dim, dtype=torch.bool, device="cuda")
+    keys, fixed = call.c.rows(0)
+    exact_v = fixed.clone()
+    for slot, group in slots.items():
+        set_scale(call, 1, slot, group, scale)
+        columns = slice(32 * group, 32 * group + 32)
+        hit[see[:, slot], columns] = True
+        exact_v[slot, 0, columns] = 0
+    assert hit.any() and not hit.all() or dim == 64
+    exact, size, most = formula(call.q, keys, exact_v, past, window, sinks)
+    for ws, x in zip((True, False), want):
+        got = call.run(ws)
+        status = call.c.pool.status()
+        if call.many:
+            assert status == ekv.DEV_ERR_F16_RANGE
+            bad = (got.double() - exact).abs() > tolerance("q8_0", True, size, most)
+            assert torch.isfinite(got).all() and not bad.any()
+        else:
+            assert status == 0
+            assert torch.isfinite(got).logical_not().eq(hit[:, None]).all()
+        assert torch.equal(got.masked_fill(hit[:, None], 0), x.masked_fill(hit[:, None], 0))

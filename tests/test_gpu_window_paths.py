@@ -196,3 +196,17 @@ def test_the_first_call_of_a_process_is_captured(rows, dim, store):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(os.path.abspath(ekv.__file__)), os.environ.get("PYTHONPATH", "")]))
     r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST, str(rows), str(dim), store], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("store,dim", [("bf16", 128), ("q8_0", 256)])
+def test_an_idle_sequence_far_longer(store, dim, rows):
+    """The longest live sequence stands for the call's where max_len is not given: work is shared for 6000 slots, then for the call's own."""
+    call = Call([700, 30, 300], [rows] * 3, 8, 2, dim, store=store, sinks=4, width=400, spare=400)
+    call.check(call.run())
+    idle = call.c.pool.seq_create()
+    call.c.pool.seq_resize(idle, 6000)
+    call.c.pool.sync()
+    for max_len in (0, 700 + rows, 31):
+        for ws in (True, False):
+            call.check(call.run(ws, max_len=max_len))
