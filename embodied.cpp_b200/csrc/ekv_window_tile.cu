@@ -89,9 +89,9 @@ struct WShared {
     uint64_t v_clean[4];                 // V of a tile that only some rows see holds finite values
     uint32_t tmem;
     int abort;
-    int unfit;  // Q8: a scale of some tile's
     RangeScratch range;
     RangeStart start;
+    int unfit[8];  // Q8: [converting warp] some tile's scales do not fit
 };
 
 // [unit % kBadUnits] keys whose values are not all finite, 32 to an entry
@@ -412,7 +412,8 @@ __device__ __forceinline__ bool convert(const WindowArgs &a, uint8_t *smem, WSha
             }
         }
     }
-    if (!fits) sh.unfit = 1;
+    fits = __all_sync(0xffffffffu, fits);
+    if (lane == 0) sh.unfit[thread / 32] = !fits;  // (no word to clear: a store more at the kernel's start took 1.6% of eight windowed prompts)
     return ok;
 }
 
@@ -760,7 +761,7 @@ __device__ __forceinline__ bool softmax(const WindowArgs &a, uint8_t *smem, WSha
                         }
                     }
                 }
-                const float neg = m == -INFINITY ? 0.0f : C::HEADROOM - m;
+                const float neg = m == -INFINITY ? 0.0f : Q8 ? C::HEADROOM - m : -m;
                 const uint64_t neg2 = pair_of(neg, neg);
 #pragma unroll
                 for (int c = 0; c < KEYS / 32; ++c) {
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     WShared &sh = *(WShared *)(smem + C::OFF_SH);
-    static_assert(sizeof(WShared) <= 2048 && sizeof(WBad) <= 8192, "barrier block");
+    static_assert(2 * C::CONV_WARPS <= 8 && sizeof(WShared) <= 2048 && sizeof(WBad) <= 8192, "barrier block");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = a.pool.kv_heads;
 
     if (threadIdx.x == 0) {
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
             mbar_init(smem_addr(&sh.raw_full[i / C::NR][i % C::NR]), 1);
             mbar_init(smem_addr(&sh.raw_empty[i / C::NR][i % C::NR]), C::CONV_WARPS);
         }
-        sh.abort = sh.unfit = 0;
+        sh.abort = 0;
         if constexpr (!Q8)
             for (int i = 0; i < kBadUnits; ++i) ((WBad *)(smem + C::OFF_BAD))->n[i] = 0;
         mbar_init_fence();
@@ -960,12 +961,12 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
             }
             if (lane == 0) sh.start = start;
         }
-        if (threadIdx.x == 0 && rg.lo >= rg.hi) sh.start = start;
+        if (Q8 && threadIdx.x == 0 && rg.lo >= rg.hi) sh.start = start;  // (for seen_scales_fit)
         __syncthreads();
-        start = sh.start;
+        if (rg.lo < rg.hi) start = sh.start;
         __syncthreads();  // (query rows go where the places are)
     } else {
-        if (threadIdx.x == 0) sh.start = start;
+        if (Q8 && threadIdx.x == 0) sh.start = start;
         __syncthreads();
     }
     tc_fence_after();
@@ -993,7 +994,8 @@ __global__ void __launch_bounds__(WCfg<D, Q8>::THREADS, 1) window_tile_kernel(co
     __syncthreads();
     if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::COLS);
     if constexpr (Q8)
-        if (warp == 0 && sh.unfit && !seen_scales_fit<D>(a, U(sh.start), C::BN, lane) && lane == 0) report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, 0, 15);
+        if (warp == 0 && __any_sync(0xffffffffu, lane < 2 * C::CONV_WARPS && sh.unfit[lane]) && !seen_scales_fit<D>(a, U(sh.start), C::BN, lane) && lane == 0)
+            report_error(a.pool.status, DEV_ERR_F16_RANGE, blockIdx.x, 0, 15);
 }
 
 template <int D, bool Q8>
