@@ -11,8 +11,8 @@
 
 namespace ekv {
 
-// Numbers below a bound that are free, lowest first: a bit each, and the word below which none is. (As a tree of nodes 256 forks with
-// their children's release took the host 300 us, as bits 230.)
+// Numbers below a bound that are free, lowest first: a bit each, and the word below which none is. (32 sequences forked
+// eight times each, and the children before them released, take 159 us as called from Python; with a tree of nodes 209.)
 class FreeIds {
   public:
     void fill(int32_t n) {

@@ -6,10 +6,11 @@
 // two), 16 columns each, so that its sum of squares takes log2(P) shuffles and a pair's two columns are one lane's: with the split
 // layout a lane has columns 8 l .. 8 l + 7 and their partners. The sines of a row are computed once per warp, a lane's pairs and
 // weights stay in registers over its heads.
-// Bound: instructions beside DRAM. 29 k rows of 48 heads of 128 columns (683 MB read and written) take 130 us, 5.3 TB/s, 80% of the
-// measured copy rate, with half of the issue slots taken: 28 us of it go to what a warp does once a row (sines, weights, places;
-// that much more for every further warp that a row is given). Four CTAs per SM spill (145 us), two hide less (142); sines in
-// registers 135, several rows a warp in turn 139 to 150. One row takes 4.7 us.
+// Bound: instructions beside DRAM. 29 k rows of 48 heads of 128 columns (683 MB read and written) take 127 us, 5.4 TB/s, 82% of the
+// measured copy rate (8-bit pages, 630 MB: 134 us, 72%), with half of the issue slots taken: 28 us of it go to what a warp does once a
+// row (sines, weights, places; that much more for every further warp that a row is given). Three CTAs per SM leave 80 registers, of
+// which split pairs over bf16 pages spill up to 16; four spill more (145 us), two hide less (142). Sines in registers 135, several rows a
+// warp in turn 139 to 150. One row takes 5 us.
 #include <algorithm>
 
 #include "ekv_decode.cuh"

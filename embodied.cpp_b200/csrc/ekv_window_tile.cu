@@ -3,16 +3,17 @@
 // out = sum_k p_k v_k / sum_k p_k with p_k = exp(scale q.k - m) over the keys a row sees (ekv_window.cuh), m a running reference that
 // moves only when a score is 2^24 (8-bit pages: 2^8) above it. S = Q K^T with both operands in shared memory and S in tensor memory, P in
 // 16 bits over S's own columns, O += P V with P read from tensor memory. P is rounded to bf16 (bf16 pages) and the row divided by the
-// sum of the rounded ones; over 8-bit pages operands are f16 (a value's int8 times its scale keeps 11 bits, P too).
+// sum of the rounded ones; over 8-bit pages operands are f16 (a value's int8 times its scale keeps 11 bits, P too, down to 2^-21 of the
+// row's largest; below that its steps are 2^-31 of it).
 //
 // Roles of a CTA's warps, each in step with the CTA's tiles by its own count: feed (K, V), convert (8-bit pages, K and V apart) or
 // look_at_values (bf16), products (a warp per row tile), softmax (a thread per row; head_dim 256: two). What bounds it: a row
 // tile's chain of scores, maximum, exponentials, P, next products. Two row tiles fill it for the special-function unit (1024 of a
-// 64-key tile's 2450 cycles) and the tensor pipe (1300 of them); a unit's end and beginning take 9000 cycles, beside 12 tiles of a
-// window of 1024 a quarter.
+// 64-key tile's 2450 cycles) and the tensor pipe (1300 of them); a unit's end and beginning take 9000 cycles, beside the 15
+// tiles that a unit of the eight prompts below has a fifth.
 // 32 / 8 heads of 128: a prompt of 16384 tokens 2284 us (963 TFLOP/s of the products that rows see, 57% of a measured bf16 product), over
-// 8-bit pages 2561; 8 prompts of up to 4096, window 1024 and 4 first tokens: 625 us (639), over 8-bit pages 764. 8 / 1 heads of 256, 8192
-// tokens: 298 us (923).
+// 8-bit pages 2607; 8 prompts of up to 4096, window 1024 and 4 first tokens: 625 us (638), over 8-bit pages 769. 8 / 1 heads of 256, 8192
+// tokens: 297 us (926). At 1965 MHz: after a second of such calls the power limit leaves 1.8 GHz, and the eight prompts take 683.
 // Measured and left out, with the first prompt's and the eight's times, which were 2335 and 637 us then: 128 keys a tile with one S tile
 // 2386 and 773; two warps to a row in place of one for head_dim 128 2654 and 718 (for 256, where one row tile leaves the schedulers a
 // warp each, 343 instead of 396); a part of the exponentials by polynomial 2333 and 645 (an eighth), 2448 and 711 (a quarter).
@@ -57,8 +58,9 @@ struct WCfg {
     // K's feeder, V's feeder; bf16: four warps that look at V; Q8: four that convert K, four that convert V
     static constexpr int SCRUB_WARP = FEED_WARP + 2, SCRUB_WARPS = 4, CONV_WARP = FEED_WARP + 2, CONV_WARPS = 4;
     static constexpr int WARPS = Q8 ? CONV_WARP + 2 * CONV_WARPS : SCRUB_WARP + SCRUB_WARPS, THREADS = WARPS * 32;
-    // 8-bit pages, two row tiles: 20 warps leave 96 registers to a thread at launch, and a row's 64 scores take more. (With two warps in
-    // place of four for each conversion there is room for 128; 16384 tokens of head_dim 128 then took 2960 us instead of 2620.)
+    // 8-bit pages, two row tiles: 20 warps leave 96 registers to a thread at launch, and a row's 64 scores take more. (The compiler allots
+    // 96 to all and spills 130 words, whatever the row warps raise themselves to. With two warps in place of four for each conversion
+    // there is room for 128; 16384 tokens of head_dim 128 then took 2960 us instead of 2620.)
     static constexpr bool SPLIT_REGS = Q8 && RT == 2;
     static constexpr int ROW_REGS = 136, OTHER_REGS = 64;
     static_assert(!SPLIT_REGS || (THREADS == 640 && 256 * ROW_REGS + 384 * OTHER_REGS <= 640 * 96), "registers");
@@ -355,7 +357,7 @@ __device__ __forceinline__ bool feed(const WindowArgs &a, uint8_t *smem, WShared
 }
 
 // Whether the scales that the rows of this CTA's units see fit, one lane a key. Asked once some tile's did not: tiles hold up to 14 rows
-// that no row sees. (Told apart where a tile is converted, they cost 2 to 4% of a prompt; here, up to 1%.)
+// that no row sees. (Told apart where a tile is converted, they cost 2 to 4% of a prompt; here, less than 1%.)
 template <int D, class U>
 __device__ __forceinline__ bool seen_scales_fit(const WindowArgs &a, U u, int bn, int lane) {
     const PoolView &p = a.pool;

@@ -493,7 +493,8 @@ typedef struct ekv_compact_params {
  * n_keep[b]. Order among rows is kept, and slots at or above n_keep[b] keep what they hold. Lengths do not change here: call
  * ekv_seq_resize(pool, seq, n_keep) afterwards. Rows keep the positions that they were turned by. An entry that is not above the
  * one before it, or not a slot of the sequence, is reported through the pool's status and its row does not move; so is a request
- * whose n_keep is not in 0 .. slot_stride, or above the sequence's length, of which nothing moves. */
+ * whose n_keep is not in 0 .. slot_stride, or above the sequence's length, of which nothing moves. With a slot_stride of 0 the call
+ * does nothing. */
 int ekv_compact(ekv_pool *pool, const ekv_compact_params *p, ekv_stream_t stream);
 
 /* ---- ggml op surface: GGML_OP_FLASH_ATTN_EXT on strided device tensors ----
